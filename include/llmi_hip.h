@@ -278,6 +278,117 @@ int llmi_hip_silu_dev(float* x, size_t n, void* stream);
 /* argmax (transformer.cpp:22-24): index of the first maximum of x[0..n). */
 int llmi_hip_argmax_dev(const float* x, size_t n, int32_t* out, void* stream);
 
+/* ------------------------------------- paged 8-bit key/value cache (device) */
+/* A key/value cache for many sequences at once, beside the fp32 cache of one
+ * sequence that the model calls below keep.  No counterpart in the reference
+ * (its KVCache holds one sequence in fp32, include/llmi/model/transformer.hpp:
+ * 29-45).  The cache of one transformer layer is a pool of pages; a page holds
+ * page_tokens positions of every key/value head as int8 codes, in blocks of
+ * LLMI_KV8_BLOCK positions with one fp32 scale per block and head, for keys
+ * and for values apart:
+ *   value = code * scale, scale = float(amax / 127), amax = the largest |value|
+ *   of the block and head, code = the exact value / scale rounded to the
+ *   nearest integer, ties to even, clamped to -127..127 (scale 0: code 0).
+ * A block that is not full is quantized as a whole at every append, from the
+ * fp32 rows in `open`: codes depend on the values alone, not on how they were
+ * split into calls, and each value is rounded once.  An inf or NaN makes its
+ * block's scale inf or NaN and its codes 0, so that every value of the block
+ * reads back as NaN.
+ *
+ * Layouts (device memory of the caller, llmi_hip_kv8_sizes gives the sizes;
+ * 16-byte aligned; nothing has to be cleared beforehand):
+ *   k       [pages][kv_heads][page_tokens/16][head_dim/16][16 positions][16 dims]
+ *   v       [pages][kv_heads][page_tokens/16][head_dim/16][16 dims][16 positions]
+ *   scales  [pages][kv_heads][page_tokens/16][2]   (the keys', the values')
+ *   open    [slots][kv_heads][2][2][16][head_dim]  block parity, then k / v:
+ *           the fp32 rows of the last two blocks that a sequence's appends
+ *           wrote, under the sequence's slot.
+ * Which pages a sequence has is the caller's: page p of its table holds
+ * positions p * page_tokens ...  Full pages may be shared by sequences. */
+#define LLMI_KV8_BLOCK 16
+typedef struct llmi_kv8_shape {
+  uint32_t heads;       /* query heads, a multiple of kv_heads */
+  uint32_t kv_heads;
+  uint32_t head_dim;    /* a multiple of 32, 32..256 */
+  uint32_t page_tokens; /* positions per page, a multiple of 16, at most 65536 */
+  uint32_t pages;       /* pages of the pool */
+  uint32_t slots;       /* sequences that `open` has room for */
+} llmi_kv8_shape;
+typedef struct llmi_kv8_layer { /* one layer's cache */
+  int8_t* k;
+  int8_t* v;
+  float* scales;
+  float* open;
+} llmi_kv8_layer;
+/* Bytes of k (and of v), floats of scales and of open.  Needs no GPU. */
+int llmi_hip_kv8_sizes(const llmi_kv8_shape* shape, size_t* code_bytes, size_t* scale_floats, size_t* open_floats);
+
+/* A batch: sequence i brings counts[i] >= 0 new tokens at positions starts[i],
+ * starts[i] + 1, ...; its pages are tables[i * table_stride ...], enough for
+ * starts[i] + counts[i] positions; slots[i] is its place in `open`.  Token
+ * rows are ragged: the tokens of sequence 0, then those of sequence 1, ...
+ * All arrays are host memory, read before the call returns.
+ * A plan holds a batch's work lists on the device and the attention's
+ * workspace, and serves every layer of the same shape.  It is created for at
+ * most max_seqs sequences, max_tokens tokens and max_pages page entries in
+ * all (0: shape->pages); plan_set replaces the batch.
+ * plan_set queues one copy on `stream`; the calls below that use the plan
+ * follow on that stream.  Launches captured into a graph work on whatever
+ * batch is set when they are replayed, in buffers with room for its tokens
+ * (plan_set itself is not captured: LLMI_ERR_STATE; after a captured append
+ * it takes only batches that can be appended, within that call's rotation
+ * tables).  Launches of one plan must not overlap; two streams or two graphs
+ * that run at once need a plan each.
+ * Refused (LLMI_ERR_ARG): a slot or page out of range, a negative start or
+ * count, a table too short, more than the plan was created for.
+ * llmi_hip_kv8_check makes the same checks, without limits of a plan, and
+ * those of an append: it needs no GPU. */
+typedef struct llmi_hip_kv8_plan llmi_hip_kv8_plan;
+int llmi_hip_kv8_check(const llmi_kv8_shape* shape, size_t seqs, const int32_t* slots, const int32_t* starts,
+                       const int32_t* counts, const int32_t* tables, size_t table_stride);
+int llmi_hip_kv8_plan_create(const llmi_kv8_shape* shape, size_t max_seqs, size_t max_tokens, size_t max_pages,
+                             llmi_hip_kv8_plan** plan);
+int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* plan, size_t seqs, const int32_t* slots, const int32_t* starts,
+                          const int32_t* counts, const int32_t* tables, size_t table_stride, void* stream);
+int llmi_hip_kv8_plan_free(llmi_hip_kv8_plan* plan);
+
+/* Appends the batch's tokens.  q [tokens][heads][head_dim], k and v [tokens]
+ * [kv_heads][head_dim], with strides (in floats) from token to token, at
+ * least a row's length.  For every head of q and k:
+ *   x <- x * w / sqrt(mean(x^2) + eps)     with q_norm / k_norm = w (head_dim
+ *                                          floats; both or neither NULL)
+ *   (x[i], x[i + d/2]) <- rotation by (cos, sin)[position][i]  with cos_t and
+ *                                          sin_t [positions][head_dim / 2];
+ *                                          both NULL: none
+ * in 64 bits, rounded once to fp32.  q goes to q_out (q_out == q with equal
+ * strides: in place); q NULL leaves q out (q_out is not touched).  k and v go
+ * to the cache.  A sequence's start is its length so far, or a whole number
+ * of blocks (pages shared with another sequence before it); of what was
+ * appended under its slot it may be taken back to any position from the block
+ * before its last one on, and written again from there.
+ * LLMI_ERR_ARG: NULL pointers, strides too short, tables of fewer positions
+ * than the batch has; LLMI_ERR_STATE: no batch set, or a batch that cannot be
+ * appended (set without slots, two sequences with one slot, a page for new
+ * tokens that appears twice). */
+int llmi_hip_kv8_append_dev(const llmi_hip_kv8_plan* plan, const llmi_kv8_layer* layer, const float* q,
+                            size_t q_stride, const float* k, size_t k_stride, const float* v, size_t v_stride,
+                            const float* q_norm, const float* k_norm, float eps, const float* cos_t,
+                            const float* sin_t, size_t positions, float* q_out, size_t q_out_stride, void* stream);
+/* Causal attention of the batch's tokens over their sequences: token row t of
+ * head h at position p,
+ *   out[t][h] = sum_{j <= p} softmax_j(scale * q[t][h] . key_j) value_j
+ * with the keys and values of head h / (heads / kv_heads), as the cache holds
+ * them (the batch's own tokens have been appended before).  q and out [tokens]
+ * [heads][head_dim] with strides as above; out may be q.  Sums and the
+ * softmax in fp32 with q and the weights carried to 22 bits or more; results do not depend on
+ * the order in which workgroups run. */
+int llmi_hip_kv8_attention_dev(const llmi_hip_kv8_plan* plan, const llmi_kv8_layer* layer, const float* q,
+                               size_t q_stride, float scale, float* out, size_t out_stride, void* stream);
+/* The cached keys and values of the batch's positions, code * scale, as fp32
+ * rows [tokens][kv_heads][head_dim] (k or v NULL: left out). */
+int llmi_hip_kv8_read_dev(const llmi_hip_kv8_plan* plan, const llmi_kv8_layer* layer, float* k, size_t k_stride,
+                          float* v, size_t v_stride, void* stream);
+
 /* ------------------------------------------------------------- the model */
 
 typedef struct llmi_hip_model llmi_hip_model; /* device-resident quantized decoder */

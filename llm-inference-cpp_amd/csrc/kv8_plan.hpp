@@ -1,0 +1,132 @@
+// The host side of the paged 8-bit key/value cache (llmi_hip_kv8_*): checks
+// of a cache's shape and of a ragged batch, and the work lists that the
+// kernels read.  No HIP here: a CPU test builds these lists and walks them.
+#pragma once
+
+#include <algorithm>
+#include <cstddef>
+#include <cstdint>
+#include <string>
+#include <vector>
+
+#include "../../include/llmi_hip.h"
+
+namespace llmi_hip::kv8 {
+
+constexpr int kBlk = LLMI_KV8_BLOCK;  // positions per scale
+
+// One sequence of a batch as the kernels read it: its tokens are rows
+// row .. row + count - 1 of q, k and v, at positions start .. start + count - 1;
+// its pages are table[table ..].
+struct Seq {
+  std::int32_t start, count, row, table, slot;
+};
+
+// One block that an append writes (one wavefront per key/value head for its
+// keys and one for its values).  then >= 0: the same wavefront goes on with
+// block `then` of the sequence, whose new rows replace rows of the open-block
+// store that `block` reads first.
+struct AppendItem {
+  std::int32_t seq, block, then;
+};
+
+struct Lists {
+  std::vector<Seq> seqs;
+  std::vector<std::int32_t> table;
+  std::vector<AppendItem> append;  // every block that holds a new token
+  std::size_t tokens = 0, longest = 0;
+  bool writable = false;
+  std::string why_not;  // why the batch cannot be appended
+};
+
+inline std::string check_shape(const llmi_kv8_shape* s) {
+  if (s == nullptr) return "null shape";
+  if (s->heads == 0 || s->kv_heads == 0 || s->heads % s->kv_heads != 0)
+    return "heads must be a positive multiple of kv_heads";
+  if (s->heads > 4096) return "at most 4096 heads";
+  if (s->head_dim < 32 || s->head_dim > 256 || s->head_dim % 32 != 0)
+    return "head_dim must be a multiple of 32 from 32 to 256";
+  if (s->page_tokens == 0 || s->page_tokens % kBlk != 0 || s->page_tokens > 65536)
+    return "page_tokens must be a multiple of 16 up to 65536";
+  if (s->pages == 0 || s->pages > 0x7FFFFFFFu) return "pages must be positive and below 2^31";
+  if (s->slots == 0 || s->slots > 0x7FFFFFFFu) return "slots must be positive and below 2^31";
+  return {};
+}
+
+inline bool same_shape(const llmi_kv8_shape& a, const llmi_kv8_shape& b) {
+  return a.heads == b.heads && a.kv_heads == b.kv_heads && a.head_dim == b.head_dim &&
+         a.page_tokens == b.page_tokens && a.pages == b.pages && a.slots == b.slots;
+}
+
+// Checks a batch and builds its lists; returns the reason of a refusal.
+inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::int32_t* slots,
+                         const std::int32_t* starts, const std::int32_t* counts, const std::int32_t* tables,
+                         std::size_t stride, std::size_t max_seqs, std::size_t max_tokens, std::size_t max_pages,
+                         Lists* out) {
+  Lists& l = *out;
+  l = Lists{};
+  if (seqs > max_seqs) return "more sequences than the plan was created for";
+  if (seqs > 0 && (starts == nullptr || counts == nullptr || tables == nullptr)) return "null array";
+  for (std::size_t i = 0; i < seqs; ++i) {
+    const std::string of = " of sequence " + std::to_string(i);
+    if (starts[i] < 0) return "negative start" + of;
+    if (counts[i] < 0) return "negative count" + of;
+    const std::int64_t len = std::int64_t{starts[i]} + counts[i];
+    // Positions stay below 2^31 - 512, so that a tile's last position fits 32 bits.
+    if (len > 0x7FFFFFFF - 512) return "too many positions" + of;
+    const std::size_t need = (static_cast<std::size_t>(len) + sh.page_tokens - 1) / sh.page_tokens;
+    if (need > stride) return "the page table is too short for the positions" + of;
+    if (l.table.size() + need > max_pages) return "more page entries than the plan was created for";
+    l.tokens += static_cast<std::size_t>(counts[i]);
+    if (l.tokens > max_tokens) return "more tokens than the plan was created for";
+    l.longest = std::max(l.longest, static_cast<std::size_t>(len));
+    if (slots != nullptr && (slots[i] < 0 || static_cast<std::uint32_t>(slots[i]) >= sh.slots))
+      return "slot out of range" + of;
+    l.seqs.push_back({starts[i], counts[i], static_cast<std::int32_t>(l.tokens) - counts[i],
+                      static_cast<std::int32_t>(l.table.size()), slots != nullptr ? slots[i] : 0});
+    for (std::size_t p = 0; p < need; ++p) {
+      const std::int32_t page = tables[i * stride + p];
+      if (page < 0 || static_cast<std::uint32_t>(page) >= sh.pages) return "page out of range" + of;
+      l.table.push_back(page);
+    }
+  }
+  // An append needs a slot of its own for each sequence with new tokens, and
+  // pages under them that nothing else in the batch reads or writes.
+  l.writable = slots != nullptr || seqs == 0;
+  if (!l.writable) l.why_not = "the batch was set without slots";
+  if (l.writable) {
+    std::vector<std::uint8_t> uses(sh.pages, 0), held(sh.slots, 0);
+    for (const std::int32_t p : l.table) uses[static_cast<std::size_t>(p)] += uses[static_cast<std::size_t>(p)] < 2;
+    for (const Seq& q : l.seqs) {
+      if (q.count == 0) continue;
+      if (held[static_cast<std::size_t>(q.slot)]++) {
+        l.writable = false;
+        l.why_not = "two sequences with new tokens have the same slot";
+        break;
+      }
+      const std::int32_t page = static_cast<std::int32_t>(sh.page_tokens);
+      for (std::int32_t p = q.start / page; p <= (q.start + q.count - 1) / page && l.writable; ++p)
+        if (uses[static_cast<std::size_t>(l.table[static_cast<std::size_t>(q.table + p)])] > 1) {
+          l.writable = false;
+          l.why_not = "a page that takes new tokens appears twice in the batch";
+        }
+      if (!l.writable) break;
+    }
+  }
+  for (std::size_t i = 0; i < seqs; ++i) {
+    const Seq& q = l.seqs[i];
+    if (q.count == 0) continue;
+    const std::int32_t first = q.start / kBlk, last = (q.start + q.count - 1) / kBlk;
+    // The rows of the last two blocks go to the open-block store, by parity.
+    // If the first block has rows in there that one of these would replace,
+    // one wavefront does both, in order.
+    std::int32_t then = -1;
+    if (q.start % kBlk != 0 && last >= first + 2) then = (last - first) % 2 == 0 ? last : last - 1;
+    const auto seq = static_cast<std::int32_t>(i);
+    for (std::int32_t b = first; b <= last; ++b)
+      if (b != then) l.append.push_back({seq, b, b == first ? then : -1});
+  }
+  return {};
+}
+
+}  // namespace llmi_hip::kv8

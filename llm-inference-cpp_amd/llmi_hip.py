@@ -78,6 +78,15 @@ SIGNATURES = {
     "llmi_hip_softmax_dev": (_i, [_vp, _sz, _sz, _vp]),
     "llmi_hip_silu_dev": (_i, [_vp, _sz, _vp]),
     "llmi_hip_argmax_dev": (_i, [_vp, _sz, _vp, _vp]),
+    "llmi_hip_kv8_sizes": (_i, [_vp, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz)]),
+    "llmi_hip_kv8_check": (_i, [_vp, _sz, _vp, _vp, _vp, _vp, _sz]),
+    "llmi_hip_kv8_plan_create": (_i, [_vp, _sz, _sz, _sz, C.POINTER(_vp)]),
+    "llmi_hip_kv8_plan_set": (_i, [_vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "llmi_hip_kv8_plan_free": (_i, [_vp]),
+    "llmi_hip_kv8_append_dev": (_i, [_vp, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _f, _vp, _vp, _sz, _vp, _sz,
+                                     _vp]),
+    "llmi_hip_kv8_attention_dev": (_i, [_vp, _vp, _vp, _sz, _f, _vp, _sz, _vp]),
+    "llmi_hip_kv8_read_dev": (_i, [_vp, _vp, _vp, _sz, _vp, _sz, _vp]),
     "llmi_hip_model_create": (_i, [_vp, _vp, _i, C.POINTER(_vp)]),
     "llmi_hip_model_create_dev": (_i, [_vp, _vp, _i, C.POINTER(_vp)]),
     "llmi_hip_model_free": (_i, [_vp]),
@@ -631,6 +640,90 @@ class TolGroup(Group):
     launched together (llmi_hip_tol_group_*)."""
 
     _create, _launch, _free = "llmi_hip_tol_group_create", "llmi_hip_tol_group_launch", "llmi_hip_tol_group_free"
+
+
+class Kv8Shape(C.Structure):
+    """llmi_kv8_shape: the shape of a paged 8-bit key/value cache."""
+
+    _fields_ = [(n, C.c_uint32) for n in ("heads", "kv_heads", "head_dim", "page_tokens", "pages", "slots")]
+
+    def sizes(self):
+        """(bytes of k and of v, floats of scales, floats of open)."""
+        a, b, c = _sz(), _sz(), _sz()
+        check(load().llmi_hip_kv8_sizes(C.byref(self), C.byref(a), C.byref(b), C.byref(c)))
+        return a.value, b.value, c.value
+
+
+class Kv8Layer(C.Structure):
+    """llmi_kv8_layer: one layer's cache (device pointers k, v, scales, open)."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "scales", "open")]
+
+
+def _batch(slots, starts, counts, tables):
+    """The host arrays of a ragged batch as contiguous int32, and the table's stride."""
+    starts, counts = (np.ascontiguousarray(a, dtype=np.int32).reshape(-1) for a in (starts, counts))
+    tables = np.ascontiguousarray(tables, dtype=np.int32)
+    tables = tables.reshape(len(starts), -1) if len(starts) else tables.reshape(0, 0)
+    slots = None if slots is None else np.ascontiguousarray(slots, dtype=np.int32).reshape(-1)
+    if len(counts) != len(starts) or (slots is not None and len(slots) != len(starts)):
+        raise ValueError("slots, starts, counts and tables must have one entry per sequence")
+    return slots, starts, counts, tables, tables.shape[1]
+
+
+def kv8_check(shape: Kv8Shape, slots, starts, counts, tables) -> None:
+    """Raises HipError where the batch cannot be set and appended (no GPU needed)."""
+    s, a, c, t, stride = _batch(slots, starts, counts, tables)
+    check(load().llmi_hip_kv8_check(C.byref(shape), len(a), _p(s), _p(a), _p(c), _p(t), stride))
+
+
+class Kv8Plan:
+    """A ragged batch over a paged 8-bit key/value cache (llmi_hip_kv8_plan_*).
+
+    set() takes host arrays; append(), attention() and read() take device
+    pointers, token strides in floats (None: rows side by side) and queue on
+    `stream` (None: the library's)."""
+
+    def __init__(self, shape: Kv8Shape, max_seqs: int, max_tokens: int, max_pages: int = 0):
+        self.lib = init()
+        self.h = None
+        self.q_row, self.kv_row = shape.heads * shape.head_dim, shape.kv_heads * shape.head_dim
+        h = C.c_void_p()
+        check(self.lib.llmi_hip_kv8_plan_create(C.byref(shape), max_seqs, max_tokens, max_pages, C.byref(h)))
+        self.h = h.value
+
+    def set(self, slots, starts, counts, tables, stream=None) -> None:
+        s, a, c, t, stride = _batch(slots, starts, counts, tables)
+        check(self.lib.llmi_hip_kv8_plan_set(self.h, len(a), _p(s), _p(a), _p(c), _p(t), stride, stream))
+
+    def append(self, layer: Kv8Layer, q, k: int, v: int, q_out, *, q_stride=None, k_stride=None, v_stride=None,
+               q_out_stride=None, q_norm=None, k_norm=None, eps: float = 0.0, cos=None, sin=None, positions: int = 0,
+               stream=None) -> None:
+        check(self.lib.llmi_hip_kv8_append_dev(
+            self.h, C.byref(layer), q, self.q_row if q_stride is None else q_stride, k,
+            self.kv_row if k_stride is None else k_stride, v, self.kv_row if v_stride is None else v_stride, q_norm,
+            k_norm, eps, cos, sin, positions, q_out, self.q_row if q_out_stride is None else q_out_stride, stream))
+
+    def attention(self, layer: Kv8Layer, q: int, scale: float, out: int, *, q_stride=None, out_stride=None,
+                  stream=None) -> None:
+        check(self.lib.llmi_hip_kv8_attention_dev(self.h, C.byref(layer), q,
+                                                  self.q_row if q_stride is None else q_stride, scale, out,
+                                                  self.q_row if out_stride is None else out_stride, stream))
+
+    def read(self, layer: Kv8Layer, k, v, *, k_stride=None, v_stride=None, stream=None) -> None:
+        check(self.lib.llmi_hip_kv8_read_dev(self.h, C.byref(layer), k, self.kv_row if k_stride is None else k_stride,
+                                             v, self.kv_row if v_stride is None else v_stride, stream))
+
+    def free(self) -> None:
+        if self.h:
+            check(self.lib.llmi_hip_kv8_plan_free(self.h))
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
 
 
 class Graph:

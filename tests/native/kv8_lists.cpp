@@ -1,0 +1,81 @@
+// Walks the work lists of the paged 8-bit key/value cache (csrc/kv8_plan.hpp)
+// for random batches: every block of new tokens is written once, inside its
+// sequence's table, and no open-block row is replaced before the wavefront
+// that needs it has read it.
+#include <cstdio>
+#include <cstdlib>
+#include <random>
+#include <set>
+#include <utility>
+
+#include "../../llm-inference-cpp_amd/csrc/kv8_plan.hpp"
+
+#define CHECK(c)                                                     \
+  do {                                                               \
+    if (!(c)) {                                                      \
+      std::printf("%s:%d: %s\n", __FILE__, __LINE__, #c);            \
+      return 1;                                                      \
+    }                                                                \
+  } while (0)
+
+using namespace llmi_hip::kv8;
+
+int main() {
+  std::mt19937 rng(1);
+  const auto pick = [&](int lo, int hi) { return lo + static_cast<int>(rng() % static_cast<unsigned>(hi - lo + 1)); };
+  for (int round = 0; round < 3000; ++round) {
+    llmi_kv8_shape sh{};
+    sh.kv_heads = static_cast<std::uint32_t>(pick(1, 4));
+    sh.heads = sh.kv_heads * static_cast<std::uint32_t>(pick(1, 20));
+    sh.head_dim = 32u * static_cast<std::uint32_t>(pick(1, 8));
+    sh.page_tokens = 16u * static_cast<std::uint32_t>(pick(1, 5));
+    const int n = pick(0, 6);
+    sh.slots = 6;
+    std::vector<std::int32_t> slots, starts, counts;
+    std::size_t stride = 1, pages = 1, tokens = 0;
+    const int longest = pick(0, 2) == 0 ? 4000 : 120;
+    for (int i = 0; i < n; ++i) {
+      slots.push_back(i);
+      starts.push_back(pick(0, longest));
+      counts.push_back(pick(0, 3) == 0 ? pick(0, 300) : pick(0, 5));
+      const std::size_t need = (static_cast<std::size_t>(starts.back() + counts.back()) + sh.page_tokens - 1) / sh.page_tokens;
+      stride = std::max(stride, need);
+      pages += need;
+      tokens += static_cast<std::size_t>(counts.back());
+    }
+    sh.pages = static_cast<std::uint32_t>(pages);
+    std::vector<std::int32_t> tables(stride * static_cast<std::size_t>(n), -1);
+    std::int32_t next = 0;
+    for (int i = 0; i < n; ++i)
+      for (std::size_t p = 0; p * sh.page_tokens < static_cast<std::size_t>(starts[static_cast<std::size_t>(i)] + counts[static_cast<std::size_t>(i)]); ++p)
+        tables[static_cast<std::size_t>(i) * stride + p] = next++;
+    Lists l;
+    const std::string why = build(sh, static_cast<std::size_t>(n), slots.data(), starts.data(), counts.data(), tables.data(), stride, 6, 4000, 4000, &l);
+    CHECK(why.empty());
+    CHECK(l.writable && l.tokens == tokens);
+    std::set<std::pair<int, int>> written;
+    for (const AppendItem& it : l.append) {
+      CHECK(it.seq >= 0 && it.seq < n);
+      const Seq& s = l.seqs[static_cast<std::size_t>(it.seq)];
+      const int last = (s.start + s.count - 1) / kBlk;
+      for (const int b : {it.block, it.then}) {
+        if (b < 0) continue;
+        CHECK(s.count > 0 && b >= s.start / kBlk && b <= last);
+        CHECK(static_cast<std::size_t>(s.table) + static_cast<std::size_t>(b * kBlk) / sh.page_tokens < l.table.size());
+        CHECK(written.insert({it.seq, b}).second);
+      }
+      // A block that reads rows of the store, against every other writer of
+      // the same rows (blocks last and last - 1, by parity).
+      if (it.block * kBlk < s.start)
+        for (int b = last - 1; b <= last; ++b)
+          if (b > it.block && b % 2 == it.block % 2) CHECK(it.then == b);
+    }
+    std::size_t blocks = 0;
+    for (const Seq& s : l.seqs)
+      if (s.count > 0) blocks += static_cast<std::size_t>((s.start + s.count - 1) / kBlk - s.start / kBlk + 1);
+    CHECK(written.size() == blocks);
+    CHECK(l.append.size() <= tokens / kBlk + 2 * std::min<std::size_t>(static_cast<std::size_t>(n), tokens));
+  }
+  std::puts("ok");
+  return 0;
+}
