@@ -380,6 +380,7 @@ using namespace llmi_hip::kv8;
 llmi_hip_kv8_plan::~llmi_hip_kv8_plan() {
   if (copied != nullptr) (void)hipEventDestroy(copied);
   if (dev != nullptr) (void)hipFree(dev);
+  if (parts != nullptr) (void)hipFree(parts);
   if (pinned != nullptr) (void)hipHostFree(pinned);
 }
 
@@ -438,6 +439,11 @@ int llmi_hip_kv8_plan_create(const llmi_kv8_shape* shape, size_t max_seqs, size_
   // Every block of new tokens: a whole number of them per sequence, and up
   // to two that are not full.
   p->max_append = max_tokens / kBlk + 2 * std::min(max_seqs, max_tokens);
+  // Splits: see build(); a batch's row groups that are not split add one item each.
+  const std::size_t splits = kFewTarget / shape->kv_heads;
+  p->max_few = splits + (kFewMax / kFewRows) * std::min(max_seqs, max_tokens);
+  p->max_join = splits;
+  p->max_parts = 2 * splits;
   const auto take = [&](std::size_t bytes) {
     const std::size_t at = p->bytes;
     p->bytes += (bytes + 255) / 256 * 256;
@@ -446,9 +452,13 @@ int llmi_hip_kv8_plan_create(const llmi_kv8_shape* shape, size_t max_seqs, size_
   (void)take(sizeof(Counts));
   p->off_seqs = take(max_seqs * sizeof(Seq));
   p->off_append = take(p->max_append * sizeof(AppendItem));
+  p->off_few = take(p->max_few * sizeof(FewItem));
+  p->off_join = take(p->max_join * sizeof(JoinItem));
   p->off_table = take(max_pages * sizeof(std::int32_t));
   LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&p->dev), p->bytes));
   LLMI_TRY_HIP(hipHostMalloc(reinterpret_cast<void**>(&p->pinned), p->bytes, hipHostMallocDefault));
+  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&p->parts), p->max_parts * shape->kv_heads * kFewRows *
+                                                                  (shape->head_dim + 2) * sizeof(float)));
   LLMI_TRY_HIP(hipEventCreateWithFlags(&p->copied, hipEventDisableTiming));
   *plan = p.release();
   return LLMI_OK;
@@ -465,7 +475,9 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     const std::string why = build(p->shape, seqs, slots, starts, counts, tables, table_stride, p->max_seqs,
                                   p->max_tokens, p->max_pages, &l);
     LLMI_REQUIRE(why.empty(), "kv8_plan_set: " + why);
-    LLMI_REQUIRE(l.append.size() <= p->max_append, "kv8_plan_set: more blocks than the plan was created for");
+    LLMI_REQUIRE(l.append.size() <= p->max_append && l.few.size() <= p->max_few && l.join.size() <= p->max_join &&
+                     l.parts <= p->max_parts,
+                 "kv8_plan_set: more work than the plan was created for");
     if (p->append_captured) {
       LLMI_REQUIRE(l.writable, "kv8_plan_set: an append of this plan was captured, and " + l.why_not);
       LLMI_REQUIRE(l.longest <= p->captured_positions,
@@ -473,13 +485,16 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     }
     LLMI_TRY_HIP(hipEventSynchronize(p->copied));
     const Counts c{static_cast<std::int32_t>(l.append.size()), static_cast<std::int32_t>(l.tokens),
-                   static_cast<std::int32_t>(l.seqs.size())};
+                   static_cast<std::int32_t>(l.seqs.size()), static_cast<std::int32_t>(l.few.size()),
+                   static_cast<std::int32_t>(l.join.size())};
     const auto put = [&](std::size_t at, const auto& v) {
       if (!v.empty()) std::memcpy(p->pinned + at, v.data(), v.size() * sizeof(v[0]));
     };
     std::memcpy(p->pinned, &c, sizeof c);
     put(p->off_seqs, l.seqs);
     put(p->off_append, l.append);
+    put(p->off_few, l.few);
+    put(p->off_join, l.join);
     put(p->off_table, l.table);
     const std::size_t used = p->off_table + l.table.size() * sizeof(std::int32_t);
     p->set = false;

@@ -9,7 +9,7 @@ namespace llmi_hip::kv8 {
 // Item counts of the batch that is set, in device memory (launches replayed
 // from a graph read them there).
 struct Counts {
-  std::int32_t append, tokens, seqs;
+  std::int32_t append, tokens, seqs, few, join;
 };
 
 // A plan's device lists.
@@ -18,6 +18,8 @@ struct View {
   const Seq* seqs;
   const std::int32_t* table;
   const AppendItem* append;
+  const FewItem* few;
+  const JoinItem* join;
 };
 
 struct Geometry {
@@ -47,8 +49,10 @@ struct llmi_hip_kv8_plan {
   // marks the copy's end, before which the pinned side is not written again.
   std::uint8_t* dev = nullptr;
   std::uint8_t* pinned = nullptr;
-  std::size_t bytes = 0, off_seqs = 0, off_table = 0, off_append = 0;
-  std::size_t max_append = 0;
+  std::size_t bytes = 0, off_seqs = 0, off_table = 0, off_append = 0, off_few = 0, off_join = 0;
+  std::size_t max_append = 0, max_few = 0, max_join = 0, max_parts = 0;
+  // The attention's partial states (launches of one plan follow each other).
+  float* parts = nullptr;
   hipEvent_t copied = nullptr;
   bool set = false;
   llmi_hip::kv8::Lists lists;
@@ -60,7 +64,8 @@ struct llmi_hip_kv8_plan {
     using namespace llmi_hip::kv8;
     return {reinterpret_cast<const Counts*>(dev), reinterpret_cast<const Seq*>(dev + off_seqs),
             reinterpret_cast<const std::int32_t*>(dev + off_table),
-            reinterpret_cast<const AppendItem*>(dev + off_append)};
+            reinterpret_cast<const AppendItem*>(dev + off_append), reinterpret_cast<const FewItem*>(dev + off_few),
+            reinterpret_cast<const JoinItem*>(dev + off_join)};
   }
   ~llmi_hip_kv8_plan();
 };

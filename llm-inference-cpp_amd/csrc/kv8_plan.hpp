@@ -30,7 +30,32 @@ struct AppendItem {
   std::int32_t seq, block, then;
 };
 
+// The rows of a sequence for one key/value head are its tokens' query heads
+// of that head: row r is token r / group, head r % group.  `few` work is up to
+// kFewRows rows over positions lo .. hi - 1 (lo a multiple of a tile); part
+// >= 0: one of several over the same rows, its state goes to partial slot
+// `part`; part < 0: the whole history, the rows' output.
+constexpr int kTile = 64, kFewRows = 16;
+constexpr int kFewMax = 64;  // most rows of a sequence and key/value head that go as `few` work
+struct FewItem {
+  std::int32_t seq, row0, rows, lo, hi, part;
+};
+// Partial slots part .. part + n - 1 hold the states of these rows.
+struct JoinItem {
+  std::int32_t seq, row0, rows, part, n;
+};
+// Positions per split are chosen so that a batch makes about this many units
+// of work (item and key/value head); a split is at least kMinSplit positions.
+constexpr std::size_t kFewTarget = 2048;
+constexpr std::size_t kMinSplit = 4 * kTile;
+// Most partial slots of any batch: every split but a sequence's last one is
+// full, so there are at most kFewTarget / kv_heads full ones, and one more
+// for each of the row groups that are split.
+
 struct Lists {
+  std::vector<FewItem> few;
+  std::vector<JoinItem> join;
+  std::size_t parts = 0;
   std::vector<Seq> seqs;
   std::vector<std::int32_t> table;
   std::vector<AppendItem> append;  // every block that holds a new token
@@ -125,6 +150,34 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
     const auto seq = static_cast<std::int32_t>(i);
     for (std::int32_t b = first; b <= last; ++b)
       if (b != then) l.append.push_back({seq, b, b == first ? then : -1});
+  }
+  // Attention: sequences with few rows per key/value head are split over
+  // their history where the batch alone does not make enough work.
+  const std::size_t group = sh.heads / sh.kv_heads;
+  std::size_t reach = 0;  // positions x row groups x heads of all few work
+  const auto row_groups = [&](const Seq& q) { return (q.count * group + kFewRows - 1) / kFewRows; };
+  for (const Seq& q : l.seqs)
+    if (q.count > 0 && q.count * group <= kFewMax)
+      reach += static_cast<std::size_t>(q.start + q.count) * row_groups(q) * sh.kv_heads;
+  const std::size_t split = std::max(kMinSplit, (reach / kFewTarget + kMinSplit - 1) / kMinSplit * kMinSplit);
+  for (std::size_t i = 0; i < seqs; ++i) {
+    const Seq& q = l.seqs[i];
+    const std::size_t rows = q.count * group;
+    if (rows == 0 || rows > kFewMax) continue;
+    for (std::size_t r = 0; r < rows; r += kFewRows) {
+      const auto row0 = static_cast<std::int32_t>(r);
+      const auto nrows = static_cast<std::int32_t>(std::min<std::size_t>(kFewRows, rows - r));
+      // The last row's position bounds what this group of rows sees.
+      const std::size_t len = static_cast<std::size_t>(q.start) + (r + static_cast<std::size_t>(nrows) - 1) / group + 1;
+      const std::size_t n = (len + split - 1) / split;
+      const auto seq = static_cast<std::int32_t>(i);
+      if (n > 1) l.join.push_back({seq, row0, nrows, static_cast<std::int32_t>(l.parts), static_cast<std::int32_t>(n)});
+      for (std::size_t c = 0; c < n; ++c)
+        l.few.push_back({seq, row0, nrows, static_cast<std::int32_t>(c * split),
+                         static_cast<std::int32_t>(std::min(len, (c + 1) * split)),
+                         n > 1 ? static_cast<std::int32_t>(l.parts + c) : -1});
+      if (n > 1) l.parts += n;
+    }
   }
   return {};
 }
