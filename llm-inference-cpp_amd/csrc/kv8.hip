@@ -439,11 +439,15 @@ int llmi_hip_kv8_plan_create(const llmi_kv8_shape* shape, size_t max_seqs, size_
   // Every block of new tokens: a whole number of them per sequence, and up
   // to two that are not full.
   p->max_append = max_tokens / kBlk + 2 * std::min(max_seqs, max_tokens);
-  // Splits: see build(); a batch's row groups that are not split add one item each.
-  const std::size_t splits = kFewTarget / shape->kv_heads;
-  p->max_few = splits + (kFewMax / kFewRows) * std::min(max_seqs, max_tokens);
-  p->max_join = splits;
-  p->max_parts = 2 * splits;
+  // Splits: a kind's positions x heads over its split size are at most its
+  // target, so are the full splits x heads, and a group of rows that is split
+  // has at most twice its full ones; every group adds one item at most.
+  const std::size_t few_splits = kFewTarget / shape->kv_heads, many_splits = kManyTarget / shape->kv_heads;
+  const std::size_t busy = std::min(max_seqs, max_tokens), group = shape->heads / shape->kv_heads;
+  p->max_few = few_splits + (kFewMax / kFewRows) * busy;
+  p->max_many = many_splits + max_tokens * group / kManyRows + busy;
+  p->max_join = few_splits + kManySlots * many_splits;
+  p->max_parts = 2 * few_splits + 2 * kManySlots * many_splits;
   const auto take = [&](std::size_t bytes) {
     const std::size_t at = p->bytes;
     p->bytes += (bytes + 255) / 256 * 256;
@@ -453,6 +457,7 @@ int llmi_hip_kv8_plan_create(const llmi_kv8_shape* shape, size_t max_seqs, size_
   p->off_seqs = take(max_seqs * sizeof(Seq));
   p->off_append = take(p->max_append * sizeof(AppendItem));
   p->off_few = take(p->max_few * sizeof(FewItem));
+  p->off_many = take(p->max_many * sizeof(ManyItem));
   p->off_join = take(p->max_join * sizeof(JoinItem));
   p->off_table = take(max_pages * sizeof(std::int32_t));
   LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&p->dev), p->bytes));
@@ -475,7 +480,8 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     const std::string why = build(p->shape, seqs, slots, starts, counts, tables, table_stride, p->max_seqs,
                                   p->max_tokens, p->max_pages, &l);
     LLMI_REQUIRE(why.empty(), "kv8_plan_set: " + why);
-    LLMI_REQUIRE(l.append.size() <= p->max_append && l.few.size() <= p->max_few && l.join.size() <= p->max_join &&
+    LLMI_REQUIRE(l.append.size() <= p->max_append && l.few.size() <= p->max_few &&
+                     l.many.size() <= p->max_many && l.join.size() <= p->max_join &&
                      l.parts <= p->max_parts,
                  "kv8_plan_set: more work than the plan was created for");
     if (p->append_captured) {
@@ -486,7 +492,7 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     LLMI_TRY_HIP(hipEventSynchronize(p->copied));
     const Counts c{static_cast<std::int32_t>(l.append.size()), static_cast<std::int32_t>(l.tokens),
                    static_cast<std::int32_t>(l.seqs.size()), static_cast<std::int32_t>(l.few.size()),
-                   static_cast<std::int32_t>(l.join.size())};
+                   static_cast<std::int32_t>(l.many.size()), static_cast<std::int32_t>(l.join.size())};
     const auto put = [&](std::size_t at, const auto& v) {
       if (!v.empty()) std::memcpy(p->pinned + at, v.data(), v.size() * sizeof(v[0]));
     };
@@ -494,6 +500,7 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     put(p->off_seqs, l.seqs);
     put(p->off_append, l.append);
     put(p->off_few, l.few);
+    put(p->off_many, l.many);
     put(p->off_join, l.join);
     put(p->off_table, l.table);
     const std::size_t used = p->off_table + l.table.size() * sizeof(std::int32_t);

@@ -9,7 +9,7 @@ namespace llmi_hip::kv8 {
 // Item counts of the batch that is set, in device memory (launches replayed
 // from a graph read them there).
 struct Counts {
-  std::int32_t append, tokens, seqs, few, join;
+  std::int32_t append, tokens, seqs, few, many, join;
 };
 
 // A plan's device lists.
@@ -19,6 +19,7 @@ struct View {
   const std::int32_t* table;
   const AppendItem* append;
   const FewItem* few;
+  const ManyItem* many;
   const JoinItem* join;
 };
 
@@ -49,8 +50,8 @@ struct llmi_hip_kv8_plan {
   // marks the copy's end, before which the pinned side is not written again.
   std::uint8_t* dev = nullptr;
   std::uint8_t* pinned = nullptr;
-  std::size_t bytes = 0, off_seqs = 0, off_table = 0, off_append = 0, off_few = 0, off_join = 0;
-  std::size_t max_append = 0, max_few = 0, max_join = 0, max_parts = 0;
+  std::size_t bytes = 0, off_seqs = 0, off_table = 0, off_append = 0, off_few = 0, off_many = 0, off_join = 0;
+  std::size_t max_append = 0, max_few = 0, max_many = 0, max_join = 0, max_parts = 0;
   // The attention's partial states (launches of one plan follow each other).
   float* parts = nullptr;
   hipEvent_t copied = nullptr;
@@ -65,7 +66,7 @@ struct llmi_hip_kv8_plan {
     return {reinterpret_cast<const Counts*>(dev), reinterpret_cast<const Seq*>(dev + off_seqs),
             reinterpret_cast<const std::int32_t*>(dev + off_table),
             reinterpret_cast<const AppendItem*>(dev + off_append), reinterpret_cast<const FewItem*>(dev + off_few),
-            reinterpret_cast<const JoinItem*>(dev + off_join)};
+            reinterpret_cast<const ManyItem*>(dev + off_many), reinterpret_cast<const JoinItem*>(dev + off_join)};
   }
   ~llmi_hip_kv8_plan();
 };

@@ -13,10 +13,10 @@ struct AttnArgs {
   const float* scales;
   const float* q;
   float* out;
-  float* parts;  // [part][kv head][16 rows]: o (dim floats), then the same of (maximum, sum)
+  float* parts;  // rows of partial states: o (dim floats each), then (maximum, sum) each
   std::size_t q_stride, out_stride, part_states;  // part_states: float offset of the (maximum, sum) pairs
   float scale;
-  int ntokens, nfew, njoin;  // -1: from v.counts (a captured launch)
+  int nfew, nmany, njoin;  // -1: from v.counts (a captured launch)
 };
 
 // ------------------------------------------------------------- few rows
@@ -33,6 +33,7 @@ struct AttnArgs {
 // against the running maximum.  A wavefront takes tiles of 64 positions = 4
 // blocks; a workgroup's four wavefronts take a range's tiles in turn and merge.
 typedef int i4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // rows may start at any float
 
 // Maximum over the 16 lanes of a row of lanes, in every lane.
 __device__ __forceinline__ float row16_max(float v) {
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(kThreads) attention_join(AttnArgs A) {
     const JoinItem it = A.v.join[u / kFewRows / A.g.kv_heads];
     if (r >= it.rows) continue;
     const auto slot = [&](int c) {
-      return (static_cast<std::size_t>(it.part + c) * A.g.kv_heads + h) * kFewRows + r;
+      return (static_cast<std::size_t>(it.part + c * it.step) * A.g.kv_heads + h * it.step) * kFewRows + it.off + r;
     };
     const auto state = [&](int c) { return *reinterpret_cast<const float2*>(A.parts + A.part_states + 2 * slot(c)); };
     float top = -INFINITY;
@@ -325,84 +326,258 @@ __global__ void __launch_bounds__(kThreads) attention_join(AttnArgs A) {
   }
 }
 
-__device__ __forceinline__ float wave_maxf(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
-}
-__device__ __forceinline__ float wave_sumf(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+// ------------------------------------------------------------ many rows
+// Prompts and chunks: 128 rows (tokens x query heads of one key/value head) a
+// workgroup, 32 a wavefront, on the 16-bit matrix instructions.  The codes are
+// exact in fp16; the fp32 side enters as two fp16 parts (22 bits):
+//   S^T[position][row] = K Q^T   A = codes of 32 positions, B = q * 2^s, two parts
+//   O^T[dim][row]      = V^T W^T A = codes of 32 dims, B = w, two parts
+// A row is a column of both, so its maximum, sum and rescaling are one lane's
+// (and its partner's 32 lanes on), and the weights go from the first product's
+// accumulators to the second's operand without leaving the registers: a lane
+// holds positions 4h .. 4h+3 and 8+4h .. of each 16 (h = lane / 32), and the
+// value tile is staged in that order.
+// w = p * (value scale / the largest so far) * 2^kWeightBits: block scales
+// differ along the sum, so they ride on the weights.
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+constexpr int kWeightBits = 14;
+
+// The four signed bytes of w as fp16, exact: 1024 + (byte + 128) is an fp16
+// whose low byte is the code plus 128.
+__device__ __forceinline__ void halves(std::uint32_t w, std::uint32_t* out) {
+  const std::uint32_t u = w ^ 0x80808080u;
+  const h2 bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+  const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
+  const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+  out[0] = __builtin_bit_cast(std::uint32_t, static_cast<h2>(a - bias));
+  out[1] = __builtin_bit_cast(std::uint32_t, static_cast<h2>(b - bias));
 }
 
-// One wavefront per token and head; 64 positions at a time, one pass with the
-// running maximum and sum.
-__global__ void __launch_bounds__(kThreads) attention_simple(AttnArgs A) {
-  __shared__ float q_s[kWaves][256];
-  __shared__ float p_s[kWaves][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int dim = A.g.dim;
-  const int ntokens = A.ntokens >= 0 ? A.ntokens : A.v.counts->tokens;
-  const long rows = static_cast<long>(ntokens) * A.g.heads;
-  for (long r = static_cast<long>(blockIdx.x) * kWaves + wave; r < rows; r += static_cast<long>(gridDim.x) * kWaves) {
-    const long t = r / A.g.heads;
-    const int h = static_cast<int>(r % A.g.heads), kvh = h / A.g.group;
-    int lo = 0, hi = A.v.counts->seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (A.v.seqs[mid].row <= t)
-        lo = mid;
-      else
-        hi = mid - 1;
+template <int HD>
+__global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) attention_many(AttnArgs A) {
+  constexpr int kG = HD / 16;
+  constexpr int kChunks = 4 * HD;  // 16-byte pieces of a tile's keys (and of its values)
+  constexpr int kPer = (kChunks + kThreads - 1) / kThreads;
+  constexpr float kLog2e = 1.44269504088896340736f;
+  __shared__ uint4 sh_k[2][kG][2][kTile];     // [16-dim group][half of it][position]: 8 fp16
+  __shared__ uint4 sh_v[2][kTile / 16][2][HD];  // [block][h][dim]: positions 4h.., 8 + 4h..
+  __shared__ float2 sh_s[2][4];
+  const int lane = threadIdx.x & 63, col = lane & 31, h2nd = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nmany = A.nmany >= 0 ? A.nmany : A.v.counts->many;
+  const int units = nmany * A.g.kv_heads;
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const int item = u / A.g.kv_heads, head = u - item * A.g.kv_heads;
+    const ManyItem it = A.v.many[item];
+    const Seq s = A.v.seqs[it.seq];
+    const int r = wave * 32 + col;
+    const bool live = r < it.rows;
+    const int row = it.row0 + (live ? r : 0), tok = row / A.g.group;
+    const int limit = live ? s.start + tok : -1;
+    const std::size_t head_off = static_cast<std::size_t>(head * A.g.group + (row - tok * A.g.group)) * HD;
+
+    // q * 2^qs, its largest below 2^14, as two fp16 parts.
+    h8 qh[kG], ql[kG];
+    int qs;
+    {
+      const float* qp = A.q + static_cast<std::size_t>(s.row + tok) * A.q_stride + head_off;
+      float x[kG][8], top = 0.0f;
+#pragma unroll
+      for (int g = 0; g < kG; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[g][i] = live ? qp[16 * g + 8 * h2nd + i] : 0.0f;
+          top = fmaxf(top, fabsf(x[g][i]));
+        }
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      int e = 0;
+      (void)frexpf(top, &e);
+      if (!(top > 0.0f && top < INFINITY)) e = 0;
+      qs = 14 - e;
+#pragma unroll
+      for (int g = 0; g < kG; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float y = ldexpf(x[g][i], qs);
+          qh[g][i] = static_cast<_Float16>(y);
+          ql[g][i] = static_cast<_Float16>(y - static_cast<float>(qh[g][i]));
+        }
     }
-    const Seq s = A.v.seqs[lo];
-    if (static_cast<long>(s.count) * A.g.group <= kFewMax) continue;
-    const int npos = s.start + static_cast<int>(t) - s.row + 1;
-    for (int d = lane; d < dim; d += 64) q_s[wave][d] = A.q[t * A.q_stride + static_cast<std::size_t>(h) * dim + d];
-    __builtin_amdgcn_wave_barrier();
-    float m = -INFINITY, l = 0.0f, o[4] = {};
-    for (int base = 0; base < npos; base += 64) {
-      const int pos = base + lane, block = pos / kBlk;
-      float sc = -INFINITY, vs = 0.0f;
-      std::size_t at = 0;
-      if (pos < npos) {
-        at = block_index(A.g, A.v.table, s, block, kvh);
-        const std::int8_t* kp = A.k + at * A.g.block_bytes + (pos % kBlk) * 16;
-        float acc = 0.0f;
-        for (int g = 0; g < dim / 16; ++g)
-          for (int j = 0; j < 16; ++j) acc = fmaf(q_s[wave][g * 16 + j], static_cast<float>(kp[g * 256 + j]), acc);
-        sc = acc * A.scales[2 * at] * A.scale;
-        vs = A.scales[2 * at + 1];
+    // The wavefront's rows see at most up to `reach`, and all of them up to `all`.
+    int reach = limit, all = live ? limit : 0x7FFFFFFF;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      reach = max(reach, __shfl_xor(reach, o, 64));
+      all = min(all, __shfl_xor(all, o, 64));
+    }
+    reach = __builtin_amdgcn_readfirstlane(reach);
+    all = __builtin_amdgcn_readfirstlane(all);
+
+    f16v o[HD / 32];
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f, vtop = 0x1p-96f;
+
+    const int last_block = (it.hi - 1) / kBlk;
+    uint4 kreg[kPer], vreg[kPer];
+    float2 sreg = make_float2(0.0f, 0.0f);
+    const auto fetch = [&](int base) {
+#pragma unroll
+      for (int n = 0; n < kPer; ++n) {
+        const int c = n * kThreads + threadIdx.x;
+        if (kChunks % kThreads != 0 && c >= kChunks) break;
+        const int b = c / HD, at_chunk = c - b * HD;
+        const std::size_t at = block_index(A.g, A.v.table, s, min(base / kBlk + b, last_block), head);
+        kreg[n] = reinterpret_cast<const uint4*>(A.k + at * (16 * HD))[at_chunk];
+        vreg[n] = reinterpret_cast<const uint4*>(A.val + at * (16 * HD))[at_chunk];
       }
-      const float mx = fmaxf(m, wave_maxf(sc));
-      const float keep = expf(m - mx);
-      const float p = pos < npos ? expf(sc - mx) : 0.0f;
-      l = l * keep + wave_sumf(p);
-      m = mx;
-      p_s[wave][lane] = pos < npos ? p * vs : 0.0f;
-      __builtin_amdgcn_wave_barrier();
-      const int nhere = min(64, npos - base);
-      for (int n = 0; n * 64 < dim; ++n) {
-        const int d = n * 64 + lane;
-        float acc = 0.0f;
-        for (int b = 0; b * kBlk < nhere; ++b) {
-          const std::size_t bi = block_index(A.g, A.v.table, s, base / kBlk + b, kvh);
-          if (d < dim) {
-            const std::int8_t* vp = A.val + bi * A.g.block_bytes + d * 16;
-            for (int j = 0; j < kBlk && b * kBlk + j < nhere; ++j)
-              acc = fmaf(p_s[wave][b * kBlk + j], static_cast<float>(vp[j]), acc);
+      if (threadIdx.x < 4) {
+        const int b = base / kBlk + static_cast<int>(threadIdx.x);
+        sreg = make_float2(0.0f, 0.0f);
+        if (b <= last_block)
+          sreg = reinterpret_cast<const float2*>(A.scales)[block_index(A.g, A.v.table, s, b, head)];
+      }
+    };
+    const auto stage = [&](int buf) {
+#pragma unroll
+      for (int n = 0; n < kPer; ++n) {
+        const int c = n * kThreads + threadIdx.x;
+        if (kChunks % kThreads != 0 && c >= kChunks) break;
+        const int b = c / HD, at_chunk = c - b * HD;
+        std::uint32_t x[8];
+        halves(kreg[n].x, x);
+        halves(kreg[n].y, x + 2);
+        halves(kreg[n].z, x + 4);
+        halves(kreg[n].w, x + 6);
+        const int g = at_chunk / 16, p = b * 16 + at_chunk % 16;
+        sh_k[buf][g][0][p] = make_uint4(x[0], x[1], x[2], x[3]);
+        sh_k[buf][g][1][p] = make_uint4(x[4], x[5], x[6], x[7]);
+        halves(vreg[n].x, x);
+        halves(vreg[n].y, x + 2);
+        halves(vreg[n].z, x + 4);
+        halves(vreg[n].w, x + 6);
+        sh_v[buf][b][0][at_chunk] = make_uint4(x[0], x[1], x[4], x[5]);
+        sh_v[buf][b][1][at_chunk] = make_uint4(x[2], x[3], x[6], x[7]);
+      }
+      if (threadIdx.x < 4) sh_s[buf][threadIdx.x] = sreg;
+    };
+
+    fetch(it.lo);
+    stage(0);
+    __syncthreads();
+    int buf = 0;
+    for (int base = it.lo; base < it.hi; base += kTile, buf ^= 1) {
+      const bool more = base + kTile < it.hi;
+      if (more) fetch(base + kTile);
+      if (base <= reach) {
+        f16v st[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) st[t][i] = 0.0f;
+#pragma unroll
+          for (int g = 0; g < kG; ++g) {
+            const h8 a = __builtin_bit_cast(h8, sh_k[buf][g][h2nd][32 * t + col]);
+            st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[g], st[t], 0, 0, 0);
+            st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[g], st[t], 0, 0, 0);
           }
         }
-        o[n] = o[n] * keep + acc;
+        // Scores in base-2 units; positions behind a row's own leave nothing.
+        float2 sc[4];
+        float vf[4], tile_top = vtop;
+        bool whole = true;  // every value scale of the tile is finite
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          sc[b] = sh_s[buf][b];
+          const bool fin = sc[b].y < INFINITY;
+          whole = whole && fin;
+          vf[b] = fin ? sc[b].y : 0.0f;
+          tile_top = fmaxf(tile_top, vf[b]);
+        }
+        float mx = m;
+        const bool edge = base + kTile - 1 > all;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const float f = ldexpf(A.scale * kLog2e * sc[b].x, -qs);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float x = st[b / 2][8 * (b & 1) + i] * f;
+            if (edge && base + 16 * b + 8 * (i / 4) + 4 * h2nd + i % 4 > limit) x = -INFINITY;
+            st[b / 2][8 * (b & 1) + i] = x;
+            mx = fmaxf(mx, x);
+          }
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        const float keep = exp2f(m - ref);
+        const float rescale = keep * (vtop / tile_top);
+        m = mx;
+        vtop = tile_top;
+        if (__any(rescale != 1.0f)) {
+#pragma unroll
+          for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= rescale;
+        }
+        const float to_w = ldexpf(1.0f, kWeightBits) / tile_top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const float fw = vf[b] * to_w;
+          h8 wh, wl;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float p = exp2f(st[b / 2][8 * (b & 1) + i] - ref);
+            sum += p;
+            const float w = p * fw;
+            wh[i] = static_cast<_Float16>(w);
+            wl[i] = static_cast<_Float16>(w - static_cast<float>(wh[i]));
+          }
+#pragma unroll
+          for (int d = 0; d < HD / 32; ++d) {
+            const h8 a = __builtin_bit_cast(h8, sh_v[buf][b][h2nd][32 * d + col]);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wh, o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wl, o[d], 0, 0, 0);
+          }
+        }
+        if (!whole) {
+          // A value scale that is inf or NaN shows in the rows that see a position of its block.
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if (base + 16 * b <= limit) sum = fmaf(sc[b].y, 0.0f, sum);
+        }
+        l = fmaf(l, keep, sum);
       }
-      __builtin_amdgcn_wave_barrier();
+      if (more) stage(buf ^ 1);
+      __syncthreads();
     }
-    for (int n = 0; n * 64 < dim; ++n) {
-      const int d = n * 64 + lane;
-      if (d < dim) A.out[t * A.out_stride + static_cast<std::size_t>(h) * dim + d] = o[n] / l;
+
+    l += __shfl_xor(l, 32, 64);
+    const float unit = vtop * ldexpf(1.0f, -kWeightBits);
+    if (live) {
+      float* dst;
+      float f;
+      if (it.part >= 0) {
+        const std::size_t slot =
+            (static_cast<std::size_t>(it.part) * A.g.kv_heads + head * kManySlots) * kFewRows + r;
+        dst = A.parts + slot * HD;
+        f = unit;
+        if (h2nd == 0) *reinterpret_cast<float2*>(A.parts + A.part_states + 2 * slot) = make_float2(m, l);
+      } else {
+        dst = A.out + static_cast<std::size_t>(s.row + tok) * A.out_stride + head_off;
+        f = unit / l;
+      }
+#pragma unroll
+      for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f4*>(dst + 32 * d + 8 * i + 4 * h2nd) =
+              f4{o[d][4 * i] * f, o[d][4 * i + 1] * f, o[d][4 * i + 2] * f, o[d][4 * i + 3] * f};
     }
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -420,7 +595,7 @@ int launch_attention(const llmi_hip_kv8_plan* p, const llmi_kv8_layer& layer, co
   const Lists& l = p->lists;
   AttnArgs a{p->view(), p->g, layer.k, layer.v, layer.scales, q, out, p->parts, q_stride, out_stride,
              p->max_parts * p->g.kv_heads * kFewRows * p->g.dim, scale,
-             captured ? -1 : static_cast<int>(l.tokens), captured ? -1 : static_cast<int>(l.few.size()),
+             captured ? -1 : static_cast<int>(l.few.size()), captured ? -1 : static_cast<int>(l.many.size()),
              captured ? -1 : static_cast<int>(l.join.size())};
   const std::size_t heads = static_cast<std::size_t>(p->g.kv_heads);
   const auto grid = [](std::size_t units) {
@@ -441,14 +616,21 @@ int launch_attention(const llmi_hip_kv8_plan* p, const llmi_kv8_layer& layer, co
       default: launch_few<256>(a, n, sizes, s); break;
     }
   }
+  if (captured || !l.many.empty()) {
+    const unsigned n = grid((captured ? p->max_many : l.many.size()) * heads);
+    switch (p->g.dim) {
+      case 32: attention_many<32><<<n, kThreads, 0, s>>>(a); break;
+      case 64: attention_many<64><<<n, kThreads, 0, s>>>(a); break;
+      case 96: attention_many<96><<<n, kThreads, 0, s>>>(a); break;
+      case 128: attention_many<128><<<n, kThreads, 0, s>>>(a); break;
+      case 160: attention_many<160><<<n, kThreads, 0, s>>>(a); break;
+      case 192: attention_many<192><<<n, kThreads, 0, s>>>(a); break;
+      case 224: attention_many<224><<<n, kThreads, 0, s>>>(a); break;
+      default: attention_many<256><<<n, kThreads, 0, s>>>(a); break;
+    }
+  }
   if (captured || !l.join.empty())
     attention_join<<<grid((captured ? p->max_join : l.join.size()) * heads * kFewRows), kThreads, 0, s>>>(a);
-  bool many = captured;
-  for (const Seq& q1 : l.seqs) many = many || static_cast<long>(q1.count) * p->g.group > kFewMax;
-  if (many) {
-    const std::size_t rows = (captured ? p->max_tokens : l.tokens) * static_cast<std::size_t>(p->g.heads);
-    attention_simple<<<grid(ceil_div(rows, kWaves)), kThreads, 0, s>>>(a);
-  }
   LLMI_TRY_HIP(hipGetLastError());
   return LLMI_OK;
 }

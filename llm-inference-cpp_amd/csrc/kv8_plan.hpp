@@ -40,20 +40,29 @@ constexpr int kFewMax = 64;  // most rows of a sequence and key/value head that 
 struct FewItem {
   std::int32_t seq, row0, rows, lo, hi, part;
 };
-// Partial slots part .. part + n - 1 hold the states of these rows.
+// `many` work: up to kManyRows rows over positions lo .. hi - 1 in the same
+// way; a partial state takes kManySlots slots.
+constexpr int kManyRows = 128, kManySlots = kManyRows / kFewRows;
+struct ManyItem {
+  std::int32_t seq, row0, rows, lo, hi, part;
+};
+// Up to 16 rows whose states are in the slots part + c * step, c < n, from
+// row `off` of each head's 16 * step rows on.
 struct JoinItem {
-  std::int32_t seq, row0, rows, part, n;
+  std::int32_t seq, row0, rows, part, n, step, off;
 };
 // Positions per split are chosen so that a batch makes about this many units
 // of work (item and key/value head); a split is at least kMinSplit positions.
 constexpr std::size_t kFewTarget = 2048;
 constexpr std::size_t kMinSplit = 4 * kTile;
+constexpr std::size_t kManyTarget = 512, kManyMinSplit = 8 * kTile;
 // Most partial slots of any batch: every split but a sequence's last one is
 // full, so there are at most kFewTarget / kv_heads full ones, and one more
 // for each of the row groups that are split.
 
 struct Lists {
   std::vector<FewItem> few;
+  std::vector<ManyItem> many;
   std::vector<JoinItem> join;
   std::size_t parts = 0;
   std::vector<Seq> seqs;
@@ -151,34 +160,48 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
     for (std::int32_t b = first; b <= last; ++b)
       if (b != then) l.append.push_back({seq, b, b == first ? then : -1});
   }
-  // Attention: sequences with few rows per key/value head are split over
-  // their history where the batch alone does not make enough work.
+  // Attention: rows are split over their history where the batch alone does
+  // not make enough work.
   const std::size_t group = sh.heads / sh.kv_heads;
-  std::size_t reach = 0;  // positions x row groups x heads of all few work
-  const auto row_groups = [&](const Seq& q) { return (q.count * group + kFewRows - 1) / kFewRows; };
-  for (const Seq& q : l.seqs)
-    if (q.count > 0 && q.count * group <= kFewMax)
-      reach += static_cast<std::size_t>(q.start + q.count) * row_groups(q) * sh.kv_heads;
-  const std::size_t split = std::max(kMinSplit, (reach / kFewTarget + kMinSplit - 1) / kMinSplit * kMinSplit);
-  for (std::size_t i = 0; i < seqs; ++i) {
-    const Seq& q = l.seqs[i];
-    const std::size_t rows = q.count * group;
-    if (rows == 0 || rows > kFewMax) continue;
-    for (std::size_t r = 0; r < rows; r += kFewRows) {
-      const auto row0 = static_cast<std::int32_t>(r);
-      const auto nrows = static_cast<std::int32_t>(std::min<std::size_t>(kFewRows, rows - r));
-      // The last row's position bounds what this group of rows sees.
-      const std::size_t len = static_cast<std::size_t>(q.start) + (r + static_cast<std::size_t>(nrows) - 1) / group + 1;
-      const std::size_t n = (len + split - 1) / split;
-      const auto seq = static_cast<std::int32_t>(i);
-      if (n > 1) l.join.push_back({seq, row0, nrows, static_cast<std::int32_t>(l.parts), static_cast<std::int32_t>(n)});
-      for (std::size_t c = 0; c < n; ++c)
-        l.few.push_back({seq, row0, nrows, static_cast<std::int32_t>(c * split),
-                         static_cast<std::int32_t>(std::min(len, (c + 1) * split)),
-                         n > 1 ? static_cast<std::int32_t>(l.parts + c) : -1});
-      if (n > 1) l.parts += n;
+  const auto rows_of = [&](const Seq& q) { return static_cast<std::size_t>(q.count) * group; };
+  // Positions that rows row0 .. row0 + n - 1 see: up to the last row's own.
+  const auto seen = [&](const Seq& q, std::size_t row0, std::size_t n) {
+    return static_cast<std::size_t>(q.start) + (row0 + n - 1) / group + 1;
+  };
+  // Over all groups of rows of one kind: fn(sequence, first row, rows, positions seen).
+  const auto each = [&](bool few, auto&& fn) {
+    const std::size_t most = few ? kFewRows : kManyRows;
+    for (std::size_t i = 0; i < seqs; ++i) {
+      const std::size_t rows = rows_of(l.seqs[i]);
+      if (rows == 0 || (rows <= kFewMax) != few) continue;
+      for (std::size_t r = 0; r < rows; r += most) {
+        const std::size_t n = std::min(most, rows - r);
+        fn(static_cast<std::int32_t>(i), r, n, seen(l.seqs[i], r, n));
+      }
     }
-  }
+  };
+  const auto split_of = [&](bool few, std::size_t target, std::size_t least) {
+    std::size_t reach = 0;
+    each(few, [&](std::int32_t, std::size_t, std::size_t, std::size_t len) { reach += len * sh.kv_heads; });
+    return std::max(least, (reach / target + least - 1) / least * least);
+  };
+  const auto lay = [&](bool few, std::size_t split, auto& items) {
+    const std::size_t slots = few ? 1 : kManySlots;
+    each(few, [&](std::int32_t seq, std::size_t r, std::size_t rows, std::size_t len) {
+      const std::size_t n = (len + split - 1) / split;
+      const auto i32 = [](std::size_t x) { return static_cast<std::int32_t>(x); };
+      for (std::size_t c = 0; c < n; ++c)
+        items.push_back({seq, i32(r), i32(rows), i32(c * split), i32(std::min(len, (c + 1) * split)),
+                         n > 1 ? i32(l.parts + c * slots) : -1});
+      if (n == 1) return;
+      for (std::size_t o = 0; o < rows; o += kFewRows)
+        l.join.push_back({seq, i32(r + o), i32(std::min<std::size_t>(kFewRows, rows - o)), i32(l.parts), i32(n),
+                          i32(slots), i32(o)});
+      l.parts += n * slots;
+    });
+  };
+  lay(true, split_of(true, kFewTarget, kMinSplit), l.few);
+  lay(false, split_of(false, kManyTarget, kManyMinSplit), l.many);
   return {};
 }
 

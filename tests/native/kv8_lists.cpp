@@ -74,6 +74,46 @@ int main() {
     for (const Seq& s : l.seqs)
       if (s.count > 0) blocks += static_cast<std::size_t>((s.start + s.count - 1) / kBlk - s.start / kBlk + 1);
     CHECK(written.size() == blocks);
+    // Attention: every row and position it may see once, each partial state
+    // in slots of its own, and within the limits that a plan is created for.
+    const std::size_t group = sh.heads / sh.kv_heads;
+    std::vector<std::vector<long>> reach(l.seqs.size());
+    for (std::size_t i = 0; i < l.seqs.size(); ++i) reach[i].assign(static_cast<std::size_t>(l.seqs[i].count) * group, 0);
+    std::vector<int> slot(l.parts, 0);
+    const auto walk = [&](const auto& items, int most, int slots, bool few) {
+      for (const auto& it : items) {
+        CHECK(it.rows > 0 && it.rows <= most && it.lo % kTile == 0 && it.lo < it.hi);
+        const Seq& s = l.seqs[static_cast<std::size_t>(it.seq)];
+        const std::size_t rows = static_cast<std::size_t>(s.count) * group;
+        CHECK((rows <= kFewMax) == few && static_cast<std::size_t>(it.row0 + it.rows) <= rows);
+        CHECK(it.hi <= s.start + s.count);
+        for (int r = it.row0; r < it.row0 + it.rows; ++r) {
+          const int own = s.start + r / static_cast<int>(group);  // the row's position
+          reach[static_cast<std::size_t>(it.seq)][static_cast<std::size_t>(r)] += std::max(0, std::min(it.hi, own + 1) - it.lo);
+        }
+        if (it.part >= 0)
+          for (int k = 0; k < slots; ++k) CHECK(++slot.at(static_cast<std::size_t>(it.part + k)) == 1);
+      }
+      return 0;
+    };
+    CHECK(walk(l.few, kFewRows, 1, true) == 0 && walk(l.many, kManyRows, kManySlots, false) == 0);
+    for (std::size_t i = 0; i < l.seqs.size(); ++i)
+      for (std::size_t r = 0; r < reach[i].size(); ++r) CHECK(reach[i][r] == l.seqs[i].start + static_cast<long>(r / group) + 1);
+    for (const int n_of : slot) CHECK(n_of == 1);
+    std::set<std::pair<int, int>> joined;
+    for (const JoinItem& j : l.join) {
+      CHECK(j.n > 1 && j.rows > 0 && j.rows <= kFewRows && j.off >= 0 && j.off + j.rows <= kFewRows * j.step);
+      CHECK(j.part >= 0 && static_cast<std::size_t>(j.part + j.n * j.step) <= l.parts);
+      for (int r = 0; r < j.rows; ++r) CHECK(joined.insert({j.seq, j.row0 + r}).second);
+    }
+    for (const auto* items : {&l.few}) for (const auto& it : *items) CHECK((it.part >= 0) == (joined.count({it.seq, it.row0}) > 0));
+    for (const auto& it : l.many) CHECK((it.part >= 0) == (joined.count({it.seq, it.row0}) > 0));
+    const std::size_t few_splits = kFewTarget / sh.kv_heads, many_splits = kManyTarget / sh.kv_heads;
+    const std::size_t busy = std::min<std::size_t>(static_cast<std::size_t>(n), tokens);
+    CHECK(l.few.size() <= few_splits + (kFewMax / kFewRows) * busy);
+    CHECK(l.many.size() <= many_splits + tokens * group / kManyRows + busy);
+    CHECK(l.join.size() <= few_splits + kManySlots * many_splits);
+    CHECK(l.parts <= 2 * few_splits + 2 * kManySlots * many_splits);
     CHECK(l.append.size() <= tokens / kBlk + 2 * std::min<std::size_t>(static_cast<std::size_t>(n), tokens));
   }
   std::puts("ok");
