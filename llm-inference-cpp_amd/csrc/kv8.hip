@@ -381,6 +381,7 @@ llmi_hip_kv8_plan::~llmi_hip_kv8_plan() {
   if (copied != nullptr) (void)hipEventDestroy(copied);
   if (dev != nullptr) (void)hipFree(dev);
   if (parts != nullptr) (void)hipFree(parts);
+  if (joins != nullptr) (void)hipFree(joins);
   if (pinned != nullptr) (void)hipHostFree(pinned);
 }
 
@@ -436,18 +437,11 @@ int llmi_hip_kv8_plan_create(const llmi_kv8_shape* shape, size_t max_seqs, size_
   p->g.dim = static_cast<int>(shape->head_dim);
   p->g.page_blocks = static_cast<int>(shape->page_tokens) / kBlk;
   p->g.block_bytes = static_cast<std::size_t>(kBlk) * shape->head_dim;
-  // Every block of new tokens: a whole number of them per sequence, and up
-  // to two that are not full.
-  p->max_append = max_tokens / kBlk + 2 * std::min(max_seqs, max_tokens);
-  // Splits: a kind's positions x heads over its split size are at most its
-  // target, so are the full splits x heads, and a group of rows that is split
-  // has at most twice its full ones; every group adds one item at most.
-  const std::size_t few_splits = kFewTarget / shape->kv_heads, many_splits = kManyTarget / shape->kv_heads;
-  const std::size_t busy = std::min(max_seqs, max_tokens), group = shape->heads / shape->kv_heads;
-  p->max_few = few_splits + (kFewMax / kFewRows) * busy;
-  p->max_many = many_splits + max_tokens * group / kManyRows + busy;
-  p->max_join = few_splits + kManySlots * many_splits;
-  p->max_parts = 2 * few_splits + 2 * kManySlots * many_splits;
+  p->g.by_page = divisor(static_cast<std::uint32_t>(p->g.page_blocks));
+  p->most = limits(*shape, max_seqs, max_tokens);
+  // Kernels count units of work (item and key/value head) in 32 bits.
+  LLMI_REQUIRE(std::max({2 * p->most.append, p->most.few, p->most.many}) * shape->kv_heads <= 0x7FFFFFFFu,
+               "kv8_plan_create: too many sequences and tokens for the heads");
   const auto take = [&](std::size_t bytes) {
     const std::size_t at = p->bytes;
     p->bytes += (bytes + 255) / 256 * 256;
@@ -455,15 +449,16 @@ int llmi_hip_kv8_plan_create(const llmi_kv8_shape* shape, size_t max_seqs, size_
   };
   (void)take(sizeof(Counts));
   p->off_seqs = take(max_seqs * sizeof(Seq));
-  p->off_append = take(p->max_append * sizeof(AppendItem));
-  p->off_few = take(p->max_few * sizeof(FewItem));
-  p->off_many = take(p->max_many * sizeof(ManyItem));
-  p->off_join = take(p->max_join * sizeof(JoinItem));
+  p->off_append = take(p->most.append * sizeof(AppendItem));
+  p->off_few = take(p->most.few * sizeof(AttnItem));
+  p->off_many = take(p->most.many * sizeof(AttnItem));
   p->off_table = take(max_pages * sizeof(std::int32_t));
   LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&p->dev), p->bytes));
   LLMI_TRY_HIP(hipHostMalloc(reinterpret_cast<void**>(&p->pinned), p->bytes, hipHostMallocDefault));
-  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&p->parts), p->max_parts * shape->kv_heads * kFewRows *
-                                                                  (shape->head_dim + 2) * sizeof(float)));
+  const std::size_t rows = p->most.parts * shape->kv_heads * kSlotRows, joins = p->most.joins * shape->kv_heads + 1;
+  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&p->parts), (rows + 1) * (shape->head_dim + 2) * sizeof(float)));
+  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&p->joins), joins * sizeof(int)));
+  LLMI_TRY_HIP(hipMemset(p->joins, 0, joins * sizeof(int)));
   LLMI_TRY_HIP(hipEventCreateWithFlags(&p->copied, hipEventDisableTiming));
   *plan = p.release();
   return LLMI_OK;
@@ -480,9 +475,8 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     const std::string why = build(p->shape, seqs, slots, starts, counts, tables, table_stride, p->max_seqs,
                                   p->max_tokens, p->max_pages, &l);
     LLMI_REQUIRE(why.empty(), "kv8_plan_set: " + why);
-    LLMI_REQUIRE(l.append.size() <= p->max_append && l.few.size() <= p->max_few &&
-                     l.many.size() <= p->max_many && l.join.size() <= p->max_join &&
-                     l.parts <= p->max_parts,
+    LLMI_REQUIRE(l.append.size() <= p->most.append && l.few.size() <= p->most.few &&
+                     l.many.size() <= p->most.many && l.parts <= p->most.parts && l.joins <= p->most.joins,
                  "kv8_plan_set: more work than the plan was created for");
     if (p->append_captured) {
       LLMI_REQUIRE(l.writable, "kv8_plan_set: an append of this plan was captured, and " + l.why_not);
@@ -492,7 +486,7 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     LLMI_TRY_HIP(hipEventSynchronize(p->copied));
     const Counts c{static_cast<std::int32_t>(l.append.size()), static_cast<std::int32_t>(l.tokens),
                    static_cast<std::int32_t>(l.seqs.size()), static_cast<std::int32_t>(l.few.size()),
-                   static_cast<std::int32_t>(l.many.size()), static_cast<std::int32_t>(l.join.size())};
+                   static_cast<std::int32_t>(l.many.size())};
     const auto put = [&](std::size_t at, const auto& v) {
       if (!v.empty()) std::memcpy(p->pinned + at, v.data(), v.size() * sizeof(v[0]));
     };
@@ -501,7 +495,6 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     put(p->off_append, l.append);
     put(p->off_few, l.few);
     put(p->off_many, l.many);
-    put(p->off_join, l.join);
     put(p->off_table, l.table);
     const std::size_t used = p->off_table + l.table.size() * sizeof(std::int32_t);
     p->set = false;
@@ -556,7 +549,7 @@ int llmi_hip_kv8_append_dev(const llmi_hip_kv8_plan* p, const llmi_kv8_layer* la
     p->append_captured = true;
     if (cos_t != nullptr) p->captured_positions = std::min(p->captured_positions, positions);
     a.nappend = a.ntokens = -1;
-    blocks = p->max_append;
+    blocks = p->most.append;
     tokens = p->max_tokens;
   }
   const std::size_t units = 2 * blocks * g.kv_heads + (q != nullptr ? ceil_div(tokens * g.heads * lpr, 64) : 0);
@@ -605,7 +598,7 @@ int llmi_hip_kv8_read_dev(const llmi_hip_kv8_plan* p, const llmi_kv8_layer* laye
   std::size_t blocks = p->lists.append.size();
   if (captured) {
     a.nappend = -1;
-    blocks = p->max_append;
+    blocks = p->most.append;
   }
   read_kernel<<<grid_for(2 * blocks * p->g.kv_heads), kThreads, 0, pick(stream)>>>(a);
   LLMI_TRY_HIP(hipGetLastError());

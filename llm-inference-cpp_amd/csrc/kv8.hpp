@@ -9,7 +9,7 @@ namespace llmi_hip::kv8 {
 // Item counts of the batch that is set, in device memory (launches replayed
 // from a graph read them there).
 struct Counts {
-  std::int32_t append, tokens, seqs, few, many, join;
+  std::int32_t append, tokens, seqs, few, many;
 };
 
 // A plan's device lists.
@@ -18,23 +18,30 @@ struct View {
   const Seq* seqs;
   const std::int32_t* table;
   const AppendItem* append;
-  const FewItem* few;
-  const ManyItem* many;
-  const JoinItem* join;
+  const AttnItem* few;
+  const AttnItem* many;
 };
 
 struct Geometry {
   int heads, kv_heads, group, dim, page_blocks;
+  Divisor by_page;  // divides a block by page_blocks
   std::size_t block_bytes;  // of one head's block of k (or v): 16 * dim
 };
 
-// Block `block` of sequence s for head h: its index in [page][kv head][block].
-// Page ids and positions were checked on the host, so the index is in range.
+// Which page of its sequence's table holds a block.
+__device__ __forceinline__ int page_of(const Geometry& g, int block) {
+  return static_cast<int>((static_cast<std::uint64_t>(static_cast<std::uint32_t>(block)) * g.by_page.m) >> g.by_page.k);
+}
+// A block of head h in [page][kv head][block], given the page's id and its
+// place in the table.  Ids and positions were checked on the host, so the
+// index is in range.
+__device__ __forceinline__ std::size_t block_at(const Geometry& g, int id, int page, int block, int h) {
+  return (static_cast<std::size_t>(id) * g.kv_heads + h) * g.page_blocks + (block - page * g.page_blocks);
+}
 __device__ __forceinline__ std::size_t block_index(const Geometry& g, const std::int32_t* __restrict__ table,
                                                    const Seq& s, int block, int h) {
-  const int page = block / g.page_blocks;
-  const std::size_t id = static_cast<std::size_t>(table[s.table + page]);
-  return (id * g.kv_heads + h) * g.page_blocks + (block - page * g.page_blocks);
+  const int page = page_of(g, block);
+  return block_at(g, table[s.table + page], page, block, h);
 }
 
 int launch_attention(const llmi_hip_kv8_plan* p, const llmi_kv8_layer& layer, const float* q, std::size_t q_stride,
@@ -50,10 +57,12 @@ struct llmi_hip_kv8_plan {
   // marks the copy's end, before which the pinned side is not written again.
   std::uint8_t* dev = nullptr;
   std::uint8_t* pinned = nullptr;
-  std::size_t bytes = 0, off_seqs = 0, off_table = 0, off_append = 0, off_few = 0, off_many = 0, off_join = 0;
-  std::size_t max_append = 0, max_few = 0, max_many = 0, max_join = 0, max_parts = 0;
-  // The attention's partial states (launches of one plan follow each other).
+  std::size_t bytes = 0, off_seqs = 0, off_table = 0, off_append = 0, off_few = 0, off_many = 0;
+  llmi_hip::kv8::Limits most{};
+  // The attention's partial states, and how many pieces of split rows have
+  // ended (0 between launches; launches of one plan follow each other).
   float* parts = nullptr;
+  int* joins = nullptr;
   hipEvent_t copied = nullptr;
   bool set = false;
   llmi_hip::kv8::Lists lists;
@@ -65,8 +74,8 @@ struct llmi_hip_kv8_plan {
     using namespace llmi_hip::kv8;
     return {reinterpret_cast<const Counts*>(dev), reinterpret_cast<const Seq*>(dev + off_seqs),
             reinterpret_cast<const std::int32_t*>(dev + off_table),
-            reinterpret_cast<const AppendItem*>(dev + off_append), reinterpret_cast<const FewItem*>(dev + off_few),
-            reinterpret_cast<const ManyItem*>(dev + off_many), reinterpret_cast<const JoinItem*>(dev + off_join)};
+            reinterpret_cast<const AppendItem*>(dev + off_append), reinterpret_cast<const AttnItem*>(dev + off_few),
+            reinterpret_cast<const AttnItem*>(dev + off_many)};
   }
   ~llmi_hip_kv8_plan();
 };

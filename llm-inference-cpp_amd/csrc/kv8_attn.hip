@@ -4,7 +4,9 @@
 namespace llmi_hip::kv8 {
 namespace {
 
-constexpr int kThreads = 256, kWaves = 4;
+typedef int i4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // rows may start at any float
+constexpr float kLog2e = 1.44269504088896340736f;
 
 struct AttnArgs {
   View v;
@@ -14,10 +16,181 @@ struct AttnArgs {
   const float* q;
   float* out;
   float* parts;  // rows of partial states: o (dim floats each), then (maximum, sum) each
-  std::size_t q_stride, out_stride, part_states;  // part_states: float offset of the (maximum, sum) pairs
+  int* joins;    // per split rows and head: how many pieces have ended
+  std::size_t q_stride, out_stride, part_states;  // part_states: where the (maximum, sum) pairs begin, in floats
   float scale;
-  int nfew, nmany, njoin;  // -1: from v.counts (a captured launch)
+  int nfew, nmany;  // -1: from v.counts (a captured launch)
 };
+
+// 2^x by the hardware instruction: one rounding; results below 2^-126, which
+// no sum here keeps, are 0.
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Row r of a work item: its token and its place in q and out.
+struct Row {
+  int tok;
+  std::size_t off;  // of head_dim floats in the token's row
+};
+__device__ __forceinline__ Row row_of(const AttnArgs& A, const AttnItem& it, int head, int r) {
+  const int row = it.row0 + r, tok = row / A.g.group;
+  return {tok, static_cast<std::size_t>(head * A.g.group + (row - tok * A.g.group)) * A.g.dim};
+}
+
+// Partial states cross workgroups, so they go past the caches that other
+// parts of the chip do not see: device-scope relaxed atomics, in pairs of
+// floats, one store or load each.
+__device__ __forceinline__ void put2(float* p, float a, float b) {
+  __hip_atomic_store(reinterpret_cast<std::uint64_t*>(p),
+                     (static_cast<std::uint64_t>(__float_as_uint(b)) << 32) | __float_as_uint(a), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float* p) {
+  const std::uint64_t u = __hip_atomic_load(reinterpret_cast<const std::uint64_t*>(p), __ATOMIC_RELAXED,
+                                            __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float(static_cast<std::uint32_t>(u)), __uint_as_float(static_cast<std::uint32_t>(u >> 32)));
+}
+// Row r of piece c's partial state (MOST rows a piece).
+template <int MOST>
+__device__ __forceinline__ std::size_t part_row(const AttnArgs& A, int part, int head, int r) {
+  return static_cast<std::size_t>(part) * A.g.kv_heads * kSlotRows + static_cast<std::size_t>(head) * MOST + r;
+}
+
+// Called by every thread of a workgroup after its stores of a piece's state:
+// true for the workgroup that ends last, with the counter back at 0.  Every
+// thread's stores have reached device scope (the wait) before its workgroup
+// counts, so the last one sees all of them.
+__device__ __forceinline__ bool last_piece(const AttnArgs& A, const AttnItem& it, int head, int* flag) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int* c = A.joins + static_cast<std::size_t>(it.join) * A.g.kv_heads + head;
+    const bool last = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.n - 1;
+    if (last) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = last;
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+// Joins the n pieces of up to MOST rows in the pieces' order: a thread takes
+// two dims of a row over every `share`-th piece, eight loads in flight, with
+// the running maximum; the shares meet in `sh` (THREADS x 4 floats).
+template <int HD, int MOST, int THREADS>
+__device__ void join_pieces(const AttnArgs& A, const AttnItem& it, int head, float4* sh) {
+  constexpr int kPairs = HD / 2;
+  const int cells = it.rows * kPairs;
+  const int share = cells >= THREADS ? 1 : min(THREADS / cells, it.n);
+  const int step = (MOST / kSlotRows);
+  for (int base = 0; base < cells; base += THREADS) {
+    const int mine = static_cast<int>(threadIdx.x) % min(cells, THREADS), cell = base + mine;
+    const int of = static_cast<int>(threadIdx.x) / min(cells, THREADS);
+    const int r = cell / kPairs, d = 2 * (cell - r * kPairs);
+    float m = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
+    if (cell < cells && of < share) {
+      for (int c0 = of; c0 < it.n; c0 += 8 * share) {
+        float2 st[8], o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int c = c0 + j * share;
+          st[j] = make_float2(-INFINITY, 0.0f);
+          o[j] = make_float2(0.0f, 0.0f);
+          if (c < it.n) {
+            const std::size_t row = part_row<MOST>(A, it.first + c * step, head, r);
+            st[j] = get2(A.parts + A.part_states + 2 * row);
+            o[j] = get2(A.parts + row * HD + d);
+          }
+        }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, st[j].x);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        const float keep = exp2_hw(m - ref);
+        l *= keep;
+        x *= keep;
+        y *= keep;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float f = exp2_hw(st[j].x - ref);
+          l = fmaf(st[j].y, f, l);
+          x = fmaf(o[j].x, f, x);
+          y = fmaf(o[j].y, f, y);
+        }
+        m = top;
+      }
+    }
+    if (share > 1) {
+      sh[threadIdx.x] = make_float4(m, l, x, y);
+      __syncthreads();
+      if (of == 0) {
+        for (int w = 1; w < share; ++w) {
+          const float4 p = sh[w * cells + mine];
+          const float top = fmaxf(m, p.x), ref = top == -INFINITY ? 0.0f : top;
+          const float f = exp2_hw(m - ref), g = exp2_hw(p.x - ref);
+          l = fmaf(p.y, g, l * f);
+          x = fmaf(p.z, g, x * f);
+          y = fmaf(p.w, g, y * f);
+          m = top;
+        }
+      }
+    }
+    if (cell < cells && of == 0) {
+      const Row w = row_of(A, it, head, r);
+      float* dst = A.out + static_cast<std::size_t>(it.row + w.tok) * A.out_stride + w.off + d;
+      dst[0] = x / l;
+      dst[1] = y / l;
+    }
+  }
+}
+
+// The same for many rows of few pieces: four dims of each of kAt rows at a
+// time, a piece after the other.  Plain loads, behind an acquire of what the
+// other workgroups stored.
+template <int HD, int MOST, int THREADS>
+__device__ void join_rows(const AttnArgs& A, const AttnItem& it, int head) {
+  constexpr int kQuads = HD / 4, kAt = 8, kStep = MOST / kSlotRows;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  const int cells = it.rows * kQuads;
+  for (int base = threadIdx.x; base < cells; base += kAt * THREADS) {
+    float m[kAt], l[kAt];
+    float4 o[kAt];
+#pragma unroll
+    for (int j = 0; j < kAt; ++j) {
+      m[j] = -INFINITY;
+      l[j] = 0.0f;
+      o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    for (int c = 0; c < it.n; ++c) {
+      float2 st[kAt];
+      float4 x[kAt];
+#pragma unroll
+      for (int j = 0; j < kAt; ++j) {
+        const int cell = min(base + j * THREADS, cells - 1), r = cell / kQuads;
+        const std::size_t row = part_row<MOST>(A, it.first + c * kStep, head, r);
+        st[j] = *reinterpret_cast<const float2*>(A.parts + A.part_states + 2 * row);
+        x[j] = *reinterpret_cast<const float4*>(A.parts + row * HD + 4 * (cell - r * kQuads));
+      }
+#pragma unroll
+      for (int j = 0; j < kAt; ++j) {
+        const float top = fmaxf(m[j], st[j].x), ref = top == -INFINITY ? 0.0f : top;
+        const float f = exp2_hw(m[j] - ref), g = exp2_hw(st[j].x - ref);
+        m[j] = top;
+        l[j] = fmaf(st[j].y, g, l[j] * f);
+        o[j].x = fmaf(x[j].x, g, o[j].x * f);
+        o[j].y = fmaf(x[j].y, g, o[j].y * f);
+        o[j].z = fmaf(x[j].z, g, o[j].z * f);
+        o[j].w = fmaf(x[j].w, g, o[j].w * f);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAt; ++j) {
+      const int cell = base + j * THREADS, r = cell / kQuads;
+      if (cell >= cells) break;
+      const Row w = row_of(A, it, head, r);
+      *reinterpret_cast<f4*>(A.out + static_cast<std::size_t>(it.row + w.tok) * A.out_stride + w.off +
+                             4 * (cell - r * kQuads)) = f4{o[j].x / l[j], o[j].y / l[j], o[j].z / l[j], o[j].w / l[j]};
+    }
+  }
+}
 
 // ------------------------------------------------------------- few rows
 // Single tokens and drafts: up to 16 rows (tokens x query heads of one
@@ -31,9 +204,8 @@ struct AttnArgs {
 //   output   O[head][dim]      = W V     A = digits of w, B = value codes
 // with w = p * (value scale / the tile's largest) in [0, 1], p the weight
 // against the running maximum.  A wavefront takes tiles of 64 positions = 4
-// blocks; a workgroup's four wavefronts take a range's tiles in turn and merge.
-typedef int i4 __attribute__((ext_vector_type(4)));
-typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // rows may start at any float
+// blocks; a workgroup's wavefronts take a range's tiles in turn and merge.
+constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
 
 // Maximum over the 16 lanes of a row of lanes, in every lane.
 __device__ __forceinline__ float row16_max(float v) {
@@ -60,17 +232,20 @@ __device__ __forceinline__ float undigit(i4 s) {
   return fmaf(x, 256.0f, static_cast<float>(s[0]));
 }
 
-// HD: head_dim; MT: tiles of 4 rows (16 digit rows).
+// HD: head_dim; MT: tiles of 4 rows (16 digit rows) there is room for.
 template <int HD, int MT>
-__global__ void __launch_bounds__(kThreads) attention_few(AttnArgs A) {
+__global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
+  constexpr int kWaves = kFewWaves, kThreads = kFewThreads;
   constexpr int kG = HD / 16;            // 16-dim groups of a block
   constexpr int kC = (HD + 63) / 64;     // 64-dim steps of a score product
   constexpr int kRows = 4 * MT;
-  constexpr float kLog2e = 1.44269504088896340736f;
   __shared__ union {
     std::uint32_t w[kWaves][4][4][16];   // a tile's weight digits: [block][head of the 4][position]
-    float o[kWaves][kRows][HD];          // the wavefronts' outputs, merged at the end
+    float o[kWaves][kRows][HD + 16];     // (16: a row of lanes writes other banks than the next)
+                                         // the wavefronts' outputs, merged at the end
+    float4 join[kThreads];
   } sh;
+  __shared__ int sh_last;
   __shared__ float sh_m[kWaves][kRows], sh_l[kWaves][kRows];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -79,9 +254,7 @@ __global__ void __launch_bounds__(kThreads) attention_few(AttnArgs A) {
   const int units = nfew * A.g.kv_heads;
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     const int item = u / A.g.kv_heads, h = u - item * A.g.kv_heads;
-    const FewItem it = A.v.few[item];
-    if ((it.rows + 3) / 4 > MT || (MT > 1 && (it.rows + 3) / 4 <= MT / 2)) continue;  // another instance's
-    const Seq s = A.v.seqs[it.seq];
+    const AttnItem it = A.v.few[item];
 
     // The digits of q: lane (digit row lo16, dims 16 grp ..) of each 64-dim step.
     i4 qd[MT][kC];
@@ -91,9 +264,9 @@ __global__ void __launch_bounds__(kThreads) attention_few(AttnArgs A) {
     for (int mt = 0; mt < MT; ++mt) {
       const int r = 4 * mt + lo16 / 4;
       const bool live = r < it.rows;
-      const int row = it.row0 + (live ? r : 0), tok = row / A.g.group;
-      const float* qp = A.q + static_cast<std::size_t>(s.row + tok) * A.q_stride +
-                        static_cast<std::size_t>(h * A.g.group + (row - tok * A.g.group)) * HD;
+      const Row w = row_of(A, it, h, live ? r : 0);
+      const float* qp = A.q + static_cast<std::size_t>(it.row + w.tok) * A.q_stride + w.off;
+      // Rows of nobody repeat the first one; nothing of theirs is kept.
       float x[kC][16];
       float top = 0.0f;
       bool bad = false;
@@ -101,10 +274,14 @@ __global__ void __launch_bounds__(kThreads) attention_few(AttnArgs A) {
       for (int c = 0; c < kC; ++c) {
         const int g = 4 * c + grp;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          x[c][i] = live && g < kG ? qp[g * 16 + i] : 0.0f;
-          top = fmaxf(top, fabsf(x[c][i]));
-          bad |= !(fabsf(x[c][i]) < INFINITY);
+        for (int i = 0; i < 16; i += 4) {
+          const f4 y = *reinterpret_cast<const f4*>(qp + min(g, kG - 1) * 16 + i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[c][i + j] = g < kG ? y[j] : 0.0f;
+            top = fmaxf(top, fabsf(x[c][i + j]));
+            bad |= !(fabsf(x[c][i + j]) < INFINITY);
+          }
         }
       }
       top = fmaxf(top, __shfl_xor(top, 16, 64));
@@ -128,6 +305,7 @@ __global__ void __launch_bounds__(kThreads) attention_few(AttnArgs A) {
         }
       // Lanes 4 hd .. of any group hold head hd's; an inf or NaN in q makes the row's sum NaN.
       qe[mt] = __shfl(e - 30, 4 * grp, 64);
+      __builtin_amdgcn_sched_barrier(0);  // one tile of rows at a time: registers
       l[mt] = __shfl(static_cast<int>(bad), 4 * grp, 64) != 0 ? __builtin_nanf("") : 0.0f;
     }
 
@@ -135,7 +313,7 @@ __global__ void __launch_bounds__(kThreads) attention_few(AttnArgs A) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int r = 4 * mt + grp;
-      limit[mt] = r < it.rows ? s.start + (it.row0 + r) / A.g.group : -1;
+      limit[mt] = r < it.rows ? it.start + (it.row0 + r) / A.g.group : -1;
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -145,13 +323,17 @@ __global__ void __launch_bounds__(kThreads) attention_few(AttnArgs A) {
     }
 
     const int last_block = (it.hi - 1) / kBlk;
+    // This lane's block of a tile is block base / 16 + grp; behind the range,
+    // the last one again (its positions there are masked), with scales of 0.
+    // Its page id is read a tile ahead.
+    const auto page_id = [&](int base) { return A.v.table[it.table + page_of(A.g, min(base / kBlk + grp, last_block))]; };
+    int id = page_id(min(it.lo + wave * kTile, it.hi - 1));
     for (int base = it.lo + wave * kTile; base < it.hi; base += kWaves * kTile) {
-      // This lane's block of the tile; behind the range, the last one again
-      // (its positions there are masked), with scales of 0.
-      const int block = base / kBlk + grp;
-      const std::size_t at = block_index(A.g, A.v.table, s, min(block, last_block), h);
+      const int want = base / kBlk + grp, block = min(want, last_block);
+      const std::size_t at = block_at(A.g, id, page_of(A.g, block), block, h);
+      if (base + kWaves * kTile < it.hi) id = page_id(base + kWaves * kTile);
       float2 sc = reinterpret_cast<const float2*>(A.scales)[at];
-      if (block > last_block) sc = make_float2(0.0f, 0.0f);
+      if (want > last_block) sc = make_float2(0.0f, 0.0f);
       const std::int8_t* kp = A.k + at * (16 * HD);
       const std::int8_t* vp = A.val + at * (16 * HD) + lo16 * 16;
       // Keys: every lane needs all four blocks, position lo16, dims 16 (4c + grp) ...
@@ -186,6 +368,7 @@ __global__ void __launch_bounds__(kThreads) attention_few(AttnArgs A) {
       const float to_fix = 0x1p30f / top;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
+        if (4 * mt >= it.rows) break;
         float x[4];
         float mx = m[mt];
 #pragma unroll
@@ -199,13 +382,13 @@ __global__ void __launch_bounds__(kThreads) attention_few(AttnArgs A) {
         }
         mx = row16_max(mx);
         const float ref = mx == -INFINITY ? 0.0f : mx;
-        const float keep = exp2f(m[mt] - ref);
+        const float keep = exp2_hw(m[mt] - ref);
         m[mt] = mx;
         float sum = 0.0f;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           const bool seen = base + b * kBlk + lo16 <= limit[mt];
-          const float p = exp2f(x[b] - ref);
+          const float p = exp2_hw(x[b] - ref);
           // A value scale that is inf or NaN shows in the sum of the rows that see the block.
           if (seen) sum += fmaf(vs[b], 0.0f, p);
           const int w = static_cast<int>(rintf(p * (vf_s[b] * to_fix)));
@@ -233,6 +416,7 @@ __global__ void __launch_bounds__(kThreads) attention_few(AttnArgs A) {
           acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wd, vf[g], acc, 0, 0, 0);
           o[mt][g] = fmaf(o[mt][g], keep, undigit(acc) * from_fix);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
 
@@ -249,80 +433,33 @@ __global__ void __launch_bounds__(kThreads) attention_few(AttnArgs A) {
       for (int g = 0; g < kG; ++g) sh.o[wave][4 * mt + grp][16 * g + lo16] = o[mt][g];
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < it.rows * HD; e += kThreads) {
-      const int r = e / HD, d = e - r * HD;
+    for (int e = threadIdx.x; e < it.rows * (HD / 2); e += kThreads) {
+      const int r = e / (HD / 2), d = 2 * (e - r * (HD / 2));
       float top = sh_m[0][r];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sh_m[w][r]);
       const float ref = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f, acc = 0.0f;
+      float sum = 0.0f, x = 0.0f, y = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        const float f = exp2f(sh_m[w][r] - ref);
+        const float f = exp2_hw(sh_m[w][r] - ref);
         sum = fmaf(sh_l[w][r], f, sum);
-        acc = fmaf(sh.o[w][r][d], f, acc);
+        x = fmaf(sh.o[w][r][d], f, x);
+        y = fmaf(sh.o[w][r][d + 1], f, y);
       }
-      if (it.part >= 0) {
-        const std::size_t slot = (static_cast<std::size_t>(it.part) * A.g.kv_heads + h) * kFewRows + r;
-        A.parts[slot * HD + d] = acc;
-        if (d == 0) *reinterpret_cast<float2*>(A.parts + A.part_states + 2 * slot) = make_float2(top, sum);
+      if (it.n > 1) {
+        const std::size_t row = part_row<few_rows(HD)>(A, it.part, h, r);
+        put2(A.parts + row * HD + d, x, y);
+        if (d == 0) put2(A.parts + A.part_states + 2 * row, top, sum);
       } else {
-        const int row = it.row0 + r, tok = row / A.g.group;
-        A.out[static_cast<std::size_t>(s.row + tok) * A.out_stride +
-              static_cast<std::size_t>(h * A.g.group + (row - tok * A.g.group)) * HD + d] = acc / sum;
+        const Row w = row_of(A, it, h, r);
+        float* dst = A.out + static_cast<std::size_t>(it.row + w.tok) * A.out_stride + w.off + d;
+        dst[0] = x / sum;
+        dst[1] = y / sum;
       }
     }
+    if (it.n > 1 && last_piece(A, it, h, &sh_last)) join_pieces<HD, few_rows(HD), kThreads>(A, it, h, sh.join);
     __syncthreads();
-  }
-}
-
-// Joins the partial states of split rows: one workgroup per row group, head
-// and row, in the splits' order.
-__global__ void __launch_bounds__(kThreads) attention_join(AttnArgs A) {
-  __shared__ float sh_o[kThreads], sh_l[kThreads];
-  const int njoin = A.njoin >= 0 ? A.njoin : A.v.counts->join;
-  const int dim = A.g.dim;
-  const long units = static_cast<long>(njoin) * A.g.kv_heads * kFewRows;
-  for (long u = blockIdx.x; u < units; u += gridDim.x) {
-    const int r = static_cast<int>(u % kFewRows);
-    const int h = static_cast<int>(u / kFewRows % A.g.kv_heads);
-    const JoinItem it = A.v.join[u / kFewRows / A.g.kv_heads];
-    if (r >= it.rows) continue;
-    const auto slot = [&](int c) {
-      return (static_cast<std::size_t>(it.part + c * it.step) * A.g.kv_heads + h * it.step) * kFewRows + it.off + r;
-    };
-    const auto state = [&](int c) { return *reinterpret_cast<const float2*>(A.parts + A.part_states + 2 * slot(c)); };
-    float top = -INFINITY;
-    for (int c = threadIdx.x & 63; c < it.n; c += 64) top = fmaxf(top, state(c).x);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    const float ref = top == -INFINITY ? 0.0f : top;
-    // 64 dims at a time, a quarter of the splits to each wavefront.
-    const Seq s = A.v.seqs[it.seq];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int d0 = 0; d0 < dim; d0 += 64) {
-      const int d = d0 + lane;
-      float sum = 0.0f, acc = 0.0f;
-      for (int c = wave; c < it.n; c += kWaves) {
-        const float2 ml = state(c);
-        const float f = exp2f(ml.x - ref);
-        sum = fmaf(ml.y, f, sum);
-        if (d < dim) acc = fmaf(A.parts[slot(c) * dim + d], f, acc);
-      }
-      sh_o[threadIdx.x] = acc;
-      sh_l[threadIdx.x] = sum;
-      __syncthreads();
-      if (wave == 0 && d < dim) {
-        for (int w = 1; w < kWaves; ++w) {
-          acc += sh_o[64 * w + lane];
-          sum += sh_l[64 * w + lane];
-        }
-        const int row = it.row0 + r, tok = row / A.g.group;
-        A.out[static_cast<std::size_t>(s.row + tok) * A.out_stride +
-              static_cast<std::size_t>(h * A.g.group + (row - tok * A.g.group)) * dim + d] = acc / sum;
-      }
-      __syncthreads();
-    }
   }
 }
 
@@ -356,40 +493,45 @@ __device__ __forceinline__ void halves(std::uint32_t w, std::uint32_t* out) {
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) attention_many(AttnArgs A) {
+__global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArgs A) {
+  constexpr int kThreads = 256;
   constexpr int kG = HD / 16;
   constexpr int kChunks = 4 * HD;  // 16-byte pieces of a tile's keys (and of its values)
   constexpr int kPer = (kChunks + kThreads - 1) / kThreads;
-  constexpr float kLog2e = 1.44269504088896340736f;
   __shared__ uint4 sh_k[2][kG][2][kTile];     // [16-dim group][half of it][position]: 8 fp16
   __shared__ uint4 sh_v[2][kTile / 16][2][HD];  // [block][h][dim]: positions 4h.., 8 + 4h..
   __shared__ float2 sh_s[2][4];
+  __shared__ int sh_last;
   const int lane = threadIdx.x & 63, col = lane & 31, h2nd = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nmany = A.nmany >= 0 ? A.nmany : A.v.counts->many;
   const int units = nmany * A.g.kv_heads;
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     const int item = u / A.g.kv_heads, head = u - item * A.g.kv_heads;
-    const ManyItem it = A.v.many[item];
-    const Seq s = A.v.seqs[it.seq];
+    const AttnItem it = A.v.many[item];
     const int r = wave * 32 + col;
     const bool live = r < it.rows;
-    const int row = it.row0 + (live ? r : 0), tok = row / A.g.group;
-    const int limit = live ? s.start + tok : -1;
-    const std::size_t head_off = static_cast<std::size_t>(head * A.g.group + (row - tok * A.g.group)) * HD;
+    const Row own = row_of(A, it, head, live ? r : 0);
+    const int limit = live ? it.start + own.tok : -1;
+    // A negative scale goes to q, so that a block's largest score is its largest product.
+    const float q_sign = A.scale < 0.0f ? -1.0f : 1.0f, scale = fabsf(A.scale) * kLog2e;
 
     // q * 2^qs, its largest below 2^14, as two fp16 parts.
     h8 qh[kG], ql[kG];
     int qs;
     {
-      const float* qp = A.q + static_cast<std::size_t>(s.row + tok) * A.q_stride + head_off;
+      const float* qp = A.q + static_cast<std::size_t>(it.row + own.tok) * A.q_stride + own.off;
       float x[kG][8], top = 0.0f;
 #pragma unroll
       for (int g = 0; g < kG; ++g)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[g][i] = live ? qp[16 * g + 8 * h2nd + i] : 0.0f;
-          top = fmaxf(top, fabsf(x[g][i]));
+        for (int i = 0; i < 8; i += 4) {
+          const f4 y = *reinterpret_cast<const f4*>(qp + 16 * g + 8 * h2nd + i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[g][i + j] = y[j] * q_sign;
+            top = fmaxf(top, fabsf(y[j]));
+          }
         }
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       int e = 0;
@@ -423,23 +565,35 @@ __global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) attention_many(At
     float m = -INFINITY, l = 0.0f, vtop = 0x1p-96f;
 
     const int last_block = (it.hi - 1) / kBlk;
+    // A tile's pieces on their way to LDS; the page ids are read a tile ahead
+    // of the pieces (behind the range: the last block's, whose positions there
+    // are masked).
     uint4 kreg[kPer], vreg[kPer];
     float2 sreg = make_float2(0.0f, 0.0f);
+    int ids[kPer], sid = 0;
+    const auto block_of = [&](int base, int n) {
+      return min(base / kBlk + (n * kThreads + static_cast<int>(threadIdx.x)) / HD, last_block);
+    };
+    const auto lookup = [&](int base) {
+#pragma unroll
+      for (int n = 0; n < kPer; ++n) ids[n] = A.v.table[it.table + page_of(A.g, block_of(base, n))];
+      if (threadIdx.x < 4)
+        sid = A.v.table[it.table + page_of(A.g, min(base / kBlk + static_cast<int>(threadIdx.x), last_block))];
+    };
     const auto fetch = [&](int base) {
 #pragma unroll
       for (int n = 0; n < kPer; ++n) {
         const int c = n * kThreads + threadIdx.x;
         if (kChunks % kThreads != 0 && c >= kChunks) break;
-        const int b = c / HD, at_chunk = c - b * HD;
-        const std::size_t at = block_index(A.g, A.v.table, s, min(base / kBlk + b, last_block), head);
-        kreg[n] = reinterpret_cast<const uint4*>(A.k + at * (16 * HD))[at_chunk];
-        vreg[n] = reinterpret_cast<const uint4*>(A.val + at * (16 * HD))[at_chunk];
+        const int block = block_of(base, n);
+        const std::size_t at = block_at(A.g, ids[n], page_of(A.g, block), block, head) * HD + c % HD;
+        kreg[n] = reinterpret_cast<const uint4*>(A.k)[at];
+        vreg[n] = reinterpret_cast<const uint4*>(A.val)[at];
       }
       if (threadIdx.x < 4) {
-        const int b = base / kBlk + static_cast<int>(threadIdx.x);
-        sreg = make_float2(0.0f, 0.0f);
-        if (b <= last_block)
-          sreg = reinterpret_cast<const float2*>(A.scales)[block_index(A.g, A.v.table, s, b, head)];
+        const int want = base / kBlk + static_cast<int>(threadIdx.x), block = min(want, last_block);
+        sreg = reinterpret_cast<const float2*>(A.scales)[block_at(A.g, sid, page_of(A.g, block), block, head)];
+        if (want > last_block) sreg = make_float2(0.0f, 0.0f);
       }
     };
     const auto stage = [&](int buf) {
@@ -466,13 +620,16 @@ __global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) attention_many(At
       if (threadIdx.x < 4) sh_s[buf][threadIdx.x] = sreg;
     };
 
+    lookup(it.lo);
     fetch(it.lo);
+    if (it.lo + kTile < it.hi) lookup(it.lo + kTile);
     stage(0);
     __syncthreads();
     int buf = 0;
     for (int base = it.lo; base < it.hi; base += kTile, buf ^= 1) {
       const bool more = base + kTile < it.hi;
       if (more) fetch(base + kTile);
+      if (base + 2 * kTile < it.hi) lookup(base + 2 * kTile);
       if (base <= reach) {
         f16v st[2];
 #pragma unroll
@@ -498,22 +655,28 @@ __global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) attention_many(At
           vf[b] = fin ? sc[b].y : 0.0f;
           tile_top = fmaxf(tile_top, vf[b]);
         }
-        float mx = m;
-        const bool edge = base + kTile - 1 > all;
+        if (base + kTile - 1 > all) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (base + 16 * b + 8 * (i / 4) + 4 * h2nd + i % 4 > limit) st[b / 2][8 * (b & 1) + i] = -INFINITY;
+        }
+        // Scores are f[b] times the products; f is positive (where it is 0 the
+        // products are, and 2^-126 of them; a masked -inf stays -inf).
+        float f[4], mx = m;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          const float f = ldexpf(A.scale * kLog2e * sc[b].x, -qs);
+          f[b] = ldexpf(scale * sc[b].x, -qs);
+          if (f[b] == 0.0f) f[b] = 0x1p-126f;
+          float top = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float x = st[b / 2][8 * (b & 1) + i] * f;
-            if (edge && base + 16 * b + 8 * (i / 4) + 4 * h2nd + i % 4 > limit) x = -INFINITY;
-            st[b / 2][8 * (b & 1) + i] = x;
-            mx = fmaxf(mx, x);
-          }
+          for (int i = 0; i < 8; ++i) top = fmaxf(top, st[b / 2][8 * (b & 1) + i]);
+          mx = fmaxf(mx, top == -INFINITY ? top : top * f[b]);
         }
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
         const float ref = mx == -INFINITY ? 0.0f : mx;
-        const float keep = exp2f(m - ref);
+        const float keep = exp2_hw(m - ref);
         const float rescale = keep * (vtop / tile_top);
         m = mx;
         vtop = tile_top;
@@ -530,12 +693,19 @@ __global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) attention_many(At
           const float fw = vf[b] * to_w;
           h8 wh, wl;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float p = exp2f(st[b / 2][8 * (b & 1) + i] - ref);
-            sum += p;
-            const float w = p * fw;
-            wh[i] = static_cast<_Float16>(w);
-            wl[i] = static_cast<_Float16>(w - static_cast<float>(wh[i]));
+          for (int i = 0; i < 8; i += 2) {
+            const float p0 = exp2_hw(fmaf(st[b / 2][8 * (b & 1) + i], f[b], -ref));
+            const float p1 = exp2_hw(fmaf(st[b / 2][8 * (b & 1) + i + 1], f[b], -ref));
+            sum += p0;
+            sum += p1;
+            const float w0 = p0 * fw, w1 = p1 * fw;
+            const h2 hi = {static_cast<_Float16>(w0), static_cast<_Float16>(w1)};
+            const h2 lo = {static_cast<_Float16>(w0 - static_cast<float>(hi[0])),
+                           static_cast<_Float16>(w1 - static_cast<float>(hi[1]))};
+            wh[i] = hi[0];
+            wh[i + 1] = hi[1];
+            wl[i] = lo[0];
+            wl[i + 1] = lo[1];
           }
 #pragma unroll
           for (int d = 0; d < HD / 32; ++d) {
@@ -558,19 +728,17 @@ __global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) attention_many(At
 
     l += __shfl_xor(l, 32, 64);
     const float unit = vtop * ldexpf(1.0f, -kWeightBits);
-    if (live) {
-      float* dst;
-      float f;
-      if (it.part >= 0) {
-        const std::size_t slot =
-            (static_cast<std::size_t>(it.part) * A.g.kv_heads + head * kManySlots) * kFewRows + r;
-        dst = A.parts + slot * HD;
-        f = unit;
-        if (h2nd == 0) *reinterpret_cast<float2*>(A.parts + A.part_states + 2 * slot) = make_float2(m, l);
-      } else {
-        dst = A.out + static_cast<std::size_t>(s.row + tok) * A.out_stride + head_off;
-        f = unit / l;
-      }
+    if (live && it.n > 1) {
+      const std::size_t part = part_row<kManyRows>(A, it.part, head, r);
+      if (h2nd == 0) put2(A.parts + A.part_states + 2 * part, m, l);
+#pragma unroll
+      for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2)
+          put2(A.parts + part * HD + 32 * d + 8 * (i / 4) + 4 * h2nd + i % 4, o[d][i] * unit, o[d][i + 1] * unit);
+    } else if (live) {
+      float* dst = A.out + static_cast<std::size_t>(it.row + own.tok) * A.out_stride + own.off;
+      const float f = unit / l;
 #pragma unroll
       for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
@@ -578,14 +746,28 @@ __global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) attention_many(At
           *reinterpret_cast<f4*>(dst + 32 * d + 8 * i + 4 * h2nd) =
               f4{o[d][4 * i] * f, o[d][4 * i + 1] * f, o[d][4 * i + 2] * f, o[d][4 * i + 3] * f};
     }
+    if (it.n > 1) {
+      if (last_piece(A, it, head, &sh_last)) join_rows<HD, kManyRows, kThreads>(A, it, head);
+      __syncthreads();
+    }
   }
 }
 
 template <int HD>
-void launch_few(const AttnArgs& a, unsigned grid, unsigned sizes, hipStream_t s) {
-  if (sizes & 1) attention_few<HD, 1><<<grid, kThreads, 0, s>>>(a);
-  if (sizes & 2) attention_few<HD, 2><<<grid, kThreads, 0, s>>>(a);
-  if (sizes & 4) attention_few<HD, 4><<<grid, kThreads, 0, s>>>(a);
+void launch(const AttnArgs& a, unsigned few, unsigned many, int rows, hipStream_t s) {
+  if (few > 0) {
+    if (rows <= 4)
+      attention_few<HD, 1><<<few, kFewThreads, 0, s>>>(a);
+    else if (rows <= 8)
+      attention_few<HD, 2><<<few, kFewThreads, 0, s>>>(a);
+    else if constexpr (few_rows(HD) > 8) {
+      if (rows <= 12)
+        attention_few<HD, 3><<<few, kFewThreads, 0, s>>>(a);
+      else
+        attention_few<HD, 4><<<few, kFewThreads, 0, s>>>(a);
+    }
+  }
+  if (many > 0) attention_many<HD><<<many, 256, 0, s>>>(a);
 }
 
 }  // namespace
@@ -593,44 +775,28 @@ void launch_few(const AttnArgs& a, unsigned grid, unsigned sizes, hipStream_t s)
 int launch_attention(const llmi_hip_kv8_plan* p, const llmi_kv8_layer& layer, const float* q, std::size_t q_stride,
                      float scale, float* out, std::size_t out_stride, hipStream_t s, bool captured) {
   const Lists& l = p->lists;
-  AttnArgs a{p->view(), p->g, layer.k, layer.v, layer.scales, q, out, p->parts, q_stride, out_stride,
-             p->max_parts * p->g.kv_heads * kFewRows * p->g.dim, scale,
-             captured ? -1 : static_cast<int>(l.few.size()), captured ? -1 : static_cast<int>(l.many.size()),
-             captured ? -1 : static_cast<int>(l.join.size())};
-  const std::size_t heads = static_cast<std::size_t>(p->g.kv_heads);
-  const auto grid = [](std::size_t units) {
-    return static_cast<unsigned>(std::min<std::size_t>(std::max<std::size_t>(units, 1), 1u << 20));
+  const std::size_t part_rows = p->most.parts * static_cast<std::size_t>(p->g.kv_heads) * kSlotRows;
+  AttnArgs a{p->view(), p->g, layer.k, layer.v, layer.scales, q, out, p->parts, p->joins, q_stride, out_stride,
+             part_rows * static_cast<std::size_t>(p->g.dim), scale, captured ? -1 : static_cast<int>(l.few.size()),
+             captured ? -1 : static_cast<int>(l.many.size())};
+  // Captured: room for any batch that the plan takes, but no more workgroups
+  // than fill the chip several times (each takes further units in turn).
+  const auto grid = [&](std::size_t items, std::size_t most) {
+    const std::size_t units = (captured ? most : items) * static_cast<std::size_t>(p->g.kv_heads);
+    return static_cast<unsigned>(std::min<std::size_t>(units, captured ? 4096 : 1u << 30));
   };
-  unsigned sizes = captured ? 7 : 0;  // which tile counts the batch has
-  for (const FewItem& it : l.few) sizes |= it.rows <= 4 ? 1 : it.rows <= 8 ? 2 : 4;
-  if (sizes != 0) {
-    const unsigned n = grid((captured ? p->max_few : l.few.size()) * heads);
-    switch (p->g.dim) {
-      case 32: launch_few<32>(a, n, sizes, s); break;
-      case 64: launch_few<64>(a, n, sizes, s); break;
-      case 96: launch_few<96>(a, n, sizes, s); break;
-      case 128: launch_few<128>(a, n, sizes, s); break;
-      case 160: launch_few<160>(a, n, sizes, s); break;
-      case 192: launch_few<192>(a, n, sizes, s); break;
-      case 224: launch_few<224>(a, n, sizes, s); break;
-      default: launch_few<256>(a, n, sizes, s); break;
-    }
+  const unsigned few = grid(l.few.size(), p->most.few), many = grid(l.many.size(), p->most.many);
+  const int rows = captured ? few_rows(p->g.dim) : l.few_rows;
+  switch (p->g.dim) {
+    case 32: launch<32>(a, few, many, rows, s); break;
+    case 64: launch<64>(a, few, many, rows, s); break;
+    case 96: launch<96>(a, few, many, rows, s); break;
+    case 128: launch<128>(a, few, many, rows, s); break;
+    case 160: launch<160>(a, few, many, rows, s); break;
+    case 192: launch<192>(a, few, many, rows, s); break;
+    case 224: launch<224>(a, few, many, rows, s); break;
+    default: launch<256>(a, few, many, rows, s); break;
   }
-  if (captured || !l.many.empty()) {
-    const unsigned n = grid((captured ? p->max_many : l.many.size()) * heads);
-    switch (p->g.dim) {
-      case 32: attention_many<32><<<n, kThreads, 0, s>>>(a); break;
-      case 64: attention_many<64><<<n, kThreads, 0, s>>>(a); break;
-      case 96: attention_many<96><<<n, kThreads, 0, s>>>(a); break;
-      case 128: attention_many<128><<<n, kThreads, 0, s>>>(a); break;
-      case 160: attention_many<160><<<n, kThreads, 0, s>>>(a); break;
-      case 192: attention_many<192><<<n, kThreads, 0, s>>>(a); break;
-      case 224: attention_many<224><<<n, kThreads, 0, s>>>(a); break;
-      default: attention_many<256><<<n, kThreads, 0, s>>>(a); break;
-    }
-  }
-  if (captured || !l.join.empty())
-    attention_join<<<grid((captured ? p->max_join : l.join.size()) * heads * kFewRows), kThreads, 0, s>>>(a);
   LLMI_TRY_HIP(hipGetLastError());
   return LLMI_OK;
 }

@@ -31,40 +31,45 @@ struct AppendItem {
 };
 
 // The rows of a sequence for one key/value head are its tokens' query heads
-// of that head: row r is token r / group, head r % group.  `few` work is up to
-// kFewRows rows over positions lo .. hi - 1 (lo a multiple of a tile); part
-// >= 0: one of several over the same rows, its state goes to partial slot
-// `part`; part < 0: the whole history, the rows' output.
-constexpr int kTile = 64, kFewRows = 16;
+// of that head: row r is token r / group, head r % group.  Work of the
+// attention: up to few_rows(head_dim) rows (`few`: single tokens and drafts)
+// or kManyRows rows (`many`: prompts) over positions lo .. hi - 1, lo a
+// multiple of a tile.  n > 1: one of the n pieces of these rows' history; its
+// state goes to partial slots part .., `first` being the first piece's, and
+// the last of the n to end, by the counter `join`, joins them.
+constexpr int kTile = 64;
 constexpr int kFewMax = 64;  // most rows of a sequence and key/value head that go as `few` work
-struct FewItem {
-  std::int32_t seq, row0, rows, lo, hi, part;
+constexpr int kManyRows = 128;
+constexpr int kSlotRows = 8;  // rows of a partial slot
+// 16 rows keep four tiles of accumulators; past 128 dims they are too many registers.
+constexpr int few_rows(int dim) { return dim <= 128 ? 16 : 8; }
+struct AttnItem {
+  std::int32_t row, start, table;  // the sequence's, as in Seq
+  std::int32_t row0, rows, lo, hi, part, first, n, join;
 };
-// `many` work: up to kManyRows rows over positions lo .. hi - 1 in the same
-// way; a partial state takes kManySlots slots.
-constexpr int kManyRows = 128, kManySlots = kManyRows / kFewRows;
-struct ManyItem {
-  std::int32_t seq, row0, rows, lo, hi, part;
+// A history is split so that a batch makes about this many units of work
+// (item and key/value head), in pieces of at least the second number.
+constexpr std::size_t kFewTarget = 1024, kFewLeast = 8 * kTile;
+constexpr std::size_t kManyTarget = 1024, kManyLeast = 2 * kTile;
+
+// block / d for block < 2^27 (positions below 2^31) and d = the blocks of a
+// page, at most 4096: (block * m) >> k with m = 2^k / d + 1, k = 27 + ceil(log2 d):
+// m * d exceeds 2^k by at most d <= 2^(k - 27), so the product's excess over
+// block / d stays below 1 / d.
+struct Divisor {
+  std::uint32_t m;
+  std::int32_t k;
 };
-// Up to 16 rows whose states are in the slots part + c * step, c < n, from
-// row `off` of each head's 16 * step rows on.
-struct JoinItem {
-  std::int32_t seq, row0, rows, part, n, step, off;
-};
-// Positions per split are chosen so that a batch makes about this many units
-// of work (item and key/value head); a split is at least kMinSplit positions.
-constexpr std::size_t kFewTarget = 2048;
-constexpr std::size_t kMinSplit = 4 * kTile;
-constexpr std::size_t kManyTarget = 512, kManyMinSplit = 8 * kTile;
-// Most partial slots of any batch: every split but a sequence's last one is
-// full, so there are at most kFewTarget / kv_heads full ones, and one more
-// for each of the row groups that are split.
+constexpr Divisor divisor(std::uint32_t d) {
+  int log = 0;
+  while ((1u << log) < d) ++log;
+  return {static_cast<std::uint32_t>((std::uint64_t{1} << (27 + log)) / d + 1), 27 + log};
+}
 
 struct Lists {
-  std::vector<FewItem> few;
-  std::vector<ManyItem> many;
-  std::vector<JoinItem> join;
-  std::size_t parts = 0;
+  std::vector<AttnItem> few, many;
+  std::int32_t few_rows = 0;  // most rows of a `few` item
+  std::size_t parts = 0, joins = 0;  // partial slots and join counters of a key/value head
   std::vector<Seq> seqs;
   std::vector<std::int32_t> table;
   std::vector<AppendItem> append;  // every block that holds a new token
@@ -90,6 +95,21 @@ inline std::string check_shape(const llmi_kv8_shape* s) {
 inline bool same_shape(const llmi_kv8_shape& a, const llmi_kv8_shape& b) {
   return a.heads == b.heads && a.kv_heads == b.kv_heads && a.head_dim == b.head_dim &&
          a.page_tokens == b.page_tokens && a.pages == b.pages && a.slots == b.slots;
+}
+
+// The most that a batch of at most `seqs` sequences and `tokens` tokens makes.
+// A kind's positions x heads over its split size are at most its target, so
+// are its full pieces x heads; rows that are split have at most twice their
+// full pieces; every group of rows adds one item at most.
+struct Limits {
+  std::size_t append, few, many, parts, joins;
+};
+inline Limits limits(const llmi_kv8_shape& sh, std::size_t seqs, std::size_t tokens) {
+  const std::size_t few = kFewTarget / sh.kv_heads, many = kManyTarget / sh.kv_heads;
+  const std::size_t busy = std::min(seqs, tokens), group = sh.heads / sh.kv_heads;
+  const std::size_t rows = static_cast<std::size_t>(few_rows(static_cast<int>(sh.head_dim)));
+  return {tokens / kBlk + 2 * busy, few + kFewMax / rows * busy, many + tokens * group / kManyRows + busy,
+          2 * few * (rows / kSlotRows) + 2 * many * (kManyRows / kSlotRows), few + many};
 }
 
 // Checks a batch and builds its lists; returns the reason of a refusal.
@@ -170,38 +190,45 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
   };
   // Over all groups of rows of one kind: fn(sequence, first row, rows, positions seen).
   const auto each = [&](bool few, auto&& fn) {
-    const std::size_t most = few ? kFewRows : kManyRows;
+    const std::size_t most = few ? static_cast<std::size_t>(few_rows(static_cast<int>(sh.head_dim))) : kManyRows;
     for (std::size_t i = 0; i < seqs; ++i) {
       const std::size_t rows = rows_of(l.seqs[i]);
       if (rows == 0 || (rows <= kFewMax) != few) continue;
-      for (std::size_t r = 0; r < rows; r += most) {
-        const std::size_t n = std::min(most, rows - r);
-        fn(static_cast<std::int32_t>(i), r, n, seen(l.seqs[i], r, n));
+      // Rows of several groups are shared out evenly, in tiles of 4 rows.
+      const std::size_t groups = (rows + most - 1) / most;
+      const std::size_t even = few ? (rows + 4 * groups - 1) / (4 * groups) * 4 : most;
+      for (std::size_t r = 0; r < rows;) {
+        const std::size_t n = std::min(even, rows - r);
+        fn(i, r, n, seen(l.seqs[i], r, n));
+        r += n;
       }
     }
   };
   const auto split_of = [&](bool few, std::size_t target, std::size_t least) {
     std::size_t reach = 0;
-    each(few, [&](std::int32_t, std::size_t, std::size_t, std::size_t len) { reach += len * sh.kv_heads; });
+    each(few, [&](std::size_t, std::size_t, std::size_t, std::size_t len) { reach += len * sh.kv_heads; });
     return std::max(least, (reach / target + least - 1) / least * least);
   };
-  const auto lay = [&](bool few, std::size_t split, auto& items) {
-    const std::size_t slots = few ? 1 : kManySlots;
-    each(few, [&](std::int32_t seq, std::size_t r, std::size_t rows, std::size_t len) {
+  const auto lay = [&](bool few, std::size_t split, std::vector<AttnItem>& items) {
+    each(few, [&](std::size_t seq, std::size_t r, std::size_t rows, std::size_t len) {
       const std::size_t n = (len + split - 1) / split;
+      const std::size_t slots = few ? few_rows(static_cast<int>(sh.head_dim)) / kSlotRows : kManyRows / kSlotRows;
       const auto i32 = [](std::size_t x) { return static_cast<std::int32_t>(x); };
       for (std::size_t c = 0; c < n; ++c)
-        items.push_back({seq, i32(r), i32(rows), i32(c * split), i32(std::min(len, (c + 1) * split)),
-                         n > 1 ? i32(l.parts + c * slots) : -1});
+        items.push_back({l.seqs[seq].row, l.seqs[seq].start, l.seqs[seq].table, i32(r), i32(rows), i32(c * split), i32(std::min(len, (c + 1) * split)),
+                         i32(l.parts + c * slots), i32(l.parts), i32(n), i32(l.joins)});
       if (n == 1) return;
-      for (std::size_t o = 0; o < rows; o += kFewRows)
-        l.join.push_back({seq, i32(r + o), i32(std::min<std::size_t>(kFewRows, rows - o)), i32(l.parts), i32(n),
-                          i32(slots), i32(o)});
       l.parts += n * slots;
+      l.joins += 1;
     });
   };
-  lay(true, split_of(true, kFewTarget, kMinSplit), l.few);
-  lay(false, split_of(false, kManyTarget, kManyMinSplit), l.many);
+  lay(true, split_of(true, kFewTarget, kFewLeast), l.few);
+  lay(false, split_of(false, kManyTarget, kManyLeast), l.many);
+  // The longest first, so that the last to start are short.
+  const auto longer = [](const AttnItem& a, const AttnItem& b) { return a.hi - a.lo > b.hi - b.lo; };
+  std::stable_sort(l.few.begin(), l.few.end(), longer);
+  std::stable_sort(l.many.begin(), l.many.end(), longer);
+  for (const AttnItem& it : l.few) l.few_rows = std::max(l.few_rows, it.rows);
   return {};
 }
 

@@ -80,41 +80,43 @@ int main() {
     std::vector<std::vector<long>> reach(l.seqs.size());
     for (std::size_t i = 0; i < l.seqs.size(); ++i) reach[i].assign(static_cast<std::size_t>(l.seqs[i].count) * group, 0);
     std::vector<int> slot(l.parts, 0);
-    const auto walk = [&](const auto& items, int most, int slots, bool few) {
-      for (const auto& it : items) {
+    const int few_most = few_rows(static_cast<int>(sh.head_dim));
+    std::vector<int> pieces(l.joins, 0);
+    const auto walk = [&](const std::vector<AttnItem>& items, int most, bool few) {
+      for (const AttnItem& it : items) {
         CHECK(it.rows > 0 && it.rows <= most && it.lo % kTile == 0 && it.lo < it.hi);
-        const Seq& s = l.seqs[static_cast<std::size_t>(it.seq)];
+        std::size_t of = 0;  // the sequence with these tokens
+        while (l.seqs[of].count == 0 || l.seqs[of].row != it.row) ++of;
+        const Seq& s = l.seqs[of];
+        CHECK(it.start == s.start && it.table == s.table);
         const std::size_t rows = static_cast<std::size_t>(s.count) * group;
         CHECK((rows <= kFewMax) == few && static_cast<std::size_t>(it.row0 + it.rows) <= rows);
         CHECK(it.hi <= s.start + s.count);
         for (int r = it.row0; r < it.row0 + it.rows; ++r) {
           const int own = s.start + r / static_cast<int>(group);  // the row's position
-          reach[static_cast<std::size_t>(it.seq)][static_cast<std::size_t>(r)] += std::max(0, std::min(it.hi, own + 1) - it.lo);
+          reach[of][static_cast<std::size_t>(r)] += std::max(0, std::min(it.hi, own + 1) - it.lo);
         }
-        if (it.part >= 0)
-          for (int k = 0; k < slots; ++k) CHECK(++slot.at(static_cast<std::size_t>(it.part + k)) == 1);
+        if (it.n == 1) continue;
+        CHECK((it.part - it.first) % (most / kSlotRows) == 0 && (it.part - it.first) / (most / kSlotRows) < it.n);
+        CHECK(++pieces.at(static_cast<std::size_t>(it.join)) <= it.n);
+        for (int k = 0; k < most / kSlotRows; ++k) CHECK(++slot.at(static_cast<std::size_t>(it.part + k)) == 1);
       }
+      for (const AttnItem& it : items) CHECK(it.n == 1 || pieces[static_cast<std::size_t>(it.join)] == it.n);
       return 0;
     };
-    CHECK(walk(l.few, kFewRows, 1, true) == 0 && walk(l.many, kManyRows, kManySlots, false) == 0);
+    CHECK(walk(l.few, few_most, true) == 0 && walk(l.many, kManyRows, false) == 0);
     for (std::size_t i = 0; i < l.seqs.size(); ++i)
       for (std::size_t r = 0; r < reach[i].size(); ++r) CHECK(reach[i][r] == l.seqs[i].start + static_cast<long>(r / group) + 1);
     for (const int n_of : slot) CHECK(n_of == 1);
-    std::set<std::pair<int, int>> joined;
-    for (const JoinItem& j : l.join) {
-      CHECK(j.n > 1 && j.rows > 0 && j.rows <= kFewRows && j.off >= 0 && j.off + j.rows <= kFewRows * j.step);
-      CHECK(j.part >= 0 && static_cast<std::size_t>(j.part + j.n * j.step) <= l.parts);
-      for (int r = 0; r < j.rows; ++r) CHECK(joined.insert({j.seq, j.row0 + r}).second);
-    }
-    for (const auto* items : {&l.few}) for (const auto& it : *items) CHECK((it.part >= 0) == (joined.count({it.seq, it.row0}) > 0));
-    for (const auto& it : l.many) CHECK((it.part >= 0) == (joined.count({it.seq, it.row0}) > 0));
-    const std::size_t few_splits = kFewTarget / sh.kv_heads, many_splits = kManyTarget / sh.kv_heads;
-    const std::size_t busy = std::min<std::size_t>(static_cast<std::size_t>(n), tokens);
-    CHECK(l.few.size() <= few_splits + (kFewMax / kFewRows) * busy);
-    CHECK(l.many.size() <= many_splits + tokens * group / kManyRows + busy);
-    CHECK(l.join.size() <= few_splits + kManySlots * many_splits);
-    CHECK(l.parts <= 2 * few_splits + 2 * kManySlots * many_splits);
-    CHECK(l.append.size() <= tokens / kBlk + 2 * std::min<std::size_t>(static_cast<std::size_t>(n), tokens));
+    const Limits m = limits(sh, static_cast<std::size_t>(n), tokens);
+    CHECK(l.append.size() <= m.append && l.few.size() <= m.few && l.many.size() <= m.many);
+    CHECK(l.parts <= m.parts && l.joins <= m.joins);
+  }
+  for (std::uint32_t d = 1; d <= 4096; ++d) {
+    const Divisor v = divisor(d);
+    for (std::uint32_t q = 0; q < 40; ++q)
+      for (std::uint32_t x : {q * d, q * d + d - 1, (1u << 27) - 1 - q, ((1u << 27) - 1) / d * d - (q < 1 ? 0 : q * d), static_cast<std::uint32_t>(rng()) >> 5})
+        CHECK(x >= (1u << 27) || (std::uint64_t{x} * v.m) >> v.k == x / d);
   }
   std::puts("ok");
   return 0;
