@@ -149,8 +149,10 @@ template <int HD, int MOST, int THREADS>
 __device__ void join_rows(const AttnArgs& A, const AttnItem& it, int head) {
   constexpr int kQuads = HD / 4, kAt = 8, kStep = MOST / kSlotRows;
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  int first = threadIdx.x;
+  asm volatile("" : "+v"(first));  // keeps this function's indexes out of the caller's loop: registers
   const int cells = it.rows * kQuads;
-  for (int base = threadIdx.x; base < cells; base += kAt * THREADS) {
+  for (int base = first; base < cells; base += kAt * THREADS) {
     float m[kAt], l[kAt];
     float4 o[kAt];
 #pragma unroll
@@ -479,7 +481,14 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
-constexpr int kWeightBits = 14;
+constexpr int kWeightBits = 8;  // with kSlack: weights stay below 2^14
+constexpr float kSlack = 6.0f;
+
+// x of the lane 32 on (or back).
+__device__ __forceinline__ float other_half(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float((threadIdx.x & 32) != 0 ? r[0] : r[1]);
+}
 
 // The four signed bytes of w as fp16, exact: 1024 + (byte + 128) is an fp16
 // whose low byte is the code plus 128.
@@ -492,23 +501,27 @@ __device__ __forceinline__ void halves(std::uint32_t w, std::uint32_t* out) {
   out[1] = __builtin_bit_cast(std::uint32_t, static_cast<h2>(b - bias));
 }
 
+constexpr int kAhead = 4;
+
 template <int HD>
 __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArgs A) {
   constexpr int kThreads = 256;
   constexpr int kG = HD / 16;
-  constexpr int kChunks = 4 * HD;  // 16-byte pieces of a tile's keys (and of its values)
-  constexpr int kPer = (kChunks + kThreads - 1) / kThreads;
+  constexpr int kPer = (HD + 63) / 64;  // 16-byte pieces a lane has of a block's keys (and of its values)
   __shared__ uint4 sh_k[2][kG][2][kTile];     // [16-dim group][half of it][position]: 8 fp16
   __shared__ uint4 sh_v[2][kTile / 16][2][HD];  // [block][h][dim]: positions 4h.., 8 + 4h..
-  __shared__ float2 sh_s[2][4];
+  __shared__ float4 sh_s[2][4];               // a tile's blocks: see block_terms
   __shared__ int sh_last;
-  const int lane = threadIdx.x & 63, col = lane & 31, h2nd = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nmany = A.nmany >= 0 ? A.nmany : A.v.counts->many;
   const int units = nmany * A.g.kv_heads;
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     const int item = u / A.g.kv_heads, head = u - item * A.g.kv_heads;
     const AttnItem it = A.v.many[item];
+    // (Opaque: what is computed from it is not kept in registers around the loop over units.)
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int col = lane & 31, h2nd = lane >> 5;
     const int r = wave * 32 + col;
     const bool live = r < it.rows;
     const Row own = row_of(A, it, head, live ? r : 0);
@@ -547,14 +560,10 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
           ql[g][i] = static_cast<_Float16>(y - static_cast<float>(qh[g][i]));
         }
     }
-    // The wavefront's rows see at most up to `reach`, and all of them up to `all`.
-    int reach = limit, all = live ? limit : 0x7FFFFFFF;
+    // All of the wavefront's rows see positions up to `all`.
+    int all = live ? limit : 0x7FFFFFFF;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      reach = max(reach, __shfl_xor(reach, o, 64));
-      all = min(all, __shfl_xor(all, o, 64));
-    }
-    reach = __builtin_amdgcn_readfirstlane(reach);
+    for (int o = 1; o < 32; o <<= 1) all = min(all, __shfl_xor(all, o, 64));
     all = __builtin_amdgcn_readfirstlane(all);
 
     f16v o[HD / 32];
@@ -562,188 +571,246 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
     for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f, vtop = 0x1p-96f;
+    // m: what scores are taken against, at most kSlack below the largest so
+    // far; vtop: log2 of the largest value scale so far (below all to begin).
+    float m = -INFINITY, l = 0.0f, vtop = -200.0f;
 
     const int last_block = (it.hi - 1) / kBlk;
-    // A tile's pieces on their way to LDS; the page ids are read a tile ahead
-    // of the pieces (behind the range: the last block's, whose positions there
-    // are masked).
+    // A wavefront brings one of the tile's four blocks; its page id is read a
+    // tile ahead of it (behind the range: the last block again, whose
+    // positions there are masked).
     uint4 kreg[kPer], vreg[kPer];
     float2 sreg = make_float2(0.0f, 0.0f);
-    int ids[kPer], sid = 0;
-    const auto block_of = [&](int base, int n) {
-      return min(base / kBlk + (n * kThreads + static_cast<int>(threadIdx.x)) / HD, last_block);
-    };
-    const auto lookup = [&](int base) {
-#pragma unroll
-      for (int n = 0; n < kPer; ++n) ids[n] = A.v.table[it.table + page_of(A.g, block_of(base, n))];
-      if (threadIdx.x < 4)
-        sid = A.v.table[it.table + page_of(A.g, min(base / kBlk + static_cast<int>(threadIdx.x), last_block))];
-    };
+    bool sreg_live = true;
+    int id = 0;
+    const auto lookup = [&](int base) { id = A.v.table[it.table + page_of(A.g, min(base / kBlk + wave, last_block))]; };
     const auto fetch = [&](int base) {
+      const int want = base / kBlk + wave, block = min(want, last_block);
+      const std::size_t at = block_at(A.g, id, page_of(A.g, block), block, head);
+      const auto* kp = reinterpret_cast<const uint4*>(A.k + at * (16 * HD));
+      const auto* vp = reinterpret_cast<const uint4*>(A.val + at * (16 * HD));
 #pragma unroll
       for (int n = 0; n < kPer; ++n) {
-        const int c = n * kThreads + threadIdx.x;
-        if (kChunks % kThreads != 0 && c >= kChunks) break;
-        const int block = block_of(base, n);
-        const std::size_t at = block_at(A.g, ids[n], page_of(A.g, block), block, head) * HD + c % HD;
-        kreg[n] = reinterpret_cast<const uint4*>(A.k)[at];
-        vreg[n] = reinterpret_cast<const uint4*>(A.val)[at];
+        const int c = min(n * 64 + lane, HD - 1);
+        kreg[n] = kp[c];
+        vreg[n] = vp[c];
       }
-      if (threadIdx.x < 4) {
-        const int want = base / kBlk + static_cast<int>(threadIdx.x), block = min(want, last_block);
-        sreg = reinterpret_cast<const float2*>(A.scales)[block_at(A.g, sid, page_of(A.g, block), block, head)];
-        if (want > last_block) sreg = make_float2(0.0f, 0.0f);
-      }
+      sreg = reinterpret_cast<const float2*>(A.scales)[at];
+      sreg_live = want <= last_block;
     };
-    const auto stage = [&](int buf) {
+    // What the products take of the block that `fetch` brought: the key scale
+    // times the softmax's, log2 of the value scale (-inf: its codes are 0, or
+    // masked), and NaN if a scale is not finite.
+    const auto block_terms = [&]() {
+      const bool fin = sreg.y > 0.0f && sreg.y < INFINITY;
+      const float lg = __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(sreg.y)) +
+                       static_cast<float>(__builtin_amdgcn_frexp_expf(sreg.y));
+      return sreg_live ? make_float4(scale * sreg.x, fin ? lg : -INFINITY, fmaf(sreg.x, 0.0f, sreg.y * 0.0f), 0.0f)
+                       : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+    };
+    // Staging in kPieces steps, each four codes of every lane to fp16; every
+    // second one stores eight of them: dims 0-7 or 8-15 of a position's keys,
+    // positions 0-3, 8-11 or 4-7, 12-15 of a dim's values.
+    constexpr int kPieces = 8 * kPer;
+    std::uint32_t half[4];
+    const auto stage_step = [&](int to, int q) {
+      const int n = q / 8, j = q % 4, side = j / 2;
+      const bool keys = q % 8 < 4;
+      const uint4 u = keys ? kreg[n] : vreg[n];
+      const int from = keys ? j : (j % 2) * 2 + side;  // which four of the sixteen
+      halves(from == 0 ? u.x : from == 1 ? u.y : from == 2 ? u.z : u.w, half + 2 * (j % 2));
+      if (j % 2 == 0) return;
+      const int c = n * 64 + lane;
+      if (HD % 64 != 0 && c >= HD) return;
+      const uint4 out = make_uint4(half[0], half[1], half[2], half[3]);
+      if (keys)
+        sh_k[to][c / 16][side][16 * wave + c % 16] = out;
+      else
+        sh_v[to][wave][side][c] = out;
+    };
+    const auto stage = [&](int to) {
 #pragma unroll
-      for (int n = 0; n < kPer; ++n) {
-        const int c = n * kThreads + threadIdx.x;
-        if (kChunks % kThreads != 0 && c >= kChunks) break;
-        const int b = c / HD, at_chunk = c - b * HD;
-        std::uint32_t x[8];
-        halves(kreg[n].x, x);
-        halves(kreg[n].y, x + 2);
-        halves(kreg[n].z, x + 4);
-        halves(kreg[n].w, x + 6);
-        const int g = at_chunk / 16, p = b * 16 + at_chunk % 16;
-        sh_k[buf][g][0][p] = make_uint4(x[0], x[1], x[2], x[3]);
-        sh_k[buf][g][1][p] = make_uint4(x[4], x[5], x[6], x[7]);
-        halves(vreg[n].x, x);
-        halves(vreg[n].y, x + 2);
-        halves(vreg[n].z, x + 4);
-        halves(vreg[n].w, x + 6);
-        sh_v[buf][b][0][at_chunk] = make_uint4(x[0], x[1], x[4], x[5]);
-        sh_v[buf][b][1][at_chunk] = make_uint4(x[2], x[3], x[6], x[7]);
-      }
-      if (threadIdx.x < 4) sh_s[buf][threadIdx.x] = sreg;
+      for (int q = 0; q < kPieces; ++q) stage_step(to, q);
+      if (lane == 0) sh_s[to][wave] = block_terms();
     };
 
     lookup(it.lo);
     fetch(it.lo);
-    if (it.lo + kTile < it.hi) lookup(it.lo + kTile);
     stage(0);
+    if (it.lo + kTile < it.hi) {
+      lookup(it.lo + kTile);
+      fetch(it.lo + kTile);
+    }
+    if (it.lo + 2 * kTile < it.hi) lookup(it.lo + 2 * kTile);
     __syncthreads();
     int buf = 0;
+    // Per tile: the score products, with the next tile's staging between
+    // them; the tile after that fetched; the weights; the output products,
+    // with the next block's weights between them.  The order is fixed by
+    // scheduling barriers: kAhead operands are on their way from LDS while
+    // the products of earlier ones run.
     for (int base = it.lo; base < it.hi; base += kTile, buf ^= 1) {
-      const bool more = base + kTile < it.hi;
-      if (more) fetch(base + kTile);
-      if (base + 2 * kTile < it.hi) lookup(base + 2 * kTile);
-      if (base <= reach) {
-        f16v st[2];
+      f16v st[2];
+      float4 term[4];
+      const f16v zero = {};
+
+      h8 kf[kAhead];
+      const auto key = [&](int n) { return __builtin_bit_cast(h8, sh_k[buf][n / 2][h2nd][32 * (n & 1) + col]); };
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+      for (int n = 0; n < kAhead; ++n) kf[n] = key(n);
+      constexpr int kSteps = 2 * kG, kEach = (kPieces + kSteps - 1) / kSteps;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) st[t][i] = 0.0f;
+      for (int n = 0; n < kSteps; ++n) {
+        __builtin_amdgcn_sched_barrier(0);
+        f16v& s = st[n & 1];
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n % kAhead], qh[n / 2], n < 2 ? zero : s, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        // (Behind the last tile the pieces are the one before's, and go to the buffer that is free.)
 #pragma unroll
-          for (int g = 0; g < kG; ++g) {
-            const h8 a = __builtin_bit_cast(h8, sh_k[buf][g][h2nd][32 * t + col]);
-            st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[g], st[t], 0, 0, 0);
-            st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[g], st[t], 0, 0, 0);
-          }
+        for (int q = n * kEach; q < (n + 1) * kEach && q < kPieces; ++q) stage_step(buf ^ 1, q);
+        if (n == kSteps - 2) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) term[b] = sh_s[buf][b];
         }
-        // Scores in base-2 units; positions behind a row's own leave nothing.
-        float2 sc[4];
-        float vf[4], tile_top = vtop;
-        bool whole = true;  // every value scale of the tile is finite
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          sc[b] = sh_s[buf][b];
-          const bool fin = sc[b].y < INFINITY;
-          whole = whole && fin;
-          vf[b] = fin ? sc[b].y : 0.0f;
-          tile_top = fmaxf(tile_top, vf[b]);
-        }
-        if (base + kTile - 1 > all) {
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (base + 16 * b + 8 * (i / 4) + 4 * h2nd + i % 4 > limit) st[b / 2][8 * (b & 1) + i] = -INFINITY;
-        }
-        // Scores are f[b] times the products; f is positive (where it is 0 the
-        // products are, and 2^-126 of them; a masked -inf stays -inf).
-        float f[4], mx = m;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          f[b] = ldexpf(scale * sc[b].x, -qs);
-          if (f[b] == 0.0f) f[b] = 0x1p-126f;
-          float top = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) top = fmaxf(top, st[b / 2][8 * (b & 1) + i]);
-          mx = fmaxf(mx, top == -INFINITY ? top : top * f[b]);
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float ref = mx == -INFINITY ? 0.0f : mx;
-        const float keep = exp2_hw(m - ref);
-        const float rescale = keep * (vtop / tile_top);
-        m = mx;
-        vtop = tile_top;
-        if (__any(rescale != 1.0f)) {
-#pragma unroll
-          for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] *= rescale;
-        }
-        const float to_w = ldexpf(1.0f, kWeightBits) / tile_top;
-        float sum = 0.0f;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const float fw = vf[b] * to_w;
-          h8 wh, wl;
-#pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            const float p0 = exp2_hw(fmaf(st[b / 2][8 * (b & 1) + i], f[b], -ref));
-            const float p1 = exp2_hw(fmaf(st[b / 2][8 * (b & 1) + i + 1], f[b], -ref));
-            sum += p0;
-            sum += p1;
-            const float w0 = p0 * fw, w1 = p1 * fw;
-            const h2 hi = {static_cast<_Float16>(w0), static_cast<_Float16>(w1)};
-            const h2 lo = {static_cast<_Float16>(w0 - static_cast<float>(hi[0])),
-                           static_cast<_Float16>(w1 - static_cast<float>(hi[1]))};
-            wh[i] = hi[0];
-            wh[i + 1] = hi[1];
-            wl[i] = lo[0];
-            wl[i + 1] = lo[1];
-          }
-#pragma unroll
-          for (int d = 0; d < HD / 32; ++d) {
-            const h8 a = __builtin_bit_cast(h8, sh_v[buf][b][h2nd][32 * d + col]);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wh, o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wl, o[d], 0, 0, 0);
-          }
-        }
-        if (!whole) {
-          // A value scale that is inf or NaN shows in the rows that see a position of its block.
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-            if (base + 16 * b <= limit) sum = fmaf(sc[b].y, 0.0f, sum);
-        }
-        l = fmaf(l, keep, sum);
+        __builtin_amdgcn_sched_barrier(0);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n % kAhead], ql[n / 2], s, 0, 0, 0);
+        if (n + kAhead < kSteps) kf[n % kAhead] = key(n + kAhead);
       }
-      if (more) stage(buf ^ 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if (lane == 0) sh_s[buf ^ 1][wave] = block_terms();
+      if (base + 2 * kTile < it.hi) fetch(base + 2 * kTile);
+      if (base + 3 * kTile < it.hi) lookup(base + 3 * kTile);
+      // Per block: scores are f times the products (f is positive: where
+      // the scale is 0 the products are, and a masked -inf stays -inf);
+      // weights carry 2^ratio, the value scale over the largest.  A scale
+      // below 2^-60 of the largest counts as that; one of 0 has codes of 0.
+      float f[4], ratio[4], bad = 0.0f, tile_top = vtop;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        tile_top = fmaxf(tile_top, term[b].y);
+        f[b] = fmaxf(ldexpf(term[b].x, -qs), 0x1p-126f);
+        bad += term[b].z;
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) ratio[b] = term[b].y == -INFINITY ? 0.0f : fmaxf(term[b].y - tile_top, -60.0f);
+      // Positions behind a row's own leave nothing.
+      if (base + kTile - 1 > all) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (base + 16 * b + 8 * (i / 4) + 4 * h2nd + i % 4 > limit) st[b / 2][8 * (b & 1) + i] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, st[b / 2][8 * (b & 1) + i]);
+        mx = fmaxf(mx, top * f[b]);
+      }
+      mx = fmaxf(mx, other_half(mx));
+      // The sums are rescaled where the largest score has grown by more
+      // than kSlack (weights may be up to 2^kSlack before that), or a value scale.
+      const bool grown = mx > m + kSlack;
+      if (__any(grown) || tile_top > vtop) {
+        const float now = grown ? mx : m, keep = now == -INFINITY ? 0.0f : exp2_hw(m - now);
+        const float rescale = keep * exp2_hw(vtop - tile_top);
+        m = now;
+        vtop = tile_top;
+        l *= keep;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[d][i] *= rescale;
+      }
+      const float ref = static_cast<float>(kWeightBits) - (m == -INFINITY ? 0.0f : m);
+      float off[4], part[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        off[b] = ratio[b] + ref;
+        part[b] = 0.0f;
+      }
+      // Weights i and i + 1 of block b, in their two fp16 parts.
+      std::uint32_t wh[2][4], wl[2][4];
+      const auto weigh = [&](int b, int i) {
+        const float w0 = exp2_hw(fmaf(st[b / 2][8 * (b & 1) + i], f[b], off[b]));
+        const float w1 = exp2_hw(fmaf(st[b / 2][8 * (b & 1) + i + 1], f[b], off[b]));
+        part[b] += w0;
+        part[b] += w1;
+        const h2 hi = {static_cast<_Float16>(w0), static_cast<_Float16>(w1)};
+        const std::uint32_t hi_bits = __builtin_bit_cast(std::uint32_t, hi);
+        std::uint32_t lo;  // fp16(w - hi), each half in one instruction
+        asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(lo) : "v"(hi_bits), "v"(w0));
+        asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(lo) : "v"(hi_bits), "v"(w1));
+        wh[b & 1][i / 2] = hi_bits;
+        wl[b & 1][i / 2] = lo;
+      };
+      const auto both = [&](const std::uint32_t (&w)[4]) {
+        return __builtin_bit_cast(h8, make_uint4(w[0], w[1], w[2], w[3]));
+      };
+      constexpr int kD = HD / 32;
+      h8 vfr[kAhead];
+      const auto value = [&](int n) { return __builtin_bit_cast(h8, sh_v[buf][n / kD][h2nd][32 * (n % kD) + col]); };
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) vfr[n] = value(n);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) weigh(0, i);
+#pragma unroll
+      for (int n = 0; n < 4 * kD; ++n) {
+        __builtin_amdgcn_sched_barrier(0);
+        const int b = n / kD, d = n % kD;
+        // Pairs of the next block's weights that this step computes.
+        const int i0 = d * 4 / kD, i1 = (d + 1) * 4 / kD;
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vfr[n % kAhead], both(wh[b & 1]), o[d], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = i0; i < (i0 + i1 + 1) / 2; ++i)
+          if (b < 3) weigh(b + 1, 2 * i);
+        __builtin_amdgcn_sched_barrier(0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vfr[n % kAhead], both(wl[b & 1]), o[d], 0, 0, 0);
+        if (n + kAhead < 4 * kD) vfr[n % kAhead] = value(n + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = (i0 + i1 + 1) / 2; i < i1; ++i)
+          if (b < 3) weigh(b + 1, 2 * i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      float sum = 0.0f;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) sum = fmaf(part[b], exp2_hw(-static_cast<float>(kWeightBits) - ratio[b]), sum);
+      if (bad != bad) {
+        // A scale that is inf or NaN shows in the rows that see a position of its block.
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (base + 16 * b <= limit) sum += sh_s[buf][b].z;
+      }
+      l += sum;
       __syncthreads();
     }
 
     l += __shfl_xor(l, 32, 64);
-    const float unit = vtop * ldexpf(1.0f, -kWeightBits);
+    const float unit = exp2_hw(vtop) * ldexpf(1.0f, -kWeightBits);
+    int end_lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(end_lane));
+    const int end_h = end_lane >> 5, end_r = wave * 32 + (end_lane & 31);
+    const Row mine = row_of(A, it, head, live ? end_r : 0);
     if (live && it.n > 1) {
-      const std::size_t part = part_row<kManyRows>(A, it.part, head, r);
-      if (h2nd == 0) put2(A.parts + A.part_states + 2 * part, m, l);
+      const std::size_t part = part_row<kManyRows>(A, it.part, head, end_r);
+      if (end_h == 0) put2(A.parts + A.part_states + 2 * part, m, l);
 #pragma unroll
       for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; i += 2)
-          put2(A.parts + part * HD + 32 * d + 8 * (i / 4) + 4 * h2nd + i % 4, o[d][i] * unit, o[d][i + 1] * unit);
+          put2(A.parts + part * HD + 32 * d + 8 * (i / 4) + 4 * end_h + i % 4, o[d][i] * unit, o[d][i + 1] * unit);
     } else if (live) {
-      float* dst = A.out + static_cast<std::size_t>(it.row + own.tok) * A.out_stride + own.off;
+      float* dst = A.out + static_cast<std::size_t>(it.row + mine.tok) * A.out_stride + mine.off;
       const float f = unit / l;
 #pragma unroll
       for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<f4*>(dst + 32 * d + 8 * i + 4 * h2nd) =
+          *reinterpret_cast<f4*>(dst + 32 * d + 8 * i + 4 * end_h) =
               f4{o[d][4 * i] * f, o[d][4 * i + 1] * f, o[d][4 * i + 2] * f, o[d][4 * i + 3] * f};
     }
     if (it.n > 1) {

@@ -211,11 +211,13 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
   };
   const auto lay = [&](bool few, std::size_t split, std::vector<AttnItem>& items) {
     each(few, [&](std::size_t seq, std::size_t r, std::size_t rows, std::size_t len) {
-      const std::size_t n = (len + split - 1) / split;
+      // Pieces of one size, in whole units (of a tile for each of its wavefronts, if few).
+      const std::size_t unit = few ? kFewLeast : kTile, most = (len + split - 1) / split;
+      const std::size_t piece = ((len + most - 1) / most + unit - 1) / unit * unit, n = (len + piece - 1) / piece;
       const std::size_t slots = few ? few_rows(static_cast<int>(sh.head_dim)) / kSlotRows : kManyRows / kSlotRows;
       const auto i32 = [](std::size_t x) { return static_cast<std::int32_t>(x); };
       for (std::size_t c = 0; c < n; ++c)
-        items.push_back({l.seqs[seq].row, l.seqs[seq].start, l.seqs[seq].table, i32(r), i32(rows), i32(c * split), i32(std::min(len, (c + 1) * split)),
+        items.push_back({l.seqs[seq].row, l.seqs[seq].start, l.seqs[seq].table, i32(r), i32(rows), i32(c * piece), i32(std::min(len, (c + 1) * piece)),
                          i32(l.parts + c * slots), i32(l.parts), i32(n), i32(l.joins)});
       if (n == 1) return;
       l.parts += n * slots;
