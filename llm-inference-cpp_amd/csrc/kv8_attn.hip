@@ -582,11 +582,17 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
     uint4 kreg[kPer], vreg[kPer];
     float2 sreg = make_float2(0.0f, 0.0f);
     bool sreg_live = true;
+    // (The index is the wavefront's; kept in a vector register, so that the
+    // load is waited for where the id is used and not where it is made.)
     int id = 0;
-    const auto lookup = [&](int base) { id = A.v.table[it.table + page_of(A.g, min(base / kBlk + wave, last_block))]; };
+    const auto lookup = [&](int base) {
+      int at = it.table + page_of(A.g, min(base / kBlk + wave, last_block));
+      asm volatile("" : "+v"(at));
+      id = A.v.table[at];
+    };
     const auto fetch = [&](int base) {
       const int want = base / kBlk + wave, block = min(want, last_block);
-      const std::size_t at = block_at(A.g, id, page_of(A.g, block), block, head);
+      const std::size_t at = block_at(A.g, __builtin_amdgcn_readfirstlane(id), page_of(A.g, block), block, head);
       const auto* kp = reinterpret_cast<const uint4*>(A.k + at * (16 * HD));
       const auto* vp = reinterpret_cast<const uint4*>(A.val + at * (16 * HD));
 #pragma unroll
