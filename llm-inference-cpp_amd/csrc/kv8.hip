@@ -381,7 +381,6 @@ llmi_hip_kv8_plan::~llmi_hip_kv8_plan() {
   if (copied != nullptr) (void)hipEventDestroy(copied);
   if (dev != nullptr) (void)hipFree(dev);
   if (parts != nullptr) (void)hipFree(parts);
-  if (joins != nullptr) (void)hipFree(joins);
   if (pinned != nullptr) (void)hipHostFree(pinned);
 }
 
@@ -452,13 +451,12 @@ int llmi_hip_kv8_plan_create(const llmi_kv8_shape* shape, size_t max_seqs, size_
   p->off_append = take(p->most.append * sizeof(AppendItem));
   p->off_few = take(p->most.few * sizeof(AttnItem));
   p->off_many = take(p->most.many * sizeof(AttnItem));
+  p->off_join = take(p->most.join * sizeof(JoinItem));
   p->off_table = take(max_pages * sizeof(std::int32_t));
   LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&p->dev), p->bytes));
   LLMI_TRY_HIP(hipHostMalloc(reinterpret_cast<void**>(&p->pinned), p->bytes, hipHostMallocDefault));
-  const std::size_t rows = p->most.parts * shape->kv_heads * kSlotRows, joins = p->most.joins * shape->kv_heads + 1;
+  const std::size_t rows = p->most.parts * shape->kv_heads * kSlotRows;
   LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&p->parts), (rows + 1) * (shape->head_dim + 2) * sizeof(float)));
-  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&p->joins), joins * sizeof(int)));
-  LLMI_TRY_HIP(hipMemset(p->joins, 0, joins * sizeof(int)));
   LLMI_TRY_HIP(hipEventCreateWithFlags(&p->copied, hipEventDisableTiming));
   *plan = p.release();
   return LLMI_OK;
@@ -476,7 +474,7 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
                                   p->max_tokens, p->max_pages, &l);
     LLMI_REQUIRE(why.empty(), "kv8_plan_set: " + why);
     LLMI_REQUIRE(l.append.size() <= p->most.append && l.few.size() <= p->most.few &&
-                     l.many.size() <= p->most.many && l.parts <= p->most.parts && l.joins <= p->most.joins,
+                     l.many.size() <= p->most.many && l.parts <= p->most.parts && l.join.size() <= p->most.join,
                  "kv8_plan_set: more work than the plan was created for");
     if (p->append_captured) {
       LLMI_REQUIRE(l.writable, "kv8_plan_set: an append of this plan was captured, and " + l.why_not);
@@ -486,7 +484,7 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     LLMI_TRY_HIP(hipEventSynchronize(p->copied));
     const Counts c{static_cast<std::int32_t>(l.append.size()), static_cast<std::int32_t>(l.tokens),
                    static_cast<std::int32_t>(l.seqs.size()), static_cast<std::int32_t>(l.few.size()),
-                   static_cast<std::int32_t>(l.many.size())};
+                   static_cast<std::int32_t>(l.many.size()), static_cast<std::int32_t>(l.join.size())};
     const auto put = [&](std::size_t at, const auto& v) {
       if (!v.empty()) std::memcpy(p->pinned + at, v.data(), v.size() * sizeof(v[0]));
     };
@@ -495,6 +493,7 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     put(p->off_append, l.append);
     put(p->off_few, l.few);
     put(p->off_many, l.many);
+    put(p->off_join, l.join);
     put(p->off_table, l.table);
     const std::size_t used = p->off_table + l.table.size() * sizeof(std::int32_t);
     p->set = false;

@@ -9,7 +9,7 @@ namespace llmi_hip::kv8 {
 // Item counts of the batch that is set, in device memory (launches replayed
 // from a graph read them there).
 struct Counts {
-  std::int32_t append, tokens, seqs, few, many;
+  std::int32_t append, tokens, seqs, few, many, join;
 };
 
 // A plan's device lists.
@@ -20,6 +20,7 @@ struct View {
   const AppendItem* append;
   const AttnItem* few;
   const AttnItem* many;
+  const JoinItem* join;
 };
 
 struct Geometry {
@@ -57,12 +58,9 @@ struct llmi_hip_kv8_plan {
   // marks the copy's end, before which the pinned side is not written again.
   std::uint8_t* dev = nullptr;
   std::uint8_t* pinned = nullptr;
-  std::size_t bytes = 0, off_seqs = 0, off_table = 0, off_append = 0, off_few = 0, off_many = 0;
+  std::size_t bytes = 0, off_seqs = 0, off_table = 0, off_append = 0, off_few = 0, off_many = 0, off_join = 0;
   llmi_hip::kv8::Limits most{};
-  // The attention's partial states, and how many pieces of split rows have
-  // ended (0 between launches; launches of one plan follow each other).
-  float* parts = nullptr;
-  int* joins = nullptr;
+  float* parts = nullptr;  // the attention's partial states (launches of one plan follow each other)
   hipEvent_t copied = nullptr;
   bool set = false;
   llmi_hip::kv8::Lists lists;
@@ -75,7 +73,7 @@ struct llmi_hip_kv8_plan {
     return {reinterpret_cast<const Counts*>(dev), reinterpret_cast<const Seq*>(dev + off_seqs),
             reinterpret_cast<const std::int32_t*>(dev + off_table),
             reinterpret_cast<const AppendItem*>(dev + off_append), reinterpret_cast<const AttnItem*>(dev + off_few),
-            reinterpret_cast<const AttnItem*>(dev + off_many)};
+            reinterpret_cast<const AttnItem*>(dev + off_many), reinterpret_cast<const JoinItem*>(dev + off_join)};
   }
   ~llmi_hip_kv8_plan();
 };

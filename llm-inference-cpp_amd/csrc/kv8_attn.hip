@@ -16,181 +16,95 @@ struct AttnArgs {
   const float* q;
   float* out;
   float* parts;  // rows of partial states: o (dim floats each), then (maximum, sum) each
-  int* joins;    // per split rows and head: how many pieces have ended
   std::size_t q_stride, out_stride, part_states;  // part_states: where the (maximum, sum) pairs begin, in floats
   float scale;
-  int nfew, nmany;  // -1: from v.counts (a captured launch)
+  int nfew, nmany, njoin;  // -1: from v.counts (a captured launch)
 };
 
 // 2^x by the hardware instruction: one rounding; results below 2^-126, which
 // no sum here keeps, are 0.
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Row r of a work item: its token and its place in q and out.
+// Row r of a work item (row0 being its first): its token and its place in q and out.
 struct Row {
   int tok;
   std::size_t off;  // of head_dim floats in the token's row
 };
-__device__ __forceinline__ Row row_of(const AttnArgs& A, const AttnItem& it, int head, int r) {
-  const int row = it.row0 + r, tok = row / A.g.group;
+__device__ __forceinline__ Row row_of(const AttnArgs& A, int row0, int head, int r) {
+  const int row = row0 + r, tok = row / A.g.group;
   return {tok, static_cast<std::size_t>(head * A.g.group + (row - tok * A.g.group)) * A.g.dim};
 }
-
-// Partial states cross workgroups, so they go past the caches that other
-// parts of the chip do not see: device-scope relaxed atomics, in pairs of
-// floats, one store or load each.
-__device__ __forceinline__ void put2(float* p, float a, float b) {
-  __hip_atomic_store(reinterpret_cast<std::uint64_t*>(p),
-                     (static_cast<std::uint64_t>(__float_as_uint(b)) << 32) | __float_as_uint(a), __ATOMIC_RELAXED,
-                     __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float2 get2(const float* p) {
-  const std::uint64_t u = __hip_atomic_load(reinterpret_cast<const std::uint64_t*>(p), __ATOMIC_RELAXED,
-                                            __HIP_MEMORY_SCOPE_AGENT);
-  return make_float2(__uint_as_float(static_cast<std::uint32_t>(u)), __uint_as_float(static_cast<std::uint32_t>(u >> 32)));
-}
-// Row r of piece c's partial state (MOST rows a piece).
-template <int MOST>
-__device__ __forceinline__ std::size_t part_row(const AttnArgs& A, int part, int head, int r) {
-  return static_cast<std::size_t>(part) * A.g.kv_heads * kSlotRows + static_cast<std::size_t>(head) * MOST + r;
+// Row r of a piece whose state is in slots `part` .. part + step - 1.
+__device__ __forceinline__ std::size_t part_row(const AttnArgs& A, int part, int step, int head, int r) {
+  return (static_cast<std::size_t>(part) * A.g.kv_heads + static_cast<std::size_t>(head) * step) * kSlotRows + r;
 }
 
-// Called by every thread of a workgroup after its stores of a piece's state:
-// true for the workgroup that ends last, with the counter back at 0.  Every
-// thread's stores have reached device scope (the wait) before its workgroup
-// counts, so the last one sees all of them.
-__device__ __forceinline__ bool last_piece(const AttnArgs& A, const AttnItem& it, int head, int* flag) {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int* c = A.joins + static_cast<std::size_t>(it.join) * A.g.kv_heads + head;
-    const bool last = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.n - 1;
-    if (last) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    *flag = last;
-  }
-  __syncthreads();
-  return *flag != 0;
-}
-
-// Joins the n pieces of up to MOST rows in the pieces' order: a thread takes
-// two dims of a row over every `share`-th piece, eight loads in flight, with
-// the running maximum; the shares meet in `sh` (THREADS x 4 floats).
-template <int HD, int MOST, int THREADS>
-__device__ void join_pieces(const AttnArgs& A, const AttnItem& it, int head, float4* sh) {
-  constexpr int kPairs = HD / 2;
-  const int cells = it.rows * kPairs;
-  const int share = cells >= THREADS ? 1 : min(THREADS / cells, it.n);
-  const int step = (MOST / kSlotRows);
-  for (int base = 0; base < cells; base += THREADS) {
-    const int mine = static_cast<int>(threadIdx.x) % min(cells, THREADS), cell = base + mine;
-    const int of = static_cast<int>(threadIdx.x) / min(cells, THREADS);
-    const int r = cell / kPairs, d = 2 * (cell - r * kPairs);
-    float m = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
-    if (cell < cells && of < share) {
+// Joins the pieces of split rows, in the pieces' order within a share.  A
+// workgroup takes `at` rows of one head; a thread four dims of a row over
+// every `share`-th piece, eight loads of each kind in flight (what bounds
+// this is their latency), with the running maximum; the shares meet in LDS.
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads) attention_join(AttnArgs A, int at, int chunks) {
+  __shared__ float2 sh_state[kJoinThreads];
+  __shared__ float4 sh_o[kJoinThreads];
+  const int quads = A.g.dim / 4, cells = at * quads, share = kJoinThreads / cells;
+  const int mine = static_cast<int>(threadIdx.x) % cells, of = static_cast<int>(threadIdx.x) / cells;
+  const int njoin = A.njoin >= 0 ? A.njoin : A.v.counts->join;
+  const int units = njoin * A.g.kv_heads * chunks;
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const int item = u / (A.g.kv_heads * chunks), rest = u - item * A.g.kv_heads * chunks;
+    const int head = rest / chunks, r = (rest - head * chunks) * at + mine / quads, d = 4 * (mine % quads);
+    const JoinItem it = A.v.join[item];
+    float m = -INFINITY, l = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (r < it.rows && of < share) {
       for (int c0 = of; c0 < it.n; c0 += 8 * share) {
-        float2 st[8], o[8];
+        float2 st[8];
+        float4 o[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int c = c0 + j * share;
-          st[j] = make_float2(-INFINITY, 0.0f);
-          o[j] = make_float2(0.0f, 0.0f);
-          if (c < it.n) {
-            const std::size_t row = part_row<MOST>(A, it.first + c * step, head, r);
-            st[j] = get2(A.parts + A.part_states + 2 * row);
-            o[j] = get2(A.parts + row * HD + d);
-          }
+          const std::size_t row = part_row(A, it.part + min(c0 + j * share, it.n - 1) * it.step, it.step, head, r);
+          st[j] = *reinterpret_cast<const float2*>(A.parts + A.part_states + 2 * row);
+          o[j] = *reinterpret_cast<const float4*>(A.parts + row * A.g.dim + d);
         }
         float top = m;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, st[j].x);
+        for (int j = 0; j < 8; ++j) {
+          if (c0 + j * share >= it.n) st[j] = make_float2(-INFINITY, 0.0f);
+          top = fmaxf(top, st[j].x);
+        }
         const float ref = top == -INFINITY ? 0.0f : top;
         const float keep = exp2_hw(m - ref);
         l *= keep;
-        x *= keep;
-        y *= keep;
+        x = make_float4(x.x * keep, x.y * keep, x.z * keep, x.w * keep);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
+          if (c0 + j * share >= it.n) continue;  // (a repeated piece may hold NaN)
           const float f = exp2_hw(st[j].x - ref);
           l = fmaf(st[j].y, f, l);
-          x = fmaf(o[j].x, f, x);
-          y = fmaf(o[j].y, f, y);
+          x = make_float4(fmaf(o[j].x, f, x.x), fmaf(o[j].y, f, x.y), fmaf(o[j].z, f, x.z), fmaf(o[j].w, f, x.w));
         }
         m = top;
       }
     }
-    if (share > 1) {
-      sh[threadIdx.x] = make_float4(m, l, x, y);
-      __syncthreads();
-      if (of == 0) {
-        for (int w = 1; w < share; ++w) {
-          const float4 p = sh[w * cells + mine];
-          const float top = fmaxf(m, p.x), ref = top == -INFINITY ? 0.0f : top;
-          const float f = exp2_hw(m - ref), g = exp2_hw(p.x - ref);
-          l = fmaf(p.y, g, l * f);
-          x = fmaf(p.z, g, x * f);
-          y = fmaf(p.w, g, y * f);
-          m = top;
-        }
+    sh_state[threadIdx.x] = make_float2(m, l);
+    sh_o[threadIdx.x] = x;
+    __syncthreads();
+    if (of == 0 && r < it.rows) {
+      for (int w = 1; w < share; ++w) {
+        const float2 s = sh_state[w * cells + mine];
+        const float4 o = sh_o[w * cells + mine];
+        const float top = fmaxf(m, s.x), ref = top == -INFINITY ? 0.0f : top;
+        const float f = exp2_hw(m - ref), g = exp2_hw(s.x - ref);
+        l = fmaf(s.y, g, l * f);
+        x = make_float4(fmaf(o.x, g, x.x * f), fmaf(o.y, g, x.y * f), fmaf(o.z, g, x.z * f), fmaf(o.w, g, x.w * f));
+        m = top;
       }
+      const Row w = row_of(A, it.row0, head, r);
+      *reinterpret_cast<f4*>(A.out + static_cast<std::size_t>(it.row + w.tok) * A.out_stride + w.off + d) =
+          f4{x.x / l, x.y / l, x.z / l, x.w / l};
     }
-    if (cell < cells && of == 0) {
-      const Row w = row_of(A, it, head, r);
-      float* dst = A.out + static_cast<std::size_t>(it.row + w.tok) * A.out_stride + w.off + d;
-      dst[0] = x / l;
-      dst[1] = y / l;
-    }
-  }
-}
-
-// The same for many rows of few pieces: four dims of each of kAt rows at a
-// time, a piece after the other.  Plain loads, behind an acquire of what the
-// other workgroups stored.
-template <int HD, int MOST, int THREADS>
-__device__ void join_rows(const AttnArgs& A, const AttnItem& it, int head) {
-  constexpr int kQuads = HD / 4, kAt = 8, kStep = MOST / kSlotRows;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  int first = threadIdx.x;
-  asm volatile("" : "+v"(first));  // keeps this function's indexes out of the caller's loop: registers
-  const int cells = it.rows * kQuads;
-  for (int base = first; base < cells; base += kAt * THREADS) {
-    float m[kAt], l[kAt];
-    float4 o[kAt];
-#pragma unroll
-    for (int j = 0; j < kAt; ++j) {
-      m[j] = -INFINITY;
-      l[j] = 0.0f;
-      o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-    for (int c = 0; c < it.n; ++c) {
-      float2 st[kAt];
-      float4 x[kAt];
-#pragma unroll
-      for (int j = 0; j < kAt; ++j) {
-        const int cell = min(base + j * THREADS, cells - 1), r = cell / kQuads;
-        const std::size_t row = part_row<MOST>(A, it.first + c * kStep, head, r);
-        st[j] = *reinterpret_cast<const float2*>(A.parts + A.part_states + 2 * row);
-        x[j] = *reinterpret_cast<const float4*>(A.parts + row * HD + 4 * (cell - r * kQuads));
-      }
-#pragma unroll
-      for (int j = 0; j < kAt; ++j) {
-        const float top = fmaxf(m[j], st[j].x), ref = top == -INFINITY ? 0.0f : top;
-        const float f = exp2_hw(m[j] - ref), g = exp2_hw(st[j].x - ref);
-        m[j] = top;
-        l[j] = fmaf(st[j].y, g, l[j] * f);
-        o[j].x = fmaf(x[j].x, g, o[j].x * f);
-        o[j].y = fmaf(x[j].y, g, o[j].y * f);
-        o[j].z = fmaf(x[j].z, g, o[j].z * f);
-        o[j].w = fmaf(x[j].w, g, o[j].w * f);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < kAt; ++j) {
-      const int cell = base + j * THREADS, r = cell / kQuads;
-      if (cell >= cells) break;
-      const Row w = row_of(A, it, head, r);
-      *reinterpret_cast<f4*>(A.out + static_cast<std::size_t>(it.row + w.tok) * A.out_stride + w.off +
-                             4 * (cell - r * kQuads)) = f4{o[j].x / l[j], o[j].y / l[j], o[j].z / l[j], o[j].w / l[j]};
-    }
+    __syncthreads();
   }
 }
 
@@ -245,9 +159,7 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
     std::uint32_t w[kWaves][4][4][16];   // a tile's weight digits: [block][head of the 4][position]
     float o[kWaves][kRows][HD + 16];     // (16: a row of lanes writes other banks than the next)
                                          // the wavefronts' outputs, merged at the end
-    float4 join[kThreads];
   } sh;
-  __shared__ int sh_last;
   __shared__ float sh_m[kWaves][kRows], sh_l[kWaves][kRows];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -266,7 +178,7 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
     for (int mt = 0; mt < MT; ++mt) {
       const int r = 4 * mt + lo16 / 4;
       const bool live = r < it.rows;
-      const Row w = row_of(A, it, h, live ? r : 0);
+      const Row w = row_of(A, it.row0, h, live ? r : 0);
       const float* qp = A.q + static_cast<std::size_t>(it.row + w.tok) * A.q_stride + w.off;
       // Rows of nobody repeat the first one; nothing of theirs is kept.
       float x[kC][16];
@@ -449,18 +361,17 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
         x = fmaf(sh.o[w][r][d], f, x);
         y = fmaf(sh.o[w][r][d + 1], f, y);
       }
-      if (it.n > 1) {
-        const std::size_t row = part_row<few_rows(HD)>(A, it.part, h, r);
-        put2(A.parts + row * HD + d, x, y);
-        if (d == 0) put2(A.parts + A.part_states + 2 * row, top, sum);
+      if (it.part >= 0) {
+        const std::size_t row = part_row(A, it.part, few_rows(HD) / kSlotRows, h, r);
+        *reinterpret_cast<float2*>(A.parts + row * HD + d) = make_float2(x, y);
+        if (d == 0) *reinterpret_cast<float2*>(A.parts + A.part_states + 2 * row) = make_float2(top, sum);
       } else {
-        const Row w = row_of(A, it, h, r);
+        const Row w = row_of(A, it.row0, h, r);
         float* dst = A.out + static_cast<std::size_t>(it.row + w.tok) * A.out_stride + w.off + d;
         dst[0] = x / sum;
         dst[1] = y / sum;
       }
     }
-    if (it.n > 1 && last_piece(A, it, h, &sh_last)) join_pieces<HD, few_rows(HD), kThreads>(A, it, h, sh.join);
     __syncthreads();
   }
 }
@@ -505,13 +416,12 @@ constexpr int kAhead = 4;
 
 template <int HD>
 __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArgs A) {
-  constexpr int kThreads = 256;
+
   constexpr int kG = HD / 16;
   constexpr int kPer = (HD + 63) / 64;  // 16-byte pieces a lane has of a block's keys (and of its values)
   __shared__ uint4 sh_k[2][kG][2][kTile];     // [16-dim group][half of it][position]: 8 fp16
   __shared__ uint4 sh_v[2][kTile / 16][2][HD];  // [block][h][dim]: positions 4h.., 8 + 4h..
   __shared__ float4 sh_s[2][4];               // a tile's blocks: see block_terms
-  __shared__ int sh_last;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nmany = A.nmany >= 0 ? A.nmany : A.v.counts->many;
   const int units = nmany * A.g.kv_heads;
@@ -524,7 +434,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
     const int col = lane & 31, h2nd = lane >> 5;
     const int r = wave * 32 + col;
     const bool live = r < it.rows;
-    const Row own = row_of(A, it, head, live ? r : 0);
+    const Row own = row_of(A, it.row0, head, live ? r : 0);
     const int limit = live ? it.start + own.tok : -1;
     // A negative scale goes to q, so that a block's largest score is its largest product.
     const float q_sign = A.scale < 0.0f ? -1.0f : 1.0f, scale = fabsf(A.scale) * kLog2e;
@@ -800,15 +710,16 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
     int end_lane = threadIdx.x & 63;
     asm volatile("" : "+v"(end_lane));
     const int end_h = end_lane >> 5, end_r = wave * 32 + (end_lane & 31);
-    const Row mine = row_of(A, it, head, live ? end_r : 0);
-    if (live && it.n > 1) {
-      const std::size_t part = part_row<kManyRows>(A, it.part, head, end_r);
-      if (end_h == 0) put2(A.parts + A.part_states + 2 * part, m, l);
+    const Row mine = row_of(A, it.row0, head, live ? end_r : 0);
+    if (live && it.part >= 0) {
+      const std::size_t part = part_row(A, it.part, kManyRows / kSlotRows, head, end_r);
+      if (end_h == 0) *reinterpret_cast<float2*>(A.parts + A.part_states + 2 * part) = make_float2(m, l);
 #pragma unroll
       for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; i += 2)
-          put2(A.parts + part * HD + 32 * d + 8 * (i / 4) + 4 * end_h + i % 4, o[d][i] * unit, o[d][i + 1] * unit);
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4*>(A.parts + part * HD + 32 * d + 8 * i + 4 * end_h) =
+              make_float4(o[d][4 * i] * unit, o[d][4 * i + 1] * unit, o[d][4 * i + 2] * unit, o[d][4 * i + 3] * unit);
     } else if (live) {
       float* dst = A.out + static_cast<std::size_t>(it.row + mine.tok) * A.out_stride + mine.off;
       const float f = unit / l;
@@ -818,10 +729,6 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<f4*>(dst + 32 * d + 8 * i + 4 * end_h) =
               f4{o[d][4 * i] * f, o[d][4 * i + 1] * f, o[d][4 * i + 2] * f, o[d][4 * i + 3] * f};
-    }
-    if (it.n > 1) {
-      if (last_piece(A, it, head, &sh_last)) join_rows<HD, kManyRows, kThreads>(A, it, head);
-      __syncthreads();
     }
   }
 }
@@ -848,10 +755,12 @@ void launch(const AttnArgs& a, unsigned few, unsigned many, int rows, hipStream_
 int launch_attention(const llmi_hip_kv8_plan* p, const llmi_kv8_layer& layer, const float* q, std::size_t q_stride,
                      float scale, float* out, std::size_t out_stride, hipStream_t s, bool captured) {
   const Lists& l = p->lists;
+  const std::size_t heads = static_cast<std::size_t>(p->g.kv_heads);
   const std::size_t part_rows = p->most.parts * static_cast<std::size_t>(p->g.kv_heads) * kSlotRows;
-  AttnArgs a{p->view(), p->g, layer.k, layer.v, layer.scales, q, out, p->parts, p->joins, q_stride, out_stride,
+  AttnArgs a{p->view(), p->g, layer.k, layer.v, layer.scales, q, out, p->parts, q_stride, out_stride,
              part_rows * static_cast<std::size_t>(p->g.dim), scale, captured ? -1 : static_cast<int>(l.few.size()),
-             captured ? -1 : static_cast<int>(l.many.size())};
+             captured ? -1 : static_cast<int>(l.many.size()),
+             captured ? -1 : static_cast<int>(l.join.size())};
   // Captured: room for any batch that the plan takes, but no more workgroups
   // than fill the chip several times (each takes further units in turn).
   const auto grid = [&](std::size_t items, std::size_t most) {
@@ -869,6 +778,17 @@ int launch_attention(const llmi_hip_kv8_plan* p, const llmi_kv8_layer& layer, co
     case 192: launch<192>(a, few, many, rows, s); break;
     case 224: launch<224>(a, few, many, rows, s); break;
     default: launch<256>(a, few, many, rows, s); break;
+  }
+  if (captured || !l.join.empty()) {
+    // One row a workgroup where rows are few (and pieces many), up to as many
+    // as its threads hold where they are enough to fill the chip.
+    const std::size_t items = captured ? p->most.join : l.join.size();
+    const int most = captured ? kManyRows : l.join_rows;
+    const int at = items * heads * most <= 2048 ? 1 : kJoinThreads / (p->g.dim / 4);
+    const int chunks = (most + at - 1) / at;
+    const std::size_t units = items * heads * static_cast<std::size_t>(chunks);
+    attention_join<<<static_cast<unsigned>(std::min<std::size_t>(units, captured ? 4096 : 1u << 30)), kJoinThreads, 0,
+                     s>>>(a, at, chunks);
   }
   LLMI_TRY_HIP(hipGetLastError());
   return LLMI_OK;

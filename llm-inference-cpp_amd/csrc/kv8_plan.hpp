@@ -34,9 +34,8 @@ struct AppendItem {
 // of that head: row r is token r / group, head r % group.  Work of the
 // attention: up to few_rows(head_dim) rows (`few`: single tokens and drafts)
 // or kManyRows rows (`many`: prompts) over positions lo .. hi - 1, lo a
-// multiple of a tile.  n > 1: one of the n pieces of these rows' history; its
-// state goes to partial slots part .., `first` being the first piece's, and
-// the last of the n to end, by the counter `join`, joins them.
+// multiple of a tile.  part >= 0: one of several pieces of these rows'
+// history, whose state goes to partial slots part ..
 constexpr int kTile = 64;
 constexpr int kFewMax = 64;  // most rows of a sequence and key/value head that go as `few` work
 constexpr int kManyRows = 128;
@@ -45,12 +44,17 @@ constexpr int kSlotRows = 8;  // rows of a partial slot
 constexpr int few_rows(int dim) { return dim <= 128 ? 16 : 8; }
 struct AttnItem {
   std::int32_t row, start, table;  // the sequence's, as in Seq
-  std::int32_t row0, rows, lo, hi, part, first, n, join;
+  std::int32_t row0, rows, lo, hi, part;
+};
+// The n pieces of rows row0 .. (at most 16 or kManyRows of them): piece c is
+// in slots part + c * step ...
+struct JoinItem {
+  std::int32_t row, row0, rows, part, n, step;
 };
 // A history is split so that a batch makes about this many units of work
 // (item and key/value head), in pieces of at least the second number.
 constexpr std::size_t kFewTarget = 1024, kFewLeast = 8 * kTile;
-constexpr std::size_t kManyTarget = 1024, kManyLeast = 2 * kTile;
+constexpr std::size_t kManyTarget = 1024, kManyLeast = 4 * kTile;
 
 // block / d for block < 2^27 (positions below 2^31) and d = the blocks of a
 // page, at most 4096: (block * m) >> k with m = 2^k / d + 1, k = 27 + ceil(log2 d):
@@ -68,8 +72,10 @@ constexpr Divisor divisor(std::uint32_t d) {
 
 struct Lists {
   std::vector<AttnItem> few, many;
+  std::vector<JoinItem> join;
   std::int32_t few_rows = 0;  // most rows of a `few` item
-  std::size_t parts = 0, joins = 0;  // partial slots and join counters of a key/value head
+  std::int32_t join_rows = 0;  // most rows of a `join` item
+  std::size_t parts = 0;       // partial slots of a key/value head
   std::vector<Seq> seqs;
   std::vector<std::int32_t> table;
   std::vector<AppendItem> append;  // every block that holds a new token
@@ -102,7 +108,7 @@ inline bool same_shape(const llmi_kv8_shape& a, const llmi_kv8_shape& b) {
 // are its full pieces x heads; rows that are split have at most twice their
 // full pieces; every group of rows adds one item at most.
 struct Limits {
-  std::size_t append, few, many, parts, joins;
+  std::size_t append, few, many, parts, join;
 };
 inline Limits limits(const llmi_kv8_shape& sh, std::size_t seqs, std::size_t tokens) {
   const std::size_t few = kFewTarget / sh.kv_heads, many = kManyTarget / sh.kv_heads;
@@ -216,12 +222,14 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
       const std::size_t piece = ((len + most - 1) / most + unit - 1) / unit * unit, n = (len + piece - 1) / piece;
       const std::size_t slots = few ? few_rows(static_cast<int>(sh.head_dim)) / kSlotRows : kManyRows / kSlotRows;
       const auto i32 = [](std::size_t x) { return static_cast<std::int32_t>(x); };
+      const Seq& q = l.seqs[seq];
       for (std::size_t c = 0; c < n; ++c)
-        items.push_back({l.seqs[seq].row, l.seqs[seq].start, l.seqs[seq].table, i32(r), i32(rows), i32(c * piece), i32(std::min(len, (c + 1) * piece)),
-                         i32(l.parts + c * slots), i32(l.parts), i32(n), i32(l.joins)});
+        items.push_back({q.row, q.start, q.table, i32(r), i32(rows), i32(c * piece),
+                         i32(std::min(len, (c + 1) * piece)), n > 1 ? i32(l.parts + c * slots) : -1});
       if (n == 1) return;
+      l.join.push_back({q.row, i32(r), i32(rows), i32(l.parts), i32(n), i32(slots)});
+      l.join_rows = std::max(l.join_rows, i32(rows));
       l.parts += n * slots;
-      l.joins += 1;
     });
   };
   lay(true, split_of(true, kFewTarget, kFewLeast), l.few);

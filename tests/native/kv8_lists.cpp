@@ -81,7 +81,6 @@ int main() {
     for (std::size_t i = 0; i < l.seqs.size(); ++i) reach[i].assign(static_cast<std::size_t>(l.seqs[i].count) * group, 0);
     std::vector<int> slot(l.parts, 0);
     const int few_most = few_rows(static_cast<int>(sh.head_dim));
-    std::vector<int> pieces(l.joins, 0);
     const auto walk = [&](const std::vector<AttnItem>& items, int most, bool few) {
       for (const AttnItem& it : items) {
         CHECK(it.rows > 0 && it.rows <= most && it.lo % kTile == 0 && it.lo < it.hi);
@@ -96,12 +95,17 @@ int main() {
           const int own = s.start + r / static_cast<int>(group);  // the row's position
           reach[of][static_cast<std::size_t>(r)] += std::max(0, std::min(it.hi, own + 1) - it.lo);
         }
-        if (it.n == 1) continue;
-        CHECK((it.part - it.first) % (most / kSlotRows) == 0 && (it.part - it.first) / (most / kSlotRows) < it.n);
-        CHECK(++pieces.at(static_cast<std::size_t>(it.join)) <= it.n);
+        if (it.part < 0) continue;
         for (int k = 0; k < most / kSlotRows; ++k) CHECK(++slot.at(static_cast<std::size_t>(it.part + k)) == 1);
+        int joins = 0;  // that read this piece, and are of these rows
+        for (const JoinItem& j : l.join)
+          if (it.part >= j.part && it.part < j.part + j.n * j.step) {
+            CHECK(j.row == it.row && j.row0 == it.row0 && j.rows == it.rows && j.rows <= l.join_rows);
+            CHECK(j.step == most / kSlotRows && (it.part - j.part) % j.step == 0 && j.n > 1);
+            ++joins;
+          }
+        CHECK(joins == 1);
       }
-      for (const AttnItem& it : items) CHECK(it.n == 1 || pieces[static_cast<std::size_t>(it.join)] == it.n);
       return 0;
     };
     CHECK(walk(l.few, few_most, true) == 0 && walk(l.many, kManyRows, false) == 0);
@@ -110,7 +114,7 @@ int main() {
     for (const int n_of : slot) CHECK(n_of == 1);
     const Limits m = limits(sh, static_cast<std::size_t>(n), tokens);
     CHECK(l.append.size() <= m.append && l.few.size() <= m.few && l.many.size() <= m.many);
-    CHECK(l.parts <= m.parts && l.joins <= m.joins);
+    CHECK(l.parts <= m.parts && l.join.size() <= m.join);
   }
   for (std::uint32_t d = 1; d <= 4096; ++d) {
     const Divisor v = divisor(d);
