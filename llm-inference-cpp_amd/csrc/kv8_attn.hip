@@ -242,19 +242,23 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
     // Its page id is read a tile ahead.
     const auto page_id = [&](int base) { return A.v.table[it.table + page_of(A.g, min(base / kBlk + grp, last_block))]; };
     int id = page_id(min(it.lo + wave * kTile, it.hi - 1));
-    for (int base = it.lo + wave * kTile; base < it.hi; base += kWaves * kTile) {
-      const int want = base / kBlk + grp, block = min(want, last_block);
-      const std::size_t at = block_at(A.g, id, page_of(A.g, block), block, h);
+    // A tile's keys: every lane needs all four blocks, position lo16, dims
+    // 16 (4c + grp) ...  They are asked for as soon as the tile before has
+    // used its own, and the values once the scores are made; with one tile of
+    // rows all together, which leaves room for a second workgroup on the
+    // compute unit (64 users of 32/8 heads of 128: 109 us against 113).
+    constexpr bool kPipe = MT > 1;
+    std::size_t at = 0;
+    float2 sc = make_float2(0.0f, 0.0f);
+    i4 kf[4][kC];
+    const auto fetch_keys = [&](int base) {
+      const int block = min(base / kBlk + grp, last_block);
+      at = block_at(A.g, id, page_of(A.g, block), block, h);
       if (base + kWaves * kTile < it.hi) id = page_id(base + kWaves * kTile);
-      float2 sc = reinterpret_cast<const float2*>(A.scales)[at];
-      if (want > last_block) sc = make_float2(0.0f, 0.0f);
-      const std::int8_t* kp = A.k + at * (16 * HD);
-      const std::int8_t* vp = A.val + at * (16 * HD) + lo16 * 16;
-      // Keys: every lane needs all four blocks, position lo16, dims 16 (4c + grp) ...
-      i4 kf[4][kC];
+      sc = reinterpret_cast<const float2*>(A.scales)[at];
+      const std::uint64_t p = reinterpret_cast<std::uint64_t>(A.k + at * (16 * HD));
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const std::uint64_t p = reinterpret_cast<std::uint64_t>(kp);
         const std::uint32_t plo = __builtin_amdgcn_readlane(static_cast<int>(p), 16 * b);
         const std::uint32_t phi = __builtin_amdgcn_readlane(static_cast<int>(p >> 32), 16 * b);
         const auto* src = reinterpret_cast<const std::int8_t*>((static_cast<std::uint64_t>(phi) << 32) | plo);
@@ -262,15 +266,43 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
         for (int c = 0; c < kC; ++c)
           kf[b][c] = *reinterpret_cast<const i4*>(src + min(4 * c + grp, kG - 1) * 256 + lo16 * 16);
       }
-      i4 vf[kG];
+    };
+    i4 vf[kG];
+    const auto fetch_values = [&]() {
+      const std::int8_t* vp = A.val + at * (16 * HD) + lo16 * 16;
 #pragma unroll
       for (int g = 0; g < kG; ++g) vf[g] = *reinterpret_cast<const i4*>(vp + g * 256);
-
+    };
+    if (kPipe && it.lo + wave * kTile < it.hi) fetch_keys(it.lo + wave * kTile);
+    for (int base = it.lo + wave * kTile; base < it.hi; base += kWaves * kTile) {
+      if (!kPipe) {
+        fetch_keys(base);
+        fetch_values();
+      }
+      if (base / kBlk + grp > last_block) sc = make_float2(0.0f, 0.0f);
       float ks[4], vs[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         ks[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sc.x), 16 * b));
         vs[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sc.y), 16 * b));
+      }
+      float x[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          i4 acc = {0, 0, 0, 0};
+#pragma unroll
+          for (int c = 0; c < kC; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qd[mt][c], kf[b][c], acc, 0, 0, 0);
+          x[mt][b] = undigit(acc) * ldexpf(A.scale * kLog2e * ks[b], qe[mt]);
+          if (base + b * kBlk + lo16 > limit[mt]) x[mt][b] = -INFINITY;
+        }
+      }
+      if (kPipe) {
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_values();
+        if (base + kWaves * kTile < it.hi) fetch_keys(base + kWaves * kTile);
+        __builtin_amdgcn_sched_barrier(0);
       }
       // The tile's largest finite value scale; 2^-96 keeps 2^30 / top finite.
       float vf_s[4], top = 0x1p-96f;
@@ -282,18 +314,7 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
       const float to_fix = 0x1p30f / top;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        if (4 * mt >= it.rows) break;
-        float x[4];
-        float mx = m[mt];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          i4 acc = {0, 0, 0, 0};
-#pragma unroll
-          for (int c = 0; c < kC; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qd[mt][c], kf[b][c], acc, 0, 0, 0);
-          x[b] = undigit(acc) * ldexpf(A.scale * kLog2e * ks[b], qe[mt]);
-          if (base + b * kBlk + lo16 > limit[mt]) x[b] = -INFINITY;
-          mx = fmaxf(mx, x[b]);
-        }
+        float mx = fmaxf(fmaxf(fmaxf(x[mt][0], x[mt][1]), fmaxf(x[mt][2], x[mt][3])), m[mt]);
         mx = row16_max(mx);
         const float ref = mx == -INFINITY ? 0.0f : mx;
         const float keep = exp2_hw(m[mt] - ref);
@@ -302,7 +323,7 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           const bool seen = base + b * kBlk + lo16 <= limit[mt];
-          const float p = exp2_hw(x[b] - ref);
+          const float p = exp2_hw(x[mt][b] - ref);
           // A value scale that is inf or NaN shows in the sum of the rows that see the block.
           if (seen) sum += fmaf(vs[b], 0.0f, p);
           const int w = static_cast<int>(rintf(p * (vf_s[b] * to_fix)));

@@ -52,9 +52,16 @@ struct JoinItem {
   std::int32_t row, row0, rows, part, n, step;
 };
 // A history is split so that a batch makes about this many units of work
-// (item and key/value head), in pieces of at least the second number.
-constexpr std::size_t kFewTarget = 1024, kFewLeast = 8 * kTile;
-constexpr std::size_t kManyTarget = 1024, kManyLeast = 4 * kTile;
+// (item and key/value head), in pieces of at least the second number of
+// positions.  Measured: 512 units of `few` work against 1024, 64 users of 4000
+// positions (32/8 heads of 128) 93 us against 102; 768 units of `many` work
+// against 512 and 1024, 2048 tokens over 6144 447 us against 487 and 472.
+// The join of pieces costs 4 us, a tile of each wavefront 1.8 us: a `few`
+// history up to kFewWhole is not split (one user of 32/8 heads of 128 over
+// 1500 positions 8.8 us against 9.4 in pieces, over 3000 in pieces 9.7
+// against 14.7).
+constexpr std::size_t kFewTarget = 512, kFewLeast = 8 * kTile, kFewWhole = 24 * kTile;
+constexpr std::size_t kManyTarget = 768, kManyLeast = 4 * kTile;
 
 // block / d for block < 2^27 (positions below 2^31) and d = the blocks of a
 // page, at most 4096: (block * m) >> k with m = 2^k / d + 1, k = 27 + ceil(log2 d):
@@ -218,8 +225,10 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
   const auto lay = [&](bool few, std::size_t split, std::vector<AttnItem>& items) {
     each(few, [&](std::size_t seq, std::size_t r, std::size_t rows, std::size_t len) {
       // Pieces of one size, in whole units (of a tile for each of its wavefronts, if few).
-      const std::size_t unit = few ? kFewLeast : kTile, most = (len + split - 1) / split;
-      const std::size_t piece = ((len + most - 1) / most + unit - 1) / unit * unit, n = (len + piece - 1) / piece;
+      const std::size_t unit = few ? kFewLeast : kTile;
+      const std::size_t most = few && len <= kFewWhole ? 1 : (len + split - 1) / split;
+      const std::size_t piece = ((len + most - 1) / most + unit - 1) / unit * unit;
+      const std::size_t n = (len + piece - 1) / piece;
       const std::size_t slots = few ? few_rows(static_cast<int>(sh.head_dim)) / kSlotRows : kManyRows / kSlotRows;
       const auto i32 = [](std::size_t x) { return static_cast<std::int32_t>(x); };
       const Seq& q = l.seqs[seq];
