@@ -34,66 +34,74 @@ __device__ __forceinline__ std::uint32_t wave_umax(std::uint32_t v) {
   for (int o = 32; o > 0; o >>= 1) v = max(v, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(v), o, 64)));
   return v;
 }
-// float(amax / 127) with one rounding; NaN and inf stay what they are.
-__device__ __forceinline__ float block_scale(std::uint32_t amax) {
-  return static_cast<float>(static_cast<double>(__uint_as_float(amax)) / 127.0);
+// A block's scale, float(amax / 127) with one rounding (NaN and inf stay what
+// they are), and what its codes are computed with.
+struct Scale {
+  float s, inverse;
+  bool usable, plain;  // finite and not 0; 1 / s is a normal number too
+  __device__ __forceinline__ explicit Scale(std::uint32_t amax)
+      : s(static_cast<float>(static_cast<double>(__uint_as_float(amax)) / 127.0)),
+        inverse(1.0f / s),
+        usable(s > 0.0f && amax < 0x7F800000u),
+        plain(s >= 0x1p-120f) {}
+};
+// The nearest integer to x / s, ties to even.  |x / s| is below 128, so the
+// fp32 product with 1 / s is within 2^-15 of it and decides unless it comes
+// that near to a border.  There the 64-bit quotient does: a quotient of two
+// fp32 numbers is either a tie, which 64 bits hold exactly, or at least 2^-26
+// of itself away from one.
+__device__ __forceinline__ int code_of(float x, const Scale& s) {
+  if (!s.usable) return 0;
+  const float t = x * s.inverse;
+  float r = rintf(t);
+  if (!(fabsf(t - r) < 0.4999f) || !s.plain)
+    r = static_cast<float>(rint(static_cast<double>(x) / static_cast<double>(s.s)));
+  return static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
 }
-// The nearest integer to x / scale, ties to even.  The quotient of two fp32
-// numbers is either a tie, which 64 bits hold exactly, or at least 2^-26 of
-// itself away from one: the 64-bit quotient rounds like the exact one.
-__device__ __forceinline__ int code_of(float x, float scale, bool finite) {
-  if (!finite) return 0;
-  const double r = rint(static_cast<double>(x) / static_cast<double>(scale));
-  return static_cast<int>(fmin(fmax(r, -127.0), 127.0));
+// Byte j of a dword of codes.
+__device__ __forceinline__ float code_value(std::uint32_t four, int j) {
+  return static_cast<float>(static_cast<std::int32_t>(four << (24 - 8 * j)) >> 24);
 }
-__device__ __forceinline__ bool usable(float scale) { return scale > 0.0f && abs_bits(scale) < 0x7F800000u; }
 
-// What a lane holds of one row of a head: dims 8c .. 8c+7 (a) and their
-// rotation partners dim/2 + 8c ... (b).  `lpr` neighbouring lanes (a power
-// of two, at least dim / 16) share a row.
-// Norm and rotation in 64 bits, rounded once.
-__device__ __forceinline__ void norm_rotate(float* a, float* b, bool live, int lpr, int c, int dim,
-                                            const float* __restrict__ w, float eps, const float* __restrict__ cos_r,
-                                            const float* __restrict__ sin_r) {
-  double ss = 0.0;
-  if (w != nullptr) {
+// Lanes that share a row of a head: each holds dims 8c .. 8c+7 and their
+// rotation partners DIM/2 + 8c ..; a power of two, so that sums over the row
+// are exchanges between neighbours.
+constexpr int lanes_per_row(int dim) { return dim <= 32 ? 2 : dim <= 64 ? 4 : dim <= 128 ? 8 : 16; }
+
+// Norm and rotation of a row in 64 bits, rounded once: k's codes sit next to
+// rounding borders, and one rounding makes them independent of the order of
+// the norm's sum.  The 64-bit arithmetic is hidden behind the loads (14k
+// tokens of 32/8 heads of 128: the same time without it).
+// w, co, si: this lane's 16 (dims 8c .. and partners) and 8 + 8 numbers.
+template <int DIM>
+__device__ __forceinline__ void norm_rotate(float (&x)[16], bool live, bool norm, const float (&w)[16], float eps,
+                                            bool turn, const float (&co)[8], const float (&si)[8]) {
+  double r = 1.0;
+  if (norm) {
+    double ss = 0.0;
     if (live) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        ss = fma(static_cast<double>(a[i]), static_cast<double>(a[i]), ss);
-        ss = fma(static_cast<double>(b[i]), static_cast<double>(b[i]), ss);
-      }
+      for (int i = 0; i < 16; ++i) ss = fma(static_cast<double>(x[i]), static_cast<double>(x[i]), ss);
     }
-    for (int o = 1; o < lpr; o <<= 1) ss += __shfl_xor(ss, o, 64);
-  }
-  if (!live) return;
-  double r = 1.0;
-  float wa[8], wb[8];
-  if (w != nullptr) {
-    r = 1.0 / sqrt(ss / dim + static_cast<double>(eps));
-    load8(w + 8 * c, wa);
-    load8(w + dim / 2 + 8 * c, wb);
-  }
-  float co[8], si[8];
-  if (cos_r != nullptr) {
-    load8(cos_r + 8 * c, co);
-    load8(sin_r + 8 * c, si);
+#pragma unroll
+    for (int o = 1; o < lanes_per_row(DIM); o <<= 1) ss += __shfl_xor(ss, o, 64);
+    r = 1.0 / sqrt(ss / DIM + static_cast<double>(eps));
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    double x = a[i], y = b[i];
-    if (w != nullptr) {
-      x = x * r * static_cast<double>(wa[i]);
-      y = y * r * static_cast<double>(wb[i]);
+    double a = x[i], b = x[8 + i];
+    if (norm) {
+      a = a * r * static_cast<double>(w[i]);
+      b = b * r * static_cast<double>(w[8 + i]);
     }
-    if (cos_r != nullptr) {
-      const double cc = co[i], sn = si[i];
-      const double t = fma(x, cc, -(y * sn));
-      y = fma(y, cc, x * sn);
-      x = t;
+    if (turn) {
+      const double c = co[i], s = si[i];
+      const double t = fma(a, c, -(b * s));
+      b = fma(b, c, a * s);
+      a = t;
     }
-    a[i] = static_cast<float>(x);
-    b[i] = static_cast<float>(y);
+    x[i] = static_cast<float>(a);
+    x[8 + i] = static_cast<float>(b);
   }
 }
 
@@ -105,192 +113,237 @@ struct AppendArgs {
   float* q_out;
   std::size_t q_stride, k_stride, v_stride, q_out_stride;
   float eps;
-  int nappend, ntokens;  // -1: from v.counts (a captured launch)
+  int nblocks, ntokens;  // -1: from v.counts (a captured launch)
+  int q_each;            // head groups of a token that one wavefront takes
 };
 
-__device__ __forceinline__ float* open_rows(const AppendArgs& A, const Seq& s, int h, int block, int which) {
-  return A.layer.open + ((((static_cast<std::size_t>(s.slot) * A.g.kv_heads + h) * 2 + (block & 1)) * 2 + which) * 16) *
-                            static_cast<std::size_t>(A.g.dim);
+// A block as one wavefront sees it.
+struct Block {
+  int pos;
+  std::size_t at;  // in [page][kv head][block]
+};
+__device__ __forceinline__ Block block_of(const Geometry& g, const BlockItem& it, int h, bool then) {
+  const std::size_t page = then ? it.then_page : it.page;
+  return {then ? it.then_pos : it.pos, (page * g.kv_heads + h) * g.page_blocks + (then ? it.then_block : it.block)};
+}
+__device__ __forceinline__ float* open_rows(const AppendArgs& A, const BlockItem& it, int dim, int h, int pos,
+                                            int which) {
+  return A.layer.open +
+         ((((static_cast<std::size_t>(it.slot) * A.g.kv_heads + h) * 2 + (pos / kBlk & 1)) * 2 + which) * kBlk) * dim;
 }
 
-// Keys of one block and head: lanes take (position, 8-dim pair chunk).
-template <int LPR>
-__device__ void append_keys(const AppendArgs& A, const Seq& s, int h, int block, int last, int lane) {
-  constexpr int kRows = 64 / LPR, kPasses = LPR < 4 ? 1 : LPR / 4;
-  const int dim = A.g.dim, half = dim / 2, c = lane % LPR;
-  float* open = open_rows(A, s, h, block, 0);
+// Four codes of x / scale in a dword.
+__device__ __forceinline__ std::uint32_t codes4(const float* x, const Scale& s) {
+  std::uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w |= (static_cast<std::uint32_t>(code_of(x[j], s)) & 0xFFu) << (8 * j);
+  return w;
+}
+
+// Keys of one block and head: lanes take (position, 8 dims and partners).
+template <int DIM>
+__device__ void append_keys(const AppendArgs& A, const BlockItem& it, int h, const Block& b, int lane) {
+  constexpr int kLpr = lanes_per_row(DIM), kRows = 64 / kLpr, kPasses = (kBlk + kRows - 1) / kRows, kHalf = DIM / 2;
+  const int c = lane % kLpr;
+  float* open = open_rows(A, it, DIM, h, b.pos, 0);
   float x[kPasses][16];
+  const bool chunk = DIM / 16 == kLpr || c < DIM / 16;
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int tok = p * kRows + lane / kLpr, pos = b.pos + tok;
+    const bool in = chunk && tok < kBlk;
+    const float* src = pos < it.start ? open + tok * DIM
+                                      : A.k + static_cast<std::size_t>(it.row + (pos - it.start)) * A.k_stride +
+                                            static_cast<std::size_t>(h) * DIM;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[p][i] = 0.0f;
+    if (in && pos < it.end) {
+      load8(src + 8 * c, x[p]);
+      load8(src + kHalf + 8 * c, x[p] + 8);
+    }
+  }
+  float w[16] = {};
+  if (A.k_norm != nullptr && chunk) {
+    load8(A.k_norm + 8 * c, w);
+    load8(A.k_norm + kHalf + 8 * c, w + 8);
+  }
   std::uint32_t amax = 0;
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
-    const int tok = p * kRows + lane / LPR, pos = block * kBlk + tok;
-    const bool chunk = c < dim / 16 && tok < kBlk;
-    const bool fresh = chunk && pos >= s.start && pos < s.start + s.count;
-    const bool held = chunk && pos < s.start;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[p][i] = 0.0f;
-    if (fresh) {
-      const float* src = A.k + static_cast<std::size_t>(s.row + (pos - s.start)) * A.k_stride +
-                         static_cast<std::size_t>(h) * dim;
-      load8(src + 8 * c, x[p]);
-      load8(src + half + 8 * c, x[p] + 8);
-    } else if (held) {
-      load8(open + tok * dim + 8 * c, x[p]);
-      load8(open + tok * dim + half + 8 * c, x[p] + 8);
-    }
-    const std::size_t t = static_cast<std::size_t>(fresh ? pos : 0) * half;
-    float y[16];
+    const int tok = p * kRows + lane / kLpr, pos = b.pos + tok;
+    const bool fresh = chunk && tok < kBlk && pos >= it.start && pos < it.end;
+    float y[16], co[8] = {}, si[8] = {};
 #pragma unroll
     for (int i = 0; i < 16; ++i) y[i] = x[p][i];
-    norm_rotate(y, y + 8, fresh, LPR, c, dim, A.k_norm, A.eps, A.cos_t != nullptr ? A.cos_t + t : nullptr,
-                A.cos_t != nullptr ? A.sin_t + t : nullptr);
+    if (A.cos_t != nullptr && fresh) {
+      load8(A.cos_t + static_cast<std::size_t>(pos) * kHalf + 8 * c, co);
+      load8(A.sin_t + static_cast<std::size_t>(pos) * kHalf + 8 * c, si);
+    }
+    norm_rotate<DIM>(y, fresh, A.k_norm != nullptr, w, A.eps, A.cos_t != nullptr, co, si);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      x[p][i] = y[i];
-      amax = max(amax, abs_bits(y[i]));
+      if (fresh) x[p][i] = y[i];
+      amax = max(amax, abs_bits(x[p][i]));
     }
   }
-  amax = wave_umax(amax);
-  const float scale = block_scale(amax);
-  const bool ok = usable(scale);
-  const std::size_t at = block_index(A.g, A.v.table, s, block, h);
-  std::int8_t* dst = A.layer.k + at * A.g.block_bytes;
-  if (lane == 0) A.layer.scales[2 * at] = scale;
+  const Scale scale(wave_umax(amax));
+  std::int8_t* dst = A.layer.k + b.at * (kBlk * DIM);
+  if (lane == 0) A.layer.scales[2 * b.at] = scale.s;
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
-    const int tok = p * kRows + lane / LPR, pos = block * kBlk + tok;
-    if (c >= dim / 16 || tok >= kBlk) continue;
+    const int tok = p * kRows + lane / kLpr, pos = b.pos + tok;
+    if (!chunk || tok >= kBlk) continue;
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-      const int d = side * half + 8 * c;
-      std::uint32_t w[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        w[i] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[i] |= (static_cast<std::uint32_t>(code_of(x[p][8 * side + 4 * i + j], scale, ok)) & 0xFFu) << (8 * j);
-      }
-      *reinterpret_cast<uint2*>(dst + (d / 16) * 256 + tok * 16 + d % 16) = make_uint2(w[0], w[1]);
+      const int d = side * kHalf + 8 * c;
+      *reinterpret_cast<uint2*>(dst + (d / 16) * 256 + tok * 16 + d % 16) =
+          make_uint2(codes4(&x[p][8 * side], scale), codes4(&x[p][8 * side + 4], scale));
     }
-    if (block >= last - 1 && pos >= s.start && pos < s.start + s.count) {
-      store8(open + tok * dim + 8 * c, x[p]);
-      store8(open + tok * dim + half + 8 * c, x[p] + 8);
+    if (pos >= it.keep && pos >= it.start && pos < it.end) {
+      store8(open + tok * DIM + 8 * c, x[p]);
+      store8(open + tok * DIM + kHalf + 8 * c, x[p] + 8);
     }
+  }
+}
+
+// Dims that a lane has side by side where it takes whole dims (values, and
+// both in read_kernel).
+constexpr int dims_per_lane(int dim) { return dim % 256 == 0 ? 4 : dim % 128 == 0 ? 2 : 1; }
+template <int N>
+__device__ __forceinline__ void loadn(const float* p, float* x) {
+  typedef float v __attribute__((ext_vector_type(N), aligned(4)));
+  const v a = *reinterpret_cast<const v*>(p);
+  if constexpr (N == 1) {
+    x[0] = *p;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = a[i];
+  }
+}
+template <int N>
+__device__ __forceinline__ void storen(float* p, const float* x) {
+  if constexpr (N == 1) {
+    *p = x[0];
+  } else {
+    typedef float v __attribute__((ext_vector_type(N), aligned(4)));
+    v a;
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = x[i];
+    *reinterpret_cast<v*>(p) = a;
   }
 }
 
 // Values of one block and head: lanes take whole dims, so that a lane's 16
 // codes are the 16 neighbouring bytes of its dim.
-template <int LPR>
-__device__ void append_values(const AppendArgs& A, const Seq& s, int h, int block, int last, int lane) {
-  constexpr int kGroups = LPR < 4 ? 1 : LPR / 4;  // of 64 dims
-  const int dim = A.g.dim;
-  float* open = open_rows(A, s, h, block, 1);
-  float x[kGroups][16];
+template <int DIM>
+__device__ void append_values(const AppendArgs& A, const BlockItem& it, int h, const Block& b, int lane) {
+  constexpr int kN = dims_per_lane(DIM), kGroups = (DIM + 64 * kN - 1) / (64 * kN);
+  float* open = open_rows(A, it, DIM, h, b.pos, 1);
+  float x[kGroups][kBlk][kN];
   std::uint32_t amax = 0;
 #pragma unroll
   for (int n = 0; n < kGroups; ++n) {
-    const int d = n * 64 + lane;
+    const int d = (n * 64 + lane) * kN;
 #pragma unroll
-    for (int t = 0; t < 16; ++t) {
-      const int pos = block * kBlk + t;
-      x[n][t] = 0.0f;
-      if (d < dim) {
-        if (pos < s.start)
-          x[n][t] = open[t * dim + d];
-        else if (pos < s.start + s.count)
-          x[n][t] = A.val[static_cast<std::size_t>(s.row + (pos - s.start)) * A.v_stride +
-                          static_cast<std::size_t>(h) * dim + d];
-      }
-      amax = max(amax, abs_bits(x[n][t]));
+    for (int t = 0; t < kBlk; ++t) {
+      const int pos = b.pos + t;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) x[n][t][i] = 0.0f;
+      if (d < DIM && pos < it.end)
+        loadn<kN>((pos < it.start ? open + t * DIM
+                                  : A.val + static_cast<std::size_t>(it.row + (pos - it.start)) * A.v_stride +
+                                        static_cast<std::size_t>(h) * DIM) +
+                      d,
+                  x[n][t]);
     }
   }
-  amax = wave_umax(amax);
-  const float scale = block_scale(amax);
-  const bool ok = usable(scale);
-  const std::size_t at = block_index(A.g, A.v.table, s, block, h);
-  std::int8_t* dst = A.layer.v + at * A.g.block_bytes;
-  if (lane == 0) A.layer.scales[2 * at + 1] = scale;
+#pragma unroll
+  for (int n = 0; n < kGroups; ++n)
+#pragma unroll
+    for (int t = 0; t < kBlk; ++t)
+#pragma unroll
+      for (int i = 0; i < kN; ++i) amax = max(amax, abs_bits(x[n][t][i]));
+  const Scale scale(wave_umax(amax));
+  std::int8_t* dst = A.layer.v + b.at * (kBlk * DIM);
+  if (lane == 0) A.layer.scales[2 * b.at + 1] = scale.s;
 #pragma unroll
   for (int n = 0; n < kGroups; ++n) {
-    const int d = n * 64 + lane;
-    if (d >= dim) continue;
-    std::uint32_t w[4];
+    const int d = (n * 64 + lane) * kN;
+    if (d >= DIM) continue;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = 0;
+    for (int i = 0; i < kN; ++i) {
+      std::uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[i] |= (static_cast<std::uint32_t>(code_of(x[n][4 * i + j], scale, ok)) & 0xFFu) << (8 * j);
-    }
-    *reinterpret_cast<uint4*>(dst + d * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-    if (block >= last - 1) {
-#pragma unroll
-      for (int t = 0; t < 16; ++t) {
-        const int pos = block * kBlk + t;
-        if (pos >= s.start && pos < s.start + s.count) open[t * dim + d] = x[n][t];
+      for (int j = 0; j < 4; ++j) {
+        const float y[4] = {x[n][4 * j][i], x[n][4 * j + 1][i], x[n][4 * j + 2][i], x[n][4 * j + 3][i]};
+        w[j] = codes4(y, scale);
       }
+      *reinterpret_cast<uint4*>(dst + (d + i) * kBlk) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+#pragma unroll
+    for (int t = 0; t < kBlk; ++t) {
+      const int pos = b.pos + t;
+      if (pos >= it.keep && pos >= it.start && pos < it.end) storen<kN>(open + t * DIM + d, x[n][t]);
     }
   }
 }
 
-// One wavefront per unit of work: the blocks' keys and values first (item,
-// head, k / v), then q (64 / LPR rows of a token and head each).
-template <int LPR>
+// Units of work, one wavefront each: blocks' keys and values (item, head, k /
+// v), then tokens' q (64 / lanes_per_row heads at a time, q_each times).  HBM
+// bounds it: 14402 tokens of 32/8 heads of 128 with norms move 0.62 GB.
+template <int DIM>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs A) {
+  constexpr int kLpr = lanes_per_row(DIM), kRows = 64 / kLpr, kHalf = DIM / 2;
   const int lane = threadIdx.x & 63;
-  const int nappend = A.nappend >= 0 ? A.nappend : A.v.counts->append;
+  const int nblocks = A.nblocks >= 0 ? A.nblocks : A.v.counts->blocks;
   const int ntokens = A.ntokens >= 0 ? A.ntokens : A.v.counts->tokens;
-  const long kv_units = 2L * nappend * A.g.kv_heads;
-  const long q_rows = A.q != nullptr ? static_cast<long>(ntokens) * A.g.heads : 0;
-  const long units = kv_units + (q_rows + 64 / LPR - 1) / (64 / LPR);
-  for (long u = static_cast<long>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < units;
-       u += static_cast<long>(gridDim.x) * kWaves) {
+  const unsigned kv_units = 2u * nblocks * A.g.kv_heads;
+  const unsigned per_token = (A.g.heads + kRows * A.q_each - 1) / (kRows * A.q_each);
+  const unsigned units = kv_units + (A.q != nullptr ? ntokens * per_token : 0u);
+  for (unsigned u = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < units;
+       u += gridDim.x * kWaves) {
     if (u < kv_units) {
-      const int which = u & 1;
-      const int h = static_cast<int>((u >> 1) % A.g.kv_heads);
-      const AppendItem it = A.v.append[(u >> 1) / A.g.kv_heads];
-      const Seq s = A.v.seqs[it.seq];
-      const int last = (s.start + s.count - 1) / kBlk;
-      for (int block = it.block; block >= 0; block = block == it.block ? it.then : -1) {
-        if (which == 0)
-          append_keys<LPR>(A, s, h, block, last, lane);
+      const unsigned pair = u >> 1, item = pair / A.g.kv_heads;
+      const int h = static_cast<int>(pair - item * A.g.kv_heads);
+      const BlockItem it = A.v.blocks[item];
+      for (int then = 0; then < (it.then_pos >= 0 ? 2 : 1); ++then) {
+        const Block b = block_of(A.g, it, h, then != 0);
+        if ((u & 1) == 0)
+          append_keys<DIM>(A, it, h, b, lane);
         else
-          append_values<LPR>(A, s, h, block, last, lane);
+          append_values<DIM>(A, it, h, b, lane);
       }
       continue;
     }
-    const long r = (u - kv_units) * (64 / LPR) + lane / LPR;
-    const int c = lane % LPR, dim = A.g.dim, half = dim / 2;
-    const bool live = r < q_rows && c < dim / 16;
-    const long t = live ? r / A.g.heads : 0, h = live ? r % A.g.heads : 0;
-    int pos = 0;
-    if (A.cos_t != nullptr && live) {
-      // The token's sequence: the last one that starts at or before row t.
-      int lo = 0, hi = A.v.counts->seqs - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (A.v.seqs[mid].row <= t)
-          lo = mid;
-        else
-          hi = mid - 1;
+    const unsigned t = (u - kv_units) / per_token, part = u - kv_units - t * per_token;
+    const int c = lane % kLpr;
+    const bool chunk = DIM / 16 == kLpr || c < DIM / 16;
+    float w[16] = {}, co[8] = {}, si[8] = {};
+    if (A.q_norm != nullptr && chunk) {
+      load8(A.q_norm + 8 * c, w);
+      load8(A.q_norm + kHalf + 8 * c, w + 8);
+    }
+    if (A.cos_t != nullptr && chunk) {
+      const std::size_t at = static_cast<std::size_t>(A.v.positions[t]) * kHalf + 8 * c;
+      load8(A.cos_t + at, co);
+      load8(A.sin_t + at, si);
+    }
+    for (int e = 0; e < A.q_each; ++e) {
+      const int head = (static_cast<int>(part) * A.q_each + e) * kRows + lane / kLpr;
+      const bool live = chunk && head < A.g.heads;
+      float x[16] = {};
+      const std::size_t off = static_cast<std::size_t>(head) * DIM + 8 * c;
+      if (live) {
+        const float* src = A.q + t * A.q_stride + off;
+        load8(src, x);
+        load8(src + kHalf, x + 8);
       }
-      pos = A.v.seqs[lo].start + static_cast<int>(t) - A.v.seqs[lo].row;
-    }
-    float a[8] = {}, b[8] = {};
-    if (live) {
-      const float* src = A.q + static_cast<std::size_t>(t) * A.q_stride + static_cast<std::size_t>(h) * dim;
-      load8(src + 8 * c, a);
-      load8(src + half + 8 * c, b);
-    }
-    const std::size_t at = static_cast<std::size_t>(pos) * half;
-    norm_rotate(a, b, live, LPR, c, dim, A.q_norm, A.eps, A.cos_t != nullptr ? A.cos_t + at : nullptr,
-                A.cos_t != nullptr ? A.sin_t + at : nullptr);
-    if (live) {
-      float* dst = A.q_out + static_cast<std::size_t>(t) * A.q_out_stride + static_cast<std::size_t>(h) * dim;
-      store8(dst + 8 * c, a);
-      store8(dst + half + 8 * c, b);
+      norm_rotate<DIM>(x, live, A.q_norm != nullptr, w, A.eps, A.cos_t != nullptr, co, si);
+      if (live) {
+        float* dst = A.q_out + t * A.q_out_stride + off;
+        store8(dst, x);
+        store8(dst + kHalf, x + 8);
+      }
     }
   }
 }
@@ -301,44 +354,65 @@ struct ReadArgs {
   llmi_kv8_layer layer;
   float *k, *val;
   std::size_t k_stride, v_stride;
-  int nappend;
+  int nblocks;
 };
 
-// One wavefront per block, head and k / v: 16 dims of 16 positions at a time,
-// lane (position, 4 dims).
+// One wavefront per block, head and k / v.  Keys: a lane four dims of a
+// position; values: whole dims, as they are stored.  Either way a store
+// instruction writes whole rows side by side.
+template <int DIM>
 __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs A) {
   const int lane = threadIdx.x & 63;
-  const int nitems = A.nappend >= 0 ? A.nappend : A.v.counts->append;
-  const long units = 2L * nitems * A.g.kv_heads;
-  const int tok = lane >> 2, d4 = (lane & 3) * 4;
-  for (long u = static_cast<long>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < units;
-       u += static_cast<long>(gridDim.x) * kWaves) {
-    const int which = u & 1;
-    float* out = which == 0 ? A.k : A.val;
+  const int nblocks = A.nblocks >= 0 ? A.nblocks : A.v.counts->blocks;
+  const unsigned units = 2u * nblocks * A.g.kv_heads;
+  for (unsigned u = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < units;
+       u += gridDim.x * kWaves) {
+    const unsigned pair = u >> 1, item = pair / A.g.kv_heads;
+    const int h = static_cast<int>(pair - item * A.g.kv_heads);
+    const bool keys = (u & 1) == 0;
+    float* out = keys ? A.k : A.val;
     if (out == nullptr) continue;
-    const std::size_t stride = which == 0 ? A.k_stride : A.v_stride;
-    const int h = static_cast<int>((u >> 1) % A.g.kv_heads);
-    const AppendItem it = A.v.append[(u >> 1) / A.g.kv_heads];
-    const Seq s = A.v.seqs[it.seq];
-    for (int block = it.block; block >= 0; block = block == it.block ? it.then : -1) {
-      const int pos = block * kBlk + tok;
-      const std::size_t at = block_index(A.g, A.v.table, s, block, h);
-      const std::int8_t* src = (which == 0 ? A.layer.k : A.layer.v) + at * A.g.block_bytes;
-      const float scale = A.layer.scales[2 * at + which];
-      if (pos < s.start || pos >= s.start + s.count) continue;
-      float* row = out + static_cast<std::size_t>(s.row + (pos - s.start)) * stride +
-                   static_cast<std::size_t>(h) * A.g.dim + d4;
-      for (int g = 0; g < A.g.dim / 16; ++g) {
-        std::int8_t c[4];
-        if (which == 0) {
-          __builtin_memcpy(c, src + g * 256 + tok * 16 + d4, 4);
-        } else {
+    const std::size_t stride = keys ? A.k_stride : A.v_stride;
+    const BlockItem it = A.v.blocks[item];
+    for (int then = 0; then < (it.then_pos >= 0 ? 2 : 1); ++then) {
+      const Block b = block_of(A.g, it, h, then != 0);
+      const float scale = A.layer.scales[2 * b.at + (keys ? 0 : 1)];
+      const int lo = max(it.start - b.pos, 0), hi = min(it.end - b.pos, kBlk);  // rows of the block
+      float* rows = out + (static_cast<std::int64_t>(it.row) + b.pos - it.start) * static_cast<std::int64_t>(stride) +
+                    static_cast<std::int64_t>(h) * DIM;
+      if (keys) {
+        const std::int8_t* src = A.layer.k + b.at * (kBlk * DIM);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) c[j] = src[g * 256 + (d4 + j) * 16 + tok];
+        for (int n = 0; n < DIM / 16; ++n) {
+          const int e = n * 64 + lane, r = e / (DIM / 4), d = 4 * (e % (DIM / 4));
+          if (r < lo || r >= hi) continue;
+          const std::uint32_t c = *reinterpret_cast<const std::uint32_t*>(src + (d / 16) * 256 + r * 16 + d % 16);
+          const float x[4] = {code_value(c, 0) * scale, code_value(c, 1) * scale, code_value(c, 2) * scale,
+                              code_value(c, 3) * scale};
+          storen<4>(rows + static_cast<std::int64_t>(r) * static_cast<std::int64_t>(stride) + d, x);
         }
-        *reinterpret_cast<f4*>(row + g * 16) =
-            f4{static_cast<float>(c[0]) * scale, static_cast<float>(c[1]) * scale, static_cast<float>(c[2]) * scale,
-               static_cast<float>(c[3]) * scale};
+      } else {
+        constexpr int kN = dims_per_lane(DIM);
+        const std::int8_t* src = A.layer.v + b.at * (kBlk * DIM);
+#pragma unroll
+        for (int n = 0; n < (DIM + 64 * kN - 1) / (64 * kN); ++n) {
+          const int d = (n * 64 + lane) * kN;
+          if (d >= DIM) continue;
+          uint4 c[kN];
+#pragma unroll
+          for (int i = 0; i < kN; ++i) c[i] = *reinterpret_cast<const uint4*>(src + (d + i) * kBlk);
+#pragma unroll
+          for (int r = 0; r < kBlk; ++r) {
+            if (r < lo || r >= hi) continue;
+            float x[kN];
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+              const std::uint32_t four = r < 4 ? c[i].x : r < 8 ? c[i].y : r < 12 ? c[i].z : c[i].w;
+              x[i] = code_value(four, r % 4) * scale;
+            }
+            storen<kN>(rows + static_cast<std::int64_t>(r) * static_cast<std::int64_t>(stride) + d, x);
+          }
+        }
       }
     }
   }
@@ -349,11 +423,27 @@ bool capturing(hipStream_t s) {
   return hipStreamIsCapturing(s, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
 }
 
-unsigned grid_for(std::size_t units) {
-  return static_cast<unsigned>(std::min<std::size_t>(std::max<std::size_t>(ceil_div(units, kWaves), 1), 1u << 20));
+// Workgroups for `units` wavefronts of work; a captured launch, which has
+// room for any batch that its plan takes, fills the chip a few times and
+// goes on from there.
+unsigned grid_for(std::size_t units, bool captured) {
+  return static_cast<unsigned>(std::min<std::size_t>(std::max<std::size_t>(ceil_div(units, kWaves), 1), captured ? 8192 : 1u << 29));
 }
 
-int lanes_per_row(int dim) { return dim <= 32 ? 2 : dim <= 64 ? 4 : dim <= 128 ? 8 : 16; }
+// fn(std::integral_constant<int, head_dim>) for the plan's head size.
+template <typename Fn>
+void with_dim(int dim, Fn&& fn) {
+  switch (dim) {
+    case 32: fn(std::integral_constant<int, 32>{}); break;
+    case 64: fn(std::integral_constant<int, 64>{}); break;
+    case 96: fn(std::integral_constant<int, 96>{}); break;
+    case 128: fn(std::integral_constant<int, 128>{}); break;
+    case 160: fn(std::integral_constant<int, 160>{}); break;
+    case 192: fn(std::integral_constant<int, 192>{}); break;
+    case 224: fn(std::integral_constant<int, 224>{}); break;
+    default: fn(std::integral_constant<int, 256>{}); break;
+  }
+}
 
 std::string check_layer(const llmi_kv8_layer* l, bool open) {
   if (l == nullptr) return "null layer";
@@ -439,7 +529,7 @@ int llmi_hip_kv8_plan_create(const llmi_kv8_shape* shape, size_t max_seqs, size_
   p->g.by_page = divisor(static_cast<std::uint32_t>(p->g.page_blocks));
   p->most = limits(*shape, max_seqs, max_tokens);
   // Kernels count units of work (item and key/value head) in 32 bits.
-  LLMI_REQUIRE(std::max({2 * p->most.append, p->most.few, p->most.many}) * shape->kv_heads <= 0x7FFFFFFFu,
+  LLMI_REQUIRE(std::max({2 * p->most.blocks, p->most.few, p->most.many}) * shape->kv_heads <= 0x7FFFFFFFu,
                "kv8_plan_create: too many sequences and tokens for the heads");
   const auto take = [&](std::size_t bytes) {
     const std::size_t at = p->bytes;
@@ -447,8 +537,8 @@ int llmi_hip_kv8_plan_create(const llmi_kv8_shape* shape, size_t max_seqs, size_
     return at;
   };
   (void)take(sizeof(Counts));
-  p->off_seqs = take(max_seqs * sizeof(Seq));
-  p->off_append = take(p->most.append * sizeof(AppendItem));
+  p->off_positions = take(max_tokens * sizeof(std::int32_t));
+  p->off_blocks = take(p->most.blocks * sizeof(BlockItem));
   p->off_few = take(p->most.few * sizeof(AttnItem));
   p->off_many = take(p->most.many * sizeof(AttnItem));
   p->off_join = take(p->most.join * sizeof(JoinItem));
@@ -473,7 +563,7 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     const std::string why = build(p->shape, seqs, slots, starts, counts, tables, table_stride, p->max_seqs,
                                   p->max_tokens, p->max_pages, &l);
     LLMI_REQUIRE(why.empty(), "kv8_plan_set: " + why);
-    LLMI_REQUIRE(l.append.size() <= p->most.append && l.few.size() <= p->most.few &&
+    LLMI_REQUIRE(l.blocks.size() <= p->most.blocks && l.few.size() <= p->most.few &&
                      l.many.size() <= p->most.many && l.parts <= p->most.parts && l.join.size() <= p->most.join,
                  "kv8_plan_set: more work than the plan was created for");
     if (p->append_captured) {
@@ -482,15 +572,15 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
                    "kv8_plan_set: more positions than the rotation tables of a captured append have");
     }
     LLMI_TRY_HIP(hipEventSynchronize(p->copied));
-    const Counts c{static_cast<std::int32_t>(l.append.size()), static_cast<std::int32_t>(l.tokens),
-                   static_cast<std::int32_t>(l.seqs.size()), static_cast<std::int32_t>(l.few.size()),
+    const Counts c{static_cast<std::int32_t>(l.blocks.size()), static_cast<std::int32_t>(l.tokens),
+                   static_cast<std::int32_t>(l.few.size()),
                    static_cast<std::int32_t>(l.many.size()), static_cast<std::int32_t>(l.join.size())};
     const auto put = [&](std::size_t at, const auto& v) {
       if (!v.empty()) std::memcpy(p->pinned + at, v.data(), v.size() * sizeof(v[0]));
     };
     std::memcpy(p->pinned, &c, sizeof c);
-    put(p->off_seqs, l.seqs);
-    put(p->off_append, l.append);
+    put(p->off_positions, l.positions);
+    put(p->off_blocks, l.blocks);
     put(p->off_few, l.few);
     put(p->off_many, l.many);
     put(p->off_join, l.join);
@@ -540,28 +630,26 @@ int llmi_hip_kv8_append_dev(const llmi_hip_kv8_plan* p, const llmi_kv8_layer* la
   LLMI_REQUIRE(cos_t == nullptr || positions >= p->lists.longest,
                "kv8_append: the rotation tables have fewer positions than the batch");
   if (p->lists.tokens == 0 && !captured) return LLMI_OK;
-  const int lpr = lanes_per_row(g.dim);
-  AppendArgs a{p->view(), g, *layer, q, k, v, q_norm, k_norm, cos_t, sin_t, q_out, q_stride, k_stride, v_stride,
-               q_out_stride, eps, static_cast<int>(p->lists.append.size()), static_cast<int>(p->lists.tokens)};
-  std::size_t blocks = p->lists.append.size(), tokens = p->lists.tokens;
+  std::size_t blocks = p->lists.blocks.size(), tokens = p->lists.tokens;
   if (captured) {
     p->append_captured = true;
     if (cos_t != nullptr) p->captured_positions = std::min(p->captured_positions, positions);
-    a.nappend = a.ntokens = -1;
-    blocks = p->most.append;
+    blocks = p->most.blocks;
     tokens = p->max_tokens;
   }
-  const std::size_t units = 2 * blocks * g.kv_heads + (q != nullptr ? ceil_div(tokens * g.heads * lpr, 64) : 0);
-  const unsigned grid = grid_for(units);
+  // A wavefront takes one group of a token's heads; all of them, with the
+  // norm's and the rotation's factors loaded once, where the groups would be
+  // more than the chip holds wavefronts (8 of 4 SIMDs of 256 compute units).
+  const std::size_t rows = 64 / static_cast<std::size_t>(lanes_per_row(g.dim));
+  const std::size_t groups = ceil_div(static_cast<std::size_t>(g.heads), rows);
+  const std::size_t each = tokens * groups > 8192 ? groups : 1;
+  const std::size_t units = 2 * blocks * g.kv_heads + (q != nullptr ? tokens * ceil_div(groups, each) : 0);
+  LLMI_REQUIRE(units <= 0x7FFFFFFFu, "kv8_append: too many tokens and heads");
+  const AppendArgs a{p->view(), g, *layer, q, k, v, q_norm, k_norm, cos_t, sin_t, q_out, q_stride, k_stride, v_stride,
+                     q_out_stride, eps, captured ? -1 : static_cast<int>(blocks),
+                     captured ? -1 : static_cast<int>(tokens), static_cast<int>(each)};
   hipStream_t s = pick(stream);
-  if (lpr == 2)
-    append_kernel<2><<<grid, kThreads, 0, s>>>(a);
-  else if (lpr == 4)
-    append_kernel<4><<<grid, kThreads, 0, s>>>(a);
-  else if (lpr == 8)
-    append_kernel<8><<<grid, kThreads, 0, s>>>(a);
-  else
-    append_kernel<16><<<grid, kThreads, 0, s>>>(a);
+  with_dim(g.dim, [&](auto dim) { append_kernel<dim><<<grid_for(units, captured), kThreads, 0, s>>>(a); });
   LLMI_TRY_HIP(hipGetLastError());
   return LLMI_OK;
 }
@@ -593,13 +681,12 @@ int llmi_hip_kv8_read_dev(const llmi_hip_kv8_plan* p, const llmi_kv8_layer* laye
                "kv8_read: k_stride or v_stride shorter than a row");
   const bool captured = capturing(pick(stream));
   if ((k == nullptr && v == nullptr) || (p->lists.tokens == 0 && !captured)) return LLMI_OK;
-  ReadArgs a{p->view(), p->g, *layer, k, v, k_stride, v_stride, static_cast<int>(p->lists.append.size())};
-  std::size_t blocks = p->lists.append.size();
-  if (captured) {
-    a.nappend = -1;
-    blocks = p->most.append;
-  }
-  read_kernel<<<grid_for(2 * blocks * p->g.kv_heads), kThreads, 0, pick(stream)>>>(a);
+  const std::size_t blocks = captured ? p->most.blocks : p->lists.blocks.size();
+  const ReadArgs a{p->view(), p->g, *layer, k, v, k_stride, v_stride, captured ? -1 : static_cast<int>(blocks)};
+  hipStream_t s = pick(stream);
+  with_dim(p->g.dim, [&](auto dim) {
+    read_kernel<dim><<<grid_for(2 * blocks * p->g.kv_heads, captured), kThreads, 0, s>>>(a);
+  });
   LLMI_TRY_HIP(hipGetLastError());
   return LLMI_OK;
 }

@@ -9,15 +9,15 @@ namespace llmi_hip::kv8 {
 // Item counts of the batch that is set, in device memory (launches replayed
 // from a graph read them there).
 struct Counts {
-  std::int32_t append, tokens, seqs, few, many, join;
+  std::int32_t blocks, tokens, few, many, join;
 };
 
 // A plan's device lists.
 struct View {
   const Counts* counts;
-  const Seq* seqs;
+  const std::int32_t* positions;
   const std::int32_t* table;
-  const AppendItem* append;
+  const BlockItem* blocks;
   const AttnItem* few;
   const AttnItem* many;
   const JoinItem* join;
@@ -39,12 +39,6 @@ __device__ __forceinline__ int page_of(const Geometry& g, int block) {
 __device__ __forceinline__ std::size_t block_at(const Geometry& g, int id, int page, int block, int h) {
   return (static_cast<std::size_t>(id) * g.kv_heads + h) * g.page_blocks + (block - page * g.page_blocks);
 }
-__device__ __forceinline__ std::size_t block_index(const Geometry& g, const std::int32_t* __restrict__ table,
-                                                   const Seq& s, int block, int h) {
-  const int page = page_of(g, block);
-  return block_at(g, table[s.table + page], page, block, h);
-}
-
 int launch_attention(const llmi_hip_kv8_plan* p, const llmi_kv8_layer& layer, const float* q, std::size_t q_stride,
                      float scale, float* out, std::size_t out_stride, hipStream_t s, bool captured);
 
@@ -58,7 +52,7 @@ struct llmi_hip_kv8_plan {
   // marks the copy's end, before which the pinned side is not written again.
   std::uint8_t* dev = nullptr;
   std::uint8_t* pinned = nullptr;
-  std::size_t bytes = 0, off_seqs = 0, off_table = 0, off_append = 0, off_few = 0, off_many = 0, off_join = 0;
+  std::size_t bytes = 0, off_positions = 0, off_table = 0, off_blocks = 0, off_few = 0, off_many = 0, off_join = 0;
   llmi_hip::kv8::Limits most{};
   float* parts = nullptr;  // the attention's partial states (launches of one plan follow each other)
   hipEvent_t copied = nullptr;
@@ -70,9 +64,9 @@ struct llmi_hip_kv8_plan {
   mutable std::size_t captured_positions = SIZE_MAX;
   llmi_hip::kv8::View view() const {
     using namespace llmi_hip::kv8;
-    return {reinterpret_cast<const Counts*>(dev), reinterpret_cast<const Seq*>(dev + off_seqs),
+    return {reinterpret_cast<const Counts*>(dev), reinterpret_cast<const std::int32_t*>(dev + off_positions),
             reinterpret_cast<const std::int32_t*>(dev + off_table),
-            reinterpret_cast<const AppendItem*>(dev + off_append), reinterpret_cast<const AttnItem*>(dev + off_few),
+            reinterpret_cast<const BlockItem*>(dev + off_blocks), reinterpret_cast<const AttnItem*>(dev + off_few),
             reinterpret_cast<const AttnItem*>(dev + off_many), reinterpret_cast<const JoinItem*>(dev + off_join)};
   }
   ~llmi_hip_kv8_plan();

@@ -22,12 +22,16 @@ struct Seq {
   std::int32_t start, count, row, table, slot;
 };
 
-// One block that an append writes (one wavefront per key/value head for its
-// keys and one for its values).  then >= 0: the same wavefront goes on with
-// block `then` of the sequence, whose new rows replace rows of the open-block
-// store that `block` reads first.
-struct AppendItem {
-  std::int32_t seq, block, then;
+// One block that an append writes or a read returns (one wavefront per
+// key/value head for its keys and one for its values): positions pos .. of the
+// sequence whose tokens are rows row .. (positions start .. end - 1), block
+// `block` of page `page`.  then_pos >= 0: the same wavefront goes on with the
+// block at then_pos, whose new rows replace rows of the open-block store that
+// the first one reads.  keep: rows from this position on go to that store.
+struct BlockItem {
+  std::int32_t row, start, end, slot, keep;
+  std::int32_t pos, page, block;
+  std::int32_t then_pos, then_page, then_block;
 };
 
 // The rows of a sequence for one key/value head are its tokens' query heads
@@ -85,7 +89,8 @@ struct Lists {
   std::size_t parts = 0;       // partial slots of a key/value head
   std::vector<Seq> seqs;
   std::vector<std::int32_t> table;
-  std::vector<AppendItem> append;  // every block that holds a new token
+  std::vector<BlockItem> blocks;       // every block that holds a new token
+  std::vector<std::int32_t> positions; // of every token
   std::size_t tokens = 0, longest = 0;
   bool writable = false;
   std::string why_not;  // why the batch cannot be appended
@@ -115,7 +120,7 @@ inline bool same_shape(const llmi_kv8_shape& a, const llmi_kv8_shape& b) {
 // are its full pieces x heads; rows that are split have at most twice their
 // full pieces; every group of rows adds one item at most.
 struct Limits {
-  std::size_t append, few, many, parts, join;
+  std::size_t blocks, few, many, parts, join;
 };
 inline Limits limits(const llmi_kv8_shape& sh, std::size_t seqs, std::size_t tokens) {
   const std::size_t few = kFewTarget / sh.kv_heads, many = kManyTarget / sh.kv_heads;
@@ -189,9 +194,19 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
     // one wavefront does both, in order.
     std::int32_t then = -1;
     if (q.start % kBlk != 0 && last >= first + 2) then = (last - first) % 2 == 0 ? last : last - 1;
-    const auto seq = static_cast<std::int32_t>(i);
-    for (std::int32_t b = first; b <= last; ++b)
-      if (b != then) l.append.push_back({seq, b, b == first ? then : -1});
+    const std::int32_t per = static_cast<std::int32_t>(sh.page_tokens) / kBlk;
+    const auto page = [&](std::int32_t b) { return l.table[static_cast<std::size_t>(q.table + b / per)]; };
+    for (std::int32_t b = first; b <= last; ++b) {
+      if (b == then) continue;
+      BlockItem it{q.row, q.start, q.start + q.count, q.slot, (last - 1) * kBlk, b * kBlk, page(b), b % per, -1, 0, 0};
+      if (b == first && then >= 0) {
+        it.then_pos = then * kBlk;
+        it.then_page = page(then);
+        it.then_block = then % per;
+      }
+      l.blocks.push_back(it);
+    }
+    for (std::int32_t p = q.start; p < q.start + q.count; ++p) l.positions.push_back(p);
   }
   // Attention: rows are split over their history where the batch alone does
   // not make enough work.

@@ -53,27 +53,35 @@ int main() {
     const std::string why = build(sh, static_cast<std::size_t>(n), slots.data(), starts.data(), counts.data(), tables.data(), stride, 6, 4000, 4000, &l);
     CHECK(why.empty());
     CHECK(l.writable && l.tokens == tokens);
-    std::set<std::pair<int, int>> written;
-    for (const AppendItem& it : l.append) {
-      CHECK(it.seq >= 0 && it.seq < n);
-      const Seq& s = l.seqs[static_cast<std::size_t>(it.seq)];
-      const int last = (s.start + s.count - 1) / kBlk;
-      for (const int b : {it.block, it.then}) {
-        if (b < 0) continue;
-        CHECK(s.count > 0 && b >= s.start / kBlk && b <= last);
-        CHECK(static_cast<std::size_t>(s.table) + static_cast<std::size_t>(b * kBlk) / sh.page_tokens < l.table.size());
-        CHECK(written.insert({it.seq, b}).second);
+    std::set<std::pair<int, int>> written;  // page, block of it
+    std::size_t blocks = 0;
+    for (const BlockItem& it : l.blocks) {
+      std::size_t of = 0;  // the sequence with these tokens
+      while (l.seqs[of].count == 0 || l.seqs[of].row != it.row) ++of;
+      const Seq& s = l.seqs[of];
+      CHECK(it.start == s.start && it.end == s.start + s.count && it.slot == s.slot);
+      const int last = (it.end - 1) / kBlk, per = static_cast<int>(sh.page_tokens) / kBlk;
+      CHECK(it.keep == (last - 1) * kBlk);
+      for (int k = 0; k < 2; ++k) {
+        const int pos = k == 0 ? it.pos : it.then_pos, page = k == 0 ? it.page : it.then_page, block = k == 0 ? it.block : it.then_block;
+        if (pos < 0) continue;
+        CHECK(pos % kBlk == 0 && pos + kBlk > it.start && pos < it.end);
+        CHECK(page == l.table[static_cast<std::size_t>(s.table + pos / kBlk / per)] && block == pos / kBlk % per);
+        CHECK(written.insert({page, block}).second);
+        ++blocks;
       }
       // A block that reads rows of the store, against every other writer of
       // the same rows (blocks last and last - 1, by parity).
-      if (it.block * kBlk < s.start)
+      if (it.pos < s.start)
         for (int b = last - 1; b <= last; ++b)
-          if (b > it.block && b % 2 == it.block % 2) CHECK(it.then == b);
+          if (b > it.pos / kBlk && b % 2 == it.pos / kBlk % 2) CHECK(it.then_pos == b * kBlk);
     }
-    std::size_t blocks = 0;
-    for (const Seq& s : l.seqs)
-      if (s.count > 0) blocks += static_cast<std::size_t>((s.start + s.count - 1) / kBlk - s.start / kBlk + 1);
-    CHECK(written.size() == blocks);
+    std::size_t all = 0;
+    for (const Seq& s : l.seqs) {
+      if (s.count > 0) all += static_cast<std::size_t>((s.start + s.count - 1) / kBlk - s.start / kBlk + 1);
+      for (int i = 0; i < s.count; ++i) CHECK(l.positions.at(static_cast<std::size_t>(s.row + i)) == s.start + i);
+    }
+    CHECK(blocks == all && l.positions.size() == tokens);
     // Attention: every row and position it may see once, each partial state
     // in slots of its own, and within the limits that a plan is created for.
     const std::size_t group = sh.heads / sh.kv_heads;
@@ -113,7 +121,7 @@ int main() {
       for (std::size_t r = 0; r < reach[i].size(); ++r) CHECK(reach[i][r] == l.seqs[i].start + static_cast<long>(r / group) + 1);
     for (const int n_of : slot) CHECK(n_of == 1);
     const Limits m = limits(sh, static_cast<std::size_t>(n), tokens);
-    CHECK(l.append.size() <= m.append && l.few.size() <= m.few && l.many.size() <= m.many);
+    CHECK(l.blocks.size() <= m.blocks && l.few.size() <= m.few && l.many.size() <= m.many);
     CHECK(l.parts <= m.parts && l.join.size() <= m.join);
   }
   for (std::uint32_t d = 1; d <= 4096; ++d) {
