@@ -443,6 +443,33 @@ int llmi_hip_model_forward_cached_trace(llmi_hip_model* model, llmi_hip_cache* c
 int llmi_hip_model_forward(llmi_hip_model* model, const int32_t* tokens, size_t n, int all_positions, float* logits,
                            float* states);
 
+/* Several sequences through the model at once, over a paged 8-bit cache (the
+ * section above): a server's step, with sequences that decode and sequences
+ * whose prompt (or a piece of it) is run side by side.  No counterpart in the
+ * reference, whose server runs one request after the other
+ * (src/server/server.cpp:44-49).
+ * new_kv8_cache allocates every layer's pages: `pages` of page_tokens
+ * positions (a multiple of 16), places for `slots` sequences, steps of at
+ * most max_tokens tokens.  The model's head size must be a multiple of 32 up
+ * to 256.  Which pages a sequence has is the caller's; free the cache before
+ * the model.
+ * forward_kv8: sequence i's counts[i] new tokens (tokens: those of sequence 0,
+ * then 1, ...) at positions starts[i] .., as llmi_hip_kv8_plan_set takes them
+ * and llmi_hip_kv8_check allows them; logits receives vocab floats for the
+ * last new token of each sequence that has any.  The linear layers are the
+ * exact ones; keys and values are held in 8 bits, so logits are not the
+ * reference's: they differ by what rounding them to 1/254 of their block's
+ * largest does.  Errors: LLMI_ERR_ARG for a batch, token id or token count
+ * that is refused (nothing has run then), LLMI_ERR_STATE for a cache of
+ * another model or positions past the context. */
+typedef struct llmi_hip_kv8_cache llmi_hip_kv8_cache;
+int llmi_hip_model_new_kv8_cache(llmi_hip_model* model, size_t pages, size_t page_tokens, size_t slots,
+                                 size_t max_tokens, llmi_hip_kv8_cache** cache);
+int llmi_hip_kv8_cache_free(llmi_hip_kv8_cache* cache);
+int llmi_hip_model_forward_kv8(llmi_hip_model* model, llmi_hip_kv8_cache* cache, size_t seqs, const int32_t* slots,
+                               const int32_t* starts, const int32_t* counts, const int32_t* tables,
+                               size_t table_stride, const int32_t* tokens, float* logits);
+
 /* Transformer::generate_greedy_cached (transformer.cpp:308-327): prefill,
  * then up to max_new greedy tokens (first maximum), stopping after a token in
  * stop_ids.  Writes *n_ids ids to `ids` (room for max_new). */

@@ -27,6 +27,7 @@
 #include <cmath>
 #include <cstring>
 #include <memory>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -1430,6 +1431,14 @@ __global__ void __launch_bounds__(kThreads) silu_inplace(float* __restrict__ x, 
   if (i < n) x[i] = x[i] / (1.0f + exact::expf(-x[i]));
 }
 
+// Rows idx[0..) of x [..][n], one workgroup each.
+__global__ void __launch_bounds__(kThreads) gather_rows(const float* __restrict__ x, const std::int32_t* __restrict__ idx,
+                                                        int n, float* __restrict__ out) {
+  const float* src = x + static_cast<std::size_t>(idx[blockIdx.x]) * n;
+  float* dst = out + static_cast<std::size_t>(blockIdx.x) * n;
+  for (int i = threadIdx.x; i < n; i += kThreads) dst[i] = src[i];
+}
+
 unsigned blocks_for(std::size_t n) { return static_cast<unsigned>(ceil_div(n, kThreads)); }
 
 }  // namespace
@@ -1515,6 +1524,27 @@ struct llmi_hip_cache {
   float* v = nullptr;
   float* scores = nullptr;  // [head][cap], decode attention scratch
   std::size_t kv_elems = 0, score_elems = 0;  // allocated floats of k (= v) and scores
+};
+
+// A model's paged 8-bit cache: every layer's pages (llmi_kv8_layer, one
+// allocation of each kind, layer after layer) and the plan of its batches.
+struct llmi_hip_kv8_cache {
+  const llmi_hip_model* model = nullptr;
+  llmi_kv8_shape shape{};
+  std::size_t max_tokens = 0, code_bytes = 0, scale_floats = 0, open_floats = 0;
+  std::int8_t *k = nullptr, *v = nullptr;
+  float *scales = nullptr, *open = nullptr;
+  std::int32_t* rows = nullptr;  // the last token's row of each sequence of a step
+  llmi_hip_kv8_plan* plan = nullptr;
+  ~llmi_hip_kv8_cache() {
+    (void)llmi_hip_kv8_plan_free(plan);
+    for (void* p : {static_cast<void*>(k), static_cast<void*>(v), static_cast<void*>(scales), static_cast<void*>(open),
+                    static_cast<void*>(rows)})
+      if (p != nullptr) (void)hipFree(p);
+  }
+  llmi_kv8_layer layer(std::size_t i) const {
+    return {k + i * code_bytes, v + i * code_bytes, scales + i * scale_floats, open + i * open_floats};
+  }
 };
 
 namespace llmi_hip {
@@ -2130,6 +2160,50 @@ int validate(llmi_hip_model* m, llmi_hip_cache* cache, const std::int32_t* token
   return LLMI_OK;
 }
 
+// One step of a ragged batch over a paged 8-bit cache whose plan is set: T
+// tokens (ids in ws.ids), the rows of c->rows[0..nrows) through the lm_head,
+// logits from ws.logits row 0.  The linear layers are forward_rows' exact
+// ones; the cache and the attention are llmi_hip_kv8_append_dev / _attention_dev.
+int forward_kv8_rows(llmi_hip_model* m, const llmi_hip_kv8_cache* kv, std::size_t T, std::size_t nrows, hipStream_t s) {
+  const auto& c = m->c;
+  Workspace& w = m->ws;
+  const float eps = static_cast<float>(c.rms_norm_eps);
+  const float scale = 1.0F / std::sqrt(static_cast<float>(m->hd));
+  const unsigned tt = static_cast<unsigned>(T);
+  if (int rc = launch_dequantize_rows(m->embed, w.ids, T, w.x, s)) return rc;
+  for (std::size_t li = 0; li < m->layers.size(); ++li) {
+    const DeviceLayer& l = m->layers[li];
+    const llmi_kv8_layer layer = kv->layer(li);
+    rmsnorm_rows<<<tt, kThreads, 0, s>>>(w.x, l.attn_norm, w.h, static_cast<int>(m->H), eps);
+    const DeviceMatrix* qkv[3] = {&l.wq, &l.wk, &l.wv};
+    const float* qkv_bias[3] = {l.bq, l.bk, l.bv};
+    float* qkv_out[3] = {w.q, w.k, w.v};
+    if (int rc = launch_matmul_shared(qkv, qkv_bias, qkv_out, 3, w.h, T, s)) return rc;
+    if (int rc = llmi_hip_kv8_append_dev(kv->plan, &layer, w.q, m->Q, w.k, m->KV, w.v, m->KV, nullptr, nullptr, 0.0f,
+                                         m->cos_t, m->sin_t, m->table_len, w.q, m->Q, s))
+      return rc;
+    if (int rc = llmi_hip_kv8_attention_dev(kv->plan, &layer, w.q, m->Q, scale, w.att, m->Q, s)) return rc;
+    if (int rc = launch_matmul(l.wo, w.att, T, nullptr, w.x, s, true)) return rc;
+    rmsnorm_rows<<<tt, kThreads, 0, s>>>(w.x, l.mlp_norm, w.h, static_cast<int>(m->H), eps);
+    bool fused = false;
+    if (int rc = launch_gate_up_silu(l.gate, l.up, w.h, T, w.g, s, &fused)) return rc;
+    if (!fused) {
+      const DeviceMatrix* gu[2] = {&l.gate, &l.up};
+      const float* gu_bias[2] = {nullptr, nullptr};
+      float* gu_out[2] = {w.g, w.u};
+      if (int rc = launch_matmul_shared(gu, gu_bias, gu_out, 2, w.h, T, s)) return rc;
+      silu_mul<<<blocks_for(T * m->F), kThreads, 0, s>>>(w.g, w.u, T * m->F);
+    }
+    if (int rc = launch_matmul(l.down, w.g, T, nullptr, w.x, s, true)) return rc;
+  }
+  gather_rows<<<static_cast<unsigned>(nrows), kThreads, 0, s>>>(w.x, kv->rows, static_cast<int>(m->H), w.att);
+  rmsnorm_rows<<<static_cast<unsigned>(nrows), kThreads, 0, s>>>(w.att, m->final_norm, w.h, static_cast<int>(m->H), eps);
+  const DeviceMatrix& head = m->tied ? m->embed : m->lm_head;
+  if (int rc = launch_matmul(head, w.h, nrows, nullptr, w.logits, s)) return rc;
+  LLMI_TRY_HIP(hipGetLastError());
+  return LLMI_OK;
+}
+
 }  // namespace
 }  // namespace llmi_hip
 
@@ -2276,6 +2350,81 @@ int llmi_hip_model_forward(llmi_hip_model* m, const int32_t* tokens, size_t n, i
 int llmi_hip_model_forward_cached(llmi_hip_model* m, llmi_hip_cache* cache, const int32_t* tokens, size_t n,
                                   int all_positions, float* logits) {
   return llmi_hip_model_forward_cached_trace(m, cache, tokens, n, all_positions, logits, nullptr);
+}
+
+int llmi_hip_model_new_kv8_cache(llmi_hip_model* m, size_t pages, size_t page_tokens, size_t slots, size_t max_tokens,
+                                 llmi_hip_kv8_cache** cache) {
+  LLMI_REQUIRE_INIT();
+  LLMI_REQUIRE(m != nullptr && cache != nullptr, "new_kv8_cache: null pointer");
+  *cache = nullptr;
+  LLMI_REQUIRE(pages <= 0x7FFFFFFFu && page_tokens <= 65536 && slots <= (1u << 20),
+               "new_kv8_cache: pages below 2^31, page_tokens up to 65536, slots up to 2^20");
+  std::unique_ptr<llmi_hip_kv8_cache> c(new (std::nothrow) llmi_hip_kv8_cache);
+  if (c == nullptr) return fail(LLMI_ERR_HIP, "new_kv8_cache: out of host memory");
+  c->model = m;
+  c->max_tokens = max_tokens;
+  c->shape = {m->c.num_heads, m->c.num_kv_heads, static_cast<std::uint32_t>(m->hd),
+              static_cast<std::uint32_t>(page_tokens), static_cast<std::uint32_t>(pages),
+              static_cast<std::uint32_t>(slots)};
+  if (int rc = llmi_hip_kv8_sizes(&c->shape, &c->code_bytes, &c->scale_floats, &c->open_floats)) return rc;
+  c->scale_floats = ceil_div(c->scale_floats, 4) * 4;  // each layer's on 16 bytes
+  // Sequences may share pages, so their tables together may have more entries than there are pages.
+  const std::size_t entries = slots * ceil_div(m->c.max_position_embeddings, page_tokens);
+  if (int rc = llmi_hip_kv8_plan_create(&c->shape, slots, max_tokens, std::min<std::size_t>(entries, 1u << 28), &c->plan))
+    return rc;
+  const std::size_t n = m->layers.size();
+  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&c->k), n * c->code_bytes));
+  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&c->v), n * c->code_bytes));
+  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&c->scales), n * c->scale_floats * sizeof(float)));
+  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&c->open), n * c->open_floats * sizeof(float)));
+  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&c->rows), slots * sizeof(std::int32_t)));
+  *cache = c.release();
+  return LLMI_OK;
+}
+
+int llmi_hip_kv8_cache_free(llmi_hip_kv8_cache* c) {
+  delete c;  // the plan's release waits for the device
+  return LLMI_OK;
+}
+
+int llmi_hip_model_forward_kv8(llmi_hip_model* m, llmi_hip_kv8_cache* c, size_t seqs, const int32_t* slots,
+                               const int32_t* starts, const int32_t* counts, const int32_t* tables,
+                               size_t table_stride, const int32_t* tokens, float* logits) {
+  LLMI_REQUIRE_INIT();
+  LLMI_REQUIRE(m != nullptr, "forward_kv8: null model");
+  if (c == nullptr || c->model != m) return fail(LLMI_ERR_STATE, "forward_kv8: cache was not created by this model");
+  if (int rc = llmi_hip_kv8_check(&c->shape, seqs, slots, starts, counts, tables, table_stride)) return rc;
+  try {
+    std::vector<std::int32_t> last;
+    std::size_t T = 0, longest = 0;
+    for (std::size_t i = 0; i < seqs; ++i) {
+      const std::size_t len = static_cast<std::size_t>(starts[i]) + static_cast<std::size_t>(counts[i]);
+      if (len > m->c.max_position_embeddings)
+        return fail(LLMI_ERR_STATE, "forward_kv8: sequence longer than the model's context");
+      T += static_cast<std::size_t>(counts[i]);
+      longest = std::max(longest, len);
+      if (counts[i] > 0) last.push_back(static_cast<std::int32_t>(T) - 1);
+    }
+    if (T == 0) return fail(LLMI_ERR_ARG, "forward_kv8: no tokens");
+    LLMI_REQUIRE(T <= c->max_tokens, "forward_kv8: more tokens than the cache was created for");
+    LLMI_REQUIRE(tokens != nullptr, "forward_kv8: null tokens");
+    for (std::size_t t = 0; t < T; ++t)
+      if (tokens[t] < 0 || static_cast<std::size_t>(tokens[t]) >= m->V)
+        return fail(LLMI_ERR_ARG, "forward_kv8: token id " + std::to_string(tokens[t]) + " out of range");
+    if (int rc = ensure_tables(m, longest)) return rc;
+    if (int rc = ensure_workspace(m, T)) return rc;
+    hipStream_t s = library_stream();
+    if (int rc = llmi_hip_kv8_plan_set(c->plan, seqs, slots, starts, counts, tables, table_stride, s)) return rc;
+    LLMI_TRY_HIP(hipMemcpyAsync(m->ws.ids, tokens, T * sizeof(std::int32_t), hipMemcpyHostToDevice, s));
+    LLMI_TRY_HIP(hipMemcpyAsync(c->rows, last.data(), last.size() * sizeof(std::int32_t), hipMemcpyHostToDevice, s));
+    if (int rc = forward_kv8_rows(m, c, T, last.size(), s)) return rc;
+    if (logits != nullptr)
+      LLMI_TRY_HIP(hipMemcpyAsync(logits, m->ws.logits, last.size() * m->V * sizeof(float), hipMemcpyDeviceToHost, s));
+    LLMI_TRY_HIP(hipStreamSynchronize(s));
+    return LLMI_OK;
+  } catch (const std::bad_alloc&) {
+    return fail(LLMI_ERR_HIP, "forward_kv8: out of host memory");
+  }
 }
 
 // transformer.cpp:308-327: prefill once, then one token per step; the argmax

@@ -99,6 +99,9 @@ SIGNATURES = {
     "llmi_hip_model_forward_cached": (_i, [_vp, _vp, _vp, _sz, _i, _vp]),
     "llmi_hip_model_forward_cached_trace": (_i, [_vp, _vp, _vp, _sz, _i, _vp, _vp]),
     "llmi_hip_model_forward": (_i, [_vp, _vp, _sz, _i, _vp, _vp]),
+    "llmi_hip_model_new_kv8_cache": (_i, [_vp, _sz, _sz, _sz, _sz, C.POINTER(_vp)]),
+    "llmi_hip_kv8_cache_free": (_i, [_vp]),
+    "llmi_hip_model_forward_kv8": (_i, [_vp, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
     "llmi_hip_matmul_mfma_noalloc_dev": (_i, [_vp, _vp, _sz, _vp, _vp, _vp]),
     "llmi_hip_model_generate_greedy": (_i, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, C.POINTER(_sz)]),
     "llmi_hip_model_last_timing": (_i, [_vp, C.POINTER(_d), C.POINTER(_d)]),
@@ -421,6 +424,28 @@ class Cache:
             pass
 
 
+class Kv8Cache:
+    """A model's paged 8-bit cache (llmi_hip_kv8_cache)."""
+
+    def __init__(self, model: "Model", pages: int, page_tokens: int, slots: int, max_tokens: int):
+        self.lib = model.lib
+        self.h = None
+        h = C.c_void_p()
+        check(self.lib.llmi_hip_model_new_kv8_cache(model.h, pages, page_tokens, slots, max_tokens, C.byref(h)))
+        self.h = h.value
+
+    def free(self) -> None:
+        if self.h:
+            check(self.lib.llmi_hip_kv8_cache_free(self.h))
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
 class Model:
     """A device-resident quantized decoder (llmi_hip_model)."""
 
@@ -452,6 +477,20 @@ class Model:
         logits = np.zeros(max(rows, 1) * self.cfg["vocab_size"], dtype=np.float32)
         check(self.lib.llmi_hip_model_forward_cached(self.h, cache.h, _p(toks), toks.size, int(all_positions),
                                                      _p(logits)))
+        return logits
+
+    def new_kv8_cache(self, pages: int, page_tokens: int, slots: int, max_tokens: int) -> Kv8Cache:
+        return Kv8Cache(self, pages, page_tokens, slots, max_tokens)
+
+    def forward_kv8(self, cache: Kv8Cache, slots, starts, counts, tables, tokens) -> np.ndarray:
+        """One step of a ragged batch: logits [sequences with new tokens][vocab] (llmi_hip.h)."""
+        s, a, c, t, stride = _batch(slots, starts, counts, tables)
+        toks = np.ascontiguousarray(tokens, dtype=np.int32)
+        if toks.size != int(c.sum()):
+            raise ValueError("tokens must have as many entries as counts sum to")
+        logits = np.zeros((int((c > 0).sum()), self.cfg["vocab_size"]), dtype=np.float32)
+        check(self.lib.llmi_hip_model_forward_kv8(self.h, cache.h, len(a), _p(s), _p(a), _p(c), _p(t), stride,
+                                                  _p(toks), _p(logits)))
         return logits
 
     def forward_cached_trace(self, cache: Cache, tokens, all_positions: bool = False):
