@@ -337,7 +337,10 @@ int llmi_hip_kv8_sizes(const llmi_kv8_shape* shape, size_t* code_bytes, size_t* 
  * batch is set when they are replayed, in buffers with room for its tokens
  * (plan_set itself is not captured: LLMI_ERR_STATE; after a captured append
  * it takes only batches that can be appended, within that call's rotation
- * tables).  Launches of one plan must not overlap; two streams or two graphs
+ * tables; after a captured attention only batches with work of the kinds that
+ * it was captured for: single tokens or drafts of up to as many rows (tokens
+ * x heads / kv_heads, up to 64 a sequence) as were set then, and longer pieces
+ * if there were any; a graph captured with an empty batch serves every kind).  Launches of one plan must not overlap; two streams or two graphs
  * that run at once need a plan each.
  * Refused (LLMI_ERR_ARG): a slot or page out of range, a negative start or
  * count, a table too short, more than the plan was created for.

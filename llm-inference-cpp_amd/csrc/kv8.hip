@@ -566,6 +566,8 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     LLMI_REQUIRE(l.blocks.size() <= p->most.blocks && l.few.size() <= p->most.few &&
                      l.many.size() <= p->most.many && l.parts <= p->most.parts && l.join.size() <= p->most.join,
                  "kv8_plan_set: more work than the plan was created for");
+    LLMI_REQUIRE(l.few_rows <= p->captured_few && (l.many.empty() || p->captured_many),
+                 "kv8_plan_set: more tokens of a sequence than an attention of this plan was captured for");
     if (p->append_captured) {
       LLMI_REQUIRE(l.writable, "kv8_plan_set: an append of this plan was captured, and " + l.why_not);
       LLMI_REQUIRE(l.longest <= p->captured_positions,
@@ -574,7 +576,8 @@ int llmi_hip_kv8_plan_set(llmi_hip_kv8_plan* p, size_t seqs, const int32_t* slot
     LLMI_TRY_HIP(hipEventSynchronize(p->copied));
     const Counts c{static_cast<std::int32_t>(l.blocks.size()), static_cast<std::int32_t>(l.tokens),
                    static_cast<std::int32_t>(l.few.size()),
-                   static_cast<std::int32_t>(l.many.size()), static_cast<std::int32_t>(l.join.size())};
+                   static_cast<std::int32_t>(l.many.size()), static_cast<std::int32_t>(l.join.size()),
+                   l.join_rows, l.join_at};
     const auto put = [&](std::size_t at, const auto& v) {
       if (!v.empty()) std::memcpy(p->pinned + at, v.data(), v.size() * sizeof(v[0]));
     };

@@ -9,7 +9,7 @@ namespace llmi_hip::kv8 {
 // Item counts of the batch that is set, in device memory (launches replayed
 // from a graph read them there).
 struct Counts {
-  std::int32_t blocks, tokens, few, many, join;
+  std::int32_t blocks, tokens, few, many, join, join_rows, join_at;
 };
 
 // A plan's device lists.
@@ -59,9 +59,12 @@ struct llmi_hip_kv8_plan {
   bool set = false;
   llmi_hip::kv8::Lists lists;
   // What captured launches ask of every batch set later: appends were
-  // captured, with rotation tables of this many positions.
+  // captured, with rotation tables of this many positions; attention was, for
+  // `few` items of this many rows, with or without `many` items.
   mutable bool append_captured = false;
   mutable std::size_t captured_positions = SIZE_MAX;
+  mutable std::int32_t captured_few = 0x7FFFFFFF;
+  mutable bool captured_many = true;
   llmi_hip::kv8::View view() const {
     using namespace llmi_hip::kv8;
     return {reinterpret_cast<const Counts*>(dev), reinterpret_cast<const std::int32_t*>(dev + off_positions),

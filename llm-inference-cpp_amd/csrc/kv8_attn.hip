@@ -43,13 +43,14 @@ __device__ __forceinline__ std::size_t part_row(const AttnArgs& A, int part, int
 // workgroup takes `at` rows of one head; a thread four dims of a row over
 // every `share`-th piece, eight loads of each kind in flight (what bounds
 // this is their latency), with the running maximum; the shares meet in LDS.
-constexpr int kJoinThreads = 256;
-__global__ void __launch_bounds__(kJoinThreads) attention_join(AttnArgs A, int at, int chunks) {
+__global__ void __launch_bounds__(kJoinThreads) attention_join(AttnArgs A, int join_rows, int join_at) {
   __shared__ float2 sh_state[kJoinThreads];
   __shared__ float4 sh_o[kJoinThreads];
+  const int njoin = A.njoin >= 0 ? A.njoin : A.v.counts->join;
+  const int at = A.njoin >= 0 ? join_at : A.v.counts->join_at;
+  const int chunks = ((A.njoin >= 0 ? join_rows : A.v.counts->join_rows) + at - 1) / at;
   const int quads = A.g.dim / 4, cells = at * quads, share = kJoinThreads / cells;
   const int mine = static_cast<int>(threadIdx.x) % cells, of = static_cast<int>(threadIdx.x) / cells;
-  const int njoin = A.njoin >= 0 ? A.njoin : A.v.counts->join;
   const int units = njoin * A.g.kv_heads * chunks;
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     const int item = u / (A.g.kv_heads * chunks), rest = u - item * A.g.kv_heads * chunks;
@@ -782,14 +783,24 @@ int launch_attention(const llmi_hip_kv8_plan* p, const llmi_kv8_layer& layer, co
              part_rows * static_cast<std::size_t>(p->g.dim), scale, captured ? -1 : static_cast<int>(l.few.size()),
              captured ? -1 : static_cast<int>(l.many.size()),
              captured ? -1 : static_cast<int>(l.join.size())};
-  // Captured: room for any batch that the plan takes, but no more workgroups
-  // than fill the chip several times (each takes further units in turn).
-  const auto grid = [&](std::size_t items, std::size_t most) {
-    const std::size_t units = (captured ? most : items) * static_cast<std::size_t>(p->g.kv_heads);
+  // A captured launch has the kernels that the batch needs (an empty one:
+  // every kind), each with room for any batch that the plan takes, but no more
+  // workgroups than fill the chip several times (each takes further units in
+  // turn).  Batches of other kinds are refused from then on.
+  const bool any = captured && l.tokens == 0;
+  const bool has_few = any || !l.few.empty(), has_many = any || !l.many.empty();
+  const int most_rows = few_rows(p->g.dim);
+  const int rows = any ? most_rows : captured ? std::min((l.few_rows + 3) / 4 * 4, most_rows) : l.few_rows;
+  if (captured) {
+    p->captured_few = std::min(p->captured_few, has_few ? rows : 0);
+    p->captured_many = p->captured_many && has_many;
+  }
+  const auto grid = [&](bool has, std::size_t items, std::size_t most) {
+    if (!has) return 0u;
+    const std::size_t units = (captured ? most : items) * heads;
     return static_cast<unsigned>(std::min<std::size_t>(units, captured ? 4096 : 1u << 30));
   };
-  const unsigned few = grid(l.few.size(), p->most.few), many = grid(l.many.size(), p->most.many);
-  const int rows = captured ? few_rows(p->g.dim) : l.few_rows;
+  const unsigned few = grid(has_few, l.few.size(), p->most.few), many = grid(has_many, l.many.size(), p->most.many);
   switch (p->g.dim) {
     case 32: launch<32>(a, few, many, rows, s); break;
     case 64: launch<64>(a, few, many, rows, s); break;
@@ -801,15 +812,9 @@ int launch_attention(const llmi_hip_kv8_plan* p, const llmi_kv8_layer& layer, co
     default: launch<256>(a, few, many, rows, s); break;
   }
   if (captured || !l.join.empty()) {
-    // One row a workgroup where rows are few (and pieces many), up to as many
-    // as its threads hold where they are enough to fill the chip.
-    const std::size_t items = captured ? p->most.join : l.join.size();
-    const int most = captured ? kManyRows : l.join_rows;
-    const int at = items * heads * most <= 2048 ? 1 : kJoinThreads / (p->g.dim / 4);
-    const int chunks = (most + at - 1) / at;
-    const std::size_t units = items * heads * static_cast<std::size_t>(chunks);
-    attention_join<<<static_cast<unsigned>(std::min<std::size_t>(units, captured ? 4096 : 1u << 30)), kJoinThreads, 0,
-                     s>>>(a, at, chunks);
+    const std::size_t chunks = (l.join_rows + l.join_at - 1) / l.join_at;
+    const std::size_t units = captured ? 4096 : l.join.size() * heads * chunks;
+    attention_join<<<static_cast<unsigned>(units), kJoinThreads, 0, s>>>(a, l.join_rows, l.join_at);
   }
   LLMI_TRY_HIP(hipGetLastError());
   return LLMI_OK;

@@ -67,6 +67,9 @@ struct JoinItem {
 constexpr std::size_t kFewTarget = 512, kFewLeast = 8 * kTile, kFewWhole = 24 * kTile;
 constexpr std::size_t kManyTarget = 768, kManyLeast = 4 * kTile;
 
+constexpr std::size_t kJoinFill = 2048;  // rows of all heads that fill the chip with a workgroup each
+constexpr int kJoinThreads = 256;
+
 // block / d for block < 2^27 (positions below 2^31) and d = the blocks of a
 // page, at most 4096: (block * m) >> k with m = 2^k / d + 1, k = 27 + ceil(log2 d):
 // m * d exceeds 2^k by at most d <= 2^(k - 27), so the product's excess over
@@ -85,7 +88,11 @@ struct Lists {
   std::vector<AttnItem> few, many;
   std::vector<JoinItem> join;
   std::int32_t few_rows = 0;  // most rows of a `few` item
+  // A workgroup that joins takes join_at rows of an item at a time: one where
+  // rows are few (and pieces many), up to as many as its threads hold where
+  // they are enough to fill the chip.
   std::int32_t join_rows = 0;  // most rows of a `join` item
+  std::int32_t join_at = 1;
   std::size_t parts = 0;       // partial slots of a key/value head
   std::vector<Seq> seqs;
   std::vector<std::int32_t> table;
@@ -107,6 +114,11 @@ inline std::string check_shape(const llmi_kv8_shape* s) {
     return "page_tokens must be a multiple of 16 up to 65536";
   if (s->pages == 0 || s->pages > 0x7FFFFFFFu) return "pages must be positive and below 2^31";
   if (s->slots == 0 || s->slots > 0x7FFFFFFFu) return "slots must be positive and below 2^31";
+  // Sizes and offsets in bytes stay far from 64 bits.
+  constexpr std::uint64_t kMost = std::uint64_t{1} << 48;
+  const std::uint64_t position = std::uint64_t{s->kv_heads} * s->head_dim;  // at most 2^20
+  if (position * s->page_tokens > kMost / s->pages || position * kBlk * 16 > kMost / s->slots)
+    return "the cache would be larger than 2^48 bytes";
   return {};
 }
 
@@ -123,8 +135,9 @@ struct Limits {
   std::size_t blocks, few, many, parts, join;
 };
 inline Limits limits(const llmi_kv8_shape& sh, std::size_t seqs, std::size_t tokens) {
-  const std::size_t few = kFewTarget / sh.kv_heads, many = kManyTarget / sh.kv_heads;
   const std::size_t busy = std::min(seqs, tokens), group = sh.heads / sh.kv_heads;
+  const std::size_t few = kFewTarget / sh.kv_heads;
+  const std::size_t many = tokens * group > kFewMax ? kManyTarget / sh.kv_heads : 0;
   const std::size_t rows = static_cast<std::size_t>(few_rows(static_cast<int>(sh.head_dim)));
   return {tokens / kBlk + 2 * busy, few + kFewMax / rows * busy, many + tokens * group / kManyRows + busy,
           2 * few * (rows / kSlotRows) + 2 * many * (kManyRows / kSlotRows), few + many};
@@ -167,18 +180,24 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
   l.writable = slots != nullptr || seqs == 0;
   if (!l.writable) l.why_not = "the batch was set without slots";
   if (l.writable) {
-    std::vector<std::uint8_t> uses(sh.pages, 0), held(sh.slots, 0);
-    for (const std::int32_t p : l.table) uses[static_cast<std::size_t>(p)] += uses[static_cast<std::size_t>(p)] < 2;
+    // A bit per page that appears, and that appears again; one per slot in use.
+    std::vector<bool> once(sh.pages), again(sh.pages), held(sh.slots);
+    for (const std::int32_t p : l.table) {
+      if (once[static_cast<std::size_t>(p)]) again[static_cast<std::size_t>(p)] = true;
+      once[static_cast<std::size_t>(p)] = true;
+    }
     for (const Seq& q : l.seqs) {
       if (q.count == 0) continue;
-      if (held[static_cast<std::size_t>(q.slot)]++) {
+      const bool taken = held[static_cast<std::size_t>(q.slot)];
+      held[static_cast<std::size_t>(q.slot)] = true;
+      if (taken) {
         l.writable = false;
         l.why_not = "two sequences with new tokens have the same slot";
         break;
       }
       const std::int32_t page = static_cast<std::int32_t>(sh.page_tokens);
       for (std::int32_t p = q.start / page; p <= (q.start + q.count - 1) / page && l.writable; ++p)
-        if (uses[static_cast<std::size_t>(l.table[static_cast<std::size_t>(q.table + p)])] > 1) {
+        if (again[static_cast<std::size_t>(l.table[static_cast<std::size_t>(q.table + p)])]) {
           l.writable = false;
           l.why_not = "a page that takes new tokens appears twice in the batch";
         }
@@ -263,6 +282,8 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
   std::stable_sort(l.few.begin(), l.few.end(), longer);
   std::stable_sort(l.many.begin(), l.many.end(), longer);
   for (const AttnItem& it : l.few) l.few_rows = std::max(l.few_rows, it.rows);
+  if (l.join.size() * sh.kv_heads * static_cast<std::size_t>(l.join_rows) > kJoinFill)
+    l.join_at = kJoinThreads * 4 / static_cast<std::int32_t>(sh.head_dim);
   return {};
 }
 

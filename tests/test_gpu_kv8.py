@@ -400,6 +400,44 @@ def test_decode_steps_replayed_from_a_graph():
         assert np.array_equal(a.download(np.uint8), b.download(np.uint8))
 
 
+@pytest.mark.parametrize("empty", [True, False])
+def test_every_kind_of_batch_from_one_graph(empty):
+    """A graph captured with an empty batch (or with drafts and a prompt)
+    replayed for single tokens, drafts, prompts and mixtures, long and short,
+    against eager calls; one captured for single tokens refuses a prompt."""
+    rng = np.random.default_rng(21)
+    heads, kv, dim, page, n = 8, 2, 64, 32, 3
+    pool = Pool(rng, heads, kv, dim, page, [2600, 700, 300])
+    k, v = rows_of(rng, 3600, kv, dim), rows_of(rng, 3600, kv, dim)
+    pool.append([0, 0, 0], [2600, 700, 300], None, k, v)
+    plan = H.Kv8Plan(pool.shape, n, 400, pool.tables.size)
+    qb, ob = (H.DeviceBuffer(400 * heads * dim * 4) for _ in range(2))
+    plan.set(pool.slots, [0] * n, [0, 0, 0] if empty else [4, 60, 0], pool.tables)
+    H.synchronize()
+    graph = H.Graph(lambda: plan.attention(pool.layer, qb.ptr, 0.125, ob.ptr))
+    for starts, counts in (([2599, 699, 299], [1, 1, 1]), ([2590, 0, 0], [3, 0, 4]), ([100, 600, 0], [200, 100, 100]), ([2300, 0, 17], [300, 1, 2]), ([5, 6, 7], [1, 0, 0])):
+        q = rows_of(rng, sum(counts), heads, dim)
+        want = pool.attention(starts, counts, q, 0.125)
+        plan.set(pool.slots, starts, counts, pool.tables)
+        for _ in range(2):  # the second replay on the same batch
+            qb.upload(q)
+            ob.upload(np.full(400 * heads * dim, 5.0, np.float32))
+            graph.launch()
+            H.synchronize()
+            got = ob.download(np.float32).reshape(400, heads, dim)
+            assert np.array_equal(got[:len(q)], want) and (got[len(q):] == 5.0).all()
+    one = H.Kv8Plan(pool.shape, n, 400, pool.tables.size)
+    one.set(pool.slots, [9] * n, [1] * n, pool.tables)
+    H.synchronize()
+    single = H.Graph(lambda: one.attention(pool.layer, qb.ptr, 0.125, ob.ptr))
+    for counts in ([2, 1, 1], [100, 1, 1]):
+        with pytest.raises(H.HipError, match="captured for"):
+            one.set(pool.slots, [9] * n, counts, pool.tables)
+    one.set(pool.slots, [2000, 30, 9], [1, 0, 1], pool.tables)
+    single.launch()
+    H.synchronize()
+
+
 def new_stream():
     """A stream of the HIP runtime that the library is linked with."""
     import ctypes as C

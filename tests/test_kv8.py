@@ -26,6 +26,7 @@ def test_sizes():
     (dict(heads=5), "multiple of kv_heads"), (dict(heads=0), "multiple of kv_heads"), (dict(kv_heads=0), "multiple of kv_heads"),
     (dict(heads=4098), "4096"), (dict(head_dim=48), "head_dim"), (dict(head_dim=0), "head_dim"), (dict(head_dim=288), "head_dim"),
     (dict(page_tokens=0), "page_tokens"), (dict(page_tokens=24), "page_tokens"), (dict(page_tokens=1 << 17), "page_tokens"),
+    (dict(pages=1 << 30, page_tokens=65536, kv_heads=4, head_dim=256), "2\\^48"), (dict(slots=1 << 30, kv_heads=4096, heads=4096), "2\\^48"),
     (dict(pages=0), "pages"), (dict(pages=1 << 31), "pages"), (dict(slots=0), "slots"), (dict(slots=1 << 31), "slots"),
 ])
 def test_shapes_refused(kw, why):
