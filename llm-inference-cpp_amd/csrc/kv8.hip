@@ -30,9 +30,16 @@ __device__ __forceinline__ void store8(float* p, const float* x) {
 // every finite one, so that the largest of a block shows them.
 __device__ __forceinline__ std::uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 __device__ __forceinline__ std::uint32_t wave_umax(std::uint32_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(v), o, 64)));
-  return v;
+  const auto ror = [](std::uint32_t x, auto ctrl) {  // within the 16 lanes of a row
+    return static_cast<std::uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x120 + decltype(ctrl)::value, 0xF, 0xF, false));
+  };
+  v = max(v, ror(v, std::integral_constant<int, 8>{}));
+  v = max(v, ror(v, std::integral_constant<int, 4>{}));
+  v = max(v, ror(v, std::integral_constant<int, 2>{}));
+  v = max(v, ror(v, std::integral_constant<int, 1>{}));
+  const auto row = [&](int lane) { return static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane)); };
+  return max(max(row(0), row(16)), max(row(32), row(48)));
 }
 // A block's scale, float(amax / 127) with one rounding (NaN and inf stay what
 // they are), and what its codes are computed with.
@@ -162,24 +169,32 @@ __device__ void append_keys(const AppendArgs& A, const BlockItem& it, int h, con
       load8(src + kHalf + 8 * c, x[p] + 8);
     }
   }
-  float w[16] = {};
-  if (A.k_norm != nullptr && chunk) {
-    load8(A.k_norm + 8 * c, w);
-    load8(A.k_norm + kHalf + 8 * c, w + 8);
+  // (Every lane loads: one without a row of its own the first token's.)
+  float w[16] = {}, co[kPasses][8] = {}, si[kPasses][8] = {};
+  const int c_in = chunk ? c : 0;
+  if (A.k_norm != nullptr) {
+    load8(A.k_norm + 8 * c_in, w);
+    load8(A.k_norm + kHalf + 8 * c_in, w + 8);
+  }
+  if (A.cos_t != nullptr) {
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int pos = b.pos + p * kRows + lane / kLpr;
+      const std::size_t at =
+          static_cast<std::size_t>(pos >= it.start && pos < it.end ? pos : it.start) * kHalf + 8 * c_in;
+      load8(A.cos_t + at, co[p]);
+      load8(A.sin_t + at, si[p]);
+    }
   }
   std::uint32_t amax = 0;
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
     const int tok = p * kRows + lane / kLpr, pos = b.pos + tok;
     const bool fresh = chunk && tok < kBlk && pos >= it.start && pos < it.end;
-    float y[16], co[8] = {}, si[8] = {};
+    float y[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) y[i] = x[p][i];
-    if (A.cos_t != nullptr && fresh) {
-      load8(A.cos_t + static_cast<std::size_t>(pos) * kHalf + 8 * c, co);
-      load8(A.sin_t + static_cast<std::size_t>(pos) * kHalf + 8 * c, si);
-    }
-    norm_rotate<DIM>(y, fresh, A.k_norm != nullptr, w, A.eps, A.cos_t != nullptr, co, si);
+    norm_rotate<DIM>(y, fresh, A.k_norm != nullptr, w, A.eps, A.cos_t != nullptr, co[p], si[p]);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       if (fresh) x[p][i] = y[i];
