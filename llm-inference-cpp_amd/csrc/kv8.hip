@@ -77,8 +77,8 @@ constexpr int lanes_per_row(int dim) { return dim <= 32 ? 2 : dim <= 64 ? 4 : di
 
 // Norm and rotation of a row in 64 bits, rounded once: k's codes sit next to
 // rounding borders, and one rounding makes them independent of the order of
-// the norm's sum.  The 64-bit arithmetic is hidden behind the loads (14k
-// tokens of 32/8 heads of 128: the same time without it).
+// the norm's sum.  The 64-bit arithmetic is nearly hidden behind the loads (14k
+// tokens of 32/8 heads of 128 with the norm's weights 157 us, without them 145).
 // w, co, si: this lane's 16 (dims 8c .. and partners) and 8 + 8 numbers.
 template <int DIM>
 __device__ __forceinline__ void norm_rotate(float (&x)[16], bool live, bool norm, const float (&w)[16], float eps,
@@ -305,7 +305,10 @@ __device__ void append_values(const AppendArgs& A, const BlockItem& it, int h, c
 
 // Units of work, one wavefront each: blocks' keys and values (item, head, k /
 // v), then tokens' q (64 / lanes_per_row heads at a time, q_each times).  HBM
-// bounds it: 14402 tokens of 32/8 heads of 128 with norms move 0.62 GB.
+// bounds it: 14279 tokens of 32/8 heads of 128 with norms move 0.64 GB in 152
+// us, 4.2 TB/s (a large copy: 4.7); a launch of its own for q took as long,
+// and so did fewer registers.  One token: 4.5 us, the launch, its item, its
+// rows and the stores.
 template <int DIM>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs A) {
   constexpr int kLpr = lanes_per_row(DIM), kRows = 64 / kLpr, kHalf = DIM / 2;
@@ -374,7 +377,9 @@ struct ReadArgs {
 
 // One wavefront per block, head and k / v.  Keys: a lane four dims of a
 // position; values: whole dims, as they are stored.  Either way a store
-// instruction writes whole rows side by side.
+// instruction writes whole rows side by side.  HBM-bound, four fifths of it
+// the fp32 rows: 40k positions of 8 heads of 128 in 92 us, 4.4 TB/s (152 us
+// with 64-byte stores and the values' codes a byte at a time).
 template <int DIM>
 __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs A) {
   const int lane = threadIdx.x & 63;
