@@ -182,6 +182,46 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
     const int item = u / A.g.kv_heads, h = u - item * A.g.kv_heads;
     const AttnItem it = A.v.few[item];
 
+    const int last_block = (it.hi - 1) / kBlk;
+    // This lane's block of a tile is block base / 16 + grp; behind the range,
+    // the last one again (its positions there are masked), with scales of 0.
+    // Its page id is read a tile ahead.
+    const auto page_id = [&](int base) { return A.v.table[it.table + page_of(A.g, min(base / kBlk + grp, last_block))]; };
+    int id = page_id(min(it.lo + wave * kTile, it.hi - 1));
+    // A tile's keys: every lane needs all four blocks, position lo16, dims
+    // 16 (4c + grp) ...  They are asked for as soon as the tile before has
+    // used its own, and the values once the scores are made; with one tile of
+    // rows all together, which leaves room for a second workgroup on the
+    // compute unit (64 users of 32/8 heads of 128: 109 us against 113).
+    constexpr bool kPipe = MT > 1;
+    std::size_t at = 0;
+    float2 sc = make_float2(0.0f, 0.0f);
+    i4 kf[4][kC];
+    const auto fetch_keys = [&](int base) {
+      const int block = min(base / kBlk + grp, last_block);
+      at = block_at(A.g, id, page_of(A.g, block), block, h);
+      if (base + kWaves * kTile < it.hi) id = page_id(base + kWaves * kTile);
+      sc = reinterpret_cast<const float2*>(A.scales)[at];
+      const std::uint64_t p = reinterpret_cast<std::uint64_t>(A.k + at * (16 * HD));
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const std::uint32_t plo = __builtin_amdgcn_readlane(static_cast<int>(p), 16 * b);
+        const std::uint32_t phi = __builtin_amdgcn_readlane(static_cast<int>(p >> 32), 16 * b);
+        const auto* src = reinterpret_cast<const std::int8_t*>((static_cast<std::uint64_t>(phi) << 32) | plo);
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+          kf[b][c] = *reinterpret_cast<const i4*>(src + min(4 * c + grp, kG - 1) * 256 + lo16 * 16);
+      }
+    };
+    i4 vf[kG];
+    const auto fetch_values = [&]() {
+      const std::int8_t* vp = A.val + at * (16 * HD) + lo16 * 16;
+#pragma unroll
+      for (int g = 0; g < kG; ++g) vf[g] = *reinterpret_cast<const i4*>(vp + g * 256);
+    };
+    // (The first tile's are on their way while q is prepared.)
+    if (kPipe && it.lo + wave * kTile < it.hi) fetch_keys(it.lo + wave * kTile);
+
     // The digits of q: lane (digit row lo16, dims 16 grp ..) of each 64-dim step.
     i4 qd[MT][kC];
     float m[MT], l[MT], o[MT][kG];
@@ -248,44 +288,6 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
       for (int g = 0; g < kG; ++g) o[mt][g] = 0.0f;
     }
 
-    const int last_block = (it.hi - 1) / kBlk;
-    // This lane's block of a tile is block base / 16 + grp; behind the range,
-    // the last one again (its positions there are masked), with scales of 0.
-    // Its page id is read a tile ahead.
-    const auto page_id = [&](int base) { return A.v.table[it.table + page_of(A.g, min(base / kBlk + grp, last_block))]; };
-    int id = page_id(min(it.lo + wave * kTile, it.hi - 1));
-    // A tile's keys: every lane needs all four blocks, position lo16, dims
-    // 16 (4c + grp) ...  They are asked for as soon as the tile before has
-    // used its own, and the values once the scores are made; with one tile of
-    // rows all together, which leaves room for a second workgroup on the
-    // compute unit (64 users of 32/8 heads of 128: 109 us against 113).
-    constexpr bool kPipe = MT > 1;
-    std::size_t at = 0;
-    float2 sc = make_float2(0.0f, 0.0f);
-    i4 kf[4][kC];
-    const auto fetch_keys = [&](int base) {
-      const int block = min(base / kBlk + grp, last_block);
-      at = block_at(A.g, id, page_of(A.g, block), block, h);
-      if (base + kWaves * kTile < it.hi) id = page_id(base + kWaves * kTile);
-      sc = reinterpret_cast<const float2*>(A.scales)[at];
-      const std::uint64_t p = reinterpret_cast<std::uint64_t>(A.k + at * (16 * HD));
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const std::uint32_t plo = __builtin_amdgcn_readlane(static_cast<int>(p), 16 * b);
-        const std::uint32_t phi = __builtin_amdgcn_readlane(static_cast<int>(p >> 32), 16 * b);
-        const auto* src = reinterpret_cast<const std::int8_t*>((static_cast<std::uint64_t>(phi) << 32) | plo);
-#pragma unroll
-        for (int c = 0; c < kC; ++c)
-          kf[b][c] = *reinterpret_cast<const i4*>(src + min(4 * c + grp, kG - 1) * 256 + lo16 * 16);
-      }
-    };
-    i4 vf[kG];
-    const auto fetch_values = [&]() {
-      const std::int8_t* vp = A.val + at * (16 * HD) + lo16 * 16;
-#pragma unroll
-      for (int g = 0; g < kG; ++g) vf[g] = *reinterpret_cast<const i4*>(vp + g * 256);
-    };
-    if (kPipe && it.lo + wave * kTile < it.hi) fetch_keys(it.lo + wave * kTile);
     for (int base = it.lo + wave * kTile; base < it.hi; base += kWaves * kTile) {
       if (!kPipe) {
         fetch_keys(base);
@@ -479,6 +481,40 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
     // A negative scale goes to q, so that a block's largest score is its largest product.
     const float q_sign = A.scale < 0.0f ? -1.0f : 1.0f, scale = fabsf(A.scale) * kLog2e;
 
+    const int last_block = (it.hi - 1) / kBlk;
+    // A wavefront brings one of the tile's four blocks; its page id is read a
+    // tile ahead of it (behind the range: the last block again, whose
+    // positions there are masked).
+    uint4 kreg[kPer], vreg[kPer];
+    float2 sreg = make_float2(0.0f, 0.0f);
+    bool sreg_live = true;
+    // (The index is the wavefront's; kept in a vector register, so that the
+    // load is waited for where the id is used and not where it is made.)
+    int id = 0;
+    const auto lookup = [&](int base) {
+      int at = it.table + page_of(A.g, min(base / kBlk + wave, last_block));
+      asm volatile("" : "+v"(at));
+      id = A.v.table[at];
+    };
+    const auto fetch = [&](int base) {
+      const int want = base / kBlk + wave, block = min(want, last_block);
+      const std::size_t at = block_at(A.g, __builtin_amdgcn_readfirstlane(id), page_of(A.g, block), block, head);
+      const auto* kp = reinterpret_cast<const uint4*>(A.k + at * (16 * HD));
+      const auto* vp = reinterpret_cast<const uint4*>(A.val + at * (16 * HD));
+#pragma unroll
+      for (int n = 0; n < kPer; ++n) {
+        const int c = min(n * 64 + lane, HD - 1);
+        kreg[n] = kp[c];
+        vreg[n] = vp[c];
+      }
+      sreg = reinterpret_cast<const float2*>(A.scales)[at];
+      sreg_live = want <= last_block;
+    };
+    // The first tile's codes are on their way while q is prepared.
+    lookup(it.lo);
+    fetch(it.lo);
+    if (it.lo + kTile < it.hi) lookup(it.lo + kTile);
+
     // q * 2^qs, its largest below 2^14, as two fp16 parts.
     h8 qh[kG], ql[kG];
     int qs;
@@ -525,35 +561,6 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
     // far; vtop: log2 of the largest value scale so far (below all to begin).
     float m = -INFINITY, l = 0.0f, vtop = -200.0f;
 
-    const int last_block = (it.hi - 1) / kBlk;
-    // A wavefront brings one of the tile's four blocks; its page id is read a
-    // tile ahead of it (behind the range: the last block again, whose
-    // positions there are masked).
-    uint4 kreg[kPer], vreg[kPer];
-    float2 sreg = make_float2(0.0f, 0.0f);
-    bool sreg_live = true;
-    // (The index is the wavefront's; kept in a vector register, so that the
-    // load is waited for where the id is used and not where it is made.)
-    int id = 0;
-    const auto lookup = [&](int base) {
-      int at = it.table + page_of(A.g, min(base / kBlk + wave, last_block));
-      asm volatile("" : "+v"(at));
-      id = A.v.table[at];
-    };
-    const auto fetch = [&](int base) {
-      const int want = base / kBlk + wave, block = min(want, last_block);
-      const std::size_t at = block_at(A.g, __builtin_amdgcn_readfirstlane(id), page_of(A.g, block), block, head);
-      const auto* kp = reinterpret_cast<const uint4*>(A.k + at * (16 * HD));
-      const auto* vp = reinterpret_cast<const uint4*>(A.val + at * (16 * HD));
-#pragma unroll
-      for (int n = 0; n < kPer; ++n) {
-        const int c = min(n * 64 + lane, HD - 1);
-        kreg[n] = kp[c];
-        vreg[n] = vp[c];
-      }
-      sreg = reinterpret_cast<const float2*>(A.scales)[at];
-      sreg_live = want <= last_block;
-    };
     // What the products take of the block that `fetch` brought: the key scale
     // times the softmax's, log2 of the value scale (-inf: its codes are 0, or
     // masked), and NaN if a scale is not finite.
@@ -590,13 +597,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
       if (lane == 0) sh_s[to][wave] = block_terms();
     };
 
-    lookup(it.lo);
-    fetch(it.lo);
     stage(0);
-    if (it.lo + kTile < it.hi) {
-      lookup(it.lo + kTile);
-      fetch(it.lo + kTile);
-    }
+    if (it.lo + kTile < it.hi) fetch(it.lo + kTile);
     if (it.lo + 2 * kTile < it.hi) lookup(it.lo + 2 * kTile);
     __syncthreads();
     int buf = 0;

@@ -65,7 +65,10 @@ struct JoinItem {
 // 1500 positions 8.8 us against 9.4 in pieces, over 3000 in pieces 9.7
 // against 14.7).
 constexpr std::size_t kFewTarget = 512, kFewLeast = 8 * kTile, kFewWhole = 24 * kTile;
-constexpr std::size_t kManyTarget = 768, kManyLeast = 4 * kTile;
+constexpr std::size_t kManyTarget = 768, kManyLeast = 4 * kTile, kManyWhole = 4 * kTile;
+// Prompts whose pieces would be shorter than kManyShort that way: one unit for
+// each compute unit.
+constexpr std::size_t kUnits = 256, kManyShort = 4 * kTile;
 
 constexpr std::size_t kJoinFill = 2048;  // rows of all heads that fill the chip with a workgroup each
 constexpr int kJoinThreads = 256;
@@ -251,16 +254,19 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
       }
     }
   };
-  const auto split_of = [&](bool few, std::size_t target, std::size_t least) {
-    std::size_t reach = 0;
+  const auto split_of = [&](bool few) {
+    const std::size_t least = few ? kFewLeast : kManyLeast;
+    std::size_t reach = 0;  // positions x heads of all groups of rows
     each(few, [&](std::size_t, std::size_t, std::size_t, std::size_t len) { reach += len * sh.kv_heads; });
+    std::size_t target = few ? kFewTarget : kManyTarget;
+    if (!few && reach < kManyTarget * kManyShort) target = kUnits;
     return std::max(least, (reach / target + least - 1) / least * least);
   };
   const auto lay = [&](bool few, std::size_t split, std::vector<AttnItem>& items) {
     each(few, [&](std::size_t seq, std::size_t r, std::size_t rows, std::size_t len) {
       // Pieces of one size, in whole units (of a tile for each of its wavefronts, if few).
       const std::size_t unit = few ? kFewLeast : kTile;
-      const std::size_t most = few && len <= kFewWhole ? 1 : (len + split - 1) / split;
+      const std::size_t most = len <= (few ? kFewWhole : kManyWhole) ? 1 : (len + split - 1) / split;
       const std::size_t piece = ((len + most - 1) / most + unit - 1) / unit * unit;
       const std::size_t n = (len + piece - 1) / piece;
       const std::size_t slots = few ? few_rows(static_cast<int>(sh.head_dim)) / kSlotRows : kManyRows / kSlotRows;
@@ -275,8 +281,8 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
       l.parts += n * slots;
     });
   };
-  lay(true, split_of(true, kFewTarget, kFewLeast), l.few);
-  lay(false, split_of(false, kManyTarget, kManyLeast), l.many);
+  lay(true, split_of(true), l.few);
+  lay(false, split_of(false), l.many);
   // The longest first, so that the last to start are short.
   const auto longer = [](const AttnItem& a, const AttnItem& b) { return a.hi - a.lo > b.hi - b.lo; };
   std::stable_sort(l.few.begin(), l.few.end(), longer);
