@@ -152,12 +152,9 @@ __device__ __forceinline__ float row16_sum(float v) {
 __device__ __forceinline__ std::uint32_t digits(int x) {
   return (static_cast<std::uint32_t>(x) + 0x00808080u) ^ 0x00808080u;
 }
-// sum_i 2^(8i) s[i]
+// sum_i 2^(8i) s[i].  |s[i]| is at most 2^7 * 127 * 256 < 2^22, so pairs fit 32 bits.
 __device__ __forceinline__ float undigit(i4 s) {
-  float x = static_cast<float>(s[3]);
-  x = fmaf(x, 256.0f, static_cast<float>(s[2]));
-  x = fmaf(x, 256.0f, static_cast<float>(s[1]));
-  return fmaf(x, 256.0f, static_cast<float>(s[0]));
+  return fmaf(static_cast<float>((s[3] << 8) + s[2]), 65536.0f, static_cast<float>((s[1] << 8) + s[0]));
 }
 
 // HD: head_dim; MT: tiles of 4 rows (16 digit rows) there is room for.
@@ -173,6 +170,9 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
                                          // the wavefronts' outputs, merged at the end
   } sh;
   __shared__ float sh_m[kWaves][kRows], sh_l[kWaves][kRows];
+  __shared__ i4 sh_q[MT][kC][64];       // the digits of q as the products take them
+  __shared__ int sh_qe[MT][4];          // a row's exponent
+  __shared__ float sh_qbad[MT][4];      // NaN for a row with inf or NaN in q, else 0
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lo16 = lane & 15, grp = lane >> 4;
@@ -222,17 +222,13 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
     // (The first tile's are on their way while q is prepared.)
     if (kPipe && it.lo + wave * kTile < it.hi) fetch_keys(it.lo + wave * kTile);
 
-    // The digits of q: lane (digit row lo16, dims 16 grp ..) of each 64-dim step.
-    i4 qd[MT][kC];
-    float m[MT], l[MT], o[MT][kG];
-    int qe[MT];  // this lane's score row (head grp of the tile): its exponent
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int r = 4 * mt + lo16 / 4;
-      const bool live = r < it.rows;
-      const Row w = row_of(A, it.row0, h, live ? r : 0);
-      const float* qp = A.q + static_cast<std::size_t>(it.row + w.tok) * A.q_stride + w.off;
+    // The digits of q, by one wavefront for each tile of rows: lane (digit row
+    // lo16, dims 16 grp ..) of each 64-dim step.
+    if (wave < MT) {
+      const int r = 4 * wave + lo16 / 4;
       // Rows of nobody repeat the first one; nothing of theirs is kept.
+      const Row w = row_of(A, it.row0, h, r < it.rows ? r : 0);
+      const float* qp = A.q + static_cast<std::size_t>(it.row + w.tok) * A.q_stride + w.off;
       float x[kC][16];
       float top = 0.0f;
       bool bad = false;
@@ -258,7 +254,8 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
       (void)frexpf(top, &e);  // top < 2^e
       if (bad || !(top > 0.0f)) e = 0;
 #pragma unroll
-      for (int c = 0; c < kC; ++c)
+      for (int c = 0; c < kC; ++c) {
+        i4 d4;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           std::uint32_t d = 0;
@@ -267,12 +264,25 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
             const int X = bad ? 0 : static_cast<int>(rintf(ldexpf(x[c][4 * j + i], 30 - e)));
             d |= ((digits(X) >> (8 * (lo16 & 3))) & 0xFFu) << (8 * i);
           }
-          qd[mt][c][j] = static_cast<int>(d);
+          d4[j] = static_cast<int>(d);
         }
-      // Lanes 4 hd .. of any group hold head hd's; an inf or NaN in q makes the row's sum NaN.
-      qe[mt] = __shfl(e - 30, 4 * grp, 64);
-      __builtin_amdgcn_sched_barrier(0);  // one tile of rows at a time: registers
-      l[mt] = __shfl(static_cast<int>(bad), 4 * grp, 64) != 0 ? __builtin_nanf("") : 0.0f;
+        sh_q[wave][c][lane] = d4;
+      }
+      if (lane < 16 && (lane & 3) == 0) {
+        sh_qe[wave][lane / 4] = e - 30;
+        sh_qbad[wave][lane / 4] = bad ? __builtin_nanf("") : 0.0f;
+      }
+    }
+    __syncthreads();
+    i4 qd[MT][kC];
+    float m[MT], l[MT], o[MT][kG];
+    int qe[MT];  // this lane's score row (head grp of the tile)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int c = 0; c < kC; ++c) qd[mt][c] = sh_q[mt][c][lane];
+      qe[mt] = sh_qe[mt][grp];
+      l[mt] = sh_qbad[mt][grp];
     }
 
     int limit[MT];  // last position that this lane's row sees, -1 for rows of nobody
