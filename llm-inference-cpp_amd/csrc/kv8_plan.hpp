@@ -57,14 +57,17 @@ struct JoinItem {
 };
 // A history is split so that a batch makes about this many units of work
 // (item and key/value head), in pieces of at least the second number of
-// positions.  Measured: 512 units of `few` work against 1024, 64 users of 4000
-// positions (32/8 heads of 128) 93 us against 102; 768 units of `many` work
-// against 512 and 1024, 2048 tokens over 6144 447 us against 487 and 472.
+// positions.  Measured with 256 units of `few` work (32/8 heads of 128; one
+// unit a compute unit) against 384: 64 users over 120 to 8191 positions 95 us
+// against 105, 32 over 2000 23 against 30, 16 drafts of 3 to 6 tokens 30
+// against 32; against 128, 4 drafts of 8 tokens over 2000 15 against 18.  768
+// units of `many` work against 512 and 1024, 2048 tokens over 6144 447 us
+// against 487 and 472.
 // The join of pieces costs 4 us, a tile of each wavefront 1.8 us: a `few`
 // history up to kFewWhole is not split (one user of 32/8 heads of 128 over
 // 1500 positions 8.8 us against 9.4 in pieces, over 3000 in pieces 9.7
 // against 14.7).
-constexpr std::size_t kFewTarget = 512, kFewLeast = 8 * kTile, kFewWhole = 24 * kTile;
+constexpr std::size_t kFewTarget = 256, kFewLeast = 8 * kTile, kFewWhole = 24 * kTile;
 constexpr std::size_t kManyTarget = 768, kManyLeast = 4 * kTile, kManyWhole = 4 * kTile;
 // Prompts whose pieces would be shorter than kManyShort that way: one unit for
 // each compute unit.
