@@ -126,13 +126,13 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(AttnArgs A, int j
 // Why digits: the codes need no conversion, so the vector ALUs see only the
 // scores (one per position, head and lane group, not one per code), and 31
 // fixed-point bits are more than fp32's 24.
-// Measured: 64 users of 32/8 heads of 128 over 263k positions 101 us, 5.4 TB/s
+// Measured: 64 users of 32/8 heads of 128 over 263k positions 95 us, 5.7 TB/s
 // of codes and scales (a large copy moves 4.7, reads and writes together);
-// over 4000 positions each 93 us with the join, 5.6 TB/s.  One user over 300
-// positions (9/3 heads of 64) 4.4 us, what a launch and its four dependent
-// loads take.  Drafts of 3 to 6 tokens (12 to 24 rows a head): 35 us for 60 MB,
-// bound by the four row tiles' scores and by one workgroup a compute unit
-// (their registers).
+// over 4000 positions each 92 us.  One user over 300 positions (9/3 heads of
+// 64) 4.4 us, what a launch and its four dependent loads take.  16 drafts of 3
+// to 6 tokens (12 to 24 rows a head): 26 us with the join for 60 MB, bound by
+// the four row tiles' scores and by one workgroup a compute unit (their
+// registers).
 constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
 
 // Maximum over the 16 lanes of a row of lanes, in every lane.
@@ -190,10 +190,9 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
     int id = page_id(min(it.lo + wave * kTile, it.hi - 1));
     // A tile's keys: every lane needs all four blocks, position lo16, dims
     // 16 (4c + grp) ...  They are asked for as soon as the tile before has
-    // used its own, and the values once the scores are made; with one tile of
-    // rows all together, which leaves room for a second workgroup on the
-    // compute unit (64 users of 32/8 heads of 128: 109 us against 113).
-    constexpr bool kPipe = MT > 1;
+    // used its own, and the values once the scores are made (all together at
+    // the tile's start: 64 users of 32/8 heads of 128 over 4000 positions 94 us
+    // against 92, one user over 300 positions 5.6 against 4.7).
     std::size_t at = 0;
     float2 sc = make_float2(0.0f, 0.0f);
     i4 kf[4][kC];
@@ -220,7 +219,7 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
       for (int g = 0; g < kG; ++g) vf[g] = *reinterpret_cast<const i4*>(vp + g * 256);
     };
     // (The first tile's are on their way while q is prepared.)
-    if (kPipe && it.lo + wave * kTile < it.hi) fetch_keys(it.lo + wave * kTile);
+    if (it.lo + wave * kTile < it.hi) fetch_keys(it.lo + wave * kTile);
 
     // The digits of q, by one wavefront for each tile of rows: lane (digit row
     // lo16, dims 16 grp ..) of each 64-dim step.
@@ -299,10 +298,6 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
     }
 
     for (int base = it.lo + wave * kTile; base < it.hi; base += kWaves * kTile) {
-      if (!kPipe) {
-        fetch_keys(base);
-        fetch_values();
-      }
       if (base / kBlk + grp > last_block) sc = make_float2(0.0f, 0.0f);
       float ks[4], vs[4];
 #pragma unroll
@@ -322,12 +317,10 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
           if (base + b * kBlk + lo16 > limit[mt]) x[mt][b] = -INFINITY;
         }
       }
-      if (kPipe) {
-        __builtin_amdgcn_sched_barrier(0);
-        fetch_values();
-        if (base + kWaves * kTile < it.hi) fetch_keys(base + kWaves * kTile);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      __builtin_amdgcn_sched_barrier(0);
+      fetch_values();
+      if (base + kWaves * kTile < it.hi) fetch_keys(base + kWaves * kTile);
+      __builtin_amdgcn_sched_barrier(0);
       // The tile's largest finite value scale; 2^-96 keeps 2^30 / top finite.
       float vf_s[4], top = 0x1p-96f;
 #pragma unroll
@@ -438,8 +431,8 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
 // of the result; two are off by 2^-22 or less, below fp32's sums.  That is twice the
 // formula's products: 2048 tokens over 6144 positions of 32/8 heads of 128
 // are 481 GFLOP, 414 us at the 1162 TFLOP/s of a large fp16 library product;
-// this kernel takes 440 and the join 27.  The matrix units are busy 57 % of
-// the clocks; what is left are the staging's conversions (38 us without
+// this kernel and the join take 433 to 441 together, 27 of it the join.  The
+// matrix units are busy 53 to 57 % of the clocks; what is left are the staging's conversions (38 us without
 // them), the wait for a tile's codes (20) and the maximum's dependency.
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));

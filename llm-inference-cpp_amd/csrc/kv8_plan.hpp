@@ -63,15 +63,26 @@ struct JoinItem {
 // against 32; against 128, 4 drafts of 8 tokens over 2000 15 against 18.  768
 // units of `many` work against 512 and 1024, 2048 tokens over 6144 447 us
 // against 487 and 472.
-// The join of pieces costs 4 us, a tile of each wavefront 1.8 us: a `few`
-// history up to kFewWhole is not split (one user of 32/8 heads of 128 over
-// 1500 positions 8.8 us against 9.4 in pieces, over 3000 in pieces 9.7
-// against 14.7).
-constexpr std::size_t kFewTarget = 256, kFewLeast = 8 * kTile, kFewWhole = 24 * kTile;
-constexpr std::size_t kManyTarget = 768, kManyLeast = 4 * kTile, kManyWhole = 4 * kTile;
+constexpr std::size_t kFewTarget = 256, kFewLeast = 8 * kTile;
+constexpr std::size_t kManyTarget = 768, kManyLeast = 4 * kTile;
 // Prompts whose pieces would be shorter than kManyShort that way: one unit for
 // each compute unit.
 constexpr std::size_t kUnits = 256, kManyShort = 4 * kTile;
+// Pieces cost their join, 4 us and more: rows are split only if a piece is
+// shorter than their history by more than this.  `few`: for 512 = 4 rows x 128
+// dims (one user of 32/8 heads of 128 over 1500 positions 8.6 us whole, 11.1
+// in pieces; over 3000 12.3 and 9.7; 16 over 3000 18.2 and 21.7), less for
+// wider work by the square, since its tiles take longer and its registers
+// leave fewer wavefronts to overlap (16 drafts of 3 to 6 tokens 26 us against
+// 31 with the same for all widths, 32 users of 8/1 heads of 256 26 against
+// 35), for narrower work at most kFewGainMost (16 users over 1000 to
+// 8000 positions, 9/3 heads of 64, 16 us against 21 without that, one over
+// 5000 9.4 against 14).  `many`: nothing where whole histories leave compute units without
+// work (one prompt of 1024 tokens of 14/2 heads of 64 20.5 us against 25), else
+// kManyGain (4 prompts of 512 tokens behind 300, 32/8 heads of 128, 53 us
+// against 73; 2 of 500 behind 1000 67 against 70).
+constexpr std::size_t kFewGain = 28 * kTile, kFewGainAt = 4 * 128, kFewGainMost = 40 * kTile;
+constexpr std::size_t kManyGain = 12 * kTile;
 
 constexpr std::size_t kJoinFill = 2048;  // rows of all heads that fill the chip with a workgroup each
 constexpr int kJoinThreads = 256;
@@ -265,11 +276,18 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
     if (!few && reach < kManyTarget * kManyShort) target = kUnits;
     return std::max(least, (reach / target + least - 1) / least * least);
   };
+  std::size_t whole = 0;  // units of `many` work without pieces
+  each(false, [&](std::size_t, std::size_t, std::size_t, std::size_t) { whole += sh.kv_heads; });
+  const auto gain = [&](bool few, std::size_t rows) {
+    const std::size_t width = sh.head_dim * ((rows + 3) / 4 * 4);
+    if (few) return std::min(kFewGainMost, kFewGain * kFewGainAt * kFewGainAt / (width * width));
+    return 4 * whole >= 3 * kUnits ? kManyGain : 0;
+  };
   const auto lay = [&](bool few, std::size_t split, std::vector<AttnItem>& items) {
     each(few, [&](std::size_t seq, std::size_t r, std::size_t rows, std::size_t len) {
       // Pieces of one size, in whole units (of a tile for each of its wavefronts, if few).
       const std::size_t unit = few ? kFewLeast : kTile;
-      const std::size_t most = len <= (few ? kFewWhole : kManyWhole) ? 1 : (len + split - 1) / split;
+      const std::size_t most = len <= split + gain(few, rows) ? 1 : (len + split - 1) / split;
       const std::size_t piece = ((len + most - 1) / most + unit - 1) / unit * unit;
       const std::size_t n = (len + piece - 1) / piece;
       const std::size_t slots = few ? few_rows(static_cast<int>(sh.head_dim)) / kSlotRows : kManyRows / kSlotRows;
