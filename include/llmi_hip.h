@@ -330,8 +330,9 @@ int llmi_hip_kv8_sizes(const llmi_kv8_shape* shape, size_t* code_bytes, size_t* 
  * All arrays are host memory, read before the call returns.
  * A plan holds a batch's work lists on the device and the attention's
  * workspace, and serves every layer of the same shape.  It is created for at
- * most max_seqs sequences, max_tokens tokens and max_pages page entries in
- * all (0: shape->pages); plan_set replaces the batch.
+ * most max_seqs sequences, max_tokens tokens (x heads / kv_heads up to 2^30)
+ * and max_pages page entries in all (0: shape->pages); plan_set replaces the
+ * batch.
  * plan_set queues one copy on `stream`; the calls below that use the plan
  * follow on that stream.  Launches captured into a graph work on whatever
  * batch is set when they are replayed, in buffers with room for its tokens

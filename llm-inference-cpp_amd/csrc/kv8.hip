@@ -513,7 +513,7 @@ int llmi_hip_kv8_check(const llmi_kv8_shape* shape, size_t seqs, const int32_t* 
   if (why.empty()) {
     try {
       Lists l;
-      why = build(*shape, seqs, slots, starts, counts, tables, table_stride, 0x7FFFFFFF, 0x7FFFFFFF, 0x7FFFFFFF, &l);
+      why = check_batch(*shape, seqs, slots, starts, counts, tables, table_stride, 0x7FFFFFFF, 0x7FFFFFFF, 0x7FFFFFFF, &l);
       if (why.empty() && !l.writable) why = l.why_not;
     } catch (const std::bad_alloc&) {
       why = "out of host memory";
@@ -548,7 +548,9 @@ int llmi_hip_kv8_plan_create(const llmi_kv8_shape* shape, size_t max_seqs, size_
   p->g.block_bytes = static_cast<std::size_t>(kBlk) * shape->head_dim;
   p->g.by_page = divisor(static_cast<std::uint32_t>(p->g.page_blocks));
   p->most = limits(*shape, max_seqs, max_tokens);
-  // Kernels count units of work (item and key/value head) in 32 bits.
+  // Kernels count rows of a key/value head and units of work (item and head) in 32 bits.
+  LLMI_REQUIRE(max_tokens * (shape->heads / shape->kv_heads) <= (std::size_t{1} << 30),
+               "kv8_plan_create: more than 2^30 rows (tokens x heads / kv_heads)");
   LLMI_REQUIRE(std::max({2 * p->most.blocks, p->most.few, p->most.many}) * shape->kv_heads <= 0x7FFFFFFFu,
                "kv8_plan_create: too many sequences and tokens for the heads");
   const auto take = [&](std::size_t bytes) {

@@ -160,11 +160,12 @@ inline Limits limits(const llmi_kv8_shape& sh, std::size_t seqs, std::size_t tok
           2 * few * (rows / kSlotRows) + 2 * many * (kManyRows / kSlotRows), few + many};
 }
 
-// Checks a batch and builds its lists; returns the reason of a refusal.
-inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::int32_t* slots,
-                         const std::int32_t* starts, const std::int32_t* counts, const std::int32_t* tables,
-                         std::size_t stride, std::size_t max_seqs, std::size_t max_tokens, std::size_t max_pages,
-                         Lists* out) {
+// Checks a batch; returns the reason of a refusal.  Fills in the sequences,
+// the tables and whether it can be appended.
+inline std::string check_batch(const llmi_kv8_shape& sh, std::size_t seqs, const std::int32_t* slots,
+                               const std::int32_t* starts, const std::int32_t* counts, const std::int32_t* tables,
+                               std::size_t stride, std::size_t max_seqs, std::size_t max_tokens,
+                               std::size_t max_pages, Lists* out) {
   Lists& l = *out;
   l = Lists{};
   if (seqs > max_seqs) return "more sequences than the plan was created for";
@@ -221,6 +222,18 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
       if (!l.writable) break;
     }
   }
+  return {};
+}
+
+// Checks a batch and builds its lists.
+inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::int32_t* slots,
+                         const std::int32_t* starts, const std::int32_t* counts, const std::int32_t* tables,
+                         std::size_t stride, std::size_t max_seqs, std::size_t max_tokens, std::size_t max_pages,
+                         Lists* out) {
+  Lists& l = *out;
+  if (std::string why = check_batch(sh, seqs, slots, starts, counts, tables, stride, max_seqs, max_tokens, max_pages, out);
+      !why.empty())
+    return why;
   for (std::size_t i = 0; i < seqs; ++i) {
     const Seq& q = l.seqs[i];
     if (q.count == 0) continue;

@@ -588,3 +588,51 @@ def test_refusals():
             r.append(pool.layer, None, b.ptr, b.ptr, None)
         r.read(pool.layer, b.ptr, None)
     H.synchronize()
+
+
+def test_rows_past_32_bits_refused():
+    with pytest.raises(H.HipError, match="2\\^30 rows"):
+        H.Kv8Plan(H.Kv8Shape(4096, 1, 32, 16, 4, 1), 1, (1 << 18) + 1)
+
+
+LONG = [
+    # heads, kv, dim, page, starts, counts: single tokens and drafts whose histories are taken in pieces
+    (9, 3, 64, 64, [5200, 40], [1, 1]),
+    (5, 1, 32, 16, [4100], [1]),
+    (8, 2, 128, 32, [4000, 3500], [4, 1]),
+    (40, 1, 64, 16, [3600], [1]),
+    (16, 2, 96, 48, [3300], [2]),
+    (7, 1, 160, 64, [2500], [3]),
+    (8, 1, 256, 128, [2700, 2000], [1, 2]),
+]
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,starts,counts", LONG)
+def test_attention_in_pieces_eager_and_replayed(heads, kv, dim, page, starts, counts):
+    """Long histories, against the formula, and the same bits from a graph
+    that is replayed between batches of other lengths."""
+    rng = np.random.default_rng(heads * 131 + dim)
+    lens = [a + c for a, c in zip(starts, counts)]
+    pool = Pool(rng, heads, kv, dim, page, lens)
+    k, v = ([rows_of(rng, n, kv, dim, s) for n in lens] for s in (0.3, 0.5))
+    pool.append([0] * len(lens), lens, None, np.concatenate(k), np.concatenate(v))
+    scale = 1.0 / np.sqrt(dim)
+    plan = H.Kv8Plan(pool.shape, len(lens), sum(counts), pool.tables.size)
+    qb, ob = (H.DeviceBuffer(sum(counts) * heads * dim * 4) for _ in range(2))
+    plan.set(pool.slots, [3] * len(lens), counts, pool.tables)
+    H.synchronize()
+    graph = H.Graph(lambda: plan.attention(pool.layer, qb.ptr, scale, ob.ptr))
+    for at in (starts, [min(100, s) for s in starts], starts):
+        q = rows_of(rng, sum(counts), heads, dim, 0.5)
+        got = pool.attention(at, counts, q, scale)
+        plan.set(pool.slots, at, counts, pool.tables)
+        qb.upload(q)
+        graph.launch()
+        H.synchronize()
+        assert np.array_equal(ob.download(np.float32).reshape(q.shape), got)
+        row = 0
+        for i, c in enumerate(counts):
+            kq, vq, qi = R.quantize(k[i])[:at[i] + c], R.quantize(v[i])[:at[i] + c], q[row:row + c]
+            off = np.abs(got[row:row + c] - R.attend(qi, kq, vq, at[i], scale)).max()
+            assert off <= R.attend_bound(qi, kq, vq, scale), (i, off)
+            row += c

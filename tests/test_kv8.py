@@ -78,3 +78,15 @@ def test_work_lists(tmp_path):
                     os.path.join(ROOT, "tests", "native", "kv8_lists.cpp"), "-o", exe], check=True)
     out = subprocess.run([exe], capture_output=True, text=True)
     assert out.returncode == 0, out.stdout + out.stderr
+
+
+def test_check_holds_no_more_than_the_tables():
+    """A check makes no lists of work: 2^31 - 65536 new tokens need no memory a token."""
+    import resource
+
+    n = 32767
+    big = shape(kv_heads=1, heads=1, head_dim=32, page_tokens=65536, pages=n, slots=1)
+    table = np.arange(n, dtype=np.int32)[None]
+    before = resource.getrusage(resource.RUSAGE_SELF).ru_maxrss
+    H.kv8_check(big, [0], [0], [n * 65536], table)
+    assert resource.getrusage(resource.RUSAGE_SELF).ru_maxrss - before < 1 << 18  # KB
