@@ -60,11 +60,15 @@ struct JoinItem {
 // positions.  Measured with 256 units of `few` work (32/8 heads of 128; one
 // unit a compute unit) against 384: 64 users over 120 to 8191 positions 95 us
 // against 105, 32 over 2000 23 against 30, 16 drafts of 3 to 6 tokens 30
-// against 32; against 128, 4 drafts of 8 tokens over 2000 15 against 18.  768
-// units of `many` work against 512 and 1024, 2048 tokens over 6144 447 us
-// against 487 and 472.
+// against 32; against 128, 4 drafts of 8 tokens over 2000 15 against 18.
+// `many` work: 512, the two workgroups that a compute unit holds (up to 128
+// dims); its pieces
+// are of that size with the rest in the last one, so that the short ones fill
+// what short histories leave (512 units so against 768 in equal pieces: 2048
+// tokens over 6144 435 us against 449, 1000 over 3000 133 against 145, 8
+// prompts of 512 over 2000, 14/2 heads of 64, 86 against 97).
 constexpr std::size_t kFewTarget = 256, kFewLeast = 8 * kTile;
-constexpr std::size_t kManyTarget = 768, kManyLeast = 4 * kTile;
+constexpr std::size_t kManyTarget = 512, kManyLeast = 4 * kTile;
 // Prompts whose pieces would be shorter than kManyShort that way: one unit for
 // each compute unit.
 constexpr std::size_t kUnits = 256, kManyShort = 4 * kTile;
@@ -75,12 +79,12 @@ constexpr std::size_t kUnits = 256, kManyShort = 4 * kTile;
 // wider work by the square, since its tiles take longer and its registers
 // leave fewer wavefronts to overlap (16 drafts of 3 to 6 tokens 26 us against
 // 31 with the same for all widths, 32 users of 8/1 heads of 256 26 against
-// 35), for narrower work at most kFewGainMost (16 users over 1000 to
-// 8000 positions, 9/3 heads of 64, 16 us against 21 without that, one over
-// 5000 9.4 against 14).  `many`: nothing where whole histories leave compute units without
-// work (one prompt of 1024 tokens of 14/2 heads of 64 20.5 us against 25), else
-// kManyGain (4 prompts of 512 tokens behind 300, 32/8 heads of 128, 53 us
-// against 73; 2 of 500 behind 1000 67 against 70).
+// 35), for narrower work at most kFewGainMost (16 users over 1000 to 8000
+// positions, 9/3 heads of 64, 16 us against 21 without that, one over 5000 9.4
+// against 14).  `many`: nothing where whole histories leave compute units
+// without work (one prompt of 1024 tokens of 14/2 heads of 64 20.5 us against
+// 25), else kManyGain (4 prompts of 512 tokens behind 300, 32/8 heads of 128, 53 us
+// against 73; 2 of 500 behind 1000 56 against 70).
 constexpr std::size_t kFewGain = 28 * kTile, kFewGainAt = 4 * 128, kFewGainMost = 40 * kTile;
 constexpr std::size_t kManyGain = 12 * kTile;
 
@@ -298,10 +302,10 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
   };
   const auto lay = [&](bool few, std::size_t split, std::vector<AttnItem>& items) {
     each(few, [&](std::size_t seq, std::size_t r, std::size_t rows, std::size_t len) {
-      // Pieces of one size, in whole units (of a tile for each of its wavefronts, if few).
-      const std::size_t unit = few ? kFewLeast : kTile;
+      // `few`: pieces of one size, in whole units of a tile for each wavefront.
       const std::size_t most = len <= split + gain(few, rows) ? 1 : (len + split - 1) / split;
-      const std::size_t piece = ((len + most - 1) / most + unit - 1) / unit * unit;
+      const std::size_t even = ((len + most - 1) / most + kFewLeast - 1) / kFewLeast * kFewLeast;
+      const std::size_t piece = most == 1 ? len : few ? even : split;
       const std::size_t n = (len + piece - 1) / piece;
       const std::size_t slots = few ? few_rows(static_cast<int>(sh.head_dim)) / kSlotRows : kManyRows / kSlotRows;
       const auto i32 = [](std::size_t x) { return static_cast<std::int32_t>(x); };
