@@ -636,3 +636,42 @@ def test_attention_in_pieces_eager_and_replayed(heads, kv, dim, page, starts, co
             off = np.abs(got[row:row + c] - R.attend(qi, kq, vq, at[i], scale)).max()
             assert off <= R.attend_bound(qi, kq, vq, scale), (i, off)
             row += c
+
+
+def test_replayed_batches_larger_than_a_captured_grid():
+    """A captured launch has a bounded grid, whose workgroups take further
+    units in turn: thousands of sequences, as prompts and as single tokens,
+    give the bits of eager calls."""
+    heads, dim, page = 8, 32, 16
+    prompts, singles, length = 520, 2200, 66
+    tokens = prompts * length
+    pools = [Pool(np.random.default_rng(33), heads, heads, dim, page, [length + 1] * singles) for _ in range(2)]
+    plans = [H.Kv8Plan(pool.shape, singles, tokens, pool.tables.size) for pool in pools]
+    n = tokens * heads * dim
+    bufs = [[H.DeviceBuffer(n * 4) for _ in range(6)] for _ in pools]
+
+    def step(i):
+        q, k, v, o, rk, rv = (b.ptr for b in bufs[i])
+        plans[i].append(pools[i].layer, q, k, v, q)
+        plans[i].attention(pools[i].layer, q, 0.2, o)
+        plans[i].read(pools[i].layer, rk, rv)
+
+    plans[0].set([], [], [], np.zeros((0, 0), np.int32))
+    H.synchronize()
+    graph = H.Graph(lambda: step(0))
+    rng = np.random.default_rng(34)
+    for seqs, start, count in ((prompts, 0, length), (singles, 0, 1), (singles, 1, 2), (prompts, 3, 1)):
+        rows = [rows_of(rng, seqs * count, heads, dim) for _ in range(3)]
+        outs = []
+        for i in range(2):
+            for b, x in zip(bufs[i], rows):
+                b.upload(x)
+            plans[i].set(pools[i].slots[:seqs], [start] * seqs, [count] * seqs, pools[i].tables[:seqs])
+            if i == 0:
+                graph.launch()
+            else:
+                step(1)
+            H.synchronize()
+            outs.append([b.download(np.float32)[:seqs * count * heads * dim] for b in bufs[i][3:]])
+        for a, b in zip(*outs):
+            assert np.isfinite(a).all() and np.array_equal(a, b)
