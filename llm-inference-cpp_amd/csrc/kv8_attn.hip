@@ -120,8 +120,10 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(AttnArgs A, int j
 // lane finds the four digits' sums of one head in its four accumulators.
 //   scores   S[head][position] = Q K^T   A = digits of q, B = key codes
 //   output   O[head][dim]      = W V     A = digits of w, B = value codes
-// with w = p * (value scale / the tile's largest) in [0, 1], p the weight
-// against the running maximum.  A wavefront takes tiles of 64 positions = 4
+// with w = p * value scale, fixed-point against a power of two over the row's
+// largest of the tile (so that large values that a row does not see, or gives
+// no weight, cost the others no bits), p the weight against the running
+// maximum.  A wavefront takes tiles of 64 positions = 4
 // blocks; a workgroup's wavefronts take a range's tiles in turn and merge.
 // Why digits: the codes need no conversion, so the vector ALUs see only the
 // scores (one per position, head and lane group, not one per code), and 31
@@ -321,14 +323,9 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
       fetch_values();
       if (base + kWaves * kTile < it.hi) fetch_keys(base + kWaves * kTile);
       __builtin_amdgcn_sched_barrier(0);
-      // The tile's largest finite value scale; 2^-96 keeps 2^30 / top finite.
-      float vf_s[4], top = 0x1p-96f;
+      float vf_s[4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        vf_s[b] = vs[b] < INFINITY ? vs[b] : 0.0f;
-        top = fmaxf(top, vf_s[b]);
-      }
-      const float to_fix = 0x1p30f / top;
+      for (int b = 0; b < 4; ++b) vf_s[b] = vs[b] < INFINITY ? vs[b] : 0.0f;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         float mx = fmaxf(fmaxf(fmaxf(x[mt][0], x[mt][1]), fmaxf(x[mt][2], x[mt][3])), m[mt]);
@@ -336,16 +333,21 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
         const float ref = mx == -INFINITY ? 0.0f : mx;
         const float keep = exp2_hw(m[mt] - ref);
         m[mt] = mx;
-        float sum = 0.0f;
+        float sum = 0.0f, w[4], top = 0.0f;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           const bool seen = base + b * kBlk + lo16 <= limit[mt];
           const float p = exp2_hw(x[mt][b] - ref);
           // A value scale that is inf or NaN shows in the sum of the rows that see the block.
           if (seen) sum += fmaf(vs[b], 0.0f, p);
-          const int w = static_cast<int>(rintf(p * (vf_s[b] * to_fix)));
-          sh.w[wave][b][grp][lo16] = digits(w);
+          w[b] = p * vf_s[b];
+          top = fmaxf(top, w[b]);
         }
+        // The row's largest is below 2^we (-96: 2^(we - 30) stays a normal number).
+        const int we = max(__builtin_amdgcn_frexp_expf(row16_max(top)), -96);
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          sh.w[wave][b][grp][lo16] = digits(static_cast<int>(rintf(ldexpf(w[b], 30 - we))));
         l[mt] = fmaf(l[mt], keep, sum);
         __builtin_amdgcn_wave_barrier();
         // Digit row lo16 (head lo16 / 4, digit lo16 % 4) over this lane group's block.
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
           wd[j] = static_cast<int>(__builtin_amdgcn_perm(b2, a, 0x05040100u));
         }
         __builtin_amdgcn_wave_barrier();
-        const float from_fix = top * 0x1p-30f;
+        const float from_fix = ldexpf(1.0f, we - 30);
 #pragma unroll
         for (int g = 0; g < kG; ++g) {
           i4 acc = {0, 0, 0, 0};
@@ -425,8 +427,10 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
 // accumulators to the second's operand without leaving the registers: a lane
 // holds positions 4h .. 4h+3 and 8+4h .. of each 16 (h = lane / 32), and the
 // value tile is staged in that order.
-// w = p * (value scale / the largest so far) * 2^kWeightBits: block scales
-// differ along the sum, so they ride on the weights.
+// w = p * value scale * 2^kWeightBits / the row's largest product of the two so
+// far: block scales differ along the sum, so they ride on the weights (against
+// the largest scale alone, a block that a row does not see, or gives no weight,
+// would take bits from the others).
 // Why two parts: one fp16 part of q or w is off by 2^-12, which shows as 1e-4
 // of the result; two are off by 2^-22 or less, below fp32's sums.  That is twice the
 // formula's products: 2048 tokens over 6144 positions of 32/8 heads of 128
@@ -561,8 +565,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     // m: what scores are taken against, at most kSlack below the largest so
-    // far; vtop: log2 of the largest value scale so far (below all to begin).
-    float m = -INFINITY, l = 0.0f, vtop = -200.0f;
+    // far; rm: the same for scores plus log2 of the value scale.
+    float m = -INFINITY, l = 0.0f, rm = -INFINITY;
 
     // What the products take of the block that `fetch` brought: the key scale
     // times the softmax's, log2 of the value scale (-inf: its codes are 0, or
@@ -642,18 +646,13 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
       if (base + 2 * kTile < it.hi) fetch(base + 2 * kTile);
       if (base + 3 * kTile < it.hi) lookup(base + 3 * kTile);
       // Per block: scores are f times the products (f is positive: where
-      // the scale is 0 the products are, and a masked -inf stays -inf);
-      // weights carry 2^ratio, the value scale over the largest.  A scale
-      // below 2^-60 of the largest counts as that; one of 0 has codes of 0.
-      float f[4], ratio[4], bad = 0.0f, tile_top = vtop;
+      // the scale is 0 the products are, and a masked -inf stays -inf).
+      float f[4], ratio[4], bad = 0.0f;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        tile_top = fmaxf(tile_top, term[b].y);
         f[b] = fmaxf(ldexpf(term[b].x, -qs), 0x1p-126f);
         bad += term[b].z;
       }
-#pragma unroll
-      for (int b = 0; b < 4; ++b) ratio[b] = term[b].y == -INFINITY ? 0.0f : fmaxf(term[b].y - tile_top, -60.0f);
       // Positions behind a row's own leave nothing.
       if (base + kTile - 1 > all) {
 #pragma unroll
@@ -662,30 +661,37 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
           for (int i = 0; i < 8; ++i)
             if (base + 16 * b + 8 * (i / 4) + 4 * h2nd + i % 4 > limit) st[b / 2][8 * (b & 1) + i] = -INFINITY;
       }
-      float mx = -INFINITY;
+      float mx = -INFINITY, rx = -INFINITY;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, st[b / 2][8 * (b & 1) + i]);
         mx = fmaxf(mx, top * f[b]);
+        rx = fmaxf(rx, fmaf(top, f[b], term[b].y));
       }
       mx = fmaxf(mx, other_half(mx));
-      // The sums are rescaled where the largest score has grown by more
-      // than kSlack (weights may be up to 2^kSlack before that), or a value scale.
-      const bool grown = mx > m + kSlack;
-      if (__any(grown) || tile_top > vtop) {
-        const float now = grown ? mx : m, keep = now == -INFINITY ? 0.0f : exp2_hw(m - now);
-        const float rescale = keep * exp2_hw(vtop - tile_top);
+      rx = fmaxf(rx, other_half(rx));
+      // The sums are rescaled where one of the two has grown by more than
+      // kSlack (weights may be up to 2^kSlack before that).
+      const bool grown = mx > m + kSlack, risen = rx > rm + kSlack;
+      if (__any(grown || risen)) {
+        const float now = grown ? mx : m, r_now = risen ? rx : rm;
+        l *= now == -INFINITY ? 0.0f : exp2_hw(m - now);
+        const float rescale = r_now == -INFINITY ? 0.0f : exp2_hw(rm - r_now);
         m = now;
-        vtop = tile_top;
-        l *= keep;
+        rm = r_now;
 #pragma unroll
         for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[d][i] *= rescale;
       }
-      const float ref = static_cast<float>(kWeightBits) - (m == -INFINITY ? 0.0f : m);
+      // Weights carry 2^ratio, the value scale against rm.  One below 2^-60
+      // counts as that; a scale of 0 has codes of 0.
+      const float base_m = m == -INFINITY ? 0.0f : m, base_r = base_m - (rm == -INFINITY ? 0.0f : rm);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) ratio[b] = term[b].y == -INFINITY ? 0.0f : fmaxf(term[b].y + base_r, -60.0f);
+      const float ref = static_cast<float>(kWeightBits) - base_m;
       float off[4], part[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
@@ -751,7 +757,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
     }
 
     l += __shfl_xor(l, 32, 64);
-    const float unit = exp2_hw(vtop) * ldexpf(1.0f, -kWeightBits);
+    const float unit = rm == -INFINITY ? 0.0f : exp2_hw(rm - m - static_cast<float>(kWeightBits));
     int end_lane = threadIdx.x & 63;
     asm volatile("" : "+v"(end_lane));
     const int end_h = end_lane >> 5, end_r = wave * 32 + (end_lane & 31);

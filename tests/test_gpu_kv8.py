@@ -675,3 +675,34 @@ def test_replayed_batches_larger_than_a_captured_grid():
             outs.append([b.download(np.float32)[:seqs * count * heads * dim] for b in bufs[i][3:]])
         for a, b in zip(*outs):
             assert np.isfinite(a).all() and np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("count", [6, 60])
+@pytest.mark.parametrize("big", [2.0**20, 2.0**60])
+def test_attention_next_to_large_values(count, big, dim):
+    """Values far larger than the rest, behind a row's position or under
+    scores that leave them no weight, cost the other values no bits: a row's
+    error counts against the values that it takes."""
+    rng = np.random.default_rng(35)
+    start, heads, kv = 61, 4, 2
+    n = start + count
+    k, v = rows_of(rng, n, kv, dim, 0.0), rows_of(rng, n, kv, dim, 0.0)
+    q = rows_of(rng, count, heads, dim, 0.0)
+    k[16:32], q[:, :, 0] = 0.0, 4.0
+    k[16:32, :, 0] = -160.0  # scores of -80: weights under 2^-100
+    v[16:32] *= np.float32(big)
+    last = n - 1 - (n - 1) % 16  # the last block: rows before it do not see it
+    v[last:] *= np.float32(big)
+    pool = Pool(rng, heads, kv, dim, 32, [n])
+    pool.append([0], [n], None, k, v)
+    got = pool.attention([start], [count], q, 0.125)
+    kq, vq = R.quantize(k), R.quantize(v)
+    rows = last - start
+    assert rows > 0
+    want = R.attend(q[:rows], kq[:last], vq[:last], start, 0.125)
+    small = vq[:last].copy()
+    small[16:32] = 0.0
+    bound = R.attend_bound(q[:rows], kq[:last], small, 0.125)
+    assert np.abs(want).max() > 20 * bound
+    assert np.abs(got[:rows] - want).max() <= bound
