@@ -249,8 +249,9 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
       }
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      bad = bad || __shfl_xor(bad, 16, 64);
-      bad = bad || __shfl_xor(bad, 32, 64);
+      // (Every lane takes part in an exchange: no short-circuit.)
+      bad |= __shfl_xor(static_cast<int>(bad), 16, 64) != 0;
+      bad |= __shfl_xor(static_cast<int>(bad), 32, 64) != 0;
       int e;
       (void)frexpf(top, &e);  // top < 2^e
       if (bad || !(top > 0.0f)) e = 0;

@@ -706,3 +706,29 @@ def test_attention_next_to_large_values(count, big, dim):
     bound = R.attend_bound(q[:rows], kq[:last], small, 0.125)
     assert np.abs(want).max() > 20 * bound
     assert np.abs(got[:rows] - want).max() <= bound
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 0.2])
+@pytest.mark.parametrize("count", [1, 6, 70])
+def test_attention_odd_rows_and_scales(count, scale):
+    """A scale of 0 (the values' mean) and a negative one; a row of q with inf
+    or NaN gives NaN and leaves the others alone; blocks of zeros and of
+    denormal numbers among the history."""
+    rng = np.random.default_rng(36)
+    start, heads, kv, dim = 90, 4, 2, 64
+    n = start + count
+    k, v = rows_of(rng, n, kv, dim, 0.0), rows_of(rng, n, kv, dim, 0.0)
+    k[0:16], v[16:32] = 0.0, 0.0
+    k[32:48] *= np.float32(1e-40)
+    v[48:64] *= np.float32(1e-40)
+    pool = Pool(rng, heads, kv, dim, 32, [n])
+    pool.append([0], [n], None, k, v)
+    q = rows_of(rng, count, heads, dim, 0.0)
+    kq, vq = R.quantize(k), R.quantize(v)
+    want, bound = R.attend(q, kq, vq, start, scale), R.attend_bound(q, kq, vq, scale)
+    q[0, 1, 7], q[count - 1, 2, 63] = np.nan, np.inf
+    got = pool.attention([start], [count], q, scale)
+    odd = np.zeros((count, heads), bool)
+    odd[0, 1] = odd[count - 1, 2] = True
+    assert np.isnan(got[odd]).all()
+    assert np.abs(got[~odd] - want[~odd]).max() <= bound
