@@ -341,8 +341,9 @@ int llmi_hip_kv8_sizes(const llmi_kv8_shape* shape, size_t* code_bytes, size_t* 
  * tables; after a captured attention only batches with work of the kinds that
  * it was captured for: single tokens or drafts of up to as many rows (tokens
  * x heads / kv_heads, up to 64 a sequence) as were set then, and longer pieces
- * if there were any; a graph captured with an empty batch serves every kind).  Launches of one plan must not overlap; two streams or two graphs
- * that run at once need a plan each.
+ * if there were any; a graph captured with an empty batch serves every kind).
+ * Launches of one plan must not overlap; two streams or two graphs that run at
+ * once need a plan each.
  * Refused (LLMI_ERR_ARG): a slot or page out of range, a negative start or
  * count, a table too short, more than the plan was created for.
  * llmi_hip_kv8_check makes the same checks, without limits of a plan, and
@@ -384,8 +385,12 @@ int llmi_hip_kv8_append_dev(const llmi_hip_kv8_plan* plan, const llmi_kv8_layer*
  * with the keys and values of head h / (heads / kv_heads), as the cache holds
  * them (the batch's own tokens have been appended before).  q and out [tokens]
  * [heads][head_dim] with strides as above; out may be q.  Sums and the
- * softmax in fp32 with q and the weights carried to 22 bits or more; results do not depend on
- * the order in which workgroups run. */
+ * softmax in fp32, q carried to 22 bits or more of its row's largest, the
+ * weights (times the value scales) to 22 bits or more of their row's largest;
+ * results do not depend on the order in which workgroups run.  The sum of
+ * weights in [0, 1] times values is taken in fp32 before its division: values
+ * of more than 2^127 / positions may give inf.  inf or NaN in a row of q, or in
+ * a block that it sees, gives NaN for that row and head alone. */
 int llmi_hip_kv8_attention_dev(const llmi_hip_kv8_plan* plan, const llmi_kv8_layer* layer, const float* q,
                                size_t q_stride, float scale, float* out, size_t out_stride, void* stream);
 /* The cached keys and values of the batch's positions, code * scale, as fp32

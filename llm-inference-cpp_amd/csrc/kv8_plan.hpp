@@ -62,11 +62,10 @@ struct JoinItem {
 // against 105, 32 over 2000 23 against 30, 16 drafts of 3 to 6 tokens 30
 // against 32; against 128, 4 drafts of 8 tokens over 2000 15 against 18.
 // `many` work: 512, the two workgroups that a compute unit holds (up to 128
-// dims); its pieces
-// are of that size with the rest in the last one, so that the short ones fill
-// what short histories leave (512 units so against 768 in equal pieces: 2048
-// tokens over 6144 435 us against 449, 1000 over 3000 133 against 145, 8
-// prompts of 512 over 2000, 14/2 heads of 64, 86 against 97).
+// dims); its pieces are of that size with the rest in the last one, so that the
+// short ones fill what short histories leave (512 units so against 768 in equal
+// pieces: 2048 tokens over 6144 435 us against 449, 1000 over 3000 133 against
+// 145, 8 prompts of 512 over 2000, 14/2 heads of 64, 86 against 97).
 constexpr std::size_t kFewTarget = 256, kFewLeast = 8 * kTile;
 constexpr std::size_t kManyTarget = 512, kManyLeast = 4 * kTile;
 // Prompts whose pieces would be shorter than kManyShort that way: one unit for
@@ -83,8 +82,8 @@ constexpr std::size_t kUnits = 256, kManyShort = 4 * kTile;
 // positions, 9/3 heads of 64, 16 us against 21 without that, one over 5000 9.4
 // against 14).  `many`: nothing where whole histories leave compute units
 // without work (one prompt of 1024 tokens of 14/2 heads of 64 20.5 us against
-// 25), else kManyGain (4 prompts of 512 tokens behind 300, 32/8 heads of 128, 53 us
-// against 73; 2 of 500 behind 1000 56 against 70).
+// 25), else kManyGain (4 prompts of 512 tokens behind 300, 32/8 heads of 128,
+// 53 us against 73; 2 of 500 behind 1000 56 against 70).
 constexpr std::size_t kFewGain = 28 * kTile, kFewGainAt = 4 * 128, kFewGainMost = 40 * kTile;
 constexpr std::size_t kManyGain = 12 * kTile;
 
