@@ -28,7 +28,10 @@ inline hipStream_t pick(void* s) { return s != nullptr ? static_cast<hipStream_t
 #define LLMI_TRY_HIP(expr)                                                                        \
   do {                                                                                            \
     const hipError_t err_ = (expr);                                                               \
-    if (err_ != hipSuccess) return ::llmi_hip::fail(LLMI_ERR_HIP, std::string(#expr) + ": " + hipGetErrorString(err_)); \
+    if (err_ != hipSuccess) {                                                                     \
+      (void)hipGetLastError(); /* reported here: not by the next launch */                        \
+      return ::llmi_hip::fail(LLMI_ERR_HIP, std::string(#expr) + ": " + hipGetErrorString(err_)); \
+    }                                                                                             \
   } while (0)
 
 #define LLMI_REQUIRE(cond, msg)                                   \

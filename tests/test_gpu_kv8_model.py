@@ -185,3 +185,14 @@ def test_refusals():
     with pytest.raises(ValueError):
         step(model, [0], [0], [2], [[0]], [1])
     assert np.isfinite(step(model, [0], [0], [3], [[0]], [1, 2, 3])).all()
+
+
+def test_a_cache_that_does_not_fit_leaves_no_error_behind():
+    cfg = CONFIGS["llama_4x32"]
+    tensors, _ = weights(cfg, H.F32)
+    model = H.Model(cfg, tensors, H.F32)
+    cache = model.new_kv8_cache(4, 16, 1, 8)
+    want = model.forward_kv8(cache, [0], [0], [3], [[1]], [5, 6, 7])
+    with pytest.raises(H.HipError, match="out of memory"):
+        model.new_kv8_cache(2**31 - 1, 16, 1, 8)  # 4 TiB of keys
+    assert np.array_equal(model.forward_kv8(cache, [0], [0], [3], [[1]], [5, 6, 7]), want)
