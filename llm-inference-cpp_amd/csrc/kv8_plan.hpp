@@ -290,7 +290,9 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
     each(few, [&](std::size_t, std::size_t, std::size_t, std::size_t len) { reach += len * sh.kv_heads; });
     std::size_t target = few ? kFewTarget : kManyTarget;
     if (!few && reach < kManyTarget * kManyShort) target = kUnits;
-    return std::max(least, (reach / target + least - 1) / least * least);
+    // (Rounded up throughout: full pieces x heads are at most the target.)
+    const std::size_t each_unit = (reach + target - 1) / target;
+    return std::max(least, (each_unit + least - 1) / least * least);
   };
   std::size_t whole = 0;  // units of `many` work without pieces
   each(false, [&](std::size_t, std::size_t, std::size_t, std::size_t) { whole += sh.kv_heads; });

@@ -1,0 +1,20 @@
+"""CPU tests of the rules that the paged 8-bit key/value cache's host side
+keeps (csrc/kv8_plan.hpp), each walked by a native program."""
+
+import os
+import subprocess
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def run_native(name, tmp_path):
+    exe = str(tmp_path / name)
+    subprocess.run(["g++", "-std=c++20", "-O1", "-g", "-fsanitize=address,undefined", "-I", os.path.join(ROOT, "include"),
+                    os.path.join(ROOT, "tests", "native", name + ".cpp"), "-o", exe], check=True)
+    out = subprocess.run([exe], capture_output=True, text=True)
+    assert out.returncode == 0, out.stdout + out.stderr
+
+
+def test_batches_stay_within_a_plans_limits(tmp_path):
+    """A plan takes every batch of its sequences and tokens, however long the histories."""
+    run_native("kv8_limits", tmp_path)
