@@ -820,7 +820,7 @@ int launch_attention(const llmi_hip_kv8_plan* p, const llmi_kv8_layer& layer, co
   const bool any = captured && l.tokens == 0;
   const bool has_few = any || !l.few.empty(), has_many = any || !l.many.empty();
   const int most_rows = few_rows(p->g.dim);
-  const int rows = any ? most_rows : captured ? std::min((l.few_rows + 3) / 4 * 4, most_rows) : l.few_rows;
+  const int rows = any ? most_rows : captured ? captured_rows(l, p->g.dim) : l.few_rows;
   if (captured) {
     p->captured_few = std::min(p->captured_few, has_few ? rows : 0);
     p->captured_many = p->captured_many && has_many;

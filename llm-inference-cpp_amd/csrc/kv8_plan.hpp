@@ -108,6 +108,7 @@ struct Lists {
   std::vector<AttnItem> few, many;
   std::vector<JoinItem> join;
   std::int32_t few_rows = 0;  // most rows of a `few` item
+  std::int32_t few_seq_rows = 0;  // most rows of a sequence whose work is `few`
   // A workgroup that joins takes join_at rows of an item at a time: one where
   // rows are few (and pieces many), up to as many as its threads hold where
   // they are enough to fill the chip.
@@ -161,6 +162,14 @@ inline Limits limits(const llmi_kv8_shape& sh, std::size_t seqs, std::size_t tok
   const std::size_t rows = static_cast<std::size_t>(few_rows(static_cast<int>(sh.head_dim)));
   return {tokens / kBlk + 2 * busy, few + kFewMax / rows * busy, many + tokens * group / kManyRows + busy,
           2 * few * (rows / kSlotRows) + 2 * many * (kManyRows / kSlotRows), few + many};
+}
+
+// The rows of a `few` item that an attention captured with this batch has room
+// for: those of any batch whose sequences have no more rows than this one's.
+// (Not few_rows: shared out over several items, more rows can make shorter
+// items; 20 rows two of 12 and 8, 16 rows one of 16.)
+inline std::int32_t captured_rows(const Lists& l, int dim) {
+  return std::min((l.few_seq_rows + 3) / 4 * 4, few_rows(dim));
 }
 
 // Checks a batch; returns the reason of a refusal.  Fills in the sequences,
@@ -335,6 +344,8 @@ inline std::string build(const llmi_kv8_shape& sh, std::size_t seqs, const std::
   if (sh.head_dim <= 128 && l.many.size() > at_once && l.many.size() * sh.kv_heads <= 2 * kUnits)
     std::reverse(l.many.begin() + static_cast<std::ptrdiff_t>(at_once), l.many.end());
   for (const AttnItem& it : l.few) l.few_rows = std::max(l.few_rows, it.rows);
+  for (const Seq& q : l.seqs)
+    if (rows_of(q) <= kFewMax) l.few_seq_rows = std::max(l.few_seq_rows, static_cast<std::int32_t>(rows_of(q)));
   if (l.join.size() * sh.kv_heads * static_cast<std::size_t>(l.join_rows) > kJoinFill)
     l.join_at = kJoinThreads * 4 / static_cast<std::int32_t>(sh.head_dim);
   return {};

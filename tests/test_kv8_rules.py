@@ -18,3 +18,8 @@ def run_native(name, tmp_path):
 def test_batches_stay_within_a_plans_limits(tmp_path):
     """A plan takes every batch of its sequences and tokens, however long the histories."""
     run_native("kv8_limits", tmp_path)
+
+
+def test_captured_attention_has_room_for_shorter_drafts(tmp_path):
+    """A launch captured for drafts takes every shorter one, however their rows are shared out."""
+    run_native("kv8_captured", tmp_path)
