@@ -301,8 +301,8 @@ int llmi_hip_argmax_dev(const float* x, size_t n, int32_t* out, void* stream);
  *   v       [pages][kv_heads][page_tokens/16][head_dim/16][16 dims][16 positions]
  *   scales  [pages][kv_heads][page_tokens/16][2]   (the keys', the values')
  *   open    [slots][kv_heads][2][2][16][head_dim]  block parity, then k / v:
- *           the fp32 rows of the last two blocks that a sequence's appends
- *           wrote, under the sequence's slot.
+ *           the fp32 rows of the last block of each parity that the appends
+ *           under a slot wrote (of a call's blocks, the last two).
  * Which pages a sequence has is the caller's: page p of its table holds
  * positions p * page_tokens ...  Full pages may be shared by sequences. */
 #define LLMI_KV8_BLOCK 16
@@ -367,10 +367,18 @@ int llmi_hip_kv8_plan_free(llmi_hip_kv8_plan* plan);
  *                                          both NULL: none
  * in 64 bits, rounded once to fp32.  q goes to q_out (q_out == q with equal
  * strides: in place); q NULL leaves q out (q_out is not touched).  k and v go
- * to the cache.  A sequence's start is its length so far, or a whole number
- * of blocks (pages shared with another sequence before it); of what was
- * appended under its slot it may be taken back to any position from the block
- * before its last one on, and written again from there.
+ * to the cache.  A sequence's start is its length so far, a position that it
+ * is taken back to, to be written again from there, or a whole number of
+ * blocks (pages shared with another sequence before it).  The rows before a
+ * start that is not a whole number of blocks come from `open`, so its block
+ * must be the last one of its parity (odd or even) that appends under the
+ * slot have written: the sequence's last block and, unless a block of its
+ * parity was written since, the one before it.  A sequence of 40 positions
+ * (blocks 0 to 2) may go back to 16 or any later position; gone back to 20
+ * and written to 21, into block 1 again, but not inside block 0, whose rows
+ * block 2 has replaced (0 itself is allowed).  Nothing checks that here,
+ * `open` being the caller's: such a start quantizes rows of another block.
+ * (llmi_hip_model_forward_kv8 refuses it.)
  * LLMI_ERR_ARG: NULL pointers, strides too short, tables of fewer positions
  * than the batch has; LLMI_ERR_STATE: no batch set, or a batch that cannot be
  * appended (set without slots, two sequences with one slot, a page for new
@@ -470,7 +478,9 @@ int llmi_hip_model_forward(llmi_hip_model* model, const int32_t* tokens, size_t 
  * reference's: they differ by what rounding them to 1/254 of their block's
  * largest does.  Errors: LLMI_ERR_ARG for a batch, token id or token count
  * that is refused (nothing has run then), LLMI_ERR_STATE for a cache of
- * another model or positions past the context. */
+ * another model, positions past the context, or a start inside a block whose
+ * earlier rows are not held under the sequence's slot (llmi_hip_kv8_append_dev
+ * says which are; after a step that failed on its way, none). */
 typedef struct llmi_hip_kv8_cache llmi_hip_kv8_cache;
 int llmi_hip_model_new_kv8_cache(llmi_hip_model* model, size_t pages, size_t page_tokens, size_t slots,
                                  size_t max_tokens, llmi_hip_kv8_cache** cache);

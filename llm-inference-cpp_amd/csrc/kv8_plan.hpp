@@ -104,6 +104,30 @@ constexpr Divisor divisor(std::uint32_t d) {
   return {static_cast<std::uint32_t>((std::uint64_t{1} << (27 + log)) / d + 1), 27 + log};
 }
 
+// The blocks whose rows a slot of `open` holds: of each parity the last one
+// that an append wrote.  An append that starts inside a block reads the rows
+// before its start there.
+struct Held {
+  std::int32_t block[2] = {-1, -1}, rows[2] = {0, 0};
+  bool serves(std::int32_t start) const {
+    const std::int32_t b = start / kBlk;
+    return start % kBlk == 0 || (block[b & 1] == b && rows[b & 1] >= start % kBlk);
+  }
+  // After an append of `count` > 0 tokens at a start that was served.
+  void wrote(std::int32_t start, std::int32_t count) {
+    const std::int32_t end = start + count, first = start / kBlk, last = (end - 1) / kBlk;
+    const int p = last & 1;
+    block[p] = last;
+    rows[p] = end - last * kBlk;
+    if (first < last) {
+      block[1 - p] = last - 1;
+      rows[1 - p] = kBlk;
+    } else if (block[1 - p] > last) {  // taken back: those positions are no longer the sequence's
+      block[1 - p] = -1;
+    }
+  }
+};
+
 struct Lists {
   std::vector<AttnItem> few, many;
   std::vector<JoinItem> join;

@@ -34,6 +34,7 @@
 #include "common.hpp"
 #include "exact_math.hpp"
 #include "glue_math.hpp"
+#include "kv8_plan.hpp"
 
 namespace llmi_hip {
 namespace {
@@ -1536,6 +1537,7 @@ struct llmi_hip_kv8_cache {
   float *scales = nullptr, *open = nullptr;
   std::int32_t* rows = nullptr;  // the last token's row of each sequence of a step
   llmi_hip_kv8_plan* plan = nullptr;
+  std::vector<llmi_hip::kv8::Held> held;  // what each slot of `open` holds (all layers alike)
   ~llmi_hip_kv8_cache() {
     (void)llmi_hip_kv8_plan_free(plan);
     for (void* p : {static_cast<void*>(k), static_cast<void*>(v), static_cast<void*>(scales), static_cast<void*>(open),
@@ -2372,6 +2374,11 @@ int llmi_hip_model_new_kv8_cache(llmi_hip_model* m, size_t pages, size_t page_to
   const std::size_t entries = slots * ceil_div(m->c.max_position_embeddings, page_tokens);
   if (int rc = llmi_hip_kv8_plan_create(&c->shape, slots, max_tokens, std::min<std::size_t>(entries, 1u << 28), &c->plan))
     return rc;
+  try {
+    c->held.resize(slots);
+  } catch (const std::bad_alloc&) {
+    return fail(LLMI_ERR_HIP, "new_kv8_cache: out of host memory");
+  }
   const std::size_t n = m->layers.size();
   LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&c->k), n * c->code_bytes));
   LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&c->v), n * c->code_bytes));
@@ -2401,6 +2408,9 @@ int llmi_hip_model_forward_kv8(llmi_hip_model* m, llmi_hip_kv8_cache* c, size_t 
       const std::size_t len = static_cast<std::size_t>(starts[i]) + static_cast<std::size_t>(counts[i]);
       if (len > m->c.max_position_embeddings)
         return fail(LLMI_ERR_STATE, "forward_kv8: sequence longer than the model's context");
+      if (counts[i] > 0 && !c->held[static_cast<std::size_t>(slots[i])].serves(starts[i]))
+        return fail(LLMI_ERR_STATE, "forward_kv8: the rows before position " + std::to_string(starts[i]) + " of sequence " +
+                                        std::to_string(i) + " in its block are not held under its slot (any more)");
       T += static_cast<std::size_t>(counts[i]);
       longest = std::max(longest, len);
       if (counts[i] > 0) last.push_back(static_cast<std::int32_t>(T) - 1);
@@ -2417,10 +2427,22 @@ int llmi_hip_model_forward_kv8(llmi_hip_model* m, llmi_hip_kv8_cache* c, size_t 
     if (int rc = llmi_hip_kv8_plan_set(c->plan, seqs, slots, starts, counts, tables, table_stride, s)) return rc;
     LLMI_TRY_HIP(hipMemcpyAsync(m->ws.ids, tokens, T * sizeof(std::int32_t), hipMemcpyHostToDevice, s));
     LLMI_TRY_HIP(hipMemcpyAsync(c->rows, last.data(), last.size() * sizeof(std::int32_t), hipMemcpyHostToDevice, s));
+    // (A step that fails on its way may have written some layers' rows: what its slots hold is unknown then.)
+    std::vector<llmi_hip::kv8::Held> after;
+    for (std::size_t i = 0; i < seqs; ++i) {
+      if (counts[i] == 0) continue;
+      llmi_hip::kv8::Held& h = c->held[static_cast<std::size_t>(slots[i])];
+      after.push_back(h);
+      after.back().wrote(starts[i], counts[i]);
+    }
+    for (std::size_t i = 0; i < seqs; ++i)
+      if (counts[i] > 0) c->held[static_cast<std::size_t>(slots[i])] = {};
     if (int rc = forward_kv8_rows(m, c, T, last.size(), s)) return rc;
     if (logits != nullptr)
       LLMI_TRY_HIP(hipMemcpyAsync(logits, m->ws.logits, last.size() * m->V * sizeof(float), hipMemcpyDeviceToHost, s));
     LLMI_TRY_HIP(hipStreamSynchronize(s));
+    for (std::size_t i = 0, n = 0; i < seqs; ++i)
+      if (counts[i] > 0) c->held[static_cast<std::size_t>(slots[i])] = after[n++];
     return LLMI_OK;
   } catch (const std::bad_alloc&) {
     return fail(LLMI_ERR_HIP, "forward_kv8: out of host memory");

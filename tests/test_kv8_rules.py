@@ -23,3 +23,8 @@ def test_batches_stay_within_a_plans_limits(tmp_path):
 def test_captured_attention_has_room_for_shorter_drafts(tmp_path):
     """A launch captured for drafts takes every shorter one, however their rows are shared out."""
     run_native("kv8_captured", tmp_path)
+
+
+def test_sequences_taken_back(tmp_path):
+    """A start inside a block is allowed exactly where `open` still holds the block's earlier rows."""
+    run_native("kv8_open", tmp_path)
