@@ -397,7 +397,8 @@ int llmi_hip_kv8_append_dev(const llmi_hip_kv8_plan* plan, const llmi_kv8_layer*
  * weights (times the value scales) to 22 bits or more of their row's largest;
  * results do not depend on the order in which workgroups run.  The sum of
  * weights in [0, 1] times values is taken in fp32 before its division: values
- * of more than 2^127 / positions may give inf.  inf or NaN in a row of q, or in
+ * of more than 2^127 / positions may give inf, and results below 2^-120 have
+ * fewer bits.  inf or NaN in a row of q, or in
  * a block that it sees, gives NaN for that row and head alone. */
 int llmi_hip_kv8_attention_dev(const llmi_hip_kv8_plan* plan, const llmi_kv8_layer* layer, const float* q,
                                size_t q_stride, float scale, float* out, size_t out_stride, void* stream);

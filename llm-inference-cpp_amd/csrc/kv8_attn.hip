@@ -302,11 +302,22 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
 
     for (int base = it.lo + wave * kTile; base < it.hi; base += kWaves * kTile) {
       if (base / kBlk + grp > last_block) sc = make_float2(0.0f, 0.0f);
-      float ks[4], vs[4];
+      // The blocks' value scales (0 where not finite; NaN then in `odd`), and
+      // their mantissas and exponents apart: a weight times a scale is taken in
+      // these two steps, so that small scales cost no bits.
+      const auto of_block = [](float x, int b) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 16 * b)); };
+      const float sc_value = sc.y < INFINITY ? sc.y : 0.0f, sc_odd = sc.y * 0.0f;
+      const float sc_mant = __builtin_amdgcn_frexp_mantf(sc_value);
+      const int sc_exp = __builtin_amdgcn_frexp_expf(sc_value);
+      float ks[4], vs[4], vm[4], odd[4];
+      int ve[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        ks[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sc.x), 16 * b));
-        vs[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sc.y), 16 * b));
+        ks[b] = of_block(sc.x, b);
+        vs[b] = of_block(sc_value, b);
+        vm[b] = of_block(sc_mant, b);
+        odd[b] = of_block(sc_odd, b);
+        ve[b] = __builtin_amdgcn_readlane(sc_exp, 16 * b);
       }
       float x[MT][4];
 #pragma unroll
@@ -324,9 +335,6 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
       fetch_values();
       if (base + kWaves * kTile < it.hi) fetch_keys(base + kWaves * kTile);
       __builtin_amdgcn_sched_barrier(0);
-      float vf_s[4];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) vf_s[b] = vs[b] < INFINITY ? vs[b] : 0.0f;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         float mx = fmaxf(fmaxf(fmaxf(x[mt][0], x[mt][1]), fmaxf(x[mt][2], x[mt][3])), m[mt]);
@@ -340,15 +348,15 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
           const bool seen = base + b * kBlk + lo16 <= limit[mt];
           const float p = exp2_hw(x[mt][b] - ref);
           // A value scale that is inf or NaN shows in the sum of the rows that see the block.
-          if (seen) sum += fmaf(vs[b], 0.0f, p);
-          w[b] = p * vf_s[b];
-          top = fmaxf(top, w[b]);
+          if (seen) sum += p + odd[b];
+          w[b] = p * vm[b];
+          top = fmaxf(top, p * vs[b]);
         }
-        // The row's largest is below 2^we (-96: 2^(we - 30) stays a normal number).
-        const int we = max(__builtin_amdgcn_frexp_expf(row16_max(top)), -96);
+        // The row's largest is below 2^we (for which a denormal product will do).
+        const int we = __builtin_amdgcn_frexp_expf(row16_max(top));
 #pragma unroll
         for (int b = 0; b < 4; ++b)
-          sh.w[wave][b][grp][lo16] = digits(static_cast<int>(rintf(ldexpf(w[b], 30 - we))));
+          sh.w[wave][b][grp][lo16] = digits(static_cast<int>(rintf(ldexpf(w[b], 30 - we + ve[b]))));
         l[mt] = fmaf(l[mt], keep, sum);
         __builtin_amdgcn_wave_barrier();
         // Digit row lo16 (head lo16 / 4, digit lo16 % 4) over this lane group's block.
@@ -364,12 +372,11 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
           wd[j] = static_cast<int>(__builtin_amdgcn_perm(b2, a, 0x05040100u));
         }
         __builtin_amdgcn_wave_barrier();
-        const float from_fix = ldexpf(1.0f, we - 30);
 #pragma unroll
         for (int g = 0; g < kG; ++g) {
           i4 acc = {0, 0, 0, 0};
           acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wd, vf[g], acc, 0, 0, 0);
-          o[mt][g] = fmaf(o[mt][g], keep, undigit(acc) * from_fix);
+          o[mt][g] = fmaf(o[mt][g], keep, ldexpf(undigit(acc), we - 30));
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -428,8 +435,8 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
 // accumulators to the second's operand without leaving the registers: a lane
 // holds positions 4h .. 4h+3 and 8+4h .. of each 16 (h = lane / 32), and the
 // value tile is staged in that order.
-// w = p * value scale * 2^kWeightBits / the row's largest product of the two so
-// far: block scales differ along the sum, so they ride on the weights (against
+// w = p * value scale * 2^kWeightBits over (to a power of two) the row's
+// largest product of the two so far: block scales differ along the sum, so they ride on the weights (against
 // the largest scale alone, a block that a row does not see, or gives no weight,
 // would take bits from the others).
 // Why two parts: one fp16 part of q or w is off by 2^-12, which shows as 1e-4
@@ -565,18 +572,20 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
     for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-    // m: what scores are taken against, at most kSlack below the largest so
-    // far; rm: the same for scores plus log2 of the value scale.
+    // m: what scores are taken against, about kSlack below the largest so far
+    // at most; rm: the same for scores plus log2 of the value scale.  Both are
+    // whole numbers, so that factors between them are exact.
     float m = -INFINITY, l = 0.0f, rm = -INFINITY;
 
     // What the products take of the block that `fetch` brought: the key scale
-    // times the softmax's, log2 of the value scale (-inf: its codes are 0, or
-    // masked), and NaN if a scale is not finite.
+    // times the softmax's, the value scale's exponent (-inf: its codes are 0,
+    // or masked), NaN if a scale is not finite, and log2 of the value scale's
+    // mantissa (apart from the exponent, next to which it would lose bits).
     const auto block_terms = [&]() {
       const bool fin = sreg.y > 0.0f && sreg.y < INFINITY;
-      const float lg = __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(sreg.y)) +
-                       static_cast<float>(__builtin_amdgcn_frexp_expf(sreg.y));
-      return sreg_live ? make_float4(scale * sreg.x, fin ? lg : -INFINITY, fmaf(sreg.x, 0.0f, sreg.y * 0.0f), 0.0f)
+      return sreg_live ? make_float4(scale * sreg.x, fin ? static_cast<float>(__builtin_amdgcn_frexp_expf(sreg.y)) : -INFINITY,
+                                     fmaf(sreg.x, 0.0f, sreg.y * 0.0f),
+                                     fin ? __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(sreg.y)) : 0.0f)
                        : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
     };
     // Staging in kPieces steps, each four codes of every lane to fp16; every
@@ -677,7 +686,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
       // kSlack (weights may be up to 2^kSlack before that).
       const bool grown = mx > m + kSlack, risen = rx > rm + kSlack;
       if (__any(grown || risen)) {
-        const float now = grown ? mx : m, r_now = risen ? rx : rm;
+        const float now = grown ? rintf(mx) : m, r_now = risen ? rintf(rx) : rm;
         l *= now == -INFINITY ? 0.0f : exp2_hw(m - now);
         const float rescale = r_now == -INFINITY ? 0.0f : exp2_hw(rm - r_now);
         m = now;
@@ -691,7 +700,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
       // counts as that; a scale of 0 has codes of 0.
       const float base_m = m == -INFINITY ? 0.0f : m, base_r = base_m - (rm == -INFINITY ? 0.0f : rm);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) ratio[b] = term[b].y == -INFINITY ? 0.0f : fmaxf(term[b].y + base_r, -60.0f);
+      for (int b = 0; b < 4; ++b) ratio[b] = term[b].y == -INFINITY ? 0.0f : fmaxf(term[b].y + base_r + term[b].w, -60.0f);
       const float ref = static_cast<float>(kWeightBits) - base_m;
       float off[4], part[4];
 #pragma unroll
@@ -746,7 +755,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
       __builtin_amdgcn_sched_barrier(0);
       float sum = 0.0f;
 #pragma unroll
-      for (int b = 0; b < 4; ++b) sum = fmaf(part[b], exp2_hw(-static_cast<float>(kWeightBits) - ratio[b]), sum);
+      for (int b = 0; b < 4; ++b) sum = fmaf(part[b], exp2_hw(-ratio[b]) * (1.0f / (1 << kWeightBits)), sum);
       if (bad != bad) {
         // A scale that is inf or NaN shows in the rows that see a position of its block.
 #pragma unroll
@@ -758,7 +767,9 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
     }
 
     l += __shfl_xor(l, 32, 64);
-    const float unit = rm == -INFINITY ? 0.0f : exp2_hw(rm - m - static_cast<float>(kWeightBits));
+    // What the output's sums are to be multiplied with is 2^unit.
+    const int unit = static_cast<int>(fminf(fmaxf(rm - m, -1000.0f), 1000.0f)) - kWeightBits;
+    const float any_value = rm == -INFINITY ? 0.0f : 1.0f;
     int end_lane = threadIdx.x & 63;
     asm volatile("" : "+v"(end_lane));
     const int end_h = end_lane >> 5, end_r = wave * 32 + (end_lane & 31);
@@ -771,16 +782,18 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<float4*>(A.parts + part * HD + 32 * d + 8 * i + 4 * end_h) =
-              make_float4(o[d][4 * i] * unit, o[d][4 * i + 1] * unit, o[d][4 * i + 2] * unit, o[d][4 * i + 3] * unit);
+              make_float4(ldexpf(o[d][4 * i] * any_value, unit), ldexpf(o[d][4 * i + 1] * any_value, unit),
+                          ldexpf(o[d][4 * i + 2] * any_value, unit), ldexpf(o[d][4 * i + 3] * any_value, unit));
     } else if (live) {
       float* dst = A.out + static_cast<std::size_t>(it.row + mine.tok) * A.out_stride + mine.off;
-      const float f = unit / l;
+      const float f = any_value / l;
 #pragma unroll
       for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<f4*>(dst + 32 * d + 8 * i + 4 * end_h) =
-              f4{o[d][4 * i] * f, o[d][4 * i + 1] * f, o[d][4 * i + 2] * f, o[d][4 * i + 3] * f};
+              f4{ldexpf(o[d][4 * i] * f, unit), ldexpf(o[d][4 * i + 1] * f, unit), ldexpf(o[d][4 * i + 2] * f, unit),
+                 ldexpf(o[d][4 * i + 3] * f, unit)};
     }
   }
 }

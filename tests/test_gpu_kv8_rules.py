@@ -94,3 +94,49 @@ def test_model_refuses_rows_that_are_not_held():
     step(two, 20, 1)
     for start, n in ((21, 9), (17, 1), (18, 20), (33, 4), (0, 2), (1, 50)):
         assert np.array_equal(step(one, start, n), step(two, start, n)), start
+
+
+@pytest.mark.parametrize("power", [-113, -100, -60, 60, 90])
+@pytest.mark.parametrize("heads,kv,dim,start,count", [(4, 2, 64, 90, 1), (4, 2, 128, 90, 6), (8, 2, 64, 90, 70), (2, 1, 256, 40, 60), (4, 1, 64, 4000, 1), (4, 2, 64, 2600, 40)])
+def test_attention_of_tiny_and_huge_values(heads, kv, dim, start, count, power):
+    """Histories wholly of values about 2^power: a row's error counts against
+    its own values, whatever kernel takes it and in however many pieces."""
+    rng = np.random.default_rng(37 + dim + count)
+    n = start + count
+    k, v = rows_of(rng, n, kv, dim, 0.0), rows_of(rng, n, kv, dim, 0.0)
+    v *= np.float32(2.0**power)
+    pool = Pool(rng, heads, kv, dim, 64, [n])
+    pool.append([0], [n], None, k, v)
+    q = rows_of(rng, count, heads, dim, 0.0)
+    got = pool.attention([start], [count], q, 0.125)
+    kq, vq = R.quantize(k), R.quantize(v)
+    bound = R.attend_bound(q, kq, vq, 0.125)
+    want = R.attend(q, kq, vq, start, 0.125)
+    assert np.abs(want).max() > 20 * bound
+    assert np.abs(got - want).max() <= bound
+
+
+@pytest.mark.parametrize("heads", [16, 64])  # 32 rows a key/value head, and 128
+def test_attention_keeps_value_scales(heads):
+    """Prompts of one block under zero keys: row t is the mean of t + 1 values,
+    every weight 1.  What may be off, in roundings of 2^-24 of the largest
+    value seen: the weights' and scales' digits or parts 4, the logarithm of a
+    scale 2, an exponential 2, the sum's and the output's factors, their
+    product and quotient 8 at most; the sums of n = t + 1 weights and of n
+    products in two parts 3n.  A result this near to 2^-126 has steps of 2^-149."""
+    rng = np.random.default_rng(38)
+    kv, dim, count, seqs = 8, 64, 16, 12
+    pool = Pool(rng, heads, kv, dim, 16, [count] * seqs)
+    k, v = np.zeros((seqs * count, kv, dim), np.float32), rows_of(rng, seqs * count, kv, dim, 0.0)
+    v = v.reshape(seqs, count, kv, dim) * np.exp2(rng.uniform(-113, 100, (seqs, 1, kv, 1)))
+    v = v.astype(np.float32).reshape(k.shape)
+    pool.append([0] * seqs, [count] * seqs, None, k, v)
+    got = pool.attention([0] * seqs, [count] * seqs, rows_of(rng, seqs * count, heads, dim, 0.0), 0.125)
+    got = got.reshape(seqs, count, kv, heads // kv, dim).astype(np.float64)
+    n = np.arange(1, count + 1)[:, None, None, None]
+    for i in range(seqs):
+        vq = R.quantize(v[i * count:(i + 1) * count])[:, :, None]
+        want = np.cumsum(vq, 0) / n
+        seen = np.maximum.accumulate(np.abs(vq).max(-1, keepdims=True), 0)
+        off = np.abs(got[i] - want)
+        assert (off <= seen * (16 + 3 * n) * 2.0**-24 + 2.0**-149).all(), (i, (off / seen).max() * 2**24)
