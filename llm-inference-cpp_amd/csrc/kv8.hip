@@ -447,7 +447,7 @@ bool capturing(hipStream_t s) {
 // room for any batch that its plan takes, fills the chip a few times and
 // goes on from there.
 unsigned grid_for(std::size_t units, bool captured) {
-  return static_cast<unsigned>(std::min<std::size_t>(std::max<std::size_t>(ceil_div(units, kWaves), 1), captured ? 8192 : 1u << 29));
+  return static_cast<unsigned>(std::min<std::size_t>(std::max<std::size_t>(ceil_div(units, kWaves), 1), captured ? 8192 : kMostGroups));
 }
 
 // fn(std::integral_constant<int, head_dim>) for the plan's head size.

@@ -39,6 +39,10 @@ __device__ __forceinline__ int page_of(const Geometry& g, int block) {
 __device__ __forceinline__ std::size_t block_at(const Geometry& g, int id, int page, int block, int h) {
   return (static_cast<std::size_t>(id) * g.kv_heads + h) * g.page_blocks + (block - page * g.page_blocks);
 }
+// Workgroups (of at most 512 threads) of a launch, which has to stay below
+// 2^32 threads; every kernel here goes on with further units from there.
+constexpr std::size_t kMostGroups = std::size_t{1} << 22;
+
 int launch_attention(const llmi_hip_kv8_plan* p, const llmi_kv8_layer& layer, const float* q, std::size_t q_stride,
                      float scale, float* out, std::size_t out_stride, hipStream_t s, bool captured);
 

@@ -179,9 +179,9 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lo16 = lane & 15, grp = lane >> 4;
   const int nfew = A.nfew >= 0 ? A.nfew : A.v.counts->few;
-  const int units = nfew * A.g.kv_heads;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const int item = u / A.g.kv_heads, h = u - item * A.g.kv_heads;
+  const unsigned units = static_cast<unsigned>(nfew) * A.g.kv_heads;
+  for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
+    const int item = static_cast<int>(u / A.g.kv_heads), h = static_cast<int>(u) - item * A.g.kv_heads;
     const AttnItem it = A.v.few[item];
 
     const int last_block = (it.hi - 1) / kBlk;
@@ -481,9 +481,9 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) attention_many(AttnArg
   __shared__ float4 sh_s[2][4];               // a tile's blocks: see block_terms
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nmany = A.nmany >= 0 ? A.nmany : A.v.counts->many;
-  const int units = nmany * A.g.kv_heads;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const int item = u / A.g.kv_heads, head = u - item * A.g.kv_heads;
+  const unsigned units = static_cast<unsigned>(nmany) * A.g.kv_heads;
+  for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
+    const int item = static_cast<int>(u / A.g.kv_heads), head = static_cast<int>(u) - item * A.g.kv_heads;
     const AttnItem it = A.v.many[item];
     // (Opaque: what is computed from it is not kept in registers around the loop over units.)
     int lane = threadIdx.x & 63;
@@ -841,7 +841,7 @@ int launch_attention(const llmi_hip_kv8_plan* p, const llmi_kv8_layer& layer, co
   const auto grid = [&](bool has, std::size_t items, std::size_t most) {
     if (!has) return 0u;
     const std::size_t units = (captured ? most : items) * heads;
-    return static_cast<unsigned>(std::min<std::size_t>(units, captured ? 4096 : 1u << 30));
+    return static_cast<unsigned>(std::min<std::size_t>(units, captured ? 4096 : kMostGroups));
   };
   const unsigned few = grid(has_few, l.few.size(), p->most.few), many = grid(has_many, l.many.size(), p->most.many);
   switch (p->g.dim) {

@@ -140,3 +140,26 @@ def test_attention_keeps_value_scales(heads):
         seen = np.maximum.accumulate(np.abs(vq).max(-1, keepdims=True), 0)
         off = np.abs(got[i] - want)
         assert (off <= seen * (16 + 3 * n) * 2.0**-24 + 2.0**-149).all(), (i, (off / seen).max() * 2**24)
+
+
+def test_as_many_sequences_as_a_plan_takes():
+    """2^20 sequences that read the same page, of 8 heads each: more workgroups
+    than a launch may have (2^32 threads), so each takes several units."""
+    rng = np.random.default_rng(39)
+    kv, dim, seqs, some = 8, 32, 1 << 20, 1 << 12
+    pool = Pool(rng, kv, kv, dim, 16, [3])
+    k, v = rows_of(rng, 3, kv, dim), rows_of(rng, 3, kv, dim)
+    pool.append([0], [3], None, k, v)
+    plan = H.Kv8Plan(pool.shape, seqs, seqs, seqs)
+    plan.set(None, np.full(seqs, 2), np.ones(seqs), np.broadcast_to(pool.tables, (seqs, 1)))
+    q = rows_of(rng, some, kv, dim, 0.0)
+    qb = H.DeviceBuffer.from_array(np.tile(q.reshape(1, -1), (seqs // some, 1)))
+    ob = H.DeviceBuffer.from_array(np.full(seqs * kv * dim, np.nan, np.float32))
+    plan.attention(pool.layer, qb.ptr, 0.2, ob.ptr)
+    H.synchronize()
+    got = ob.download(np.float32).reshape(seqs // some, some, kv, dim)
+    kq, vq = R.quantize(k), R.quantize(v)
+    p = np.exp(0.2 * np.einsum("nhd,jhd->nhj", q.astype(np.float64), kq))
+    want = np.einsum("nhj,jhd->nhd", p / p.sum(-1, keepdims=True), vq)
+    assert np.abs(got[0] - want).max() <= R.attend_bound(q, kq, vq, 0.2)
+    assert all(np.array_equal(x, got[0]) for x in got[1:])
