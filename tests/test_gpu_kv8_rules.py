@@ -1,9 +1,11 @@
 """The paged 8-bit key/value cache on the GPU (llmi_hip_kv8_*): calls that its
-interface allows at the edge of what it was captured or created for."""
+interface allows at the edge of what it was captured or created for, values
+far from 1, and the precision that the attention states."""
 
 import numpy as np
 import pytest
 
+import kv8_precision as P
 import kv8_reference as R
 import llmi_hip as H
 from test_gpu_kv8 import Pool, rows_of
@@ -163,3 +165,16 @@ def test_as_many_sequences_as_a_plan_takes():
     want = np.einsum("nhj,jhd->nhd", p / p.sum(-1, keepdims=True), vq)
     assert np.abs(got[0] - want).max() <= R.attend_bound(q, kq, vq, 0.2)
     assert all(np.array_equal(x, got[0]) for x in got[1:])
+
+
+@pytest.mark.parametrize("shape", P.SHAPES)
+@pytest.mark.parametrize("largest", [1.0, 8.0])
+def test_attention_keeps_22_bits(shape, largest):
+    """q and the weights with fewer bits than promised would show (see kv8_precision)."""
+    heads, kv, dim, start, count = shape
+    q, kq, vq, k, v, _ = P.case(shape, largest)
+    pool = Pool(np.random.default_rng(40), heads, kv, dim, 32, [start + count])
+    pool.append([0], [start + count], None, k, v)
+    got = pool.attention([start], [count], q, P.SCALE)
+    off = np.abs(got - P.attend(q, kq, vq, start)) / P.bound(q, kq, vq, start)
+    assert off.max() <= 1, off.max()
