@@ -545,7 +545,6 @@ int llmi_hip_kv8_plan_create(const llmi_kv8_shape* shape, size_t max_seqs, size_
   p->g.group = p->g.heads / p->g.kv_heads;
   p->g.dim = static_cast<int>(shape->head_dim);
   p->g.page_blocks = static_cast<int>(shape->page_tokens) / kBlk;
-  p->g.block_bytes = static_cast<std::size_t>(kBlk) * shape->head_dim;
   p->g.by_page = divisor(static_cast<std::uint32_t>(p->g.page_blocks));
   p->most = limits(*shape, max_seqs, max_tokens);
   // Kernels count rows of a key/value head and units of work (item and head) in 32 bits.

@@ -26,7 +26,6 @@ struct View {
 struct Geometry {
   int heads, kv_heads, group, dim, page_blocks;
   Divisor by_page;  // divides a block by page_blocks
-  std::size_t block_bytes;  // of one head's block of k (or v): 16 * dim
 };
 
 // Which page of its sequence's table holds a block.

@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
       }
     }
 
-    // Merge the four wavefronts: lane (dim lo16 of each group, head grp).
+    // Merge the wavefronts' states: lane (dim lo16 of each group, head grp).
     __syncthreads();
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -436,9 +436,9 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
 // holds positions 4h .. 4h+3 and 8+4h .. of each 16 (h = lane / 32), and the
 // value tile is staged in that order.
 // w = p * value scale * 2^kWeightBits over (to a power of two) the row's
-// largest product of the two so far: block scales differ along the sum, so they ride on the weights (against
-// the largest scale alone, a block that a row does not see, or gives no weight,
-// would take bits from the others).
+// largest product of the two so far: block scales differ along the sum, so
+// they ride on the weights (against the largest scale alone, a block that a row
+// does not see, or gives no weight, would take bits from the others).
 // Why two parts: one fp16 part of q or w is off by 2^-12, which shows as 1e-4
 // of the result; two are off by 2^-22 or less, below fp32's sums.  That is twice the
 // formula's products: 2048 tokens over 6144 positions of 32/8 heads of 128

@@ -167,11 +167,6 @@ inline std::string check_shape(const llmi_kv8_shape* s) {
   return {};
 }
 
-inline bool same_shape(const llmi_kv8_shape& a, const llmi_kv8_shape& b) {
-  return a.heads == b.heads && a.kv_heads == b.kv_heads && a.head_dim == b.head_dim &&
-         a.page_tokens == b.page_tokens && a.pages == b.pages && a.slots == b.slots;
-}
-
 // The most that a batch of at most `seqs` sequences and `tokens` tokens makes.
 // A kind's positions x heads over its split size are at most its target, so
 // are its full pieces x heads; rows that are split have at most twice their
