@@ -468,7 +468,7 @@ int llmi_hip_model_forward(llmi_hip_model* model, const int32_t* tokens, size_t 
  * (src/server/server.cpp:44-49).
  * new_kv8_cache allocates every layer's pages: `pages` of page_tokens
  * positions (a multiple of 16), places for `slots` sequences, steps of at
- * most max_tokens tokens.  The model's head size must be a multiple of 32 up
+ * most max_tokens tokens (and 65535).  The model's head size must be a multiple of 32 up
  * to 256.  Which pages a sequence has is the caller's; free the cache before
  * the model.
  * forward_kv8: sequence i's counts[i] new tokens (tokens: those of sequence 0,

@@ -2417,6 +2417,7 @@ int llmi_hip_model_forward_kv8(llmi_hip_model* m, llmi_hip_kv8_cache* c, size_t 
     }
     if (T == 0) return fail(LLMI_ERR_ARG, "forward_kv8: no tokens");
     LLMI_REQUIRE(T <= c->max_tokens, "forward_kv8: more tokens than the cache was created for");
+    LLMI_REQUIRE(T <= 65535, "forward_kv8: at most 65535 tokens a step");  // rows of the products' and the gather's grids
     LLMI_REQUIRE(tokens != nullptr, "forward_kv8: null tokens");
     for (std::size_t t = 0; t < T; ++t)
       if (tokens[t] < 0 || static_cast<std::size_t>(tokens[t]) >= m->V)

@@ -178,3 +178,29 @@ def test_attention_keeps_22_bits(shape, largest):
     got = pool.attention([start], [count], q, P.SCALE)
     off = np.abs(got - P.attend(q, kq, vq, start)) / P.bound(q, kq, vq, start)
     assert off.max() <= 1, off.max()
+
+
+def test_model_steps_of_many_tokens():
+    """65535 tokens in one step; one more is refused before anything runs, and
+    the sequences go on from where they were."""
+    import synth
+    from test_gpu_kv8_model import CONFIGS
+
+    cfg = CONFIGS["llama_4x32"]
+    model = H.Model(cfg, synth.make_tensors(cfg, 6, "tiny"), H.Q8_0)
+    rng = np.random.default_rng(41)
+    n = 257
+    cache = model.new_kv8_cache(16 * n, 16, n, 70000)
+    tables = rng.permutation(16 * n).reshape(n, 16)
+    ids = rng.integers(0, cfg["vocab_size"], (n, 256))
+    counts = [256] * 255 + [255, 0]
+    first = model.forward_kv8(cache, range(n), [0] * n, counts, tables, np.concatenate([ids[i, :c] for i, c in enumerate(counts)]))
+    with pytest.raises(H.HipError, match="65535 tokens"):
+        model.forward_kv8(cache, range(n), [0] * n, [256] * 255 + [255, 1], tables, np.concatenate([ids[:255].reshape(-1), ids[255, :255], ids[256, :1]]))
+    then = model.forward_kv8(cache, [255], [255], [1], tables[255:256], ids[255, 255:])
+    alone = model.new_kv8_cache(16, 16, 1, 256)
+    for got, i, c in ((first, 0, 256), (first, 254, 256), (first, 255, 255)):
+        want = model.forward_kv8(alone, [0], [0], [c], [range(16)], ids[i, :c])[0]
+        assert np.abs(got[i] - want).max() <= 1e-4 * np.abs(want).max()  # the order of fp32 sums, as in test_alone_and_together_agree
+    want = model.forward_kv8(alone, [0], [255], [1], [range(16)], ids[255, 255:])[0]
+    assert np.abs(then[0] - want).max() <= 1e-4 * np.abs(want).max()
