@@ -130,9 +130,9 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(AttnArgs A, int j
 // fixed-point bits are more than fp32's 24.
 // Measured: 64 users of 32/8 heads of 128 over 263k positions 95 us, 5.7 TB/s
 // of codes and scales (a large copy moves 4.7, reads and writes together);
-// over 4000 positions each 92 us.  One user over 300 positions (9/3 heads of
-// 64) 4.4 us, what a launch and its four dependent loads take.  16 drafts of 3
-// to 6 tokens (12 to 24 rows a head): 26 us with the join for 60 MB, bound by
+// over 4000 positions each 93 us.  One user over 300 positions (9/3 heads of
+// 64) 4.5 us, what a launch and its four dependent loads take.  16 drafts of 3
+// to 6 tokens (12 to 24 rows a head): 26.7 us with the join for 60 MB, bound by
 // the four row tiles' scores and by one workgroup a compute unit (their
 // registers).
 constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kFewThreads) attention_few(AttnArgs A) {
 // of the result; two are off by 2^-22 or less, below fp32's sums.  That is twice the
 // formula's products: 2048 tokens over 6144 positions of 32/8 heads of 128
 // are 481 GFLOP, 414 us at the 1162 TFLOP/s of a large fp16 library product;
-// this kernel takes 419 (446 on a warmer card).  The matrix units are busy 52 %
+// this kernel takes 408 to 421 by card.  The matrix units are busy 52 %
 // of the clocks; what is left are the staging's conversions (38 us without
 // them), the wait for a tile's codes (20) and the maximum's dependency.
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
