@@ -407,6 +407,81 @@ int llmi_hip_kv8_attention_dev(const llmi_hip_kv8_plan* plan, const llmi_kv8_lay
 int llmi_hip_kv8_read_dev(const llmi_hip_kv8_plan* plan, const llmi_kv8_layer* layer, float* k, size_t k_stride,
                           float* v, size_t v_stride, void* stream);
 
+/* ------------------------------------------------ layers of experts (device) */
+/* A mixture-of-experts layer over quantized weights: a router that chooses
+ * top_k of the experts for every token, products whose matrix is the chosen
+ * expert's, and the whole gated MLP with its weighted sum.  No counterpart in
+ * the reference, whose decoder is dense (src/model/transformer.cpp:286-292).
+ * The choices stay on the device: nothing here waits for it or copies to the
+ * host, and every _dev call can be captured into a graph and replayed with
+ * other choices.
+ *
+ * Router.  Of each token's logits [tokens][experts] (stride floats apart) the
+ * top_k largest are chosen, in falling order, equal ones by the lower index;
+ *   p[t][e] = exp(logit - max) / sum over all experts of exp(logit - max)
+ *   weights[t][j] = scale * p of the j-th choice, or with renormalise
+ *                   scale * p / (the sum of p over the token's choices)
+ * in fp32.  A logit of -inf or NaN (an expert that is switched off) counts as
+ * p = 0 and is never chosen: where fewer than top_k are left the remaining
+ * ids are -1 and their weights 0.  Logits of +inf share the weight equally.
+ * ids and weights [tokens][top_k].  LLMI_ERR_ARG: more than 1024 experts, a
+ * top_k above 64 or the number of experts, a stride below it, more than 2^24
+ * tokens, a scale that is not finite. */
+int llmi_hip_moe_route_dev(const float* logits, size_t stride, size_t tokens, size_t experts, size_t top_k,
+                           int renormalise, float scale, int32_t* ids, float* weights, void* stream);
+
+/* The matrices [out][in] of `count` experts (at most 4096; in and out at most
+ * 2^18), of one type (Q8_0 or Q4_0), laid out for the products below.  The
+ * same codes and scales as llmi_hip_weight holds, copied: the sources may be
+ * freed afterwards.  From weights of one shape and type (loaded in any of the
+ * ways above), or from planar device memory, one expert after the other as
+ * llmi_hip_quantize_dev writes them ([count][out] rows of row_bytes codes,
+ * [count][out][ceil(in / 32)] scales), which has to be complete before the
+ * call; both return when the copy is done. */
+typedef struct llmi_hip_experts llmi_hip_experts;
+int llmi_hip_experts_create(const llmi_hip_weight* const* weights, size_t count, llmi_hip_experts** experts);
+int llmi_hip_experts_upload_dev(const uint8_t* data_dev, const float* scales_dev, size_t count, size_t out, size_t in,
+                                int type, llmi_hip_experts** experts);
+int llmi_hip_experts_free(llmi_hip_experts* experts);
+
+/* Products grouped by expert: for every slot s < slots with expert ids[s],
+ *   y[s] = W x[s / per_row]     W = expert ids[s]'s matrix
+ * x [ceil(slots / per_row)][in] and y [slots][out], rows x_stride and y_stride
+ * floats apart.  With a router's ids [tokens][top_k]: slots = tokens * top_k,
+ * and per_row = top_k for x of one row a token, 1 for one a slot.  Slots whose
+ * id is not 0 .. count - 1 (padding tokens, -1) leave their row of y as it was.
+ * Sums in fp32, x carried to 22 bits of each element (or 39 of its row's
+ * largest); not llmi_hip_matmul_dev's order of additions, so not its bits.  A
+ * row's result depends on that row, its expert and the call's sizes alone,
+ * never on the order in which workgroups run.  inf or NaN in a row of x gives inf or NaN in
+ * that row's results alone.
+ * work: device memory of at least the bytes that _bytes gives, 16-byte
+ * aligned; nothing has to be cleared, and nothing is kept in it from call to
+ * call.  Calls that may run at the same time (two streams, two graphs) need a
+ * workspace each; graphs that run one after the other may share one.
+ * LLMI_ERR_ARG: more than 2^24 slots, strides too short, a workspace too
+ * small, NULL pointers. */
+int llmi_hip_moe_matmul_bytes(const llmi_hip_experts* experts, size_t slots, size_t per_row, size_t* bytes);
+int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids, size_t slots, size_t per_row,
+                            const float* x, size_t x_stride, float* y, size_t y_stride, void* work, size_t work_bytes,
+                            void* stream);
+
+/* The gated MLP of the chosen experts (the decoder's, transformer.cpp:286-292,
+ * with each token's own matrices):
+ *   y[t] = residual[t] + sum over j < top_k of weights[t][j] *
+ *          down_e( silu(gate_e x[t]) * (up_e x[t]) ),   e = ids[t][j]
+ * the sum in the order of j, fp32.  gate and up of one shape and type, down of
+ * either type.  x [tokens][in], residual (NULL: 0) and y [tokens][down's out],
+ * rows their strides apart; y may be residual (with its stride) or x, where
+ * they have the same rows.  A choice whose id is not an expert's adds nothing,
+ * whatever its weight.  Everything else as for llmi_hip_moe_matmul_dev. */
+int llmi_hip_moe_mlp_bytes(const llmi_hip_experts* gate, const llmi_hip_experts* down, size_t tokens, size_t top_k,
+                           size_t* bytes);
+int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* up, const llmi_hip_experts* down,
+                         const int32_t* ids, const float* weights, size_t tokens, size_t top_k, const float* x,
+                         size_t x_stride, const float* residual, size_t residual_stride, float* y, size_t y_stride,
+                         void* work, size_t work_bytes, void* stream);
+
 /* ------------------------------------------------------------- the model */
 
 typedef struct llmi_hip_model llmi_hip_model; /* device-resident quantized decoder */

@@ -1,0 +1,479 @@
+// A layer of experts: the router, the experts' device layout, the grouping of
+// slots by expert, the sum of a token's experts, and the entry points.  The
+// products are in moe_products.hip.
+#include <memory>
+#include <new>
+
+#include "moe.hpp"
+
+namespace llmi_hip::moe {
+namespace {
+
+// Dword-aligned vectors: rows may start at any float.
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+
+// ------------------------------------------------------------------ router
+
+// A logit as an unsigned integer of the same order, 0 for what is never
+// chosen (-inf, NaN); +0 and -0 are equal.
+__device__ __forceinline__ std::uint32_t rank_bits(float l) {
+  if (!(l > -__builtin_inff())) return 0;
+  const std::uint32_t b = __float_as_uint(l + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+template <typename T, typename Fn>
+__device__ __forceinline__ T across(T v, Fn&& fn) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fn(v, static_cast<T>(__shfl_xor(v, o, 64)));
+  return v;
+}
+
+// One wavefront a token; lane l holds logits l, l + 64, ...  Every round takes
+// the largest (rank, lowest index) of all lanes, as one 64-bit maximum.
+template <int N>
+__global__ void __launch_bounds__(kThreads) route_kernel(const float* __restrict__ logits, std::size_t stride,
+                                                         std::size_t tokens, int experts, int top_k, int renormalise,
+                                                         float scale, std::int32_t* __restrict__ ids,
+                                                         float* __restrict__ weights) {
+  const int lane = threadIdx.x & 63;
+  for (std::size_t t = blockIdx.x * static_cast<std::size_t>(kWaves) + (threadIdx.x >> 6); t < tokens;
+       t += static_cast<std::size_t>(gridDim.x) * kWaves) {
+    float v[N];
+    std::uint64_t key[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = lane + 64 * i;
+      v[i] = e < experts ? logits[t * stride + e] : -__builtin_inff();
+      const std::uint32_t r = rank_bits(v[i]);
+      key[i] = r == 0 ? 0 : static_cast<std::uint64_t>(r) << 32 | (0xFFFFFFFFu - static_cast<std::uint32_t>(e));
+      if (r == 0) v[i] = -__builtin_inff();
+    }
+    float top = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);
+    top = across(top, [](float a, float b) { return fmaxf(a, b); });
+    // exp(l - max); equal ones (both +inf among them) give 1.
+    const auto weight = [&](float l) { return l == top ? 1.0f : expf(l - top); };
+    float total = 0.0f;
+    if (!renormalise) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (key[i] != 0) total += weight(v[i]);
+      total = across(total, [](float a, float b) { return a + b; });
+    }
+    // Choice j is kept by lane j (top_k <= 64).
+    float mine = 0.0f;
+    int id = -1;
+    for (int j = 0; j < top_k; ++j) {
+      std::uint64_t best = key[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) best = key[i] > best ? key[i] : best;
+      best = across(best, [](std::uint64_t a, std::uint64_t b) { return a > b ? a : b; });
+      if (best == 0) break;
+      const std::uint32_t e = 0xFFFFFFFFu - static_cast<std::uint32_t>(best);
+      const std::uint32_t r = static_cast<std::uint32_t>(best >> 32);
+      const float w = weight(__uint_as_float(r & 0x80000000u ? r & 0x7FFFFFFFu : ~r));
+      if (renormalise) total += w;
+      if (lane == j) {
+        mine = w;
+        id = static_cast<int>(e);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (key[i] == best) key[i] = 0;
+    }
+    if (lane < top_k) {
+      ids[t * top_k + lane] = id;
+      weights[t * top_k + lane] = id >= 0 ? scale * (mine / total) : 0.0f;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ layout
+
+// The reference's planar codes of one or more experts -> the tiles' order, a
+// thread for each lane of each chunk.
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads) lay_out(const std::uint8_t* __restrict__ data,
+                                                    const float* __restrict__ scales, std::size_t count, int out, int in,
+                                                    std::uint8_t* __restrict__ to, float* __restrict__ to_scales) {
+  const int blocks = (in + kBlock - 1) / kBlock, chunks = (blocks + kChunkBlocks - 1) / kChunkBlocks;
+  const int tiles = (out + kTile - 1) / kTile;
+  const std::size_t row_bytes = TYPE == LLMI_TYPE_Q4_0 ? (in + 1) / 2 : in;
+  const std::size_t units = count * tiles * chunks * 64;
+  for (std::size_t u = blockIdx.x * static_cast<std::size_t>(kThreads) + threadIdx.x; u < units;
+       u += static_cast<std::size_t>(gridDim.x) * kThreads) {
+    const int lane = static_cast<int>(u % 64);
+    const std::size_t c = u / 64;  // (expert * tiles + tile) * chunks + chunk
+    const int chunk = static_cast<int>(c % chunks), tile = static_cast<int>(c / chunks % tiles);
+    const std::size_t expert = c / chunks / tiles;
+    const int o = tile * kTile + lane % kTile;
+    const std::uint8_t* row = data + (expert * out + static_cast<std::size_t>(o)) * row_bytes;
+    std::uint32_t words[TYPE == LLMI_TYPE_Q4_0 ? 4 : 8];
+#pragma unroll
+    for (int b = 0; b < kChunkBlocks; ++b) {
+      const int k0 = (chunk * kChunkBlocks + b) * kBlock + 8 * (lane / kTile);
+      std::uint32_t code[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int k = k0 + i;
+        const bool live = o < out && k < in;
+        if constexpr (TYPE == LLMI_TYPE_Q4_0)
+          code[i] = live ? (row[k / 2] >> (k % 2 * 4)) & 15u : 8u;
+        else
+          code[i] = live ? (row[k] ^ 0x80u) : 0x80u;
+      }
+      if constexpr (TYPE == LLMI_TYPE_Q4_0) {
+        words[b] = code[0] | code[2] << 4 | code[4] << 8 | code[6] << 12 | code[1] << 16 | code[3] << 20 |
+                   code[5] << 24 | code[7] << 28;
+      } else {
+        words[2 * b] = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
+        words[2 * b + 1] = code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24;
+      }
+    }
+    constexpr int kHalves = TYPE == LLMI_TYPE_Q4_0 ? 1 : 2;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+      *reinterpret_cast<uint4*>(to + (c * kHalves + h) * 1024 + lane * 16) =
+          uint4{words[4 * h], words[4 * h + 1], words[4 * h + 2], words[4 * h + 3]};
+    // Lane l also moves scale l of the chunk: output l / 4, block l % 4.
+    const int so = tile * kTile + lane / 4, sb = chunk * kChunkBlocks + lane % 4;
+    to_scales[u] = so < out && sb < blocks ? scales[(expert * out + static_cast<std::size_t>(so)) * blocks + sb] : 0.0f;
+  }
+}
+
+unsigned grid_for(std::size_t units, std::size_t each) {
+  return static_cast<unsigned>(std::min<std::size_t>(std::max<std::size_t>(ceil_div(units, each), 1), kMostGroups));
+}
+
+int launch_lay_out(const std::uint8_t* data, const float* scales, const Shape& s, std::uint8_t* to, float* to_scales,
+                   hipStream_t st) {
+  const unsigned grid = grid_for(s.count * s.tiles() * s.chunks() * 64, kThreads);
+  const int out = static_cast<int>(s.out), in = static_cast<int>(s.in);
+  if (s.type == LLMI_TYPE_Q4_0)
+    lay_out<LLMI_TYPE_Q4_0><<<grid, kThreads, 0, st>>>(data, scales, s.count, out, in, to, to_scales);
+  else
+    lay_out<LLMI_TYPE_Q8_0><<<grid, kThreads, 0, st>>>(data, scales, s.count, out, in, to, to_scales);
+  LLMI_TRY_HIP(hipGetLastError());
+  return LLMI_OK;
+}
+
+int new_experts(const Shape& s, std::unique_ptr<llmi_hip_experts>* to) {
+  to->reset(new (std::nothrow) llmi_hip_experts);
+  if (*to == nullptr) return fail(LLMI_ERR_HIP, "experts: out of host memory");
+  (*to)->shape = s;
+  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&(*to)->codes), s.code_bytes()));
+  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&(*to)->scales), s.scale_floats() * sizeof(float)));
+  return LLMI_OK;
+}
+
+// ---------------------------------------------------------------- grouping
+
+// One workgroup counts the slots of every expert, lays the experts' ranges
+// one after the other and gives each slot a place in its range.  Which place
+// depends on the order of the counters' increments; no result does, since a
+// row's sums are the same at every place of a tile.
+constexpr int kGroupThreads = 1024;
+__global__ void __launch_bounds__(kGroupThreads) group_kernel(const std::int32_t* __restrict__ ids, int slots,
+                                                              int experts, Groups g) {
+  __shared__ std::int32_t count[kMaxExperts];
+  __shared__ std::int32_t waves[2][kGroupThreads / 64];
+  const int t = threadIdx.x, lane = t & 63;
+  for (int e = t; e < experts; e += kGroupThreads) count[e] = 0;
+  __syncthreads();
+  for (int i = t; i < slots; i += kGroupThreads) {
+    const std::int32_t e = ids[i];
+    if (e >= 0 && e < experts) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  // Running sums of slots and of row tiles over the experts, 1024 at a time.
+  std::int32_t base = 0, tile_base = 0;
+  for (int e0 = 0; e0 < experts; e0 += kGroupThreads) {
+    const int e = e0 + t;
+    const std::int32_t n = e < experts ? count[e] : 0;
+    const std::int32_t nt = (n + static_cast<int>(kRows) - 1) / static_cast<int>(kRows);
+    std::int32_t a = n, b = nt;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const std::int32_t x = __shfl_up(a, o, 64), y = __shfl_up(b, o, 64);
+      if (lane >= o) {
+        a += x;
+        b += y;
+      }
+    }
+    if (lane == 63) {
+      waves[0][t >> 6] = a;
+      waves[1][t >> 6] = b;
+    }
+    __syncthreads();
+    std::int32_t at = base + a - n, tile = tile_base + b - nt;
+    for (int w = 0; w < kGroupThreads / 64; ++w) {
+      if (w < t >> 6) {
+        at += waves[0][w];
+        tile += waves[1][w];
+      }
+      base += waves[0][w];
+      tile_base += waves[1][w];
+    }
+    if (e < experts) {
+      count[e] = at;
+      for (std::int32_t i = 0; i < nt; ++i)
+        g.tiles[tile + i] = RowTile{e, at + i * static_cast<int>(kRows), min(n - i * static_cast<int>(kRows), static_cast<int>(kRows)), 0};
+    }
+    __syncthreads();
+  }
+  for (int i = t; i < slots; i += kGroupThreads) {
+    const std::int32_t e = ids[i];
+    if (e >= 0 && e < experts) g.order[atomicAdd(&count[e], 1)] = i;
+  }
+  if (t == 0) {
+    g.counts[0] = base;
+    g.counts[1] = tile_base;
+  }
+}
+
+// ------------------------------------------------------- a token's sum
+
+// y[t] = residual[t] + sum over j of weights[t][j] * sums[t * top_k + j], in
+// the order of j; 4 results a thread.
+__global__ void __launch_bounds__(kThreads) sum_kernel(const float* __restrict__ sums,
+                                                       const std::int32_t* __restrict__ ids,
+                                                       const float* __restrict__ weights, std::size_t tokens, int top_k,
+                                                       int experts, int width, const float* residual,
+                                                       std::size_t r_stride, float* y, std::size_t y_stride) {
+  const std::size_t quads = (static_cast<std::size_t>(width) + 3) / 4;
+  const std::size_t units = tokens * quads;
+  for (std::size_t u = blockIdx.x * static_cast<std::size_t>(kThreads) + threadIdx.x; u < units;
+       u += static_cast<std::size_t>(gridDim.x) * kThreads) {
+    const std::size_t t = u / quads;
+    const int o = static_cast<int>(u % quads) * 4;
+    const bool whole = o + 4 <= width;
+    const auto load = [&](const float* p) {
+      if (whole) return *reinterpret_cast<const f4*>(p);
+      f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int i = 0; i < width - o; ++i) v[i] = p[i];
+      return v;
+    };
+    f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < top_k; ++j) {
+      const std::int32_t e = ids[t * top_k + j];
+      if (e < 0 || e >= experts) continue;
+      const float w = weights[t * top_k + j];
+      const f4 v = load(sums + (t * top_k + j) * width + o);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(w, v[i], acc[i]);
+    }
+    if (residual != nullptr) {
+      const f4 r = load(residual + t * r_stride + o);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = r[i] + acc[i];
+    }
+    float* to = y + t * y_stride + o;
+    if (whole)
+      *reinterpret_cast<f4*>(to) = acc;
+    else
+      for (int i = 0; i < width - o; ++i) to[i] = acc[i];
+  }
+}
+
+std::string check_workspace(const void* work, std::size_t bytes, std::size_t need) {
+  if (work == nullptr) return "null workspace";
+  if (reinterpret_cast<std::uintptr_t>(work) % 16 != 0) return "the workspace must be 16-byte aligned";
+  if (bytes < need) return "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed";
+  return {};
+}
+Groups groups_at(std::uint8_t* work, const Grouping& g) {
+  return {reinterpret_cast<std::int32_t*>(work + g.counts), reinterpret_cast<std::int32_t*>(work + g.order),
+          reinterpret_cast<RowTile*>(work + g.tiles)};
+}
+SplitRows parts_at(std::uint8_t* work, const Parts& p) {
+  return {reinterpret_cast<_Float16*>(work + p.values), reinterpret_cast<float*>(work + p.factors)};
+}
+
+}  // namespace
+
+int launch_group(const std::int32_t* ids, std::size_t slots, std::size_t experts, const Groups& g, hipStream_t s) {
+  group_kernel<<<1, kGroupThreads, 0, s>>>(ids, static_cast<int>(slots), static_cast<int>(experts), g);
+  LLMI_TRY_HIP(hipGetLastError());
+  return LLMI_OK;
+}
+
+}  // namespace llmi_hip::moe
+
+using namespace llmi_hip;
+using namespace llmi_hip::moe;
+
+extern "C" {
+
+int llmi_hip_moe_route_dev(const float* logits, size_t stride, size_t tokens, size_t experts, size_t top_k,
+                           int renormalise, float scale, int32_t* ids, float* weights, void* stream) {
+  LLMI_REQUIRE_INIT();
+  const std::string why = check_route(tokens, experts, top_k, stride);
+  LLMI_REQUIRE(why.empty(), "moe_route: " + why);
+  LLMI_REQUIRE(scale - scale == 0.0f, "moe_route: scale must be finite");
+  if (tokens == 0) return LLMI_OK;
+  LLMI_REQUIRE(logits != nullptr && ids != nullptr && weights != nullptr, "moe_route: null pointer");
+  hipStream_t s = pick(stream);
+  const unsigned grid = grid_for(tokens, kWaves);
+  const int e = static_cast<int>(experts), k = static_cast<int>(top_k);
+  const auto run = [&](auto n) {
+    route_kernel<n><<<grid, kThreads, 0, s>>>(logits, stride, tokens, e, k, renormalise, scale, ids, weights);
+  };
+  if (experts <= 64) run(std::integral_constant<int, 1>{});
+  else if (experts <= 128) run(std::integral_constant<int, 2>{});
+  else if (experts <= 256) run(std::integral_constant<int, 4>{});
+  else run(std::integral_constant<int, 16>{});
+  LLMI_TRY_HIP(hipGetLastError());
+  return LLMI_OK;
+}
+
+int llmi_hip_experts_upload_dev(const uint8_t* data, const float* scales, size_t count, size_t out, size_t in, int type,
+                                llmi_hip_experts** experts) {
+  LLMI_REQUIRE_INIT();
+  LLMI_REQUIRE(experts != nullptr, "experts_upload: null out-pointer");
+  *experts = nullptr;
+  Shape s;
+  s.type = type;
+  s.count = count;
+  s.out = out;
+  s.in = in;
+  const std::string why = check_shape(s);
+  LLMI_REQUIRE(why.empty(), "experts_upload: " + why);
+  LLMI_REQUIRE(data != nullptr && scales != nullptr, "experts_upload: null pointer");
+  std::unique_ptr<llmi_hip_experts> e;
+  if (int rc = new_experts(s, &e)) return rc;
+  if (int rc = launch_lay_out(data, scales, s, e->codes, e->scales, library_stream())) return rc;
+  LLMI_TRY_HIP(hipStreamSynchronize(library_stream()));
+  *experts = e.release();
+  return LLMI_OK;
+}
+
+int llmi_hip_experts_create(const llmi_hip_weight* const* weights, size_t count, llmi_hip_experts** experts) {
+  LLMI_REQUIRE_INIT();
+  LLMI_REQUIRE(experts != nullptr, "experts_create: null out-pointer");
+  *experts = nullptr;
+  LLMI_REQUIRE(weights != nullptr && count > 0 && weights[0] != nullptr, "experts_create: null weight");
+  Shape s;
+  s.type = weights[0]->m.type;
+  s.count = count;
+  s.out = weights[0]->m.out;
+  s.in = weights[0]->m.in;
+  const std::string why = check_shape(s);
+  LLMI_REQUIRE(why.empty(), "experts_create: " + why);
+  for (size_t i = 1; i < count; ++i) {
+    LLMI_REQUIRE(weights[i] != nullptr, "experts_create: null weight");
+    const DeviceMatrix& m = weights[i]->m;
+    LLMI_REQUIRE(m.type == s.type && m.out == s.out && m.in == s.in, "experts_create: weights of different types or shapes");
+  }
+  std::unique_ptr<llmi_hip_experts> e;
+  if (int rc = new_experts(s, &e)) return rc;
+  // One expert after the other through its planar form.
+  const std::size_t nd = s.out * row_bytes(s.in, s.type), at_scales = (nd + 255) / 256 * 256;
+  std::uint8_t* planar = nullptr;
+  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&planar), at_scales + s.out * s.blocks() * sizeof(float)));
+  float* planar_scales = reinterpret_cast<float*>(planar + at_scales);
+  Shape one = s;
+  one.count = 1;
+  int rc = LLMI_OK;
+  for (size_t i = 0; i < count && rc == LLMI_OK; ++i) {
+    rc = launch_relayout_to_planar(weights[i]->m, planar, planar_scales, library_stream());
+    if (rc == LLMI_OK)
+      rc = launch_lay_out(planar, planar_scales, one, e->codes + i * one.code_bytes(), e->scales + i * one.scale_floats(),
+                          library_stream());
+  }
+  const hipError_t end = hipStreamSynchronize(library_stream());
+  (void)hipFree(planar);
+  if (rc != LLMI_OK) return rc;
+  LLMI_TRY_HIP(end);
+  *experts = e.release();
+  return LLMI_OK;
+}
+
+int llmi_hip_experts_free(llmi_hip_experts* experts) {
+  if (experts == nullptr) return LLMI_OK;
+  (void)hipDeviceSynchronize();  // launches that use them may be queued on any stream
+  delete experts;
+  return LLMI_OK;
+}
+
+int llmi_hip_moe_matmul_bytes(const llmi_hip_experts* experts, size_t slots, size_t per_row, size_t* bytes) {
+  LLMI_REQUIRE(experts != nullptr && bytes != nullptr, "moe_matmul_bytes: null pointer");
+  const std::string why = check_matmul(experts->shape, slots, per_row);
+  LLMI_REQUIRE(why.empty(), "moe_matmul_bytes: " + why);
+  *bytes = MatmulLayout(experts->shape, slots, per_row).all.bytes;
+  return LLMI_OK;
+}
+
+int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids, size_t slots, size_t per_row,
+                            const float* x, size_t x_stride, float* y, size_t y_stride, void* work, size_t work_bytes,
+                            void* stream) {
+  LLMI_REQUIRE_INIT();
+  LLMI_REQUIRE(experts != nullptr, "moe_matmul: null experts");
+  const Shape& sh = experts->shape;
+  std::string why = check_matmul(sh, slots, per_row);
+  LLMI_REQUIRE(why.empty(), "moe_matmul: " + why);
+  LLMI_REQUIRE(x_stride >= sh.in && y_stride >= sh.out, "moe_matmul: x_stride or y_stride shorter than a row");
+  if (slots == 0) return LLMI_OK;
+  LLMI_REQUIRE(ids != nullptr && x != nullptr && y != nullptr, "moe_matmul: null pointer");
+  const MatmulLayout l(sh, slots, per_row);
+  why = check_workspace(work, work_bytes, l.all.bytes);
+  LLMI_REQUIRE(why.empty(), "moe_matmul: " + why);
+  hipStream_t s = pick(stream);
+  auto* w = static_cast<std::uint8_t*>(work);
+  const Groups g = groups_at(w, l.group);
+  const SplitRows xs = parts_at(w, l.x);
+  if (int rc = launch_group(ids, slots, sh.count, g, s)) return rc;
+  if (int rc = launch_split(x, ceil_div(slots, per_row), sh.in, sh.chunks(), x_stride, nullptr, xs, s)) return rc;
+  return launch_product(Product{sh, experts->view(), {}, xs, g, slots, per_row, false, false, y, y_stride}, s);
+}
+
+int llmi_hip_moe_mlp_bytes(const llmi_hip_experts* gate, const llmi_hip_experts* down, size_t tokens, size_t top_k,
+                           size_t* bytes) {
+  LLMI_REQUIRE(gate != nullptr && down != nullptr && bytes != nullptr, "moe_mlp_bytes: null pointer");
+  const std::string why = check_mlp(gate->shape, down->shape, tokens, top_k);
+  LLMI_REQUIRE(why.empty(), "moe_mlp_bytes: " + why);
+  *bytes = MlpLayout(gate->shape, down->shape, tokens, top_k).all.bytes;
+  return LLMI_OK;
+}
+
+int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* up, const llmi_hip_experts* down,
+                         const int32_t* ids, const float* weights, size_t tokens, size_t top_k, const float* x,
+                         size_t x_stride, const float* residual, size_t residual_stride, float* y, size_t y_stride,
+                         void* work, size_t work_bytes, void* stream) {
+  LLMI_REQUIRE_INIT();
+  LLMI_REQUIRE(gate != nullptr && up != nullptr && down != nullptr, "moe_mlp: null experts");
+  const Shape &gs = gate->shape, &us = up->shape, &ds = down->shape;
+  LLMI_REQUIRE(gs.type == us.type && gs.count == us.count && gs.out == us.out && gs.in == us.in,
+               "moe_mlp: gate and up of different types or shapes");
+  std::string why = check_mlp(gs, ds, tokens, top_k);
+  LLMI_REQUIRE(why.empty(), "moe_mlp: " + why);
+  LLMI_REQUIRE(x_stride >= gs.in && y_stride >= ds.out, "moe_mlp: x_stride or y_stride shorter than a row");
+  LLMI_REQUIRE(residual == nullptr || residual_stride >= ds.out, "moe_mlp: residual_stride shorter than a row");
+  LLMI_REQUIRE(residual != y || residual == nullptr || residual_stride == y_stride, "moe_mlp: residual in place needs equal strides");
+  if (tokens == 0) return LLMI_OK;
+  LLMI_REQUIRE(ids != nullptr && weights != nullptr && x != nullptr && y != nullptr, "moe_mlp: null pointer");
+  const MlpLayout l(gs, ds, tokens, top_k);
+  why = check_workspace(work, work_bytes, l.all.bytes);
+  LLMI_REQUIRE(why.empty(), "moe_mlp: " + why);
+  hipStream_t s = pick(stream);
+  auto* w = static_cast<std::uint8_t*>(work);
+  const std::size_t slots = tokens * top_k;
+  const Groups g = groups_at(w, l.group);
+  const SplitRows xs = parts_at(w, l.x), hs = parts_at(w, l.h_parts);
+  auto* h = reinterpret_cast<float*>(w + l.h);
+  auto* sums = reinterpret_cast<float*>(w + l.sums);
+  if (int rc = launch_group(ids, slots, gs.count, g, s)) return rc;
+  if (int rc = launch_split(x, tokens, gs.in, gs.chunks(), x_stride, nullptr, xs, s)) return rc;
+  if (int rc = launch_product(Product{gs, gate->view(), up->view(), xs, g, slots, top_k, false, true, h, gs.out}, s)) return rc;
+  if (int rc = launch_split(h, slots, ds.in, ds.chunks(), ds.in, g.counts, hs, s)) return rc;
+  if (int rc = launch_product(Product{ds, down->view(), {}, hs, g, slots, top_k, true, false, sums, ds.out}, s)) return rc;
+  sum_kernel<<<grid_for(tokens * ceil_div(ds.out, 4), kThreads), kThreads, 0, s>>>(
+      sums, ids, weights, tokens, static_cast<int>(top_k), static_cast<int>(ds.count), static_cast<int>(ds.out), residual,
+      residual_stride, y, y_stride);
+  LLMI_TRY_HIP(hipGetLastError());
+  return LLMI_OK;
+}
+
+}  // extern "C"

@@ -87,6 +87,14 @@ SIGNATURES = {
                                      _vp]),
     "llmi_hip_kv8_attention_dev": (_i, [_vp, _vp, _vp, _sz, _f, _vp, _sz, _vp]),
     "llmi_hip_kv8_read_dev": (_i, [_vp, _vp, _vp, _sz, _vp, _sz, _vp]),
+    "llmi_hip_moe_route_dev": (_i, [_vp, _sz, _sz, _sz, _sz, _i, _f, _vp, _vp, _vp]),
+    "llmi_hip_experts_create": (_i, [_vp, _sz, C.POINTER(_vp)]),
+    "llmi_hip_experts_upload_dev": (_i, [_vp, _vp, _sz, _sz, _sz, _i, C.POINTER(_vp)]),
+    "llmi_hip_experts_free": (_i, [_vp]),
+    "llmi_hip_moe_matmul_bytes": (_i, [_vp, _sz, _sz, C.POINTER(_sz)]),
+    "llmi_hip_moe_matmul_dev": (_i, [_vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp]),
+    "llmi_hip_moe_mlp_bytes": (_i, [_vp, _vp, _sz, _sz, C.POINTER(_sz)]),
+    "llmi_hip_moe_mlp_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp]),
     "llmi_hip_model_create": (_i, [_vp, _vp, _i, C.POINTER(_vp)]),
     "llmi_hip_model_create_dev": (_i, [_vp, _vp, _i, C.POINTER(_vp)]),
     "llmi_hip_model_free": (_i, [_vp]),
@@ -763,6 +771,79 @@ class Kv8Plan:
             self.free()
         except Exception:
             pass
+
+
+class Experts:
+    """The matrices [out][in] of a layer's experts (llmi_hip_experts_*)."""
+
+    def __init__(self, handle: int, lib, count: int, out: int, n_in: int):
+        self.h, self.lib = handle, lib
+        self.count, self.out, self.n_in = count, out, n_in
+
+    @classmethod
+    def from_weights(cls, weights) -> "Experts":
+        """Copies Weights of one shape and type (quantized or from GGUF tensors)."""
+        lib, n = init(), len(weights)
+        h = C.c_void_p()
+        check(lib.llmi_hip_experts_create((C.c_void_p * n)(*[w.h for w in weights]), n, C.byref(h)))
+        return cls(h.value, lib, n, weights[0].out, weights[0].n_in)
+
+    @classmethod
+    def upload_dev(cls, data_dev: int, scales_dev: int, count: int, out: int, n_in: int, qtype: int) -> "Experts":
+        """From planar codes and scales in device memory, one expert after the other."""
+        lib = init()
+        h = C.c_void_p()
+        check(lib.llmi_hip_experts_upload_dev(data_dev, scales_dev, count, out, n_in, qtype, C.byref(h)))
+        return cls(h.value, lib, count, out, n_in)
+
+    def free(self) -> None:
+        if self.h:
+            check(self.lib.llmi_hip_experts_free(self.h))
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def moe_route(logits: int, tokens: int, experts: int, top_k: int, ids: int, weights: int, *, stride=None,
+              renormalise: bool = True, scale: float = 1.0, stream=None) -> None:
+    """Chooses top_k experts a token (device pointers; llmi_hip_moe_route_dev)."""
+    check(init().llmi_hip_moe_route_dev(logits, experts if stride is None else stride, tokens, experts, top_k,
+                                        int(renormalise), scale, ids, weights, stream))
+
+
+def moe_matmul_bytes(experts: Experts, slots: int, per_row: int = 1) -> int:
+    """Bytes of workspace that moe_matmul needs."""
+    n = _sz()
+    check(init().llmi_hip_moe_matmul_bytes(experts.h, slots, per_row, C.byref(n)))
+    return n.value
+
+
+def moe_matmul(experts: Experts, ids: int, slots: int, x: int, y: int, work: int, work_bytes: int, *, per_row: int = 1,
+               x_stride=None, y_stride=None, stream=None) -> None:
+    """y[s] = W[ids[s]] x[s // per_row] (device pointers; llmi_hip_moe_matmul_dev)."""
+    check(init().llmi_hip_moe_matmul_dev(experts.h, ids, slots, per_row, x, experts.n_in if x_stride is None else x_stride,
+                                         y, experts.out if y_stride is None else y_stride, work, work_bytes, stream))
+
+
+def moe_mlp_bytes(gate: Experts, down: Experts, tokens: int, top_k: int) -> int:
+    """Bytes of workspace that moe_mlp needs."""
+    n = _sz()
+    check(init().llmi_hip_moe_mlp_bytes(gate.h, down.h, tokens, top_k, C.byref(n)))
+    return n.value
+
+
+def moe_mlp(gate: Experts, up: Experts, down: Experts, ids: int, weights: int, tokens: int, top_k: int, x: int, y: int,
+            work: int, work_bytes: int, *, residual=None, x_stride=None, residual_stride=None, y_stride=None,
+            stream=None) -> None:
+    """The chosen experts' gated MLPs, weighted and summed (device pointers; llmi_hip_moe_mlp_dev)."""
+    check(init().llmi_hip_moe_mlp_dev(gate.h, up.h, down.h, ids, weights, tokens, top_k, x,
+                                      gate.n_in if x_stride is None else x_stride, residual,
+                                      down.out if residual_stride is None else residual_stride, y,
+                                      down.out if y_stride is None else y_stride, work, work_bytes, stream))
 
 
 class Graph:

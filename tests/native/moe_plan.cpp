@@ -1,0 +1,79 @@
+// Limits, refusals and workspace layouts of a layer of experts
+// (csrc/moe_plan.hpp).
+#include <cstdio>
+#include <vector>
+
+#include "../../llm-inference-cpp_amd/csrc/moe_plan.hpp"
+
+using namespace llmi_hip::moe;
+
+namespace {
+int bad = 0;
+void expect(bool ok, const char* what, std::size_t a = 0, std::size_t b = 0) {
+  if (ok) return;
+  std::printf("%s (%zu, %zu)\n", what, a, b);
+  ++bad;
+}
+Shape shape(int type, std::size_t count, std::size_t out, std::size_t in) {
+  Shape s;
+  s.type = type;
+  s.count = count;
+  s.out = out;
+  s.in = in;
+  return s;
+}
+}  // namespace
+
+int main() {
+  expect(check_shape(shape(LLMI_TYPE_Q4_0, 1, 1, 1)).empty(), "smallest shape");
+  expect(check_shape(shape(LLMI_TYPE_Q8_0, kMaxExperts, kMaxInner, kMaxInner)).empty(), "largest shape");
+  expect(!check_shape(shape(LLMI_TYPE_F32, 1, 1, 1)).empty(), "fp32");
+  expect(!check_shape(shape(LLMI_TYPE_Q4_0, 0, 1, 1)).empty(), "no experts");
+  expect(!check_shape(shape(LLMI_TYPE_Q4_0, kMaxExperts + 1, 1, 1)).empty(), "too many experts");
+  expect(!check_shape(shape(LLMI_TYPE_Q4_0, 1, 0, 1)).empty(), "no results");
+  expect(!check_shape(shape(LLMI_TYPE_Q4_0, 1, 1, 0)).empty(), "no inputs");
+  expect(!check_shape(shape(LLMI_TYPE_Q4_0, 1, kMaxInner + 1, 1)).empty(), "too many results");
+  expect(!check_shape(shape(LLMI_TYPE_Q4_0, 1, 1, kMaxInner + 1)).empty(), "too many inputs");
+
+  const Shape g = shape(LLMI_TYPE_Q4_0, 8, 96, 64), d = shape(LLMI_TYPE_Q8_0, 8, 64, 96);
+  expect(check_matmul(g, 0, 1).empty() && check_matmul(g, kMaxSlots, 3).empty(), "slots taken");
+  expect(!check_matmul(g, 1, 0).empty(), "no slots a row");
+  expect(!check_matmul(g, kMaxSlots + 1, 1).empty(), "too many slots");
+  expect(check_mlp(g, d, 5, 2).empty() && check_mlp(g, d, kMaxSlots / kMaxTopK, kMaxTopK).empty(), "tokens taken");
+  expect(!check_mlp(g, g, 5, 2).empty(), "down of other inputs");
+  expect(!check_mlp(g, shape(LLMI_TYPE_Q8_0, 7, 64, 96), 5, 2).empty(), "down of other experts");
+  expect(!check_mlp(g, d, 5, 0).empty() && !check_mlp(g, d, 5, kMaxTopK + 1).empty(), "top_k");
+  expect(!check_mlp(g, d, kMaxSlots / 2 + 1, 2).empty() && !check_mlp(g, d, SIZE_MAX, 2).empty(), "too many tokens");
+  expect(check_route(0, 1, 1, 1).empty() && check_route(kMaxSlots, kMaxRouted, kMaxTopK, kMaxRouted).empty(), "routes taken");
+  expect(!check_route(1, 0, 1, 1).empty() && !check_route(1, kMaxRouted + 1, 1, kMaxRouted + 1).empty(), "routed experts");
+  expect(!check_route(1, 8, 0, 8).empty() && !check_route(1, 8, 9, 8).empty() && !check_route(1, 128, kMaxTopK + 1, 128).empty(), "routed top_k");
+  expect(!check_route(1, 8, 2, 7).empty(), "route's stride");
+  expect(!check_route(kMaxSlots + 1, 8, 2, 8).empty(), "too many routed tokens");
+
+  // Row tiles never exceed the bound: the worst spread leaves one slot over in every expert.
+  for (std::size_t experts : {1u, 2u, 7u, 64u})
+    for (std::size_t slots = 0; slots < 700; ++slots)
+      for (std::size_t spare = 0; spare <= std::min(slots, experts); ++spare) {
+        std::size_t tiles = spare > 0 ? spare - 1 : 0;  // spare - 1 experts with one slot each, the rest in one
+        const std::size_t rest = slots - tiles;
+        tiles += (rest + kRows - 1) / kRows;
+        expect(tiles <= most_tiles(slots, experts), "row tiles", slots, experts);
+      }
+  // A workspace for more slots holds fewer, and the last region ends inside it.
+  std::size_t before = 0;
+  for (std::size_t slots = 0; slots < 300; ++slots) {
+    const MatmulLayout m(g, slots, 2);
+    expect(m.all.bytes >= before, "workspace shrinks", slots);
+    expect(m.x.factors + (slots + 1) / 2 * 4 <= m.all.bytes, "factors end", slots);
+    before = m.all.bytes;
+  }
+  before = 0;
+  for (std::size_t tokens = 0; tokens < 100; ++tokens) {
+    const MlpLayout m(g, d, tokens, 3);
+    expect(m.all.bytes >= before, "workspace shrinks", tokens);
+    expect(m.sums + tokens * 3 * d.out * 4 <= m.all.bytes, "sums end", tokens);
+    before = m.all.bytes;
+  }
+  if (bad == 0) std::puts("ok");
+  return bad != 0;
+}
