@@ -421,6 +421,8 @@ int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids,
   why = check_workspace(work, work_bytes, l.all.bytes);
   LLMI_REQUIRE(why.empty(), "moe_matmul: " + why);
   hipStream_t s = pick(stream);
+  if (few_matmul(slots))
+    return launch_few(FewProduct{sh, experts->view(), {}, ids, slots, per_row, x, x_stride, y, y_stride}, s);
   auto* w = static_cast<std::uint8_t*>(work);
   const Groups g = groups_at(w, l.group);
   const SplitRows xs = parts_at(w, l.x);
@@ -464,6 +466,10 @@ int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* u
   const SplitRows xs = parts_at(w, l.x), hs = parts_at(w, l.h_parts);
   auto* h = reinterpret_cast<float*>(w + l.h);
   auto* sums = reinterpret_cast<float*>(w + l.sums);
+  if (few_mlp(tokens, top_k)) {
+    if (int rc = launch_few(FewProduct{gs, gate->view(), up->view(), ids, slots, top_k, x, x_stride, h, gs.out}, s)) return rc;
+    return launch_few_sum(FewSum{ds, down->view(), ids, weights, tokens, top_k, h, residual, residual_stride, y, y_stride}, s);
+  }
   if (int rc = launch_group(ids, slots, gs.count, g, s)) return rc;
   if (int rc = launch_split(x, tokens, gs.in, gs.chunks(), x_stride, nullptr, xs, s)) return rc;
   if (int rc = launch_product(Product{gs, gate->view(), up->view(), xs, g, slots, top_k, false, true, h, gs.out}, s)) return rc;

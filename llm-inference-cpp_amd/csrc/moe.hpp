@@ -61,6 +61,34 @@ struct Product {
 };
 int launch_product(const Product& p, hipStream_t s);
 
+// The same for at most kFewSlots slots, in one launch: y[slot] = W_expert
+// x[slot / per_row] (or the gated pair).
+struct FewProduct {
+  Shape shape;
+  Matrices m, up;
+  const std::int32_t* ids;
+  std::size_t slots, per_row;
+  const float* x;
+  std::size_t x_stride;
+  float* y;
+  std::size_t y_stride;
+};
+int launch_few(const FewProduct& p, hipStream_t s);
+// y[t] = residual[t] + sum over j of weights[t][j] W_expert h[t * top_k + j]
+// for at most kFewSlots slots of at most kFewTokens tokens, h's rows side by side.
+struct FewSum {
+  Shape shape;
+  Matrices m;
+  const std::int32_t* ids;
+  const float* weights;
+  std::size_t tokens, top_k;
+  const float *h, *residual;
+  std::size_t r_stride;
+  float* y;
+  std::size_t y_stride;
+};
+int launch_few_sum(const FewSum& p, hipStream_t s);
+
 }  // namespace llmi_hip::moe
 
 struct llmi_hip_experts {

@@ -1,0 +1,371 @@
+// The experts' products for few slots (up to 64): decoding users.
+//
+// What bounds them is the weights' way from memory and the time until the
+// first of them arrives.  So there is one launch a product (two for an MLP):
+// every workgroup finds its expert's slots in the ids by itself, its
+// wavefronts share the inputs of one tile of 16 outputs and ask for all of
+// their weights at once, and x is brought into its two fp16 parts on the way,
+// each chunk of 128 inputs of a row with its own power of two, by the
+// wavefront that uses it: no barrier until the wavefronts' sums meet.
+#include <type_traits>
+
+#include "moe_device.hpp"
+
+namespace llmi_hip::moe {
+namespace {
+
+constexpr int kMostRows = 8;  // rows of an expert that a wavefront takes at a time
+constexpr int kRowBytes = kChunk * 4 + 16;  // a row of a chunk in LDS, both parts; 16 bytes keep rows off each other's banks
+
+// Orders the lanes' LDS exchange of one wavefront for the compiler.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// A wavefront's part of LDS: 2 or kMostRows rows of a chunk in two parts, and what
+// each row's sum is multiplied by.
+struct WaveLds {
+  std::uint8_t* rows;
+  float* factors;
+};
+
+// Four inputs of each of 2 * PAIRS rows: lanes 0 .. 31 hold row 2p of pair p,
+// the others row 2p + 1; lane l inputs 4 (l % 32) .. of the chunk.
+// QUADS: rows of a multiple of 4 inputs.
+template <int PAIRS, bool QUADS>
+struct Rows {
+  f32x4 v[PAIRS];
+  // Every address is inside the row; what lies behind it is put to 0 when the
+  // rows are stored, so that nothing here waits for a load.
+  __device__ __forceinline__ void load(int p, const float* row, int chunk, int in, int lane) {
+    const int k = chunk * kChunk + lane % 32 * 4;
+    if constexpr (QUADS) {
+      v[p] = *reinterpret_cast<const f4*>(row + min(k, in - 4));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[p][i] = row[min(k + i, in - 1)];
+    }
+  }
+  // times: what a row's sum is multiplied by besides; rows without `live` count as 0.
+  __device__ __forceinline__ void store(const WaveLds& to, const float (&times)[PAIRS], const bool (&live)[PAIRS], int chunk,
+                                        int in, int lane) const {
+    const int k = lane % 32 * 4, left = in - chunk * kChunk - k;
+#pragma unroll
+    for (int p = 0; p < PAIRS; ++p) {
+      float x[4];
+      std::uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = live[p] && i < left ? v[p][i] : 0.0f;
+        top = max(top, finite_bits(x[i]));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = max(top, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
+      const Factor f(top);
+      f16x4 high, low;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        _Float16 a, b;
+        two_parts(x[i] * f.up, a, b);
+        high[i] = a;
+        low[i] = b;
+      }
+      const int row = 2 * p + lane / 32;
+      std::uint8_t* at = to.rows + row * kRowBytes + k / kBlock * (4 * kBlock) + k % kBlock * 2;
+      *reinterpret_cast<f16x4*>(at) = high;
+      *reinterpret_cast<f16x4*>(at + 2 * kBlock) = low;
+      if (lane % 32 == 0) to.factors[row] = live[p] ? f.back * times[p] : 0.0f;
+    }
+  }
+};
+
+// acc += factor * (x W^T) over one chunk: rows 4 (l / 16) .. + 3, output l % 16.
+template <int TYPE, int MATS>
+__device__ __forceinline__ void add_chunk(f32x4 (&acc)[MATS], const Chunk<TYPE> (&w)[MATS], const WaveLds& x, int last_row,
+                                          int lane) {
+  const std::uint8_t* at = x.rows + min(lane % kTile, last_row) * kRowBytes + lane / kTile * 16;
+  f32x4 sum[MATS] = {};
+#pragma unroll
+  for (int b = 0; b < kChunkBlocks; ++b) {
+    const f16x8 high = *reinterpret_cast<const f16x8*>(at + b * (4 * kBlock));
+    const f16x8 low = *reinterpret_cast<const f16x8*>(at + b * (4 * kBlock) + 2 * kBlock);
+#pragma unroll
+    for (int m = 0; m < MATS; ++m) {
+      const f16x8 code = w[m].codes(b);
+      f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+      d = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, code, d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_f32_16x16x32_f16(low, code, d, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[m][r] = __builtin_fmaf(d[r], w[m].s[b], sum[m][r]);
+    }
+  }
+  const f32x4 f = *reinterpret_cast<const f32x4*>(x.factors + lane / kTile * 4);
+#pragma unroll
+  for (int m = 0; m < MATS; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[m][r] = __builtin_fmaf(sum[m][r], f[r], acc[m][r]);
+}
+
+struct FewArgs {
+  Matrices m, up;
+  const std::int32_t* ids;
+  const float* x;
+  float* y;
+  std::size_t x_stride, y_stride;
+  int slots, per_row, experts, out, in, tiles, chunks, rows;  // rows: LDS rows of a wavefront (even)
+};
+
+// ------------------------------------------------- products of each slot
+
+constexpr int kWaves = 8, kThreads = kWaves * 64;
+
+// One workgroup for each slot and tile of 16 outputs; the first slot of an
+// expert takes all of its slots, the others leave.
+template <int TYPE, bool GATED, bool MORE, bool QUADS>
+__global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
+  extern __shared__ __attribute__((aligned(16))) std::uint8_t lds[];
+  constexpr int kMats = GATED ? 2 : 1;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int slot = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
+  const std::int32_t mine = lane < p.slots ? p.ids[lane] : -1;
+  const int expert = __builtin_amdgcn_readlane(mine, slot);
+  if (expert < 0 || expert >= p.experts) return;
+  std::uint64_t same = __ballot(mine == expert);
+  if (__builtin_ctzll(same) != slot) return;
+  const std::size_t chunk0 = (static_cast<std::size_t>(expert) * p.tiles + tile) * p.chunks;
+  const int each = (p.chunks + kWaves - 1) / kWaves;
+  const int c0 = min(wave * each, p.chunks), c1 = min(c0 + each, p.chunks);
+  const WaveLds w{lds + wave * (p.rows * kRowBytes + 64), reinterpret_cast<float*>(lds + wave * (p.rows * kRowBytes + 64) + p.rows * kRowBytes)};
+  float* const meet = reinterpret_cast<float*>(lds);
+
+  while (same != 0) {
+    // Up to kMostRows of the expert's slots at a time: lane r holds the r-th.
+    const int rows = min(__builtin_popcountll(same), MORE ? kMostRows : 2);
+    int row_slot = 0;
+    for (int r = 0; r < rows; ++r) {
+      const int at = __builtin_ctzll(same);
+      same &= same - 1;
+      if (lane == r) row_slot = at;
+    }
+    f32x4 acc[kMats] = {};
+    const auto take = [&](auto pairs, auto depth) {
+      constexpr int kPairs = decltype(pairs)::value, kDepth = decltype(depth)::value;
+      const float* at[kPairs];
+      float times[kPairs];
+      bool live[kPairs];
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        const int r = min(2 * i + lane / 32, rows - 1);
+        at[i] = p.x + static_cast<std::size_t>(__shfl(row_slot, r, 64) / p.per_row) * p.x_stride;
+        times[i] = 1.0f;
+        live[i] = true;
+      }
+      // Chunks in flight: the ring's places are filled kDepth chunks ahead.
+      Chunk<TYPE> ring[kDepth][kMats];
+      Rows<kPairs, QUADS> x[kDepth];
+      const auto ask = [&](int i, int c) {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) x[i].load(j, at[j], c, p.in, lane);
+        ring[i][0].load(p.m, chunk0 + c, lane);
+        if constexpr (GATED) ring[i][1].load(p.up, chunk0 + c, lane);
+      };
+#pragma unroll
+      for (int i = 0; i < kDepth; ++i)
+        if (c0 + i < c1) ask(i, c0 + i);
+      for (int c = c0; c < c1; c += kDepth)
+#pragma unroll
+        for (int i = 0; i < kDepth; ++i) {
+          if (c + i >= c1) break;
+          x[i].store(w, times, live, c + i, p.in, lane);
+          wave_sync();
+          add_chunk<TYPE, kMats>(acc, ring[i], w, 2 * kPairs - 1, lane);
+          wave_sync();
+          if (c + i + kDepth < c1) ask(i, c + i + kDepth);
+        }
+    };
+    if (!MORE || rows <= 2) take(std::integral_constant<int, 1>{}, std::integral_constant<int, GATED ? 2 : 4>{});
+    else if constexpr (MORE) take(std::integral_constant<int, kMostRows / 2>{}, std::integral_constant<int, 2>{});
+
+    // The wavefronts' sums meet, in their order.
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < kMats; ++m)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) meet[((wave * kMats + m) * kTile + lane / kTile * 4 + r) * kTile + lane % kTile] = acc[m][r];
+    __syncthreads();
+    const int row = threadIdx.x / kTile, o = tile * kTile + threadIdx.x % kTile;
+    // The slot of output row `row`: threads of one wavefront hold 4 rows.
+    const int to = __shfl(row_slot, min(row, rows - 1), 64);
+    if (row < rows && o < p.out) {
+      float v[kMats] = {};
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i)
+#pragma unroll
+        for (int m = 0; m < kMats; ++m) v[m] += meet[(i * kMats + m) * kTile * kTile + threadIdx.x];
+      p.y[static_cast<std::size_t>(to) * p.y_stride + o] = GATED ? silu(v[0]) * v[kMats - 1] : v[0];
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------ the second product and a token's sum
+
+constexpr int kSumWaves = 16, kSumThreads = kSumWaves * 64;
+
+struct SumArgs {
+  Matrices m;
+  const std::int32_t* ids;
+  const float *weights, *h, *residual;
+  float* y;
+  std::size_t r_stride, y_stride;
+  int tokens, top_k, experts, out, in, tiles, chunks, rows;
+};
+
+// One workgroup a tile of 16 outputs, for all tokens (up to 16): its
+// wavefronts share the chunks of all chosen experts.  Row m of a product is
+// token m, with the weight that it gives the expert (0 where it has not
+// chosen it), so the sums over inputs and over experts are one.
+template <int TYPE, int PAIRS, bool QUADS>
+__global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
+  extern __shared__ __attribute__((aligned(16))) std::uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = blockIdx.x, slots = p.tokens * p.top_k;
+  const std::int32_t mine = lane < slots ? p.ids[lane] : -1;
+  const float weight = lane < slots ? p.weights[lane] : 0.0f;
+  // Bit s: slot s is the first of its expert.
+  std::uint64_t firsts = 0;
+  for (int s = 0; s < slots; ++s) {
+    const int e = __builtin_amdgcn_readlane(mine, s);
+    if (e >= 0 && e < p.experts && __builtin_ctzll(__ballot(mine == e)) == s) firsts |= std::uint64_t{1} << s;
+  }
+  const int units = __builtin_popcountll(firsts) * p.chunks;  // (expert, chunk)
+  const int each = (units + kSumWaves - 1) / kSumWaves;
+  const int u0 = min(wave * each, units), u1 = min(u0 + each, units);
+  const WaveLds w{lds + wave * (p.rows * kRowBytes + 64), reinterpret_cast<float*>(lds + wave * (p.rows * kRowBytes + 64) + p.rows * kRowBytes)};
+  float* const meet = reinterpret_cast<float*>(lds);
+  constexpr int kDepth = PAIRS == 1 ? 4 : 2;
+  for (int t0 = 0; t0 < p.tokens; t0 += 2 * PAIRS) {
+    f32x4 acc[1] = {};
+    Chunk<TYPE> ring[kDepth][1];
+    Rows<PAIRS, QUADS> x[kDepth];
+    float times[kDepth][PAIRS];
+    bool live[kDepth][PAIRS];
+    int at[kDepth];
+    // The unit that is asked for next: its number, chunk and expert (the
+    // lowest bit that is left).
+    std::uint64_t left = firsts;
+    for (int i = u0 / p.chunks; i > 0 && left != 0; --i) left &= left - 1;
+    int next = u0, chunk = u0 % p.chunks;
+    const auto ask = [&](int i) {
+      const int s = __builtin_ctzll(left), e = __builtin_amdgcn_readlane(mine, s);
+      const std::uint64_t same = __ballot(mine == e);
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j) {
+        const int t = min(t0 + 2 * j + lane / 32, p.tokens - 1);
+        std::uint64_t bits = same >> (t * p.top_k);
+        if (p.top_k < 64) bits &= (std::uint64_t{1} << p.top_k) - 1;
+        live[i][j] = bits != 0;
+        const int slot = bits != 0 ? t * p.top_k + __builtin_ctzll(bits) : s;
+        float sum = 0.0f;
+        while (__any(bits != 0)) {  // an expert chosen twice counts with both weights
+          const float one = __shfl(weight, bits != 0 ? t * p.top_k + __builtin_ctzll(bits) : 0, 64);
+          if (bits != 0) sum += one;
+          bits &= bits - 1;
+        }
+        times[i][j] = sum;
+        x[i].load(j, p.h + static_cast<std::size_t>(slot) * p.in, chunk, p.in, lane);
+      }
+      ring[i][0].load(p.m, (static_cast<std::size_t>(e) * p.tiles + tile) * p.chunks + chunk, lane);
+      at[i] = chunk;
+      ++next;
+      if (++chunk == p.chunks) {
+        chunk = 0;
+        left &= left - 1;
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i)
+      if (next < u1) ask(i);
+    for (int u = u0; u < u1; u += kDepth)
+#pragma unroll
+      for (int i = 0; i < kDepth; ++i) {
+        if (u + i >= u1) break;
+        x[i].store(w, times[i], live[i], at[i], p.in, lane);
+        wave_sync();
+        add_chunk<TYPE, 1>(acc, ring[i], w, 2 * PAIRS - 1, lane);
+        wave_sync();
+        if (next < u1) ask(i);
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) meet[(wave * kTile + lane / kTile * 4 + r) * kTile + lane % kTile] = acc[0][r];
+    __syncthreads();
+    const int row = threadIdx.x / kTile, t = t0 + row, o = tile * kTile + threadIdx.x % kTile;
+    if (row < 2 * PAIRS && t < p.tokens && o < p.out) {
+      float v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kSumWaves; ++i) v += meet[i * kTile * kTile + threadIdx.x];
+      if (p.residual != nullptr) v = p.residual[static_cast<std::size_t>(t) * p.r_stride + o] + v;
+      p.y[static_cast<std::size_t>(t) * p.y_stride + o] = v;
+    }
+    __syncthreads();
+  }
+}
+
+// fn of each flag as a std::bool_constant.
+template <typename Fn>
+void with_flags(Fn&& fn) {
+  fn();
+}
+template <typename Fn, typename... More>
+void with_flags(Fn&& fn, bool flag, More... more) {
+  if (flag) with_flags([&](auto... rest) { fn(std::true_type{}, rest...); }, more...);
+  else with_flags([&](auto... rest) { fn(std::false_type{}, rest...); }, more...);
+}
+
+std::size_t lds_bytes(int waves, int rows, int mats) {
+  return std::max<std::size_t>(static_cast<std::size_t>(waves) * (rows * kRowBytes + 64),
+                               static_cast<std::size_t>(waves) * mats * kTile * kTile * sizeof(float));
+}
+
+}  // namespace
+
+int launch_few(const FewProduct& f, hipStream_t s) {
+  const Shape& sh = f.shape;
+  // An expert has more than two rows only where x has, or where ids repeat.
+  const bool more = ceil_div(f.slots, f.per_row) > 2;
+  const int rows = more ? kMostRows : 2;
+  const FewArgs a{f.m, f.up, f.ids, f.x, f.y, f.x_stride, f.y_stride, static_cast<int>(f.slots), static_cast<int>(f.per_row),
+                  static_cast<int>(sh.count), static_cast<int>(sh.out), static_cast<int>(sh.in), static_cast<int>(sh.tiles()),
+                  static_cast<int>(sh.chunks()), rows};
+  const unsigned grid = static_cast<unsigned>(f.slots * sh.tiles());
+  with_flags([&](auto gated, auto more, auto quads) {
+    const std::size_t lds = lds_bytes(kWaves, rows, gated ? 2 : 1);
+    if (sh.type == LLMI_TYPE_Q4_0) few_kernel<LLMI_TYPE_Q4_0, gated, more, quads><<<grid, kThreads, lds, s>>>(a);
+    else few_kernel<LLMI_TYPE_Q8_0, gated, more, quads><<<grid, kThreads, lds, s>>>(a);
+  }, f.up.codes != nullptr, more, sh.in % 4 == 0);
+  LLMI_TRY_HIP(hipGetLastError());
+  return LLMI_OK;
+}
+
+int launch_few_sum(const FewSum& f, hipStream_t s) {
+  const Shape& sh = f.shape;
+  const bool more = f.tokens > 2;
+  const int rows = more ? kMostRows : 2;
+  const SumArgs a{f.m, f.ids, f.weights, f.h, f.residual, f.y, f.r_stride, f.y_stride, static_cast<int>(f.tokens),
+                  static_cast<int>(f.top_k), static_cast<int>(sh.count), static_cast<int>(sh.out), static_cast<int>(sh.in),
+                  static_cast<int>(sh.tiles()), static_cast<int>(sh.chunks()), rows};
+  const unsigned grid = static_cast<unsigned>(sh.tiles());
+  const std::size_t lds = lds_bytes(kSumWaves, rows, 1);
+  with_flags([&](auto more, auto quads) {
+    constexpr int kPairs = more ? kMostRows / 2 : 1;
+    if (sh.type == LLMI_TYPE_Q4_0) few_sum_kernel<LLMI_TYPE_Q4_0, kPairs, quads><<<grid, kSumThreads, lds, s>>>(a);
+    else few_sum_kernel<LLMI_TYPE_Q8_0, kPairs, quads><<<grid, kSumThreads, lds, s>>>(a);
+  }, more, sh.in % 4 == 0);
+  LLMI_TRY_HIP(hipGetLastError());
+  return LLMI_OK;
+}
+
+}  // namespace llmi_hip::moe

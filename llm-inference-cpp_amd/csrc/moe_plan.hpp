@@ -48,6 +48,12 @@ inline std::size_t most_tiles(std::size_t slots, std::size_t experts) {
   return slots / kRows + std::min(slots, experts);
 }
 
+// Up to this many slots (a wavefront's lanes) and tokens (rows of a matrix
+// instruction) go without a grouping.
+constexpr std::size_t kFewSlots = 64, kFewTokens = 16;
+inline bool few_matmul(std::size_t slots) { return slots <= kFewSlots; }
+inline bool few_mlp(std::size_t tokens, std::size_t top_k) { return tokens * top_k <= kFewSlots && tokens <= kFewTokens; }
+
 // Places in a call's workspace, each a multiple of 256 bytes.
 struct Layout {
   std::size_t bytes = 0;

@@ -9,62 +9,13 @@
 // fp32 scale and added in fp32.
 #include <type_traits>
 
-#include "moe.hpp"
+#include "moe_device.hpp"
 
 namespace llmi_hip::moe {
 namespace {
 
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-typedef std::uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kRowTiles = static_cast<int>(kRows) / kTile;
-
-__device__ __forceinline__ f16x2 as_f16(std::uint32_t v) { return __builtin_bit_cast(f16x2, v); }
-
-// Eight 4-bit codes of a dword: nibbles moved into fp16 mantissas give 1024 +
-// n or 1024 + 16 n, from which n - 8 is exact in one operation.
-__device__ __forceinline__ f16x8 codes_q4(std::uint32_t w) {
-  const f16x2 one = {static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
-  const f16x2 by = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
-  const f16x2 off = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
-  const std::uint32_t v = w >> 8;
-  const f16x2 a = as_f16((w & 0x000F000Fu) | 0x64006400u) + one;
-  const f16x2 b = __builtin_elementwise_fma(as_f16((w & 0x00F000F0u) | 0x64006400u), by, off);
-  const f16x2 c = as_f16((v & 0x000F000Fu) | 0x64006400u) + one;
-  const f16x2 d = __builtin_elementwise_fma(as_f16((v & 0x00F000F0u) | 0x64006400u), by, off);
-  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-// Eight codes + 128 of two dwords, likewise.
-__device__ __forceinline__ f16x8 codes_q8(std::uint32_t lo, std::uint32_t hi) {
-  const f16x2 off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
-  const auto two = [&](std::uint32_t w, std::uint32_t sel) {
-    return as_f16(__builtin_amdgcn_perm(0x64646464u, w, sel)) + off;
-  };
-  const f16x2 a = two(lo, 0x04010400u), b = two(lo, 0x04030402u), c = two(hi, 0x04010400u), d = two(hi, 0x04030402u);
-  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
-// A lane's weights of one tile and chunk.
-template <int TYPE>
-struct Chunk {
-  u32x4 c[TYPE == LLMI_TYPE_Q4_0 ? 1 : 2];
-  f32x4 s;
-  __device__ __forceinline__ void load(const Matrices& m, std::size_t chunk, int lane) {
-    constexpr int kParts = TYPE == LLMI_TYPE_Q4_0 ? 1 : 2;
-#pragma unroll
-    for (int i = 0; i < kParts; ++i)
-      c[i] = *reinterpret_cast<const u32x4*>(m.codes + (chunk * kParts + i) * 1024 + lane * 16);
-    s = *reinterpret_cast<const f32x4*>(m.scales + chunk * 64 + (lane % kTile) * kChunkBlocks);
-  }
-  __device__ __forceinline__ f16x8 codes(int b) const {
-    if constexpr (TYPE == LLMI_TYPE_Q4_0) return codes_q4(c[0][b]);
-    else return codes_q8(c[b / 2][b % 2 * 2], c[b / 2][b % 2 * 2 + 1]);
-  }
-};
 
 // x in two parts: one wavefront a row.  The factor is taken from the largest
 // finite |x|: an inf or NaN stays one in the high part and shows in its own
@@ -94,18 +45,12 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const float* __restrict
       float v[8];
       load8(k, v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const std::uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-        if (b < 0x7F800000u) top = max(top, b);
-      }
+      for (int i = 0; i < 8; ++i) top = max(top, finite_bits(v[i]));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = max(top, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
-    // 2^e <= largest < 2^(e+1); e at least -112, so that 2^(14 - e) and its
-    // inverse are normal numbers.
-    const int e = max(static_cast<int>(top >> 23) - 127, -112);
-    const float up = __uint_as_float(static_cast<std::uint32_t>(127 + 14 - e) << 23);
-    if (lane == 0) to.factors[r] = __uint_as_float(static_cast<std::uint32_t>(127 - 14 + e) << 23);
+    const Factor f(top);
+    if (lane == 0) to.factors[r] = f.back;
     _Float16* out = to.values + static_cast<std::size_t>(r) * chunks * (kChunkBlocks * kBlock * 2);
     for (int k = lane * 8; k < chunks * kChunkBlocks * kBlock; k += 512) {
       float v[8];
@@ -113,9 +58,10 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const float* __restrict
       f16x8 high, low;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float a = v[i] * up;
-        high[i] = static_cast<_Float16>(a);
-        low[i] = fabsf(a) < __builtin_inff() ? static_cast<_Float16>(a - static_cast<float>(high[i])) : static_cast<_Float16>(0.0f);
+        _Float16 a, b;
+        two_parts(v[i] * f.up, a, b);
+        high[i] = a;
+        low[i] = b;
       }
       _Float16* at = out + (k / kBlock) * 2 * kBlock + k % kBlock;
       *reinterpret_cast<f16x8*>(at) = high;
@@ -123,8 +69,6 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const float* __restrict
     }
   }
 }
-
-__device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
 
 struct ProductArgs {
   Matrices m, up;
