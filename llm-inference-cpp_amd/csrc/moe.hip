@@ -94,27 +94,27 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const float* __restrict
 // ------------------------------------------------------------------ layout
 
 // The reference's planar codes of one or more experts -> the tiles' order, a
-// thread for each lane of each chunk.
+// thread for each lane of each step.
 template <int TYPE>
 __global__ void __launch_bounds__(kThreads) lay_out(const std::uint8_t* __restrict__ data,
                                                     const float* __restrict__ scales, std::size_t count, int out, int in,
                                                     std::uint8_t* __restrict__ to, float* __restrict__ to_scales) {
-  const int blocks = (in + kBlock - 1) / kBlock, chunks = (blocks + kChunkBlocks - 1) / kChunkBlocks;
+  const int blocks = (in + kBlock - 1) / kBlock, steps = (in + kStep - 1) / kStep;
   const int tiles = (out + kTile - 1) / kTile;
   const std::size_t row_bytes = TYPE == LLMI_TYPE_Q4_0 ? (in + 1) / 2 : in;
-  const std::size_t units = count * tiles * chunks * 64;
+  const std::size_t units = count * tiles * steps * 64;
   for (std::size_t u = blockIdx.x * static_cast<std::size_t>(kThreads) + threadIdx.x; u < units;
        u += static_cast<std::size_t>(gridDim.x) * kThreads) {
     const int lane = static_cast<int>(u % 64);
-    const std::size_t c = u / 64;  // (expert * tiles + tile) * chunks + chunk
-    const int chunk = static_cast<int>(c % chunks), tile = static_cast<int>(c / chunks % tiles);
-    const std::size_t expert = c / chunks / tiles;
+    const std::size_t c = u / 64;  // (expert * tiles + tile) * steps + step
+    const int step = static_cast<int>(c % steps), tile = static_cast<int>(c / steps % tiles);
+    const std::size_t expert = c / steps / tiles;
     const int o = tile * kTile + lane % kTile;
     const std::uint8_t* row = data + (expert * out + static_cast<std::size_t>(o)) * row_bytes;
-    std::uint32_t words[TYPE == LLMI_TYPE_Q4_0 ? 4 : 8];
+    std::uint32_t words[TYPE == LLMI_TYPE_Q4_0 ? 2 : 4];
 #pragma unroll
-    for (int b = 0; b < kChunkBlocks; ++b) {
-      const int k0 = (chunk * kChunkBlocks + b) * kBlock + 8 * (lane / kTile);
+    for (int b = 0; b < 2; ++b) {
+      const int k0 = step * kStep + b * kBlock + 8 * (lane / kTile);
       std::uint32_t code[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -133,14 +133,12 @@ __global__ void __launch_bounds__(kThreads) lay_out(const std::uint8_t* __restri
         words[2 * b + 1] = code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24;
       }
     }
-    constexpr int kHalves = TYPE == LLMI_TYPE_Q4_0 ? 1 : 2;
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h)
-      *reinterpret_cast<uint4*>(to + (c * kHalves + h) * 1024 + lane * 16) =
-          uint4{words[4 * h], words[4 * h + 1], words[4 * h + 2], words[4 * h + 3]};
-    // Lane l also moves scale l of the chunk: output l / 4, block l % 4.
-    const int so = tile * kTile + lane / 4, sb = chunk * kChunkBlocks + lane % 4;
-    to_scales[u] = so < out && sb < blocks ? scales[(expert * out + static_cast<std::size_t>(so)) * blocks + sb] : 0.0f;
+    if constexpr (TYPE == LLMI_TYPE_Q4_0) *reinterpret_cast<uint2*>(to + u * 8) = uint2{words[0], words[1]};
+    else *reinterpret_cast<uint4*>(to + u * 16) = uint4{words[0], words[1], words[2], words[3]};
+    if (lane < static_cast<int>(kStepScales)) {  // output lane / 2, block lane % 2
+      const int so = tile * kTile + lane / 2, sb = step * 2 + lane % 2;
+      to_scales[c * kStepScales + lane] = so < out && sb < blocks ? scales[(expert * out + static_cast<std::size_t>(so)) * blocks + sb] : 0.0f;
+    }
   }
 }
 
@@ -150,7 +148,7 @@ unsigned grid_for(std::size_t units, std::size_t each) {
 
 int launch_lay_out(const std::uint8_t* data, const float* scales, const Shape& s, std::uint8_t* to, float* to_scales,
                    hipStream_t st) {
-  const unsigned grid = grid_for(s.count * s.tiles() * s.chunks() * 64, kThreads);
+  const unsigned grid = grid_for(s.count * s.tiles() * s.steps() * 64, kThreads);
   const int out = static_cast<int>(s.out), in = static_cast<int>(s.in);
   if (s.type == LLMI_TYPE_Q4_0)
     lay_out<LLMI_TYPE_Q4_0><<<grid, kThreads, 0, st>>>(data, scales, s.count, out, in, to, to_scales);
@@ -179,7 +177,7 @@ constexpr int kGroupThreads = 1024;
 __global__ void __launch_bounds__(kGroupThreads) group_kernel(const std::int32_t* __restrict__ ids, int slots,
                                                               int experts, Groups g) {
   __shared__ std::int32_t count[kMaxExperts];
-  __shared__ std::int32_t waves[2][kGroupThreads / 64];
+  __shared__ std::int32_t waves[3][kGroupThreads / 64];
   const int t = threadIdx.x, lane = t & 63;
   for (int e = t; e < experts; e += kGroupThreads) count[e] = 0;
   __syncthreads();
@@ -189,38 +187,36 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const std::int32_t
   }
   __syncthreads();
   // Running sums of slots and of row tiles over the experts, 1024 at a time.
-  std::int32_t base = 0, tile_base = 0;
+  std::int32_t base[3] = {0, 0, 0};
   for (int e0 = 0; e0 < experts; e0 += kGroupThreads) {
     const int e = e0 + t;
     const std::int32_t n = e < experts ? count[e] : 0;
-    const std::int32_t nt = (n + static_cast<int>(kRows) - 1) / static_cast<int>(kRows);
-    std::int32_t a = n, b = nt;
+    const std::int32_t own[3] = {n, (n + g.rows[0] - 1) / g.rows[0], (n + g.rows[1] - 1) / g.rows[1]};
+    std::int32_t at[3];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const std::int32_t x = __shfl_up(a, o, 64), y = __shfl_up(b, o, 64);
-      if (lane >= o) {
-        a += x;
-        b += y;
+    for (int i = 0; i < 3; ++i) {
+      std::int32_t a = own[i];
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const std::int32_t x = __shfl_up(a, o, 64);
+        if (lane >= o) a += x;
       }
-    }
-    if (lane == 63) {
-      waves[0][t >> 6] = a;
-      waves[1][t >> 6] = b;
+      if (lane == 63) waves[i][t >> 6] = a;
+      at[i] = base[i] + a - own[i];
     }
     __syncthreads();
-    std::int32_t at = base + a - n, tile = tile_base + b - nt;
-    for (int w = 0; w < kGroupThreads / 64; ++w) {
-      if (w < t >> 6) {
-        at += waves[0][w];
-        tile += waves[1][w];
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      for (int w = 0; w < kGroupThreads / 64; ++w) {
+        if (w < t >> 6) at[i] += waves[i][w];
+        base[i] += waves[i][w];
       }
-      base += waves[0][w];
-      tile_base += waves[1][w];
-    }
     if (e < experts) {
-      count[e] = at;
-      for (std::int32_t i = 0; i < nt; ++i)
-        g.tiles[tile + i] = RowTile{e, at + i * static_cast<int>(kRows), min(n - i * static_cast<int>(kRows), static_cast<int>(kRows)), 0};
+      count[e] = at[0];
+#pragma unroll
+      for (int l = 0; l < 2; ++l)
+        for (std::int32_t i = 0; i < own[1 + l]; ++i)
+          g.tiles[l][at[1 + l] + i] = RowTile{e, at[0] + i * g.rows[l], min(n - i * g.rows[l], g.rows[l]), 0};
     }
     __syncthreads();
   }
@@ -228,10 +224,7 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const std::int32_t
     const std::int32_t e = ids[i];
     if (e >= 0 && e < experts) g.order[atomicAdd(&count[e], 1)] = i;
   }
-  if (t == 0) {
-    g.counts[0] = base;
-    g.counts[1] = tile_base;
-  }
+  if (t < 3) g.counts[t] = base[t];
 }
 
 // ------------------------------------------------------- a token's sum
@@ -284,9 +277,17 @@ std::string check_workspace(const void* work, std::size_t bytes, std::size_t nee
   if (bytes < need) return "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed";
   return {};
 }
-Groups groups_at(std::uint8_t* work, const Grouping& g) {
-  return {reinterpret_cast<std::int32_t*>(work + g.counts), reinterpret_cast<std::int32_t*>(work + g.order),
-          reinterpret_cast<RowTile*>(work + g.tiles)};
+Groups groups_at(std::uint8_t* work, const Grouping& g, std::size_t rows0, std::size_t rows1) {
+  return {reinterpret_cast<std::int32_t*>(work + g.counts),
+          reinterpret_cast<std::int32_t*>(work + g.order),
+          {reinterpret_cast<RowTile*>(work + g.tiles[0]), reinterpret_cast<RowTile*>(work + g.tiles[1])},
+          {static_cast<int>(rows0), static_cast<int>(rows1)}};
+}
+// Rows in the layout of the list's product.
+int split_rows(const RowSource& x, std::size_t rows, const std::int32_t* live, const Groups& g, int list, std::size_t slots,
+               std::size_t experts, const SplitRows& to, hipStream_t s) {
+  if (g.rows[list] <= static_cast<int>(kMostShortRows)) return launch_split_tiles(x, g, list, slots, experts, to, s);
+  return launch_split(x, rows, live, to, s);
 }
 SplitRows parts_at(std::uint8_t* work, const Parts& p) {
   return {reinterpret_cast<_Float16*>(work + p.values), reinterpret_cast<float*>(work + p.factors)};
@@ -424,11 +425,13 @@ int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids,
   if (few_matmul(slots))
     return launch_few(FewProduct{sh, experts->view(), {}, ids, slots, per_row, x, x_stride, y, y_stride}, s);
   auto* w = static_cast<std::uint8_t*>(work);
-  const Groups g = groups_at(w, l.group);
+  const std::size_t rows = pick_rows(sh, slots, false);
+  const Groups g = groups_at(w, l.group, rows, rows);
   const SplitRows xs = parts_at(w, l.x);
   if (int rc = launch_group(ids, slots, sh.count, g, s)) return rc;
-  if (int rc = launch_split(x, ceil_div(slots, per_row), sh.in, sh.chunks(), x_stride, nullptr, xs, s)) return rc;
-  return launch_product(Product{sh, experts->view(), {}, xs, g, slots, per_row, false, false, y, y_stride}, s);
+  const RowSource src{x, x_stride, sh.in, sh.steps(), per_row};
+  if (int rc = split_rows(src, ceil_div(slots, per_row), nullptr, g, 0, slots, sh.count, xs, s)) return rc;
+  return launch_product(Product{sh, experts->view(), {}, xs, g, 0, slots, per_row, false, y, y_stride}, s);
 }
 
 int llmi_hip_moe_mlp_bytes(const llmi_hip_experts* gate, const llmi_hip_experts* down, size_t tokens, size_t top_k,
@@ -462,7 +465,7 @@ int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* u
   hipStream_t s = pick(stream);
   auto* w = static_cast<std::uint8_t*>(work);
   const std::size_t slots = tokens * top_k;
-  const Groups g = groups_at(w, l.group);
+  const Groups g = groups_at(w, l.group, pick_rows(gs, slots, true), pick_rows(ds, slots, false));
   const SplitRows xs = parts_at(w, l.x), hs = parts_at(w, l.h_parts);
   auto* h = reinterpret_cast<float*>(w + l.h);
   auto* sums = reinterpret_cast<float*>(w + l.sums);
@@ -471,10 +474,11 @@ int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* u
     return launch_few_sum(FewSum{ds, down->view(), ids, weights, tokens, top_k, h, residual, residual_stride, y, y_stride}, s);
   }
   if (int rc = launch_group(ids, slots, gs.count, g, s)) return rc;
-  if (int rc = launch_split(x, tokens, gs.in, gs.chunks(), x_stride, nullptr, xs, s)) return rc;
-  if (int rc = launch_product(Product{gs, gate->view(), up->view(), xs, g, slots, top_k, false, true, h, gs.out}, s)) return rc;
-  if (int rc = launch_split(h, slots, ds.in, ds.chunks(), ds.in, g.counts, hs, s)) return rc;
-  if (int rc = launch_product(Product{ds, down->view(), {}, hs, g, slots, top_k, true, false, sums, ds.out}, s)) return rc;
+  const RowSource src{x, x_stride, gs.in, gs.steps(), top_k}, h_src{h, ds.in, ds.in, ds.steps(), 0};
+  if (int rc = split_rows(src, tokens, nullptr, g, 0, slots, gs.count, xs, s)) return rc;
+  if (int rc = launch_product(Product{gs, gate->view(), up->view(), xs, g, 0, slots, top_k, true, h, gs.out}, s)) return rc;
+  if (int rc = split_rows(h_src, slots, g.counts, g, 1, slots, ds.count, hs, s)) return rc;
+  if (int rc = launch_product(Product{ds, down->view(), {}, hs, g, 1, slots, 0, false, sums, ds.out}, s)) return rc;
   sum_kernel<<<grid_for(tokens * ceil_div(ds.out, 4), kThreads), kThreads, 0, s>>>(
       sums, ids, weights, tokens, static_cast<int>(top_k), static_cast<int>(ds.count), static_cast<int>(ds.out), residual,
       residual_stride, y, y_stride);

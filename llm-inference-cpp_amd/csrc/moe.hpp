@@ -6,16 +6,14 @@
 
 namespace llmi_hip::moe {
 
-// One expert's matrices of all tiles: codes in the order in which the matrix
-// instructions take them.  Lane l of a wavefront holds output l % 16 of a
-// tile and, of each block, the 8 inputs 8 (l / 16) ...:
-//   Q4_0  codes[((expert * tiles + tile) * chunks + chunk) * 1024 + lane * 16]:
-//         four dwords, one of each block of the chunk; its nibbles, from the
-//         lowest, are the codes + 8 of inputs 0 2 4 6 1 3 5 7;
-//   Q8_0  the same with 2048 bytes a chunk: 1024 for its first two blocks,
-//         1024 for the others; a lane's 16 bytes are codes + 128 of 8 inputs of
-//         the one block, then of the other.
-//   scales[((expert * tiles + tile) * chunks + chunk) * 64 + output * 4 + block].
+// The experts' codes in the order in which the matrix instructions take them.
+// Lane l of a wavefront holds output l % 16 of a tile and, of each block, the
+// 8 inputs 8 (l / 16) ...; at (expert * tiles + tile) * steps + step:
+//   Q4_0  codes[at * 512 + lane * 8]: two dwords, one of each block; its
+//         nibbles, from the lowest, are the codes + 8 of inputs 0 2 4 6 1 3 5 7;
+//   Q8_0  codes[at * 1024 + lane * 16]: codes + 128 of the 8 inputs of the one
+//         block, then of the other;
+//   scales[at * 32 + output * 2 + block].
 struct Matrices {
   const std::uint8_t* codes = nullptr;
   const float* scales = nullptr;
@@ -26,9 +24,10 @@ struct RowTile {
   std::int32_t expert, first, rows, pad;
 };
 struct Groups {
-  std::int32_t* counts;  // slots that have an expert, row tiles
+  std::int32_t* counts;  // slots that have an expert, row tiles of both lists
   std::int32_t* order;   // slots, those of expert 0 first
-  RowTile* tiles;
+  RowTile* tiles[2];     // of rows[0] and rows[1] rows each
+  int rows[2];
 };
 int launch_group(const std::int32_t* ids, std::size_t slots, std::size_t experts, const Groups& g, hipStream_t s);
 
@@ -36,26 +35,41 @@ int launch_group(const std::int32_t* ids, std::size_t slots, std::size_t experts
 // go on with further units from there.
 constexpr std::size_t kMostGroups = std::size_t{1} << 22;
 
-// Rows x [rows][in] (stride floats apart) in two fp16 parts: x = factor *
-// (high + low), with the row's largest |x| between 2^14 and 2^15 times the
-// factor, a power of two.  live: the number of rows in device memory (NULL: all).
+// Rows in two fp16 parts: x = factor * (high + low), with the row's largest
+// |x| between 2^14 and 2^15 times the factor, a power of two.
+//   rows as they are: values [row][step][block][high, low][32], factors [row];
+//   in row tiles of MT * 16 rows: values [tile][step][16 rows of MT][block]
+//     [high, low][lane][8], lane l holding inputs 8 (l / 16) .. of row l % 16,
+//     factors [tile][row].
 struct SplitRows {
-  _Float16* values;  // [row][chunks * 4 blocks][high, low][32]
+  _Float16* values;
   float* factors;
 };
-int launch_split(const float* x, std::size_t rows, std::size_t in, std::size_t chunks, std::size_t stride,
-                 const std::int32_t* live, const SplitRows& to, hipStream_t s);
+// Where rows come from: position `pos` of the order has x's row pos, or
+// order[pos] / per_row (per_row > 0).
+struct RowSource {
+  const float* x;
+  std::size_t stride, in, steps;
+  std::size_t per_row;
+};
+// All of `rows` rows as they are (at most *live where it is given).
+int launch_split(const RowSource& x, std::size_t rows, const std::int32_t* live, const SplitRows& to, hipStream_t s);
+// The rows of tile list `list`.
+int launch_split_tiles(const RowSource& x, const Groups& g, int list, std::size_t slots, std::size_t experts,
+                       const SplitRows& to, hipStream_t s);
 
-// y[slot or position] = W_expert x[row] over all row tiles; with `up`,
-// silu(gate x) * (up x).  per_row > 0: x's rows are slot / per_row and y's the
-// slots; 0: x's rows are positions of the order.
+// y[slot or position] = W_expert x over all row tiles of a list; with `up`,
+// silu(gate x) * (up x).  x: in row tiles where the list's have at most
+// kMostShortRows rows; else rows as they are, x's row of a position being the
+// position (per_row 0) or order[position] / per_row.
 struct Product {
   Shape shape;
   Matrices m, up;
   SplitRows x;
   Groups g;
+  int list;  // which of its tile lists
   std::size_t slots, per_row;
-  bool x_by_position, y_by_position;
+  bool y_by_position;
   float* y;
   std::size_t y_stride;
 };

@@ -13,8 +13,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // rows may start at any float
 typedef std::uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kChunk = kChunkBlocks * kBlock;  // inputs of a chunk
-
 // A constant in a vector register: v_and_or_b32 takes one scalar operand only.
 __device__ __forceinline__ std::uint32_t magic() {
   std::uint32_t m;
@@ -46,24 +44,45 @@ __device__ __forceinline__ f16x8 codes_q8(std::uint32_t lo, std::uint32_t hi) {
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// A lane's weights of one tile and chunk.
+typedef const __attribute__((address_space(1))) std::uint8_t* GlobalBytes;
+
+// A lane's weights of one tile and step.
 template <int TYPE>
-struct Chunk {
-  static constexpr int kParts = TYPE == LLMI_TYPE_Q4_0 ? 1 : 2;
-  u32x4 c[kParts];
-  f32x4 s;
-  __device__ __forceinline__ void load(const Matrices& m, std::size_t chunk, int lane) {
-    // A base common to the wavefront and a lane's offset.
-    const std::uint8_t* const codes_at = m.codes + chunk * (kParts * 1024);
-    const float* const scales_at = m.scales + chunk * 64;
-    const std::uint32_t at = static_cast<std::uint32_t>(lane) * 16;
+struct Weights {
+  typedef std::uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  std::uint32_t c[TYPE == LLMI_TYPE_Q4_0 ? 2 : 4];
+  float s[2];
+  // at: (expert * tiles + tile) * steps + step, common to the wavefront.
+  __device__ __forceinline__ void load(const Matrices& m, std::size_t at, int lane) {
+    // Lane offsets made here each time, so that the addresses stay a scalar
+    // base and a 32-bit offset.
+    std::uint32_t code_at = static_cast<std::uint32_t>(lane) * (TYPE == LLMI_TYPE_Q4_0 ? 8 : 16);
+    std::uint32_t scale_at = static_cast<std::uint32_t>(lane % kTile) * 8;
+    asm volatile("" : "+v"(code_at), "+v"(scale_at));
+    if constexpr (TYPE == LLMI_TYPE_Q4_0) {
+      const u32x2 v = *(const __attribute__((address_space(1))) u32x2*)((GlobalBytes)m.codes + at * 512 + code_at);
+      c[0] = v[0];
+      c[1] = v[1];
+    } else {
+      const u32x4 v = *(const __attribute__((address_space(1))) u32x4*)((GlobalBytes)m.codes + at * 1024 + code_at);
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) c[i] = *reinterpret_cast<const u32x4*>(codes_at + i * 1024 + at);
-    s = *reinterpret_cast<const f32x4*>(scales_at + static_cast<std::uint32_t>(lane % kTile) * kChunkBlocks);
+      for (int i = 0; i < 4; ++i) c[i] = v[i];
+    }
+    const f32x2 v = *(const __attribute__((address_space(1))) f32x2*)((GlobalBytes)(m.scales + at * kStepScales) + scale_at);
+    s[0] = v[0];
+    s[1] = v[1];
+  }
+  // For the compiler: the loads are complete.
+  __device__ __forceinline__ void here() {
+#pragma unroll
+    for (std::uint32_t& v : c) asm volatile("" : "+v"(v));
+#pragma unroll
+    for (float& v : s) asm volatile("" : "+v"(v));
   }
   __device__ __forceinline__ f16x8 codes(int b) const {
-    if constexpr (TYPE == LLMI_TYPE_Q4_0) return codes_q4(c[0][b]);
-    else return codes_q8(c[b / 2][b % 2 * 2], c[b / 2][b % 2 * 2 + 1]);
+    if constexpr (TYPE == LLMI_TYPE_Q4_0) return codes_q4(c[b]);
+    else return codes_q8(c[2 * b], c[2 * b + 1]);
   }
 };
 

@@ -14,6 +14,7 @@
 namespace llmi_hip::moe {
 namespace {
 
+constexpr int kChunk = 2 * kStep;  // inputs that a wavefront takes at a time
 constexpr int kMostRows = 8;  // rows of an expert that a wavefront takes at a time
 constexpr int kRowBytes = kChunk * 4 + 16;  // a row of a chunk in LDS, both parts; 16 bytes keep rows off each other's banks
 
@@ -83,22 +84,22 @@ struct Rows {
 
 // acc += factor * (x W^T) over one chunk: rows 4 (l / 16) .. + 3, output l % 16.
 template <int TYPE, int MATS>
-__device__ __forceinline__ void add_chunk(f32x4 (&acc)[MATS], const Chunk<TYPE> (&w)[MATS], const WaveLds& x, int last_row,
+__device__ __forceinline__ void add_chunk(f32x4 (&acc)[MATS], const Weights<TYPE> (&w)[MATS][2], const WaveLds& x, int last_row,
                                           int lane) {
   const std::uint8_t* at = x.rows + min(lane % kTile, last_row) * kRowBytes + lane / kTile * 16;
   f32x4 sum[MATS] = {};
 #pragma unroll
-  for (int b = 0; b < kChunkBlocks; ++b) {
+  for (int b = 0; b < 4; ++b) {
     const f16x8 high = *reinterpret_cast<const f16x8*>(at + b * (4 * kBlock));
     const f16x8 low = *reinterpret_cast<const f16x8*>(at + b * (4 * kBlock) + 2 * kBlock);
 #pragma unroll
     for (int m = 0; m < MATS; ++m) {
-      const f16x8 code = w[m].codes(b);
+      const f16x8 code = w[m][b / 2].codes(b % 2);
       f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
       d = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, code, d, 0, 0, 0);
       d = __builtin_amdgcn_mfma_f32_16x16x32_f16(low, code, d, 0, 0, 0);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sum[m][r] = __builtin_fmaf(d[r], w[m].s[b], sum[m][r]);
+      for (int r = 0; r < 4; ++r) sum[m][r] = __builtin_fmaf(d[r], w[m][b / 2].s[b % 2], sum[m][r]);
     }
   }
   const f32x4 f = *reinterpret_cast<const f32x4*>(x.factors + lane / kTile * 4);
@@ -114,7 +115,7 @@ struct FewArgs {
   const float* x;
   float* y;
   std::size_t x_stride, y_stride;
-  int slots, per_row, experts, out, in, tiles, chunks, rows;  // rows: LDS rows of a wavefront (even)
+  int slots, per_row, experts, out, in, tiles, steps, chunks, rows;  // rows: LDS rows of a wavefront (even)
 };
 
 // ------------------------------------------------- products of each slot
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
   if (expert < 0 || expert >= p.experts) return;
   std::uint64_t same = __ballot(mine == expert);
   if (__builtin_ctzll(same) != slot) return;
-  const std::size_t chunk0 = (static_cast<std::size_t>(expert) * p.tiles + tile) * p.chunks;
+  const std::size_t at0 = (static_cast<std::size_t>(expert) * p.tiles + tile) * p.steps;
   const int each = (p.chunks + kWaves - 1) / kWaves;
   const int c0 = min(wave * each, p.chunks), c1 = min(c0 + each, p.chunks);
   const WaveLds w{lds + wave * (p.rows * kRowBytes + 64), reinterpret_cast<float*>(lds + wave * (p.rows * kRowBytes + 64) + p.rows * kRowBytes)};
@@ -163,13 +164,18 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
         live[i] = true;
       }
       // Chunks in flight: the ring's places are filled kDepth chunks ahead.
-      Chunk<TYPE> ring[kDepth][kMats];
+      Weights<TYPE> ring[kDepth][kMats][2];
       Rows<kPairs, QUADS> x[kDepth];
       const auto ask = [&](int i, int c) {
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) x[i].load(j, at[j], c, p.in, lane);
-        ring[i][0].load(p.m, chunk0 + c, lane);
-        if constexpr (GATED) ring[i][1].load(p.up, chunk0 + c, lane);
+        // The last chunk may have one step only: taken twice, with x 0 behind its end.
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const std::size_t at = at0 + min(2 * c + t, p.steps - 1);
+          ring[i][0][t].load(p.m, at, lane);
+          if constexpr (GATED) ring[i][1][t].load(p.up, at, lane);
+        }
       };
 #pragma unroll
       for (int i = 0; i < kDepth; ++i)
@@ -220,7 +226,7 @@ struct SumArgs {
   const float *weights, *h, *residual;
   float* y;
   std::size_t r_stride, y_stride;
-  int tokens, top_k, experts, out, in, tiles, chunks, rows;
+  int tokens, top_k, experts, out, in, tiles, steps, chunks, rows;
 };
 
 // One workgroup a tile of 16 outputs, for all tokens (up to 16): its
@@ -248,7 +254,7 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
   constexpr int kDepth = PAIRS == 1 ? 4 : 2;
   for (int t0 = 0; t0 < p.tokens; t0 += 2 * PAIRS) {
     f32x4 acc[1] = {};
-    Chunk<TYPE> ring[kDepth][1];
+    Weights<TYPE> ring[kDepth][1][2];
     Rows<PAIRS, QUADS> x[kDepth];
     float times[kDepth][PAIRS];
     bool live[kDepth][PAIRS];
@@ -277,7 +283,9 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
         times[i][j] = sum;
         x[i].load(j, p.h + static_cast<std::size_t>(slot) * p.in, chunk, p.in, lane);
       }
-      ring[i][0].load(p.m, (static_cast<std::size_t>(e) * p.tiles + tile) * p.chunks + chunk, lane);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        ring[i][0][t].load(p.m, (static_cast<std::size_t>(e) * p.tiles + tile) * p.steps + min(2 * chunk + t, p.steps - 1), lane);
       at[i] = chunk;
       ++next;
       if (++chunk == p.chunks) {
@@ -339,7 +347,7 @@ int launch_few(const FewProduct& f, hipStream_t s) {
   const int rows = more ? kMostRows : 2;
   const FewArgs a{f.m, f.up, f.ids, f.x, f.y, f.x_stride, f.y_stride, static_cast<int>(f.slots), static_cast<int>(f.per_row),
                   static_cast<int>(sh.count), static_cast<int>(sh.out), static_cast<int>(sh.in), static_cast<int>(sh.tiles()),
-                  static_cast<int>(sh.chunks()), rows};
+                  static_cast<int>(sh.steps()), static_cast<int>(ceil_div(sh.steps(), 2)), rows};
   const unsigned grid = static_cast<unsigned>(f.slots * sh.tiles());
   with_flags([&](auto gated, auto more, auto quads) {
     const std::size_t lds = lds_bytes(kWaves, rows, gated ? 2 : 1);
@@ -356,7 +364,7 @@ int launch_few_sum(const FewSum& f, hipStream_t s) {
   const int rows = more ? kMostRows : 2;
   const SumArgs a{f.m, f.ids, f.weights, f.h, f.residual, f.y, f.r_stride, f.y_stride, static_cast<int>(f.tokens),
                   static_cast<int>(f.top_k), static_cast<int>(sh.count), static_cast<int>(sh.out), static_cast<int>(sh.in),
-                  static_cast<int>(sh.tiles()), static_cast<int>(sh.chunks()), rows};
+                  static_cast<int>(sh.tiles()), static_cast<int>(sh.steps()), static_cast<int>(ceil_div(sh.steps(), 2)), rows};
   const unsigned grid = static_cast<unsigned>(sh.tiles());
   const std::size_t lds = lds_bytes(kSumWaves, rows, 1);
   with_flags([&](auto more, auto quads) {

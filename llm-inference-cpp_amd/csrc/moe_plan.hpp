@@ -17,21 +17,22 @@ constexpr std::size_t kMaxTopK = 64;
 constexpr std::size_t kMaxSlots = std::size_t{1} << 24;  // rows of all experts together
 constexpr std::size_t kMaxInner = std::size_t{1} << 18;  // inputs, and results, of an expert's matrix
 
-constexpr int kTile = 16;        // outputs and rows of a matrix instruction
-constexpr int kChunkBlocks = 4;  // blocks of 32 weights that one 16-byte load of a lane covers (Q4_0)
+constexpr int kTile = 16;                         // outputs and rows of a matrix instruction
+constexpr int kStep = 2 * LLMI_BLOCK_SIZE;        // inputs of a step: two blocks
+constexpr std::size_t kStepScales = 2 * kTile;    // a tile's scales of a step
 
 // The shape of a set of experts as the device holds it: per expert, tiles of
-// 16 outputs; per tile, chunks of 4 blocks (128 inputs; the last one filled
-// up with codes and scales of 0).
+// 16 outputs; per tile, steps of 64 inputs (outputs and inputs behind the last
+// ones have codes and scales of 0).
 struct Shape {
   int type = 0;
   std::size_t count = 0, out = 0, in = 0;
   std::size_t blocks() const { return (in + LLMI_BLOCK_SIZE - 1) / LLMI_BLOCK_SIZE; }
-  std::size_t chunks() const { return (blocks() + kChunkBlocks - 1) / kChunkBlocks; }
+  std::size_t steps() const { return (in + kStep - 1) / kStep; }
   std::size_t tiles() const { return (out + kTile - 1) / kTile; }
-  std::size_t chunk_bytes() const { return type == LLMI_TYPE_Q4_0 ? 1024 : 2048; }
-  std::size_t code_bytes() const { return count * tiles() * chunks() * chunk_bytes(); }
-  std::size_t scale_floats() const { return count * tiles() * chunks() * kTile * kChunkBlocks; }
+  std::size_t step_bytes() const { return type == LLMI_TYPE_Q4_0 ? 512 : 1024; }
+  std::size_t code_bytes() const { return count * tiles() * steps() * step_bytes(); }
+  std::size_t scale_floats() const { return count * tiles() * steps() * kStepScales; }
 };
 
 inline std::string check_shape(const Shape& s) {
@@ -41,12 +42,25 @@ inline std::string check_shape(const Shape& s) {
   return {};
 }
 
-// Rows of an expert that a workgroup of the grouped products takes.
-constexpr std::size_t kRows = 64;
-// Groups of kRows rows of at most: every expert may leave one unfilled.
-inline std::size_t most_tiles(std::size_t slots, std::size_t experts) {
-  return slots / kRows + std::min(slots, experts);
+// Groups of so many rows of at most: every expert may leave one unfilled.
+inline std::size_t most_tiles(std::size_t slots, std::size_t experts, std::size_t rows) {
+  return slots / rows + std::min(slots, experts);
 }
+// Tiles of outputs of a workgroup: of the kernel for short work, of the one for long.
+inline std::size_t short_columns(bool gated) { return gated ? 2 : 4; }
+inline std::size_t long_columns(bool gated) { return 4 * short_columns(gated); }
+// The largest number of slots that goes to the kernel for short work.
+inline std::size_t most_short(const Shape& s, bool gated) {
+  const std::size_t columns = (s.tiles() + long_columns(gated) - 1) / long_columns(gated);
+  const std::size_t room = 256 / columns, left = s.count / 2;
+  return std::max(48 * s.count, room > left ? 64 * (room - left) : 0);
+}
+// Rows of an expert that a workgroup of a grouped product takes.
+inline std::size_t pick_rows(const Shape& s, std::size_t slots, bool gated) {
+  if (slots > most_short(s, gated)) return 64;
+  return slots <= 16 * s.count ? 16 : 32;
+}
+constexpr std::size_t kLeastRows = 16, kMostShortRows = 32;
 
 // Up to this many slots (a wavefront's lanes) and tokens (rows of a matrix
 // instruction) go without a grouping.
@@ -63,21 +77,29 @@ struct Layout {
     return at;
   }
 };
-// The slots in the order of their experts, and their groups of rows.
+// The slots in the order of their experts, and their groups of rows, for the
+// two products of an MLP.
 struct Grouping {
-  std::size_t counts, order, tiles;
+  std::size_t counts, order, tiles[2];
   void place(Layout* l, std::size_t slots, std::size_t experts) {
-    counts = l->take(2 * sizeof(std::int32_t));
+    counts = l->take(3 * sizeof(std::int32_t));
     order = l->take(slots * sizeof(std::int32_t));
-    tiles = l->take(most_tiles(slots, experts) * 4 * sizeof(std::int32_t));
+    for (std::size_t& t : tiles) t = l->take(most_tiles(slots, experts, kLeastRows) * 4 * sizeof(std::int32_t));
   }
 };
-// Rows in two fp16 parts (4 bytes an element, whole chunks) and their factors.
+// Rows in two fp16 parts (4 bytes an element, whole steps) and their factors:
+// `rows` rows as they are for the kernel for long work, or row tiles for the
+// one for short, whichever is more over all calls of at most so many slots,
+// so that a workspace for a number of slots holds every smaller one.
 struct Parts {
   std::size_t values, factors;
-  void place(Layout* l, std::size_t rows, const Shape& s) {
-    values = l->take(rows * s.chunks() * kChunkBlocks * LLMI_BLOCK_SIZE * 4);
-    factors = l->take(rows * sizeof(float));
+  void place(Layout* l, std::size_t rows, const Shape& s, std::size_t slots, bool gated) {
+    const std::size_t small = std::min(slots, most_short(s, gated));
+    const std::size_t tiled = std::max(most_tiles(small, s.count, kLeastRows) * kLeastRows,
+                                       most_tiles(small, s.count, kMostShortRows) * kMostShortRows);
+    const std::size_t n = std::max(rows, tiled);
+    values = l->take(n * s.steps() * kStep * 4);
+    factors = l->take(n * sizeof(float));
   }
 };
 struct MatmulLayout {
@@ -86,7 +108,7 @@ struct MatmulLayout {
   Parts x;
   MatmulLayout(const Shape& s, std::size_t slots, std::size_t per_row) {
     group.place(&all, slots, s.count);
-    x.place(&all, (slots + per_row - 1) / per_row, s);
+    x.place(&all, (slots + per_row - 1) / per_row, s, slots, false);
   }
 };
 struct MlpLayout {
@@ -97,9 +119,9 @@ struct MlpLayout {
   MlpLayout(const Shape& gate, const Shape& down, std::size_t tokens, std::size_t top_k) {
     const std::size_t slots = tokens * top_k;
     group.place(&all, slots, gate.count);
-    x.place(&all, tokens, gate);
+    x.place(&all, tokens, gate, slots, true);
     h = all.take(slots * gate.out * sizeof(float));
-    h_parts.place(&all, slots, down);
+    h_parts.place(&all, slots, down, slots, false);
     sums = all.take(slots * down.out * sizeof(float));
   }
 };

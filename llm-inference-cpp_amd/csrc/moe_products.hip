@@ -15,18 +15,26 @@ namespace llmi_hip::moe {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kRowTiles = static_cast<int>(kRows) / kTile;
 
 // x in two parts: one wavefront a row.  The factor is taken from the largest
 // finite |x|: an inf or NaN stays one in the high part and shows in its own
-// row alone.
-__global__ void __launch_bounds__(kThreads) split_kernel(const float* __restrict__ x, int rows, int in, int chunks,
-                                                         std::size_t stride, const std::int32_t* __restrict__ live,
-                                                         SplitRows to) {
+// row alone.  MT: in row tiles of 16 MT rows; 0: rows as they are.
+template <int MT>
+__global__ void __launch_bounds__(kThreads) split_kernel(RowSource src, int rows, const std::int32_t* __restrict__ live,
+                                                         Groups g, int list, SplitRows to) {
   const int lane = threadIdx.x & 63;
-  const int most = live != nullptr ? min(*live, rows) : rows;
+  const int in = static_cast<int>(src.in), padded = static_cast<int>(src.steps) * kStep;
+  constexpr int kRows = MT * kTile;
+  const int most = MT > 0 ? g.counts[1 + list] * kRows : live != nullptr ? min(*live, rows) : rows;
   for (int r = blockIdx.x * kWaves + (threadIdx.x >> 6); r < most; r += gridDim.x * kWaves) {
-    const float* row = x + static_cast<std::size_t>(r) * stride;
+    std::size_t from = static_cast<std::size_t>(r);
+    if constexpr (MT > 0) {
+      const RowTile t = (list == 0 ? g.tiles[0] : g.tiles[1])[r / kRows];
+      if (r % kRows >= t.rows) continue;  // nothing reads its results
+      const int pos = t.first + r % kRows;
+      from = src.per_row > 0 ? static_cast<std::size_t>(g.order[pos]) / src.per_row : static_cast<std::size_t>(pos);
+    }
+    const float* row = src.x + from * src.stride;
     const auto load8 = [&](int k, float (&v)[8]) {
       if (k + 8 <= in) {
         const f4 a = *reinterpret_cast<const f4*>(row + k), b = *reinterpret_cast<const f4*>(row + k + 4);
@@ -51,8 +59,7 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const float* __restrict
     for (int o = 32; o > 0; o >>= 1) top = max(top, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
     const Factor f(top);
     if (lane == 0) to.factors[r] = f.back;
-    _Float16* out = to.values + static_cast<std::size_t>(r) * chunks * (kChunkBlocks * kBlock * 2);
-    for (int k = lane * 8; k < chunks * kChunkBlocks * kBlock; k += 512) {
+    for (int k = lane * 8; k < padded; k += 512) {
       float v[8];
       load8(k, v);
       f16x8 high, low;
@@ -63,9 +70,16 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const float* __restrict
         high[i] = a;
         low[i] = b;
       }
-      _Float16* at = out + (k / kBlock) * 2 * kBlock + k % kBlock;
-      *reinterpret_cast<f16x8*>(at) = high;
-      *reinterpret_cast<f16x8*>(at + kBlock) = low;
+      if constexpr (MT > 0) {
+        const std::size_t piece = ((static_cast<std::size_t>(r / kRows) * src.steps + k / kStep) * MT + r % kRows / kTile) * 4 + k % kStep / kBlock * 2;
+        f16x8* at = reinterpret_cast<f16x8*>(to.values) + piece * 64 + k % kBlock / 8 * kTile + r % kTile;
+        at[0] = high;
+        at[64] = low;
+      } else {
+        _Float16* at = to.values + (static_cast<std::size_t>(r) * padded + k / kBlock * kBlock) * 2 + k % kBlock;
+        *reinterpret_cast<f16x8*>(at) = high;
+        *reinterpret_cast<f16x8*>(at + kBlock) = low;
+      }
     }
   }
 }
@@ -76,111 +90,317 @@ struct ProductArgs {
   Groups g;
   float* y;
   std::size_t y_stride;
-  int out, tiles, chunks, per_row, x_by_position, y_by_position, columns;  // columns: groups of 16 * kWaves * NT outputs
+  int out, tiles, steps, per_row, y_by_position, columns;  // columns: groups of outputs that a workgroup takes
+  int first, list;  // unit of the first workgroup; which tile list
 };
 
-// A workgroup takes 64 rows of one expert and 4 wavefronts' outputs beside
-// each other; the rows' parts of a chunk go through LDS.
-template <int TYPE, int NT, bool GATED>
-__global__ void __launch_bounds__(kThreads) product_kernel(ProductArgs p) {
-  __shared__ __attribute__((aligned(16))) f16x8 xs[kRowTiles * kChunkBlocks * 2][64];
-  constexpr int kMats = GATED ? 2 : 1;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int units = p.g.counts[1] * p.columns;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const RowTile rt = p.g.tiles[u / p.columns];
-    const int col0 = (u % p.columns) * kWaves * NT + wave * NT;
-    // The row that this lane stages: row lane % 16 of each tile of 16, rows
-    // past the last one repeating it (their results are not stored).
-    const _Float16* src[kRowTiles];
+// 16 bytes of each lane, OFFSET behind its own address, into LDS, lane after
+// lane from `to` (common to the wavefront).  Nothing waits for it but landed().
+// The instruction adds its offset to both addresses.
+template <int OFFSET>
+__device__ __forceinline__ void to_lds(const std::uint8_t* from, std::uint32_t to) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(from), "s"(to - OFFSET), "n"(OFFSET) : "memory");
+}
+// All of this wavefront's loads have landed and its reads of LDS are done;
+// then those of the workgroup's.
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// fn of 0 .. N - 1 as constants.
+template <int N, typename Fn>
+__device__ __forceinline__ void each(Fn&& fn) {
+  if constexpr (N > 0) {
+    each<N - 1>(fn);
+    fn(std::integral_constant<int, N - 1>{});
+  }
+}
+
+// A workgroup takes 16 MT rows of one expert and, with its 4 wavefronts beside
+// each other, 64 NT outputs (32 NT of each matrix of a gated pair).  The rows'
+// parts go through LDS, 64 inputs at a time in two buffers, filled while the
+// other one is used; the weights stay in the registers of the wavefront that
+// uses them.
+template <int TYPE, int MT, int NT, bool GATED>
+__global__ void __launch_bounds__(kThreads, 2) long_kernel(ProductArgs p) {
+  constexpr int kParts = MT * 4;  // 1 KiB pieces of a buffer: (16 rows, block, high / low)
+  __shared__ __attribute__((aligned(16))) f16x8 xs[2][kParts][64];
+  __shared__ std::int32_t to_row[MT * kTile];  // y's rows, and the factors of x's
+  __shared__ float back[MT * kTile];
+  constexpr int kCols = GATED ? NT / 2 : NT;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int units = p.g.counts[1 + p.list] * p.columns;
+  // Workgroups go to the 8 XCDs in turn: each XCD takes neighbouring units.
+  const int per = (units + 7) / 8, b = p.first + static_cast<int>(blockIdx.x), u = b % 8 * per + b / 8;
+  if (b / 8 >= per || u >= units) return;
+  const int tile = u / p.columns;
+  const RowTile rt = (p.list == 0 ? p.g.tiles[0] : p.g.tiles[1])[tile];
+  const int expert = __builtin_amdgcn_readfirstlane(rt.expert), first = __builtin_amdgcn_readfirstlane(rt.first);
+  const int rows = __builtin_amdgcn_readfirstlane(rt.rows);
+  const int col0 = (u % p.columns) * kWaves * kCols + wave * kCols;
+  // Rows past the last one repeat it; their results are not stored.
+  const auto x_row = [&](int pos) { return p.per_row == 0 ? pos : p.g.order[pos] / p.per_row; };
+  if (threadIdx.x < MT * kTile) {
+    const int pos = first + min(static_cast<int>(threadIdx.x), rows - 1);
+    to_row[threadIdx.x] = p.y_by_position ? pos : p.g.order[pos];
+    back[threadIdx.x] = p.x.factors[x_row(pos)];
+  }
+  // The rows that this lane brings in: row lane / 4 of each of the wavefront's
+  // tiles of 16, so that 4 lanes read 64 bytes beside each other.  In LDS a
+  // row's four 16 bytes lie side by side, in an order that differs from 4 rows
+  // to the next: lanes that read one input group of 16 rows use all banks.
+  constexpr int kOwn = (MT + kWaves - 1) / kWaves;
+  const std::uint8_t* src[kOwn];
 #pragma unroll
-    for (int i = 0; i < kRowTiles; ++i) {
-      const int pos = rt.first + min(i * kTile + lane % kTile, rt.rows - 1);
-      const std::size_t row = p.x_by_position ? static_cast<std::size_t>(pos) : static_cast<std::size_t>(p.g.order[pos] / p.per_row);
-      src[i] = p.x.values + row * p.chunks * (kChunkBlocks * kBlock * 2) + lane / kTile * 8;
+  for (int i = 0; i < kOwn; ++i) {
+    const int pos = first + min((wave * kOwn + i) * kTile + lane / 4, rows - 1);
+    src[i] = reinterpret_cast<const std::uint8_t*>(p.x.values) + static_cast<std::size_t>(x_row(pos)) * p.steps * (kStep * 4) + (lane % 4 ^ lane / 16) * 16;
+  }
+  const int read_at = lane % kTile * 4 + (lane / kTile ^ lane % kTile / 4);
+  const std::uint32_t lds = static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>(&xs[0][0][0]));
+  const auto bring = [&](int buf) {  // the next 64 inputs
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+      if (MT % kWaves == 0 || wave * kOwn + i < MT) {
+        const std::uint32_t to = lds + ((buf * MT + wave * kOwn + i) * 4) * 1024;
+        to_lds<0>(src[i], to);
+        to_lds<64>(src[i], to + 1024);
+        to_lds<128>(src[i], to + 2048);
+        to_lds<192>(src[i], to + 3072);
+        src[i] += 256;
+      }
+  };
+  std::size_t at[kCols];
+#pragma unroll
+  for (int n = 0; n < kCols; ++n) at[n] = (static_cast<std::size_t>(expert) * p.tiles + min(col0 + n, p.tiles - 1)) * p.steps;
+  Weights<TYPE> w[2][NT];
+  const auto weights = [&](Weights<TYPE> (&to)[NT], int step) {
+#pragma unroll
+    for (int n = 0; n < kCols; ++n) {
+      to[n].load(p.m, at[n] + step, lane);
+      if constexpr (GATED) to[kCols + n].load(p.up, at[n] + step, lane);
     }
-    f32x4 acc[kMats][NT][kRowTiles] = {};
-    for (int c = 0; c < p.chunks; ++c) {
-      __syncthreads();
+  };
+  f32x4 acc[NT][MT] = {};
+  bring(0);
+  weights(w[0], 0);
+  landed();
 #pragma unroll
-      for (int i = 0; i < kRowTiles; ++i)
+  for (int n = 0; n < NT; ++n) w[0][n].here();
+  for (int h = 0; h < p.steps; h += 2) {
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const int part = wave * 2 + f;  // block, high / low
-          xs[i * kChunkBlocks * 2 + part][lane] = *reinterpret_cast<const f16x8*>(src[i] + (c * kChunkBlocks * 2 + part) * kBlock);
+      for (int j = 0; j < 2; ++j) {
+        if (h + j >= p.steps) break;
+        if (h + j + 1 < p.steps) {
+          bring(1 - j);
+          weights(w[1 - j], h + j + 1);
         }
-      __syncthreads();
-      Chunk<TYPE> w[kMats][NT];
+// Two outputs' tiles at a time: their four instructions, then the
+        // additions of the two before them, whose results are there by now.
+        // The regions keep the compiler from holding more operands at once
+        // than the registers have room for.
+        f16x8 code[NT];
+        f16x8 x[2][2];
+        f32x4 d[3][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) code[n] = w[j][n].codes(0);
+        x[0][0] = xs[j][0][read_at];
+        x[0][1] = xs[j][1][read_at];
+        constexpr int kPairs = NT / 2, kSteps = 2 * MT * kPairs;
+        const auto add = [&](auto step) {
+          constexpr int q = decltype(step)::value, i = q / kPairs % MT, n0 = q % kPairs * 2, b2 = q / (kPairs * MT);
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[n0 + n][i][r] = __builtin_fmaf(d[q % 3][n][r], w[j][n0 + n].s[b2], acc[n0 + n][i][r]);
+          // Here, not at the end of the block, where the compiler would put them all.
+#pragma unroll
+          for (int n = 0; n < 2; ++n) asm volatile("" : "+v"(acc[n0 + n][i]));
+        };
+        each<kSteps>([&](auto step) {
+          constexpr int q = decltype(step)::value, ib = q / kPairs, i = ib % MT, n0 = q % kPairs * 2, b2 = ib / MT;
+          if constexpr (n0 == 0 && ib + 1 < 2 * MT) {  // the next rows' parts
+            x[(ib + 1) % 2][0] = xs[j][(ib + 1) % MT * 4 + (ib + 1) / MT * 2][read_at];
+            x[(ib + 1) % 2][1] = xs[j][(ib + 1) % MT * 4 + (ib + 1) / MT * 2 + 1][read_at];
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) d[q % 3][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ib % 2][0], code[n0 + n], f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+          for (int n = 0; n < 2; ++n) d[q % 3][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ib % 2][1], code[n0 + n], d[q % 3][n], 0, 0, 0);
+          if constexpr (q > 1) add(std::integral_constant<int, q - 2>{});
+          if constexpr (b2 == 0 && i == MT - 1) {  // the next block's codes
+#pragma unroll
+            for (int n = 0; n < 2; ++n) code[n0 + n] = w[j][n0 + n].codes(1);
+          }
+#pragma unroll
+          for (int i2 = 0; i2 < 4; ++i2) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                              // one matrix instruction,
+            __builtin_amdgcn_sched_group_barrier(0x002, b2 == 0 && i == MT - 1 ? 6 : 2, 0);  // vector ones beside it
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        add(std::integral_constant<int, kSteps - 2>{});
+        add(std::integral_constant<int, kSteps - 1>{});
+        landed();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) w[1 - j][n].here();
+      }
+  }
+  // Lane l holds output l % 16 of rows 4 (l / 16) .. + 3.
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    if (i * kTile >= rows) break;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = i * kTile + lane / kTile * 4 + r;
+      const float f = back[row];
+      float* const to = p.y + static_cast<std::size_t>(to_row[row]) * p.y_stride;
+#pragma unroll
+      for (int n = 0; n < kCols; ++n) {
+        const int o = (col0 + n) * kTile + lane % kTile;
+        float v = acc[n][i][r] * f;
+        if constexpr (GATED) v = silu(v) * (acc[kCols + n][i][r] * f);
+        if (row < rows && o < p.out) to[o] = v;
+      }
+    }
+  }
+}
+
+// The same for few rows an expert, or little work: no LDS on the way.  A
+// workgroup takes 16 MT rows and 16 NT outputs (8 NT of each matrix of a
+// gated pair); its 4 wavefronts share the inputs, each with its own loads of
+// rows and weights in flight while it works on those before them, and their
+// sums meet in LDS, in their order.
+template <int TYPE, int MT, int NT, bool GATED>
+__global__ void __launch_bounds__(kThreads) short_kernel(ProductArgs p) {
+  constexpr int kCols = GATED ? NT / 2 : NT;
+  __shared__ float meet[kWaves][NT][MT][kTile][kTile];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int units = p.g.counts[1 + p.list] * p.columns;
+  const int per = (units + 7) / 8, b = p.first + static_cast<int>(blockIdx.x), u = b % 8 * per + b / 8;
+  if (b / 8 >= per || u >= units) return;
+  const int tile = u / p.columns, col0 = u % p.columns * kCols;
+  const RowTile rt = (p.list == 0 ? p.g.tiles[0] : p.g.tiles[1])[tile];
+  const int expert = __builtin_amdgcn_readfirstlane(rt.expert), first = __builtin_amdgcn_readfirstlane(rt.first);
+  const int rows = __builtin_amdgcn_readfirstlane(rt.rows);
+  // This wavefront's steps.
+  const int share = (p.steps + kWaves - 1) / kWaves;
+  const int h0 = min(wave * share, p.steps), h1 = min(h0 + share, p.steps);
+  const std::uint8_t* const src = reinterpret_cast<const std::uint8_t*>(p.x.values) + static_cast<std::size_t>(tile) * p.steps * (MT * 4096);
+  std::size_t at[kCols];
+#pragma unroll
+  for (int n = 0; n < kCols; ++n) at[n] = (static_cast<std::size_t>(expert) * p.tiles + min(col0 + n, p.tiles - 1)) * p.steps;
+  struct Stage {
+    Weights<TYPE> w[NT];
+    f16x8 x[MT][4];  // block, high / low
+  };
+  const auto ask = [&](Stage& s, int h) {
+#pragma unroll
+    for (int n = 0; n < kCols; ++n) {
+      s.w[n].load(p.m, at[n] + h, lane);
+      if constexpr (GATED) s.w[kCols + n].load(p.up, at[n] + h, lane);
+    }
+    std::uint32_t x_at = static_cast<std::uint32_t>(lane) * 16;
+    asm volatile("" : "+v"(x_at));
+    const GlobalBytes from = (GlobalBytes)src + static_cast<std::size_t>(h) * (MT * 4096);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) s.x[i][f] = *(const __attribute__((address_space(1))) f16x8*)(from + (i * 4 + f) * 1024 + x_at);
+  };
+  f32x4 acc[NT][MT] = {};
+  const auto work = [&](const Stage& s) {
+#pragma unroll
+    for (int b2 = 0; b2 < 2; ++b2)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const std::size_t at = (static_cast<std::size_t>(rt.expert) * p.tiles + min(col0 + n, p.tiles - 1)) * p.chunks + c;
-        w[0][n].load(p.m, at, lane);
-        if constexpr (GATED) w[1][n].load(p.up, at, lane);
+        const f16x8 code = s.w[n].codes(b2);
+        f32x4 d[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) d[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(s.x[i][2 * b2], code, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) d[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(s.x[i][2 * b2 + 1], code, d[i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[n][i][r] = __builtin_fmaf(d[i][r], s.w[n].s[b2], acc[n][i][r]);
       }
-#pragma unroll
-      for (int b = 0; b < kChunkBlocks; ++b)
-#pragma unroll
-        for (int m = 0; m < kMats; ++m)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const f16x8 code = w[m][n].codes(b);
-#pragma unroll
-            for (int i = 0; i < kRowTiles; ++i) {
-              f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
-              d = __builtin_amdgcn_mfma_f32_16x16x32_f16(xs[(i * kChunkBlocks + b) * 2][lane], code, d, 0, 0, 0);
-              d = __builtin_amdgcn_mfma_f32_16x16x32_f16(xs[(i * kChunkBlocks + b) * 2 + 1][lane], code, d, 0, 0, 0);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) acc[m][n][i][r] = __builtin_fmaf(d[r], w[m][n].s[b], acc[m][n][i][r]);
-            }
-          }
+  };
+  if (h0 < h1) {
+    Stage s0, s1;
+    ask(s0, h0);
+    for (int h = h0; h < h1; h += 2) {
+      ask(s1, min(h + 1, h1 - 1));
+      work(s0);
+      if (h + 1 >= h1) break;
+      ask(s0, min(h + 2, h1 - 1));
+      work(s1);
     }
-    // Lane l holds output l % 16 of rows 4 (l / 16) .. + 3.
+  }
 #pragma unroll
-    for (int i = 0; i < kRowTiles; ++i)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int at = i * kTile + lane / kTile * 4 + r;
-        if (at >= rt.rows) continue;
-        const int pos = rt.first + at, slot = p.g.order[pos];
-        const float back = p.x.factors[p.x_by_position ? pos : slot / p.per_row];
-        float* to = p.y + static_cast<std::size_t>(p.y_by_position ? pos : slot) * p.y_stride;
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int o = (col0 + n) * kTile + lane % kTile;
-          float v = acc[0][n][i][r] * back;
-          if constexpr (GATED) v = silu(v) * (acc[kMats - 1][n][i][r] * back);
-          if (o < p.out) to[o] = v;
-        }
-      }
+      for (int r = 0; r < 4; ++r) meet[wave][n][i][lane / kTile * 4 + r][lane % kTile] = acc[n][i][r];
+  __syncthreads();
+  for (int t = threadIdx.x; t < min(rows, MT * kTile) * (kCols * kTile); t += kThreads) {
+    const int row = t / (kCols * kTile), col = t % (kCols * kTile), o = col0 * kTile + col;
+    const int n = col / kTile, i = row / kTile;
+    if (o >= p.out) continue;
+    float v[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      v[0] += meet[w][n][i][row % kTile][col % kTile];
+      if constexpr (GATED) v[1] += meet[w][kCols + n][i][row % kTile][col % kTile];
+    }
+    const int pos = first + row;
+    const float f = p.x.factors[tile * (MT * kTile) + row];
+    float* const to = p.y + static_cast<std::size_t>(p.y_by_position ? pos : p.g.order[pos]) * p.y_stride;
+    to[o] = GATED ? silu(v[0] * f) * (v[1] * f) : v[0] * f;
   }
 }
 
 }  // namespace
 
-int launch_split(const float* x, std::size_t rows, std::size_t in, std::size_t chunks, std::size_t stride,
-                 const std::int32_t* live, const SplitRows& to, hipStream_t s) {
+int launch_split(const RowSource& x, std::size_t rows, const std::int32_t* live, const SplitRows& to, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(std::min<std::size_t>(ceil_div(rows, kWaves), kMostGroups));
-  split_kernel<<<grid, kThreads, 0, s>>>(x, static_cast<int>(rows), static_cast<int>(in), static_cast<int>(chunks), stride, live, to);
+  split_kernel<0><<<grid, kThreads, 0, s>>>(x, static_cast<int>(rows), live, Groups{}, 0, to);
+  LLMI_TRY_HIP(hipGetLastError());
+  return LLMI_OK;
+}
+
+int launch_split_tiles(const RowSource& x, const Groups& g, int list, std::size_t slots, std::size_t experts,
+                       const SplitRows& to, hipStream_t s) {
+  const std::size_t rows = static_cast<std::size_t>(g.rows[list]);
+  const unsigned grid = static_cast<unsigned>(std::min<std::size_t>(ceil_div(most_tiles(slots, experts, rows) * rows, kWaves), kMostGroups));
+  if (rows == 16) split_kernel<1><<<grid, kThreads, 0, s>>>(x, 0, nullptr, g, list, to);
+  else split_kernel<2><<<grid, kThreads, 0, s>>>(x, 0, nullptr, g, list, to);
   LLMI_TRY_HIP(hipGetLastError());
   return LLMI_OK;
 }
 
 int launch_product(const Product& p, hipStream_t s) {
   const bool gated = p.up.codes != nullptr;
-  const int nt = gated ? 1 : 2;
-  const std::size_t columns = ceil_div(p.shape.tiles(), static_cast<std::size_t>(kWaves * nt));
-  const std::size_t most = most_tiles(p.slots, p.shape.count) * columns;
-  LLMI_REQUIRE(most <= 0x7FFFFFFFu, "moe: too many slots and results");
-  const unsigned grid = static_cast<unsigned>(std::min<std::size_t>(most, kMostGroups));
-  const ProductArgs a{p.m, p.up, p.x, p.g, p.y, p.y_stride, static_cast<int>(p.shape.out), static_cast<int>(p.shape.tiles()),
-                      static_cast<int>(p.shape.chunks()), static_cast<int>(p.per_row), p.x_by_position, p.y_by_position,
-                      static_cast<int>(columns)};
-  if (p.shape.type == LLMI_TYPE_Q4_0) {
-    if (gated) product_kernel<LLMI_TYPE_Q4_0, 1, true><<<grid, kThreads, 0, s>>>(a);
-    else product_kernel<LLMI_TYPE_Q4_0, 2, false><<<grid, kThreads, 0, s>>>(a);
-  } else {
-    if (gated) product_kernel<LLMI_TYPE_Q8_0, 1, true><<<grid, kThreads, 0, s>>>(a);
-    else product_kernel<LLMI_TYPE_Q8_0, 2, false><<<grid, kThreads, 0, s>>>(a);
+  constexpr int kNT = 4;
+  const int rows = p.g.rows[p.list];
+  const std::size_t cols = rows <= static_cast<int>(kMostShortRows) ? short_columns(gated) : long_columns(gated);
+  const std::size_t columns = ceil_div(p.shape.tiles(), cols);
+  const std::size_t all = ceil_div(most_tiles(p.slots, p.shape.count, static_cast<std::size_t>(rows)) * columns, 8) * 8;
+  ProductArgs a{p.m, p.up, p.x, p.g, p.y, p.y_stride, static_cast<int>(p.shape.out), static_cast<int>(p.shape.tiles()),
+                static_cast<int>(p.shape.steps()), static_cast<int>(p.per_row), p.y_by_position, static_cast<int>(columns), 0, p.list};
+  for (std::size_t first = 0; first < all; first += kMostGroups) {
+    a.first = static_cast<int>(first);
+    const unsigned grid = static_cast<unsigned>(std::min(all - first, kMostGroups));
+    const auto run = [&](auto type, auto gate) {
+      switch (rows) {
+        case 16: short_kernel<type, 1, kNT, gate><<<grid, kThreads, 0, s>>>(a); break;
+        case 32: short_kernel<type, 2, kNT, gate><<<grid, kThreads, 0, s>>>(a); break;
+        default: long_kernel<type, 4, kNT, gate><<<grid, kThreads, 0, s>>>(a); break;
+      }
+    };
+    constexpr std::integral_constant<int, LLMI_TYPE_Q4_0> q4{};
+    constexpr std::integral_constant<int, LLMI_TYPE_Q8_0> q8{};
+    if (p.shape.type == LLMI_TYPE_Q4_0) gated ? run(q4, std::true_type{}) : run(q4, std::false_type{});
+    else gated ? run(q8, std::true_type{}) : run(q8, std::false_type{});
   }
   LLMI_TRY_HIP(hipGetLastError());
   return LLMI_OK;

@@ -51,13 +51,14 @@ int main() {
   expect(!check_route(kMaxSlots + 1, 8, 2, 8).empty(), "too many routed tokens");
 
   // Row tiles never exceed the bound: the worst spread leaves one slot over in every expert.
+  for (std::size_t rows : {16u, 32u, 64u, 128u})
   for (std::size_t experts : {1u, 2u, 7u, 64u})
     for (std::size_t slots = 0; slots < 700; ++slots)
       for (std::size_t spare = 0; spare <= std::min(slots, experts); ++spare) {
         std::size_t tiles = spare > 0 ? spare - 1 : 0;  // spare - 1 experts with one slot each, the rest in one
         const std::size_t rest = slots - tiles;
-        tiles += (rest + kRows - 1) / kRows;
-        expect(tiles <= most_tiles(slots, experts), "row tiles", slots, experts);
+        tiles += (rest + rows - 1) / rows;
+        expect(tiles <= most_tiles(slots, experts, rows), "row tiles", slots, experts);
       }
   // A workspace for more slots holds fewer, and the last region ends inside it.
   std::size_t before = 0;
