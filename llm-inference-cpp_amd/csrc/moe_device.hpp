@@ -46,6 +46,16 @@ __device__ __forceinline__ f16x8 codes_q8(std::uint32_t lo, std::uint32_t hi) {
 
 typedef const __attribute__((address_space(1))) std::uint8_t* GlobalBytes;
 
+// A lane's offsets, opaque at each use: addresses stay a scalar base and a
+// 32-bit offset (hoisted out of a loop, the compiler would make them 64 bits).
+struct LaneAt {
+  std::uint32_t by8, by16, scale;
+  __device__ __forceinline__ explicit LaneAt(int lane)
+      : by8(static_cast<std::uint32_t>(lane) * 8), by16(static_cast<std::uint32_t>(lane) * 16),
+        scale(static_cast<std::uint32_t>(lane % kTile) * 8) {}
+  __device__ __forceinline__ void here() { asm volatile("" : "+v"(by8), "+v"(by16), "+v"(scale)); }
+};
+
 // A lane's weights of one tile and step.
 template <int TYPE>
 struct Weights {
@@ -54,12 +64,9 @@ struct Weights {
   std::uint32_t c[TYPE == LLMI_TYPE_Q4_0 ? 2 : 4];
   float s[2];
   // at: (expert * tiles + tile) * steps + step, common to the wavefront.
-  __device__ __forceinline__ void load(const Matrices& m, std::size_t at, int lane) {
-    // Lane offsets made here each time, so that the addresses stay a scalar
-    // base and a 32-bit offset.
-    std::uint32_t code_at = static_cast<std::uint32_t>(lane) * (TYPE == LLMI_TYPE_Q4_0 ? 8 : 16);
-    std::uint32_t scale_at = static_cast<std::uint32_t>(lane % kTile) * 8;
-    asm volatile("" : "+v"(code_at), "+v"(scale_at));
+  __device__ __forceinline__ void load(const Matrices& m, std::size_t at, LaneAt& lane) {
+    lane.here();
+    const std::uint32_t code_at = TYPE == LLMI_TYPE_Q4_0 ? lane.by8 : lane.by16, scale_at = lane.scale;
     if constexpr (TYPE == LLMI_TYPE_Q4_0) {
       const u32x2 v = *(const __attribute__((address_space(1))) u32x2*)((GlobalBytes)m.codes + at * 512 + code_at);
       c[0] = v[0];

@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
   const int c0 = min(wave * each, p.chunks), c1 = min(c0 + each, p.chunks);
   const WaveLds w{lds + wave * (p.rows * kRowBytes + 64), reinterpret_cast<float*>(lds + wave * (p.rows * kRowBytes + 64) + p.rows * kRowBytes)};
   float* const meet = reinterpret_cast<float*>(lds);
+  LaneAt lane_at(lane);
 
   while (same != 0) {
     // Up to kMostRows of the expert's slots at a time: lane r holds the r-th.
@@ -173,8 +174,8 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const std::size_t at = at0 + min(2 * c + t, p.steps - 1);
-          ring[i][0][t].load(p.m, at, lane);
-          if constexpr (GATED) ring[i][1][t].load(p.up, at, lane);
+          ring[i][0][t].load(p.m, at, lane_at);
+          if constexpr (GATED) ring[i][1][t].load(p.up, at, lane_at);
         }
       };
 #pragma unroll
@@ -251,6 +252,7 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
   const int u0 = min(wave * each, units), u1 = min(u0 + each, units);
   const WaveLds w{lds + wave * (p.rows * kRowBytes + 64), reinterpret_cast<float*>(lds + wave * (p.rows * kRowBytes + 64) + p.rows * kRowBytes)};
   float* const meet = reinterpret_cast<float*>(lds);
+  LaneAt lane_at(lane);
   constexpr int kDepth = PAIRS == 1 ? 4 : 2;
   for (int t0 = 0; t0 < p.tokens; t0 += 2 * PAIRS) {
     f32x4 acc[1] = {};
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        ring[i][0][t].load(p.m, (static_cast<std::size_t>(e) * p.tiles + tile) * p.steps + min(2 * chunk + t, p.steps - 1), lane);
+        ring[i][0][t].load(p.m, (static_cast<std::size_t>(e) * p.tiles + tile) * p.steps + min(2 * chunk + t, p.steps - 1), lane_at);
       at[i] = chunk;
       ++next;
       if (++chunk == p.chunks) {

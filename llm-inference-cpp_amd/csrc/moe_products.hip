@@ -152,9 +152,9 @@ __global__ void __launch_bounds__(kThreads, 2) long_kernel(ProductArgs p) {
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
     const int pos = first + min((wave * kOwn + i) * kTile + lane / 4, rows - 1);
-    src[i] = reinterpret_cast<const std::uint8_t*>(p.x.values) + static_cast<std::size_t>(x_row(pos)) * p.steps * (kStep * 4) + (lane % 4 ^ lane / 16) * 16;
+    src[i] = reinterpret_cast<const std::uint8_t*>(p.x.values) + static_cast<std::size_t>(x_row(pos)) * p.steps * (kStep * 4) + (lane % 4 ^ (4 - lane / 16) % 4) * 16;
   }
-  const int read_at = lane % kTile * 4 + (lane / kTile ^ lane % kTile / 4);
+  const int read_at = lane % kTile * 4 + (lane / kTile ^ (4 - lane % kTile / 4) % 4);
   const std::uint32_t lds = static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>(&xs[0][0][0]));
   const auto bring = [&](int buf) {  // the next 64 inputs
 #pragma unroll
@@ -172,11 +172,12 @@ __global__ void __launch_bounds__(kThreads, 2) long_kernel(ProductArgs p) {
 #pragma unroll
   for (int n = 0; n < kCols; ++n) at[n] = (static_cast<std::size_t>(expert) * p.tiles + min(col0 + n, p.tiles - 1)) * p.steps;
   Weights<TYPE> w[2][NT];
+  LaneAt lane_at(lane);
   const auto weights = [&](Weights<TYPE> (&to)[NT], int step) {
 #pragma unroll
     for (int n = 0; n < kCols; ++n) {
-      to[n].load(p.m, at[n] + step, lane);
-      if constexpr (GATED) to[kCols + n].load(p.up, at[n] + step, lane);
+      to[n].load(p.m, at[n] + step, lane_at);
+      if constexpr (GATED) to[kCols + n].load(p.up, at[n] + step, lane_at);
     }
   };
   f32x4 acc[NT][MT] = {};
@@ -292,19 +293,19 @@ __global__ void __launch_bounds__(kThreads) short_kernel(ProductArgs p) {
     Weights<TYPE> w[NT];
     f16x8 x[MT][4];  // block, high / low
   };
+  LaneAt lane_at(lane);
   const auto ask = [&](Stage& s, int h) {
 #pragma unroll
     for (int n = 0; n < kCols; ++n) {
-      s.w[n].load(p.m, at[n] + h, lane);
-      if constexpr (GATED) s.w[kCols + n].load(p.up, at[n] + h, lane);
+      s.w[n].load(p.m, at[n] + h, lane_at);
+      if constexpr (GATED) s.w[kCols + n].load(p.up, at[n] + h, lane_at);
     }
-    std::uint32_t x_at = static_cast<std::uint32_t>(lane) * 16;
-    asm volatile("" : "+v"(x_at));
+    lane_at.here();
     const GlobalBytes from = (GlobalBytes)src + static_cast<std::size_t>(h) * (MT * 4096);
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int f = 0; f < 4; ++f) s.x[i][f] = *(const __attribute__((address_space(1))) f16x8*)(from + (i * 4 + f) * 1024 + x_at);
+      for (int f = 0; f < 4; ++f) s.x[i][f] = *(const __attribute__((address_space(1))) f16x8*)(from + (i * 4 + f) * 1024 + lane_at.by16);
   };
   f32x4 acc[NT][MT] = {};
   const auto work = [&](const Stage& s) {
