@@ -471,7 +471,7 @@ int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* u
   auto* sums = reinterpret_cast<float*>(w + l.sums);
   if (few_mlp(tokens, top_k)) {
     if (int rc = launch_few(FewProduct{gs, gate->view(), up->view(), ids, slots, top_k, x, x_stride, h, gs.out}, s)) return rc;
-    return launch_few_sum(FewSum{ds, down->view(), ids, weights, tokens, top_k, h, residual, residual_stride, y, y_stride}, s);
+    return launch_few_sum(FewSum{ds, down->view(), ids, weights, tokens, top_k, h, residual, residual_stride, y, y_stride, sums}, s);
   }
   if (int rc = launch_group(ids, slots, gs.count, g, s)) return rc;
   const RowSource src{x, x_stride, gs.in, gs.steps(), top_k}, h_src{h, ds.in, ds.in, ds.steps(), 0};

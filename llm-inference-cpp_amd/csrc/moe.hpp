@@ -100,6 +100,7 @@ struct FewSum {
   std::size_t r_stride;
   float* y;
   std::size_t y_stride;
+  float* parts;  // few_splits(shape) * tokens * out floats where there are several
 };
 int launch_few_sum(const FewSum& p, hipStream_t s);
 

@@ -25,6 +25,21 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// The largest of 32 lanes, in all of them: rotations within 16 lanes, then an
+// exchange of the two sixteens.
+__device__ __forceinline__ std::uint32_t max_of_half(std::uint32_t v) {
+  const auto ror = [](std::uint32_t x, auto by) {
+    return static_cast<std::uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x120 + decltype(by)::value, 0xF, 0xF, false));
+  };
+  v = max(v, ror(v, std::integral_constant<int, 8>{}));
+  v = max(v, ror(v, std::integral_constant<int, 4>{}));
+  v = max(v, ror(v, std::integral_constant<int, 2>{}));
+  v = max(v, ror(v, std::integral_constant<int, 1>{}));
+  const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return max(both[0], both[1]);
+}
+
 // A wavefront's part of LDS: 2 or kMostRows rows of a chunk in two parts, and what
 // each row's sum is multiplied by.
 struct WaveLds {
@@ -62,8 +77,7 @@ struct Rows {
         x[i] = live[p] && i < left ? v[p][i] : 0.0f;
         top = max(top, finite_bits(x[i]));
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = max(top, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
+      top = max_of_half(top);
       const Factor f(top);
       f16x4 high, low;
 #pragma unroll
@@ -225,20 +239,21 @@ struct SumArgs {
   Matrices m;
   const std::int32_t* ids;
   const float *weights, *h, *residual;
-  float* y;
-  std::size_t r_stride, y_stride;
-  int tokens, top_k, experts, out, in, tiles, steps, chunks, rows;
+  float* y;  // or partial sums [split][token][out], without the residual
+  std::size_t r_stride, y_stride, split_stride;
+  int tokens, top_k, experts, out, in, tiles, steps, chunks, rows, splits;
 };
 
-// One workgroup a tile of 16 outputs, for all tokens (up to 16): its
-// wavefronts share the chunks of all chosen experts.  Row m of a product is
-// token m, with the weight that it gives the expert (0 where it has not
-// chosen it), so the sums over inputs and over experts are one.
+// One workgroup a tile of 16 outputs (or, where the tiles are too few for the
+// chip, a part of its inputs), for all tokens (up to 16): its wavefronts
+// share the chunks of all chosen experts.  Row m of a product is token m, with
+// the weight that it gives the expert (0 where it has not chosen it), so the
+// sums over inputs and over experts are one.
 template <int TYPE, int PAIRS, bool QUADS>
 __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
   extern __shared__ __attribute__((aligned(16))) std::uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = blockIdx.x, slots = p.tokens * p.top_k;
+  const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles, slots = p.tokens * p.top_k;
   const std::int32_t mine = lane < slots ? p.ids[lane] : -1;
   const float weight = lane < slots ? p.weights[lane] : 0.0f;
   // Bit s: slot s is the first of its expert.
@@ -247,9 +262,10 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
     const int e = __builtin_amdgcn_readlane(mine, s);
     if (e >= 0 && e < p.experts && __builtin_ctzll(__ballot(mine == e)) == s) firsts |= std::uint64_t{1} << s;
   }
-  const int units = __builtin_popcountll(firsts) * p.chunks;  // (expert, chunk)
-  const int each = (units + kSumWaves - 1) / kSumWaves;
-  const int u0 = min(wave * each, units), u1 = min(u0 + each, units);
+  // Units (expert, chunk), in equal shares of the splits and their wavefronts.
+  const int units = __builtin_popcountll(firsts) * p.chunks, sharers = p.splits * kSumWaves;
+  const int each = (units + sharers - 1) / sharers;
+  const int u0 = min((split * kSumWaves + wave) * each, units), u1 = min(u0 + each, units);
   const WaveLds w{lds + wave * (p.rows * kRowBytes + 64), reinterpret_cast<float*>(lds + wave * (p.rows * kRowBytes + 64) + p.rows * kRowBytes)};
   float* const meet = reinterpret_cast<float*>(lds);
   LaneAt lane_at(lane);
@@ -261,38 +277,50 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
     float times[kDepth][PAIRS];
     bool live[kDepth][PAIRS];
     int at[kDepth];
-    // The unit that is asked for next: its number, chunk and expert (the
-    // lowest bit that is left).
+    // The unit that is asked for next: its number and chunk, its expert (the
+    // lowest bit that is left) and this lane's rows of it.
     std::uint64_t left = firsts;
     for (int i = u0 / p.chunks; i > 0 && left != 0; --i) left &= left - 1;
     int next = u0, chunk = u0 % p.chunks;
-    const auto ask = [&](int i) {
+    std::size_t w_at = 0;
+    const float* row[PAIRS];
+    float row_times[PAIRS];
+    bool row_live[PAIRS];
+    const auto enter = [&] {
       const int s = __builtin_ctzll(left), e = __builtin_amdgcn_readlane(mine, s);
       const std::uint64_t same = __ballot(mine == e);
+      w_at = (static_cast<std::size_t>(e) * p.tiles + tile) * p.steps;
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) {
         const int t = min(t0 + 2 * j + lane / 32, p.tokens - 1);
         std::uint64_t bits = same >> (t * p.top_k);
         if (p.top_k < 64) bits &= (std::uint64_t{1} << p.top_k) - 1;
-        live[i][j] = bits != 0;
+        row_live[j] = bits != 0;
         const int slot = bits != 0 ? t * p.top_k + __builtin_ctzll(bits) : s;
-        float sum = 0.0f;
+        row[j] = p.h + static_cast<std::size_t>(slot) * p.in;
+        row_times[j] = 0.0f;
         while (__any(bits != 0)) {  // an expert chosen twice counts with both weights
           const float one = __shfl(weight, bits != 0 ? t * p.top_k + __builtin_ctzll(bits) : 0, 64);
-          if (bits != 0) sum += one;
+          if (bits != 0) row_times[j] += one;
           bits &= bits - 1;
         }
-        times[i][j] = sum;
-        x[i].load(j, p.h + static_cast<std::size_t>(slot) * p.in, chunk, p.in, lane);
       }
+    };
+    if (u0 < u1) enter();
+    const auto ask = [&](int i) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-        ring[i][0][t].load(p.m, (static_cast<std::size_t>(e) * p.tiles + tile) * p.steps + min(2 * chunk + t, p.steps - 1), lane_at);
+      for (int t = 0; t < 2; ++t) ring[i][0][t].load(p.m, w_at + min(2 * chunk + t, p.steps - 1), lane_at);
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j) {
+        x[i].load(j, row[j], chunk, p.in, lane);
+        times[i][j] = row_times[j];
+        live[i][j] = row_live[j];
+      }
       at[i] = chunk;
-      ++next;
-      if (++chunk == p.chunks) {
+      if (++next < u1 && ++chunk == p.chunks) {
         chunk = 0;
         left &= left - 1;
+        enter();
       }
     };
 #pragma unroll
@@ -312,16 +340,28 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) meet[(wave * kTile + lane / kTile * 4 + r) * kTile + lane % kTile] = acc[0][r];
     __syncthreads();
-    const int row = threadIdx.x / kTile, t = t0 + row, o = tile * kTile + threadIdx.x % kTile;
-    if (row < 2 * PAIRS && t < p.tokens && o < p.out) {
+    const int r = threadIdx.x / kTile, t = t0 + r, o = tile * kTile + threadIdx.x % kTile;
+    if (r < 2 * PAIRS && t < p.tokens && o < p.out) {
       float v = 0.0f;
 #pragma unroll
       for (int i = 0; i < kSumWaves; ++i) v += meet[i * kTile * kTile + threadIdx.x];
       if (p.residual != nullptr) v = p.residual[static_cast<std::size_t>(t) * p.r_stride + o] + v;
-      p.y[static_cast<std::size_t>(t) * p.y_stride + o] = v;
+      p.y[static_cast<std::size_t>(split) * p.split_stride + static_cast<std::size_t>(t) * p.y_stride + o] = v;
     }
     __syncthreads();
   }
+}
+
+// y = residual + the sum of the splits, in their order.
+__global__ void __launch_bounds__(256) few_join_kernel(const float* __restrict__ parts, int splits, int tokens, int out,
+                                                       const float* residual, std::size_t r_stride, float* y,
+                                                       std::size_t y_stride) {
+  const int u = blockIdx.x * 256 + threadIdx.x, t = u / out, o = u % out;
+  if (t >= tokens) return;
+  float v = 0.0f;
+  for (int i = 0; i < splits; ++i) v += parts[(static_cast<std::size_t>(i) * tokens + t) * out + o];
+  if (residual != nullptr) v = residual[static_cast<std::size_t>(t) * r_stride + o] + v;
+  y[static_cast<std::size_t>(t) * y_stride + o] = v;
 }
 
 // fn of each flag as a std::bool_constant.
@@ -364,10 +404,13 @@ int launch_few_sum(const FewSum& f, hipStream_t s) {
   const Shape& sh = f.shape;
   const bool more = f.tokens > 2;
   const int rows = more ? kMostRows : 2;
-  const SumArgs a{f.m, f.ids, f.weights, f.h, f.residual, f.y, f.r_stride, f.y_stride, static_cast<int>(f.tokens),
-                  static_cast<int>(f.top_k), static_cast<int>(sh.count), static_cast<int>(sh.out), static_cast<int>(sh.in),
-                  static_cast<int>(sh.tiles()), static_cast<int>(sh.steps()), static_cast<int>(ceil_div(sh.steps(), 2)), rows};
-  const unsigned grid = static_cast<unsigned>(sh.tiles());
+  const std::size_t splits = few_splits(sh);
+  const bool joined = splits > 1;
+  const SumArgs a{f.m, f.ids, f.weights, f.h, joined ? nullptr : f.residual, joined ? f.parts : f.y, f.r_stride,
+                  joined ? sh.out : f.y_stride, f.tokens * sh.out, static_cast<int>(f.tokens), static_cast<int>(f.top_k),
+                  static_cast<int>(sh.count), static_cast<int>(sh.out), static_cast<int>(sh.in), static_cast<int>(sh.tiles()),
+                  static_cast<int>(sh.steps()), static_cast<int>(ceil_div(sh.steps(), 2)), rows, static_cast<int>(splits)};
+  const unsigned grid = static_cast<unsigned>(sh.tiles() * splits);
   const std::size_t lds = lds_bytes(kSumWaves, rows, 1);
   with_flags([&](auto more, auto quads) {
     constexpr int kPairs = more ? kMostRows / 2 : 1;
@@ -375,6 +418,12 @@ int launch_few_sum(const FewSum& f, hipStream_t s) {
     else few_sum_kernel<LLMI_TYPE_Q8_0, kPairs, quads><<<grid, kSumThreads, lds, s>>>(a);
   }, more, sh.in % 4 == 0);
   LLMI_TRY_HIP(hipGetLastError());
+  if (joined) {
+    few_join_kernel<<<static_cast<unsigned>(ceil_div(f.tokens * sh.out, 256)), 256, 0, s>>>(
+        f.parts, static_cast<int>(splits), static_cast<int>(f.tokens), static_cast<int>(sh.out), f.residual, f.r_stride, f.y,
+        f.y_stride);
+    LLMI_TRY_HIP(hipGetLastError());
+  }
   return LLMI_OK;
 }
 

@@ -67,6 +67,10 @@ constexpr std::size_t kLeastRows = 16, kMostShortRows = 32;
 constexpr std::size_t kFewSlots = 64, kFewTokens = 16;
 inline bool few_matmul(std::size_t slots) { return slots <= kFewSlots; }
 inline bool few_mlp(std::size_t tokens, std::size_t top_k) { return tokens * top_k <= kFewSlots && tokens <= kFewTokens; }
+// Workgroups that share the inputs of a tile in the second product of few
+// tokens, whose sums a launch of its own joins: where the tiles alone would
+// leave most of the chip idle.
+inline std::size_t few_splits(const Shape& s) { return s.tiles() >= 96 ? 1 : (128 + s.tiles() - 1) / s.tiles(); }
 
 // Places in a call's workspace, each a multiple of 256 bytes.
 struct Layout {
@@ -115,14 +119,15 @@ struct MlpLayout {
   Layout all;
   Grouping group;
   Parts x, h_parts;
-  std::size_t h, sums;
+  std::size_t h, sums;  // sums of each slot, or of each split
   MlpLayout(const Shape& gate, const Shape& down, std::size_t tokens, std::size_t top_k) {
     const std::size_t slots = tokens * top_k;
     group.place(&all, slots, gate.count);
     x.place(&all, tokens, gate, slots, true);
     h = all.take(slots * gate.out * sizeof(float));
     h_parts.place(&all, slots, down, slots, false);
-    sums = all.take(slots * down.out * sizeof(float));
+    const std::size_t few = std::min(tokens, kFewTokens) * few_splits(down);
+    sums = all.take(std::max(slots, few) * down.out * sizeof(float));
   }
 };
 
