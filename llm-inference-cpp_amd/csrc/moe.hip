@@ -423,7 +423,7 @@ int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids,
   LLMI_REQUIRE(why.empty(), "moe_matmul: " + why);
   hipStream_t s = pick(stream);
   if (few_matmul(slots))
-    return launch_few(FewProduct{sh, experts->view(), {}, ids, slots, per_row, x, x_stride, y, y_stride}, s);
+    return launch_few(FewProduct{sh, experts->view(), {}, ids, slots, per_row, x, x_stride, y, y_stride, {}}, s);
   auto* w = static_cast<std::uint8_t*>(work);
   const std::size_t rows = pick_rows(sh, slots, false);
   const Groups g = groups_at(w, l.group, rows, rows);
@@ -470,8 +470,10 @@ int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* u
   auto* h = reinterpret_cast<float*>(w + l.h);
   auto* sums = reinterpret_cast<float*>(w + l.sums);
   if (few_mlp(tokens, top_k)) {
-    if (int rc = launch_few(FewProduct{gs, gate->view(), up->view(), ids, slots, top_k, x, x_stride, h, gs.out}, s)) return rc;
-    return launch_few_sum(FewSum{ds, down->view(), ids, weights, tokens, top_k, h, residual, residual_stride, y, y_stride, sums}, s);
+    const FewParts parts{reinterpret_cast<_Float16*>(w + l.h), reinterpret_cast<float*>(w + l.h + l.few_factors),
+                         static_cast<int>(few_blocks(ds))};
+    if (int rc = launch_few(FewProduct{gs, gate->view(), up->view(), ids, slots, top_k, x, x_stride, nullptr, 0, parts}, s)) return rc;
+    return launch_few_sum(FewSum{ds, down->view(), ids, weights, tokens, top_k, parts, residual, residual_stride, y, y_stride, sums}, s);
   }
   if (int rc = launch_group(ids, slots, gs.count, g, s)) return rc;
   const RowSource src{x, x_stride, gs.in, gs.steps(), top_k}, h_src{h, ds.in, ds.in, ds.steps(), 0};

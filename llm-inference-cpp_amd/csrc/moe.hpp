@@ -75,8 +75,16 @@ struct Product {
 };
 int launch_product(const Product& p, hipStream_t s);
 
-// The same for at most kFewSlots slots, in one launch: y[slot] = W_expert
-// x[slot / per_row] (or the gated pair).
+// Results of a gated pair for the second product of few tokens, in two fp16
+// parts, each 32 of a row with a factor of their own: values [slot][block]
+// [high, low][32], factors [slot][block], a multiple of 4 blocks.
+struct FewParts {
+  _Float16* values;
+  float* factors;
+  int blocks;
+};
+// A product for at most kFewSlots slots, in one launch: y[slot] = W_expert
+// x[slot / per_row], or the gated pair into h.
 struct FewProduct {
   Shape shape;
   Matrices m, up;
@@ -86,17 +94,19 @@ struct FewProduct {
   std::size_t x_stride;
   float* y;
   std::size_t y_stride;
+  FewParts h;
 };
 int launch_few(const FewProduct& p, hipStream_t s);
 // y[t] = residual[t] + sum over j of weights[t][j] W_expert h[t * top_k + j]
-// for at most kFewSlots slots of at most kFewTokens tokens, h's rows side by side.
+// for at most kFewSlots slots of at most kFewTokens tokens.
 struct FewSum {
   Shape shape;
   Matrices m;
   const std::int32_t* ids;
   const float* weights;
   std::size_t tokens, top_k;
-  const float *h, *residual;
+  FewParts h;
+  const float* residual;
   std::size_t r_stride;
   float* y;
   std::size_t y_stride;

@@ -16,6 +16,7 @@ namespace {
 
 constexpr int kChunk = 2 * kStep;  // inputs that a wavefront takes at a time
 constexpr int kMostRows = 8;  // rows of an expert that a wavefront takes at a time
+constexpr int kFactorBytes = 4 * kMostRows * 4;  // factors of a chunk's blocks
 constexpr int kRowBytes = kChunk * 4 + 16;  // a row of a chunk in LDS, both parts; 16 bytes keep rows off each other's banks
 
 // Orders the lanes' LDS exchange of one wavefront for the compiler.
@@ -96,31 +97,40 @@ struct Rows {
   }
 };
 
-// acc += factor * (x W^T) over one chunk: rows 4 (l / 16) .. + 3, output l % 16.
-template <int TYPE, int MATS>
-__device__ __forceinline__ void add_chunk(f32x4 (&acc)[MATS], const Weights<TYPE> (&w)[MATS][2], const WaveLds& x, int last_row,
-                                          int lane) {
-  const std::uint8_t* at = x.rows + min(lane % kTile, last_row) * kRowBytes + lane / kTile * 16;
+// Block b of a chunk's rows times one tile's codes: rows 4 (l / 16) .., output
+// l % 16.  at: this lane's row and inputs.
+__device__ __forceinline__ f32x4 times_codes(const std::uint8_t* at, int b, const f16x8& code) {
+  const f16x8 high = *reinterpret_cast<const f16x8*>(at + b * (4 * kBlock));
+  const f16x8 low = *reinterpret_cast<const f16x8*>(at + b * (4 * kBlock) + 2 * kBlock);
+  f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+  d = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, code, d, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(low, code, d, 0, 0, 0);
+}
+// Rows past the ROWS that count read the last one: their results mean nothing.
+template <int ROWS>
+__device__ __forceinline__ const std::uint8_t* lane_row(const std::uint8_t* rows, int lane) {
+  return rows + min(lane % kTile, ROWS - 1) * kRowBytes + lane / kTile * 16;
+}
+
+// acc += factor * (x W^T) over one chunk, of MATS tiles.
+template <int TYPE, int MATS, int ROWS>
+__device__ __forceinline__ void add_chunk(f32x4 (&acc)[MATS], const Weights<TYPE> (&w)[MATS][2], const WaveLds& lds, int lane) {
+  constexpr int kR = ROWS < 4 ? ROWS : 4;
+  const std::uint8_t* const at = lane_row<ROWS>(lds.rows, lane);
   f32x4 sum[MATS] = {};
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const f16x8 high = *reinterpret_cast<const f16x8*>(at + b * (4 * kBlock));
-    const f16x8 low = *reinterpret_cast<const f16x8*>(at + b * (4 * kBlock) + 2 * kBlock);
+  for (int b = 0; b < 4; ++b)
 #pragma unroll
     for (int m = 0; m < MATS; ++m) {
-      const f16x8 code = w[m][b / 2].codes(b % 2);
-      f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
-      d = __builtin_amdgcn_mfma_f32_16x16x32_f16(high, code, d, 0, 0, 0);
-      d = __builtin_amdgcn_mfma_f32_16x16x32_f16(low, code, d, 0, 0, 0);
+      const f32x4 d = times_codes(at, b, w[m][b / 2].codes(b % 2));
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sum[m][r] = __builtin_fmaf(d[r], w[m][b / 2].s[b % 2], sum[m][r]);
+      for (int r = 0; r < kR; ++r) sum[m][r] = __builtin_fmaf(d[r], w[m][b / 2].s[b % 2], sum[m][r]);
     }
-  }
-  const f32x4 f = *reinterpret_cast<const f32x4*>(x.factors + lane / kTile * 4);
+  const f32x4 f = *reinterpret_cast<const f32x4*>(lds.factors + lane / kTile * 4);
 #pragma unroll
   for (int m = 0; m < MATS; ++m)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) acc[m][r] = __builtin_fmaf(sum[m][r], f[r], acc[m][r]);
+    for (int r = 0; r < kR; ++r) acc[m][r] = __builtin_fmaf(sum[m][r], f[r], acc[m][r]);
 }
 
 struct FewArgs {
@@ -128,28 +138,31 @@ struct FewArgs {
   const std::int32_t* ids;
   const float* x;
   float* y;
+  FewParts h;
   std::size_t x_stride, y_stride;
-  int slots, per_row, experts, out, in, tiles, steps, chunks, rows;  // rows: LDS rows of a wavefront (even)
+  int slots, per_row, experts, out, in, tiles, pairs, steps, chunks, rows;  // rows: LDS rows of a wavefront
 };
 
 // ------------------------------------------------- products of each slot
 
 constexpr int kWaves = 8, kThreads = kWaves * 64;
 
-// One workgroup for each slot and tile of 16 outputs; the first slot of an
-// expert takes all of its slots, the others leave.
+// One workgroup for each slot and 32 outputs (two tiles); the first slot of
+// an expert takes all of its slots, the others leave.  A gated pair's results
+// go to p.h in two parts, each 32 of a row with their own power of two.
 template <int TYPE, bool GATED, bool MORE, bool QUADS>
 __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
   extern __shared__ __attribute__((aligned(16))) std::uint8_t lds[];
-  constexpr int kMats = GATED ? 2 : 1;
+  constexpr int kMats = GATED ? 4 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int slot = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
+  const int slot = blockIdx.x / p.pairs, pair = blockIdx.x % p.pairs;
   const std::int32_t mine = lane < p.slots ? p.ids[lane] : -1;
   const int expert = __builtin_amdgcn_readlane(mine, slot);
   if (expert < 0 || expert >= p.experts) return;
   std::uint64_t same = __ballot(mine == expert);
   if (__builtin_ctzll(same) != slot) return;
-  const std::size_t at0 = (static_cast<std::size_t>(expert) * p.tiles + tile) * p.steps;
+  const std::size_t tile0 = static_cast<std::size_t>(expert) * p.tiles;
+  const std::size_t at0 = (tile0 + pair * 2) * p.steps, at1 = (tile0 + min(pair * 2 + 1, p.tiles - 1)) * p.steps;
   const int each = (p.chunks + kWaves - 1) / kWaves;
   const int c0 = min(wave * each, p.chunks), c1 = min(c0 + each, p.chunks);
   const WaveLds w{lds + wave * (p.rows * kRowBytes + 64), reinterpret_cast<float*>(lds + wave * (p.rows * kRowBytes + 64) + p.rows * kRowBytes)};
@@ -166,8 +179,8 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
       if (lane == r) row_slot = at;
     }
     f32x4 acc[kMats] = {};
-    const auto take = [&](auto pairs, auto depth) {
-      constexpr int kPairs = decltype(pairs)::value, kDepth = decltype(depth)::value;
+    const auto take = [&](auto count) {
+      constexpr int kRows = decltype(count)::value, kPairs = (kRows + 1) / 2, kDepth = 2;
       const float* at[kPairs];
       float times[kPairs];
       bool live[kPairs];
@@ -182,15 +195,19 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
       Weights<TYPE> ring[kDepth][kMats][2];
       Rows<kPairs, QUADS> x[kDepth];
       const auto ask = [&](int i, int c) {
-#pragma unroll
-        for (int j = 0; j < kPairs; ++j) x[i].load(j, at[j], c, p.in, lane);
         // The last chunk may have one step only: taken twice, with x 0 behind its end.
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const std::size_t at = at0 + min(2 * c + t, p.steps - 1);
-          ring[i][0][t].load(p.m, at, lane_at);
-          if constexpr (GATED) ring[i][1][t].load(p.up, at, lane_at);
+          const int step = min(2 * c + t, p.steps - 1);
+          ring[i][0][t].load(p.m, at0 + step, lane_at);
+          ring[i][1][t].load(p.m, at1 + step, lane_at);
+          if constexpr (GATED) {
+            ring[i][2][t].load(p.up, at0 + step, lane_at);
+            ring[i][3][t].load(p.up, at1 + step, lane_at);
+          }
         }
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) x[i].load(j, at[j], c, p.in, lane);
       };
 #pragma unroll
       for (int i = 0; i < kDepth; ++i)
@@ -201,13 +218,14 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
           if (c + i >= c1) break;
           x[i].store(w, times, live, c + i, p.in, lane);
           wave_sync();
-          add_chunk<TYPE, kMats>(acc, ring[i], w, 2 * kPairs - 1, lane);
+          add_chunk<TYPE, kMats, kRows>(acc, ring[i], w, lane);
           wave_sync();
           if (c + i + kDepth < c1) ask(i, c + i + kDepth);
         }
     };
-    if (!MORE || rows <= 2) take(std::integral_constant<int, 1>{}, std::integral_constant<int, GATED ? 2 : 4>{});
-    else if constexpr (MORE) take(std::integral_constant<int, kMostRows / 2>{}, std::integral_constant<int, 2>{});
+    if (rows == 1) take(std::integral_constant<int, 1>{});
+    else if (!MORE || rows == 2) take(std::integral_constant<int, 2>{});
+    else if constexpr (MORE) take(std::integral_constant<int, kMostRows>{});
 
     // The wavefronts' sums meet, in their order.
     __syncthreads();
@@ -216,16 +234,33 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) meet[((wave * kMats + m) * kTile + lane / kTile * 4 + r) * kTile + lane % kTile] = acc[m][r];
     __syncthreads();
-    const int row = threadIdx.x / kTile, o = tile * kTile + threadIdx.x % kTile;
-    // The slot of output row `row`: threads of one wavefront hold 4 rows.
+    // 32 threads a row, their outputs side by side.
+    const int row = threadIdx.x / 32, col = threadIdx.x % 32, o = pair * 32 + col;
     const int to = __shfl(row_slot, min(row, rows - 1), 64);
-    if (row < rows && o < p.out) {
-      float v[kMats] = {};
+    if (row < rows) {
+      float v[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < kWaves; ++i)
 #pragma unroll
-        for (int m = 0; m < kMats; ++m) v[m] += meet[(i * kMats + m) * kTile * kTile + threadIdx.x];
-      p.y[static_cast<std::size_t>(to) * p.y_stride + o] = GATED ? silu(v[0]) * v[kMats - 1] : v[0];
+        for (int m = 0; m < kMats / 2; ++m) v[m] += meet[((i * kMats + 2 * m + col / kTile) * kTile + row) * kTile + col % kTile];
+      if constexpr (GATED) {
+        const float h = o < p.out ? silu(v[0]) * v[1] : 0.0f;
+        const Factor f(max_of_half(finite_bits(h)));
+        _Float16 high, low;
+        two_parts(h * f.up, high, low);
+        const std::size_t block = static_cast<std::size_t>(to) * p.h.blocks + pair;
+        p.h.values[block * 64 + col] = high;
+        p.h.values[block * 64 + 32 + col] = low;
+        if (col == 0) p.h.factors[block] = f.back;
+        // Blocks up to a whole chunk, which the second product reads, are 0.
+        if (pair == p.pairs - 1)
+          for (std::size_t i = 1; pair + i < static_cast<std::size_t>(p.h.blocks); ++i) {
+            reinterpret_cast<std::uint32_t*>(p.h.values)[(block + i) * 32 + col] = 0;
+            if (col == 0) p.h.factors[block + i] = 0.0f;
+          }
+      } else if (o < p.out) {
+        p.y[static_cast<std::size_t>(to) * p.y_stride + o] = v[0];
+      }
     }
     __syncthreads();
   }
@@ -238,10 +273,11 @@ constexpr int kSumWaves = 16, kSumThreads = kSumWaves * 64;
 struct SumArgs {
   Matrices m;
   const std::int32_t* ids;
-  const float *weights, *h, *residual;
+  const float *weights, *residual;
+  FewParts h;
   float* y;  // or partial sums [split][token][out], without the residual
   std::size_t r_stride, y_stride, split_stride;
-  int tokens, top_k, experts, out, in, tiles, steps, chunks, rows, splits;
+  int tokens, top_k, experts, out, tiles, steps, chunks, splits;
 };
 
 // One workgroup a tile of 16 outputs (or, where the tiles are too few for the
@@ -249,9 +285,10 @@ struct SumArgs {
 // share the chunks of all chosen experts.  Row m of a product is token m, with
 // the weight that it gives the expert (0 where it has not chosen it), so the
 // sums over inputs and over experts are one.
-template <int TYPE, int PAIRS, bool QUADS>
+template <int TYPE, int ROWS>
 __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
   extern __shared__ __attribute__((aligned(16))) std::uint8_t lds[];
+  constexpr int PAIRS = (ROWS + 1) / 2, kRows = 2 * PAIRS, kR = ROWS < 4 ? ROWS : 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles, slots = p.tokens * p.top_k;
   const std::int32_t mine = lane < slots ? p.ids[lane] : -1;
@@ -266,57 +303,71 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
   const int units = __builtin_popcountll(firsts) * p.chunks, sharers = p.splits * kSumWaves;
   const int each = (units + sharers - 1) / sharers;
   const int u0 = min((split * kSumWaves + wave) * each, units), u1 = min(u0 + each, units);
-  const WaveLds w{lds + wave * (p.rows * kRowBytes + 64), reinterpret_cast<float*>(lds + wave * (p.rows * kRowBytes + 64) + p.rows * kRowBytes)};
+  // This wavefront's rows of a chunk, and their factors [block][kMostRows].
+  std::uint8_t* const rows_at = lds + wave * (kRows * kRowBytes + kFactorBytes);
+  float* const factors_at = reinterpret_cast<float*>(rows_at + kRows * kRowBytes);
   float* const meet = reinterpret_cast<float*>(lds);
   LaneAt lane_at(lane);
-  constexpr int kDepth = PAIRS == 1 ? 4 : 2;
-  for (int t0 = 0; t0 < p.tokens; t0 += 2 * PAIRS) {
-    f32x4 acc[1] = {};
-    Weights<TYPE> ring[kDepth][1][2];
-    Rows<PAIRS, QUADS> x[kDepth];
-    float times[kDepth][PAIRS];
+  constexpr int kDepth = PAIRS > 1 ? 2 : TYPE == LLMI_TYPE_Q4_0 ? 4 : 3;
+  for (int t0 = 0; t0 < p.tokens; t0 += kRows) {
+    f32x4 acc = {};
+    Weights<TYPE> ring[kDepth][2];
+    u32x4 x[kDepth][PAIRS];
+    float factor[kDepth], times[kDepth];
     bool live[kDepth][PAIRS];
-    int at[kDepth];
     // The unit that is asked for next: its number and chunk, its expert (the
-    // lowest bit that is left) and this lane's rows of it.
+    // lowest bit that is left) and this lane's rows of it: for the values row
+    // 2 j + lane / 32 of pair j, 16 bytes of each chunk's 512; for the factors
+    // row lane / 4, one of a chunk's four.
     std::uint64_t left = firsts;
     for (int i = u0 / p.chunks; i > 0 && left != 0; --i) left &= left - 1;
     int next = u0, chunk = u0 % p.chunks;
     std::size_t w_at = 0;
-    const float* row[PAIRS];
-    float row_times[PAIRS];
+    const _Float16* row[PAIRS];
+    const float* factor_row = nullptr;
+    float row_times = 0.0f;
     bool row_live[PAIRS];
     const auto enter = [&] {
       const int s = __builtin_ctzll(left), e = __builtin_amdgcn_readlane(mine, s);
       const std::uint64_t same = __ballot(mine == e);
       w_at = (static_cast<std::size_t>(e) * p.tiles + tile) * p.steps;
+      // The token's slots of this expert, as bits from its first slot on.
+      const auto chosen = [&](int t) {
+        const std::uint64_t bits = same >> (t * p.top_k);
+        return p.top_k < 64 ? bits & ((std::uint64_t{1} << p.top_k) - 1) : bits;
+      };
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) {
         const int t = min(t0 + 2 * j + lane / 32, p.tokens - 1);
-        std::uint64_t bits = same >> (t * p.top_k);
-        if (p.top_k < 64) bits &= (std::uint64_t{1} << p.top_k) - 1;
+        const std::uint64_t bits = chosen(t);
         row_live[j] = bits != 0;
         const int slot = bits != 0 ? t * p.top_k + __builtin_ctzll(bits) : s;
-        row[j] = p.h + static_cast<std::size_t>(slot) * p.in;
-        row_times[j] = 0.0f;
-        while (__any(bits != 0)) {  // an expert chosen twice counts with both weights
-          const float one = __shfl(weight, bits != 0 ? t * p.top_k + __builtin_ctzll(bits) : 0, 64);
-          if (bits != 0) row_times[j] += one;
-          bits &= bits - 1;
-        }
+        row[j] = p.h.values + (static_cast<std::size_t>(slot) * p.h.blocks + chunk * 4) * 64 + lane % 32 * 8;
+      }
+      const int t = min(t0 + min(lane / 4, kRows - 1), p.tokens - 1);
+      std::uint64_t bits = chosen(t);
+      const int slot = bits != 0 ? t * p.top_k + __builtin_ctzll(bits) : s;
+      factor_row = p.h.factors + static_cast<std::size_t>(slot) * p.h.blocks + chunk * 4 + lane % 4;
+      row_times = 0.0f;  // of a token that has not chosen it
+      while (__any(bits != 0)) {  // an expert chosen twice counts with both weights
+        const float one = __shfl(weight, bits != 0 ? t * p.top_k + __builtin_ctzll(bits) : 0, 64);
+        if (bits != 0) row_times += one;
+        bits &= bits - 1;
       }
     };
     if (u0 < u1) enter();
     const auto ask = [&](int i) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) ring[i][0][t].load(p.m, w_at + min(2 * chunk + t, p.steps - 1), lane_at);
+      for (int t = 0; t < 2; ++t) ring[i][t].load(p.m, w_at + min(2 * chunk + t, p.steps - 1), lane_at);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) {
-        x[i].load(j, row[j], chunk, p.in, lane);
-        times[i][j] = row_times[j];
+        x[i][j] = *reinterpret_cast<const u32x4*>(row[j]);
         live[i][j] = row_live[j];
+        row[j] += 4 * 64;
       }
-      at[i] = chunk;
+      factor[i] = *factor_row;
+      times[i] = row_times;
+      factor_row += 4;
       if (++next < u1 && ++chunk == p.chunks) {
         chunk = 0;
         left &= left - 1;
@@ -330,18 +381,29 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
 #pragma unroll
       for (int i = 0; i < kDepth; ++i) {
         if (u + i >= u1) break;
-        x[i].store(w, times[i], live[i], at[i], p.in, lane);
+        // A row that does not count is 0, whatever stands there.
+#pragma unroll
+        for (int j = 0; j < PAIRS; ++j)
+          *reinterpret_cast<u32x4*>(rows_at + (2 * j + lane / 32) * kRowBytes + lane % 32 * 16) = ROWS == 1 || live[i][j] ? x[i][j] : u32x4{0, 0, 0, 0};
+        if (lane / 4 < kRows) factors_at[lane % 4 * kMostRows + lane / 4] = factor[i] * times[i];
         wave_sync();
-        add_chunk<TYPE, 1>(acc, ring[i], w, 2 * PAIRS - 1, lane);
+        const std::uint8_t* const from = lane_row<ROWS>(rows_at, lane);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const f32x4 d = times_codes(from, b, ring[i][b / 2].codes(b % 2));
+          const f32x4 f = *reinterpret_cast<const f32x4*>(factors_at + b * kMostRows + lane / kTile % (kMostRows / 4) * 4);
+#pragma unroll
+          for (int r = 0; r < kR; ++r) acc[r] = __builtin_fmaf(d[r] * ring[i][b / 2].s[b % 2], f[r], acc[r]);
+        }
         wave_sync();
         if (next < u1) ask(i);
       }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < 4; ++r) meet[(wave * kTile + lane / kTile * 4 + r) * kTile + lane % kTile] = acc[0][r];
+    for (int r = 0; r < 4; ++r) meet[(wave * kTile + lane / kTile * 4 + r) * kTile + lane % kTile] = acc[r];
     __syncthreads();
     const int r = threadIdx.x / kTile, t = t0 + r, o = tile * kTile + threadIdx.x % kTile;
-    if (r < 2 * PAIRS && t < p.tokens && o < p.out) {
+    if (r < kRows && t < p.tokens && o < p.out) {
       float v = 0.0f;
 #pragma unroll
       for (int i = 0; i < kSumWaves; ++i) v += meet[i * kTile * kTile + threadIdx.x];
@@ -375,8 +437,9 @@ void with_flags(Fn&& fn, bool flag, More... more) {
   else with_flags([&](auto... rest) { fn(std::false_type{}, rest...); }, more...);
 }
 
-std::size_t lds_bytes(int waves, int rows, int mats) {
-  return std::max<std::size_t>(static_cast<std::size_t>(waves) * (rows * kRowBytes + 64),
+// LDS of a workgroup: its wavefronts' rows, then their sums of MATS tiles.
+std::size_t lds_bytes(int waves, int rows, int extra, int mats) {
+  return std::max<std::size_t>(static_cast<std::size_t>(waves) * (rows * kRowBytes + extra),
                                static_cast<std::size_t>(waves) * mats * kTile * kTile * sizeof(float));
 }
 
@@ -387,12 +450,13 @@ int launch_few(const FewProduct& f, hipStream_t s) {
   // An expert has more than two rows only where x has, or where ids repeat.
   const bool more = ceil_div(f.slots, f.per_row) > 2;
   const int rows = more ? kMostRows : 2;
-  const FewArgs a{f.m, f.up, f.ids, f.x, f.y, f.x_stride, f.y_stride, static_cast<int>(f.slots), static_cast<int>(f.per_row),
+  const std::size_t pairs = ceil_div(sh.tiles(), 2);
+  const FewArgs a{f.m, f.up, f.ids, f.x, f.y, f.h, f.x_stride, f.y_stride, static_cast<int>(f.slots), static_cast<int>(f.per_row),
                   static_cast<int>(sh.count), static_cast<int>(sh.out), static_cast<int>(sh.in), static_cast<int>(sh.tiles()),
-                  static_cast<int>(sh.steps()), static_cast<int>(ceil_div(sh.steps(), 2)), rows};
-  const unsigned grid = static_cast<unsigned>(f.slots * sh.tiles());
+                  static_cast<int>(pairs), static_cast<int>(sh.steps()), static_cast<int>(ceil_div(sh.steps(), 2)), rows};
+  const unsigned grid = static_cast<unsigned>(f.slots * pairs);
   with_flags([&](auto gated, auto more, auto quads) {
-    const std::size_t lds = lds_bytes(kWaves, rows, gated ? 2 : 1);
+    const std::size_t lds = lds_bytes(kWaves, rows, 64, gated ? 4 : 2);
     if (sh.type == LLMI_TYPE_Q4_0) few_kernel<LLMI_TYPE_Q4_0, gated, more, quads><<<grid, kThreads, lds, s>>>(a);
     else few_kernel<LLMI_TYPE_Q8_0, gated, more, quads><<<grid, kThreads, lds, s>>>(a);
   }, f.up.codes != nullptr, more, sh.in % 4 == 0);
@@ -402,21 +466,22 @@ int launch_few(const FewProduct& f, hipStream_t s) {
 
 int launch_few_sum(const FewSum& f, hipStream_t s) {
   const Shape& sh = f.shape;
-  const bool more = f.tokens > 2;
-  const int rows = more ? kMostRows : 2;
+  const int rows = f.tokens > 2 ? kMostRows : 2;
   const std::size_t splits = few_splits(sh);
   const bool joined = splits > 1;
-  const SumArgs a{f.m, f.ids, f.weights, f.h, joined ? nullptr : f.residual, joined ? f.parts : f.y, f.r_stride,
+  const SumArgs a{f.m, f.ids, f.weights, joined ? nullptr : f.residual, f.h, joined ? f.parts : f.y, f.r_stride,
                   joined ? sh.out : f.y_stride, f.tokens * sh.out, static_cast<int>(f.tokens), static_cast<int>(f.top_k),
-                  static_cast<int>(sh.count), static_cast<int>(sh.out), static_cast<int>(sh.in), static_cast<int>(sh.tiles()),
-                  static_cast<int>(sh.steps()), static_cast<int>(ceil_div(sh.steps(), 2)), rows, static_cast<int>(splits)};
+                  static_cast<int>(sh.count), static_cast<int>(sh.out), static_cast<int>(sh.tiles()),
+                  static_cast<int>(sh.steps()), static_cast<int>(ceil_div(sh.steps(), 2)), static_cast<int>(splits)};
   const unsigned grid = static_cast<unsigned>(sh.tiles() * splits);
-  const std::size_t lds = lds_bytes(kSumWaves, rows, 1);
-  with_flags([&](auto more, auto quads) {
-    constexpr int kPairs = more ? kMostRows / 2 : 1;
-    if (sh.type == LLMI_TYPE_Q4_0) few_sum_kernel<LLMI_TYPE_Q4_0, kPairs, quads><<<grid, kSumThreads, lds, s>>>(a);
-    else few_sum_kernel<LLMI_TYPE_Q8_0, kPairs, quads><<<grid, kSumThreads, lds, s>>>(a);
-  }, more, sh.in % 4 == 0);
+  const std::size_t lds = lds_bytes(kSumWaves, rows, kFactorBytes, 1);
+  const auto run = [&](auto count) {
+    if (sh.type == LLMI_TYPE_Q4_0) few_sum_kernel<LLMI_TYPE_Q4_0, count><<<grid, kSumThreads, lds, s>>>(a);
+    else few_sum_kernel<LLMI_TYPE_Q8_0, count><<<grid, kSumThreads, lds, s>>>(a);
+  };
+  if (f.tokens == 1) run(std::integral_constant<int, 1>{});
+  else if (f.tokens == 2) run(std::integral_constant<int, 2>{});
+  else run(std::integral_constant<int, kMostRows>{});
   LLMI_TRY_HIP(hipGetLastError());
   if (joined) {
     few_join_kernel<<<static_cast<unsigned>(ceil_div(f.tokens * sh.out, 256)), 256, 0, s>>>(

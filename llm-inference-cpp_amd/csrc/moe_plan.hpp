@@ -71,6 +71,8 @@ inline bool few_mlp(std::size_t tokens, std::size_t top_k) { return tokens * top
 // tokens, whose sums a launch of its own joins: where the tiles alone would
 // leave most of the chip idle.
 inline std::size_t few_splits(const Shape& s) { return s.tiles() >= 96 ? 1 : (128 + s.tiles() - 1) / s.tiles(); }
+// Blocks of a row between the products of few tokens: whole chunks of four.
+inline std::size_t few_blocks(const Shape& s) { return (s.blocks() + 3) / 4 * 4; }
 
 // Places in a call's workspace, each a multiple of 256 bytes.
 struct Layout {
@@ -119,15 +121,18 @@ struct MlpLayout {
   Layout all;
   Grouping group;
   Parts x, h_parts;
-  std::size_t h, sums;  // sums of each slot, or of each split
+  std::size_t h, few_factors, sums;  // sums of each slot, or of each split
   MlpLayout(const Shape& gate, const Shape& down, std::size_t tokens, std::size_t top_k) {
     const std::size_t slots = tokens * top_k;
     group.place(&all, slots, gate.count);
     x.place(&all, tokens, gate, slots, true);
-    h = all.take(slots * gate.out * sizeof(float));
+    // Of many slots fp32 rows; of few their parts and factors (whole blocks).
+    const std::size_t few = std::min(slots, kFewSlots) * few_blocks(down);
+    few_factors = few * 2 * LLMI_BLOCK_SIZE * 2;
+    h = all.take(std::max(slots * gate.out * sizeof(float), few_factors + few * sizeof(float)));
     h_parts.place(&all, slots, down, slots, false);
-    const std::size_t few = std::min(tokens, kFewTokens) * few_splits(down);
-    sums = all.take(std::max(slots, few) * down.out * sizeof(float));
+    const std::size_t split = std::min(tokens, kFewTokens) * few_splits(down);
+    sums = all.take(std::max(slots, split) * down.out * sizeof(float));
   }
 };
 
