@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const std::int32_t
 #pragma unroll
       for (int l = 0; l < 2; ++l)
         for (std::int32_t i = 0; i < own[1 + l]; ++i)
-          g.tiles[l][at[1 + l] + i] = RowTile{e, at[0] + i * g.rows[l], min(n - i * g.rows[l], g.rows[l]), 0};
+          g.tiles[l][at[1 + l] + i] = RowTile{e, at[0] + i * g.rows[l], min(n - i * g.rows[l], g.rows[l]), at[2] + i * (g.rows[0] / g.rows[1])};
     }
     __syncthreads();
   }
@@ -431,7 +431,7 @@ int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids,
   if (int rc = launch_group(ids, slots, sh.count, g, s)) return rc;
   const RowSource src{x, x_stride, sh.in, sh.steps(), per_row};
   if (int rc = split_rows(src, ceil_div(slots, per_row), nullptr, g, 0, slots, sh.count, xs, s)) return rc;
-  return launch_product(Product{sh, experts->view(), {}, xs, g, 0, slots, per_row, false, y, y_stride}, s);
+  return launch_product(Product{sh, experts->view(), {}, xs, g, 0, slots, per_row, false, y, y_stride, {}, 0, false}, s);
 }
 
 int llmi_hip_moe_mlp_bytes(const llmi_hip_experts* gate, const llmi_hip_experts* down, size_t tokens, size_t top_k,
@@ -478,9 +478,19 @@ int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* u
   if (int rc = launch_group(ids, slots, gs.count, g, s)) return rc;
   const RowSource src{x, x_stride, gs.in, gs.steps(), top_k}, h_src{h, ds.in, ds.in, ds.steps(), 0};
   if (int rc = split_rows(src, tokens, nullptr, g, 0, slots, gs.count, xs, s)) return rc;
-  if (int rc = launch_product(Product{gs, gate->view(), up->view(), xs, g, 0, slots, top_k, true, h, gs.out}, s)) return rc;
-  if (int rc = split_rows(h_src, slots, g.counts, g, 1, slots, ds.count, hs, s)) return rc;
-  if (int rc = launch_product(Product{ds, down->view(), {}, hs, g, 1, slots, 0, false, sums, ds.out}, s)) return rc;
+  // The results between the products: for short work in its row tiles at once,
+  // else as fp32 rows, whose parts need each whole row's largest.
+  const bool tiled = g.rows[1] <= static_cast<int>(kMostShortRows);
+  Product first{gs, gate->view(), up->view(), xs, g, 0, slots, top_k, true, h, gs.out, {}, 0, false};
+  if (tiled) {
+    first.y = nullptr;
+    first.h = hs;
+    first.h_steps = ds.steps();
+  }
+  if (int rc = launch_product(first, s)) return rc;
+  if (!tiled)
+    if (int rc = launch_split(h_src, slots, g.counts, hs, s)) return rc;
+  if (int rc = launch_product(Product{ds, down->view(), {}, hs, g, 1, slots, 0, false, sums, ds.out, {}, 0, tiled}, s)) return rc;
   sum_kernel<<<grid_for(tokens * ceil_div(ds.out, 4), kThreads), kThreads, 0, s>>>(
       sums, ids, weights, tokens, static_cast<int>(top_k), static_cast<int>(ds.count), static_cast<int>(ds.out), residual,
       residual_stride, y, y_stride);

@@ -19,9 +19,11 @@ struct Matrices {
   const float* scales = nullptr;
 };
 
-// A group of rows of one expert: positions first .. first + rows - 1 of the order.
+// A group of rows of one expert: positions first .. first + rows - 1 of the
+// order.  next: where the second list's groups are as large or smaller, the one
+// of this group's first row.
 struct RowTile {
-  std::int32_t expert, first, rows, pad;
+  std::int32_t expert, first, rows, next;
 };
 struct Groups {
   std::int32_t* counts;  // slots that have an expert, row tiles of both lists
@@ -72,6 +74,11 @@ struct Product {
   bool y_by_position;
   float* y;
   std::size_t y_stride;
+  // A gated pair's results in the row tiles of the second list (y NULL), each
+  // block of a row with a factor of its own: factors [tile][step][block][row].
+  SplitRows h;
+  std::size_t h_steps;
+  bool block_factors;  // x comes so
 };
 int launch_product(const Product& p, hipStream_t s);
 

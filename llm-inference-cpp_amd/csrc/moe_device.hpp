@@ -2,6 +2,8 @@
 // lane's weights of a chunk, and rows in two fp16 parts.
 #pragma once
 
+#include <type_traits>
+
 #include "moe.hpp"
 
 namespace llmi_hip::moe {
@@ -93,6 +95,13 @@ struct Weights {
   }
 };
 
+// Orders the lanes' LDS exchange of one wavefront for the compiler.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // |x| as an unsigned integer, 0 for inf and NaN: the largest finite one.
 __device__ __forceinline__ std::uint32_t finite_bits(float x) {
   const std::uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
@@ -116,6 +125,49 @@ __device__ __forceinline__ void two_parts(float a, _Float16& high, _Float16& low
   low = fabsf(a) < __builtin_inff() ? static_cast<_Float16>(a - static_cast<float>(high)) : static_cast<_Float16>(0.0f);
 }
 
-__device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
+// The largest of 16 lanes (a row of them), in all: rotations.
+__device__ __forceinline__ std::uint32_t max_of_row(std::uint32_t v) {
+  const auto ror = [](std::uint32_t x, auto by) {
+    return static_cast<std::uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x120 + decltype(by)::value, 0xF, 0xF, false));
+  };
+  v = max(v, ror(v, std::integral_constant<int, 8>{}));
+  v = max(v, ror(v, std::integral_constant<int, 4>{}));
+  v = max(v, ror(v, std::integral_constant<int, 2>{}));
+  return max(v, ror(v, std::integral_constant<int, 1>{}));
+}
+// The largest of 32 lanes: then an exchange of the two sixteens.
+__device__ __forceinline__ std::uint32_t max_of_half(std::uint32_t v) {
+  v = max_of_row(v);
+  const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return max(both[0], both[1]);
+}
+
+// The largest of lanes l, l + 16, l + 32 and l + 48.
+__device__ __forceinline__ std::uint32_t max_of_rows(std::uint32_t v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(b[0], b[1]);
+}
+
+// g / (1 + exp(-g)) to a few units of the last place, without the branches of
+// expf and of an IEEE quotient (they were a seventh of the vector work of a
+// prompt's gated product): exp(-g) = 2^t with t = -g log2(e) in two parts, the
+// hardware's 2^t and reciprocal (1 unit each), the reciprocal refined once.
+// Beyond +-150 the exponential is inf or 0 either way; NaN stays one.
+__device__ __forceinline__ float silu(float g) {
+  const float c = fminf(fmaxf(g, -150.0f), 150.0f);
+  constexpr float kLog2e = 0x1.715476p+0f, kRest = 0x1.4ae0bep-26f, kLn2 = 0x1.62e43p-1f;
+  const float t = -c * kLog2e;
+  const float rest = __builtin_fmaf(-c, kLog2e, -t) - c * kRest;
+  float e = __builtin_amdgcn_exp2f(t);
+  e *= __builtin_fmaf(rest, kLn2, 1.0f);
+  const float d = 1.0f + e;
+  float r = __builtin_amdgcn_rcpf(d);
+  const float refined = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+  r = d < 0x1p126f ? refined : r;  // of an inf, or where the refinement's product would be one
+  return g * r;
+}
 
 }  // namespace llmi_hip::moe

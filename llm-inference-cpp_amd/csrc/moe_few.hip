@@ -19,28 +19,6 @@ constexpr int kMostRows = 8;  // rows of an expert that a wavefront takes at a t
 constexpr int kFactorBytes = 4 * kMostRows * 4;  // factors of a chunk's blocks
 constexpr int kRowBytes = kChunk * 4 + 16;  // a row of a chunk in LDS, both parts; 16 bytes keep rows off each other's banks
 
-// Orders the lanes' LDS exchange of one wavefront for the compiler.
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_sched_barrier(0);
-}
-
-// The largest of 32 lanes, in all of them: rotations within 16 lanes, then an
-// exchange of the two sixteens.
-__device__ __forceinline__ std::uint32_t max_of_half(std::uint32_t v) {
-  const auto ror = [](std::uint32_t x, auto by) {
-    return static_cast<std::uint32_t>(
-        __builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x120 + decltype(by)::value, 0xF, 0xF, false));
-  };
-  v = max(v, ror(v, std::integral_constant<int, 8>{}));
-  v = max(v, ror(v, std::integral_constant<int, 4>{}));
-  v = max(v, ror(v, std::integral_constant<int, 2>{}));
-  v = max(v, ror(v, std::integral_constant<int, 1>{}));
-  const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  return max(both[0], both[1]);
-}
-
 // A wavefront's part of LDS: 2 or kMostRows rows of a chunk in two parts, and what
 // each row's sum is multiplied by.
 struct WaveLds {

@@ -97,15 +97,16 @@ struct Grouping {
 // `rows` rows as they are for the kernel for long work, or row tiles for the
 // one for short, whichever is more over all calls of at most so many slots,
 // so that a workspace for a number of slots holds every smaller one.
+// An MLP's second product for short work has a factor for each block of a row.
 struct Parts {
   std::size_t values, factors;
-  void place(Layout* l, std::size_t rows, const Shape& s, std::size_t slots, bool gated) {
+  void place(Layout* l, std::size_t rows, const Shape& s, std::size_t slots, bool gated, bool block_factors = false) {
     const std::size_t small = std::min(slots, most_short(s, gated));
     const std::size_t tiled = std::max(most_tiles(small, s.count, kLeastRows) * kLeastRows,
                                        most_tiles(small, s.count, kMostShortRows) * kMostShortRows);
     const std::size_t n = std::max(rows, tiled);
     values = l->take(n * s.steps() * kStep * 4);
-    factors = l->take(n * sizeof(float));
+    factors = l->take((block_factors ? std::max(rows, tiled * s.steps() * 2) : n) * sizeof(float));
   }
 };
 struct MatmulLayout {
@@ -126,11 +127,12 @@ struct MlpLayout {
     const std::size_t slots = tokens * top_k;
     group.place(&all, slots, gate.count);
     x.place(&all, tokens, gate, slots, true);
-    // Of many slots fp32 rows; of few their parts and factors (whole blocks).
-    const std::size_t few = std::min(slots, kFewSlots) * few_blocks(down);
+    // For long work fp32 rows; of few slots their parts and factors (whole
+    // blocks); for short work row tiles (h_parts) alone.
+    const std::size_t few = std::min(slots, kFewSlots) * few_blocks(down), many = slots > most_short(down, false) ? slots : 0;
     few_factors = few * 2 * LLMI_BLOCK_SIZE * 2;
-    h = all.take(std::max(slots * gate.out * sizeof(float), few_factors + few * sizeof(float)));
-    h_parts.place(&all, slots, down, slots, false);
+    h = all.take(std::max(many * gate.out * sizeof(float), few_factors + few * sizeof(float)));
+    h_parts.place(&all, many, down, slots, false, true);
     const std::size_t split = std::min(tokens, kFewTokens) * few_splits(down);
     sums = all.take(std::max(slots, split) * down.out * sizeof(float));
   }

@@ -92,7 +92,34 @@ struct ProductArgs {
   std::size_t y_stride;
   int out, tiles, steps, per_row, y_by_position, columns;  // columns: groups of outputs that a workgroup takes
   int first, list;  // unit of the first workgroup; which tile list
+  SplitRows h;      // a gated pair's results in row tiles (values NULL: in y)
+  int h_steps, h_rows;
 };
+
+// 8 results side by side of a gated pair (outputs 8 g .. of block `block`, by
+// the lane of the row and g; rows beside each other's lanes write beside each
+// other) in the row tiles of the second product, row `row` of tile `tile`.
+// Lanes l, l + 16, l + 32, l + 48 hold a row's block and have to be active together.
+__device__ __forceinline__ void store_parts(const ProductArgs& p, int tile, int row, int block, int g, const float (&v)[8], bool live) {
+  std::uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, finite_bits(v[i]));
+  const Factor f(max_of_rows(top));
+  f16x8 high, low;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    _Float16 a, b;
+    two_parts(v[i] * f.up, a, b);
+    high[i] = a;
+    low[i] = b;
+  }
+  if (!live) return;
+  const std::size_t piece = ((static_cast<std::size_t>(tile) * p.h_steps + block / 2) * (p.h_rows / kTile) + row / kTile) * 4 + block % 2 * 2;
+  f16x8* const at = reinterpret_cast<f16x8*>(p.h.values) + piece * 64 + g * kTile + row % kTile;
+  at[0] = high;
+  at[64] = low;
+  if (g == 0) p.h.factors[(static_cast<std::size_t>(tile) * p.h_steps * 2 + block) * p.h_rows + row] = f.back;
+}
 
 // 16 bytes of each lane, OFFSET behind its own address, into LDS, lane after
 // lane from `to` (common to the wavefront).  Nothing waits for it but landed().
@@ -245,6 +272,37 @@ __global__ void __launch_bounds__(kThreads, 2) long_kernel(ProductArgs p) {
         for (int n = 0; n < NT; ++n) w[1 - j][n].here();
       }
   }
+  if constexpr (GATED) {
+    if (p.h.values != nullptr) {
+      // The wavefront's outputs of a row are one block (kCols is 2).  16 rows at
+      // a time go through its part of LDS, from a lane's rows to a lane's outputs.
+      constexpr int kStride = kCols * kTile + 4;  // 16-byte rows whose quads meet all banks
+      float* const turn = reinterpret_cast<float*>(&xs[0][0][0]) + wave * kTile * kStride;
+      const int block = col0 / kCols;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if (i * kTile >= rows) break;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = lane / kTile * 4 + r;
+          const float f = back[i * kTile + row];
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) {
+            const float v = silu(acc[n][i][r] * f) * (acc[kCols + n][i][r] * f);
+            turn[row * kStride + n * kTile + lane % kTile] = (col0 + n) * kTile + lane % kTile < p.out ? v : 0.0f;
+          }
+        }
+        wave_sync();
+        const f32x4* const at = reinterpret_cast<const f32x4*>(turn + lane % kTile * kStride + lane / kTile * 8);
+        const f32x4 a = at[0], b8 = at[1];
+        const float v[8] = {a[0], a[1], a[2], a[3], b8[0], b8[1], b8[2], b8[3]};
+        const int row = i * kTile + lane % kTile;
+        store_parts(p, rt.next + i * kTile / p.h_rows, row % p.h_rows, block, lane / kTile, v, row < rows && block < p.h_steps * 2);
+        wave_sync();
+      }
+      return;
+    }
+  }
   // Lane l holds output l % 16 of rows 4 (l / 16) .. + 3.
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
@@ -253,13 +311,23 @@ __global__ void __launch_bounds__(kThreads, 2) long_kernel(ProductArgs p) {
     for (int r = 0; r < 4; ++r) {
       const int row = i * kTile + lane / kTile * 4 + r;
       const float f = back[row];
-      float* const to = p.y + static_cast<std::size_t>(to_row[row]) * p.y_stride;
+      if constexpr (GATED) {
+        float v[kCols];
 #pragma unroll
-      for (int n = 0; n < kCols; ++n) {
-        const int o = (col0 + n) * kTile + lane % kTile;
-        float v = acc[n][i][r] * f;
-        if constexpr (GATED) v = silu(v) * (acc[kCols + n][i][r] * f);
-        if (row < rows && o < p.out) to[o] = v;
+        for (int n = 0; n < kCols; ++n) v[n] = silu(acc[n][i][r] * f) * (acc[kCols + n][i][r] * f);
+        float* const to = p.y + static_cast<std::size_t>(to_row[row]) * p.y_stride;
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
+          const int o = (col0 + n) * kTile + lane % kTile;
+          if (row < rows && o < p.out) to[o] = v[n];
+        }
+      } else {
+        float* const to = p.y + static_cast<std::size_t>(to_row[row]) * p.y_stride;
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
+          const int o = (col0 + n) * kTile + lane % kTile;
+          if (row < rows && o < p.out) to[o] = acc[n][i][r] * f;
+        }
       }
     }
   }
@@ -270,10 +338,11 @@ __global__ void __launch_bounds__(kThreads, 2) long_kernel(ProductArgs p) {
 // gated pair); its 4 wavefronts share the inputs, each with its own loads of
 // rows and weights in flight while it works on those before them, and their
 // sums meet in LDS, in their order.
-template <int TYPE, int MT, int NT, bool GATED>
+// BLOCKS: every block of a row of x has a factor of its own.
+template <int TYPE, int MT, int NT, bool GATED, bool BLOCKS>
 __global__ void __launch_bounds__(kThreads) short_kernel(ProductArgs p) {
   constexpr int kCols = GATED ? NT / 2 : NT;
-  __shared__ float meet[kWaves][NT][MT][kTile][kTile];
+  __shared__ __attribute__((aligned(16))) float meet[kWaves][NT][MT][kTile][kTile];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int units = p.g.counts[1 + p.list] * p.columns;
   const int per = (units + 7) / 8, b = p.first + static_cast<int>(blockIdx.x), u = b % 8 * per + b / 8;
@@ -291,7 +360,8 @@ __global__ void __launch_bounds__(kThreads) short_kernel(ProductArgs p) {
   for (int n = 0; n < kCols; ++n) at[n] = (static_cast<std::size_t>(expert) * p.tiles + min(col0 + n, p.tiles - 1)) * p.steps;
   struct Stage {
     Weights<TYPE> w[NT];
-    f16x8 x[MT][4];  // block, high / low
+    f16x8 x[MT][4];              // block, high / low
+    f32x4 f[BLOCKS ? MT : 1][2];  // factors of the lane's rows of a result
   };
   LaneAt lane_at(lane);
   const auto ask = [&](Stage& s, int h) {
@@ -306,6 +376,13 @@ __global__ void __launch_bounds__(kThreads) short_kernel(ProductArgs p) {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int f = 0; f < 4; ++f) s.x[i][f] = *(const __attribute__((address_space(1))) f16x8*)(from + (i * 4 + f) * 1024 + lane_at.by16);
+    if constexpr (BLOCKS) {
+      const float* const at_factors = p.x.factors + (static_cast<std::size_t>(tile) * p.steps + h) * (2 * MT * kTile);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int b2 = 0; b2 < 2; ++b2) s.f[i][b2] = *reinterpret_cast<const f32x4*>(at_factors + (b2 * MT + i) * kTile + lane / kTile * 4);
+    }
   };
   f32x4 acc[NT][MT] = {};
   const auto work = [&](const Stage& s) {
@@ -322,7 +399,8 @@ __global__ void __launch_bounds__(kThreads) short_kernel(ProductArgs p) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[n][i][r] = __builtin_fmaf(d[i][r], s.w[n].s[b2], acc[n][i][r]);
+          for (int r = 0; r < 4; ++r)
+            acc[n][i][r] = __builtin_fmaf(d[i][r], BLOCKS ? s.w[n].s[b2] * s.f[BLOCKS ? i : 0][b2][r] : s.w[n].s[b2], acc[n][i][r]);
       }
   };
   if (h0 < h1) {
@@ -343,6 +421,40 @@ __global__ void __launch_bounds__(kThreads) short_kernel(ProductArgs p) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) meet[wave][n][i][lane / kTile * 4 + r][lane % kTile] = acc[n][i][r];
   __syncthreads();
+  if constexpr (GATED) {
+    if (p.h.values != nullptr) {
+      // A wavefront 16 rows, a lane 8 outputs of one (the 32 of kCols 2 are a block).
+      if (wave >= MT) return;
+      const int row = wave * kTile + lane % kTile, g = lane / kTile, block = col0 / kCols;
+      float v[8], u[8] = {};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const f32x4 a = *reinterpret_cast<const f32x4*>(&meet[w][g / 2][wave][lane % kTile][g % 2 * 8 + q * 4]);
+          const f32x4 c = *reinterpret_cast<const f32x4*>(&meet[w][kCols + g / 2][wave][lane % kTile][g % 2 * 8 + q * 4]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[q * 4 + i] += a[i];
+            u[q * 4 + i] += c[i];
+          }
+        }
+      const bool live = row < rows;
+      const float f = live ? p.x.factors[tile * (MT * kTile) + row] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (col0 * kTile + g * 8 + i < p.out) ? silu(v[i] * f) * (u[i] * f) : 0.0f;
+      const int to = rt.next + wave * kTile / p.h_rows;
+      store_parts(p, to, row % p.h_rows, block, g, v, live);
+      // A last step's second block without outputs is 0.
+      if (block == p.columns - 1 && block + 1 < p.h_steps * 2) {
+        const float none[8] = {};
+        store_parts(p, to, row % p.h_rows, block + 1, g, none, live);
+      }
+      return;
+    }
+  }
   for (int t = threadIdx.x; t < min(rows, MT * kTile) * (kCols * kTile); t += kThreads) {
     const int row = t / (kCols * kTile), col = t % (kCols * kTile), o = col0 * kTile + col;
     const int n = col / kTile, i = row / kTile;
@@ -354,9 +466,12 @@ __global__ void __launch_bounds__(kThreads) short_kernel(ProductArgs p) {
       if constexpr (GATED) v[1] += meet[w][kCols + n][i][row % kTile][col % kTile];
     }
     const int pos = first + row;
-    const float f = p.x.factors[tile * (MT * kTile) + row];
-    float* const to = p.y + static_cast<std::size_t>(p.y_by_position ? pos : p.g.order[pos]) * p.y_stride;
-    to[o] = GATED ? silu(v[0] * f) * (v[1] * f) : v[0] * f;
+    if constexpr (!BLOCKS) {
+      const float f = p.x.factors[tile * (MT * kTile) + row];
+      v[0] *= f;
+      v[1] *= f;
+    }
+    p.y[static_cast<std::size_t>(p.y_by_position ? pos : p.g.order[pos]) * p.y_stride + o] = GATED ? silu(v[0]) * v[1] : v[0];
   }
 }
 
@@ -387,14 +502,21 @@ int launch_product(const Product& p, hipStream_t s) {
   const std::size_t columns = ceil_div(p.shape.tiles(), cols);
   const std::size_t all = ceil_div(most_tiles(p.slots, p.shape.count, static_cast<std::size_t>(rows)) * columns, 8) * 8;
   ProductArgs a{p.m, p.up, p.x, p.g, p.y, p.y_stride, static_cast<int>(p.shape.out), static_cast<int>(p.shape.tiles()),
-                static_cast<int>(p.shape.steps()), static_cast<int>(p.per_row), p.y_by_position, static_cast<int>(columns), 0, p.list};
+                static_cast<int>(p.shape.steps()), static_cast<int>(p.per_row), p.y_by_position, static_cast<int>(columns), 0, p.list,
+                p.h, static_cast<int>(p.h_steps), p.g.rows[1]};
   for (std::size_t first = 0; first < all; first += kMostGroups) {
     a.first = static_cast<int>(first);
     const unsigned grid = static_cast<unsigned>(std::min(all - first, kMostGroups));
     const auto run = [&](auto type, auto gate) {
       switch (rows) {
-        case 16: short_kernel<type, 1, kNT, gate><<<grid, kThreads, 0, s>>>(a); break;
-        case 32: short_kernel<type, 2, kNT, gate><<<grid, kThreads, 0, s>>>(a); break;
+        case 16:
+          if (!gate && p.block_factors) short_kernel<type, 1, kNT, false, true><<<grid, kThreads, 0, s>>>(a);
+          else short_kernel<type, 1, kNT, gate, false><<<grid, kThreads, 0, s>>>(a);
+          break;
+        case 32:
+          if (!gate && p.block_factors) short_kernel<type, 2, kNT, false, true><<<grid, kThreads, 0, s>>>(a);
+          else short_kernel<type, 2, kNT, gate, false><<<grid, kThreads, 0, s>>>(a);
+          break;
         default: long_kernel<type, 4, kNT, gate><<<grid, kThreads, 0, s>>>(a); break;
       }
     };

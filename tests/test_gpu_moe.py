@@ -117,8 +117,16 @@ def run_matmul(experts, ids, x, per_row, x_stride=None, y_stride=None, y0=None, 
     return y[:slots, :experts.out]
 
 
+def some(n, rng):
+    """All of n rows, or enough of many."""
+    return range(n) if n <= 400 else np.unique(np.concatenate([np.arange(8), n - 1 - np.arange(8), rng.integers(0, n, 150)]))
+
+
 def check_matmul(y, ids, x, per_row, values):
-    for s, e in enumerate(ids.reshape(-1)):
+    flat = ids.reshape(-1)
+    assert np.array_equal((y == GUARD).all(1), (flat < 0) | (flat >= len(values)))
+    for s in some(len(flat), np.random.default_rng(2)):
+        e = flat[s]
         if e < 0 or e >= len(values):
             assert (y[s] == GUARD).all(), s
             continue
@@ -132,6 +140,8 @@ MATMULS = [
     (H.Q4_0, 8, 1, 2, 576, 96, 2), (H.Q8_0, 8, 1, 8, 127, 64, 8), (H.Q4_0, 5, 7, 3, 129, 65, 3), (H.Q8_0, 5, 7, 3, 100, 130, 1),
     (H.Q4_0, 4, 40, 2, 256, 48, 2), (H.Q8_0, 64, 20, 8, 160, 32, 8), (H.Q4_0, 2, 100, 1, 97, 200, 1), (H.Q8_0, 2, 300, 2, 64, 33, 2),
     (H.Q4_0, 16, 130, 4, 320, 128, 4), (H.Q8_0, 13, 50, 3, 1000, 77, 3), (H.Q4_0, 300, 30, 6, 64, 16, 6),
+    # Long work: more slots than the kernel for short work takes.
+    (H.Q4_0, 8, 500, 2, 100, 4112, 2), (H.Q8_0, 8, 900, 1, 192, 4090, 1), (H.Q4_0, 2, 1300, 1, 33, 4100, 1), (H.Q8_0, 70, 1200, 3, 64, 2048, 3),
 ]
 
 
@@ -243,7 +253,7 @@ class Layer:
 
     def check(self, y, ids, weights, x, residual=None):
         top_k = ids.shape[1]
-        for t in range(len(ids)):
+        for t in some(len(ids), np.random.default_rng(3)):
             want, bound, size = np.zeros(y.shape[1]), np.zeros(y.shape[1]), np.zeros(y.shape[1])
             for e, w in zip(ids[t], weights[t].astype(np.float64)):
                 if not 0 <= e < self.gate.count:
@@ -262,6 +272,9 @@ MLPS = [
     (H.Q4_0, H.Q8_0, 8, 1, 8, 96, 50, True, 0.0), (H.Q4_0, H.Q4_0, 8, 2, 2, 576, 130, True, 0.0),
     (H.Q8_0, H.Q4_0, 4, 8, 3, 33, 77, False, 0.2), (H.Q4_0, H.Q4_0, 64, 16, 8, 128, 64, True, 0.1),
     (H.Q8_0, H.Q8_0, 3, 100, 2, 72, 160, True, 0.1), (H.Q4_0, H.Q4_0, 6, 90, 4, 100, 36, False, 0.3),
+    # Long work in the first product alone, in the second alone, in both.
+    (H.Q4_0, H.Q8_0, 8, 600, 2, 64, 2080, True, 0.1), (H.Q8_0, H.Q4_0, 4, 700, 2, 2100, 40, False, 0.0),
+    (H.Q4_0, H.Q4_0, 8, 1500, 2, 1040, 1100, True, 0.05),
 ]
 
 
