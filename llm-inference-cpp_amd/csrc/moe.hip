@@ -167,66 +167,6 @@ int new_experts(const Shape& s, std::unique_ptr<llmi_hip_experts>* to) {
   return LLMI_OK;
 }
 
-// ---------------------------------------------------------------- grouping
-
-// One workgroup counts the slots of every expert, lays the experts' ranges
-// one after the other and gives each slot a place in its range.  Which place
-// depends on the order of the counters' increments; no result does, since a
-// row's sums are the same at every place of a tile.
-constexpr int kGroupThreads = 1024;
-__global__ void __launch_bounds__(kGroupThreads) group_kernel(const std::int32_t* __restrict__ ids, int slots,
-                                                              int experts, Groups g) {
-  __shared__ std::int32_t count[kMaxExperts];
-  __shared__ std::int32_t waves[3][kGroupThreads / 64];
-  const int t = threadIdx.x, lane = t & 63;
-  for (int e = t; e < experts; e += kGroupThreads) count[e] = 0;
-  __syncthreads();
-  for (int i = t; i < slots; i += kGroupThreads) {
-    const std::int32_t e = ids[i];
-    if (e >= 0 && e < experts) atomicAdd(&count[e], 1);
-  }
-  __syncthreads();
-  // Running sums of slots and of row tiles over the experts, 1024 at a time.
-  std::int32_t base[3] = {0, 0, 0};
-  for (int e0 = 0; e0 < experts; e0 += kGroupThreads) {
-    const int e = e0 + t;
-    const std::int32_t n = e < experts ? count[e] : 0;
-    const std::int32_t own[3] = {n, (n + g.rows[0] - 1) / g.rows[0], (n + g.rows[1] - 1) / g.rows[1]};
-    std::int32_t at[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      std::int32_t a = own[i];
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const std::int32_t x = __shfl_up(a, o, 64);
-        if (lane >= o) a += x;
-      }
-      if (lane == 63) waves[i][t >> 6] = a;
-      at[i] = base[i] + a - own[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      for (int w = 0; w < kGroupThreads / 64; ++w) {
-        if (w < t >> 6) at[i] += waves[i][w];
-        base[i] += waves[i][w];
-      }
-    if (e < experts) {
-      count[e] = at[0];
-#pragma unroll
-      for (int l = 0; l < 2; ++l)
-        for (std::int32_t i = 0; i < own[1 + l]; ++i)
-          g.tiles[l][at[1 + l] + i] = RowTile{e, at[0] + i * g.rows[l], min(n - i * g.rows[l], g.rows[l]), at[2] + i * (g.rows[0] / g.rows[1])};
-    }
-    __syncthreads();
-  }
-  for (int i = t; i < slots; i += kGroupThreads) {
-    const std::int32_t e = ids[i];
-    if (e >= 0 && e < experts) g.order[atomicAdd(&count[e], 1)] = i;
-  }
-  if (t < 3) g.counts[t] = base[t];
-}
-
 // ------------------------------------------------------- a token's sum
 
 // y[t] = residual[t] + sum over j of weights[t][j] * sums[t * top_k + j], in
@@ -281,25 +221,14 @@ Groups groups_at(std::uint8_t* work, const Grouping& g, std::size_t rows0, std::
   return {reinterpret_cast<std::int32_t*>(work + g.counts),
           reinterpret_cast<std::int32_t*>(work + g.order),
           {reinterpret_cast<RowTile*>(work + g.tiles[0]), reinterpret_cast<RowTile*>(work + g.tiles[1])},
-          {static_cast<int>(rows0), static_cast<int>(rows1)}};
-}
-// Rows in the layout of the list's product.
-int split_rows(const RowSource& x, std::size_t rows, const std::int32_t* live, const Groups& g, int list, std::size_t slots,
-               std::size_t experts, const SplitRows& to, hipStream_t s) {
-  if (g.rows[list] <= static_cast<int>(kMostShortRows)) return launch_split_tiles(x, g, list, slots, experts, to, s);
-  return launch_split(x, rows, live, to, s);
+          {static_cast<int>(rows0), static_cast<int>(rows1)},
+          reinterpret_cast<std::int32_t*>(work + g.hist)};
 }
 SplitRows parts_at(std::uint8_t* work, const Parts& p) {
   return {reinterpret_cast<_Float16*>(work + p.values), reinterpret_cast<float*>(work + p.factors)};
 }
 
 }  // namespace
-
-int launch_group(const std::int32_t* ids, std::size_t slots, std::size_t experts, const Groups& g, hipStream_t s) {
-  group_kernel<<<1, kGroupThreads, 0, s>>>(ids, static_cast<int>(slots), static_cast<int>(experts), g);
-  LLMI_TRY_HIP(hipGetLastError());
-  return LLMI_OK;
-}
 
 }  // namespace llmi_hip::moe
 
@@ -428,9 +357,8 @@ int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids,
   const std::size_t rows = pick_rows(sh, slots, false);
   const Groups g = groups_at(w, l.group, rows, rows);
   const SplitRows xs = parts_at(w, l.x);
-  if (int rc = launch_group(ids, slots, sh.count, g, s)) return rc;
   const RowSource src{x, x_stride, sh.in, sh.steps(), per_row};
-  if (int rc = split_rows(src, ceil_div(slots, per_row), nullptr, g, 0, slots, sh.count, xs, s)) return rc;
+  if (int rc = launch_prepare(ids, slots, sh.count, g, src, xs, s)) return rc;
   return launch_product(Product{sh, experts->view(), {}, xs, g, 0, slots, per_row, false, y, y_stride, {}, 0, false}, s);
 }
 
@@ -475,9 +403,8 @@ int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* u
     if (int rc = launch_few(FewProduct{gs, gate->view(), up->view(), ids, slots, top_k, x, x_stride, nullptr, 0, parts}, s)) return rc;
     return launch_few_sum(FewSum{ds, down->view(), ids, weights, tokens, top_k, parts, residual, residual_stride, y, y_stride, sums}, s);
   }
-  if (int rc = launch_group(ids, slots, gs.count, g, s)) return rc;
   const RowSource src{x, x_stride, gs.in, gs.steps(), top_k}, h_src{h, ds.in, ds.in, ds.steps(), 0};
-  if (int rc = split_rows(src, tokens, nullptr, g, 0, slots, gs.count, xs, s)) return rc;
+  if (int rc = launch_prepare(ids, slots, gs.count, g, src, xs, s)) return rc;
   // The results between the products: for short work in its row tiles at once,
   // else as fp32 rows, whose parts need each whole row's largest.
   const bool tiled = g.rows[1] <= static_cast<int>(kMostShortRows);

@@ -30,8 +30,8 @@ struct Groups {
   std::int32_t* order;   // slots, those of expert 0 first
   RowTile* tiles[2];     // of rows[0] and rows[1] rows each
   int rows[2];
+  std::int32_t* hist;    // [grouping_blocks][expert], of more than kOneGroup slots
 };
-int launch_group(const std::int32_t* ids, std::size_t slots, std::size_t experts, const Groups& g, hipStream_t s);
 
 // Workgroups of a launch, which has to stay below 2^32 threads; the kernels
 // go on with further units from there.
@@ -54,11 +54,11 @@ struct RowSource {
   std::size_t stride, in, steps;
   std::size_t per_row;
 };
-// All of `rows` rows as they are (at most *live where it is given).
+// Groups the slots, and brings x into the layout that list 0's product takes.
+int launch_prepare(const std::int32_t* ids, std::size_t slots, std::size_t experts, const Groups& g, const RowSource& x,
+                   const SplitRows& to, hipStream_t s);
+// The *live rows of x (at most `rows`) as they are.
 int launch_split(const RowSource& x, std::size_t rows, const std::int32_t* live, const SplitRows& to, hipStream_t s);
-// The rows of tile list `list`.
-int launch_split_tiles(const RowSource& x, const Groups& g, int list, std::size_t slots, std::size_t experts,
-                       const SplitRows& to, hipStream_t s);
 
 // y[slot or position] = W_expert x over all row tiles of a list; with `up`,
 // silu(gate x) * (up x).  x: in row tiles where the list's have at most

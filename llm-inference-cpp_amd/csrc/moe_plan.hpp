@@ -83,12 +83,21 @@ struct Layout {
     return at;
   }
 };
+// How slots are grouped: up to kOneGroup of them by one workgroup, more by
+// grouping_blocks() of them, which count first and then place.  With up to
+// kSelfGroup slots of up to kSelfExperts experts, every workgroup that brings
+// rows into row tiles finds the grouping by itself, which spares a launch.
+constexpr std::size_t kOneGroup = 4096, kSelfGroup = 2048, kSelfExperts = 256;
+inline std::size_t grouping_blocks(std::size_t slots) { return slots <= kOneGroup ? 1 : std::min<std::size_t>((slots + 2047) / 2048, 64); }
+inline bool self_grouped(std::size_t slots, std::size_t experts) { return slots <= kSelfGroup && experts <= kSelfExperts; }
+
 // The slots in the order of their experts, and their groups of rows, for the
 // two products of an MLP.
 struct Grouping {
-  std::size_t counts, order, tiles[2];
+  std::size_t counts, order, tiles[2], hist;
   void place(Layout* l, std::size_t slots, std::size_t experts) {
     counts = l->take(3 * sizeof(std::int32_t));
+    hist = l->take(slots > kOneGroup ? 64 * experts * sizeof(std::int32_t) : 0);
     order = l->take(slots * sizeof(std::int32_t));
     for (std::size_t& t : tiles) t = l->take(most_tiles(slots, experts, kLeastRows) * 4 * sizeof(std::int32_t));
   }

@@ -1,0 +1,364 @@
+// What the experts' products of many slots need beforehand: the slots grouped
+// by expert, and their rows in two fp16 parts.
+#include "moe_device.hpp"
+
+namespace llmi_hip::moe {
+namespace {
+
+// -------------------------------------------------------------------- rows
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+
+// One row of x in two parts, by a wavefront.  The factor is taken from the
+// largest finite |x|: an inf or NaN stays one in the high part and shows in its
+// own row alone.  MT > 0: row r of the row tiles of 16 MT rows; 0: row r as it is.
+template <int MT>
+__device__ __forceinline__ void split_row(const RowSource& src, std::size_t from, int r, const SplitRows& to, int lane) {
+  constexpr int kRows = MT * kTile;
+  const int in = static_cast<int>(src.in), padded = static_cast<int>(src.steps) * kStep;
+  const float* row = src.x + from * src.stride;
+  // Up to 2048 inputs at a time, all asked for before the first is used; what a
+  // shorter row has stays in registers between the two passes.
+  constexpr int kBatch = 4;
+  float v[kBatch][8];
+  const auto load = [&](int base) {
+#pragma unroll
+    for (int c = 0; c < kBatch; ++c) {
+      const int k = base + c * 512 + lane * 8;
+      if (k + 8 <= in) {
+        const f4 a = *reinterpret_cast<const f4*>(row + k), b = *reinterpret_cast<const f4*>(row + k + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[c][i] = a[i];
+          v[c][4 + i] = b[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c][i] = k + i < in ? row[k + i] : 0.0f;
+      }
+    }
+  };
+  std::uint32_t top = 0;
+  for (int base = 0; base < in; base += kBatch * 512) {
+    load(base);
+#pragma unroll
+    for (int c = 0; c < kBatch; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, finite_bits(v[c][i]));
+  }
+  const Factor f(max_of_rows(max_of_row(top)));
+  if (lane == 0) to.factors[r] = f.back;
+  for (int base = 0; base < padded; base += kBatch * 512) {
+    if (in > kBatch * 512) load(base);
+#pragma unroll
+    for (int c = 0; c < kBatch; ++c) {
+      const int k = base + c * 512 + lane * 8;
+      if (k >= padded) continue;
+      f16x8 high, low;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        _Float16 a, b;
+        two_parts(v[c][i] * f.up, a, b);
+        high[i] = a;
+        low[i] = b;
+      }
+      if constexpr (MT > 0) {
+        const std::size_t piece = ((static_cast<std::size_t>(r / kRows) * src.steps + k / kStep) * MT + r % kRows / kTile) * 4 + k % kStep / kBlock * 2;
+        f16x8* at = reinterpret_cast<f16x8*>(to.values) + piece * 64 + k % kBlock / 8 * kTile + r % kTile;
+        at[0] = high;
+        at[64] = low;
+      } else {
+        _Float16* at = to.values + (static_cast<std::size_t>(r) * padded + k / kBlock * kBlock) * 2 + k % kBlock;
+        *reinterpret_cast<f16x8*>(at) = high;
+        *reinterpret_cast<f16x8*>(at + kBlock) = low;
+      }
+    }
+  }
+}
+__device__ __forceinline__ std::size_t row_of(const RowSource& src, int pos, int slot) {
+  return src.per_row > 0 ? static_cast<std::size_t>(slot) / src.per_row : static_cast<std::size_t>(pos);
+}
+
+// Rows as they are.
+__global__ void __launch_bounds__(kThreads) split_kernel(RowSource src, int rows, const std::int32_t* __restrict__ live,
+                                                         SplitRows to) {
+  const int most = min(*live, rows);
+  for (int r = blockIdx.x * kWaves + (threadIdx.x >> 6); r < most; r += gridDim.x * kWaves)
+    split_row<0>(src, static_cast<std::size_t>(r), r, to, threadIdx.x & 63);
+}
+
+// The rows of list 0, into row tiles.
+template <int MT>
+__global__ void __launch_bounds__(kThreads) split_tiles_kernel(RowSource src, Groups g, SplitRows to) {
+  constexpr int kRows = MT * kTile;
+  const int most = g.counts[1] * kRows;
+  for (int r = blockIdx.x * kWaves + (threadIdx.x >> 6); r < most; r += gridDim.x * kWaves) {
+    const RowTile t = g.tiles[0][r / kRows];
+    if (r % kRows >= t.rows) continue;  // nothing reads its results
+    const int pos = t.first + r % kRows;
+    split_row<MT>(src, row_of(src, pos, g.order[pos]), r, to, threadIdx.x & 63);
+  }
+}
+
+// ---------------------------------------------------------------- grouping
+
+constexpr int kGroupThreads = 1024;
+
+// Running sums over the experts: count[e] becomes the place of e's first slot;
+// tile(list, index, RowTile) gets every group of rows, by the thread of its
+// expert; the totals (slots, groups of both lists) come back in all threads.
+// SMALL: all three fit into one word (at most kSelfGroup slots).
+template <int THREADS, bool SMALL, typename Fn>
+__device__ __forceinline__ void lay_ranges(std::int32_t* count, int experts, const Groups& g, std::int32_t (&total)[3], Fn&& tile) {
+  constexpr int kWords = SMALL ? 1 : 3, kAt1 = 12, kAt2 = 22;  // bits of a small word: slots, groups of either list
+  static_assert(!SMALL || (kSelfGroup < (1 << kAt1) && kSelfGroup / kLeastRows + kSelfExperts < (1 << (kAt2 - kAt1))));
+  __shared__ std::uint32_t waves[kWords][THREADS / 64];
+  const int t = threadIdx.x, lane = t & 63;
+  total[0] = total[1] = total[2] = 0;
+  for (int e0 = 0; e0 < experts; e0 += THREADS) {
+    const int e = e0 + t;
+    const std::int32_t n = e < experts ? count[e] : 0;
+    const std::int32_t own[3] = {n, (n + g.rows[0] - 1) / g.rows[0], (n + g.rows[1] - 1) / g.rows[1]};
+    std::uint32_t word[kWords], sum[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      word[i] = SMALL ? static_cast<std::uint32_t>(own[0] | own[1] << kAt1 | own[2] << kAt2) : static_cast<std::uint32_t>(own[i]);
+      std::uint32_t a = word[i];
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const std::uint32_t x = static_cast<std::uint32_t>(__shfl_up(static_cast<int>(a), o, 64));
+        if (lane >= o) a += x;
+      }
+      if (lane == 63) waves[i][t >> 6] = a;
+      sum[i] = a - word[i];
+    }
+    __syncthreads();
+    std::uint32_t whole[kWords] = {};
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+#pragma unroll
+      for (int w = 0; w < THREADS / 64; ++w) {
+        const std::uint32_t x = waves[i][w];
+        if (w < t >> 6) sum[i] += x;
+        whole[i] += x;
+      }
+    std::int32_t at[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const auto part = [&](const std::uint32_t (&v)[kWords]) {
+        if constexpr (!SMALL) return static_cast<std::int32_t>(v[i]);
+        else return static_cast<std::int32_t>(i == 0 ? v[0] & ((1u << kAt1) - 1) : i == 1 ? v[0] >> kAt1 & ((1u << (kAt2 - kAt1)) - 1) : v[0] >> kAt2);
+      };
+      at[i] = total[i] + part(sum);
+      total[i] += part(whole);
+    }
+    if (e < experts) {
+      count[e] = at[0];
+#pragma unroll
+      for (int l = 0; l < 2; ++l)
+        for (std::int32_t i = 0; i < own[1 + l]; ++i)
+          tile(l, at[1 + l] + i,
+               RowTile{e, at[0] + i * g.rows[l], min(n - i * g.rows[l], g.rows[l]), at[2] + i * (g.rows[0] / g.rows[1])});
+    }
+    __syncthreads();
+  }
+}
+
+// All slots, by one workgroup.  Which place of its expert's range a slot gets
+// depends on the order of the counters' increments; no result does, since a
+// row's sums are the same at every place of a tile.
+__device__ void group_slots(const std::int32_t* __restrict__ ids, int slots, int experts, const Groups& g, std::int32_t* count) {
+  const int t = threadIdx.x;
+  for (int e = t; e < experts; e += kGroupThreads) count[e] = 0;
+  __syncthreads();
+  for (int i = t; i < slots; i += kGroupThreads) {
+    const std::int32_t e = ids[i];
+    if (e >= 0 && e < experts) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  std::int32_t total[3];
+  lay_ranges<kGroupThreads, false>(count, experts, g, total, [&](int l, std::int32_t at, const RowTile& r) { g.tiles[l][at] = r; });
+  for (int i = t; i < slots; i += kGroupThreads) {
+    const std::int32_t e = ids[i];
+    if (e >= 0 && e < experts) g.order[atomicAdd(&count[e], 1)] = i;
+  }
+  if (t < 3) g.counts[t] = total[t];
+}
+
+// The first launch for many slots.  Workgroups below `blocks` group (one: all
+// of it; several: each counts its part of the slots), the others bring rows as
+// they are into two parts meanwhile.
+__global__ void __launch_bounds__(kGroupThreads) prepare_kernel(const std::int32_t* __restrict__ ids, int slots, int experts,
+                                                                Groups g, int blocks, RowSource src, int rows, SplitRows to) {
+  __shared__ std::int32_t count[kMaxExperts];
+  const int t = threadIdx.x, b = blockIdx.x;
+  if (b >= blocks) {
+    const int waves = (static_cast<int>(gridDim.x) - blocks) * (kGroupThreads / 64);
+    for (int r = (b - blocks) * (kGroupThreads / 64) + (t >> 6); r < rows; r += waves)
+      split_row<0>(src, static_cast<std::size_t>(r), r, to, t & 63);
+    return;
+  }
+  if (blocks == 1) {
+    group_slots(ids, slots, experts, g, count);
+    return;
+  }
+  for (int e = t; e < experts; e += kGroupThreads) count[e] = 0;
+  __syncthreads();
+  const int each = (slots + blocks - 1) / blocks, end = min((b + 1) * each, slots);
+  for (int i = b * each + t; i < end; i += kGroupThreads) {
+    const std::int32_t e = ids[i];
+    if (e >= 0 && e < experts) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  for (int e = t; e < experts; e += kGroupThreads) g.hist[b * experts + e] = count[e];
+}
+// The second one, of several parts: every workgroup sums up the counts and
+// places its part of the slots.
+__global__ void __launch_bounds__(kGroupThreads) place_kernel(const std::int32_t* __restrict__ ids, int slots, int experts,
+                                                              Groups g, int blocks) {
+  __shared__ std::int32_t count[kMaxExperts];
+  const int t = threadIdx.x, b = blockIdx.x;
+  for (int e = t; e < experts; e += kGroupThreads) {
+    std::int32_t n = 0;
+    for (int i = 0; i < blocks; ++i) n += g.hist[i * experts + e];
+    count[e] = n;
+  }
+  __syncthreads();
+  std::int32_t total[3];
+  lay_ranges<kGroupThreads, false>(count, experts, g, total, [&](int l, std::int32_t at, const RowTile& r) {
+    if (r.expert % blocks == b) g.tiles[l][at] = r;
+  });
+  for (int e = t; e < experts; e += kGroupThreads) {
+    std::int32_t n = 0;
+    for (int i = 0; i < b; ++i) n += g.hist[i * experts + e];
+    count[e] += n;
+  }
+  __syncthreads();
+  const int each = (slots + blocks - 1) / blocks, end = min((b + 1) * each, slots);
+  for (int i = b * each + t; i < end; i += kGroupThreads) {
+    const std::int32_t e = ids[i];
+    if (e >= 0 && e < experts) g.order[atomicAdd(&count[e], 1)] = i;
+  }
+  if (b == 0 && t < 3) g.counts[t] = total[t];
+}
+
+// Up to kSelfGroup slots: every workgroup finds the grouping for itself (the
+// same one: slots keep their order) and brings its share of the rows into row
+// tiles; the first one also stores it for the products.
+template <int MT>
+__global__ void __launch_bounds__(kThreads) self_kernel(const std::int32_t* __restrict__ ids, int slots, int experts, Groups g,
+                                                        RowSource src, SplitRows to) {
+  constexpr int kRows = MT * kTile, kChunks = static_cast<int>(kSelfGroup) / 64;
+  __shared__ std::int32_t count[kSelfExperts];
+  __shared__ std::uint16_t before[kChunks][kSelfExperts];  // slots of an expert in 64 of the slots, then in all before them
+  __shared__ std::uint16_t order[kSelfGroup];
+  __shared__ RowTile tiles[kSelfGroup / kRows + kSelfExperts];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, chunks = (slots + 63) / 64;
+  for (int i = t; i < chunks * static_cast<int>(kSelfExperts) / 2; i += kThreads) reinterpret_cast<std::uint32_t*>(&before[0][0])[i] = 0;
+  __syncthreads();
+  // The lanes with this lane's expert: one ballot a bit of its number.
+  const auto expert_of = [&](int c) {
+    const int i = c * 64 + lane;
+    const std::int32_t e = i < slots ? ids[i] : -1;
+    return e >= 0 && e < experts ? e : -1;
+  };
+  const auto same_lanes = [&](std::int32_t e) {
+    std::uint64_t same = __ballot(e >= 0);
+#pragma unroll
+    for (int bit = 1; bit < static_cast<int>(kSelfExperts); bit <<= 1) {
+      const std::uint64_t set = __ballot((e & bit) != 0);
+      same &= (e & bit) != 0 ? set : ~set;
+    }
+    return same;
+  };
+  const std::uint64_t below = (std::uint64_t{1} << lane) - 1;
+  std::int32_t mine[kChunks / kWaves], rank[kChunks / kWaves];
+#pragma unroll
+  for (int i = 0; i < kChunks / kWaves; ++i) mine[i] = expert_of(wave + i * kWaves);
+#pragma unroll
+  for (int i = 0; i < kChunks / kWaves; ++i) {
+    const int c = wave + i * kWaves;
+    if (c >= chunks) break;
+    const std::uint64_t same = same_lanes(mine[i]);
+    rank[i] = __builtin_popcountll(same & below);
+    if (mine[i] >= 0 && rank[i] == 0) before[c][mine[i]] = static_cast<std::uint16_t>(__builtin_popcountll(same));
+  }
+  __syncthreads();
+  for (int e = t; e < experts; e += kThreads) {
+    std::uint32_t n = 0;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      if (c >= chunks) break;
+      const std::uint32_t own = before[c][e];
+      before[c][e] = static_cast<std::uint16_t>(n);
+      n += own;
+    }
+    count[e] = static_cast<std::int32_t>(n);
+  }
+  __syncthreads();
+  std::int32_t total[3];
+  const bool store = blockIdx.x == 0;
+  lay_ranges<kThreads, true>(count, experts, g, total, [&](int l, std::int32_t at, const RowTile& r) {
+    if (l == 0) tiles[at] = r;
+    if (store) g.tiles[l][at] = r;
+  });
+#pragma unroll
+  for (int i = 0; i < kChunks / kWaves; ++i) {
+    const int c = wave + i * kWaves, e = mine[i];
+    if (c >= chunks) break;
+    if (e < 0) continue;
+    const std::int32_t at = count[e] + rank[i] + before[c][e];
+    order[at] = static_cast<std::uint16_t>(c * 64 + lane);
+    if (store) g.order[at] = c * 64 + lane;
+  }
+  if (store && t < 3) g.counts[t] = total[t];
+  __syncthreads();
+  const int most = total[1] * kRows;
+  for (int r = blockIdx.x * kWaves + wave; r < most; r += gridDim.x * kWaves) {
+    const RowTile rt = tiles[r / kRows];
+    if (r % kRows >= rt.rows) continue;  // nothing reads its results
+    const int pos = rt.first + r % kRows;
+    split_row<MT>(src, row_of(src, pos, order[pos]), r, to, lane);
+  }
+}
+
+}  // namespace
+
+int launch_prepare(const std::int32_t* ids, std::size_t slots, std::size_t experts, const Groups& g, const RowSource& x,
+                   const SplitRows& to, hipStream_t s) {
+  const int n = static_cast<int>(slots), e = static_cast<int>(experts), r0 = g.rows[0];
+  const bool tiled = r0 <= static_cast<int>(kMostShortRows);
+  const std::size_t tile_rows = most_tiles(slots, experts, static_cast<std::size_t>(r0)) * static_cast<std::size_t>(r0);
+  if (tiled && self_grouped(slots, experts)) {
+    const unsigned grid = static_cast<unsigned>(std::min<std::size_t>(ceil_div(tile_rows, kWaves), 512));
+    if (r0 == 16) self_kernel<1><<<grid, kThreads, 0, s>>>(ids, n, e, g, x, to);
+    else self_kernel<2><<<grid, kThreads, 0, s>>>(ids, n, e, g, x, to);
+    LLMI_TRY_HIP(hipGetLastError());
+    return LLMI_OK;
+  }
+  const int blocks = static_cast<int>(grouping_blocks(slots));
+  const std::size_t rows = tiled ? 0 : x.per_row > 0 ? ceil_div(slots, x.per_row) : slots;
+  const unsigned grid = static_cast<unsigned>(blocks + std::min<std::size_t>(ceil_div(rows, kGroupThreads / 64), 1 << 16));
+  prepare_kernel<<<grid, kGroupThreads, 0, s>>>(ids, n, e, g, blocks, x, static_cast<int>(rows), to);
+  LLMI_TRY_HIP(hipGetLastError());
+  if (blocks > 1) {
+    place_kernel<<<static_cast<unsigned>(blocks), kGroupThreads, 0, s>>>(ids, n, e, g, blocks);
+    LLMI_TRY_HIP(hipGetLastError());
+  }
+  if (tiled) {
+    const unsigned tile_grid = static_cast<unsigned>(std::min<std::size_t>(ceil_div(tile_rows, kWaves), kMostGroups));
+    if (r0 == 16) split_tiles_kernel<1><<<tile_grid, kThreads, 0, s>>>(x, g, to);
+    else split_tiles_kernel<2><<<tile_grid, kThreads, 0, s>>>(x, g, to);
+    LLMI_TRY_HIP(hipGetLastError());
+  }
+  return LLMI_OK;
+}
+
+int launch_split(const RowSource& x, std::size_t rows, const std::int32_t* live, const SplitRows& to, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(std::min<std::size_t>(ceil_div(rows, kWaves), kMostGroups));
+  split_kernel<<<grid, kThreads, 0, s>>>(x, static_cast<int>(rows), live, to);
+  LLMI_TRY_HIP(hipGetLastError());
+  return LLMI_OK;
+}
+
+}  // namespace llmi_hip::moe

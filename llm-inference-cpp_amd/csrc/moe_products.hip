@@ -16,74 +16,6 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 
-// x in two parts: one wavefront a row.  The factor is taken from the largest
-// finite |x|: an inf or NaN stays one in the high part and shows in its own
-// row alone.  MT: in row tiles of 16 MT rows; 0: rows as they are.
-template <int MT>
-__global__ void __launch_bounds__(kThreads) split_kernel(RowSource src, int rows, const std::int32_t* __restrict__ live,
-                                                         Groups g, int list, SplitRows to) {
-  const int lane = threadIdx.x & 63;
-  const int in = static_cast<int>(src.in), padded = static_cast<int>(src.steps) * kStep;
-  constexpr int kRows = MT * kTile;
-  const int most = MT > 0 ? g.counts[1 + list] * kRows : live != nullptr ? min(*live, rows) : rows;
-  for (int r = blockIdx.x * kWaves + (threadIdx.x >> 6); r < most; r += gridDim.x * kWaves) {
-    std::size_t from = static_cast<std::size_t>(r);
-    if constexpr (MT > 0) {
-      const RowTile t = (list == 0 ? g.tiles[0] : g.tiles[1])[r / kRows];
-      if (r % kRows >= t.rows) continue;  // nothing reads its results
-      const int pos = t.first + r % kRows;
-      from = src.per_row > 0 ? static_cast<std::size_t>(g.order[pos]) / src.per_row : static_cast<std::size_t>(pos);
-    }
-    const float* row = src.x + from * src.stride;
-    const auto load8 = [&](int k, float (&v)[8]) {
-      if (k + 8 <= in) {
-        const f4 a = *reinterpret_cast<const f4*>(row + k), b = *reinterpret_cast<const f4*>(row + k + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = a[i];
-          v[4 + i] = b[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = k + i < in ? row[k + i] : 0.0f;
-      }
-    };
-    std::uint32_t top = 0;
-    for (int k = lane * 8; k < in; k += 512) {
-      float v[8];
-      load8(k, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, finite_bits(v[i]));
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = max(top, static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
-    const Factor f(top);
-    if (lane == 0) to.factors[r] = f.back;
-    for (int k = lane * 8; k < padded; k += 512) {
-      float v[8];
-      load8(k, v);
-      f16x8 high, low;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        _Float16 a, b;
-        two_parts(v[i] * f.up, a, b);
-        high[i] = a;
-        low[i] = b;
-      }
-      if constexpr (MT > 0) {
-        const std::size_t piece = ((static_cast<std::size_t>(r / kRows) * src.steps + k / kStep) * MT + r % kRows / kTile) * 4 + k % kStep / kBlock * 2;
-        f16x8* at = reinterpret_cast<f16x8*>(to.values) + piece * 64 + k % kBlock / 8 * kTile + r % kTile;
-        at[0] = high;
-        at[64] = low;
-      } else {
-        _Float16* at = to.values + (static_cast<std::size_t>(r) * padded + k / kBlock * kBlock) * 2 + k % kBlock;
-        *reinterpret_cast<f16x8*>(at) = high;
-        *reinterpret_cast<f16x8*>(at + kBlock) = low;
-      }
-    }
-  }
-}
-
 struct ProductArgs {
   Matrices m, up;
   SplitRows x;
@@ -340,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 2) long_kernel(ProductArgs p) {
 // sums meet in LDS, in their order.
 // BLOCKS: every block of a row of x has a factor of its own.
 template <int TYPE, int MT, int NT, bool GATED, bool BLOCKS>
-__global__ void __launch_bounds__(kThreads) short_kernel(ProductArgs p) {
+__global__ void __launch_bounds__(kThreads, MT == 1 ? 4 : 3) short_kernel(ProductArgs p) {
   constexpr int kCols = GATED ? NT / 2 : NT;
   __shared__ __attribute__((aligned(16))) float meet[kWaves][NT][MT][kTile][kTile];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -404,6 +336,8 @@ __global__ void __launch_bounds__(kThreads) short_kernel(ProductArgs p) {
       }
   };
   if (h0 < h1) {
+    // One step in flight behind the one that is worked on, by many wavefronts:
+    // with two, half as many fit and a kernel takes a tenth longer.
     Stage s0, s1;
     ask(s0, h0);
     for (int h = h0; h < h1; h += 2) {
@@ -476,23 +410,6 @@ __global__ void __launch_bounds__(kThreads) short_kernel(ProductArgs p) {
 }
 
 }  // namespace
-
-int launch_split(const RowSource& x, std::size_t rows, const std::int32_t* live, const SplitRows& to, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(std::min<std::size_t>(ceil_div(rows, kWaves), kMostGroups));
-  split_kernel<0><<<grid, kThreads, 0, s>>>(x, static_cast<int>(rows), live, Groups{}, 0, to);
-  LLMI_TRY_HIP(hipGetLastError());
-  return LLMI_OK;
-}
-
-int launch_split_tiles(const RowSource& x, const Groups& g, int list, std::size_t slots, std::size_t experts,
-                       const SplitRows& to, hipStream_t s) {
-  const std::size_t rows = static_cast<std::size_t>(g.rows[list]);
-  const unsigned grid = static_cast<unsigned>(std::min<std::size_t>(ceil_div(most_tiles(slots, experts, rows) * rows, kWaves), kMostGroups));
-  if (rows == 16) split_kernel<1><<<grid, kThreads, 0, s>>>(x, 0, nullptr, g, list, to);
-  else split_kernel<2><<<grid, kThreads, 0, s>>>(x, 0, nullptr, g, list, to);
-  LLMI_TRY_HIP(hipGetLastError());
-  return LLMI_OK;
-}
 
 int launch_product(const Product& p, hipStream_t s) {
   const bool gated = p.up.codes != nullptr;

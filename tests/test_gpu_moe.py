@@ -142,6 +142,9 @@ MATMULS = [
     (H.Q4_0, 16, 130, 4, 320, 128, 4), (H.Q8_0, 13, 50, 3, 1000, 77, 3), (H.Q4_0, 300, 30, 6, 64, 16, 6),
     # Long work: more slots than the kernel for short work takes.
     (H.Q4_0, 8, 500, 2, 100, 4112, 2), (H.Q8_0, 8, 900, 1, 192, 4090, 1), (H.Q4_0, 2, 1300, 1, 33, 4100, 1), (H.Q8_0, 70, 1200, 3, 64, 2048, 3),
+    # Each way of grouping: by every workgroup (above), by one, by several.
+    (H.Q4_0, 8, 1500, 2, 32, 16, 2), (H.Q8_0, 100, 2047, 1, 40, 20, 1), (H.Q8_0, 100, 2049, 1, 40, 20, 1), (H.Q4_0, 40, 4500, 2, 33, 17, 2),
+    (H.Q8_0, 4, 5000, 1, 24, 2100, 1), (H.Q4_0, 2000, 2100, 2, 32, 16, 1),
 ]
 
 
