@@ -23,70 +23,92 @@ __device__ __forceinline__ std::uint32_t rank_bits(float l) {
   const std::uint32_t b = __float_as_uint(l + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-template <typename T, typename Fn>
-__device__ __forceinline__ T across(T v, Fn&& fn) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fn(v, static_cast<T>(__shfl_xor(v, o, 64)));
-  return v;
+// A 32-bit value of all 64 lanes: rotations within 16 lanes, then exchanges of
+// sixteens and of halves.
+template <typename Fn>
+__device__ __forceinline__ std::uint32_t across(std::uint32_t v, Fn&& fn) {
+  const auto ror = [](std::uint32_t x, auto by) {
+    return static_cast<std::uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x120 + decltype(by)::value, 0xF, 0xF, false));
+  };
+  v = fn(v, ror(v, std::integral_constant<int, 8>{}));
+  v = fn(v, ror(v, std::integral_constant<int, 4>{}));
+  v = fn(v, ror(v, std::integral_constant<int, 2>{}));
+  v = fn(v, ror(v, std::integral_constant<int, 1>{}));
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = fn(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return fn(b[0], b[1]);
 }
 
 // One wavefront a token; lane l holds logits l, l + 64, ...  Every round takes
-// the largest (rank, lowest index) of all lanes, as one 64-bit maximum.
+// the largest rank of all lanes, and of the logits that have it the first: the
+// lowest place of a lane's, then the lowest lane.
 template <int N>
 __global__ void __launch_bounds__(kThreads) route_kernel(const float* __restrict__ logits, std::size_t stride,
                                                          std::size_t tokens, int experts, int top_k, int renormalise,
                                                          float scale, std::int32_t* __restrict__ ids,
                                                          float* __restrict__ weights) {
   const int lane = threadIdx.x & 63;
+  const auto larger = [](std::uint32_t a, std::uint32_t b) { return max(a, b); };
   for (std::size_t t = blockIdx.x * static_cast<std::size_t>(kWaves) + (threadIdx.x >> 6); t < tokens;
        t += static_cast<std::size_t>(gridDim.x) * kWaves) {
-    float v[N];
-    std::uint64_t key[N];
+    std::uint32_t rank[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = lane + 64 * i;
-      v[i] = e < experts ? logits[t * stride + e] : -__builtin_inff();
-      const std::uint32_t r = rank_bits(v[i]);
-      key[i] = r == 0 ? 0 : static_cast<std::uint64_t>(r) << 32 | (0xFFFFFFFFu - static_cast<std::uint32_t>(e));
-      if (r == 0) v[i] = -__builtin_inff();
+      rank[i] = e < experts ? rank_bits(logits[t * stride + e]) : 0;
     }
-    float top = v[0];
+    const auto most = [&] {
+      std::uint32_t r = rank[0];
 #pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);
-    top = across(top, [](float a, float b) { return fmaxf(a, b); });
+      for (int i = 1; i < N; ++i) r = max(r, rank[i]);
+      return across(r, larger);
+    };
+    const auto logit = [](std::uint32_t r) { return __uint_as_float(r & 0x80000000u ? r & 0x7FFFFFFFu : ~r); };
+    std::uint32_t best = most();
+    const float top = logit(best);
     // exp(l - max); equal ones (both +inf among them) give 1.
-    const auto weight = [&](float l) { return l == top ? 1.0f : expf(l - top); };
+    const auto weight = [&](std::uint32_t r) {
+      const float l = logit(r);
+      return l == top ? 1.0f : expf(l - top);
+    };
     float total = 0.0f;
     if (!renormalise) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (key[i] != 0) total += weight(v[i]);
-      total = across(total, [](float a, float b) { return a + b; });
+        if (rank[i] != 0) total += weight(rank[i]);
+      total = __uint_as_float(across(__float_as_uint(total), [](std::uint32_t a, std::uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+      }));
     }
     // Choice j is kept by lane j (top_k <= 64).
-    float mine = 0.0f;
+    std::uint32_t mine = 0;
     int id = -1;
-    for (int j = 0; j < top_k; ++j) {
-      std::uint64_t best = key[0];
+    for (int j = 0; j < top_k && best != 0; ++j) {
+      bool found = false;
 #pragma unroll
-      for (int i = 1; i < N; ++i) best = key[i] > best ? key[i] : best;
-      best = across(best, [](std::uint64_t a, std::uint64_t b) { return a > b ? a : b; });
-      if (best == 0) break;
-      const std::uint32_t e = 0xFFFFFFFFu - static_cast<std::uint32_t>(best);
-      const std::uint32_t r = static_cast<std::uint32_t>(best >> 32);
-      const float w = weight(__uint_as_float(r & 0x80000000u ? r & 0x7FFFFFFFu : ~r));
-      if (renormalise) total += w;
-      if (lane == j) {
-        mine = w;
-        id = static_cast<int>(e);
+      for (int i = 0; i < N; ++i) {
+        const std::uint64_t has = __ballot(rank[i] == best);
+        if (found || has == 0) continue;
+        found = true;
+        const int first = __builtin_ctzll(has);
+        if (lane == j) {
+          mine = best;
+          id = first + 64 * i;
+        }
+        if (lane == first) rank[i] = 0;
       }
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (key[i] == best) key[i] = 0;
+      best = most();
     }
+    const float w = id >= 0 ? weight(mine) : 0.0f;
+    if (renormalise)  // lanes hold the choices: their sum, like that of all
+      total = __uint_as_float(across(__float_as_uint(w), [](std::uint32_t a, std::uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+      }));
     if (lane < top_k) {
       ids[t * top_k + lane] = id;
-      weights[t * top_k + lane] = id >= 0 ? scale * (mine / total) : 0.0f;
+      weights[t * top_k + lane] = id >= 0 ? scale * (w / total) : 0.0f;
     }
   }
 }
@@ -351,7 +373,7 @@ int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids,
   why = check_workspace(work, work_bytes, l.all.bytes);
   LLMI_REQUIRE(why.empty(), "moe_matmul: " + why);
   hipStream_t s = pick(stream);
-  if (few_matmul(slots))
+  if (few_matmul(slots, per_row))
     return launch_few(FewProduct{sh, experts->view(), {}, ids, slots, per_row, x, x_stride, y, y_stride, {}}, s);
   auto* w = static_cast<std::uint8_t*>(work);
   const std::size_t rows = pick_rows(sh, slots, false);

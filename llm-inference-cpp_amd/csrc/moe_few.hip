@@ -444,7 +444,7 @@ int launch_few(const FewProduct& f, hipStream_t s) {
 
 int launch_few_sum(const FewSum& f, hipStream_t s) {
   const Shape& sh = f.shape;
-  const int rows = f.tokens > 2 ? kMostRows : 2;
+  const int rows = 2;
   const std::size_t splits = few_splits(sh);
   const bool joined = splits > 1;
   const SumArgs a{f.m, f.ids, f.weights, joined ? nullptr : f.residual, f.h, joined ? f.parts : f.y, f.r_stride,
@@ -458,8 +458,7 @@ int launch_few_sum(const FewSum& f, hipStream_t s) {
     else few_sum_kernel<LLMI_TYPE_Q8_0, count><<<grid, kSumThreads, lds, s>>>(a);
   };
   if (f.tokens == 1) run(std::integral_constant<int, 1>{});
-  else if (f.tokens == 2) run(std::integral_constant<int, 2>{});
-  else run(std::integral_constant<int, kMostRows>{});
+  else run(std::integral_constant<int, 2>{});
   LLMI_TRY_HIP(hipGetLastError());
   if (joined) {
     few_join_kernel<<<static_cast<unsigned>(ceil_div(f.tokens * sh.out, 256)), 256, 0, s>>>(

@@ -62,11 +62,17 @@ inline std::size_t pick_rows(const Shape& s, std::size_t slots, bool gated) {
 }
 constexpr std::size_t kLeastRows = 16, kMostShortRows = 32;
 
-// Up to this many slots (a wavefront's lanes) and tokens (rows of a matrix
-// instruction) go without a grouping.
-constexpr std::size_t kFewSlots = 64, kFewTokens = 16;
-inline bool few_matmul(std::size_t slots) { return slots <= kFewSlots; }
+// Up to this many slots (a wavefront's lanes) go without a grouping, where few
+// rows share an expert: products of up to 8 rows of x (8 rows of 2 experts of
+// 2048 x 1024: 8 us, grouped 14; 16 rows of 4 experts of 4096 x 4096: 88 and
+// 68), MLPs of up to 2 tokens (2 of 8 experts 2048 / 1024: 29 us, grouped 32;
+// 4 of them: 59 and 47).
+constexpr std::size_t kFewSlots = 64, kFewRows = 8, kFewTokens = 2;
+inline bool few_matmul(std::size_t slots, std::size_t per_row) {
+  return slots <= kFewSlots && (slots + per_row - 1) / per_row <= kFewRows;
+}
 inline bool few_mlp(std::size_t tokens, std::size_t top_k) { return tokens * top_k <= kFewSlots && tokens <= kFewTokens; }
+
 // Workgroups that share the inputs of a tile in the second product of few
 // tokens, whose sums a launch of its own joins: where the tiles alone would
 // leave most of the chip idle.

@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(kGroupThreads) place_kernel(const std::int32_t
   const int t = threadIdx.x, b = blockIdx.x;
   for (int e = t; e < experts; e += kGroupThreads) {
     std::int32_t n = 0;
+#pragma unroll 8
     for (int i = 0; i < blocks; ++i) n += g.hist[i * experts + e];
     count[e] = n;
   }
@@ -230,6 +231,7 @@ __global__ void __launch_bounds__(kGroupThreads) place_kernel(const std::int32_t
   });
   for (int e = t; e < experts; e += kGroupThreads) {
     std::int32_t n = 0;
+#pragma unroll 8
     for (int i = 0; i < b; ++i) n += g.hist[i * experts + e];
     count[e] += n;
   }
