@@ -16,7 +16,6 @@ namespace {
 
 constexpr int kChunk = 2 * kStep;  // inputs that a wavefront takes at a time
 constexpr int kMostRows = 8;  // rows of an expert that a wavefront takes at a time
-constexpr int kFactorBytes = 4 * kMostRows * 4;  // factors of a chunk's blocks
 constexpr int kRowBytes = kChunk * 4 + 16;  // a row of a chunk in LDS, both parts; 16 bytes keep rows off each other's banks
 
 // A wavefront's part of LDS: 2 or kMostRows rows of a chunk in two parts, and what
@@ -43,9 +42,7 @@ struct Rows {
       for (int i = 0; i < 4; ++i) v[p][i] = row[min(k + i, in - 1)];
     }
   }
-  // times: what a row's sum is multiplied by besides; rows without `live` count as 0.
-  __device__ __forceinline__ void store(const WaveLds& to, const float (&times)[PAIRS], const bool (&live)[PAIRS], int chunk,
-                                        int in, int lane) const {
+  __device__ __forceinline__ void store(const WaveLds& to, int chunk, int in, int lane) const {
     const int k = lane % 32 * 4, left = in - chunk * kChunk - k;
 #pragma unroll
     for (int p = 0; p < PAIRS; ++p) {
@@ -53,7 +50,7 @@ struct Rows {
       std::uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i] = live[p] && i < left ? v[p][i] : 0.0f;
+        x[i] = i < left ? v[p][i] : 0.0f;
         top = max(top, finite_bits(x[i]));
       }
       top = max_of_half(top);
@@ -70,7 +67,7 @@ struct Rows {
       std::uint8_t* at = to.rows + row * kRowBytes + k / kBlock * (4 * kBlock) + k % kBlock * 2;
       *reinterpret_cast<f16x4*>(at) = high;
       *reinterpret_cast<f16x4*>(at + 2 * kBlock) = low;
-      if (lane % 32 == 0) to.factors[row] = live[p] ? f.back * times[p] : 0.0f;
+      if (lane % 32 == 0) to.factors[row] = f.back;
     }
   }
 };
@@ -160,14 +157,10 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
     const auto take = [&](auto count) {
       constexpr int kRows = decltype(count)::value, kPairs = (kRows + 1) / 2, kDepth = 2;
       const float* at[kPairs];
-      float times[kPairs];
-      bool live[kPairs];
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
         const int r = min(2 * i + lane / 32, rows - 1);
         at[i] = p.x + static_cast<std::size_t>(__shfl(row_slot, r, 64) / p.per_row) * p.x_stride;
-        times[i] = 1.0f;
-        live[i] = true;
       }
       // Chunks in flight: the ring's places are filled kDepth chunks ahead.
       Weights<TYPE> ring[kDepth][kMats][2];
@@ -194,7 +187,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
 #pragma unroll
         for (int i = 0; i < kDepth; ++i) {
           if (c + i >= c1) break;
-          x[i].store(w, times, live, c + i, p.in, lane);
+          x[i].store(w, c + i, p.in, lane);
           wave_sync();
           add_chunk<TYPE, kMats, kRows>(acc, ring[i], w, lane);
           wave_sync();
@@ -247,6 +240,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
 // ------------------------------------ the second product and a token's sum
 
 constexpr int kSumWaves = 16, kSumThreads = kSumWaves * 64;
+constexpr int kSumRows = 4, kSumFactorBytes = 4 * kSumRows * 4;  // factors of a chunk's blocks, 16 bytes a block
 
 struct SumArgs {
   Matrices m;
@@ -259,14 +253,14 @@ struct SumArgs {
 };
 
 // One workgroup a tile of 16 outputs (or, where the tiles are too few for the
-// chip, a part of its inputs), for all tokens (up to 16): its wavefronts
-// share the chunks of all chosen experts.  Row m of a product is token m, with
-// the weight that it gives the expert (0 where it has not chosen it), so the
-// sums over inputs and over experts are one.
+// chip, a part of its inputs), for both tokens: its wavefronts share the
+// chunks of all chosen experts.  Row m of a product is token m, with the
+// weight that it gives the expert (0 where it has not chosen it), so the sums
+// over inputs and over experts are one.
 template <int TYPE, int ROWS>
 __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
+  static_assert(ROWS <= static_cast<int>(kFewTokens) && kFewTokens == 2);
   extern __shared__ __attribute__((aligned(16))) std::uint8_t lds[];
-  constexpr int PAIRS = (ROWS + 1) / 2, kRows = 2 * PAIRS, kR = ROWS < 4 ? ROWS : 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles, slots = p.tokens * p.top_k;
   const std::int32_t mine = lane < slots ? p.ids[lane] : -1;
@@ -281,114 +275,104 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
   const int units = __builtin_popcountll(firsts) * p.chunks, sharers = p.splits * kSumWaves;
   const int each = (units + sharers - 1) / sharers;
   const int u0 = min((split * kSumWaves + wave) * each, units), u1 = min(u0 + each, units);
-  // This wavefront's rows of a chunk, and their factors [block][kMostRows].
-  std::uint8_t* const rows_at = lds + wave * (kRows * kRowBytes + kFactorBytes);
-  float* const factors_at = reinterpret_cast<float*>(rows_at + kRows * kRowBytes);
+  // This wavefront's rows of a chunk, and their factors [block][kSumRows].
+  std::uint8_t* const rows_at = lds + wave * (2 * kRowBytes + kSumFactorBytes);
+  float* const factors_at = reinterpret_cast<float*>(rows_at + 2 * kRowBytes);
   float* const meet = reinterpret_cast<float*>(lds);
   LaneAt lane_at(lane);
-  constexpr int kDepth = PAIRS > 1 ? 2 : TYPE == LLMI_TYPE_Q4_0 ? 4 : 3;
-  for (int t0 = 0; t0 < p.tokens; t0 += kRows) {
-    f32x4 acc = {};
-    Weights<TYPE> ring[kDepth][2];
-    u32x4 x[kDepth][PAIRS];
-    float factor[kDepth], times[kDepth];
-    bool live[kDepth][PAIRS];
-    // The unit that is asked for next: its number and chunk, its expert (the
-    // lowest bit that is left) and this lane's rows of it: for the values row
-    // 2 j + lane / 32 of pair j, 16 bytes of each chunk's 512; for the factors
-    // row lane / 4, one of a chunk's four.
-    std::uint64_t left = firsts;
-    for (int i = u0 / p.chunks; i > 0 && left != 0; --i) left &= left - 1;
-    int next = u0, chunk = u0 % p.chunks;
-    std::size_t w_at = 0;
-    const _Float16* row[PAIRS];
-    const float* factor_row = nullptr;
-    float row_times = 0.0f;
-    bool row_live[PAIRS];
-    const auto enter = [&] {
-      const int s = __builtin_ctzll(left), e = __builtin_amdgcn_readlane(mine, s);
-      const std::uint64_t same = __ballot(mine == e);
-      w_at = (static_cast<std::size_t>(e) * p.tiles + tile) * p.steps;
-      // The token's slots of this expert, as bits from its first slot on.
-      const auto chosen = [&](int t) {
-        const std::uint64_t bits = same >> (t * p.top_k);
-        return p.top_k < 64 ? bits & ((std::uint64_t{1} << p.top_k) - 1) : bits;
-      };
-#pragma unroll
-      for (int j = 0; j < PAIRS; ++j) {
-        const int t = min(t0 + 2 * j + lane / 32, p.tokens - 1);
-        const std::uint64_t bits = chosen(t);
-        row_live[j] = bits != 0;
-        const int slot = bits != 0 ? t * p.top_k + __builtin_ctzll(bits) : s;
-        row[j] = p.h.values + (static_cast<std::size_t>(slot) * p.h.blocks + chunk * 4) * 64 + lane % 32 * 8;
-      }
-      const int t = min(t0 + min(lane / 4, kRows - 1), p.tokens - 1);
-      std::uint64_t bits = chosen(t);
-      const int slot = bits != 0 ? t * p.top_k + __builtin_ctzll(bits) : s;
-      factor_row = p.h.factors + static_cast<std::size_t>(slot) * p.h.blocks + chunk * 4 + lane % 4;
-      row_times = 0.0f;  // of a token that has not chosen it
-      while (__any(bits != 0)) {  // an expert chosen twice counts with both weights
-        const float one = __shfl(weight, bits != 0 ? t * p.top_k + __builtin_ctzll(bits) : 0, 64);
-        if (bits != 0) row_times += one;
-        bits &= bits - 1;
-      }
+  constexpr int kDepth = TYPE == LLMI_TYPE_Q4_0 ? 4 : 3;
+  f32x4 acc = {};
+  Weights<TYPE> ring[kDepth][2];
+  u32x4 x[kDepth];
+  float factor[kDepth], times[kDepth];
+  bool live[kDepth];
+  // The unit that is asked for next: its number and chunk, its expert (the
+  // lowest bit that is left) and this lane's row of it: for the values row
+  // lane / 32, 16 bytes of each chunk's 512; for the factors row lane / 4, one
+  // of a chunk's four.
+  std::uint64_t left = firsts;
+  for (int i = u0 / p.chunks; i > 0 && left != 0; --i) left &= left - 1;
+  int next = u0, chunk = u0 % p.chunks;
+  std::size_t w_at = 0;
+  const _Float16* row = nullptr;
+  const float* factor_row = nullptr;
+  float row_times = 0.0f;
+  bool row_live = false;
+  const auto enter = [&] {
+    const int s = __builtin_ctzll(left), e = __builtin_amdgcn_readlane(mine, s);
+    const std::uint64_t same = __ballot(mine == e);
+    w_at = (static_cast<std::size_t>(e) * p.tiles + tile) * p.steps;
+    // The token's slots of this expert, as bits from its first slot on.
+    const auto chosen = [&](int t) {
+      const std::uint64_t bits = same >> (t * p.top_k);
+      return p.top_k < 64 ? bits & ((std::uint64_t{1} << p.top_k) - 1) : bits;
     };
-    if (u0 < u1) enter();
-    const auto ask = [&](int i) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) ring[i][t].load(p.m, w_at + min(2 * chunk + t, p.steps - 1), lane_at);
-#pragma unroll
-      for (int j = 0; j < PAIRS; ++j) {
-        x[i][j] = *reinterpret_cast<const u32x4*>(row[j]);
-        live[i][j] = row_live[j];
-        row[j] += 4 * 64;
-      }
-      factor[i] = *factor_row;
-      times[i] = row_times;
-      factor_row += 4;
-      if (++next < u1 && ++chunk == p.chunks) {
-        chunk = 0;
-        left &= left - 1;
-        enter();
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < kDepth; ++i)
-      if (next < u1) ask(i);
-    for (int u = u0; u < u1; u += kDepth)
-#pragma unroll
-      for (int i = 0; i < kDepth; ++i) {
-        if (u + i >= u1) break;
-        // A row that does not count is 0, whatever stands there.
-#pragma unroll
-        for (int j = 0; j < PAIRS; ++j)
-          *reinterpret_cast<u32x4*>(rows_at + (2 * j + lane / 32) * kRowBytes + lane % 32 * 16) = ROWS == 1 || live[i][j] ? x[i][j] : u32x4{0, 0, 0, 0};
-        if (lane / 4 < kRows) factors_at[lane % 4 * kMostRows + lane / 4] = factor[i] * times[i];
-        wave_sync();
-        const std::uint8_t* const from = lane_row<ROWS>(rows_at, lane);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const f32x4 d = times_codes(from, b, ring[i][b / 2].codes(b % 2));
-          const f32x4 f = *reinterpret_cast<const f32x4*>(factors_at + b * kMostRows + lane / kTile % (kMostRows / 4) * 4);
-#pragma unroll
-          for (int r = 0; r < kR; ++r) acc[r] = __builtin_fmaf(d[r] * ring[i][b / 2].s[b % 2], f[r], acc[r]);
-        }
-        wave_sync();
-        if (next < u1) ask(i);
-      }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 4; ++r) meet[(wave * kTile + lane / kTile * 4 + r) * kTile + lane % kTile] = acc[r];
-    __syncthreads();
-    const int r = threadIdx.x / kTile, t = t0 + r, o = tile * kTile + threadIdx.x % kTile;
-    if (r < kRows && t < p.tokens && o < p.out) {
-      float v = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kSumWaves; ++i) v += meet[i * kTile * kTile + threadIdx.x];
-      if (p.residual != nullptr) v = p.residual[static_cast<std::size_t>(t) * p.r_stride + o] + v;
-      p.y[static_cast<std::size_t>(split) * p.split_stride + static_cast<std::size_t>(t) * p.y_stride + o] = v;
+    const auto slot_of = [&](int t, std::uint64_t bits) { return bits != 0 ? t * p.top_k + __builtin_ctzll(bits) : s; };
+    const int tv = min(lane / 32, p.tokens - 1), tf = min(min(lane / 4, 1), p.tokens - 1);
+    std::uint64_t bits = chosen(tv);
+    row_live = bits != 0;
+    row = p.h.values + (static_cast<std::size_t>(slot_of(tv, bits)) * p.h.blocks + chunk * 4) * 64 + lane % 32 * 8;
+    bits = chosen(tf);
+    factor_row = p.h.factors + static_cast<std::size_t>(slot_of(tf, bits)) * p.h.blocks + chunk * 4 + lane % 4;
+    row_times = 0.0f;  // of a token that has not chosen it
+    while (__any(bits != 0)) {  // an expert chosen twice counts with both weights
+      const float one = __shfl(weight, bits != 0 ? slot_of(tf, bits) : 0, 64);
+      if (bits != 0) row_times += one;
+      bits &= bits - 1;
     }
-    __syncthreads();
+  };
+  if (u0 < u1) enter();
+  const auto ask = [&](int i) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) ring[i][t].load(p.m, w_at + min(2 * chunk + t, p.steps - 1), lane_at);
+    x[i] = *reinterpret_cast<const u32x4*>(row);
+    live[i] = row_live;
+    row += 4 * 64;
+    factor[i] = *factor_row;
+    times[i] = row_times;
+    factor_row += 4;
+    if (++next < u1 && ++chunk == p.chunks) {
+      chunk = 0;
+      left &= left - 1;
+      enter();
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i)
+    if (next < u1) ask(i);
+  for (int u = u0; u < u1; u += kDepth)
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i) {
+      if (u + i >= u1) break;
+      // A row that does not count is 0, whatever stands there.
+      *reinterpret_cast<u32x4*>(rows_at + lane / 32 * kRowBytes + lane % 32 * 16) = ROWS == 1 || live[i] ? x[i] : u32x4{0, 0, 0, 0};
+      if (lane / 4 < 2) factors_at[lane % 4 * kSumRows + lane / 4] = factor[i] * times[i];
+      wave_sync();
+      const std::uint8_t* const from = lane_row<ROWS>(rows_at, lane);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const f32x4 d = times_codes(from, b, ring[i][b / 2].codes(b % 2));
+        const f32x4 f = *reinterpret_cast<const f32x4*>(factors_at + b * kSumRows);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) acc[r] = __builtin_fmaf(d[r] * ring[i][b / 2].s[b % 2], f[r], acc[r]);
+      }
+      wave_sync();
+      if (next < u1) ask(i);
+    }
+  // Lanes 0 .. 15 hold the rows that count.
+  __syncthreads();
+  if (lane < kTile) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) meet[(wave * ROWS + r) * kTile + lane] = acc[r];
+  }
+  __syncthreads();
+  const int t = threadIdx.x / kTile, o = tile * kTile + threadIdx.x % kTile;
+  if (t < p.tokens && o < p.out) {
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSumWaves; ++i) v += meet[(i * ROWS + t) * kTile + threadIdx.x % kTile];
+    if (p.residual != nullptr) v = p.residual[static_cast<std::size_t>(t) * p.r_stride + o] + v;
+    p.y[static_cast<std::size_t>(split) * p.split_stride + static_cast<std::size_t>(t) * p.y_stride + o] = v;
   }
 }
 
@@ -433,18 +417,21 @@ int launch_few(const FewProduct& f, hipStream_t s) {
                   static_cast<int>(sh.count), static_cast<int>(sh.out), static_cast<int>(sh.in), static_cast<int>(sh.tiles()),
                   static_cast<int>(pairs), static_cast<int>(sh.steps()), static_cast<int>(ceil_div(sh.steps(), 2)), rows};
   const unsigned grid = static_cast<unsigned>(f.slots * pairs);
-  with_flags([&](auto gated, auto more, auto quads) {
-    const std::size_t lds = lds_bytes(kWaves, rows, 64, gated ? 4 : 2);
-    if (sh.type == LLMI_TYPE_Q4_0) few_kernel<LLMI_TYPE_Q4_0, gated, more, quads><<<grid, kThreads, lds, s>>>(a);
-    else few_kernel<LLMI_TYPE_Q8_0, gated, more, quads><<<grid, kThreads, lds, s>>>(a);
-  }, f.up.codes != nullptr, more, sh.in % 4 == 0);
+  const bool gated = f.up.codes != nullptr;
+  LLMI_REQUIRE(!gated || !more, "moe: too many rows of x for a gated pair");
+  with_flags([&](auto gate, auto many, auto quads) {
+    if constexpr (!(gate && many)) {
+      const std::size_t lds = lds_bytes(kWaves, rows, 64, gate ? 4 : 2);
+      if (sh.type == LLMI_TYPE_Q4_0) few_kernel<LLMI_TYPE_Q4_0, gate, many, quads><<<grid, kThreads, lds, s>>>(a);
+      else few_kernel<LLMI_TYPE_Q8_0, gate, many, quads><<<grid, kThreads, lds, s>>>(a);
+    }
+  }, gated, more, sh.in % 4 == 0);
   LLMI_TRY_HIP(hipGetLastError());
   return LLMI_OK;
 }
 
 int launch_few_sum(const FewSum& f, hipStream_t s) {
   const Shape& sh = f.shape;
-  const int rows = 2;
   const std::size_t splits = few_splits(sh);
   const bool joined = splits > 1;
   const SumArgs a{f.m, f.ids, f.weights, joined ? nullptr : f.residual, f.h, joined ? f.parts : f.y, f.r_stride,
@@ -452,7 +439,7 @@ int launch_few_sum(const FewSum& f, hipStream_t s) {
                   static_cast<int>(sh.count), static_cast<int>(sh.out), static_cast<int>(sh.tiles()),
                   static_cast<int>(sh.steps()), static_cast<int>(ceil_div(sh.steps(), 2)), static_cast<int>(splits)};
   const unsigned grid = static_cast<unsigned>(sh.tiles() * splits);
-  const std::size_t lds = lds_bytes(kSumWaves, rows, kFactorBytes, 1);
+  constexpr std::size_t lds = kSumWaves * (2 * kRowBytes + kSumFactorBytes);  // the sums that meet in it take less
   const auto run = [&](auto count) {
     if (sh.type == LLMI_TYPE_Q4_0) few_sum_kernel<LLMI_TYPE_Q4_0, count><<<grid, kSumThreads, lds, s>>>(a);
     else few_sum_kernel<LLMI_TYPE_Q8_0, count><<<grid, kSumThreads, lds, s>>>(a);
