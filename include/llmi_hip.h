@@ -459,7 +459,7 @@ int llmi_hip_experts_free(llmi_hip_experts* experts);
  * aligned; nothing has to be cleared, and nothing is kept in it from call to
  * call.  Calls that may run at the same time (two streams, two graphs) need a
  * workspace each; graphs that run one after the other may share one.
- * LLMI_ERR_ARG: more than 2^24 slots, strides too short, a workspace too
+ * y must not overlap x.  LLMI_ERR_ARG: more than 2^24 slots, strides too short, y = x, a workspace too
  * small, NULL pointers. */
 int llmi_hip_moe_matmul_bytes(const llmi_hip_experts* experts, size_t slots, size_t per_row, size_t* bytes);
 int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids, size_t slots, size_t per_row,

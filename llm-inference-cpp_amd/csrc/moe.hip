@@ -352,7 +352,7 @@ int llmi_hip_experts_free(llmi_hip_experts* experts) {
 
 int llmi_hip_moe_matmul_bytes(const llmi_hip_experts* experts, size_t slots, size_t per_row, size_t* bytes) {
   LLMI_REQUIRE(experts != nullptr && bytes != nullptr, "moe_matmul_bytes: null pointer");
-  const std::string why = check_matmul(experts->shape, slots, per_row);
+  const std::string why = check_matmul(slots, per_row);
   LLMI_REQUIRE(why.empty(), "moe_matmul_bytes: " + why);
   *bytes = MatmulLayout(experts->shape, slots, per_row).all.bytes;
   return LLMI_OK;
@@ -364,15 +364,17 @@ int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids,
   LLMI_REQUIRE_INIT();
   LLMI_REQUIRE(experts != nullptr, "moe_matmul: null experts");
   const Shape& sh = experts->shape;
-  std::string why = check_matmul(sh, slots, per_row);
+  std::string why = check_matmul(slots, per_row);
   LLMI_REQUIRE(why.empty(), "moe_matmul: " + why);
   LLMI_REQUIRE(x_stride >= sh.in && y_stride >= sh.out, "moe_matmul: x_stride or y_stride shorter than a row");
   if (slots == 0) return LLMI_OK;
   LLMI_REQUIRE(ids != nullptr && x != nullptr && y != nullptr, "moe_matmul: null pointer");
+  LLMI_REQUIRE(x != y, "moe_matmul: y must not be x");
   const MatmulLayout l(sh, slots, per_row);
   why = check_workspace(work, work_bytes, l.all.bytes);
   LLMI_REQUIRE(why.empty(), "moe_matmul: " + why);
   hipStream_t s = pick(stream);
+  per_row = std::min(per_row, slots);  // more than all slots mean the same row; the kernels have 32 bits for it
   if (few_matmul(slots, per_row))
     return launch_few(FewProduct{sh, experts->view(), {}, ids, slots, per_row, x, x_stride, y, y_stride, {}}, s);
   auto* w = static_cast<std::uint8_t*>(work);

@@ -42,6 +42,9 @@ inline std::string check_shape(const Shape& s) {
   return {};
 }
 
+// Rows of x that slots come from, per_row of each (any number of them).
+inline std::size_t rows_of(std::size_t slots, std::size_t per_row) { return slots == 0 ? 0 : (slots - 1) / per_row + 1; }
+
 // Groups of so many rows of at most: every expert may leave one unfilled.
 inline std::size_t most_tiles(std::size_t slots, std::size_t experts, std::size_t rows) {
   return slots / rows + std::min(slots, experts);
@@ -69,7 +72,7 @@ constexpr std::size_t kLeastRows = 16, kMostShortRows = 32;
 // 4 of them: 59 and 47).
 constexpr std::size_t kFewSlots = 64, kFewRows = 8, kFewTokens = 2;
 inline bool few_matmul(std::size_t slots, std::size_t per_row) {
-  return slots <= kFewSlots && (slots + per_row - 1) / per_row <= kFewRows;
+  return slots <= kFewSlots && rows_of(slots, per_row) <= kFewRows;
 }
 inline bool few_mlp(std::size_t tokens, std::size_t top_k) { return tokens * top_k <= kFewSlots && tokens <= kFewTokens; }
 
@@ -130,7 +133,7 @@ struct MatmulLayout {
   Parts x;
   MatmulLayout(const Shape& s, std::size_t slots, std::size_t per_row) {
     group.place(&all, slots, s.count);
-    x.place(&all, (slots + per_row - 1) / per_row, s, slots, false);
+    x.place(&all, rows_of(slots, per_row), s, slots, false);
   }
 };
 struct MlpLayout {
@@ -153,10 +156,9 @@ struct MlpLayout {
   }
 };
 
-inline std::string check_matmul(const Shape& s, std::size_t slots, std::size_t per_row) {
+inline std::string check_matmul(std::size_t slots, std::size_t per_row) {
   if (per_row == 0) return "slots of a row must be at least 1";
   if (slots > kMaxSlots) return "more than 2^24 slots";
-  (void)s;
   return {};
 }
 inline std::string check_mlp(const Shape& gate, const Shape& down, std::size_t tokens, std::size_t top_k) {

@@ -36,9 +36,9 @@ int main() {
   expect(!check_shape(shape(LLMI_TYPE_Q4_0, 1, 1, kMaxInner + 1)).empty(), "too many inputs");
 
   const Shape g = shape(LLMI_TYPE_Q4_0, 8, 96, 64), d = shape(LLMI_TYPE_Q8_0, 8, 64, 96);
-  expect(check_matmul(g, 0, 1).empty() && check_matmul(g, kMaxSlots, 3).empty(), "slots taken");
-  expect(!check_matmul(g, 1, 0).empty(), "no slots a row");
-  expect(!check_matmul(g, kMaxSlots + 1, 1).empty(), "too many slots");
+  expect(check_matmul(0, 1).empty() && check_matmul(kMaxSlots, 3).empty(), "slots taken");
+  expect(!check_matmul(1, 0).empty(), "no slots a row");
+  expect(!check_matmul(kMaxSlots + 1, 1).empty(), "too many slots");
   expect(check_mlp(g, d, 5, 2).empty() && check_mlp(g, d, kMaxSlots / kMaxTopK, kMaxTopK).empty(), "tokens taken");
   expect(!check_mlp(g, g, 5, 2).empty(), "down of other inputs");
   expect(!check_mlp(g, shape(LLMI_TYPE_Q8_0, 7, 64, 96), 5, 2).empty(), "down of other experts");
@@ -51,15 +51,15 @@ int main() {
   expect(!check_route(kMaxSlots + 1, 8, 2, 8).empty(), "too many routed tokens");
 
   // Row tiles never exceed the bound: the worst spread leaves one slot over in every expert.
-  for (std::size_t rows : {16u, 32u, 64u, 128u})
-  for (std::size_t experts : {1u, 2u, 7u, 64u})
-    for (std::size_t slots = 0; slots < 700; ++slots)
-      for (std::size_t spare = 0; spare <= std::min(slots, experts); ++spare) {
-        std::size_t tiles = spare > 0 ? spare - 1 : 0;  // spare - 1 experts with one slot each, the rest in one
-        const std::size_t rest = slots - tiles;
-        tiles += (rest + rows - 1) / rows;
-        expect(tiles <= most_tiles(slots, experts, rows), "row tiles", slots, experts);
-      }
+  for (std::size_t rows : {16u, 32u, 64u})
+    for (std::size_t experts : {1u, 2u, 7u, 64u})
+      for (std::size_t slots = 0; slots < 700; ++slots)
+        for (std::size_t spare = 0; spare <= std::min(slots, experts); ++spare) {
+          std::size_t tiles = spare > 0 ? spare - 1 : 0;  // spare - 1 experts with one slot each, the rest in one
+          const std::size_t rest = slots - tiles;
+          tiles += (rest + rows - 1) / rows;
+          expect(tiles <= most_tiles(slots, experts, rows), "row tiles", slots, experts);
+        }
   // A workspace for more slots holds fewer, and the last region ends inside it.
   std::size_t before = 0;
   for (std::size_t slots = 0; slots < 300; ++slots) {
@@ -75,6 +75,50 @@ int main() {
     expect(m.sums + tokens * 3 * d.out * 4 <= m.all.bytes, "sums end", tokens);
     before = m.all.bytes;
   }
+  // Also over the sizes at which the kernels and the grouping change, and
+  // whatever such a call takes of each region is there.
+  const auto takes = [&](const Parts& x, const Shape& s, std::size_t slots, std::size_t rows, bool gated, bool blocks) {
+    const std::size_t r = pick_rows(s, slots, gated);
+    const std::size_t n = r <= kMostShortRows ? most_tiles(slots, s.count, r) * r : rows;
+    const std::size_t factors = r <= kMostShortRows && blocks ? n * s.steps() * 2 : n;
+    return x.values % 256 == 0 && x.values + n * s.steps() * kStep * 4 <= x.factors && factors * 4 <= SIZE_MAX - x.factors ? x.factors + factors * 4 : SIZE_MAX;
+  };
+  const std::size_t turns[] = {1, 2, 3, 7, 8, 9, 16, 32, 63, 64, 65, 127, 128, 129, 255, 256, 257, 383, 384, 385, 511, 512, 513, 1023, 1024, 1025, 2047, 2048,
+                               2049, 4095, 4096, 4097, 6143, 6144, 6145, 8192, 16384, 16385, 100000, 131072, 131073};
+  for (std::size_t count : {1u, 2u, 8u, 64u, 257u, 4096u})
+    for (std::size_t width : {16u, 40u, 1024u, 4100u}) {
+      const Shape a = shape(LLMI_TYPE_Q4_0, count, width, 100), b = shape(LLMI_TYPE_Q8_0, count, 48, width);
+      for (std::size_t per_row : {std::size_t{1}, std::size_t{6}, std::size_t{1} << 32, SIZE_MAX}) {
+        before = 0;
+        for (std::size_t slots : turns) {
+          const MatmulLayout m(a, slots, per_row);
+          expect(m.all.bytes >= before, "workspace shrinks", count, slots);
+          expect(rows_of(slots, per_row) >= 1 && rows_of(slots, per_row) <= slots, "rows", slots, per_row);
+          expect(m.group.tiles[1] + most_tiles(slots, count, 16) * 16 <= m.x.values, "groups end", count, slots);
+          expect(takes(m.x, a, slots, rows_of(slots, per_row), false, false) <= m.all.bytes, "rows end", count, slots);
+          before = m.all.bytes;
+        }
+      }
+      for (std::size_t top_k : {1u, 2u, 8u}) {
+        before = 0;
+        for (std::size_t tokens : turns) {
+          const MlpLayout m(a, b, tokens, top_k);
+          const std::size_t slots = tokens * top_k;
+          expect(m.all.bytes >= before, "workspace shrinks", count, tokens);
+          expect(takes(m.x, a, slots, tokens, true, false) <= m.h, "rows end", count, tokens);
+          expect(takes(m.h_parts, b, slots, slots, false, true) <= m.sums, "results end", count, tokens);
+          expect(m.sums + slots * b.out * 4 <= m.all.bytes, "sums end", count, tokens);
+          if (pick_rows(b, slots, false) > kMostShortRows) expect(m.h + slots * a.out * 4 <= m.h_parts.values, "fp32 results end", count, tokens);
+          if (few_mlp(tokens, top_k)) {
+            const std::size_t n = slots * few_blocks(b);
+            expect(m.few_factors >= n * 128 && m.h + m.few_factors + n * 4 <= m.h_parts.values, "few results end", count, tokens);
+            expect(m.sums + few_splits(b) * tokens * b.out * 4 <= m.all.bytes, "few sums end", count, tokens);
+          }
+          // The first product writes row tiles that the second list's groups have.
+          if (pick_rows(b, slots, false) <= kMostShortRows) expect(pick_rows(a, slots, true) >= pick_rows(b, slots, false), "groups of the lists", count, tokens);
+        }
+      }
+    }
   if (bad == 0) std::puts("ok");
   return bad != 0;
 }

@@ -1,6 +1,8 @@
 """A layer of experts on the GPU (llmi_hip_moe_*): router, grouped products
 and expert MLPs against tests/moe_reference.py, alone and together."""
 
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -130,7 +132,7 @@ def check_matmul(y, ids, x, per_row, values):
         if e < 0 or e >= len(values):
             assert (y[s] == GUARD).all(), s
             continue
-        want, bound = R.product(x[s // per_row], values[e])
+        want, bound = R.product(x[int(s) // per_row], values[e])
         assert np.all(np.abs(y[s] - want) <= bound), (s, e, np.abs(y[s] - want).max(), bound.min())
 
 
@@ -333,11 +335,11 @@ def test_layer_together():
         layer.check(sb.download(np.float32).reshape(tokens, hidden), ids, got, x, x * 2)
 
 
-@pytest.mark.parametrize("tokens", [1, 6, 60])
-def test_captured_and_replayed(tokens):
+@pytest.mark.parametrize("tokens,hidden,ffn", [(1, 128, 80), (6, 128, 80), (60, 128, 80), (600, 64, 2080), (2100, 48, 2080), (2100, 1100, 64)])
+def test_captured_and_replayed(tokens, hidden, ffn):
     """Two graphs that share a workspace, replayed in turn with other inputs and other choices."""
     rng = np.random.default_rng(41)
-    hidden, ffn, count, top_k = 128, 80, 8, 2
+    count, top_k = 8, 2
     layer = Layer(rng, H.Q4_0, H.Q4_0, count, hidden, ffn)
     lb, xb = H.DeviceBuffer(tokens * count * 4), H.DeviceBuffer(tokens * hidden * 4)
     ib, wb = H.DeviceBuffer(tokens * top_k * 4), H.DeviceBuffer(tokens * top_k * 4)
@@ -376,6 +378,148 @@ def test_captured_and_replayed(tokens):
         assert np.array_equal(z.view(np.uint32), zb.download(np.float32).view(np.uint32))
 
 
+@pytest.mark.parametrize("tokens,hidden,ffn,count", [(1, 64, 48, 4), (2, 64, 48, 4), (9, 64, 48, 4), (300, 64, 48, 4), (900, 64, 2080, 4)])
+def test_mlp_in_place_of_x(tokens, hidden, ffn, count):
+    """y may be x, with a residual of its own or x itself as the residual."""
+    rng = np.random.default_rng(51)
+    layer = Layer(rng, H.Q8_0, H.Q4_0, count, hidden, ffn)
+    ids = draw_ids(rng, tokens, 2, count, 0.2)
+    weights = rng.random(ids.shape).astype(np.float32)
+    x, r = rng.standard_normal((2, tokens, hidden)).astype(np.float32)
+    ib, wb, rb = dev(ids), dev(weights), dev(r)
+    work = Workspace(H.moe_mlp_bytes(layer.gate, layer.down, tokens, 2))
+    for residual in (None, r, x):
+        want = layer.run(ids, weights, x, residual)
+        xb = dev(x)
+        H.moe_mlp(layer.gate, layer.up, layer.down, ib.ptr, wb.ptr, tokens, 2, xb.ptr, xb.ptr, work.buf.ptr, work.n,
+                  residual=None if residual is None else rb.ptr if residual is r else xb.ptr)
+        H.synchronize()
+        assert np.array_equal(xb.download(np.float32).view(np.uint32).reshape(tokens, hidden), want.view(np.uint32))
+        layer.check(want, ids, weights, x, residual)
+
+
+@pytest.mark.parametrize("tokens,ffn", [(1, 96), (2, 96), (7, 96), (150, 96), (700, 2080)])
+@pytest.mark.parametrize("qtype", [H.Q4_0, H.Q8_0])
+def test_mlp_nonfinite_rows(tokens, ffn, qtype):
+    """inf and NaN of a row of x, of a weight or of the residual show in that token alone."""
+    rng = np.random.default_rng(52)
+    layer = Layer(rng, qtype, qtype, 4, 48, ffn)
+    ids = draw_ids(rng, tokens, 2, 4)
+    weights = rng.random(ids.shape).astype(np.float32) + 0.1
+    x, r = rng.standard_normal((2, tokens, 48)).astype(np.float32)
+    for t in (0, 3, tokens - 1):
+        for kind, v in ((0, INF), (0, NAN), (1, INF), (1, NAN), (2, -INF), (2, NAN)):
+            if t >= tokens:
+                continue
+            a = [x.copy(), weights.copy(), r.copy()]
+            a[kind][t, 1] = v
+            y = layer.run(ids, a[1], a[0], a[2])
+            if kind == 2:
+                assert np.isnan(y[t, 1]) if np.isnan(v) else y[t, 1] == v
+                a[2][t, 1], y[t, 1] = 0, layer.run(ids, weights, x, np.where(np.isfinite(a[2]), a[2], 0).astype(np.float32))[t, 1]
+                assert np.isfinite(y[t]).all()
+            else:
+                assert not np.isfinite(y[t]).any() if np.isnan(v) else not np.isfinite(y[t]).all()
+                y, a[0], a[1] = y.copy(), x, weights
+                y[t] = layer.run(ids, weights, x, a[2])[t]
+            if tokens < 10 or t == 0:
+                layer.check(y, ids, weights, x, a[2])
+
+
+@pytest.mark.parametrize("tokens,ffn", [(1, 96), (5, 96), (120, 96), (700, 2080)])
+def test_mlp_saturated_gates(tokens, ffn):
+    """Gates from deep below 0 to far above: silu at its ends."""
+    rng = np.random.default_rng(53)
+    layer = Layer(rng, H.Q8_0, H.Q4_0, 4, 64, ffn)
+    ids = draw_ids(rng, tokens, 2, 4)
+    weights = rng.random(ids.shape).astype(np.float32)
+    for size in (20.0, 100.0, 3e4):
+        x = (rng.standard_normal((tokens, 64)) * size).astype(np.float32)
+        layer.check(layer.run(ids, weights, x), ids, weights, x)
+
+
+def test_one_workspace_for_smaller_calls():
+    """The bytes for the most tokens hold every smaller call, whichever kernels that takes; nothing of one call is left for the next."""
+    rng = np.random.default_rng(54)
+    layer = Layer(rng, H.Q4_0, H.Q8_0, 8, 40, 2080)
+    most = 2200
+    work = Workspace(max(H.moe_mlp_bytes(layer.gate, layer.down, most, 2), H.moe_matmul_bytes(layer.gate, 2 * most, 2)))
+    for tokens in (most, 1, 700, 2, 64, 3, 300, 1000, 9):
+        ids = draw_ids(rng, tokens, 2, 8, 0.2)
+        weights = rng.random(ids.shape).astype(np.float32)
+        x = rng.standard_normal((tokens, 40)).astype(np.float32)
+        ib, wb, xb, yb, zb = dev(ids), dev(weights), dev(x), H.DeviceBuffer(tokens * 160), dev(np.full((tokens * 2, 2080), GUARD, np.float32))
+        H.moe_mlp(layer.gate, layer.up, layer.down, ib.ptr, wb.ptr, tokens, 2, xb.ptr, yb.ptr, work.buf.ptr, work.n)
+        H.moe_matmul(layer.gate, ib.ptr, tokens * 2, xb.ptr, zb.ptr, work.buf.ptr, work.n, per_row=2)
+        H.synchronize()
+        work.intact()
+        layer.check(yb.download(np.float32).reshape(tokens, 40), ids, weights, x)
+        check_matmul(zb.download(np.float32).reshape(tokens * 2, 2080), ids, x, 2, layer.vg)
+
+
+@pytest.mark.parametrize("per_row", [2**31 - 1, 2**31, 2**32, 2**32 + 1, 2**64 - 1])
+@pytest.mark.parametrize("slots,out", [(5, 40), (70, 40), (1300, 4100)])
+def test_matmul_one_row_for_all(per_row, slots, out):
+    """More slots a row than there are, beyond 32 bits too: the one row of x."""
+    rng = np.random.default_rng(55)
+    experts, values = make(rng, H.Q4_0, 2, out, 64)
+    ids = rng.integers(-1, 2, slots).astype(np.int32)
+    x = rng.standard_normal((1, 64)).astype(np.float32)
+    check_matmul(run_matmul(experts, ids, x, per_row), ids, x, per_row, values)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams of the caller's, with a workspace each: the results of each alone."""
+    create = H.load().hipStreamCreateWithFlags  # found through the library's own dependencies
+    rng = np.random.default_rng(56)
+    layer = Layer(rng, H.Q4_0, H.Q8_0, 8, 64, 2080)
+    streams, calls = [], []
+    for tokens in (700, 40, 1, 2100):
+        ids = draw_ids(rng, tokens, 2, 8, 0.1)
+        weights = rng.random(ids.shape).astype(np.float32)
+        x = rng.standard_normal((tokens, 64)).astype(np.float32)
+        want = layer.run(ids, weights, x)
+        layer.check(want, ids, weights, x)
+        work = Workspace(H.moe_mlp_bytes(layer.gate, layer.down, tokens, 2))
+        calls.append((tokens, dev(ids), dev(weights), dev(x), dev(np.zeros_like(x)), work, want))
+    for _ in range(2):
+        s = C.c_void_p()
+        assert create(C.byref(s), 1) == 0  # non-blocking
+        streams.append(s.value)
+    H.synchronize()
+    for _ in range(5):
+        for i, (tokens, ib, wb, xb, yb, work, _) in enumerate(calls):
+            H.moe_mlp(layer.gate, layer.up, layer.down, ib.ptr, wb.ptr, tokens, 2, xb.ptr, yb.ptr, work.buf.ptr, work.n, stream=streams[i % 2])
+    for s in streams:
+        assert H.load().hipStreamSynchronize(C.c_void_p(s)) == 0
+    for tokens, *_, yb, work, want in calls:
+        work.intact()
+        assert np.array_equal(yb.download(np.float32).reshape(want.shape).view(np.uint32), want.view(np.uint32))
+    for s in streams:
+        assert H.load().hipStreamDestroy(C.c_void_p(s)) == 0
+
+
+def test_route_on_a_stream_and_repeated():
+    """The router on a stream of the caller's, many tokens, twice: the same bits."""
+    create = H.load().hipStreamCreateWithFlags
+    rng = np.random.default_rng(57)
+    logits = rng.standard_normal((20000, 60)).astype(np.float32)
+    lb = dev(logits)
+    s = C.c_void_p()
+    assert create(C.byref(s), 1) == 0
+    got = []
+    for _ in range(2):
+        ib, wb = dev(np.zeros((20000, 4), np.int32)), dev(np.zeros((20000, 4), np.float32))
+        H.moe_route(lb.ptr, 20000, 60, 4, ib.ptr, wb.ptr, stream=s.value)
+        assert H.load().hipStreamSynchronize(s) == 0
+        got.append((ib.download(np.int32).reshape(-1, 4), wb.download(np.float32).reshape(-1, 4)))
+    assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1].view(np.uint32), got[1][1].view(np.uint32))
+    some_rows = np.arange(0, 20000, 97)
+    ids, w = R.route(logits[some_rows], 4, True, 1.0)
+    assert np.array_equal(got[0][0][some_rows], ids) and np.all(np.abs(got[0][1][some_rows] - w) <= w * 2.0**-24 * 80)
+    assert H.load().hipStreamDestroy(s) == 0
+
+
 # ---------------------------------------------------------------- refusals
 
 
@@ -403,14 +547,16 @@ def test_refusals():
     refused("at least 1", H.moe_matmul_bytes, gate, 4, 0)
     refused("2\\^24", H.moe_matmul_bytes, gate, 2**24 + 1)
     n = H.moe_matmul_bytes(gate, 4)
-    refused("needed", H.moe_matmul, gate, p, 4, p, p, p, n - 1)
-    refused("aligned", H.moe_matmul, gate, p, 4, p, p, p + 8, n)
-    refused("null", H.moe_matmul, gate, None, 4, p, p, p, n)
+    refused("needed", H.moe_matmul, gate, p, 4, p, p + 4096, p, n - 1)
+    refused("aligned", H.moe_matmul, gate, p, 4, p, p + 4096, p + 8, n)
+    y = p + 4096
+    refused("y must not be x", H.moe_matmul, gate, p, 4, p, p, p, n)
+    refused("null", H.moe_matmul, gate, None, 4, p, y, p, n)
     refused("null", H.moe_matmul, gate, p, 4, None, p, p, n)
     refused("null", H.moe_matmul, gate, p, 4, p, None, p, n)
-    refused("null", H.moe_matmul, gate, p, 4, p, p, None, n)
-    refused("stride", H.moe_matmul, gate, p, 4, p, p, p, n, x_stride=31)
-    refused("stride", H.moe_matmul, gate, p, 4, p, p, p, n, y_stride=7)
+    refused("null", H.moe_matmul, gate, p, 4, p, p + 4096, None, n)
+    refused("stride", H.moe_matmul, gate, p, 4, p, p + 4096, p, n, x_stride=31)
+    refused("stride", H.moe_matmul, gate, p, 4, p, p + 4096, p, n, y_stride=7)
     n = H.moe_mlp_bytes(gate, down, 2, 2)
     mlp = dict(ids=p, weights=p, tokens=2, top_k=2, x=p, y=p, work=p, work_bytes=n)
     refused("different types", H.moe_mlp, gate, other, down, **mlp)
