@@ -296,18 +296,19 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 4 : 3) short_kernel(Produc
     f32x4 f[BLOCKS ? MT : 1][2];  // factors of the lane's rows of a result
   };
   LaneAt lane_at(lane);
+  std::uint32_t x_at = (lane / kTile * kTile + min(lane % kTile, rows - 1)) * 16;
   const auto ask = [&](Stage& s, int h) {
 #pragma unroll
     for (int n = 0; n < kCols; ++n) {
       s.w[n].load(p.m, at[n] + h, lane_at);
       if constexpr (GATED) s.w[kCols + n].load(p.up, at[n] + h, lane_at);
     }
-    lane_at.here();
+    asm volatile("" : "+v"(x_at));
     const GlobalBytes from = (GlobalBytes)src + static_cast<std::size_t>(h) * (MT * 4096);
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int f = 0; f < 4; ++f) s.x[i][f] = *(const __attribute__((address_space(1))) f16x8*)(from + (i * 4 + f) * 1024 + lane_at.by16);
+      for (int f = 0; f < 4; ++f) s.x[i][f] = *(const __attribute__((address_space(1))) f16x8*)(from + (i * 4 + f) * 1024 + x_at);
     if constexpr (BLOCKS) {
       const float* const at_factors = p.x.factors + (static_cast<std::size_t>(tile) * p.steps + h) * (2 * MT * kTile);
 #pragma unroll
