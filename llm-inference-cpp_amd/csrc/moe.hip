@@ -4,13 +4,10 @@
 #include <memory>
 #include <new>
 
-#include "moe.hpp"
+#include "moe_device.hpp"
 
 namespace llmi_hip::moe {
 namespace {
-
-// Dword-aligned vectors: rows may start at any float.
-typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 
@@ -23,24 +20,6 @@ __device__ __forceinline__ std::uint32_t rank_bits(float l) {
   const std::uint32_t b = __float_as_uint(l + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-// A 32-bit value of all 64 lanes: rotations within 16 lanes, then exchanges of
-// sixteens and of halves.
-template <typename Fn>
-__device__ __forceinline__ std::uint32_t across(std::uint32_t v, Fn&& fn) {
-  const auto ror = [](std::uint32_t x, auto by) {
-    return static_cast<std::uint32_t>(
-        __builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x120 + decltype(by)::value, 0xF, 0xF, false));
-  };
-  v = fn(v, ror(v, std::integral_constant<int, 8>{}));
-  v = fn(v, ror(v, std::integral_constant<int, 4>{}));
-  v = fn(v, ror(v, std::integral_constant<int, 2>{}));
-  v = fn(v, ror(v, std::integral_constant<int, 1>{}));
-  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  v = fn(a[0], a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return fn(b[0], b[1]);
-}
-
 // One wavefront a token; lane l holds logits l, l + 64, ...  Every round takes
 // the largest rank of all lanes, and of the logits that have it the first: the
 // lowest place of a lane's, then the lowest lane.
@@ -50,7 +29,6 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const float* __restrict
                                                          float scale, std::int32_t* __restrict__ ids,
                                                          float* __restrict__ weights) {
   const int lane = threadIdx.x & 63;
-  const auto larger = [](std::uint32_t a, std::uint32_t b) { return max(a, b); };
   for (std::size_t t = blockIdx.x * static_cast<std::size_t>(kWaves) + (threadIdx.x >> 6); t < tokens;
        t += static_cast<std::size_t>(gridDim.x) * kWaves) {
     std::uint32_t rank[N];
@@ -63,7 +41,7 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const float* __restrict
       std::uint32_t r = rank[0];
 #pragma unroll
       for (int i = 1; i < N; ++i) r = max(r, rank[i]);
-      return across(r, larger);
+      return across(r, Larger{});
     };
     const auto logit = [](std::uint32_t r) { return __uint_as_float(r & 0x80000000u ? r & 0x7FFFFFFFu : ~r); };
     std::uint32_t best = most();

@@ -125,30 +125,39 @@ __device__ __forceinline__ void two_parts(float a, _Float16& high, _Float16& low
   low = fabsf(a) < __builtin_inff() ? static_cast<_Float16>(a - static_cast<float>(high)) : static_cast<_Float16>(0.0f);
 }
 
-// The largest of 16 lanes (a row of them), in all: rotations.
-__device__ __forceinline__ std::uint32_t max_of_row(std::uint32_t v) {
+// fn over a 32-bit value of 16 lanes (a row of them), in all: rotations.
+template <typename Fn>
+__device__ __forceinline__ std::uint32_t across_row(std::uint32_t v, Fn&& fn) {
   const auto ror = [](std::uint32_t x, auto by) {
     return static_cast<std::uint32_t>(
         __builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x120 + decltype(by)::value, 0xF, 0xF, false));
   };
-  v = max(v, ror(v, std::integral_constant<int, 8>{}));
-  v = max(v, ror(v, std::integral_constant<int, 4>{}));
-  v = max(v, ror(v, std::integral_constant<int, 2>{}));
-  return max(v, ror(v, std::integral_constant<int, 1>{}));
+  v = fn(v, ror(v, std::integral_constant<int, 8>{}));
+  v = fn(v, ror(v, std::integral_constant<int, 4>{}));
+  v = fn(v, ror(v, std::integral_constant<int, 2>{}));
+  return fn(v, ror(v, std::integral_constant<int, 1>{}));
 }
-// The largest of 32 lanes: then an exchange of the two sixteens.
+// Of lanes l, l + 16, l + 32 and l + 48: exchanges of sixteens and of halves.
+template <typename Fn>
+__device__ __forceinline__ std::uint32_t across_rows(std::uint32_t v, Fn&& fn) {
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = fn(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return fn(b[0], b[1]);
+}
+// Of all 64 lanes.
+template <typename Fn>
+__device__ __forceinline__ std::uint32_t across(std::uint32_t v, Fn&& fn) {
+  return across_rows(across_row(v, fn), fn);
+}
+struct Larger {
+  __device__ __forceinline__ std::uint32_t operator()(std::uint32_t a, std::uint32_t b) const { return max(a, b); }
+};
+// The largest of 32 lanes: 16, then an exchange of the two sixteens.
 __device__ __forceinline__ std::uint32_t max_of_half(std::uint32_t v) {
-  v = max_of_row(v);
+  v = across_row(v, Larger{});
   const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
   return max(both[0], both[1]);
-}
-
-// The largest of lanes l, l + 16, l + 32 and l + 48.
-__device__ __forceinline__ std::uint32_t max_of_rows(std::uint32_t v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  v = max(a[0], a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return max(b[0], b[1]);
 }
 
 // g / (1 + exp(-g)) to a few units of the last place, without the branches of

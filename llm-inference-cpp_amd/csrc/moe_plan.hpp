@@ -94,8 +94,8 @@ struct Layout {
 };
 // How slots are grouped: up to kOneGroup of them by one workgroup, more by
 // grouping_blocks() of them, which count first and then place.  With up to
-// kSelfGroup slots of up to kSelfExperts experts, every workgroup that brings
-// rows into row tiles finds the grouping by itself, which spares a launch.
+// kSelfGroup slots of up to kSelfExperts experts, every wavefront that brings
+// a row into its row tile finds the place by itself, which spares a launch.
 constexpr std::size_t kOneGroup = 4096, kSelfGroup = 2048, kSelfExperts = 256;
 inline std::size_t grouping_blocks(std::size_t slots) { return slots <= kOneGroup ? 1 : std::min<std::size_t>((slots + 2047) / 2048, 64); }
 inline bool self_grouped(std::size_t slots, std::size_t experts) { return slots <= kSelfGroup && experts <= kSelfExperts; }

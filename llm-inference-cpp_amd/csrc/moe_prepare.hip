@@ -9,19 +9,18 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 
-// One row of x in two parts, by a wavefront.  The factor is taken from the
-// largest finite |x|: an inf or NaN stays one in the high part and shows in its
-// own row alone.  MT > 0: row r of the row tiles of 16 MT rows; 0: row r as it is.
-template <int MT>
-__device__ __forceinline__ void split_row(const RowSource& src, std::size_t from, int r, const SplitRows& to, int lane) {
-  constexpr int kRows = MT * kTile;
-  const int in = static_cast<int>(src.in), padded = static_cast<int>(src.steps) * kStep;
-  const float* row = src.x + from * src.stride;
-  // Up to 2048 inputs at a time, all asked for before the first is used; what a
-  // shorter row has stays in registers between the two passes.
-  constexpr int kBatch = 4;
+// A row of x for a wavefront: up to 2048 inputs at a time, all asked for before
+// the first is used; a row that is no longer stays in registers.
+struct Row {
+  static constexpr int kBatch = 4, kInputs = kBatch * 512;
+  const float* row;
+  int in, lane;
   float v[kBatch][8];
-  const auto load = [&](int base) {
+  __device__ __forceinline__ Row(const RowSource& src, std::size_t from, int l)
+      : row(src.x + from * src.stride), in(static_cast<int>(src.in)), lane(l) {
+    load(0);
+  }
+  __device__ __forceinline__ void load(int base) {
 #pragma unroll
     for (int c = 0; c < kBatch; ++c) {
       const int k = base + c * 512 + lane * 8;
@@ -37,28 +36,37 @@ __device__ __forceinline__ void split_row(const RowSource& src, std::size_t from
         for (int i = 0; i < 8; ++i) v[c][i] = k + i < in ? row[k + i] : 0.0f;
       }
     }
-  };
-  std::uint32_t top = 0;
-  for (int base = 0; base < in; base += kBatch * 512) {
-    load(base);
-#pragma unroll
-    for (int c = 0; c < kBatch; ++c)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, finite_bits(v[c][i]));
   }
-  const Factor f(max_of_rows(max_of_row(top)));
-  if (lane == 0) to.factors[r] = f.back;
-  for (int base = 0; base < padded; base += kBatch * 512) {
-    if (in > kBatch * 512) load(base);
+};
+
+// The row in two parts.  The factor is taken from the largest finite |x|: an
+// inf or NaN stays one in the high part and shows in its own row alone.
+// MT > 0: row r of the row tiles of 16 MT rows; 0: row r as it is.
+template <int MT>
+__device__ __forceinline__ void store_row(Row& x, const RowSource& src, int r, const SplitRows& to) {
+  constexpr int kRows = MT * kTile;
+  const int padded = static_cast<int>(src.steps) * kStep;
+  std::uint32_t top = 0;
+  for (int base = 0; base < x.in; base += Row::kInputs) {
+    if (base > 0) x.load(base);
 #pragma unroll
-    for (int c = 0; c < kBatch; ++c) {
-      const int k = base + c * 512 + lane * 8;
+    for (int c = 0; c < Row::kBatch; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, finite_bits(x.v[c][i]));
+  }
+  const Factor f(across(top, Larger{}));
+  if (x.lane == 0) to.factors[r] = f.back;
+  for (int base = 0; base < padded; base += Row::kInputs) {
+    if (x.in > Row::kInputs) x.load(base);
+#pragma unroll
+    for (int c = 0; c < Row::kBatch; ++c) {
+      const int k = base + c * 512 + x.lane * 8;
       if (k >= padded) continue;
       f16x8 high, low;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         _Float16 a, b;
-        two_parts(v[c][i] * f.up, a, b);
+        two_parts(x.v[c][i] * f.up, a, b);
         high[i] = a;
         low[i] = b;
       }
@@ -74,6 +82,11 @@ __device__ __forceinline__ void split_row(const RowSource& src, std::size_t from
       }
     }
   }
+}
+template <int MT>
+__device__ __forceinline__ void split_row(const RowSource& src, std::size_t from, int r, const SplitRows& to, int lane) {
+  Row x(src, from, lane);
+  store_row<MT>(x, src, r, to);
 }
 __device__ __forceinline__ std::size_t row_of(const RowSource& src, int pos, int slot) {
   return src.per_row > 0 ? static_cast<std::size_t>(slot) / src.per_row : static_cast<std::size_t>(pos);
@@ -107,51 +120,36 @@ constexpr int kGroupThreads = 1024;
 // Running sums over the experts: count[e] becomes the place of e's first slot;
 // tile(list, index, RowTile) gets every group of rows, by the thread of its
 // expert; the totals (slots, groups of both lists) come back in all threads.
-// SMALL: all three fit into one word (at most kSelfGroup slots).
-template <int THREADS, bool SMALL, typename Fn>
+template <typename Fn>
 __device__ __forceinline__ void lay_ranges(std::int32_t* count, int experts, const Groups& g, std::int32_t (&total)[3], Fn&& tile) {
-  constexpr int kWords = SMALL ? 1 : 3, kAt1 = 12, kAt2 = 22;  // bits of a small word: slots, groups of either list
-  static_assert(!SMALL || (kSelfGroup < (1 << kAt1) && kSelfGroup / kLeastRows + kSelfExperts < (1 << (kAt2 - kAt1))));
-  __shared__ std::uint32_t waves[kWords][THREADS / 64];
+  __shared__ std::int32_t waves[3][kGroupThreads / 64];
   const int t = threadIdx.x, lane = t & 63;
   total[0] = total[1] = total[2] = 0;
-  for (int e0 = 0; e0 < experts; e0 += THREADS) {
+  for (int e0 = 0; e0 < experts; e0 += kGroupThreads) {
     const int e = e0 + t;
     const std::int32_t n = e < experts ? count[e] : 0;
     const std::int32_t own[3] = {n, (n + g.rows[0] - 1) / g.rows[0], (n + g.rows[1] - 1) / g.rows[1]};
-    std::uint32_t word[kWords], sum[kWords];
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      word[i] = SMALL ? static_cast<std::uint32_t>(own[0] | own[1] << kAt1 | own[2] << kAt2) : static_cast<std::uint32_t>(own[i]);
-      std::uint32_t a = word[i];
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const std::uint32_t x = static_cast<std::uint32_t>(__shfl_up(static_cast<int>(a), o, 64));
-        if (lane >= o) a += x;
-      }
-      if (lane == 63) waves[i][t >> 6] = a;
-      sum[i] = a - word[i];
-    }
-    __syncthreads();
-    std::uint32_t whole[kWords] = {};
-#pragma unroll
-    for (int i = 0; i < kWords; ++i)
-#pragma unroll
-      for (int w = 0; w < THREADS / 64; ++w) {
-        const std::uint32_t x = waves[i][w];
-        if (w < t >> 6) sum[i] += x;
-        whole[i] += x;
-      }
     std::int32_t at[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-      const auto part = [&](const std::uint32_t (&v)[kWords]) {
-        if constexpr (!SMALL) return static_cast<std::int32_t>(v[i]);
-        else return static_cast<std::int32_t>(i == 0 ? v[0] & ((1u << kAt1) - 1) : i == 1 ? v[0] >> kAt1 & ((1u << (kAt2 - kAt1)) - 1) : v[0] >> kAt2);
-      };
-      at[i] = total[i] + part(sum);
-      total[i] += part(whole);
+      std::int32_t a = own[i];
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const std::int32_t x = __shfl_up(a, o, 64);
+        if (lane >= o) a += x;
+      }
+      if (lane == 63) waves[i][t >> 6] = a;
+      at[i] = total[i] + a - own[i];
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+      for (int w = 0; w < kGroupThreads / 64; ++w) {
+        const std::int32_t x = waves[i][w];
+        if (w < t >> 6) at[i] += x;
+        total[i] += x;
+      }
     if (e < experts) {
       count[e] = at[0];
 #pragma unroll
@@ -177,7 +175,7 @@ __device__ void group_slots(const std::int32_t* __restrict__ ids, int slots, int
   }
   __syncthreads();
   std::int32_t total[3];
-  lay_ranges<kGroupThreads, false>(count, experts, g, total, [&](int l, std::int32_t at, const RowTile& r) { g.tiles[l][at] = r; });
+  lay_ranges(count, experts, g, total, [&](int l, std::int32_t at, const RowTile& r) { g.tiles[l][at] = r; });
   for (int i = t; i < slots; i += kGroupThreads) {
     const std::int32_t e = ids[i];
     if (e >= 0 && e < experts) g.order[atomicAdd(&count[e], 1)] = i;
@@ -226,7 +224,7 @@ __global__ void __launch_bounds__(kGroupThreads) place_kernel(const std::int32_t
   }
   __syncthreads();
   std::int32_t total[3];
-  lay_ranges<kGroupThreads, false>(count, experts, g, total, [&](int l, std::int32_t at, const RowTile& r) {
+  lay_ranges(count, experts, g, total, [&](int l, std::int32_t at, const RowTile& r) {
     if (r.expert % blocks == b) g.tiles[l][at] = r;
   });
   for (int e = t; e < experts; e += kGroupThreads) {
@@ -244,84 +242,69 @@ __global__ void __launch_bounds__(kGroupThreads) place_kernel(const std::int32_t
   if (b == 0 && t < 3) g.counts[t] = total[t];
 }
 
-// Up to kSelfGroup slots: every workgroup finds the grouping for itself (the
-// same one: slots keep their order) and brings its share of the rows into row
-// tiles; the first one also stores it for the products.
+// Up to kSelfGroup slots, a wavefront each: it asks for its row of x, counts
+// with its workgroup every expert's slots, and so finds its own place (slots
+// keep their order), to which it brings the row; the place in the order and the
+// groups of rows that start with its slot it stores for the products.
 template <int MT>
 __global__ void __launch_bounds__(kThreads) self_kernel(const std::int32_t* __restrict__ ids, int slots, int experts, Groups g,
                                                         RowSource src, SplitRows to) {
-  constexpr int kRows = MT * kTile, kChunks = static_cast<int>(kSelfGroup) / 64;
+  constexpr int kEach = static_cast<int>(kSelfExperts) / 64;
+  // Three counts in a word: slots, groups of either list.
+  constexpr int kAt1 = 12, kAt2 = 22;
+  static_assert(kSelfGroup < (1 << kAt1) && kSelfGroup / kLeastRows + kSelfExperts < (1 << (kAt2 - kAt1)));
   __shared__ std::int32_t count[kSelfExperts];
-  __shared__ std::uint16_t before[kChunks][kSelfExperts];  // slots of an expert in 64 of the slots, then in all before them
-  __shared__ std::uint16_t order[kSelfGroup];
-  __shared__ RowTile tiles[kSelfGroup / kRows + kSelfExperts];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, chunks = (slots + 63) / 64;
-  for (int i = t; i < chunks * static_cast<int>(kSelfExperts) / 2; i += kThreads) reinterpret_cast<std::uint32_t*>(&before[0][0])[i] = 0;
+  __shared__ std::int16_t all[kSelfGroup];  // the slots' experts, -1: none
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int slot = blockIdx.x * kWaves + wave;
+  for (int e = t; e < static_cast<int>(kSelfExperts); e += kThreads) count[e] = 0;
   __syncthreads();
-  // The lanes with this lane's expert: one ballot a bit of its number.
-  const auto expert_of = [&](int c) {
+  const int own_slot = min(slot, slots - 1);
+  Row x(src, row_of(src, own_slot, own_slot), lane);
+  for (int i = t; i < slots; i += kThreads) {
+    const std::int32_t e = ids[i];
+    const bool live = e >= 0 && e < experts;
+    all[i] = static_cast<std::int16_t>(live ? e : -1);
+    if (live) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  if (slot >= slots) return;
+  const auto add = [](std::uint32_t a, std::uint32_t b) { return a + b; };
+  std::uint32_t word[kEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const std::uint32_t n = static_cast<std::uint32_t>(count[i * 64 + lane]);
+    const auto groups = [&](int l) { return (n + static_cast<std::uint32_t>(g.rows[l]) - 1) / static_cast<std::uint32_t>(g.rows[l]); };
+    word[i] = n | groups(0) << kAt1 | groups(1) << kAt2;
+    sum += word[i];
+  }
+  const auto part = [](std::uint32_t w, int i) {
+    return static_cast<std::int32_t>(i == 0 ? w & ((1u << kAt1) - 1) : i == 1 ? w >> kAt1 & ((1u << (kAt2 - kAt1)) - 1) : w >> kAt2);
+  };
+  if (slot == 0) {
+    sum = across(sum, add);
+    if (lane < 3) g.counts[lane] = part(sum, lane);
+  }
+  const int e = __builtin_amdgcn_readfirstlane(all[slot]);
+  if (e < 0) return;
+  std::uint32_t before = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (i * 64 + lane < e) before += word[i];
+  before = across(before, add);
+  int rank = 0;
+  for (int c = 0; c <= slot / 64; ++c) {
     const int i = c * 64 + lane;
-    const std::int32_t e = i < slots ? ids[i] : -1;
-    return e >= 0 && e < experts ? e : -1;
-  };
-  const auto same_lanes = [&](std::int32_t e) {
-    std::uint64_t same = __ballot(e >= 0);
-#pragma unroll
-    for (int bit = 1; bit < static_cast<int>(kSelfExperts); bit <<= 1) {
-      const std::uint64_t set = __ballot((e & bit) != 0);
-      same &= (e & bit) != 0 ? set : ~set;
-    }
-    return same;
-  };
-  const std::uint64_t below = (std::uint64_t{1} << lane) - 1;
-  std::int32_t mine[kChunks / kWaves], rank[kChunks / kWaves];
-#pragma unroll
-  for (int i = 0; i < kChunks / kWaves; ++i) mine[i] = expert_of(wave + i * kWaves);
-#pragma unroll
-  for (int i = 0; i < kChunks / kWaves; ++i) {
-    const int c = wave + i * kWaves;
-    if (c >= chunks) break;
-    const std::uint64_t same = same_lanes(mine[i]);
-    rank[i] = __builtin_popcountll(same & below);
-    if (mine[i] >= 0 && rank[i] == 0) before[c][mine[i]] = static_cast<std::uint16_t>(__builtin_popcountll(same));
+    rank += __builtin_popcountll(__ballot(i < slot && all[i] == e));
   }
-  __syncthreads();
-  for (int e = t; e < experts; e += kThreads) {
-    std::uint32_t n = 0;
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      if (c >= chunks) break;
-      const std::uint32_t own = before[c][e];
-      before[c][e] = static_cast<std::uint16_t>(n);
-      n += own;
-    }
-    count[e] = static_cast<std::int32_t>(n);
+  const int r0 = g.rows[0], r1 = g.rows[1], n = count[e], first = part(before, 0) + rank;
+  const int tile0 = part(before, 1) + rank / r0, tile1 = part(before, 2) + rank / r1;
+  if (lane == 0) {
+    g.order[first] = slot;
+    if (rank % r0 == 0) g.tiles[0][tile0] = RowTile{e, first, min(n - rank, r0), tile1};
+    if (rank % r1 == 0) g.tiles[1][tile1] = RowTile{e, first, min(n - rank, r1), 0};
   }
-  __syncthreads();
-  std::int32_t total[3];
-  const bool store = blockIdx.x == 0;
-  lay_ranges<kThreads, true>(count, experts, g, total, [&](int l, std::int32_t at, const RowTile& r) {
-    if (l == 0) tiles[at] = r;
-    if (store) g.tiles[l][at] = r;
-  });
-#pragma unroll
-  for (int i = 0; i < kChunks / kWaves; ++i) {
-    const int c = wave + i * kWaves, e = mine[i];
-    if (c >= chunks) break;
-    if (e < 0) continue;
-    const std::int32_t at = count[e] + rank[i] + before[c][e];
-    order[at] = static_cast<std::uint16_t>(c * 64 + lane);
-    if (store) g.order[at] = c * 64 + lane;
-  }
-  if (store && t < 3) g.counts[t] = total[t];
-  __syncthreads();
-  const int most = total[1] * kRows;
-  for (int r = blockIdx.x * kWaves + wave; r < most; r += gridDim.x * kWaves) {
-    const RowTile rt = tiles[r / kRows];
-    if (r % kRows >= rt.rows) continue;  // nothing reads its results
-    const int pos = rt.first + r % kRows;
-    split_row<MT>(src, row_of(src, pos, order[pos]), r, to, lane);
-  }
+  store_row<MT>(x, src, tile0 * (MT * kTile) + rank % (MT * kTile), to);
 }
 
 }  // namespace
@@ -332,7 +315,7 @@ int launch_prepare(const std::int32_t* ids, std::size_t slots, std::size_t exper
   const bool tiled = r0 <= static_cast<int>(kMostShortRows);
   const std::size_t tile_rows = most_tiles(slots, experts, static_cast<std::size_t>(r0)) * static_cast<std::size_t>(r0);
   if (tiled && self_grouped(slots, experts)) {
-    const unsigned grid = static_cast<unsigned>(std::min<std::size_t>(ceil_div(tile_rows, kWaves), 512));
+    const unsigned grid = static_cast<unsigned>(ceil_div(slots, kWaves));
     if (r0 == 16) self_kernel<1><<<grid, kThreads, 0, s>>>(ids, n, e, g, x, to);
     else self_kernel<2><<<grid, kThreads, 0, s>>>(ids, n, e, g, x, to);
     LLMI_TRY_HIP(hipGetLastError());

@@ -36,7 +36,7 @@ __device__ __forceinline__ void store_parts(const ProductArgs& p, int tile, int 
   std::uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, finite_bits(v[i]));
-  const Factor f(max_of_rows(top));
+  const Factor f(across_rows(top, Larger{}));
   f16x8 high, low;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
