@@ -79,7 +79,7 @@ __device__ __forceinline__ void each(Fn&& fn) {
 // other one is used; the weights stay in the registers of the wavefront that
 // uses them.
 template <int TYPE, int MT, int NT, bool GATED>
-__global__ void __launch_bounds__(kThreads, 2) long_kernel(ProductArgs p) {
+__global__ void __launch_bounds__(kThreads, TYPE == LLMI_TYPE_Q4_0 ? 2 : 3) long_kernel(ProductArgs p) {
   constexpr int kParts = MT * 4;  // 1 KiB pieces of a buffer: (16 rows, block, high / low)
   __shared__ __attribute__((aligned(16))) f16x8 xs[2][kParts][64];
   __shared__ std::int32_t to_row[MT * kTile];  // y's rows, and the factors of x's
@@ -147,62 +147,64 @@ __global__ void __launch_bounds__(kThreads, 2) long_kernel(ProductArgs p) {
   for (int n = 0; n < NT; ++n) w[0][n].here();
   for (int h = 0; h < p.steps; h += 2) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (h + j >= p.steps) break;
-        if (h + j + 1 < p.steps) {
-          bring(1 - j);
-          weights(w[1 - j], h + j + 1);
-        }
-// Two outputs' tiles at a time: their four instructions, then the
-        // additions of the two before them, whose results are there by now.
-        // The regions keep the compiler from holding more operands at once
-        // than the registers have room for.
-        f16x8 code[NT];
-        f16x8 x[2][2];
-        f32x4 d[3][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) code[n] = w[j][n].codes(0);
-        x[0][0] = xs[j][0][read_at];
-        x[0][1] = xs[j][1][read_at];
-        constexpr int kPairs = NT / 2, kSteps = 2 * MT * kPairs;
-        const auto add = [&](auto step) {
-          constexpr int q = decltype(step)::value, i = q / kPairs % MT, n0 = q % kPairs * 2, b2 = q / (kPairs * MT);
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[n0 + n][i][r] = __builtin_fmaf(d[q % 3][n][r], w[j][n0 + n].s[b2], acc[n0 + n][i][r]);
-          // Here, not at the end of the block, where the compiler would put them all.
-#pragma unroll
-          for (int n = 0; n < 2; ++n) asm volatile("" : "+v"(acc[n0 + n][i]));
-        };
-        each<kSteps>([&](auto step) {
-          constexpr int q = decltype(step)::value, ib = q / kPairs, i = ib % MT, n0 = q % kPairs * 2, b2 = ib / MT;
-          if constexpr (n0 == 0 && ib + 1 < 2 * MT) {  // the next rows' parts
-            x[(ib + 1) % 2][0] = xs[j][(ib + 1) % MT * 4 + (ib + 1) / MT * 2][read_at];
-            x[(ib + 1) % 2][1] = xs[j][(ib + 1) % MT * 4 + (ib + 1) / MT * 2 + 1][read_at];
-          }
-#pragma unroll
-          for (int n = 0; n < 2; ++n) d[q % 3][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ib % 2][0], code[n0 + n], f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-          for (int n = 0; n < 2; ++n) d[q % 3][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ib % 2][1], code[n0 + n], d[q % 3][n], 0, 0, 0);
-          if constexpr (q > 1) add(std::integral_constant<int, q - 2>{});
-          if constexpr (b2 == 0 && i == MT - 1) {  // the next block's codes
-#pragma unroll
-            for (int n = 0; n < 2; ++n) code[n0 + n] = w[j][n0 + n].codes(1);
-          }
-#pragma unroll
-          for (int i2 = 0; i2 < 4; ++i2) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                              // one matrix instruction,
-            __builtin_amdgcn_sched_group_barrier(0x002, b2 == 0 && i == MT - 1 ? 6 : 2, 0);  // vector ones beside it
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        });
-        add(std::integral_constant<int, kSteps - 2>{});
-        add(std::integral_constant<int, kSteps - 1>{});
-        landed();
-#pragma unroll
-        for (int n = 0; n < NT; ++n) w[1 - j][n].here();
+    for (int j = 0; j < 2; ++j) {
+      if (h + j >= p.steps) break;
+      if (h + j + 1 < p.steps) {
+        bring(1 - j);
+        if constexpr (TYPE == LLMI_TYPE_Q4_0) weights(w[1 - j], h + j + 1);
       }
+      // Two outputs' tiles at a time: their four instructions, then the
+      // additions of the two before them, whose results are there by now.
+      // The regions keep the compiler from holding more operands at once
+      // than the registers have room for.
+      f16x8 code[NT];
+      f16x8 x[2][2];
+      constexpr int kLag = TYPE == LLMI_TYPE_Q4_0 ? 2 : 1, kD = kLag + 1;
+      f32x4 d[kD][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) code[n] = w[j][n].codes(0);
+      x[0][0] = xs[j][0][read_at];
+      x[0][1] = xs[j][1][read_at];
+      constexpr int kPairs = NT / 2, kSteps = 2 * MT * kPairs;
+      const auto add = [&](auto step) {
+        constexpr int q = decltype(step)::value, i = q / kPairs % MT, n0 = q % kPairs * 2, b2 = q / (kPairs * MT);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[n0 + n][i][r] = __builtin_fmaf(d[q % kD][n][r], w[j][n0 + n].s[b2], acc[n0 + n][i][r]);
+        // Here, not at the end of the block, where the compiler would put them all.
+#pragma unroll
+        for (int n = 0; n < 2; ++n) asm volatile("" : "+v"(acc[n0 + n][i]));
+      };
+      each<kSteps>([&](auto step) {
+        constexpr int q = decltype(step)::value, ib = q / kPairs, i = ib % MT, n0 = q % kPairs * 2, b2 = ib / MT;
+        if constexpr (TYPE != LLMI_TYPE_Q4_0 && q == kSteps / 2) weights(w[1 - j], min(h + j + 1, p.steps - 1));
+        if constexpr (n0 == 0 && ib + 1 < 2 * MT) {  // the next rows' parts
+          x[(ib + 1) % 2][0] = xs[j][(ib + 1) % MT * 4 + (ib + 1) / MT * 2][read_at];
+          x[(ib + 1) % 2][1] = xs[j][(ib + 1) % MT * 4 + (ib + 1) / MT * 2 + 1][read_at];
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) d[q % kD][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ib % 2][0], code[n0 + n], f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) d[q % kD][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ib % 2][1], code[n0 + n], d[q % kD][n], 0, 0, 0);
+        if constexpr (q >= kLag) add(std::integral_constant<int, q - kLag>{});
+        if constexpr (b2 == 0 && i == MT - 1) {  // the next block's codes
+#pragma unroll
+          for (int n = 0; n < 2; ++n) code[n0 + n] = w[j][n0 + n].codes(1);
+        }
+#pragma unroll
+        for (int i2 = 0; i2 < 4; ++i2) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                              // one matrix instruction,
+          __builtin_amdgcn_sched_group_barrier(0x002, b2 == 0 && i == MT - 1 ? 6 : 2, 0);  // vector ones beside it
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if constexpr (kLag > 1) add(std::integral_constant<int, kSteps - 2>{});
+      add(std::integral_constant<int, kSteps - 1>{});
+      landed();
+#pragma unroll
+      for (int n = 0; n < NT; ++n) w[1 - j][n].here();
+    }
   }
   if constexpr (GATED) {
     if (p.h.values != nullptr) {
