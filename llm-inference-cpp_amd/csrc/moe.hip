@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const float* __restrict
 template <int TYPE>
 __global__ void __launch_bounds__(kThreads) lay_out(const std::uint8_t* __restrict__ data,
                                                     const float* __restrict__ scales, std::size_t count, int out, int in,
-                                                    std::uint8_t* __restrict__ to, float* __restrict__ to_scales) {
+                                                    std::uint8_t* __restrict__ to) {
   const int blocks = (in + kBlock - 1) / kBlock, steps = (in + kStep - 1) / kStep;
   const int tiles = (out + kTile - 1) / kTile;
   const std::size_t row_bytes = TYPE == LLMI_TYPE_Q4_0 ? (in + 1) / 2 : in;
@@ -133,11 +133,12 @@ __global__ void __launch_bounds__(kThreads) lay_out(const std::uint8_t* __restri
         words[2 * b + 1] = code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24;
       }
     }
-    if constexpr (TYPE == LLMI_TYPE_Q4_0) *reinterpret_cast<uint2*>(to + u * 8) = uint2{words[0], words[1]};
-    else *reinterpret_cast<uint4*>(to + u * 16) = uint4{words[0], words[1], words[2], words[3]};
+    std::uint8_t* const at = to + c * step_bytes(TYPE);
+    if constexpr (TYPE == LLMI_TYPE_Q4_0) *reinterpret_cast<uint2*>(at + lane * 8) = uint2{words[0], words[1]};
+    else *reinterpret_cast<uint4*>(at + lane * 16) = uint4{words[0], words[1], words[2], words[3]};
     if (lane < static_cast<int>(kStepScales)) {  // output lane / 2, block lane % 2
       const int so = tile * kTile + lane / 2, sb = step * 2 + lane % 2;
-      to_scales[c * kStepScales + lane] = so < out && sb < blocks ? scales[(expert * out + static_cast<std::size_t>(so)) * blocks + sb] : 0.0f;
+      reinterpret_cast<float*>(at + code_bytes(TYPE))[lane] = so < out && sb < blocks ? scales[(expert * out + static_cast<std::size_t>(so)) * blocks + sb] : 0.0f;
     }
   }
 }
@@ -146,14 +147,13 @@ unsigned grid_for(std::size_t units, std::size_t each) {
   return static_cast<unsigned>(std::min<std::size_t>(std::max<std::size_t>(ceil_div(units, each), 1), kMostGroups));
 }
 
-int launch_lay_out(const std::uint8_t* data, const float* scales, const Shape& s, std::uint8_t* to, float* to_scales,
-                   hipStream_t st) {
+int launch_lay_out(const std::uint8_t* data, const float* scales, const Shape& s, std::uint8_t* to, hipStream_t st) {
   const unsigned grid = grid_for(s.count * s.tiles() * s.steps() * 64, kThreads);
   const int out = static_cast<int>(s.out), in = static_cast<int>(s.in);
   if (s.type == LLMI_TYPE_Q4_0)
-    lay_out<LLMI_TYPE_Q4_0><<<grid, kThreads, 0, st>>>(data, scales, s.count, out, in, to, to_scales);
+    lay_out<LLMI_TYPE_Q4_0><<<grid, kThreads, 0, st>>>(data, scales, s.count, out, in, to);
   else
-    lay_out<LLMI_TYPE_Q8_0><<<grid, kThreads, 0, st>>>(data, scales, s.count, out, in, to, to_scales);
+    lay_out<LLMI_TYPE_Q8_0><<<grid, kThreads, 0, st>>>(data, scales, s.count, out, in, to);
   LLMI_TRY_HIP(hipGetLastError());
   return LLMI_OK;
 }
@@ -162,8 +162,7 @@ int new_experts(const Shape& s, std::unique_ptr<llmi_hip_experts>* to) {
   to->reset(new (std::nothrow) llmi_hip_experts);
   if (*to == nullptr) return fail(LLMI_ERR_HIP, "experts: out of host memory");
   (*to)->shape = s;
-  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&(*to)->codes), s.code_bytes()));
-  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&(*to)->scales), s.scale_floats() * sizeof(float)));
+  LLMI_TRY_HIP(hipMalloc(reinterpret_cast<void**>(&(*to)->steps), s.bytes()));
   return LLMI_OK;
 }
 
@@ -274,7 +273,7 @@ int llmi_hip_experts_upload_dev(const uint8_t* data, const float* scales, size_t
   LLMI_REQUIRE(data != nullptr && scales != nullptr, "experts_upload: null pointer");
   std::unique_ptr<llmi_hip_experts> e;
   if (int rc = new_experts(s, &e)) return rc;
-  if (int rc = launch_lay_out(data, scales, s, e->codes, e->scales, library_stream())) return rc;
+  if (int rc = launch_lay_out(data, scales, s, e->steps, library_stream())) return rc;
   LLMI_TRY_HIP(hipStreamSynchronize(library_stream()));
   *experts = e.release();
   return LLMI_OK;
@@ -310,8 +309,7 @@ int llmi_hip_experts_create(const llmi_hip_weight* const* weights, size_t count,
   for (size_t i = 0; i < count && rc == LLMI_OK; ++i) {
     rc = launch_relayout_to_planar(weights[i]->m, planar, planar_scales, library_stream());
     if (rc == LLMI_OK)
-      rc = launch_lay_out(planar, planar_scales, one, e->codes + i * one.code_bytes(), e->scales + i * one.scale_floats(),
-                          library_stream());
+      rc = launch_lay_out(planar, planar_scales, one, e->steps + i * one.bytes(), library_stream());
   }
   const hipError_t end = hipStreamSynchronize(library_stream());
   (void)hipFree(planar);

@@ -8,15 +8,15 @@ namespace llmi_hip::moe {
 
 // The experts' codes in the order in which the matrix instructions take them.
 // Lane l of a wavefront holds output l % 16 of a tile and, of each block, the
-// 8 inputs 8 (l / 16) ...; at (expert * tiles + tile) * steps + step:
-//   Q4_0  codes[at * 512 + lane * 8]: two dwords, one of each block; its
-//         nibbles, from the lowest, are the codes + 8 of inputs 0 2 4 6 1 3 5 7;
-//   Q8_0  codes[at * 1024 + lane * 16]: codes + 128 of the 8 inputs of the one
-//         block, then of the other;
-//   scales[at * 32 + output * 2 + block].
+// 8 inputs 8 (l / 16) ...  Step ((expert * tiles + tile) * steps + step) takes
+// step_bytes(type), so that a tile's steps are one stream:
+//   Q4_0  at lane * 8: two dwords, one of each block; its nibbles, from the
+//         lowest, are the codes + 8 of inputs 0 2 4 6 1 3 5 7;
+//   Q8_0  at lane * 16: codes + 128 of the 8 inputs of the one block, then of
+//         the other;
+//   behind the codes 32 floats: the scale of output o and block b at 2 o + b.
 struct Matrices {
-  const std::uint8_t* codes = nullptr;
-  const float* scales = nullptr;
+  const std::uint8_t* steps = nullptr;
 };
 
 // A group of rows of one expert: positions first .. first + rows - 1 of the
@@ -125,11 +125,9 @@ int launch_few_sum(const FewSum& p, hipStream_t s);
 
 struct llmi_hip_experts {
   llmi_hip::moe::Shape shape;
-  std::uint8_t* codes = nullptr;
-  float* scales = nullptr;
-  llmi_hip::moe::Matrices view() const { return {codes, scales}; }
+  std::uint8_t* steps = nullptr;
+  llmi_hip::moe::Matrices view() const { return {steps}; }
   ~llmi_hip_experts() {
-    if (codes != nullptr) (void)hipFree(codes);
-    if (scales != nullptr) (void)hipFree(scales);
+    if (steps != nullptr) (void)hipFree(steps);
   }
 };

@@ -68,17 +68,18 @@ struct Weights {
   // at: (expert * tiles + tile) * steps + step, common to the wavefront.
   __device__ __forceinline__ void load(const Matrices& m, std::size_t at, LaneAt& lane) {
     lane.here();
-    const std::uint32_t code_at = TYPE == LLMI_TYPE_Q4_0 ? lane.by8 : lane.by16, scale_at = lane.scale;
+    const std::uint32_t code_at = TYPE == LLMI_TYPE_Q4_0 ? lane.by8 : lane.by16;
+    const GlobalBytes step = (GlobalBytes)m.steps + at * step_bytes(TYPE);
     if constexpr (TYPE == LLMI_TYPE_Q4_0) {
-      const u32x2 v = *(const __attribute__((address_space(1))) u32x2*)((GlobalBytes)m.codes + at * 512 + code_at);
+      const u32x2 v = *(const __attribute__((address_space(1))) u32x2*)(step + code_at);
       c[0] = v[0];
       c[1] = v[1];
     } else {
-      const u32x4 v = *(const __attribute__((address_space(1))) u32x4*)((GlobalBytes)m.codes + at * 1024 + code_at);
+      const u32x4 v = *(const __attribute__((address_space(1))) u32x4*)(step + code_at);
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[i] = v[i];
     }
-    const f32x2 v = *(const __attribute__((address_space(1))) f32x2*)((GlobalBytes)(m.scales + at * kStepScales) + scale_at);
+    const f32x2 v = *(const __attribute__((address_space(1))) f32x2*)(step + code_bytes(TYPE) + lane.scale);
     s[0] = v[0];
     s[1] = v[1];
   }

@@ -417,7 +417,7 @@ int launch_few(const FewProduct& f, hipStream_t s) {
                   static_cast<int>(sh.count), static_cast<int>(sh.out), static_cast<int>(sh.in), static_cast<int>(sh.tiles()),
                   static_cast<int>(pairs), static_cast<int>(sh.steps()), static_cast<int>(ceil_div(sh.steps(), 2)), rows};
   const unsigned grid = static_cast<unsigned>(f.slots * pairs);
-  const bool gated = f.up.codes != nullptr;
+  const bool gated = f.up.steps != nullptr;
   LLMI_REQUIRE(!gated || !more, "moe: too many rows of x for a gated pair");
   with_flags([&](auto gate, auto many, auto quads) {
     if constexpr (!(gate && many)) {

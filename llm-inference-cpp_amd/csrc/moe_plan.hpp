@@ -20,6 +20,9 @@ constexpr std::size_t kMaxInner = std::size_t{1} << 18;  // inputs, and results,
 constexpr int kTile = 16;                         // outputs and rows of a matrix instruction
 constexpr int kStep = 2 * LLMI_BLOCK_SIZE;        // inputs of a step: two blocks
 constexpr std::size_t kStepScales = 2 * kTile;    // a tile's scales of a step
+// Bytes of a tile's codes of a step, behind which its scales lie.
+constexpr std::size_t code_bytes(int type) { return type == LLMI_TYPE_Q4_0 ? 512 : 1024; }
+constexpr std::size_t step_bytes(int type) { return code_bytes(type) + kStepScales * sizeof(float); }
 
 // The shape of a set of experts as the device holds it: per expert, tiles of
 // 16 outputs; per tile, steps of 64 inputs (outputs and inputs behind the last
@@ -30,9 +33,7 @@ struct Shape {
   std::size_t blocks() const { return (in + LLMI_BLOCK_SIZE - 1) / LLMI_BLOCK_SIZE; }
   std::size_t steps() const { return (in + kStep - 1) / kStep; }
   std::size_t tiles() const { return (out + kTile - 1) / kTile; }
-  std::size_t step_bytes() const { return type == LLMI_TYPE_Q4_0 ? 512 : 1024; }
-  std::size_t code_bytes() const { return count * tiles() * steps() * step_bytes(); }
-  std::size_t scale_floats() const { return count * tiles() * steps() * kStepScales; }
+  std::size_t bytes() const { return count * tiles() * steps() * step_bytes(type); }
 };
 
 inline std::string check_shape(const Shape& s) {

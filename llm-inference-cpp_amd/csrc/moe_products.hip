@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 4 : 3) short_kernel(Produc
 }  // namespace
 
 int launch_product(const Product& p, hipStream_t s) {
-  const bool gated = p.up.codes != nullptr;
+  const bool gated = p.up.steps != nullptr;
   constexpr int kNT = 4;
   const int rows = p.g.rows[p.list];
   const std::size_t cols = rows <= static_cast<int>(kMostShortRows) ? short_columns(gated) : long_columns(gated);
