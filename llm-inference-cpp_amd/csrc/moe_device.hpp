@@ -58,6 +58,12 @@ struct LaneAt {
   __device__ __forceinline__ void here() { asm volatile("" : "+v"(by8), "+v"(by16), "+v"(scale)); }
 };
 
+// Where the steps of an expert's tile are; tile: expert * tiles + tile.
+template <int TYPE>
+__device__ __forceinline__ GlobalBytes tile_at(const Matrices& m, std::size_t tile, int steps) {
+  return (GlobalBytes)m.steps + tile * steps * step_bytes(TYPE);
+}
+
 // A lane's weights of one tile and step.
 template <int TYPE>
 struct Weights {
@@ -65,21 +71,21 @@ struct Weights {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   std::uint32_t c[TYPE == LLMI_TYPE_Q4_0 ? 2 : 4];
   float s[2];
-  // at: (expert * tiles + tile) * steps + step, common to the wavefront.
-  __device__ __forceinline__ void load(const Matrices& m, std::size_t at, LaneAt& lane) {
+  // Step `step` of a tile whose steps are at `from`, common to the wavefront.
+  __device__ __forceinline__ void load(GlobalBytes from, int step, LaneAt& lane) {
     lane.here();
     const std::uint32_t code_at = TYPE == LLMI_TYPE_Q4_0 ? lane.by8 : lane.by16;
-    const GlobalBytes step = (GlobalBytes)m.steps + at * step_bytes(TYPE);
+    const GlobalBytes at = from + static_cast<std::uint32_t>(step) * static_cast<std::uint32_t>(step_bytes(TYPE));  // at most 2^12 steps
     if constexpr (TYPE == LLMI_TYPE_Q4_0) {
-      const u32x2 v = *(const __attribute__((address_space(1))) u32x2*)(step + code_at);
+      const u32x2 v = *(const __attribute__((address_space(1))) u32x2*)(at + code_at);
       c[0] = v[0];
       c[1] = v[1];
     } else {
-      const u32x4 v = *(const __attribute__((address_space(1))) u32x4*)(step + code_at);
+      const u32x4 v = *(const __attribute__((address_space(1))) u32x4*)(at + code_at);
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[i] = v[i];
     }
-    const f32x2 v = *(const __attribute__((address_space(1))) f32x2*)(step + code_bytes(TYPE) + lane.scale);
+    const f32x2 v = *(const __attribute__((address_space(1))) f32x2*)(at + code_bytes(TYPE) + lane.scale);
     s[0] = v[0];
     s[1] = v[1];
   }

@@ -137,7 +137,9 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
   std::uint64_t same = __ballot(mine == expert);
   if (__builtin_ctzll(same) != slot) return;
   const std::size_t tile0 = static_cast<std::size_t>(expert) * p.tiles;
-  const std::size_t at0 = (tile0 + pair * 2) * p.steps, at1 = (tile0 + min(pair * 2 + 1, p.tiles - 1)) * p.steps;
+  GlobalBytes from[kMats];
+#pragma unroll
+  for (int m = 0; m < kMats; ++m) from[m] = tile_at<TYPE>(m < 2 ? p.m : p.up, tile0 + min(pair * 2 + m % 2, p.tiles - 1), p.steps);
   const int each = (p.chunks + kWaves - 1) / kWaves;
   const int c0 = min(wave * each, p.chunks), c1 = min(c0 + each, p.chunks);
   const WaveLds w{lds + wave * (p.rows * kRowBytes + 64), reinterpret_cast<float*>(lds + wave * (p.rows * kRowBytes + 64) + p.rows * kRowBytes)};
@@ -170,12 +172,8 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int step = min(2 * c + t, p.steps - 1);
-          ring[i][0][t].load(p.m, at0 + step, lane_at);
-          ring[i][1][t].load(p.m, at1 + step, lane_at);
-          if constexpr (GATED) {
-            ring[i][2][t].load(p.up, at0 + step, lane_at);
-            ring[i][3][t].load(p.up, at1 + step, lane_at);
-          }
+#pragma unroll
+          for (int m = 0; m < kMats; ++m) ring[i][m][t].load(from[m], step, lane_at);
         }
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) x[i].load(j, at[j], c, p.in, lane);
@@ -293,7 +291,7 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
   std::uint64_t left = firsts;
   for (int i = u0 / p.chunks; i > 0 && left != 0; --i) left &= left - 1;
   int next = u0, chunk = u0 % p.chunks;
-  std::size_t w_at = 0;
+  GlobalBytes w_at = nullptr;
   const _Float16* row = nullptr;
   const float* factor_row = nullptr;
   float row_times = 0.0f;
@@ -301,7 +299,7 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
   const auto enter = [&] {
     const int s = __builtin_ctzll(left), e = __builtin_amdgcn_readlane(mine, s);
     const std::uint64_t same = __ballot(mine == e);
-    w_at = (static_cast<std::size_t>(e) * p.tiles + tile) * p.steps;
+    w_at = tile_at<TYPE>(p.m, static_cast<std::size_t>(e) * p.tiles + tile, p.steps);
     // The token's slots of this expert, as bits from its first slot on.
     const auto chosen = [&](int t) {
       const std::uint64_t bits = same >> (t * p.top_k);
@@ -324,7 +322,7 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
   if (u0 < u1) enter();
   const auto ask = [&](int i) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) ring[i][t].load(p.m, w_at + min(2 * chunk + t, p.steps - 1), lane_at);
+    for (int t = 0; t < 2; ++t) ring[i][t].load(w_at, min(2 * chunk + t, p.steps - 1), lane_at);
     x[i] = *reinterpret_cast<const u32x4*>(row);
     live[i] = row_live;
     row += 4 * 64;

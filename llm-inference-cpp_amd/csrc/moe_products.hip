@@ -127,17 +127,15 @@ __global__ void __launch_bounds__(kThreads, TYPE == LLMI_TYPE_Q4_0 ? 2 : 3) long
         src[i] += 256;
       }
   };
-  std::size_t at[kCols];
+  GlobalBytes at[NT];
 #pragma unroll
-  for (int n = 0; n < kCols; ++n) at[n] = (static_cast<std::size_t>(expert) * p.tiles + min(col0 + n, p.tiles - 1)) * p.steps;
+  for (int n = 0; n < NT; ++n)
+    at[n] = tile_at<TYPE>(n < kCols ? p.m : p.up, static_cast<std::size_t>(expert) * p.tiles + min(col0 + n % kCols, p.tiles - 1), p.steps);
   Weights<TYPE> w[2][NT];
   LaneAt lane_at(lane);
   const auto weights = [&](Weights<TYPE> (&to)[NT], int step) {
 #pragma unroll
-    for (int n = 0; n < kCols; ++n) {
-      to[n].load(p.m, at[n] + step, lane_at);
-      if constexpr (GATED) to[kCols + n].load(p.up, at[n] + step, lane_at);
-    }
+    for (int n = 0; n < NT; ++n) to[n].load(at[n], step, lane_at);
   };
   f32x4 acc[NT][MT] = {};
   bring(0);
@@ -289,9 +287,10 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 4 : 3) short_kernel(Produc
   const int share = (p.steps + kWaves - 1) / kWaves;
   const int h0 = min(wave * share, p.steps), h1 = min(h0 + share, p.steps);
   const std::uint8_t* const src = reinterpret_cast<const std::uint8_t*>(p.x.values) + static_cast<std::size_t>(tile) * p.steps * (MT * 4096);
-  std::size_t at[kCols];
+  GlobalBytes at[NT];
 #pragma unroll
-  for (int n = 0; n < kCols; ++n) at[n] = (static_cast<std::size_t>(expert) * p.tiles + min(col0 + n, p.tiles - 1)) * p.steps;
+  for (int n = 0; n < NT; ++n)
+    at[n] = tile_at<TYPE>(n < kCols ? p.m : p.up, static_cast<std::size_t>(expert) * p.tiles + min(col0 + n % kCols, p.tiles - 1), p.steps);
   struct Stage {
     Weights<TYPE> w[NT];
     f16x8 x[MT][4];              // block, high / low
@@ -301,10 +300,7 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 4 : 3) short_kernel(Produc
   std::uint32_t x_at = (lane / kTile * kTile + min(lane % kTile, rows - 1)) * 16;
   const auto ask = [&](Stage& s, int h) {
 #pragma unroll
-    for (int n = 0; n < kCols; ++n) {
-      s.w[n].load(p.m, at[n] + h, lane_at);
-      if constexpr (GATED) s.w[kCols + n].load(p.up, at[n] + h, lane_at);
-    }
+    for (int n = 0; n < NT; ++n) s.w[n].load(at[n], h, lane_at);
     asm volatile("" : "+v"(x_at));
     const GlobalBytes from = (GlobalBytes)src + static_cast<std::size_t>(h) * (MT * 4096);
 #pragma unroll
