@@ -53,16 +53,24 @@ inline std::size_t most_tiles(std::size_t slots, std::size_t experts, std::size_
 // Tiles of outputs of a workgroup: of the kernel for short work, of the one for long.
 inline std::size_t short_columns(bool gated) { return gated ? 2 : 4; }
 inline std::size_t long_columns(bool gated) { return 4 * short_columns(gated); }
-// The largest number of slots that goes to the kernel for short work.
+// The largest number of slots that goes to the kernel for short work: up to 28
+// an expert, or what leaves the one for long work fewer than about 160
+// workgroups (tiles of 64 rows, half of one left unfilled by each expert).
+// Short and long took, of experts of 2048 x 1024: Q4_0, 57 and 66 us for 24
+// slots of each of 64; Q8_0, 80 and 70 for 32; Q4_0, 24 and 45 for 96 of each of 8, 48
+// and 47 for 256, 56 and 49 for 350; MLPs of 8: 45 and 75 for 64 of each, 95
+// and 87 for 192; Q8_0 896 x 4864: 24 and 27 for 32 of each of 8, 34 and 29 for 64.
 inline std::size_t most_short(const Shape& s, bool gated) {
   const std::size_t columns = (s.tiles() + long_columns(gated) - 1) / long_columns(gated);
-  const std::size_t room = 256 / columns, left = s.count / 2;
-  return std::max(48 * s.count, room > left ? 64 * (room - left) : 0);
+  const std::size_t room = 160 / columns, left = s.count / 2;
+  return std::max(28 * s.count, room > left ? 64 * (room - left) : 0);
 }
-// Rows of an expert that a workgroup of a grouped product takes.
+// Rows of an expert that a workgroup of a grouped product takes: 16, 32 or, of
+// long work, 64.  16 and 32 took, of 8 Q4_0 experts of 2048 x 1024: 15.1 and
+// 17.2 us for 24 slots of each, 18.0 and 19.2 for 48, 27.1 and 24.1 for 96.
 inline std::size_t pick_rows(const Shape& s, std::size_t slots, bool gated) {
   if (slots > most_short(s, gated)) return 64;
-  return slots <= 16 * s.count ? 16 : 32;
+  return slots <= 48 * s.count ? 16 : 32;
 }
 constexpr std::size_t kLeastRows = 16, kMostShortRows = 32;
 
