@@ -351,7 +351,7 @@ int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids,
   LLMI_REQUIRE(why.empty(), "moe_matmul: " + why);
   hipStream_t s = pick(stream);
   per_row = std::min(per_row, slots);  // more than all slots mean the same row; the kernels have 32 bits for it
-  if (few_matmul(slots, per_row))
+  if (few_matmul(sh, slots, per_row))
     return launch_few(FewProduct{sh, experts->view(), {}, ids, slots, per_row, x, x_stride, y, y_stride, {}}, s);
   auto* w = static_cast<std::uint8_t*>(work);
   const std::size_t rows = pick_rows(sh, slots, false);

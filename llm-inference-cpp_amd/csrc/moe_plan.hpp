@@ -74,14 +74,18 @@ inline std::size_t pick_rows(const Shape& s, std::size_t slots, bool gated) {
 }
 constexpr std::size_t kLeastRows = 16, kMostShortRows = 32;
 
-// Up to this many slots (a wavefront's lanes) go without a grouping, where few
-// rows share an expert: products of up to 8 rows of x (8 rows of 2 experts of
-// 2048 x 1024: 8 us, grouped 14; 16 rows of 4 experts of 4096 x 4096: 88 and
-// 68), MLPs of up to 2 tokens (2 of 8 experts 2048 / 1024: 29 us, grouped 32;
-// 4 of them: 59 and 47).
-constexpr std::size_t kFewSlots = 64, kFewRows = 8, kFewTokens = 2;
-inline bool few_matmul(std::size_t slots, std::size_t per_row) {
-  return slots <= kFewSlots && rows_of(slots, per_row) <= kFewRows;
+// Up to this many slots (a wavefront's lanes) go without a grouping, a
+// workgroup for each slot and 32 outputs, of which only those of an expert's
+// first slot work.  Products of one or two rows of x, or of up to 16 where the
+// workgroups are few (4, 12, 16 and 32 rows of 2 of 8 Q4_0 experts of 2048 x
+// 1024: 7.2, 8.2, 9.9 and 14.6 us, grouped 12.3, 13.1, 13.0 and 13.5; 4, 8 and
+// 16 rows of 4 of 16 Q8_0 experts of 4096 x 4096: 49, 69 and 90, grouped 51, 64
+// and 68).  MLPs of up to 2 tokens (8 of 64 Q4_0 experts 2048 /
+// 1024: 28.7 us, grouped 30.9; 4 tokens 59 and 47).
+constexpr std::size_t kFewSlots = 64, kFewRows = 16, kFewGroups = 2048, kFewTokens = 2;
+inline bool few_matmul(const Shape& s, std::size_t slots, std::size_t per_row) {
+  const std::size_t rows = rows_of(slots, per_row);
+  return slots <= kFewSlots && (rows <= 2 || (rows <= kFewRows && slots * ((s.tiles() + 1) / 2) <= kFewGroups));
 }
 inline bool few_mlp(std::size_t tokens, std::size_t top_k) { return tokens * top_k <= kFewSlots && tokens <= kFewTokens; }
 

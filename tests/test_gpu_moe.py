@@ -142,6 +142,8 @@ MATMULS = [
     (H.Q4_0, 8, 1, 2, 576, 96, 2), (H.Q8_0, 8, 1, 8, 127, 64, 8), (H.Q4_0, 5, 7, 3, 129, 65, 3), (H.Q8_0, 5, 7, 3, 100, 130, 1),
     (H.Q4_0, 4, 40, 2, 256, 48, 2), (H.Q8_0, 64, 20, 8, 160, 32, 8), (H.Q4_0, 2, 100, 1, 97, 200, 1), (H.Q8_0, 2, 300, 2, 64, 33, 2),
     (H.Q4_0, 16, 130, 4, 320, 128, 4), (H.Q8_0, 13, 50, 3, 1000, 77, 3), (H.Q4_0, 300, 30, 6, 64, 16, 6),
+    # Several rows an expert without a grouping (twice 8 of them), and just too many for that.
+    (H.Q4_0, 3, 16, 2, 200, 70, 2), (H.Q8_0, 1, 16, 1, 130, 40, 1), (H.Q8_0, 1, 17, 1, 130, 40, 1), (H.Q4_0, 4, 6, 3, 64, 6000, 3),
     # Long work: more slots than the kernel for short work takes.
     (H.Q4_0, 8, 500, 2, 100, 4112, 2), (H.Q8_0, 8, 900, 1, 192, 4090, 1), (H.Q4_0, 2, 1300, 1, 33, 4100, 1), (H.Q8_0, 70, 1200, 3, 64, 2048, 3),
     # Each way of grouping: by every workgroup (above), by one, by several.
