@@ -450,17 +450,18 @@ int llmi_hip_experts_free(llmi_hip_experts* experts);
  * floats apart.  With a router's ids [tokens][top_k]: slots = tokens * top_k,
  * and per_row = top_k for x of one row a token, 1 for one a slot.  Slots whose
  * id is not 0 .. count - 1 (padding tokens, -1) leave their row of y as it was.
+ * per_row may be any number from 1 on (more than slots: one row for all).
  * Sums in fp32, x carried to 22 bits of each element (or 39 of its row's
  * largest); not llmi_hip_matmul_dev's order of additions, so not its bits.  A
  * row's result depends on that row, its expert and the call's sizes alone,
- * never on the order in which workgroups run.  inf or NaN in a row of x gives inf or NaN in
- * that row's results alone.
+ * never on the other rows or on the order in which workgroups run.  inf or NaN
+ * in a row of x gives inf or NaN in that row's results alone.
  * work: device memory of at least the bytes that _bytes gives, 16-byte
  * aligned; nothing has to be cleared, and nothing is kept in it from call to
  * call.  Calls that may run at the same time (two streams, two graphs) need a
  * workspace each; graphs that run one after the other may share one.
- * y must not overlap x.  LLMI_ERR_ARG: more than 2^24 slots, strides too short, y = x, a workspace too
- * small, NULL pointers. */
+ * y must not overlap x.  LLMI_ERR_ARG: more than 2^24 slots, strides too
+ * short, y = x, a workspace too small, NULL pointers. */
 int llmi_hip_moe_matmul_bytes(const llmi_hip_experts* experts, size_t slots, size_t per_row, size_t* bytes);
 int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids, size_t slots, size_t per_row,
                             const float* x, size_t x_stride, float* y, size_t y_stride, void* work, size_t work_bytes,
@@ -470,11 +471,14 @@ int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids,
  * with each token's own matrices):
  *   y[t] = residual[t] + sum over j < top_k of weights[t][j] *
  *          down_e( silu(gate_e x[t]) * (up_e x[t]) ),   e = ids[t][j]
- * the sum in the order of j, fp32.  gate and up of one shape and type, down of
- * either type.  x [tokens][in], residual (NULL: 0) and y [tokens][down's out],
- * rows their strides apart; y may be residual (with its stride) or x, where
- * they have the same rows.  A choice whose id is not an expert's adds nothing,
- * whatever its weight.  Everything else as for llmi_hip_moe_matmul_dev. */
+ * the sum in fp32, in the order of j (of up to two tokens in the order of the
+ * experts' first slots, inputs and experts in one sum, so that the other token's
+ * choices may change its last bits).  h = silu(..) * (..) is carried like x.
+ * gate and up of one shape and type, down of either type.  x [tokens][in],
+ * residual (NULL: 0) and y [tokens][down's out], rows their strides apart; y may
+ * be residual (with its stride) or x, where they have the same rows.  A choice
+ * whose id is not an expert's adds nothing, whatever its weight.  Everything
+ * else as for llmi_hip_moe_matmul_dev. */
 int llmi_hip_moe_mlp_bytes(const llmi_hip_experts* gate, const llmi_hip_experts* down, size_t tokens, size_t top_k,
                            size_t* bytes);
 int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* up, const llmi_hip_experts* down,

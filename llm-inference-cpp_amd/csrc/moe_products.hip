@@ -77,7 +77,14 @@ __device__ __forceinline__ void each(Fn&& fn) {
 // each other, 64 NT outputs (32 NT of each matrix of a gated pair).  The rows'
 // parts go through LDS, 64 inputs at a time in two buffers, filled while the
 // other one is used; the weights stay in the registers of the wavefront that
-// uses them.
+// uses them.  Bound by the vector units beside the matrix units: two matrix
+// instructions (32 clocks) have 4 additions (16), a quarter of a block's 10
+// conversions and the reads of LDS beside them.  32768 rows against Q4_0 pairs
+// of 2048 x 1024: 500 to 560 us by the card's clock, 1.0 to 1.1 PFLOP/s of matrix
+// instructions (a large fp16 library product reaches 1.37); back to 2048: 270 to
+// 300 us.  128 rows a workgroup halve the conversions but take the registers of
+// a third wavefront, and were no faster; chains of 32 x 32 x 16 instructions,
+// with a quarter of the scales' additions hidden, were slower.
 template <int TYPE, int MT, int NT, bool GATED>
 __global__ void __launch_bounds__(kThreads, TYPE == LLMI_TYPE_Q4_0 ? 2 : 3) long_kernel(ProductArgs p) {
   constexpr int kParts = MT * 4;  // 1 KiB pieces of a buffer: (16 rows, block, high / low)
@@ -152,9 +159,9 @@ __global__ void __launch_bounds__(kThreads, TYPE == LLMI_TYPE_Q4_0 ? 2 : 3) long
         if constexpr (TYPE == LLMI_TYPE_Q4_0) weights(w[1 - j], h + j + 1);
       }
       // Two outputs' tiles at a time: their four instructions, then the
-      // additions of the two before them, whose results are there by now.
-      // The regions keep the compiler from holding more operands at once
-      // than the registers have room for.
+      // additions of the two (Q8_0: the one) before them, whose results are
+      // there by now.  The regions keep the compiler from holding more operands
+      // at once than the registers have room for.
       f16x8 code[NT];
       f16x8 x[2][2];
       constexpr int kLag = TYPE == LLMI_TYPE_Q4_0 ? 2 : 1, kD = kLag + 1;
@@ -176,6 +183,9 @@ __global__ void __launch_bounds__(kThreads, TYPE == LLMI_TYPE_Q4_0 ? 2 : 3) long
       };
       each<kSteps>([&](auto step) {
         constexpr int q = decltype(step)::value, ib = q / kPairs, i = ib % MT, n0 = q % kPairs * 2, b2 = ib / MT;
+        // Q8_0's weights of the next step take the registers of this one's, whose
+        // second block has become fp16 by now: three wavefronts a SIMD instead of
+        // two (512 tokens, 2 of 8 experts, pairs of 896 x 4864: 56 -> 50 us).
         if constexpr (TYPE != LLMI_TYPE_Q4_0 && q == kSteps / 2) weights(w[1 - j], min(h + j + 1, p.steps - 1));
         if constexpr (n0 == 0 && ib + 1 < 2 * MT) {  // the next rows' parts
           x[(ib + 1) % 2][0] = xs[j][(ib + 1) % MT * 4 + (ib + 1) / MT * 2][read_at];
@@ -269,7 +279,13 @@ __global__ void __launch_bounds__(kThreads, TYPE == LLMI_TYPE_Q4_0 ? 2 : 3) long
 // workgroup takes 16 MT rows and 16 NT outputs (8 NT of each matrix of a
 // gated pair); its 4 wavefronts share the inputs, each with its own loads of
 // rows and weights in flight while it works on those before them, and their
-// sums meet in LDS, in their order.
+// sums meet in LDS, in their order.  Bound by the weights' way from memory and
+// its latency: 512 rows of 64 Q4_0 experts, pairs of 2048 x 1024 40 us at 4.2 TB/s
+// of weights, back to 2048 25 us at 3.4, Q8_0 2048 x 1024 28 us at 5.4 (out of the
+// last-level cache); vector units issue in 38 % of the clocks, matrix units are
+// busy in 17 %.  Wavefronts beside each other that share a ring of 4 steps of
+// rows in LDS halve the reads from L2 and were a tenth slower: a CU then has 2 or
+// 3 workgroups, where it has 9 of these.
 // BLOCKS: every block of a row of x has a factor of its own.
 template <int TYPE, int MT, int NT, bool GATED, bool BLOCKS>
 __global__ void __launch_bounds__(kThreads, MT == 1 ? 4 : 3) short_kernel(ProductArgs p) {

@@ -471,6 +471,40 @@ def test_matmul_one_row_for_all(per_row, slots, out):
     check_matmul(run_matmul(experts, ids, x, per_row), ids, x, per_row, values)
 
 
+@pytest.mark.parametrize("slots,out", [(12, 40), (150, 40), (1300, 4100)])
+@pytest.mark.parametrize("qtype", [H.Q4_0, H.Q8_0])
+def test_matmul_rows_apart(slots, out, qtype):
+    """A row's bits do not depend on what stands in the others, nor on their experts."""
+    rng = np.random.default_rng(58)
+    experts, _ = make(rng, qtype, 5, out, 100)
+    ids = rng.integers(0, 5, slots).astype(np.int32)
+    x = rng.standard_normal((slots, 100)).astype(np.float32)
+    keep = rng.permutation(slots)[:slots // 4]
+    first = run_matmul(experts, ids, x, 1)
+    others = np.setdiff1d(np.arange(slots), keep)
+    ids[others] = rng.integers(-1, 5, len(others))
+    x[others] = (rng.standard_normal((len(others), 100)) * 1e6).astype(np.float32)
+    x[others[::3]] = NAN
+    again = run_matmul(experts, ids, x, 1)
+    assert np.array_equal(first[keep].view(np.uint32), again[keep].view(np.uint32))
+
+
+@pytest.mark.parametrize("tokens,ffn", [(5, 96), (150, 96), (900, 2080)])
+def test_mlp_tokens_apart(tokens, ffn):
+    """Nor does a token's MLP, of three tokens or more."""
+    rng = np.random.default_rng(59)
+    layer = Layer(rng, H.Q4_0, H.Q8_0, 5, 64, ffn)
+    ids, weights = draw_ids(rng, tokens, 2, 5), rng.random((tokens, 2)).astype(np.float32)
+    x = rng.standard_normal((tokens, 64)).astype(np.float32)
+    keep = rng.permutation(tokens)[:(tokens + 3) // 4]
+    first = layer.run(ids, weights, x)
+    others = np.setdiff1d(np.arange(tokens), keep)
+    ids[others], weights[others] = draw_ids(rng, len(others), 2, 5, 0.3), INF
+    x[others] = (rng.standard_normal((len(others), 64)) * 1e6).astype(np.float32)
+    again = layer.run(ids, weights, x)
+    assert np.array_equal(first[keep].view(np.uint32), again[keep].view(np.uint32))
+
+
 def test_two_streams_at_once():
     """Calls on two streams of the caller's, with a workspace each: the results of each alone."""
     create = H.load().hipStreamCreateWithFlags  # found through the library's own dependencies
