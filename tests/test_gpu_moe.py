@@ -192,6 +192,24 @@ def test_matmul_extremes(qtype, tokens):
         assert np.all(np.abs(y[s] - want) <= bound + 1e-38), s
 
 
+@pytest.mark.parametrize("qtype", [H.Q4_0, H.Q8_0])
+@pytest.mark.parametrize("slots,out", [(3, 40), (150, 40), (1300, 4100)])
+@pytest.mark.parametrize("small", [-8, -14, -18, -24, -32])
+def test_matmul_small_beside_large(qtype, slots, out, small):
+    """Elements 2^small of their row's largest, which a weight of 0 takes out: what is left of them shows."""
+    rng = np.random.default_rng(60)
+    count, n_in = 3, 100
+    data, scales, values = R.matrices(rng, qtype, count, out, n_in)
+    data[..., 0] = 0 if qtype == H.Q8_0 else (data[..., 0] & 0xF0) | 8
+    values[..., 0] = 0
+    d, s = dev(data), dev(scales)
+    experts = H.Experts.upload_dev(d.ptr, s.ptr, count, out, n_in, qtype)
+    ids = rng.integers(0, count, slots).astype(np.int32)
+    x = (rng.standard_normal((slots, n_in)) * 2.0**small).astype(np.float32)
+    x[:, 0] = 1.5
+    check_matmul(run_matmul(experts, ids, x, 1), ids, x, 1, values)
+
+
 @pytest.mark.parametrize("tokens", [1, 5, 80])
 def test_matmul_nonfinite_rows(tokens):
     """inf and NaN stay in their rows; a row with an inf keeps the signs of the products that decide."""
