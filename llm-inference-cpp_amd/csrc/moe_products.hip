@@ -128,9 +128,9 @@ __global__ void __launch_bounds__(kThreads, TYPE == LLMI_TYPE_Q4_0 ? 2 : 3) long
       if (MT % kWaves == 0 || wave * kOwn + i < MT) {
         const std::uint32_t to = lds + ((buf * MT + wave * kOwn + i) * 4) * 1024;
         to_lds<0>(src[i], to);
-        to_lds<64>(src[i], to + 1024);
-        to_lds<128>(src[i], to + 2048);
-        to_lds<192>(src[i], to + 3072);
+        to_lds<64>(src[i], to + 1 * 1024);
+        to_lds<128>(src[i], to + 2 * 1024);
+        to_lds<192>(src[i], to + 3 * 1024);
         src[i] += 256;
       }
   };
