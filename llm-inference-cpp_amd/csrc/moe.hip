@@ -362,7 +362,7 @@ int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids,
   const std::size_t rows = pick_rows(sh, slots, false);
   const Groups g = groups_at(w, l.group, rows, rows);
   const SplitRows xs = parts_at(w, l.x);
-  const RowSource src{x, x_stride, sh.in, sh.steps(), per_row};
+  const RowSource src{x, x_stride, sh.in, sh.steps(), static_cast<std::uint32_t>(per_row)};
   if (int rc = launch_prepare(ids, slots, sh.count, g, src, xs, s)) return rc;
   return launch_product(Product{sh, experts->view(), {}, xs, g, 0, slots, per_row, false, y, y_stride, {}, 0, false}, s);
 }
@@ -408,7 +408,7 @@ int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* u
     if (int rc = launch_few(FewProduct{gs, gate->view(), up->view(), ids, slots, top_k, x, x_stride, nullptr, 0, parts}, s)) return rc;
     return launch_few_sum(FewSum{ds, down->view(), ids, weights, tokens, top_k, parts, residual, residual_stride, y, y_stride, sums}, s);
   }
-  const RowSource src{x, x_stride, gs.in, gs.steps(), top_k}, h_src{h, ds.in, ds.in, ds.steps(), 0};
+  const RowSource src{x, x_stride, gs.in, gs.steps(), static_cast<std::uint32_t>(top_k)}, h_src{h, ds.in, ds.in, ds.steps(), 0};
   if (int rc = launch_prepare(ids, slots, gs.count, g, src, xs, s)) return rc;
   // The results between the products: for short work in its row tiles at once,
   // else as fp32 rows, whose parts need each whole row's largest.

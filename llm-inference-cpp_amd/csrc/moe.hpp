@@ -29,7 +29,7 @@ struct Groups {
   std::int32_t* counts;  // slots that have an expert, row tiles of both lists
   std::int32_t* order;   // slots, those of expert 0 first
   RowTile* tiles[2];     // of rows[0] and rows[1] rows each
-  int rows[2];
+  int rows[2];           // powers of two
   std::int32_t* hist;    // [grouping_blocks][expert], of more than kOneGroup slots
 };
 
@@ -52,7 +52,7 @@ struct SplitRows {
 struct RowSource {
   const float* x;
   std::size_t stride, in, steps;
-  std::size_t per_row;
+  std::uint32_t per_row;
 };
 // Groups the slots, and brings x into the layout that list 0's product takes.
 int launch_prepare(const std::int32_t* ids, std::size_t slots, std::size_t experts, const Groups& g, const RowSource& x,

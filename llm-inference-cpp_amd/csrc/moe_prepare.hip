@@ -94,7 +94,7 @@ __device__ __forceinline__ void split_row(const RowSource& src, std::size_t from
   store_row<MT>(x, src, r, to);
 }
 __device__ __forceinline__ std::size_t row_of(const RowSource& src, int pos, int slot) {
-  return src.per_row > 0 ? static_cast<std::size_t>(slot) / src.per_row : static_cast<std::size_t>(pos);
+  return src.per_row > 0 ? static_cast<std::uint32_t>(slot) / src.per_row : static_cast<std::uint32_t>(pos);
 }
 
 // Rows as they are.  Bound by memory: 32768 rows of 1024 in 47.6 us, 5.6 TB/s.
@@ -128,12 +128,12 @@ constexpr int kGroupThreads = 1024;
 template <typename Fn>
 __device__ __forceinline__ void lay_ranges(std::int32_t* count, int experts, const Groups& g, std::int32_t (&total)[3], Fn&& tile) {
   __shared__ std::int32_t waves[3][kGroupThreads / 64];
-  const int t = threadIdx.x, lane = t & 63;
+  const int t = threadIdx.x, lane = t & 63, shift0 = __builtin_ctz(g.rows[0]), shift1 = __builtin_ctz(g.rows[1]);
   total[0] = total[1] = total[2] = 0;
   for (int e0 = 0; e0 < experts; e0 += kGroupThreads) {
     const int e = e0 + t;
     const std::int32_t n = e < experts ? count[e] : 0;
-    const std::int32_t own[3] = {n, (n + g.rows[0] - 1) / g.rows[0], (n + g.rows[1] - 1) / g.rows[1]};
+    const std::int32_t own[3] = {n, (n + g.rows[0] - 1) >> shift0, (n + g.rows[1] - 1) >> shift1};
     std::int32_t at[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
@@ -161,7 +161,7 @@ __device__ __forceinline__ void lay_ranges(std::int32_t* count, int experts, con
       for (int l = 0; l < 2; ++l)
         for (std::int32_t i = 0; i < own[1 + l]; ++i)
           tile(l, at[1 + l] + i,
-               RowTile{e, at[0] + i * g.rows[l], min(n - i * g.rows[l], g.rows[l]), at[2] + i * (g.rows[0] / g.rows[1])});
+               RowTile{e, at[0] + i * g.rows[l], min(n - i * g.rows[l], g.rows[l]), at[2] + ((i << shift0) >> shift1)});
     }
     __syncthreads();
   }
@@ -275,12 +275,12 @@ __global__ void __launch_bounds__(kThreads) self_kernel(const std::int32_t* __re
   __syncthreads();
   if (slot >= slots) return;
   const auto add = [](std::uint32_t a, std::uint32_t b) { return a + b; };
+  const int shift0 = __builtin_ctz(g.rows[0]), shift1 = __builtin_ctz(g.rows[1]);
   std::uint32_t word[kEach], sum = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const std::uint32_t n = static_cast<std::uint32_t>(count[i * 64 + lane]);
-    const auto groups = [&](int l) { return (n + static_cast<std::uint32_t>(g.rows[l]) - 1) / static_cast<std::uint32_t>(g.rows[l]); };
-    word[i] = n | groups(0) << kAt1 | groups(1) << kAt2;
+    word[i] = n | (n + g.rows[0] - 1) >> shift0 << kAt1 | (n + g.rows[1] - 1) >> shift1 << kAt2;
     sum += word[i];
   }
   const auto part = [](std::uint32_t w, int i) {
@@ -303,11 +303,11 @@ __global__ void __launch_bounds__(kThreads) self_kernel(const std::int32_t* __re
     rank += __builtin_popcountll(__ballot(i < slot && all[i] == e));
   }
   const int r0 = g.rows[0], r1 = g.rows[1], n = count[e], first = part(before, 0) + rank;
-  const int tile0 = part(before, 1) + rank / r0, tile1 = part(before, 2) + rank / r1;
+  const int tile0 = part(before, 1) + (rank >> shift0), tile1 = part(before, 2) + (rank >> shift1);
   if (lane == 0) {
     g.order[first] = slot;
-    if (rank % r0 == 0) g.tiles[0][tile0] = RowTile{e, first, min(n - rank, r0), tile1};
-    if (rank % r1 == 0) g.tiles[1][tile1] = RowTile{e, first, min(n - rank, r1), 0};
+    if ((rank & (r0 - 1)) == 0) g.tiles[0][tile0] = RowTile{e, first, min(n - rank, r0), tile1};
+    if ((rank & (r1 - 1)) == 0) g.tiles[1][tile1] = RowTile{e, first, min(n - rank, r1), 0};
   }
   store_row<MT>(x, src, tile0 * (MT * kTile) + rank % (MT * kTile), to);
 }
