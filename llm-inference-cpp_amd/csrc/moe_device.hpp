@@ -89,13 +89,6 @@ struct Weights {
     s[0] = v[0];
     s[1] = v[1];
   }
-  // For the compiler: the loads are complete.
-  __device__ __forceinline__ void here() {
-#pragma unroll
-    for (std::uint32_t& v : c) asm volatile("" : "+v"(v));
-#pragma unroll
-    for (float& v : s) asm volatile("" : "+v"(v));
-  }
   __device__ __forceinline__ f16x8 codes(int b) const {
     if constexpr (TYPE == LLMI_TYPE_Q4_0) return codes_q4(c[b]);
     else return codes_q8(c[2 * b], c[2 * b + 1]);

@@ -55,10 +55,15 @@ __device__ __forceinline__ void store_parts(const ProductArgs& p, int tile, int 
 
 // 16 bytes of each lane, OFFSET behind its own address, into LDS, lane after
 // lane from `to` (common to the wavefront).  Nothing waits for it but landed().
-// The instruction adds its offset to both addresses.
+// The instruction adds its offset to both addresses; between a write of m0 and
+// such a load this family needs one wait state, which nobody inserts in here.
 template <int OFFSET>
 __device__ __forceinline__ void to_lds(const std::uint8_t* from, std::uint32_t to) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(from), "s"(to - OFFSET), "n"(OFFSET) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(from), "s"(to - OFFSET), "n"(OFFSET) : "memory");
+}
+// The same from an address common to the wavefront and each lane's offset.
+__device__ __forceinline__ void to_lds_from(GlobalBytes from, std::uint32_t offset, std::uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "s"(to) : "memory");
 }
 // All of this wavefront's loads have landed and its reads of LDS are done;
 // then those of the workgroup's.
@@ -76,19 +81,29 @@ __device__ __forceinline__ void each(Fn&& fn) {
 // A workgroup takes 16 MT rows of one expert and, with its 4 wavefronts beside
 // each other, 64 NT outputs (32 NT of each matrix of a gated pair).  The rows'
 // parts go through LDS, 64 inputs at a time in two buffers, filled while the
-// other one is used; the weights stay in the registers of the wavefront that
-// uses them.  Bound by the vector units beside the matrix units: two matrix
-// instructions (32 clocks) have 4 additions (16), a quarter of a block's 10
-// conversions and the reads of LDS beside them.  32768 rows against Q4_0 pairs
-// of 2048 x 1024: 500 to 560 us by the card's clock, 1.0 to 1.1 PFLOP/s of matrix
-// instructions (a large fp16 library product reaches 1.37); back to 2048: 270 to
-// 300 us.  128 rows a workgroup halve the conversions but take the registers of
-// a third wavefront, and were no faster; chains of 32 x 32 x 16 instructions,
-// with a quarter of the scales' additions hidden, were slower.
+// other one is used.  A wavefront's weights come through LDS of its own, a step
+// (Q8_0) or two (Q4_0) ahead, and are taken into registers in the middle of the
+// step before theirs: asked for into registers instead, they were half as long
+// on their way or left room for two wavefronts a SIMD (4096 rows against 16
+// Q4_0 experts of 896 x 4864: 85 -> 80 us).  Bound by the vector units beside
+// the matrix units, and by power: two matrix instructions (32 clocks) have 4
+// additions (16), a quarter of a block's 10 conversions and the reads of LDS
+// beside them.  32768 rows against Q4_0 pairs of 2048 x 1024: 480 to 550 us by
+// the card's clock, 1.0 to 1.1 PFLOP/s of matrix instructions (a large fp16
+// library product reaches 1.37); back to 2048: 255 to 290 us.  128 rows a
+// workgroup halve the conversions but take the registers of a third wavefront,
+// and were no faster; chains of 32 x 32 x 16 instructions, with a quarter of the
+// scales' additions hidden, were slower.
 template <int TYPE, int MT, int NT, bool GATED>
-__global__ void __launch_bounds__(kThreads, TYPE == LLMI_TYPE_Q4_0 ? 2 : 3) long_kernel(ProductArgs p) {
+__global__ void __launch_bounds__(kThreads, 3) long_kernel(ProductArgs p) {
+  static_assert(MT == kWaves && NT == 4);
   constexpr int kParts = MT * 4;  // 1 KiB pieces of a buffer: (16 rows, block, high / low)
+  constexpr int kCodes = static_cast<int>(code_bytes(TYPE)), kScales = static_cast<int>(kStepScales) * 4;
+  // Steps of weights on their way at once, as three workgroups' LDS has room;
+  // a wavefront's loads of a step of rows and of weights.
+  constexpr int kAhead = TYPE == LLMI_TYPE_Q4_0 ? 2 : 1, kRowLoads = 4, kLoads = TYPE == LLMI_TYPE_Q4_0 ? 4 : 6;
   __shared__ __attribute__((aligned(16))) f16x8 xs[2][kParts][64];
+  __shared__ __attribute__((aligned(16))) std::uint8_t ws[kWaves][kAhead][NT * (kCodes + kScales)];  // a wavefront's: codes, then scales
   __shared__ std::int32_t to_row[MT * kTile];  // y's rows, and the factors of x's
   __shared__ float back[MT * kTile];
   constexpr int kCols = GATED ? NT / 2 : NT;
@@ -109,65 +124,94 @@ __global__ void __launch_bounds__(kThreads, TYPE == LLMI_TYPE_Q4_0 ? 2 : 3) long
     to_row[threadIdx.x] = p.y_by_position ? pos : p.g.order[pos];
     back[threadIdx.x] = p.x.factors[x_row(pos)];
   }
-  // The rows that this lane brings in: row lane / 4 of each of the wavefront's
-  // tiles of 16, so that 4 lanes read 64 bytes beside each other.  In LDS a
-  // row's four 16 bytes lie side by side, in an order that differs from 4 rows
-  // to the next: lanes that read one input group of 16 rows use all banks.
-  constexpr int kOwn = (MT + kWaves - 1) / kWaves;
-  const std::uint8_t* src[kOwn];
-#pragma unroll
-  for (int i = 0; i < kOwn; ++i) {
-    const int pos = first + min((wave * kOwn + i) * kTile + lane / 4, rows - 1);
-    src[i] = reinterpret_cast<const std::uint8_t*>(p.x.values) + static_cast<std::size_t>(x_row(pos)) * p.steps * (kStep * 4) + (lane % 4 ^ (4 - lane / 16) % 4) * 16;
-  }
+  // The rows that this lane brings in: row lane / 4 of the wavefront's tile of
+  // 16, so that 4 lanes read 64 bytes beside each other.  In LDS a row's four 16
+  // bytes lie side by side, in an order that differs from 4 rows to the next:
+  // lanes that read one input group of 16 rows use all banks.
+  const std::uint8_t* src = reinterpret_cast<const std::uint8_t*>(p.x.values) +
+                            static_cast<std::size_t>(x_row(first + min(wave * kTile + lane / 4, rows - 1))) * p.steps * (kStep * 4) +
+                            (lane % 4 ^ (4 - lane / 16) % 4) * 16;
   const int read_at = lane % kTile * 4 + (lane / kTile ^ (4 - lane % kTile / 4) % 4);
   const std::uint32_t lds = static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>(&xs[0][0][0]));
   const auto bring = [&](int buf) {  // the next 64 inputs
+    const std::uint32_t to = lds + (buf * kParts + wave * 4) * 1024;
+    to_lds<0>(src, to);
+    to_lds<64>(src, to + 1 * 1024);
+    to_lds<128>(src, to + 2 * 1024);
+    to_lds<192>(src, to + 3 * 1024);
+    src += 256;
+  };
+  // Weights, two tiles of a matrix at a time: their codes, then their scales.
+  GlobalBytes at[NT / 2];
+  std::uint32_t apart[NT / 2];  // from the first tile to the second
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i)
-      if (MT % kWaves == 0 || wave * kOwn + i < MT) {
-        const std::uint32_t to = lds + ((buf * MT + wave * kOwn + i) * 4) * 1024;
-        to_lds<0>(src[i], to);
-        to_lds<64>(src[i], to + 1 * 1024);
-        to_lds<128>(src[i], to + 2 * 1024);
-        to_lds<192>(src[i], to + 3 * 1024);
-        src[i] += 256;
+  for (int n = 0; n < NT; n += 2) {
+    const int col = min(col0 + n % kCols, p.tiles - 1);
+    at[n / 2] = tile_at<TYPE>(n < kCols ? p.m : p.up, static_cast<std::size_t>(expert) * p.tiles + col, p.steps);
+    apart[n / 2] = (min(col0 + n % kCols + 1, p.tiles - 1) - col) * static_cast<std::uint32_t>(p.steps) * static_cast<std::uint32_t>(step_bytes(TYPE));
+  }
+  const std::uint32_t lds_w = static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>(&ws[0][0][0])) + wave * kAhead * NT * (kCodes + kScales);
+  const auto bring_weights = [&](int buf, int step) {
+    const std::uint32_t to = lds_w + buf * (NT * (kCodes + kScales));
+#pragma unroll
+    for (int n = 0; n < NT; n += 2) {
+      const GlobalBytes from = at[n / 2] + static_cast<std::uint32_t>(step) * static_cast<std::uint32_t>(step_bytes(TYPE));
+      if constexpr (TYPE == LLMI_TYPE_Q4_0) {
+        to_lds_from(from, lane / 32 * apart[n / 2] + lane % 32 * 16, to + n * kCodes);
+      } else {
+        to_lds_from(from, lane * 16, to + n * kCodes);
+        to_lds_from(from, apart[n / 2] + lane * 16, to + (n + 1) * kCodes);
       }
+      if (lane < 16) to_lds_from(from, lane / 8 * apart[n / 2] + kCodes + lane % 8 * 16, to + NT * kCodes + n * kScales);
+    }
   };
-  GlobalBytes at[NT];
+  std::uint32_t raw[NT][kCodes / 256];
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef std::uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  f32x2 scale[2][NT];
+  const auto take = [&](int buf, f32x2 (&s)[NT]) {
+    const std::uint8_t* const from = &ws[wave][buf][0];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-    at[n] = tile_at<TYPE>(n < kCols ? p.m : p.up, static_cast<std::size_t>(expert) * p.tiles + min(col0 + n % kCols, p.tiles - 1), p.steps);
-  Weights<TYPE> w[2][NT];
-  LaneAt lane_at(lane);
-  const auto weights = [&](Weights<TYPE> (&to)[NT], int step) {
+    for (int n = 0; n < NT; ++n) {
+      if constexpr (TYPE == LLMI_TYPE_Q4_0) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(from + n * kCodes + lane * 8);
+        raw[n][0] = v[0];
+        raw[n][1] = v[1];
+      } else {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(from + n * kCodes + lane * 16);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) to[n].load(at[n], step, lane_at);
+        for (int i = 0; i < 4; ++i) raw[n][i] = v[i];
+      }
+      s[n] = *reinterpret_cast<const f32x2*>(from + NT * kCodes + n * kScales + lane % kTile * 8);
+    }
   };
+  const auto codes = [&](int n, int block) {
+    if constexpr (TYPE == LLMI_TYPE_Q4_0) return codes_q4(raw[n][block]);
+    else return codes_q8(raw[n][2 * block], raw[n][2 * block + 1]);
+  };
+  const int last = p.steps - 1;
   f32x4 acc[NT][MT] = {};
   bring(0);
-  weights(w[0], 0);
-  landed();
 #pragma unroll
-  for (int n = 0; n < NT; ++n) w[0][n].here();
+  for (int i = 0; i < kAhead; ++i) bring_weights(i, min(i, last));
+  landed();
+  take(0, scale[0]);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  bring_weights(0, min(kAhead, last));
   for (int h = 0; h < p.steps; h += 2) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       if (h + j >= p.steps) break;
-      if (h + j + 1 < p.steps) {
-        bring(1 - j);
-        if constexpr (TYPE == LLMI_TYPE_Q4_0) weights(w[1 - j], h + j + 1);
-      }
-      // Two outputs' tiles at a time: their four instructions, then the
-      // additions of the two (Q8_0: the one) before them, whose results are
-      // there by now.  The regions keep the compiler from holding more operands
-      // at once than the registers have room for.
+      if (h + j < last) bring(1 - j);
+      // Two outputs' tiles at a time: their four instructions, beside them the
+      // additions of the two before, whose results are there by now.  The
+      // regions keep the compiler from holding more operands at once than the
+      // registers have room for.
       f16x8 code[NT];
       f16x8 x[2][2];
-      constexpr int kLag = TYPE == LLMI_TYPE_Q4_0 ? 2 : 1, kD = kLag + 1;
-      f32x4 d[kD][2];
+      f32x4 d[2][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) code[n] = w[j][n].codes(0);
+      for (int n = 0; n < NT; ++n) code[n] = codes(n, 0);
       x[0][0] = xs[j][0][read_at];
       x[0][1] = xs[j][1][read_at];
       constexpr int kPairs = NT / 2, kSteps = 2 * MT * kPairs;
@@ -176,29 +220,36 @@ __global__ void __launch_bounds__(kThreads, TYPE == LLMI_TYPE_Q4_0 ? 2 : 3) long
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[n0 + n][i][r] = __builtin_fmaf(d[q % kD][n][r], w[j][n0 + n].s[b2], acc[n0 + n][i][r]);
+          for (int r = 0; r < 4; ++r) acc[n0 + n][i][r] = __builtin_fmaf(d[q % 2][n][r], scale[j][n0 + n][b2], acc[n0 + n][i][r]);
         // Here, not at the end of the block, where the compiler would put them all.
 #pragma unroll
         for (int n = 0; n < 2; ++n) asm volatile("" : "+v"(acc[n0 + n][i]));
       };
       each<kSteps>([&](auto step) {
         constexpr int q = decltype(step)::value, ib = q / kPairs, i = ib % MT, n0 = q % kPairs * 2, b2 = ib / MT;
-        // Q8_0's weights of the next step take the registers of this one's, whose
-        // second block has become fp16 by now: three wavefronts a SIMD instead of
-        // two (512 tokens, 2 of 8 experts, pairs of 896 x 4864: 56 -> 50 us).
-        if constexpr (TYPE != LLMI_TYPE_Q4_0 && q == kSteps / 2) weights(w[1 - j], min(h + j + 1, p.steps - 1));
+        // The next step's weights, whose registers are free: this step's second
+        // block has become fp16.  Loads come back in order; younger than these
+        // weights are the next rows (and, of Q4_0, the weights after them).
+        if constexpr (q == kSteps / 2) {
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kRowLoads + (kAhead - 1) * kLoads) : "memory");
+          take((j + 1) % kAhead, scale[1 - j]);
+        }
+        if constexpr (q == kSteps / 2 + 2) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          bring_weights((j + 1) % kAhead, min(h + j + 1 + kAhead, last));
+        }
         if constexpr (n0 == 0 && ib + 1 < 2 * MT) {  // the next rows' parts
           x[(ib + 1) % 2][0] = xs[j][(ib + 1) % MT * 4 + (ib + 1) / MT * 2][read_at];
           x[(ib + 1) % 2][1] = xs[j][(ib + 1) % MT * 4 + (ib + 1) / MT * 2 + 1][read_at];
         }
 #pragma unroll
-        for (int n = 0; n < 2; ++n) d[q % kD][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ib % 2][0], code[n0 + n], f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+        for (int n = 0; n < 2; ++n) d[q % 2][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ib % 2][0], code[n0 + n], f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) d[q % kD][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ib % 2][1], code[n0 + n], d[q % kD][n], 0, 0, 0);
-        if constexpr (q >= kLag) add(std::integral_constant<int, q - kLag>{});
+        for (int n = 0; n < 2; ++n) d[q % 2][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ib % 2][1], code[n0 + n], d[q % 2][n], 0, 0, 0);
+        if constexpr (q > 0) add(std::integral_constant<int, q - 1>{});
         if constexpr (b2 == 0 && i == MT - 1) {  // the next block's codes
 #pragma unroll
-          for (int n = 0; n < 2; ++n) code[n0 + n] = w[j][n0 + n].codes(1);
+          for (int n = 0; n < 2; ++n) code[n0 + n] = codes(n0 + n, 1);
         }
 #pragma unroll
         for (int i2 = 0; i2 < 4; ++i2) {
@@ -207,13 +258,12 @@ __global__ void __launch_bounds__(kThreads, TYPE == LLMI_TYPE_Q4_0 ? 2 : 3) long
         }
         __builtin_amdgcn_sched_barrier(0);
       });
-      if constexpr (kLag > 1) add(std::integral_constant<int, kSteps - 2>{});
       add(std::integral_constant<int, kSteps - 1>{});
-      landed();
-#pragma unroll
-      for (int n = 0; n < NT; ++n) w[1 - j][n].here();
+      // The next rows have landed (only weights are younger), and all have read these.
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads) : "memory");
     }
   }
+  landed();  // nothing is on its way into LDS any more
   if constexpr (GATED) {
     if (p.h.values != nullptr) {
       // The wavefront's outputs of a row are one block (kCols is 2).  16 rows at
