@@ -398,7 +398,8 @@ int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* u
   hipStream_t s = pick(stream);
   auto* w = static_cast<std::uint8_t*>(work);
   const std::size_t slots = tokens * top_k;
-  const Groups g = groups_at(w, l.group, pick_rows(gs, slots, true), pick_rows(ds, slots, false));
+  const MlpRows rows = pick_mlp_rows(gs, ds, slots);
+  const Groups g = groups_at(w, l.group, rows.first, rows.second);
   const SplitRows xs = parts_at(w, l.x), hs = parts_at(w, l.h_parts);
   auto* h = reinterpret_cast<float*>(w + l.h);
   auto* sums = reinterpret_cast<float*>(w + l.sums);

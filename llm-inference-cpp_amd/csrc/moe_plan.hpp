@@ -66,11 +66,24 @@ inline std::size_t most_short(const Shape& s, bool gated) {
   return std::max(28 * s.count, room > left ? 64 * (room - left) : 0);
 }
 // Rows of an expert that a workgroup of a grouped product takes: 16, 32 or, of
-// long work, 64.  16 and 32 took, of 8 Q4_0 experts of 2048 x 1024: 15.1 and
-// 17.2 us for 24 slots of each, 18.0 and 19.2 for 48, 27.1 and 24.1 for 96.
+// long work, 64; 16 up to 48 slots an expert, or where 32 would leave fewer than
+// about 400 workgroups.  16 and 32 took, of 8 Q4_0 experts of 2048 x 1024: 15.1
+// and 17.2 us for 24 slots of each, 18.0 and 19.2 for 48, 27.1 and 24.1 for 96 (448
+// workgroups); of 8 Q8_0 experts of 4864 x 896: 44 and 51 for 64 (280
+// workgroups), 70 and 67 for 128 (504).
 inline std::size_t pick_rows(const Shape& s, std::size_t slots, bool gated) {
   if (slots > most_short(s, gated)) return 64;
-  return slots <= 48 * s.count ? 16 : 32;
+  const std::size_t columns = (s.tiles() + short_columns(gated) - 1) / short_columns(gated);
+  return slots <= 48 * s.count || (slots / 32 + s.count / 2) * columns < 400 ? 16 : 32;
+}
+// Of the two products of an MLP.  The first one writes the row tiles of a short
+// second one, whose groups are as large as its own or parts of them.
+struct MlpRows {
+  std::size_t first, second;
+};
+inline MlpRows pick_mlp_rows(const Shape& gate, const Shape& down, std::size_t slots) {
+  const std::size_t a = pick_rows(gate, slots, true), b = pick_rows(down, slots, false);
+  return {a, b <= 32 ? std::min(a, b) : b};
 }
 constexpr std::size_t kLeastRows = 16, kMostShortRows = 32;
 

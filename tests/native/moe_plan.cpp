@@ -77,8 +77,7 @@ int main() {
   }
   // Also over the sizes at which the kernels and the grouping change, and
   // whatever such a call takes of each region is there.
-  const auto takes = [&](const Parts& x, const Shape& s, std::size_t slots, std::size_t rows, bool gated, bool blocks) {
-    const std::size_t r = pick_rows(s, slots, gated);
+  const auto takes = [&](const Parts& x, const Shape& s, std::size_t slots, std::size_t rows, std::size_t r, bool blocks) {
     const std::size_t n = r <= kMostShortRows ? most_tiles(slots, s.count, r) * r : rows;
     const std::size_t factors = r <= kMostShortRows && blocks ? n * s.steps() * 2 : n;
     return x.values % 256 == 0 && x.values + n * s.steps() * kStep * 4 <= x.factors && factors * 4 <= SIZE_MAX - x.factors ? x.factors + factors * 4 : SIZE_MAX;
@@ -95,7 +94,7 @@ int main() {
           expect(m.all.bytes >= before, "workspace shrinks", count, slots);
           expect(rows_of(slots, per_row) >= 1 && rows_of(slots, per_row) <= slots, "rows", slots, per_row);
           expect(m.group.tiles[1] + most_tiles(slots, count, 16) * 16 <= m.x.values, "groups end", count, slots);
-          expect(takes(m.x, a, slots, rows_of(slots, per_row), false, false) <= m.all.bytes, "rows end", count, slots);
+          expect(takes(m.x, a, slots, rows_of(slots, per_row), pick_rows(a, slots, false), false) <= m.all.bytes, "rows end", count, slots);
           before = m.all.bytes;
         }
       }
@@ -104,18 +103,20 @@ int main() {
         for (std::size_t tokens : turns) {
           const MlpLayout m(a, b, tokens, top_k);
           const std::size_t slots = tokens * top_k;
+          const MlpRows rows = pick_mlp_rows(a, b, slots);
           expect(m.all.bytes >= before, "workspace shrinks", count, tokens);
-          expect(takes(m.x, a, slots, tokens, true, false) <= m.h, "rows end", count, tokens);
-          expect(takes(m.h_parts, b, slots, slots, false, true) <= m.sums, "results end", count, tokens);
+          expect(takes(m.x, a, slots, tokens, rows.first, false) <= m.h, "rows end", count, tokens);
+          expect(takes(m.h_parts, b, slots, slots, rows.second, true) <= m.sums, "results end", count, tokens);
           expect(m.sums + slots * b.out * 4 <= m.all.bytes, "sums end", count, tokens);
-          if (pick_rows(b, slots, false) > kMostShortRows) expect(m.h + slots * a.out * 4 <= m.h_parts.values, "fp32 results end", count, tokens);
+          if (rows.second > kMostShortRows) expect(m.h + slots * a.out * 4 <= m.h_parts.values, "fp32 results end", count, tokens);
           if (few_mlp(tokens, top_k)) {
             const std::size_t n = slots * few_blocks(b);
             expect(m.few_factors >= n * 128 && m.h + m.few_factors + n * 4 <= m.h_parts.values, "few results end", count, tokens);
             expect(m.sums + few_splits(b) * tokens * b.out * 4 <= m.all.bytes, "few sums end", count, tokens);
           }
           // The first product writes row tiles that the second list's groups have.
-          if (pick_rows(b, slots, false) <= kMostShortRows) expect(pick_rows(a, slots, true) >= pick_rows(b, slots, false), "groups of the lists", count, tokens);
+          if (rows.second <= kMostShortRows) expect(rows.first % rows.second == 0, "groups of the lists", count, tokens);
+          expect(rows.first == pick_rows(a, slots, true), "first product's rows", count, tokens);
         }
       }
     }
