@@ -3,7 +3,7 @@
 // matrix waits for, so what counts is the number of launches and of waits in a
 // row: one launch up to 4096 slots, where rows go as they are or every
 // wavefront finds its place by itself (512 slots of 64 experts with rows of
-// 2048: 7.8 us; 1024 slots, 512 rows of 896: 5.4 us), two for more (32768 slots,
+// 2048: 7.5 us; 1024 slots, 512 rows of 896: 5.4 us), two for more (32768 slots,
 // 4096 rows of 2048: 16.1 and 10.3 us, the counts' way through memory in both).
 #include "moe_device.hpp"
 
