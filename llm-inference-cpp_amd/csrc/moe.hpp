@@ -19,12 +19,14 @@ struct Matrices {
   const std::uint8_t* steps = nullptr;
 };
 
-// A group of rows of one expert: positions first .. first + rows - 1 of the
-// order.  next: where the second list's groups are as large or smaller, the one
-// of this group's first row.
+// An entry of a list of groups of rows, the same for all groups of an expert: its
+// positions are begin .. begin + slots - 1 of the order, its groups the list's
+// group0 .. group0 + groups - 1, each but the last one full.  next0: where the
+// second list's groups are as large or smaller, the expert's first one there.
 struct RowTile {
-  std::int32_t expert, first, rows, next;
+  std::int32_t expert, begin, slots, group0, groups, next0, unused[2];
 };
+static_assert(sizeof(RowTile) == kRowTileBytes);
 struct Groups {
   std::int32_t* counts;  // slots that have an expert, row tiles of both lists
   std::int32_t* order;   // slots, those of expert 0 first

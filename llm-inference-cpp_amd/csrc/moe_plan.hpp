@@ -85,6 +85,7 @@ inline MlpRows pick_mlp_rows(const Shape& gate, const Shape& down, std::size_t s
   const std::size_t a = pick_rows(gate, slots, true), b = pick_rows(down, slots, false);
   return {a, b <= 32 ? std::min(a, b) : b};
 }
+constexpr std::size_t kRowTileBytes = 32;  // a group of rows in a list
 constexpr std::size_t kLeastRows = 16, kMostShortRows = 32;
 
 // Up to this many slots (a wavefront's lanes) go without a grouping, a
@@ -134,7 +135,7 @@ struct Grouping {
     counts = l->take(3 * sizeof(std::int32_t));
     hist = l->take(slots > kOneGroup ? 64 * experts * sizeof(std::int32_t) : 0);
     order = l->take(slots * sizeof(std::int32_t));
-    for (std::size_t& t : tiles) t = l->take(most_tiles(slots, experts, kLeastRows) * 4 * sizeof(std::int32_t));
+    for (std::size_t& t : tiles) t = l->take(most_tiles(slots, experts, kLeastRows) * kRowTileBytes);
   }
 };
 // Rows in two fp16 parts (4 bytes an element, whole steps) and their factors:

@@ -112,8 +112,9 @@ __global__ void __launch_bounds__(kThreads) split_tiles_kernel(RowSource src, Gr
   const int most = g.counts[1] * kRows;
   for (int r = blockIdx.x * kWaves + (threadIdx.x >> 6); r < most; r += gridDim.x * kWaves) {
     const RowTile t = g.tiles[0][r / kRows];
-    if (r % kRows >= t.rows) continue;  // nothing reads its results
-    const int pos = t.first + r % kRows;
+    const int at = r - t.group0 * kRows;  // of the expert's rows
+    if (at >= t.slots) continue;          // nothing reads its results
+    const int pos = t.begin + at;
     split_row<MT>(src, row_of(src, pos, g.order[pos]), r, to, threadIdx.x & 63);
   }
 }
@@ -160,8 +161,7 @@ __device__ __forceinline__ void lay_ranges(std::int32_t* count, int experts, con
 #pragma unroll
       for (int l = 0; l < 2; ++l)
         for (std::int32_t i = 0; i < own[1 + l]; ++i)
-          tile(l, at[1 + l] + i,
-               RowTile{e, at[0] + i * g.rows[l], min(n - i * g.rows[l], g.rows[l]), at[2] + ((i << shift0) >> shift1)});
+          tile(l, at[1 + l] + i, RowTile{e, at[0], n, at[1 + l], own[1 + l], at[2], {}});
     }
     __syncthreads();
   }
@@ -302,12 +302,12 @@ __global__ void __launch_bounds__(kThreads) self_kernel(const std::int32_t* __re
     const int i = c * 64 + lane;
     rank += __builtin_popcountll(__ballot(i < slot && all[i] == e));
   }
-  const int r0 = g.rows[0], r1 = g.rows[1], n = count[e], first = part(before, 0) + rank;
-  const int tile0 = part(before, 1) + (rank >> shift0), tile1 = part(before, 2) + (rank >> shift1);
+  const int r0 = g.rows[0], r1 = g.rows[1], n = count[e], begin = part(before, 0);
+  const int group0 = part(before, 1), group1 = part(before, 2), tile0 = group0 + (rank >> shift0), tile1 = group1 + (rank >> shift1);
   if (lane == 0) {
-    g.order[first] = slot;
-    if ((rank & (r0 - 1)) == 0) g.tiles[0][tile0] = RowTile{e, first, min(n - rank, r0), tile1};
-    if ((rank & (r1 - 1)) == 0) g.tiles[1][tile1] = RowTile{e, first, min(n - rank, r1), 0};
+    g.order[begin + rank] = slot;
+    if ((rank & (r0 - 1)) == 0) g.tiles[0][tile0] = RowTile{e, begin, n, group0, (n + r0 - 1) >> shift0, group1, {}};
+    if ((rank & (r1 - 1)) == 0) g.tiles[1][tile1] = RowTile{e, begin, n, group1, (n + r1 - 1) >> shift1, group1, {}};
   }
   store_row<MT>(x, src, tile0 * (MT * kTile) + rank % (MT * kTile), to);
 }

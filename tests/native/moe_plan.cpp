@@ -93,7 +93,7 @@ int main() {
           const MatmulLayout m(a, slots, per_row);
           expect(m.all.bytes >= before, "workspace shrinks", count, slots);
           expect(rows_of(slots, per_row) >= 1 && rows_of(slots, per_row) <= slots, "rows", slots, per_row);
-          expect(m.group.tiles[1] + most_tiles(slots, count, 16) * 16 <= m.x.values, "groups end", count, slots);
+          expect(m.group.tiles[1] + most_tiles(slots, count, 16) * kRowTileBytes <= m.x.values, "groups end", count, slots);
           expect(takes(m.x, a, slots, rows_of(slots, per_row), pick_rows(a, slots, false), false) <= m.all.bytes, "rows end", count, slots);
           before = m.all.bytes;
         }
