@@ -523,6 +523,53 @@ def test_mlp_tokens_apart(tokens, ffn):
     assert np.array_equal(first[keep].view(np.uint32), again[keep].view(np.uint32))
 
 
+def put(at, a):
+    H.check(H.load().llmi_hip_memcpy_h2d(at, a.ctypes.data_as(C.c_void_p), a.nbytes))
+
+
+@pytest.mark.parametrize("slots", [3, 100])
+def test_experts_past_four_gigabytes(slots):
+    """The last of 4096 experts whose codes end past 2^32 bytes; what the others hold is left as it came."""
+    rng = np.random.default_rng(61)
+    count, out, n_in = 4096, 64, 16384
+    data, scales, values = R.matrices(rng, H.Q8_0, 2, out, n_in)
+    d, s = H.DeviceBuffer(count * data[0].nbytes), H.DeviceBuffer(count * scales[0].nbytes)
+    where = {4095: 0, 2050: 1}
+    for e, i in where.items():
+        put(d.ptr + e * data[0].nbytes, data[i])
+        put(s.ptr + e * scales[0].nbytes, scales[i])
+    experts = H.Experts.upload_dev(d.ptr, s.ptr, count, out, n_in, H.Q8_0)
+    ids = np.where(np.arange(slots) % 3 == 0, 4095, np.where(np.arange(slots) % 3 == 1, 2050, -1)).astype(np.int32)
+    x = rng.standard_normal((slots, n_in)).astype(np.float32)
+    y = run_matmul(experts, ids, x, 1)
+    for r in range(slots):
+        if ids[r] < 0:
+            assert (y[r] == GUARD).all()
+            continue
+        want, bound = R.product(x[r], values[where[ids[r]]])
+        assert np.all(np.abs(y[r] - want) <= bound), r
+
+
+@pytest.mark.parametrize("slots,out,stride", [(3, 40, 1 << 29), (70, 40, 1 << 25), (1300, 4100, 1 << 20)])
+def test_rows_past_four_gigabytes(slots, out, stride):
+    """Rows of x and y so far apart that the last ones begin past 2^32 bytes."""
+    rng = np.random.default_rng(62)
+    experts, values = make(rng, H.Q4_0, 2, out, 100)
+    ids = rng.integers(0, 2, slots).astype(np.int32)
+    x = rng.standard_normal((slots, 100)).astype(np.float32)
+    xb, yb, ib = H.DeviceBuffer(slots * stride * 4), H.DeviceBuffer(slots * stride * 4), dev(ids)
+    for r in range(slots):
+        put(xb.ptr + r * stride * 4, x[r])
+    work = Workspace(H.moe_matmul_bytes(experts, slots, 1))
+    H.moe_matmul(experts, ib.ptr, slots, xb.ptr, yb.ptr, work.buf.ptr, work.n, x_stride=stride, y_stride=stride)
+    H.synchronize()
+    work.intact()
+    y = np.zeros((slots, out), np.float32)
+    for r in range(slots):
+        H.check(H.load().llmi_hip_memcpy_d2h(y[r].ctypes.data_as(C.c_void_p), yb.ptr + r * stride * 4, out * 4))
+    check_matmul(y, ids, x, 1, values)
+
+
 def test_two_streams_at_once():
     """Calls on two streams of the caller's, with a workspace each: the results of each alone."""
     create = H.load().hipStreamCreateWithFlags  # found through the library's own dependencies
