@@ -297,7 +297,7 @@ MLPS = [
     (H.Q4_0, H.Q8_0, 8, 1, 8, 96, 50, True, 0.0), (H.Q4_0, H.Q4_0, 8, 2, 2, 576, 130, True, 0.0),
     (H.Q8_0, H.Q4_0, 4, 8, 3, 33, 77, False, 0.2), (H.Q4_0, H.Q4_0, 64, 16, 8, 128, 64, True, 0.1),
     (H.Q8_0, H.Q8_0, 3, 100, 2, 72, 160, True, 0.1), (H.Q4_0, H.Q4_0, 6, 90, 4, 100, 36, False, 0.3),
-    # Long work in the first product alone, in the second alone (after tiles of 32 rows, of 16), in both.
+    # Long work in the second product alone (after tiles of 16 rows), in the first, in the second, in both.
     (H.Q4_0, H.Q8_0, 64, 1000, 2, 4100, 40, True, 0.0),
     (H.Q4_0, H.Q8_0, 8, 600, 2, 64, 2080, True, 0.1), (H.Q8_0, H.Q4_0, 4, 700, 2, 2100, 40, False, 0.0),
     (H.Q4_0, H.Q4_0, 8, 1500, 2, 1040, 1100, True, 0.05),
