@@ -243,7 +243,9 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs p) {
 // ------------------------------------ the second product and a token's sum
 
 constexpr int kSumWaves = 16, kSumThreads = kSumWaves * 64;
-constexpr int kSumRows = 4, kSumFactorBytes = 4 * kSumRows * 4;  // factors of a chunk's blocks, 16 bytes a block
+// Of each block of a chunk 16 bytes: the factors of both rows, then what the
+// tokens weigh the expert with.
+constexpr int kSumRows = 4, kSumFactorBytes = 4 * kSumRows * 4;
 
 struct SumArgs {
   Matrices m;
@@ -278,7 +280,7 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
   const int units = __builtin_popcountll(firsts) * p.chunks, sharers = p.splits * kSumWaves;
   const int each = (units + sharers - 1) / sharers;
   const int u0 = min((split * kSumWaves + wave) * each, units), u1 = min(u0 + each, units);
-  // This wavefront's rows of a chunk, and their factors [block][kSumRows].
+  // This wavefront's rows of a chunk, and their factors and weights [block][kSumRows].
   std::uint8_t* const rows_at = lds + wave * (2 * kRowBytes + kSumFactorBytes);
   float* const factors_at = reinterpret_cast<float*>(rows_at + 2 * kRowBytes);
   float* const meet = reinterpret_cast<float*>(lds);
@@ -349,7 +351,10 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
       if (u + i >= u1) break;
       // A row that does not count is 0, whatever stands there.
       *reinterpret_cast<u32x4*>(rows_at + lane / 32 * kRowBytes + lane % 32 * 16) = ROWS == 1 || live[i] ? x[i] : u32x4{0, 0, 0, 0};
-      if (lane / 4 < 2) factors_at[lane % 4 * kSumRows + lane / 4] = factor[i] * times[i];
+      if (lane / 4 < 2) {
+        factors_at[lane % 4 * kSumRows + lane / 4] = factor[i];
+        factors_at[lane % 4 * kSumRows + 2 + lane / 4] = times[i];
+      }
       wave_sync();
       const std::uint8_t* const from = lane_row<ROWS>(rows_at, lane);
 #pragma unroll
@@ -357,7 +362,8 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(SumArgs p) {
         const f32x4 d = times_codes(from, b, ring[i][b / 2].codes(b % 2));
         const f32x4 f = *reinterpret_cast<const f32x4*>(factors_at + b * kSumRows);
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) acc[r] = __builtin_fmaf(d[r] * ring[i][b / 2].s[b % 2], f[r], acc[r]);
+        for (int r = 0; r < ROWS; ++r)  // the power of two last: with the weight it may lie below the normal numbers
+          acc[r] = __builtin_fmaf(d[r] * ring[i][b / 2].s[b % 2] * f[2 + r], f[r], acc[r]);
       }
       wave_sync();
       if (next < u1) ask(i);

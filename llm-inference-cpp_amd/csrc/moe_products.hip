@@ -423,8 +423,12 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 4 : 3) short_kernel(Produc
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            acc[n][i][r] = __builtin_fmaf(d[i][r], BLOCKS ? s.w[n].s[b2] * s.f[BLOCKS ? i : 0][b2][r] : s.w[n].s[b2], acc[n][i][r]);
+          for (int r = 0; r < 4; ++r) {
+            // The sum first by its scale, then by the power of two: scale times
+            // factor may lie below the normal numbers, where it would lose bits.
+            if constexpr (BLOCKS) acc[n][i][r] = __builtin_fmaf(d[i][r] * s.w[n].s[b2], s.f[i][b2][r], acc[n][i][r]);
+            else acc[n][i][r] = __builtin_fmaf(d[i][r], s.w[n].s[b2], acc[n][i][r]);
+          }
       }
   };
   if (h0 < h1) {
