@@ -426,7 +426,7 @@ int llmi_hip_kv8_read_dev(const llmi_hip_kv8_plan* plan, const llmi_kv8_layer* l
  * ids are -1 and their weights 0.  Logits of +inf share the weight equally.
  * ids and weights [tokens][top_k].  LLMI_ERR_ARG: more than 1024 experts, a
  * top_k above 64 or the number of experts, a stride below it, more than 2^24
- * tokens, a scale that is not finite. */
+ * tokens, a scale that is not finite, ids, weights and logits that overlap. */
 int llmi_hip_moe_route_dev(const float* logits, size_t stride, size_t tokens, size_t experts, size_t top_k,
                            int renormalise, float scale, int32_t* ids, float* weights, void* stream);
 
@@ -460,8 +460,9 @@ int llmi_hip_experts_free(llmi_hip_experts* experts);
  * aligned; nothing has to be cleared, and nothing is kept in it from call to
  * call.  Calls that may run at the same time (two streams, two graphs) need a
  * workspace each; graphs that run one after the other may share one.
- * y must not overlap x.  LLMI_ERR_ARG: more than 2^24 slots, strides too
- * short, y = x, a workspace too small, NULL pointers. */
+ * y must not overlap x or ids, nor the workspace any of them; columns of one
+ * array, rows between each other's, are apart.  LLMI_ERR_ARG: more than 2^24
+ * slots, strides too short, an overlap, a workspace too small, NULL pointers. */
 int llmi_hip_moe_matmul_bytes(const llmi_hip_experts* experts, size_t slots, size_t per_row, size_t* bytes);
 int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids, size_t slots, size_t per_row,
                             const float* x, size_t x_stride, float* y, size_t y_stride, void* work, size_t work_bytes,
@@ -476,7 +477,8 @@ int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids,
  * choices may change its last bits).  h = silu(..) * (..) is carried like x.
  * gate and up of one shape and type, down of either type.  x [tokens][in],
  * residual (NULL: 0) and y [tokens][down's out], rows their strides apart; y may
- * be residual (with its stride) or x, where they have the same rows.  A choice
+ * be residual (with its stride), otherwise they must be apart, and may be x or
+ * overlap it.  A choice
  * whose id is not an expert's adds nothing, whatever its weight.  Everything
  * else as for llmi_hip_moe_matmul_dev. */
 int llmi_hip_moe_mlp_bytes(const llmi_hip_experts* gate, const llmi_hip_experts* down, size_t tokens, size_t top_k,

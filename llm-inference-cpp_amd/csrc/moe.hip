@@ -2,6 +2,7 @@
 // token's experts, and the entry points.  Products of few slots are in
 // moe_few.hip, the others in moe_products.hip, what these need before them
 // (grouping, rows in two parts) in moe_prepare.hip.
+#include <initializer_list>
 #include <memory>
 #include <new>
 
@@ -237,6 +238,12 @@ std::string check_workspace(const void* work, std::size_t bytes, std::size_t nee
   if (bytes < need) return "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed";
   return {};
 }
+// Whether a region that the call writes meets any of the others.
+std::string check_apart(const char* name, const Region& written, std::initializer_list<Region> others) {
+  for (const Region& r : others)
+    if (overlap(written, r)) return std::string(name) + " overlaps another operand";
+  return {};
+}
 Groups groups_at(std::uint8_t* work, const Grouping& g, std::size_t rows0, std::size_t rows1) {
   return {reinterpret_cast<std::int32_t*>(work + g.counts),
           reinterpret_cast<std::int32_t*>(work + g.order),
@@ -265,6 +272,11 @@ int llmi_hip_moe_route_dev(const float* logits, size_t stride, size_t tokens, si
   LLMI_REQUIRE(scale - scale == 0.0f, "moe_route: scale must be finite");
   if (tokens == 0) return LLMI_OK;
   LLMI_REQUIRE(logits != nullptr && ids != nullptr && weights != nullptr, "moe_route: null pointer");
+  const Region r_logits = Region::matrix(logits, tokens, experts, stride), r_ids = Region::whole(ids, tokens * top_k * sizeof(*ids)),
+               r_weights = Region::whole(weights, tokens * top_k * sizeof(*weights));
+  std::string meets = check_apart("ids", r_ids, {r_logits, r_weights});
+  if (meets.empty()) meets = check_apart("weights", r_weights, {r_logits});
+  LLMI_REQUIRE(meets.empty(), "moe_route: " + meets);
   hipStream_t s = pick(stream);
   const unsigned grid = grid_for(tokens, kWaves);
   const int e = static_cast<int>(experts), k = static_cast<int>(top_k);
@@ -370,6 +382,11 @@ int llmi_hip_moe_matmul_dev(const llmi_hip_experts* experts, const int32_t* ids,
   const MatmulLayout l(sh, slots, per_row);
   why = check_workspace(work, work_bytes, l.all.bytes);
   LLMI_REQUIRE(why.empty(), "moe_matmul: " + why);
+  const Region r_ids = Region::whole(ids, slots * sizeof(*ids)), r_x = Region::matrix(x, rows_of(slots, per_row), sh.in, x_stride),
+               r_y = Region::matrix(y, slots, sh.out, y_stride);
+  why = check_apart("y", r_y, {r_ids, r_x});
+  if (why.empty()) why = check_apart("the workspace", Region::whole(work, l.all.bytes), {r_ids, r_x, r_y});
+  LLMI_REQUIRE(why.empty(), "moe_matmul: " + why);
   hipStream_t s = pick(stream);
   per_row = std::min(per_row, slots);  // more than all slots mean the same row; the kernels have 32 bits for it
   if (few_matmul(sh, slots, per_row))
@@ -411,9 +428,17 @@ int llmi_hip_moe_mlp_dev(const llmi_hip_experts* gate, const llmi_hip_experts* u
   const MlpLayout l(gs, ds, tokens, top_k);
   why = check_workspace(work, work_bytes, l.all.bytes);
   LLMI_REQUIRE(why.empty(), "moe_mlp: " + why);
+  const std::size_t slots = tokens * top_k;
+  // x may lie anywhere beside y: no launch that writes y reads it.
+  const Region r_ids = Region::whole(ids, slots * sizeof(*ids)), r_weights = Region::whole(weights, slots * sizeof(*weights)),
+               r_x = Region::matrix(x, tokens, gs.in, x_stride), r_y = Region::matrix(y, tokens, ds.out, y_stride),
+               r_residual = Region::matrix(residual, residual == nullptr ? 0 : tokens, ds.out, residual_stride);
+  why = check_apart("y", r_y, {r_ids, r_weights});
+  if (why.empty() && residual != y) why = check_apart("y", r_y, {r_residual});
+  if (why.empty()) why = check_apart("the workspace", Region::whole(work, l.all.bytes), {r_ids, r_weights, r_x, r_y, r_residual});
+  LLMI_REQUIRE(why.empty(), "moe_mlp: " + why);
   hipStream_t s = pick(stream);
   auto* w = static_cast<std::uint8_t*>(work);
-  const std::size_t slots = tokens * top_k;
   const MlpRows rows = pick_mlp_rows(gs, ds, slots);
   const Groups g = groups_at(w, l.group, rows.first, rows.second);
   const SplitRows xs = parts_at(w, l.x), hs = parts_at(w, l.h_parts);

@@ -183,6 +183,41 @@ struct MlpLayout {
   }
 };
 
+// Memory that a call reads or writes: `rows` pieces of `bytes` bytes, `stride`
+// bytes apart (at least as long).
+struct Region {
+  const void* at;
+  std::size_t rows, bytes, stride;
+  static Region whole(const void* p, std::size_t n) { return {p, 1, n, n}; }
+  static Region matrix(const float* p, std::size_t rows, std::size_t width, std::size_t stride) {
+    return {p, rows, width * sizeof(float), std::min(stride, SIZE_MAX / sizeof(float)) * sizeof(float)};
+  }
+};
+// Whether two regions have a byte in common.  Spans that are apart settle
+// nearly every call; columns of one array, rows between each other's, do not meet.
+inline bool overlap(const Region& a, const Region& b) {
+  typedef __int128 Wide;  // differences and products of any addresses and strides
+  if (a.rows == 0 || b.rows == 0 || a.bytes == 0 || b.bytes == 0) return false;
+  if (a.rows > b.rows && a.stride != b.stride) return overlap(b, a);
+  const Wide from = static_cast<Wide>(reinterpret_cast<std::uintptr_t>(b.at)) - reinterpret_cast<std::uintptr_t>(a.at);
+  const Wide a_end = static_cast<Wide>(a.rows - 1) * a.stride + a.bytes, b_end = from + static_cast<Wide>(b.rows - 1) * b.stride + b.bytes;
+  if (from >= a_end || b_end <= 0) return false;
+  // Row i of a (at i a.stride) meets row j of b (at from + j b.stride) where
+  // j b.stride lies between at - from - b.bytes and at - from + a.bytes, both excluded.
+  const auto row_meets = [&](Wide at, Wide first) {
+    const Wide below = at - from - static_cast<Wide>(b.bytes), stride = b.stride;
+    Wide j = below / stride;
+    if (j * stride > below) --j;  // the quotient rounded down
+    j = std::max(j + 1, first);
+    return j < static_cast<Wide>(b.rows) && j * stride < at - from + static_cast<Wide>(a.bytes);
+  };
+  // Of equal strides only j - i counts.
+  if (a.stride == b.stride) return row_meets(0, -static_cast<Wide>(a.rows - 1));
+  for (std::size_t i = 0; i < a.rows; ++i)
+    if (row_meets(static_cast<Wide>(i) * a.stride, 0)) return true;
+  return false;
+}
+
 inline std::string check_matmul(std::size_t slots, std::size_t per_row) {
   if (per_row == 0) return "slots of a row must be at least 1";
   if (slots > kMaxSlots) return "more than 2^24 slots";
