@@ -57,14 +57,19 @@ __device__ __forceinline__ void store_parts(const ProductArgs& p, int tile, int 
 // lane from `to` (common to the wavefront).  Nothing waits for it but landed().
 // The instruction adds its offset to both addresses; between a write of m0 and
 // such a load this family needs one wait state, which nobody inserts in here.
+// m0 is named as written, so that no m0 of the compiler's lives across it; that
+// it is no register to allocate, as the compiler would warn, is known.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int OFFSET>
 __device__ __forceinline__ void to_lds(const std::uint8_t* from, std::uint32_t to) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(from), "s"(to - OFFSET), "n"(OFFSET) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(from), "s"(to - OFFSET), "n"(OFFSET) : "memory", "m0");
 }
 // The same from an address common to the wavefront and each lane's offset.
 __device__ __forceinline__ void to_lds_from(GlobalBytes from, std::uint32_t offset, std::uint32_t to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "s"(to) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // All of this wavefront's loads have landed and its reads of LDS are done;
 // then those of the workgroup's.
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
