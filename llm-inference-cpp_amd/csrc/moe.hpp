@@ -49,8 +49,8 @@ struct SplitRows {
   _Float16* values;
   float* factors;
 };
-// Where rows come from: position `pos` of the order has x's row pos, or
-// order[pos] / per_row (per_row > 0).
+// Where rows come from: slot s has x's row s / per_row, at least 1 (launch_split,
+// which takes the rows one after the other, does not look at it).
 struct RowSource {
   const float* x;
   std::size_t stride, in, steps;

@@ -93,9 +93,7 @@ __device__ __forceinline__ void split_row(const RowSource& src, std::size_t from
   Row x(src, from, lane);
   store_row<MT>(x, src, r, to);
 }
-__device__ __forceinline__ std::size_t row_of(const RowSource& src, int pos, int slot) {
-  return src.per_row > 0 ? static_cast<std::uint32_t>(slot) / src.per_row : static_cast<std::uint32_t>(pos);
-}
+__device__ __forceinline__ std::size_t row_of(const RowSource& src, int slot) { return static_cast<std::uint32_t>(slot) / src.per_row; }
 
 // Rows as they are.  Bound by memory: 32768 rows of 1024 in 47.6 us, 5.6 TB/s.
 __global__ void __launch_bounds__(kThreads) split_kernel(RowSource src, int rows, const std::int32_t* __restrict__ live,
@@ -115,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) split_tiles_kernel(RowSource src, Gr
     const int at = r - t.group0 * kRows;  // of the expert's rows
     if (at >= t.slots) continue;          // nothing reads its results
     const int pos = t.begin + at;
-    split_row<MT>(src, row_of(src, pos, g.order[pos]), r, to, threadIdx.x & 63);
+    split_row<MT>(src, row_of(src, g.order[pos]), r, to, threadIdx.x & 63);
   }
 }
 
@@ -264,8 +262,7 @@ __global__ void __launch_bounds__(kThreads) self_kernel(const std::int32_t* __re
   const int slot = blockIdx.x * kWaves + wave;
   for (int e = t; e < static_cast<int>(kSelfExperts); e += kThreads) count[e] = 0;
   __syncthreads();
-  const int own_slot = min(slot, slots - 1);
-  Row x(src, row_of(src, own_slot, own_slot), lane);
+  Row x(src, row_of(src, min(slot, slots - 1)), lane);
   for (int i = t; i < slots; i += kThreads) {
     const std::int32_t e = ids[i];
     const bool live = e >= 0 && e < experts;
@@ -327,7 +324,7 @@ int launch_prepare(const std::int32_t* ids, std::size_t slots, std::size_t exper
     return LLMI_OK;
   }
   const int blocks = static_cast<int>(grouping_blocks(slots));
-  const std::size_t rows = tiled ? 0 : x.per_row > 0 ? ceil_div(slots, x.per_row) : slots;
+  const std::size_t rows = tiled ? 0 : ceil_div(slots, x.per_row);
   const unsigned grid = static_cast<unsigned>(blocks + std::min<std::size_t>(ceil_div(rows, kGroupThreads / 64), 1 << 16));
   prepare_kernel<<<grid, kGroupThreads, 0, s>>>(ids, n, e, g, blocks, x, static_cast<int>(rows), to);
   LLMI_TRY_HIP(hipGetLastError());
