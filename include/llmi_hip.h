@@ -437,7 +437,8 @@ int llmi_hip_moe_route_dev(const float* logits, size_t stride, size_t tokens, si
  * ways above), or from planar device memory, one expert after the other as
  * llmi_hip_quantize_dev writes them ([count][out] rows of row_bytes codes,
  * [count][out][ceil(in / 32)] scales), which has to be complete before the
- * call; both return when the copy is done. */
+ * call; both return when the copy is done.  Scales are finite and at most 2^80
+ * in magnitude: a block's sum meets its scale before its row's power of two. */
 typedef struct llmi_hip_experts llmi_hip_experts;
 int llmi_hip_experts_create(const llmi_hip_weight* const* weights, size_t count, llmi_hip_experts** experts);
 int llmi_hip_experts_upload_dev(const uint8_t* data_dev, const float* scales_dev, size_t count, size_t out, size_t in,

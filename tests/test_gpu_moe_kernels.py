@@ -122,3 +122,43 @@ def test_mlp_small_results(qtype, call, down_size, weight):
     steps = -(-ffn // 32) + 32 + 2 * top_k
     bound += top_k * weight * np.abs(mats["down"][2]).sum(2).max() * 2.0**-149 + steps * 2.0**-149
     assert np.all(np.abs(layer.run(ids, weights, x) - want) <= bound), (np.abs(layer.run(ids, weights, x) - want) / bound).max()
+
+
+@pytest.mark.parametrize("qtype", TYPES)
+@pytest.mark.parametrize("size,x_size", [(2.0**79, 2.0**-70), (2.0**-110, 2.0**100), (-(2.0**-30), 2.0**-90)])
+@pytest.mark.parametrize("call", [(2, 1, 2, 100, 40, 2, 1.0), (2, 9, 1, 300, 70, 1, 1.0)] + [K.MATMULS[i][0] for i in (2, 5, 8, 13)])
+def test_matmul_scales_of_any_size(qtype, size, x_size, call):
+    """Scales up to 2^80 with rows that bring the results back, tiny and negative ones."""
+    count, tokens, top_k, n_in, out, per_row, skew = call
+    rng = np.random.default_rng(n_in * 29 + out)
+    codes, scales, values = K.R.matrices(rng, qtype, count, out, n_in, 0.0)
+    scales, by = np.full_like(scales, size), size / scales[0, 0, 0].astype(np.float64)
+    d, s = G.dev(codes), G.dev(scales)
+    experts = H.Experts.upload_dev(d.ptr, s.ptr, count, out, n_in, qtype)
+    ids = K.draw_ids(rng, tokens, top_k, count, 0.0, skew)
+    x = (rng.standard_normal((ids.size // per_row, n_in)) * x_size).astype(np.float32)
+    y = G.run_matmul(experts, ids, x, per_row)
+    flat = ids.reshape(-1)
+    for e in range(count):
+        r = np.nonzero(flat == e)[0]
+        if len(r):
+            want, bound = K.products(x[r // per_row], values[e] * by)
+            assert np.all(np.abs(y[r] - want) <= bound + 2.0**-149 * (n_in / 32 + 16)), e
+
+
+@pytest.mark.parametrize("qtype", TYPES)
+@pytest.mark.parametrize("down_size", [2.0**80, 2.0**-100])
+@pytest.mark.parametrize("call", [K.MLPS[i][0] for i in (0, 2, 6, 11, 13, 16, 17)])
+def test_mlp_scales_of_any_size(qtype, down_size, call):
+    """The same for an MLP's second product."""
+    count, tokens, top_k, hidden, ffn, skew = call
+    rng = np.random.default_rng(hidden * 31 + ffn)
+    mats = {n: K.R.matrices(rng, qtype, count, *s, 0.0) for n, s in (("gate", (ffn, hidden)), ("up", (ffn, hidden)), ("down", (hidden, ffn)))}
+    codes, scales, values = mats["down"]
+    mats["down"] = codes, np.full_like(scales, down_size), values * (down_size / scales[0, 0, 0].astype(np.float64))
+    layer = Loaded(mats, (qtype,) * 3)
+    ids = K.draw_ids(rng, tokens, top_k, count, 0.0, skew)
+    weights = rng.random((tokens, top_k)).astype(np.float32)
+    x = rng.standard_normal((tokens, hidden)).astype(np.float32)
+    want, bound = K.sums(ids, weights, x, *(mats[n][2] for n in ("gate", "up", "down")))
+    assert np.all(np.abs(layer.run(ids, weights, x) - want) <= bound)
