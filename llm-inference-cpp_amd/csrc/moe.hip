@@ -25,9 +25,10 @@ __device__ __forceinline__ std::uint32_t rank_bits(float l) {
 // One wavefront a token; lane l holds logits l, l + 64, ...  Every round takes
 // the largest rank of all lanes, and of the logits that have it the first: the
 // lowest place of a lane's, then the lowest lane.  The rounds are bound by their
-// chains of rotations and ballots (8192 tokens, 6 of 128 experts: 5.8 us, memory
-// alone 1; with exchanges through LDS in place of the rotations 12.4); one to 64
-// tokens take a launch, 4.5 us.
+// chains of rotations and ballots (8192 tokens, 8 of 128 experts: 5.8 us, memory
+// alone 1; with exchanges through LDS in place of the rotations 12.4; 8 of 256
+// 7.3, of 512 and 1024, which share a variant, 14.9 and 17.5); one to 64 tokens
+// take a launch, 4.5 us.
 template <int N>
 __global__ void __launch_bounds__(kThreads) route_kernel(const float* __restrict__ logits, std::size_t stride,
                                                          std::size_t tokens, int experts, int top_k, int renormalise,

@@ -164,7 +164,8 @@ __device__ __forceinline__ std::uint32_t max_of_half(std::uint32_t v) {
 // expf and of an IEEE quotient (they were a seventh of the vector work of a
 // prompt's gated product): exp(-g) = 2^t with t = -g log2(e) in two parts, the
 // hardware's 2^t and reciprocal (1 unit each), the reciprocal refined once.
-// Beyond +-150 the exponential is inf or 0 either way; NaN stays one.
+// Beyond +-150 the exponential is inf or 0 either way; NaN stays one.  Gates
+// below about -87, whose 1 + exp(-g) passes fp32, give 0 (silu is -2^-120 there).
 __device__ __forceinline__ float silu(float g) {
   const float c = fminf(fmaxf(g, -150.0f), 150.0f);
   constexpr float kLog2e = 0x1.715476p+0f, kRest = 0x1.4ae0bep-26f, kLn2 = 0x1.62e43p-1f;
